@@ -500,6 +500,86 @@ int mx_foreach_f32(int op, const mx_foreach_tensor* tensors, int64_t count, int6
 int mx_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t src_pitch, int64_t row_bytes,
                  int64_t rows, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* A residual feed-forward block and its optimizer step (FP32, contiguous).  */
+/* No counterparts in the reference.  Scratch: where a call needs it, the     */
+/* caller may pass `workspace` (16-byte aligned, at least the bytes that the  */
+/* matching _workspace query names; a smaller one is MX_ERR_WORKSPACE); NULL  */
+/* takes it from the allocator, which a call on a stream under graph capture  */
+/* must not do (MX_ERR_WORKSPACE).                                            */
+/* ------------------------------------------------------------------------ */
+
+/* Layer norm over the last axis of x [rows, cols]:
+ *   y = (x - mean) * rstd * gamma + beta,  rstd = 1/sqrt(var + eps), biased variance.
+ * gamma and beta may be NULL (1 and 0); mean and rstd [rows] may be NULL (not
+ * kept).  rows == 0 is a no-op, cols == 0 with rows is invalid. */
+int mx_layer_norm_forward(const float* x, const float* gamma, const float* beta, int64_t rows, int64_t cols,
+                          float eps, float* y, float* mean, float* rstd, void* stream);
+/* Gradients from the saved mean / rstd.  Any of dx, dgamma, dbeta may be NULL
+ * (not computed); rows == 0 writes zero dgamma / dbeta.  Column sums are taken
+ * in a fixed order. */
+int mx_layer_norm_backward(const float* dy, const float* x, const float* mean, const float* rstd, const float* gamma,
+                           int64_t rows, int64_t cols, float* dx, float* dgamma, float* dbeta, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int mx_layer_norm_backward_workspace(int64_t rows, int64_t cols, int64_t* bytes);
+
+enum mx_activation { MX_ACT_NONE = 0, MX_ACT_RELU = 1, MX_ACT_SILU = 2, MX_ACT_GELU = 3, MX_ACT_GELU_TANH = 4 };
+
+/* Linear layer: z = x [m,k] w [n,k]^T + bias [n],  y [m,n] = act(z) + residual [m,n].
+ * bias and residual may be NULL; z, if not NULL, receives the activation's
+ * input (the backward's argument).  y may be the residual's own buffer; no
+ * other operands may overlap an output.  k == 0 is an empty sum. */
+int mx_linear_forward(const float* x, const float* w, const float* bias, const float* residual, int64_t m, int64_t k,
+                      int64_t n, int activation, float* y, float* z, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+/* dz = dy * act'(z);  dx = dz w,  dw = dz^T x,  db = sum_m dz.  The residual's
+ * gradient is dy itself.  z may be NULL when the activation is MX_ACT_NONE; any
+ * of dx, dw, db may be NULL. */
+int mx_linear_backward(const float* dy, const float* x, const float* w, const float* z, int64_t m, int64_t k,
+                       int64_t n, int activation, float* dx, float* dw, float* db, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+/* Bytes that a forward (`backward` == 0) or a backward of these sizes takes. */
+int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activation, int backward, int64_t* bytes);
+
+/* The polar factor's approximation by `steps` Newton-Schulz iterations
+ * X <- a X + (b G + c G^2) X, G = X X^T (on the shorter side), of
+ * X = U / max(|U|_F, eps). */
+typedef struct mx_newton_schulz {
+  int64_t steps;
+  double a, b, c, eps;
+} mx_newton_schulz;
+typedef struct mx_matrix_pair {
+  const float* in;
+  float* out; /* may be `in` */
+  int64_t rows, cols;
+} mx_matrix_pair;
+/* out[i] = that factor of in[i], matrices of one shape side by side. */
+int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_t count, int64_t* bytes);
+
+/* Orthogonalised momentum step (torch.optim.Muon's update):
+ *   buf += (1 - momentum) (grad - buf);  u = nesterov ? grad + momentum (buf - grad) : buf
+ *   param = param (1 - lr weight_decay) - lr r orth(u),
+ * r = sqrt(max(1, rows / cols)) (MX_MUON_ORIGINAL) or 0.2 sqrt(max(rows, cols))
+ * (MX_MUON_MATCH_RMS_ADAMW).  Tensors are [rows, cols], no two of which may overlap. */
+enum mx_muon_adjust { MX_MUON_ORIGINAL = 0, MX_MUON_MATCH_RMS_ADAMW = 1 };
+typedef struct mx_muon_tensor {
+  float* param;
+  const float* grad;
+  float* momentum_buffer;
+  int64_t rows, cols;
+} mx_muon_tensor;
+typedef struct mx_muon_hparams {
+  double lr, weight_decay, momentum;
+  int nesterov;
+  int adjust_lr;
+  mx_newton_schulz ns;
+} mx_muon_hparams;
+int mx_muon_step(const mx_muon_tensor* tensors, int64_t count, const mx_muon_hparams* hp, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+int mx_muon_workspace(const mx_muon_tensor* tensors, int64_t count, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "mfma_core.hpp"
+#include "mx_activation.hpp"
 #include "mx_internal.hpp"
 
 namespace mx {
@@ -40,9 +41,14 @@ struct GemmArgs {
   // writes its partial product to ws[i][batch][M][N].
   int splits, kps;
   float* ws;
+  // A linear layer's epilogue (EPI kernels): z = the product + bias, kept where
+  // z is not null; C = activation(z) + residual, both [M][N] as C is.
+  int act;
+  const float* residual;
+  float* z;
 };
 
-template <class C, Mode MA, Mode MB>
+template <class C, Mode MA, Mode MB, bool EPI>
 MX_TILE_KERNEL(C) void gemm_kernel(GemmArgs p) {
   __shared__ __attribute__((aligned(16))) float smem[C::SMEM_FLOATS];
   int tm, tn;
@@ -82,6 +88,35 @@ MX_TILE_KERNEL(C) void gemm_kernel(GemmArgs p) {
     // Column bias (nn.Linear): one value per fragment column, loaded once.
     bcol[j] = (kind == MX_BIAS_COL && ccol[j] < p.N) ? beta * bias[int64_t(ccol[j]) * p.bias_sn] : 0.f;
   }
+  if constexpr (EPI) {
+    // The linear layer's rows are N apart.  A block row's residual is read
+    // before any of it is stored: loads and stores share the vector-memory
+    // counter, so a load between stores waits for them.
+    const bool full = row0 + C::BM <= p.M && col0 + C::BN <= p.N;
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FN; ++j) {
+        float res[16];
+        if (p.residual) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int row = row0 + acc_row<C>(i, v);
+            res[v] = full || (row < p.M && ccol[j] < p.N) ? p.residual[int64_t(row) * p.ldc + ccol[j]] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int row = row0 + acc_row<C>(i, v);
+          if (!full && (row >= p.M || ccol[j] >= p.N)) continue;
+          const int64_t at = int64_t(row) * p.ldc + ccol[j];
+          const float t = acc.v[i][j][v] * scale + bcol[j];
+          if (p.z) p.z[at] = t;
+          cb[at] = activate(p.act, t) + (p.residual ? res[v] : 0.f);
+        }
+      }
+    return;
+  }
   // Two separate walks: stores and loads share the vector-memory counter, so
   // a bias load between stores makes every later store wait for the earlier
   // ones; only the matrix-bias walk (baddbmm) reads memory between stores.
@@ -119,7 +154,7 @@ MX_TILE_KERNEL(C) void gemm_kernel(GemmArgs p) {
 // C = alpha * (sum of the K splits' partial products, in split order) +
 // beta * bias.  VEC: four columns per thread (N and C's strides multiples of
 // four, C 16-byte aligned).
-template <bool VEC>
+template <bool VEC, bool EPI>
 __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs p) {
   constexpr int W = VEC ? 4 : 1;
   typedef float vec __attribute__((ext_vector_type(W)));
@@ -148,11 +183,20 @@ __global__ __launch_bounds__(256) void gemm_sum_kernel(GemmArgs p) {
         o += p.beta * b[0];
       }
     }
-    *reinterpret_cast<vec*>(p.c + bz * p.c_sb + int64_t(row) * p.ldc + n) = o;
+    const int64_t to = bz * p.c_sb + int64_t(row) * p.ldc + n;
+    if constexpr (EPI) {
+      if (p.z) *reinterpret_cast<vec*>(p.z + to) = o;
+      vec r = 0.f;
+      if (p.residual) r = *reinterpret_cast<const vec*>(p.residual + to);
+#pragma unroll
+      for (int e = 0; e < W; ++e) o[e] = activate(p.act, o[e]) + r[e];
+    }
+    *reinterpret_cast<vec*>(p.c + to) = o;
   }
 }
 
 // k == 0: C = beta * bias (or zeros when beta == 0 / no bias).
+template <bool EPI>
 __global__ void gemm_k0_kernel(GemmArgs p) {
   const int64_t total = int64_t(p.batch) * p.M * p.N;
   for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
@@ -168,7 +212,13 @@ __global__ void gemm_k0_kernel(GemmArgs p) {
                                                   : bias[int64_t(row) * p.bias_sm + int64_t(col) * p.bias_sn];
       out = p.beta * bv;
     }
-    p.c[int64_t(bz) * p.c_sb + int64_t(row) * p.ldc + col] = out;
+    const int64_t at = int64_t(bz) * p.c_sb + int64_t(row) * p.ldc + col;
+    if constexpr (EPI) {
+      const float r = p.residual ? p.residual[at] : 0.f;
+      if (p.z) p.z[at] = out;
+      out = activate(p.act, out) + r;
+    }
+    p.c[at] = out;
   }
 }
 
@@ -186,7 +236,7 @@ Mode pick_mode(const float* base, int64_t s_row, int64_t s_k, int64_t s_batch, i
   return std::llabs(s_k) <= std::llabs(s_row) ? Mode::KSCALAR : Mode::RSCALAR;
 }
 
-template <class C, Mode MA, Mode MB>
+template <class C, Mode MA, Mode MB, bool EPI = false>
 int launch3(GemmArgs p, hipStream_t s) {
   // A 128x128 tile has the registers for two slabs of each operand in flight
   // when both are read 16 bytes at a time, and for the second accumulator set
@@ -199,7 +249,7 @@ int launch3(GemmArgs p, hipStream_t s) {
   for (int b0 = 0; b0 < p.batch; b0 += 65535) {
     p.batch0 = b0;
     const dim3 grid(ntiles, p.splits, std::min(p.batch - b0, 65535));
-    hipLaunchKernelGGL((gemm_kernel<D, MA, MB>), grid, dim3(kThreads), 0, s, p);
+    hipLaunchKernelGGL((gemm_kernel<D, MA, MB, EPI>), grid, dim3(kThreads), 0, s, p);
     MX_HIP(hipGetLastError());
   }
   return MX_OK;
@@ -236,6 +286,16 @@ int launch1_vec(GemmArgs p, Mode ma, Mode mb, hipStream_t s) {
   if (ma == Mode::KVEC)
     return mb == Mode::KVEC ? launch3<C, Mode::KVEC, Mode::KVEC>(p, s) : launch3<C, Mode::KVEC, Mode::RVEC>(p, s);
   return mb == Mode::KVEC ? launch3<C, Mode::RVEC, Mode::KVEC>(p, s) : launch3<C, Mode::RVEC, Mode::RVEC>(p, s);
+}
+
+// A linear layer's product: both operands along k, 16 bytes at a time or not.
+template <class C>
+int launch_linear(GemmArgs p, bool vec, hipStream_t s) {
+  p.tiles_m = (p.M + C::BM - 1) / C::BM;
+  p.tiles_n = (p.N + C::BN - 1) / C::BN;
+  if (vec) return launch3<C, Mode::KVEC, Mode::KVEC, true>(p, s);
+  if constexpr (C::BM <= 128 && C::BN <= 128) return launch3<C, Mode::KSCALAR, Mode::KSCALAR, true>(p, s);
+  return set_error(MX_ERR_INVALID, "mx_linear_forward: no such tile");
 }
 
 bool is_vec(Mode m) { return m == Mode::KVEC || m == Mode::RVEC; }
@@ -407,24 +467,16 @@ int plan_gemm(const mx_gemm_desc* d, const float* a, const float* b, const float
   return MX_OK;
 }
 
-// A call whose stream is being captured into a graph must not take scratch
-// from the allocator: the block would return to the cache while replays of the
-// graph still use it.
-bool may_allocate(hipStream_t s) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(s, &st) == hipSuccess) return st == hipStreamCaptureStatusNone;
-  (void)hipGetLastError();
-  return false;
-}
-
+template <bool EPI>
 int launch_sum(const GemmArgs& p, hipStream_t s) {
-  const bool vec = p.N % 4 == 0 && p.ldc % 4 == 0 && p.c_sb % 4 == 0 && aligned16(p.c) && aligned16(p.ws);
+  bool vec = p.N % 4 == 0 && p.ldc % 4 == 0 && p.c_sb % 4 == 0 && aligned16(p.c) && aligned16(p.ws);
+  if constexpr (EPI) vec = vec && aligned16(p.z) && aligned16(p.residual);
   const int64_t items = int64_t(p.batch) * p.M * p.N / (vec ? 4 : 1);
   const int blocks = int(std::min<int64_t>((items + 255) / 256, 65535));
   if (vec)
-    hipLaunchKernelGGL(gemm_sum_kernel<true>, dim3(blocks), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((gemm_sum_kernel<true, EPI>), dim3(blocks), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL(gemm_sum_kernel<false>, dim3(blocks), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((gemm_sum_kernel<false, EPI>), dim3(blocks), dim3(256), 0, s, p);
   MX_HIP(hipGetLastError());
   return MX_OK;
 }
@@ -436,30 +488,54 @@ int64_t partial_bytes(const GemmArgs& p) { return p.splits > 1 ? int64_t(p.split
 }  // namespace
 
 int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const float* bias, float* c, int64_t partials,
-                hipStream_t s) {
+                hipStream_t s, const GemmEpilogue* epi, void* given) {
   GemmPlan g;
   MX_TRY(plan_gemm(d, a, b, bias, c, std::min(partials, kMaxSplitBytes), &g));
   if (g.empty) return MX_OK;
-  if (g.p.splits > 1 && !may_allocate(s)) MX_TRY(plan_gemm(d, a, b, bias, c, 0, &g));
+  if (g.p.splits > 1 && !given && !may_allocate(s)) MX_TRY(plan_gemm(d, a, b, bias, c, 0, &g));
   MX_REQUIRE(c, MX_ERR_INVALID, "mx_gemm_f32: null output");
   MX_REQUIRE(d->bias_kind == MX_BIAS_NONE || bias, MX_ERR_INVALID, "mx_gemm_f32: null bias");
   GemmArgs& p = g.p;
+  if (epi) {
+    p.act = epi->act;
+    p.residual = epi->residual;
+    p.z = epi->z;
+  }
   if (d->k == 0) {
     const int64_t total = d->batch * d->m * d->n;
     const int blocks = int(std::min<int64_t>((total + 255) / 256, 65535));
-    hipLaunchKernelGGL(gemm_k0_kernel, dim3(blocks), dim3(256), 0, s, p);
+    if (epi)
+      hipLaunchKernelGGL(gemm_k0_kernel<true>, dim3(blocks), dim3(256), 0, s, p);
+    else
+      hipLaunchKernelGGL(gemm_k0_kernel<false>, dim3(blocks), dim3(256), 0, s, p);
     MX_HIP(hipGetLastError());
     return MX_OK;
   }
   MX_REQUIRE(a && b, MX_ERR_INVALID, "mx_gemm_f32: null operand");
   Scratch ws;
   if (p.splits > 1) {
-    if (ws.alloc(size_t(partial_bytes(p)), s) == MX_OK) {
+    if (given) {
+      p.ws = static_cast<float*>(given);
+    } else if (ws.alloc(size_t(partial_bytes(p)), s) == MX_OK) {
       p.ws = ws.as<float>();
     } else {  // no room for partials: one pass over K
       clear_error();
+      const GemmArgs was = p;
       MX_TRY(plan_gemm(d, a, b, bias, c, 0, &g));
+      p.act = was.act;
+      p.residual = was.residual;
+      p.z = was.z;
     }
+  }
+  if (epi) {
+    const bool vec = g.ma == Mode::KVEC && g.mb == Mode::KVEC;
+    switch (g.tile) {
+      case 0: MX_TRY(launch_linear<TileTall>(p, vec, s)); break;
+      case 1: MX_TRY(launch_linear<TileWide>(p, vec, s)); break;
+      case 2: MX_TRY(launch_linear<TileSq>(p, vec, s)); break;
+      default: MX_TRY(launch_linear<TileSmall>(p, vec, s));
+    }
+    return p.splits > 1 ? launch_sum<true>(p, s) : MX_OK;
   }
   switch (g.tile) {
     case 0: MX_TRY(launch1_vec<TileTall>(p, g.ma, g.mb, s)); break;
@@ -467,7 +543,7 @@ int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const flo
     case 2: MX_TRY(launch1<TileSq>(p, g.ma, g.mb, s)); break;
     default: MX_TRY(launch1<TileSmall>(p, g.ma, g.mb, s));
   }
-  return p.splits > 1 ? launch_sum(p, s) : MX_OK;
+  return p.splits > 1 ? launch_sum<false>(p, s) : MX_OK;
 }
 
 int gemm_describe(const mx_gemm_desc* d, const float* a, const float* b, int64_t partials, std::string* name,

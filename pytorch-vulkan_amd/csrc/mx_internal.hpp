@@ -50,6 +50,25 @@ struct Scratch {
   }
 };
 
+// False while `s` is being captured into a graph: a block taken from the
+// allocator then would return to its cache while replays of the graph still
+// use it.
+bool may_allocate(hipStream_t s);
+
+// Scratch that the caller may have brought: `have` bytes at `given` (16-byte
+// aligned) if `given` is not null, else from the allocator.
+struct Workspace {
+  void* ptr = nullptr;
+  int take(const char* who, void* given, int64_t have, int64_t need, hipStream_t s);
+  template <class T>
+  T* as() const {
+    return static_cast<T*>(ptr);
+  }
+
+ private:
+  Scratch own_;
+};
+
 // Copies a small host table to device memory through a pinned ring buffer.
 // The returned device pointer is valid for work enqueued on `s` after this
 // call (the block is returned to the stream-ordered cache by `holder`).
@@ -58,10 +77,20 @@ int upload(const void* host, size_t bytes, hipStream_t s, Scratch& holder);
 // Number of compute units of the current device (cached).
 int cu_count();
 
-// mx_gemm_f32 with at most `partials` bytes of scratch for a K split, and the
-// kernels and scratch of such a call (mx_gemm.hip).
+// A linear layer's epilogue on a product of two operands along k whose output
+// rows are n apart: z = product + bias (kept where z is not null),
+// c = activation(z) + residual (residual may be null).
+struct GemmEpilogue {
+  int act;
+  const float* residual;
+  float* z;
+};
+
+// mx_gemm_f32 with at most `partials` bytes of scratch for a K split (the
+// caller's where `given` is not null), and the kernels and scratch of such a
+// call (mx_gemm.hip).
 int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const float* bias, float* c, int64_t partials,
-                hipStream_t s);
+                hipStream_t s, const GemmEpilogue* epi = nullptr, void* given = nullptr);
 int gemm_describe(const mx_gemm_desc* d, const float* a, const float* b, int64_t partials, std::string* name,
                   int64_t* bytes);
 

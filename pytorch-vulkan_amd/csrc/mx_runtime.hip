@@ -637,4 +637,27 @@ int upload(const void* host, size_t bytes, hipStream_t s, Scratch& holder) {
   return MX_OK;
 }
 
+// ---------------------------------------------------------------- workspaces
+bool may_allocate(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(s, &st) == hipSuccess) return st == hipStreamCaptureStatusNone;
+  (void)hipGetLastError();
+  return false;
+}
+
+int Workspace::take(const char* who, void* given, int64_t have, int64_t need, hipStream_t s) {
+  if (need <= 0) return MX_OK;
+  if (given) {
+    MX_REQUIRE(have >= need, MX_ERR_WORKSPACE, who, ": workspace of ", have, " bytes, ", need, " needed");
+    MX_REQUIRE((reinterpret_cast<uintptr_t>(given) & 15u) == 0, MX_ERR_INVALID, who, ": workspace is not 16-byte aligned");
+    ptr = given;
+    return MX_OK;
+  }
+  MX_REQUIRE(may_allocate(s), MX_ERR_WORKSPACE, who, ": a captured call takes its ", need,
+             " bytes of workspace from the caller");
+  MX_TRY(own_.alloc(size_t(need), s));
+  ptr = own_.ptr;
+  return MX_OK;
+}
+
 }  // namespace mx

@@ -43,7 +43,9 @@ EXPORTS = [
     "mx_unary_f32", "mx_unary_backward_f32", "mx_upsample_nearest2d", "mx_upsample_nearest2d_backward",
     "mx_softmax_f32", "mx_softmax_backward_f32", "mx_mse_loss_f32", "mx_mse_loss_backward_f32", "mx_copy_rows",
     "mx_foreach_f32", "mx_conv2d_plan", "mx_gemm_variant", "mx_conv2d_backward_weight_noalloc",
-    "mx_conv2d_backward_one_launch",
+    "mx_conv2d_backward_one_launch", "mx_layer_norm_forward", "mx_layer_norm_backward",
+    "mx_layer_norm_backward_workspace", "mx_linear_forward", "mx_linear_backward", "mx_linear_workspace",
+    "mx_orthogonalize", "mx_orthogonalize_workspace", "mx_muon_step", "mx_muon_workspace",
 ]
 
 
@@ -87,6 +89,24 @@ class AdamWHParams(C.Structure):
 class ForeachTensor(C.Structure):
     _fields_ = [("out", C.c_void_p), ("a", C.c_void_p), ("b", C.c_void_p), ("c", C.c_void_p),
                 ("numel", C.c_int64), ("scalar", C.c_double)]
+
+
+class NewtonSchulz(C.Structure):
+    _fields_ = [("steps", C.c_int64), ("a", C.c_double), ("b", C.c_double), ("c", C.c_double), ("eps", C.c_double)]
+
+
+class MatrixPair(C.Structure):
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
+
+
+class MuonTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("momentum_buffer", C.c_void_p), ("rows", C.c_int64),
+                ("cols", C.c_int64)]
+
+
+class MuonHParams(C.Structure):
+    _fields_ = [("lr", C.c_double), ("weight_decay", C.c_double), ("momentum", C.c_double), ("nesterov", C.c_int),
+                ("adjust_lr", C.c_int), ("ns", NewtonSchulz)]
 
 
 class MemoryStats(C.Structure):
@@ -172,6 +192,16 @@ def lib() -> C.CDLL:
             "mx_mse_loss_f32": ([vp, vp, i64, i32, vp, vp], i32),
             "mx_mse_loss_backward_f32": ([vp, vp, vp, i64, i32, vp, vp], i32),
             "mx_copy_rows": ([vp, i64, vp, i64, i64, i64, vp], i32),
+            "mx_layer_norm_forward": ([vp, vp, vp, i64, i64, C.c_float, vp, vp, vp, vp], i32),
+            "mx_layer_norm_backward": ([vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp], i32),
+            "mx_layer_norm_backward_workspace": ([i64, i64, C.POINTER(i64)], i32),
+            "mx_linear_forward": ([vp, vp, vp, vp, i64, i64, i64, i32, vp, vp, vp, i64, vp], i32),
+            "mx_linear_backward": ([vp, vp, vp, vp, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp], i32),
+            "mx_linear_workspace": ([i64, i64, i64, i32, i32, C.POINTER(i64)], i32),
+            "mx_orthogonalize": ([C.POINTER(MatrixPair), i64, C.POINTER(NewtonSchulz), vp, i64, vp], i32),
+            "mx_orthogonalize_workspace": ([C.POINTER(MatrixPair), i64, C.POINTER(i64)], i32),
+            "mx_muon_step": ([C.POINTER(MuonTensor), i64, C.POINTER(MuonHParams), vp, i64, vp], i32),
+            "mx_muon_workspace": ([C.POINTER(MuonTensor), i64, C.POINTER(i64)], i32),
             "mx_foreach_f32": ([i32, C.POINTER(ForeachTensor), i64, C.POINTER(i64), vp], i32),
         }
         for name, (args, res) in sig.items():
@@ -418,6 +448,120 @@ def foreach(op, outs, a, b=None, c=None, scalars=0.0, stream=None) -> int:
     launches = C.c_int64(0)
     check(lib().mx_foreach_f32(op, arr, n, C.byref(launches), stream))
     return launches.value
+
+
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)
+ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu": ACT_GELU, "gelu_tanh": ACT_GELU_TANH}
+MUON_ADJUST = {"original": 0, "match_rms_adamw": 1}
+
+
+def _bytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _workspace_query(fn, *args) -> int:
+    out = C.c_int64(0)
+    check(fn(*args, C.byref(out)))
+    return out.value
+
+
+def layer_norm_forward(x, gamma, beta, eps, y, mean, rstd, stream=None) -> None:
+    """Layer norm over the last axis of x (contiguous FP32); gamma, beta, mean
+    and rstd may be None."""
+    cols = x.shape[-1]
+    check(lib().mx_layer_norm_forward(ptr(x), ptr(gamma), ptr(beta), x.numel() // cols if cols else 0, cols, eps, ptr(y),
+                                      ptr(mean), ptr(rstd), stream))
+
+
+def layer_norm_backward(dy, x, mean, rstd, gamma, dx, dgamma, dbeta, workspace=None, stream=None) -> None:
+    """Any of dx, dgamma, dbeta may be None (not computed).  ``workspace``: a
+    device tensor of at least layer_norm_backward_workspace bytes, for calls
+    under graph capture; None takes it from the library's allocator."""
+    cols = x.shape[-1]
+    check(lib().mx_layer_norm_backward(ptr(dy), ptr(x), ptr(mean), ptr(rstd), ptr(gamma), x.numel() // cols if cols else 0,
+                                       cols, ptr(dx), ptr(dgamma), ptr(dbeta), ptr(workspace), _bytes(workspace), stream))
+
+
+def layer_norm_backward_workspace(rows: int, cols: int) -> int:
+    return _workspace_query(lib().mx_layer_norm_backward_workspace, rows, cols)
+
+
+def linear_forward(x, w, bias, y, activation=ACT_NONE, residual=None, z=None, workspace=None, stream=None) -> None:
+    """y = act(x w^T + bias) + residual for contiguous FP32 x [m, k], w [n, k];
+    z, if given, receives the activation's input."""
+    (m, k), n = x.shape, w.shape[0]
+    check(lib().mx_linear_forward(ptr(x), ptr(w), ptr(bias), ptr(residual), m, k, n, activation, ptr(y), ptr(z),
+                                  ptr(workspace), _bytes(workspace), stream))
+
+
+def linear_backward(dy, x, w, z, dx, dw, db, activation=ACT_NONE, workspace=None, stream=None) -> None:
+    """Gradients of linear_forward (the residual's is dy); any of dx, dw, db
+    may be None, z may be None without an activation."""
+    (m, k), n = x.shape, w.shape[0]
+    check(lib().mx_linear_backward(ptr(dy), ptr(x), ptr(w), ptr(z), m, k, n, activation, ptr(dx), ptr(dw), ptr(db),
+                                   ptr(workspace), _bytes(workspace), stream))
+
+
+def linear_workspace(m: int, k: int, n: int, activation=ACT_NONE, backward=False) -> int:
+    return _workspace_query(lib().mx_linear_workspace, m, k, n, activation, 1 if backward else 0)
+
+
+def _newton_schulz(steps, coefficients, eps) -> NewtonSchulz:
+    a, b, c = coefficients
+    return NewtonSchulz(int(steps), a, b, c, eps)
+
+
+def _pairs(inputs, outs):
+    if len(inputs) != len(outs):
+        raise ValueError(f"orthogonalize: {len(inputs)} inputs, {len(outs)} outputs")
+    arr = (MatrixPair * max(1, len(inputs)))()
+    for e, i, o in zip(arr, inputs, outs):
+        if i.shape != o.shape or i.dim() != 2:
+            raise ValueError(f"orthogonalize: expected matrices of one shape, got {tuple(i.shape)} and {tuple(o.shape)}")
+        e.in_, e.out, (e.rows, e.cols) = i.data_ptr(), o.data_ptr(), i.shape
+    return arr
+
+
+def orthogonalize(inputs, outs, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, workspace=None,
+                  stream=None) -> None:
+    """outs[i] = the Newton-Schulz approximation of inputs[i]'s polar factor
+    (lists of contiguous FP32 matrices)."""
+    arr = _pairs(inputs, outs)
+    ns = _newton_schulz(steps, coefficients, eps)
+    check(lib().mx_orthogonalize(arr, len(inputs), C.byref(ns), ptr(workspace), _bytes(workspace), stream))
+
+
+def orthogonalize_workspace(inputs) -> int:
+    return _workspace_query(lib().mx_orthogonalize_workspace, _pairs(inputs, inputs), len(inputs))
+
+
+def _muon_table(params, grads, momentum_buffers):
+    if not len(params) == len(grads) == len(momentum_buffers):
+        raise ValueError("muon_step: parameter, gradient and momentum lists differ in length")
+    arr = (MuonTensor * max(1, len(params)))()
+    for e, p, g, m in zip(arr, params, grads, momentum_buffers):
+        if p.dim() != 2 or p.shape != g.shape or p.shape != m.shape:
+            raise ValueError(f"muon_step: expected matrices of one shape, got {tuple(p.shape)}, {tuple(g.shape)}, "
+                             f"{tuple(m.shape)}")
+        e.param, e.grad, e.momentum_buffer, (e.rows, e.cols) = p.data_ptr(), g.data_ptr(), m.data_ptr(), p.shape
+    return arr
+
+
+def muon_step(params, grads, momentum_buffers, *, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, steps=5,
+              coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, adjust_lr="original", workspace=None,
+              stream=None) -> None:
+    """One orthogonalised momentum step over lists of contiguous FP32 matrices
+    (parameters and momentum buffers are updated in place)."""
+    arr = _muon_table(params, grads, momentum_buffers)
+    if adjust_lr not in MUON_ADJUST:
+        raise ValueError(f"muon_step: adjust_lr must be one of {sorted(MUON_ADJUST)}, got {adjust_lr!r}")
+    hp = MuonHParams(lr, weight_decay, momentum, 1 if nesterov else 0, MUON_ADJUST[adjust_lr],
+                     _newton_schulz(steps, coefficients, eps))
+    check(lib().mx_muon_step(arr, len(params), C.byref(hp), ptr(workspace), _bytes(workspace), stream))
+
+
+def muon_workspace(params) -> int:
+    return _workspace_query(lib().mx_muon_workspace, _muon_table(params, params, params), len(params))
 
 
 def conv2d_kernel_name(d: ConvDesc, phase: int, algo: int = ALGO_AUTO) -> str:
