@@ -25,8 +25,10 @@ namespace {
 
 using namespace pieces;
 
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
 constexpr int kBatch = 48;      // matrices of one set of launches
-constexpr int kNormParts = 64;  // partial squares of one matrix
+constexpr int kNormParts = 1024;  // most partial squares of one matrix
 constexpr int64_t kMaxScratch = int64_t(1) << 30;  // of one set, unless one matrix takes more
 
 // The matrices of one set of launches, all of one shape.
@@ -45,14 +47,34 @@ struct Update {
 };
 
 // Squares of U, in double (FP32 squares of a gradient overflow at 2^64 and
-// vanish at 2^-75), and the new momentum.
+// vanish at 2^-75), and the new momentum.  16 bytes at a time where VEC (all
+// tensors 16-byte aligned).
+template <bool VEC>
 __global__ __launch_bounds__(256) void norm_kernel(Table tab, Update up, int64_t numel, double* parts) {
   __shared__ double sum[4];
   const int b = blockIdx.y;
   const float* const in = tab.in[b];
   float* const buf = tab.buf[b];
   double s = 0;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < numel; i += int64_t(gridDim.x) * 256) {
+  const int64_t first = int64_t(blockIdx.x) * 256 + threadIdx.x, step = int64_t(gridDim.x) * 256;
+  const int64_t vecs = VEC ? numel / 4 : 0;
+#pragma unroll 4
+  for (int64_t i = first; i < vecs; i += step) {
+    f32x4 u = reinterpret_cast<const f32x4*>(in)[i];
+    if (up.muon) {
+      f32x4 m = reinterpret_cast<const f32x4*>(buf)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        m[e] = up.moved(m[e], u[e]);
+        u[e] = up.u(m[e], u[e]);
+      }
+      reinterpret_cast<f32x4*>(buf)[i] = m;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += double(u[e]) * double(u[e]);
+  }
+#pragma unroll 4
+  for (int64_t i = vecs * 4 + first; i < numel; i += step) {
     float u = in[i];
     if (up.muon) {
       const float m = up.moved(buf[i], u);
@@ -65,6 +87,17 @@ __global__ __launch_bounds__(256) void norm_kernel(Table tab, Update up, int64_t
   if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) parts[b * kNormParts + blockIdx.x] = sum[0] + sum[1] + sum[2] + sum[3];
+}
+
+// |U|_F from its partial squares, to every thread of a workgroup of 256.
+__device__ __forceinline__ double norm_of(const double* parts, int nparts) {
+  __shared__ double sum[4];
+  double s = 0;
+  for (int i = threadIdx.x; i < nparts; i += 256) s += parts[i];
+  for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
+  if ((threadIdx.x & 63) == 0) sum[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return sqrt(sum[0] + sum[1] + sum[2] + sum[3]);
 }
 
 struct Geometry {
@@ -81,35 +114,41 @@ struct Geometry {
 __global__ __launch_bounds__(256) void pack_kernel(Table tab, Update up, Geometry g, const double* parts, int nparts,
                                                    double eps, float scale, double growth, _Float16* x,
                                                    float* lift) {
-  __shared__ double inv;
   const int b = blockIdx.z;
-  if (threadIdx.x < 64) {
-    double s = int(threadIdx.x) < nparts ? parts[b * kNormParts + threadIdx.x] : 0.0;
-    for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
-    const double n = sqrt(s);
-    if (threadIdx.x == 0) {
-      // |X|_F is 1, unless eps is what divides: then X is kept times 2^e, which
-      // no iteration's growth takes past the bounds, so that fp16 holds it.
-      const double d = n < eps ? eps : n, small = n / d * growth;
-      const int e = small > 0 && small < 1 ? int(floor(-log2(small))) : 0;
-      inv = ldexp(double(scale), e) / d;
-      if (blockIdx.x == 0 && blockIdx.y == 0) lift[b] = float(ldexp(1.0, -e));
-    }
-  }
-  __syncthreads();
+  // |X|_F is 1, unless eps is what divides: then X is kept times 2^e, which no
+  // iteration's growth takes past the bounds, so that fp16 holds it.
+  const double n = norm_of(parts + b * kNormParts, nparts), d = n < eps ? eps : n, small = n / d * growth;
+  const int up2 = small > 0 && small < 1 ? int(floor(-log2(small))) : 0;
+  const double inv = ldexp(double(scale), up2) / d;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) lift[b] = float(ldexp(1.0, -up2));
   const float* const in = tab.in[b];
   const float* const buf = tab.buf[b];
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), col = blockIdx.x * 64 + (threadIdx.x >> 5) * 8;
+  float u[8] = {}, m[8] = {};
+  const auto take = [&](const float* from, float (&to)[8]) {
+    if (row >= g.s || col >= g.l) return;
+    if (g.turned) {  // neighbours along U's rows in neighbouring lanes
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = col + e < g.l ? from[int64_t(col + e) * g.cols + row] : 0.f;
+    } else if (col + 8 <= g.l) {
+      const f32x4u* const at = reinterpret_cast<const f32x4u*>(from + int64_t(row) * g.cols + col);
+      const f32x4 a = at[0], c = at[1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        to[e] = a[e];
+        to[4 + e] = c[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = col + e < g.l ? from[int64_t(row) * g.cols + col + e] : 0.f;
+    }
+  };
+  take(in, u);
+  if (up.muon) take(buf, m);
   half8 hi, lo;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float v = 0.f;
-    if (row < g.s && col + e < g.l) {
-      const int64_t at = g.turned ? int64_t(col + e) * g.cols + row : int64_t(row) * g.cols + col + e;
-      float u = in[at];
-      if (up.muon) u = up.u(buf[at], u);
-      v = float(double(u) * inv);
-    }
+    const float v = float(double(up.muon ? up.u(m[e], u[e]) : u[e]) * inv);
     hi[e] = _Float16(v);
     lo[e] = _Float16(v - float(hi[e]));
   }
@@ -119,7 +158,8 @@ __global__ __launch_bounds__(256) void pack_kernel(Table tab, Update up, Geometr
   *reinterpret_cast<half8*>(to + plane) = lo;
 }
 
-enum Kind { kGram, kPoly, kNext, kLast };
+// kLast: U's rows are X's columns; kLastRows: U's rows are X's.
+enum Kind { kGram, kPoly, kNext, kLast, kLastRows };
 
 struct StepArgs {
   const _Float16 *a, *b;  // operands (kPoly: both G)
@@ -128,6 +168,10 @@ struct StepArgs {
   int a_rows, b_rows, out_rows;
   int nk;                 // slabs
   int tiles_m, tiles_n, batch;
+  // Tiles from `whole` on are taken by `parts` workgroups each, which leave
+  // their sums of a share of the slabs in `sums` for join_kernel.
+  int whole, parts;
+  float* sums;
   float alpha;            // product of pieces -> stored value
   float diag, lin, unit;  // kPoly: a, b and 1 / G's scale, times the stored scale
   const float* lift;      // X's pieces hold X / lift[matrix]
@@ -138,72 +182,176 @@ struct StepArgs {
   float decay, step;      // 1 - lr wd, lr r
 };
 
-template <class T, int KIND>
-__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void step_kernel(StepArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
-  constexpr bool COLS = KIND == kNext || KIND == kLast;
-  const int per = p.tiles_m * p.tiles_n;
-  const int id = mfma::xcd_remap(blockIdx.x, per * p.batch), b = id / per;
-  int tm, tn;
-  mfma::tile_coords(id - b * per, p.tiles_m, p.tiles_n, tm, tn);
-  const int m0 = tm * T::BM, n0 = tn * T::BN;
-  const Planes pa{const_cast<_Float16*>(p.a) + b * 2 * p.a_plane, p.a_plane, p.a_rows};
-  const Planes pb{const_cast<_Float16*>(p.b) + b * 2 * p.b_plane, p.b_plane, p.b_rows};
-  f32x16 acc[T::FM][T::FN];
-  product<T, COLS>(acc, pa, pb, m0, n0, p.nk, smem);
-  // G's pieces hold G itself: where X is tiny, all of it that b G and c G^2 add
-  // to a I lies below what G's scale can hold.
-  float alpha = p.alpha;
-  if constexpr (KIND == kGram) alpha *= p.lift[b] * p.lift[b];
-  if constexpr (KIND == kLast) alpha *= p.lift[b];
-  if constexpr (KIND == kLast) {
-    float* const out = p.tab.out[b];
-    for_each4<T>(acc, [&](int m, int n, const float(&v)[4]) {
-      const int r = m0 + m, c = n0 + n;
-      if (r >= p.g.s) return;
+constexpr bool symmetric(int kind) { return kind == kGram || kind == kPoly; }
+
+// Tile t of the lower triangle of n x n tiles, in bands of eight tile rows
+// walked column by column: tiles that run together share rows of both operands
+// (row by row, 64 neighbours read 65 panels; so, 16).
+__device__ __forceinline__ void lower_tile(int t, int n, int& tm, int& tn) {
+  // Band g begins at 32 g^2 + 4 g.
+  int g = int((sqrtf(16.f + 128.f * float(t)) - 4.f) / 64.f);
+  while (32 * g * g + 4 * g > t) --g;
+  while (32 * (g + 1) * (g + 1) + 4 * (g + 1) <= t) ++g;
+  const int first = 8 * g, rows = min(8, n - first);
+  t -= 32 * g * g + 4 * g;
+  if (t < first * rows) {
+    tm = first + t % rows;
+    tn = t / rows;
+    return;
+  }
+  t -= first * rows;
+  int r = 0;
+  while (t > r) t -= ++r;
+  tm = first + r;
+  tn = first + t;
+}
+
+template <int KIND>
+__device__ __forceinline__ void tile_of(const StepArgs& p, int id, int& b, int& tm, int& tn) {
+  const int per = symmetric(KIND) ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  b = id / per;
+  if constexpr (symmetric(KIND))
+    lower_tile(id - b * per, p.tiles_m, tm, tn);
+  else
+    mfma::tile_coords(id - b * per, p.tiles_m, p.tiles_n, tm, tn);
+}
+
+// Stores a 32 x 32 fragment of a product at row m, column n (of X for the last
+// product).  mirror: its transpose too.
+template <int KIND>
+__device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, int m, int n, const f32x16& v) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (KIND == kLast || KIND == kLastRows) {
+    // A wave writes whole 128-byte lines of U's rows either way round.
+    const float alpha = p.alpha * p.lift[b];
+    const int col = (KIND == kLast ? m : n) + (lane & 31), row0 = (KIND == kLast ? n : m) + 4 * (lane >> 5);
+    float* const to = p.tab.out[b] + int64_t(row0) * p.g.cols + col;
+    const bool in = col < p.g.cols;
+    float was[16];
+    if (p.muon) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (c + e >= p.g.l) break;
-        const int64_t at = p.g.turned ? int64_t(c + e) * p.g.cols + r : int64_t(r) * p.g.cols + c + e;
-        const float x = v[e] * alpha;
-        out[at] = p.muon ? out[at] * p.decay - p.step * x : x;
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i >> 2) + (i & 3);
+        was[i] = in && row0 + r < p.g.rows ? to[int64_t(r) * p.g.cols] * p.decay : 0.f;
       }
-    });
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = 8 * (i >> 2) + (i & 3);
+      const float x = v[i] * alpha;
+      if (in && row0 + r < p.g.rows) to[int64_t(r) * p.g.cols] = p.muon ? was[i] - p.step * x : x;
+    }
   } else {
+    // G's pieces hold G itself: where X is tiny, all of it that b G and c G^2
+    // add to a I lies below what G's scale can hold.
+    const float alpha = KIND == kGram ? p.alpha * p.lift[b] * p.lift[b] : p.alpha;
     const Planes po{p.out + b * 2 * p.out_plane, p.out_plane, p.out_rows};
-    for_each4<T>(acc, [&](int m, int n, const float(&v)[4]) {
-      const int r = m0 + m, c = n0 + n;
+    const int r = m + (lane & 31), c0 = n + 4 * (lane >> 5);
+    half4 gh[4], gl[4];
+    if constexpr (KIND == kPoly) {
+      const _Float16* const g = p.a + b * 2 * p.a_plane;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        gh[q] = *reinterpret_cast<const half4*>(g + elem(po, r, c0 + 8 * q));
+        gl[q] = *reinterpret_cast<const half4*>(g + p.a_plane + elem(po, r, c0 + 8 * q));
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = c0 + 8 * q;
       const int64_t at = elem(po, r, c);
       float o[4];
-      if constexpr (KIND == kPoly) {
-        const half4 gh = *reinterpret_cast<const half4*>(pa.at + at), gl = *reinterpret_cast<const half4*>(pa.at + pa.plane + at);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(gh[e]) + float(gl[e])) * p.unit) + alpha * v[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = alpha * v[e];
+      for (int e = 0; e < 4; ++e) {
+        o[e] = alpha * v[4 * q + e];
+        if constexpr (KIND == kPoly)
+          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(gh[q][e]) + float(gl[q][e])) * p.unit) + o[e];
       }
       half4 hi, lo;
       split4(o, hi, lo);
       *reinterpret_cast<half4*>(po.at + at) = hi;
       *reinterpret_cast<half4*>(po.at + po.plane + at) = lo;
-    });
+      if constexpr (symmetric(KIND)) {
+        if (mirror) {  // each lane takes a row of its four lanes' block
+          const int64_t across = elem(po, c + (r & 3), r & ~3);
+          *reinterpret_cast<half4*>(po.at + across) = transpose4(hi);
+          *reinterpret_cast<half4*>(po.at + po.plane + across) = transpose4(lo);
+        }
+      }
+    }
   }
+}
+
+// One product of the iteration.  G and P are symmetric: only the tiles on and
+// below the diagonal are computed, and stored both ways.
+template <class T, int KIND>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void step_kernel(StepArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
+  constexpr bool SYM = symmetric(KIND);
+  int id = blockIdx.x, part = 0, k0 = 0, k1 = p.nk;
+  if (id < p.whole) {
+    id = mfma::xcd_remap(id, p.whole);
+  } else {
+    part = (id - p.whole) % p.parts;
+    k0 = part * (p.nk / 4) / p.parts * 4;
+    k1 = (part + 1) * (p.nk / 4) / p.parts * 4;
+    id = p.whole + (id - p.whole) / p.parts;
+  }
+  int b, tm, tn;
+  tile_of<KIND>(p, id, b, tm, tn);
+  const Planes pa{const_cast<_Float16*>(p.a) + b * 2 * p.a_plane, p.a_plane, p.a_rows};
+  const Planes pb{const_cast<_Float16*>(p.b) + b * 2 * p.b_plane, p.b_plane, p.b_rows};
+  f32x16 acc[T::FM][T::FN];
+  product<T, !SYM, KIND == kLastRows>(acc, pa, pb, tm * T::BM, tn * T::BN, k0, k1 - k0, smem);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (id >= p.whole) {
+    f32x4* const to = reinterpret_cast<f32x4*>(p.sums) +
+                      ((int64_t(id - p.whole) * p.parts + part) * T::WAVES + wave) * (T::FM * T::FN * 256) + lane;
+#pragma unroll
+    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to[((i * T::FN + j) * 4 + q) * 64] =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    return;
+  }
+  const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
+#pragma unroll
+  for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::FN; ++j) finish<KIND>(p, b, tm != tn, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+}
+
+// The tiles that were taken in parts: a wave per 32 x 32 fragment sums the
+// parts in their order.
+template <class T, int KIND>
+__global__ __launch_bounds__(64) void join_kernel(StepArgs p) {
+  constexpr int FRAGS = T::FM * T::FN, PER = T::WAVES * FRAGS;
+  const int tile = blockIdx.x / PER, wave = blockIdx.x % PER / FRAGS, f = blockIdx.x % FRAGS;
+  int b, tm, tn;
+  tile_of<KIND>(p, p.whole + tile, b, tm, tn);
+  const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) +
+                      ((int64_t(tile) * p.parts * T::WAVES + wave) * FRAGS + f) * 256 + threadIdx.x;
+  f32x4 s[4] = {};
+#pragma unroll 4
+  for (int q = 0; q < p.parts; ++q) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s[g] += from[int64_t(q) * PER * 256 + g * 64];
+  }
+  f32x16 v;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = s[e >> 2][e & 3];
+  finish<KIND>(p, b, tm != tn, tm * T::BM + wave / T::WN * (T::BM / T::WM) + f / T::FN * 32,
+               tn * T::BN + wave % T::WN * (T::BN / T::WN) + f % T::FN * 32, v);
 }
 
 // steps == 0: the scaled matrix itself.
 __global__ __launch_bounds__(256) void scaled_kernel(Table tab, Update up, int64_t numel, const double* parts, int nparts,
                                                      double eps, float decay, float step) {
-  __shared__ double inv;
   const int b = blockIdx.y;
-  if (threadIdx.x < 64) {
-    double s = int(threadIdx.x) < nparts ? parts[b * kNormParts + threadIdx.x] : 0.0;
-    for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
-    const double n = sqrt(s);
-    if (threadIdx.x == 0) inv = 1.0 / (n < eps ? eps : n);
-  }
-  __syncthreads();
+  const double n = norm_of(parts + b * kNormParts, nparts), inv = 1.0 / (n < eps ? eps : n);
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < numel; i += int64_t(gridDim.x) * 256) {
     float u = tab.in[b][i];
     if (up.muon) u = up.u(tab.buf[b][i], u);
@@ -212,58 +360,120 @@ __global__ __launch_bounds__(256) void scaled_kernel(Table tab, Update up, int64
   }
 }
 
-using Tile64 = Tile<64, 64, 2, 2, 4, 2>;     // 4 waves of 32 x 32
-using Tile128 = Tile<128, 128, 2, 2, 2, 2>;  // 4 waves of 64 x 64
-using Tile256 = Tile<256, 256, 2, 4, 2, 2>;  // 8 waves of 128 x 64
+using Tile64 = Tile<64, 64, 2, 2, 4>;     // 4 waves of 32 x 32
+using Tile128 = Tile<128, 128, 2, 2, 2>;  // 4 waves of 64 x 64
+using Tile256 = Tile<256, 256, 2, 4, 2>;  // 8 waves of 128 x 64
 
-template <class T>
-int launch(int kind, StepArgs& p, int m, int n, hipStream_t s) {
-  p.tiles_m = m / T::BM;
-  p.tiles_n = n / T::BN;
-  const dim3 grid(unsigned(p.tiles_m * p.tiles_n * p.batch)), block(T::THREADS);
-  switch (kind) {
-    case kGram: hipLaunchKernelGGL((step_kernel<T, kGram>), grid, block, 0, s, p); break;
-    case kPoly: hipLaunchKernelGGL((step_kernel<T, kPoly>), grid, block, 0, s, p); break;
-    case kNext: hipLaunchKernelGGL((step_kernel<T, kNext>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((step_kernel<T, kLast>), grid, block, 0, s, p);
-  }
+template <class T, int KIND>
+int launch(const StepArgs& p, int tiles, hipStream_t s) {
+  const int rest = tiles - p.whole;
+  hipLaunchKernelGGL((step_kernel<T, KIND>), dim3(unsigned(p.whole + rest * p.parts)), dim3(T::THREADS), 0, s, p);
   MX_HIP(hipGetLastError());
+  if (rest) {
+    hipLaunchKernelGGL((join_kernel<T, KIND>), dim3(unsigned(rest * T::WAVES * T::FM * T::FN)), dim3(64), 0, s, p);
+    MX_HIP(hipGetLastError());
+  }
   return MX_OK;
 }
 
-int launch_tile(int tile, int kind, StepArgs& p, int m, int n, hipStream_t s) {
-  if (tile == 256) return launch<Tile256>(kind, p, m, n, s);
-  if (tile == 128) return launch<Tile128>(kind, p, m, n, s);
-  return launch<Tile64>(kind, p, m, n, s);
+template <class T>
+int launch_kind(int kind, const StepArgs& p, int tiles, hipStream_t s) {
+  switch (kind) {
+    case kGram: return launch<T, kGram>(p, tiles, s);
+    case kPoly: return launch<T, kPoly>(p, tiles, s);
+    case kNext: return launch<T, kNext>(p, tiles, s);
+    case kLast: return launch<T, kLast>(p, tiles, s);
+    default: return launch<T, kLastRows>(p, tiles, s);
+  }
 }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Tile of a set: the largest that still gives every CU work in the smaller
-// products (G and P have s x s entries).
-int pick_tile(int64_t s, int64_t batch) {
-  const auto tiles = [&](int64_t t) { return up(s, t) / t * (up(s, t) / t) * batch; };
-  const int64_t cu = cu_count();
-  if (tiles(256) >= cu) return 256;
-  if (tiles(128) >= cu) return 128;
-  return 64;
+// A CU's time per slab with n workgroups of a tile on it, and how many it
+// holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.
+struct TileCost {
+  int tile, per_cu;
+  double fixed, each;
+  double slab(double n) const { return fixed + each * n; }
+};
+constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.20, 0.21}, {256, 1, 0.0, 1.15}};
+
+// How a product's tiles are dealt: whole rounds of the chip, then what is left
+// over in parts along K where a join (a launch and a pass over the sums) costs
+// less than the round that it shortens.
+struct Deal {
+  int64_t tiles, whole;
+  int parts;
+  double time;
+};
+Deal deal(const TileCost& c, int64_t tiles, int64_t nk, int64_t cu) {
+  Deal d{tiles, tiles, 1, 3.0};
+  const int64_t slots = cu * c.per_cu, full = tiles / slots, rest = tiles - full * slots;
+  d.time += double(full * nk) * c.slab(c.per_cu);
+  if (!rest) return d;
+  const double plain = double(nk) * c.slab(double((rest + cu - 1) / cu));
+  const int64_t parts = std::min<int64_t>({slots / rest, nk / 8, 16});
+  if (parts >= 2) {
+    const double share = double((nk / 4 + parts - 1) / parts * 4);
+    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 5.0 +
+                         double(rest * parts) * c.tile * c.tile * 8.0 / 3e6;
+    if (split < plain) {
+      d.whole = full * slots;
+      d.parts = int(parts);
+      d.time += split;
+      return d;
+    }
+  }
+  d.time += plain;
+  return d;
 }
 
-Geometry geometry(int64_t rows, int64_t cols, int tile) {
-  Geometry g{};
-  g.rows = int(rows);
-  g.cols = int(cols);
-  g.turned = rows > cols;
-  g.s = int(std::min(rows, cols));
-  g.l = int(std::max(rows, cols));
-  g.sp = int(up(g.s, tile));
-  g.lp = int(up(g.l, tile));
-  return g;
+// Tiles of a set's products (the symmetric ones and the others), what its sides
+// are padded to, and how the tiles are dealt.
+struct Plan {
+  Geometry g;
+  int sym, next;  // indexes into kTiles
+  Deal gram, poly, update;
+  int64_t sums;   // bytes of partial sums
+};
+
+Plan plan_set(int64_t rows, int64_t cols, int64_t batch) {
+  Plan best{};
+  double least = -1;
+  const int64_t cu = cu_count(), s = std::min(rows, cols), l = std::max(rows, cols);
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j) {
+      const TileCost &a = kTiles[i], &c = kTiles[j];
+      const int pad = std::max(a.tile, c.tile);
+      const int64_t sp = up(s, pad), lp = up(l, pad), n = sp / a.tile;
+      Plan p{};
+      p.g.rows = int(rows);
+      p.g.cols = int(cols);
+      p.g.turned = rows > cols;
+      p.g.s = int(s);
+      p.g.l = int(l);
+      p.g.sp = int(sp);
+      p.g.lp = int(lp);
+      p.sym = i;
+      p.next = j;
+      p.gram = deal(a, n * (n + 1) / 2 * batch, lp / kBK, cu);
+      p.poly = deal(a, n * (n + 1) / 2 * batch, sp / kBK, cu);
+      p.update = deal(c, (sp / c.tile) * (lp / c.tile) * batch, sp / kBK, cu);
+      const double time = p.gram.time + p.poly.time + p.update.time;
+      if (least >= 0 && time >= least) continue;
+      least = time;
+      const auto bytes = [](const Deal& d, int tile) { return (d.tiles - d.whole) * d.parts * tile * tile * 4; };
+      p.sums = std::max({bytes(p.gram, a.tile), bytes(p.poly, a.tile), bytes(p.update, c.tile)});
+      best = p;
+    }
+  return best;
 }
 
-// Scratch of a set of `batch` matrices: X twice, G, P, and the squares.
-int64_t set_bytes(const Geometry& g, int64_t batch) {
-  return batch * (2 * g.x_plane() * 4 + 2 * g.g_plane() * 4) + up(batch * (kNormParts * 8 + 4), 256);
+// Scratch of a set of `batch` matrices: X twice, G, P, the squares and the
+// partial sums.
+int64_t head_bytes(int64_t batch) { return up(batch * (kNormParts * 8 + 4), 256); }
+int64_t set_bytes(const Plan& p, int64_t batch) {
+  return batch * (2 * p.g.x_plane() * 4 + 2 * p.g.g_plane() * 4) + head_bytes(batch) + p.sums;
 }
 
 // Matrices of one shape that go through the launches together.
@@ -288,9 +498,8 @@ std::vector<Set> sets_of(int64_t count, Shape&& shape) {
       sets.push_back({rows, cols, {}});
     } else {
       // Padding is at most a 256-row tile a side.
-      const Set& f = sets[open[at]];
-      const int64_t next = int64_t(f.at.size()) + 1;
-      if (next > kBatch || set_bytes(geometry(rows, cols, 256), next) > kMaxScratch) {
+      const int64_t next = int64_t(sets[open[at]].at.size()) + 1, sp = up(std::min(rows, cols), 256);
+      if (next > kBatch || next * 8 * sp * (up(std::max(rows, cols), 256) + sp) > kMaxScratch) {
         open[at] = sets.size();
         sets.push_back({rows, cols, {}});
       }
@@ -304,7 +513,7 @@ int64_t workspace_of(const std::vector<Set>& sets) {
   int64_t most = 0;
   for (const Set& f : sets) {
     const int64_t n = int64_t(f.at.size());
-    most = std::max(most, set_bytes(geometry(f.rows, f.cols, pick_tile(std::min(f.rows, f.cols), n)), n));
+    most = std::max(most, set_bytes(plan_set(f.rows, f.cols, n), n));
   }
   return most;
 }
@@ -372,7 +581,7 @@ int check_ns(const char* who, const mx_newton_schulz& ns) {
 
 int check_shape(const char* who, int64_t i, int64_t rows, int64_t cols) {
   MX_REQUIRE(rows >= 0 && cols >= 0, MX_ERR_INVALID, who, ": negative size at ", i);
-  // Tile counts and byte offsets within a plane's 16-byte groups stay in int32.
+  // Byte offsets within a plane's groups of eight columns stay in int32.
   MX_REQUIRE(rows <= (1 << 24) && cols <= (1 << 24), MX_ERR_INVALID, who, ": side longer than 2^24 at ", i);
   return MX_OK;
 }
@@ -384,20 +593,29 @@ struct Finish {
 };
 
 // All launches of one set; `ws` holds set_bytes.
-int run_set(const Table& tab, int64_t batch, const Geometry& g, int tile, const mx_newton_schulz& ns,
-            const std::vector<Scales>& sc, const Finish& fin, char* ws, hipStream_t s) {
+int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_schulz& ns, const std::vector<Scales>& sc,
+            const Finish& fin, char* ws, hipStream_t s) {
+  const Geometry& g = plan.g;
   double* const parts = reinterpret_cast<double*>(ws);
   float* const lift = reinterpret_cast<float*>(parts + batch * kNormParts);
-  _Float16* x = reinterpret_cast<_Float16*>(ws + up(batch * (kNormParts * 8 + 4), 256));
+  _Float16* x = reinterpret_cast<_Float16*>(ws + head_bytes(batch));
   _Float16* x2 = x + batch * 2 * g.x_plane();
   _Float16* const gram = x2 + batch * 2 * g.x_plane();
   _Float16* const poly = gram + batch * 2 * g.g_plane();
   const int64_t numel = int64_t(g.rows) * g.cols;
-  const int nparts = int(std::min<int64_t>(kNormParts, std::max<int64_t>(1, (numel + 2047) / 2048)));
+  // Four 16-byte loads a thread, up to eight workgroups a CU over the set.
+  const int64_t most = std::min<int64_t>(kNormParts, std::max<int64_t>(1, int64_t(cu_count()) * 8 / batch));
+  const int nparts = int(std::min<int64_t>(most, (numel + 4095) / 4096));
   const double r = fin.adjust == MX_MUON_MATCH_RMS_ADAMW ? 0.2 * std::sqrt(double(std::max(g.rows, g.cols)))
                                                          : std::sqrt(std::max(1.0, double(g.rows) / g.cols));
   const float decay = float(1.0 - fin.lr * fin.decay), step = float(fin.lr * r);
-  hipLaunchKernelGGL(norm_kernel, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts);
+  bool vec = true;
+  for (int64_t i = 0; i < batch; ++i)
+    vec = vec && ((reinterpret_cast<uintptr_t>(tab.in[i]) | reinterpret_cast<uintptr_t>(tab.buf[i])) & 15) == 0;
+  if (vec)
+    hipLaunchKernelGGL(norm_kernel<true>, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts);
+  else
+    hipLaunchKernelGGL(norm_kernel<false>, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts);
   MX_HIP(hipGetLastError());
   if (ns.steps == 0) {
     hipLaunchKernelGGL(scaled_kernel, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts,
@@ -416,6 +634,17 @@ int run_set(const Table& tab, int64_t batch, const Geometry& g, int tile, const 
   p.muon = fin.up.muon;
   p.decay = decay;
   p.step = step;
+  p.sums = reinterpret_cast<float*>(poly + batch * 2 * g.g_plane());
+  const auto run = [&](int kind, const Deal& d, int t) -> int {
+    const int tile = kTiles[t].tile;
+    p.whole = int(d.whole);
+    p.parts = d.parts;
+    p.tiles_m = g.sp / tile;
+    p.tiles_n = (symmetric(kind) ? g.sp : g.lp) / tile;
+    if (t == 0) return launch_kind<Tile64>(kind, p, int(d.tiles), s);
+    if (t == 1) return launch_kind<Tile128>(kind, p, int(d.tiles), s);
+    return launch_kind<Tile256>(kind, p, int(d.tiles), s);
+  };
   for (int64_t i = 0; i < ns.steps; ++i) {
     const Scales c = sc[size_t(i)];
     p.a = p.b = x;
@@ -425,7 +654,7 @@ int run_set(const Table& tab, int64_t batch, const Geometry& g, int tile, const 
     p.out_plane = g.g_plane();
     p.nk = g.lp / kBK;
     p.alpha = c.g / c.x / c.x;
-    MX_TRY(launch_tile(tile, kGram, p, g.sp, g.sp, s));
+    MX_TRY(run(kGram, plan.gram, plan.sym));
     p.a = p.b = gram;
     p.a_plane = p.b_plane = g.g_plane();
     p.out = poly;
@@ -434,14 +663,14 @@ int run_set(const Table& tab, int64_t batch, const Geometry& g, int tile, const 
     p.diag = float(ns.a) * c.p;
     p.lin = float(ns.b) * c.p;
     p.unit = 1.f / c.g;
-    MX_TRY(launch_tile(tile, kPoly, p, g.sp, g.sp, s));
+    MX_TRY(run(kPoly, plan.poly, plan.sym));
     p.a = poly;
     p.b = x;
     p.b_plane = p.out_plane = g.x_plane();
     p.out = x2;
     const bool last = i + 1 == ns.steps;
     p.alpha = (last ? 1.f : sc[size_t(i) + 1].x) / c.p / c.x;
-    MX_TRY(launch_tile(tile, last ? kLast : kNext, p, g.sp, g.lp, s));
+    MX_TRY(run(!last ? kNext : g.turned ? kLast : kLastRows, plan.update, plan.next));
     std::swap(x, x2);
   }
   return MX_OK;
@@ -456,10 +685,9 @@ int run_all(const char* who, const std::vector<Set>& sets, const mx_newton_schul
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_of(sets), s));
   for (const Set& f : sets) {
     const int64_t batch = int64_t(f.at.size());
-    const int tile = pick_tile(std::min(f.rows, f.cols), batch);
     Table tab{};
     for (int64_t i = 0; i < batch; ++i) fill(f.at[size_t(i)], &tab, i);
-    MX_TRY(run_set(tab, batch, geometry(f.rows, f.cols, tile), tile, ns, sc, fin, ws.as<char>(), s));
+    MX_TRY(run_set(tab, batch, plan_set(f.rows, f.cols, batch), ns, sc, fin, ws.as<char>(), s));
   }
   return MX_OK;
 }

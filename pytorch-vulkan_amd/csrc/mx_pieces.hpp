@@ -22,6 +22,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace mx {
 namespace pieces {
@@ -32,7 +33,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBK = 32;  // columns of a slab
+constexpr int kBK = 16;     // columns of a slab: one step of the matrix instruction
+constexpr int kStages = 4;  // slabs in LDS
 
 // Planes of a matrix: hi at `at`, lo `plane` elements behind.
 struct Planes {
@@ -49,72 +51,99 @@ __device__ __forceinline__ void split4(const float (&v)[4], half4& hi, half4& lo
   }
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int OCC_>
+template <int BM_, int BN_, int WM_, int WN_, int OCC_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, OCC = OCC_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
   static constexpr int A_BYTES = 2 * BM * kBK * 2, B_BYTES = 2 * BN * kBK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int SMEM = STAGES * STAGE;
+  static constexpr int SMEM = kStages * STAGE;
   static constexpr int LA = A_BYTES / 1024 / WAVES, LB = B_BYTES / 1024 / WAVES;  // wave-wide loads of a slab
   static_assert(LA * WAVES * 1024 == A_BYTES && LB * WAVES * 1024 == B_BYTES, "whole loads");
 };
 
-typedef const __attribute__((address_space(1))) void gvoid;
-typedef __attribute__((address_space(3))) void lvoid;
+// An LDS address as the pointer that reads take.
+template <class V>
+__device__ __forceinline__ __attribute__((address_space(3))) V* lds_at(uint32_t at) {
+  return (__attribute__((address_space(3))) V*)(uintptr_t)at;
+}
 
-// 16 bytes a lane from memory to LDS, at `lds` + 16 * lane (lds wave-uniform).
-__device__ __forceinline__ void load_lds16(const char* src, char* lds) {
-  __builtin_amdgcn_global_load_lds((gvoid*)src, (lvoid*)lds, 16, 0, 0);
+// 16 bytes a lane from memory (a wave's base and each lane's offset) to LDS, at
+// lds + 16 * lane.  Written out because the compiler, which cannot tell the
+// slabs of a stage apart, waits for loads like these before any transposing
+// read; wait_loads() and barrier() are what orders them here.  No register of
+// the wave receives anything.
+__device__ __forceinline__ void load_lds16(const char* base, uint32_t lane_off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(lane_off), "s"(base)
+               : "memory");
+}
+
+// A pointer that is the same for a wave, in scalar registers.
+__device__ __forceinline__ const char* uniform(const void* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(int(uint32_t(a)));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(int(uint32_t(a >> 32)));
+  return reinterpret_cast<const char*>(uint64_t(hi) << 32 | lo);
 }
 
 // An operand's slabs.  ROWS: T rows of the matrix, the product running along
 // its columns; LDS [plane][k / 8][T][8].  COLS: T columns, the product running
-// along its rows; LDS [plane][T / 8][32][8], the rows of a group rearranged so
+// along its rows; LDS [plane][T / 8][16][8], the rows of a group rearranged so
 // that the transposing reads of 16 lanes meet every bank once.
 template <int T, int LOADS, int WAVES, bool COLS>
 struct Operand {
-  const char* src[LOADS];  // this lane's bytes of the next slab
+  const char* src[LOADS];  // the wave's part of the next slab
+  uint32_t lane_off;
   int64_t step;
-  __device__ __forceinline__ void init(const Planes& p, int first, int wave, int lane) {
+  __device__ __forceinline__ void init(const Planes& p, int first, int slab0, int wave, int lane) {
+    step = COLS ? int64_t(kBK) * 16 : int64_t(kBK / 8) * p.rows * 16;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int c = wave + i * WAVES;
       const _Float16* at;
       if constexpr (COLS) {
-        constexpr int PER = T / 16;  // loads of a plane: two groups of eight columns each
-        const int pl = c / PER, g = 2 * (c % PER) + (lane >> 5), r = (lane & 31) ^ ((g & 3) << 2);
-        at = p.at + pl * p.plane + (int64_t(first / 8 + g) * p.rows + r) * 8;
+        constexpr int PER = T / 32;  // loads of a plane: four groups of eight columns each
+        at = p.at + c / PER * p.plane + int64_t(first / 8 + 4 * (c % PER)) * p.rows * 8;
       } else {
-        constexpr int PER = 4 * T / 64;  // 64 rows of a group of eight columns each
-        const int pl = c / PER, kg = c % PER / (T / 64), r = c % (T / 64) * 64 + lane;
-        at = p.at + pl * p.plane + (int64_t(kg) * p.rows + first + r) * 8;
+        constexpr int PER = 2 * T / 64;  // 64 rows of a group of eight columns each
+        at = p.at + c / PER * p.plane + (int64_t(c % PER / (T / 64)) * p.rows + first + c % (T / 64) * 64) * 8;
       }
-      src[i] = reinterpret_cast<const char*>(at);
+      src[i] = uniform(at) + slab0 * step;
     }
-    step = COLS ? int64_t(kBK) * 16 : int64_t(kBK / 8) * p.rows * 16;
+    lane_off = COLS ? (uint32_t(lane >> 4) * uint32_t(p.rows) + uint32_t((lane & 15) ^ (lane >> 4 << 2))) * 16u : uint32_t(lane) * 16u;
   }
-  __device__ __forceinline__ void load(char* lds, int wave) {
+  __device__ __forceinline__ void load(uint32_t lds, int wave) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      load_lds16(src[i], lds + (wave + i * WAVES) * 1024);
+      load_lds16(src[i], lane_off, lds + uint32_t(wave + i * WAVES) * 1024u);
       src[i] += step;
     }
   }
-  // Rows (columns) first .. first + 31 at k 16 s .. 16 s + 15 of plane pl.
-  static __device__ __forceinline__ half8 frag(const char* lds, int pl, int first, int s, int lane) {
+  // Bytes from a slab's start to this lane's part of the fragment of rows
+  // (columns) first .. first + 31, first a multiple of 32; COLS: half h of it.
+  static __device__ __forceinline__ uint32_t lane_offset(int first, int lane, int h) {
     if constexpr (COLS) {
       const int c = lane & 15, g = first / 8 + ((lane & 16) >> 3) + ((c & 3) >> 1);
+      const int k = 8 * (lane >> 5) + (c >> 2) + 4 * h;
+      return uint32_t((g * 16 + (k ^ ((g & 3) << 2))) * 16 + 8 * (c & 1));
+    } else {
+      return uint32_t(((lane >> 5) * T + first + (lane & 31)) * 16);
+    }
+  }
+  // The fragment of plane pl, 32 j rows (columns) on, from the LDS address of
+  // this lane's parts; `off` is the slab's.
+  static __device__ __forceinline__ half8 frag(const uint32_t (&at)[COLS ? 2 : 1], int off, int pl, int j) {
+    const int to = off + pl * T * kBK * 2 + j * 32 * (COLS ? 32 : 16);
+    if constexpr (COLS) {
       s16x4 q[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = 16 * s + 8 * (lane >> 5) + (c >> 2) + 4 * h;
-        const char* at = lds + pl * T * kBK * 2 + (g * 32 + (k ^ ((g & 3) << 2))) * 16 + 8 * (c & 1);
-        q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-      }
+      for (int h = 0; h < 2; ++h)
+        q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(at[h] + to));
       return __builtin_bit_cast(half8, __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      return *reinterpret_cast<const half8*>(lds + pl * T * kBK * 2 + ((2 * s + (lane >> 5)) * T + first + (lane & 31)) * 16);
+      return *lds_at<const half8>(at[0] + to);
     }
   }
 };
@@ -124,85 +153,133 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);  // vmcnt(N) alone
 }
 
-// acc[i][j] += rows m0 + 32 i.. of A with rows (COLS: columns) n0 + 32 j.. of B
-// over nk slabs.  The matrix instruction's row operand is B: a lane ends with
-// four consecutive columns n of one row m, 8 bytes of a plane.
-template <class T, bool COLS>
+// A barrier that orders LDS accesses without waiting for loads on their way
+// there (__syncthreads waits for all of them).
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// acc[i][j] = rows m0 + 32 i.. of A with rows (COLS: columns) n0 + 32 j.. of B
+// over nk slabs from slab0 (nk a multiple of four, at least four).  The matrix instruction's
+// row operand is B, so that a lane ends with four consecutive columns n of one
+// row m, 8 bytes of a plane (ROW_LANES: A, and it ends with four rows of one
+// column, neighbours beside it).
+//
+// Slab t's products run from registers while slab t + 1's fragments are read
+// from LDS and slabs t + 2 and t + 3 come from memory, one barrier a slab.
+template <class T, bool COLS, bool ROW_LANES = false>
 __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Planes& a, const Planes& b, int m0, int n0,
-                                        int nk, char* smem) {
+                                        int slab0, int nk, char* smem) {
+  using OpA = Operand<T::BM, T::LA, T::WAVES, false>;
+  using OpB = Operand<T::BN, T::LB, T::WAVES, COLS>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN * (T::BM / T::WM), wn = wave % T::WN * (T::BN / T::WN);
-  Operand<T::BM, T::LA, T::WAVES, false> oa;
-  Operand<T::BN, T::LB, T::WAVES, COLS> ob;
-  oa.init(a, m0, wave, lane);
-  ob.init(b, n0, wave, lane);
+  OpA oa;
+  OpB ob;
+  oa.init(a, m0, slab0, wave, lane);
+  ob.init(b, n0, slab0, wave, lane);
 #pragma unroll
   for (int i = 0; i < T::FM; ++i)
 #pragma unroll
     for (int j = 0; j < T::FN; ++j) acc[i][j] = 0.f;
-  const auto issue = [&](int t) {
-    char* const st = smem + (t % T::STAGES) * T::STAGE;
-    oa.load(st, wave);
-    ob.load(st + T::A_BYTES, wave);
+  const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
+  const auto issue = [&](int stage) {
+    oa.load(lds + stage * T::STAGE, wave);
+    ob.load(lds + stage * T::STAGE + T::A_BYTES, wave);
   };
+  half8 fa[2][2][T::FM], fb[2][2][T::FN];  // [set][plane]
+  // LDS addresses of this lane's parts, for the lower and the upper two slabs
+  // (an instruction's own offset reaches 64 KiB).  Opaque to the compiler,
+  // which would keep an address register for every read otherwise.
+  uint32_t pa[2][1], pb[2][COLS ? 2 : 1];
 #pragma unroll
-  for (int t = 0; t < T::STAGES - 1; ++t)
-    if (t < nk) issue(t);
-  for (int t = 0; t < nk; ++t) {
-    // Slab t has landed for every wave, and every wave has left slab t - 1,
-    // whose stage takes slab t + STAGES - 1.
-    if (t + T::STAGES - 2 < nk)
-      wait_loads<(T::STAGES - 2) * (T::LA + T::LB)>();
-    else
-      wait_loads<0>();
-    __syncthreads();
-    if (t + T::STAGES - 1 < nk) issue(t + T::STAGES - 1);
-    const char* const sa = smem + (t % T::STAGES) * T::STAGE;
-    const char* const sb = sa + T::A_BYTES;
+  for (int half = 0; half < 2; ++half) {
+    pa[half][0] = lds + half * 2 * T::STAGE + OpA::lane_offset(wm, lane, 0);
+    asm volatile("" : "+v"(pa[half][0]));
 #pragma unroll
-    for (int s = 0; s < kBK / 16; ++s) {
-      half8 fa[2][T::FM], fb[2][T::FN];
+    for (int h = 0; h < (COLS ? 2 : 1); ++h) {
+      pb[half][h] = lds + half * 2 * T::STAGE + T::A_BYTES + OpB::lane_offset(wn, lane, h);
+      asm volatile("" : "+v"(pb[half][h]));
+    }
+  }
+  const auto read = [&](int set, int stage) {
+    const int half = stage >> 1, off = (stage & 1) * T::STAGE;
 #pragma unroll
-      for (int j = 0; j < T::FN; ++j)
+    for (int pl = 1; pl >= 0; --pl) {
 #pragma unroll
-        for (int pl = 0; pl < 2; ++pl)
-          fb[pl][j] = Operand<T::BN, T::LB, T::WAVES, COLS>::frag(sb, pl, wn + 32 * j, s, lane);
+      for (int j = 0; j < T::FN; ++j) fb[set][pl][j] = OpB::frag(pb[half], off, pl, j);
+#pragma unroll
+      for (int i = 0; i < T::FM; ++i) fa[set][pl][i] = OpA::frag(pa[half], off, pl, i);
+    }
+  };
+  constexpr int NL = T::LA + T::LB;
+  // One slab, its number's last two bits u, WAIT of this wave's loads left in
+  // flight: then slab t + 1 has landed for every wave, and every wave has long
+  // left slab t - 1, whose stage takes slab t + 3.
+  const auto slab = [&](auto u_, auto wait_, bool more) {
+    constexpr int u = decltype(u_)::value, set = u & 1;
+    wait_loads<decltype(wait_)::value>();
+    barrier();
+    if (more) issue((u + 3) % kStages);
+    read(set ^ 1, (u + 1) % kStages);
+#pragma unroll
+    for (int q = 0; q < 3; ++q)  // lo hi, hi lo, hi hi
 #pragma unroll
       for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-        for (int pl = 0; pl < 2; ++pl)
-          fa[pl][i] = Operand<T::BM, T::LA, T::WAVES, false>::frag(sa, pl, wm + 32 * i, s, lane);
-#pragma unroll
-      for (int i = 0; i < T::FM; ++i) {
-#pragma unroll
         for (int j = 0; j < T::FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[1][j], fa[0][i], acc[i][j], 0, 0, 0);
+          acc[i][j] = ROW_LANES
+                          ? __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][q == 1][i], fb[set][q == 0][j], acc[i][j], 0, 0, 0)
+                          : __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[set][q == 0][j], fa[set][q == 1][i], acc[i][j], 0, 0, 0);
+    // The next slab's reads go out among the first products.
+    constexpr int READS = 2 * T::FM + 2 * T::FN * (COLS ? 2 : 1), PRODUCTS = 3 * T::FM * T::FN;
 #pragma unroll
-        for (int j = 0; j < T::FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[0][j], fa[1][i], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < T::FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[0][j], fa[0][i], acc[i][j], 0, 0, 0);
-      }
+    for (int r = 0; r < (READS < PRODUCTS ? READS : PRODUCTS); ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, READS < PRODUCTS ? 1 : (READS + PRODUCTS - 1) / PRODUCTS, 0);
     }
+  };
+  using std::integral_constant;
+  using N0 = integral_constant<int, 0>;
+  using N1 = integral_constant<int, NL>;
+  issue(0);
+  issue(1);
+  issue(2);
+  wait_loads<2 * NL>();
+  barrier();
+  read(0, 0);
+  for (int t = kStages; t < nk; t += kStages) {
+    slab(N0{}, N1{}, true);
+    slab(integral_constant<int, 1>{}, N1{}, true);
+    slab(integral_constant<int, 2>{}, N1{}, true);
+    slab(integral_constant<int, 3>{}, N1{}, true);
   }
+  slab(N0{}, N1{}, true);
+  slab(integral_constant<int, 1>{}, N1{}, false);
+  slab(integral_constant<int, 2>{}, N0{}, false);
+  slab(integral_constant<int, 3>{}, N0{}, false);
 }
 
-// Walk of a tile's results: f(m, n, v) with four consecutive columns n.. of row
-// m (tile-relative).
-template <class T, class F>
-__device__ __forceinline__ void for_each4(const f32x16 (&acc)[T::FM][T::FN], F&& f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = wave / T::WN * (T::BM / T::WM), wn = wave % T::WN * (T::BN / T::WN);
-#pragma unroll
-  for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float v[4] = {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        f(wm + 32 * i + (lane & 31), wn + 32 * j + 8 * g + 4 * (lane >> 5), v);
-      }
+// Lanes 4 i .. 4 i + 3 hold four values each, a 4 x 4 block by columns; returns
+// it by rows.
+__device__ __forceinline__ half4 transpose4(half4 v) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  const auto dpp = [](uint32_t x, auto ctrl) {
+    return uint32_t(__builtin_amdgcn_mov_dpp(int(x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  using Near = std::integral_constant<int, 0xB1>;  // lane ^ 1
+  using Far = std::integral_constant<int, 0x4E>;   // lane ^ 2
+  const uint32_t sel = threadIdx.x & 1 ? 0x03020706u : 0x05040100u;
+  const uint32_t a = __builtin_amdgcn_perm(dpp(w[0], Near{}), w[0], sel);
+  const uint32_t b = __builtin_amdgcn_perm(dpp(w[1], Near{}), w[1], sel);
+  const bool upper = threadIdx.x & 2;
+  const uint32_t got = dpp(upper ? a : b, Far{});
+  return __builtin_bit_cast(half4, upper ? u32x2{got, b} : u32x2{a, got});
 }
 
 // Element (row, col .. col + 3) of a plane, col % 4 == 0.
