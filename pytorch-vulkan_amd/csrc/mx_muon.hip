@@ -2,8 +2,14 @@
 // shape side by side, and the optimizer step around them (FP32).
 //
 //   X = U / max(|U|_F, eps), U turned so that its shorter side is the rows
-//   steps times:  G = X X^T,  P = a I + b G + c G^2,  X = P X
+//   steps times:  G = X X^T,  P = b G + c G^2,  X = a X + P X
 //   out = X, or  param = param (1 - lr wd) - lr r X
+//
+// a X is added to the finished product, once: as a I in P it would be in the
+// sum from the first slab on, and every later rounding would be one of a X,
+// while P X is small in the first iterations, whose errors the later ones
+// multiply (4096 x 4096 against float64: 4.6e-6 so, 2.6e-6 added).  The last
+// iteration, which nothing follows, has it in P and so reads X only once.
 //
 // The iterates are this file's own, so they are kept as two fp16 pieces
 // (mx_pieces.hpp) from the first read of U to the last product, whose stores
@@ -173,7 +179,8 @@ struct StepArgs {
   int whole, parts;
   float* sums;
   float alpha;            // product of pieces -> stored value
-  float diag, lin, unit;  // kPoly: a, b and 1 / G's scale, times the stored scale
+  float diag, lin, unit;  // kPoly: a (the last iteration's) and b times the stored scale, 1 / G's scale
+  float keep;             // kNext: a times the stored scale over X's
   const float* lift;      // X's pieces hold X / lift[matrix]
   // kLast
   Table tab;
@@ -247,13 +254,14 @@ __device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, in
     const float alpha = KIND == kGram ? p.alpha * p.lift[b] * p.lift[b] : p.alpha;
     const Planes po{p.out + b * 2 * p.out_plane, p.out_plane, p.out_rows};
     const int r = m + (lane & 31), c0 = n + 4 * (lane >> 5);
-    half4 gh[4], gl[4];
-    if constexpr (KIND == kPoly) {
-      const _Float16* const g = p.a + b * 2 * p.a_plane;
+    half4 wh[4], wl[4];  // G's or X's pieces here
+    if constexpr (KIND != kGram) {
+      const int64_t plane = KIND == kPoly ? p.a_plane : p.b_plane;
+      const _Float16* const was = (KIND == kPoly ? p.a : p.b) + b * 2 * plane;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        gh[q] = *reinterpret_cast<const half4*>(g + elem(po, r, c0 + 8 * q));
-        gl[q] = *reinterpret_cast<const half4*>(g + p.a_plane + elem(po, r, c0 + 8 * q));
+        wh[q] = *reinterpret_cast<const half4*>(was + elem(po, r, c0 + 8 * q));
+        wl[q] = *reinterpret_cast<const half4*>(was + plane + elem(po, r, c0 + 8 * q));
       }
     }
 #pragma unroll
@@ -265,7 +273,8 @@ __device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, in
       for (int e = 0; e < 4; ++e) {
         o[e] = alpha * v[4 * q + e];
         if constexpr (KIND == kPoly)
-          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(gh[q][e]) + float(gl[q][e])) * p.unit) + o[e];
+          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(wh[q][e]) + float(wl[q][e])) * p.unit) + o[e];
+        if constexpr (KIND == kNext) o[e] += p.keep * (float(wh[q][e]) + float(wl[q][e]));
       }
       half4 hi, lo;
       split4(o, hi, lo);
@@ -390,13 +399,16 @@ int launch_kind(int kind, const StepArgs& p, int tiles, hipStream_t s) {
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // A CU's time per slab with n workgroups of a tile on it, and how many it
-// holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.
+// holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.  Over
+// 25 sets from one 64 x 100 to 16 x 1024^2 and 4096^2, all nine pairs of tiles
+// with and without parts timed: the choice takes 0.8% more than the best on
+// average, 11% at most.
 struct TileCost {
   int tile, per_cu;
   double fixed, each;
   double slab(double n) const { return fixed + each * n; }
 };
-constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.20, 0.21}, {256, 1, 0.0, 1.15}};
+constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.05, 0.285}, {256, 1, 0.0, 1.15}};
 
 // How a product's tiles are dealt: whole rounds of the chip, then what is left
 // over in parts along K where a join (a launch and a pass over the sums) costs
@@ -412,19 +424,17 @@ Deal deal(const TileCost& c, int64_t tiles, int64_t nk, int64_t cu) {
   d.time += double(full * nk) * c.slab(c.per_cu);
   if (!rest) return d;
   const double plain = double(nk) * c.slab(double((rest + cu - 1) / cu));
-  const int64_t parts = std::min<int64_t>({slots / rest, nk / 8, 16});
-  if (parts >= 2) {
+  double least = plain;
+  for (int64_t parts = 2; parts <= 16 && parts * rest <= slots && parts * 8 <= nk; ++parts) {
     const double share = double((nk / 4 + parts - 1) / parts * 4);
-    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 5.0 +
-                         double(rest * parts) * c.tile * c.tile * 8.0 / 3e6;
-    if (split < plain) {
-      d.whole = full * slots;
-      d.parts = int(parts);
-      d.time += split;
-      return d;
-    }
+    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 4.0 +
+                         double(rest * parts) * c.tile * c.tile * 8.0 / 6e6;
+    if (split >= least) continue;
+    least = split;
+    d.whole = full * slots;
+    d.parts = int(parts);
   }
-  d.time += plain;
+  d.time += least;
   return d;
 }
 
@@ -660,7 +670,8 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
     p.out = poly;
     p.nk = g.sp / kBK;
     p.alpha = float(ns.c) * (c.p / c.g / c.g);
-    p.diag = float(ns.a) * c.p;
+    const bool last = i + 1 == ns.steps;
+    p.diag = last ? float(ns.a) * c.p : 0.f;
     p.lin = float(ns.b) * c.p;
     p.unit = 1.f / c.g;
     MX_TRY(run(kPoly, plan.poly, plan.sym));
@@ -668,7 +679,7 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
     p.b = x;
     p.b_plane = p.out_plane = g.x_plane();
     p.out = x2;
-    const bool last = i + 1 == ns.steps;
+    p.keep = last ? 0.f : float(ns.a) * (sc[size_t(i) + 1].x / c.x);
     p.alpha = (last ? 1.f : sc[size_t(i) + 1].x) / c.p / c.x;
     MX_TRY(run(!last ? kNext : g.turned ? kLast : kLastRows, plan.update, plan.next));
     std::swap(x, x2);

@@ -59,6 +59,7 @@ struct Tile {
   static constexpr int A_BYTES = 2 * BM * kBK * 2, B_BYTES = 2 * BN * kBK * 2, STAGE = A_BYTES + B_BYTES;
   static constexpr int SMEM = kStages * STAGE;
   static constexpr int LA = A_BYTES / 1024 / WAVES, LB = B_BYTES / 1024 / WAVES;  // wave-wide loads of a slab
+  static constexpr bool DUAL = FM * FN <= 4;  // hi lo and lo hi in accumulators of their own
   static_assert(LA * WAVES * 1024 == A_BYTES && LB * WAVES * 1024 == B_BYTES, "whole loads");
 };
 
@@ -186,6 +187,7 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
   for (int i = 0; i < T::FM; ++i)
 #pragma unroll
     for (int j = 0; j < T::FN; ++j) acc[i][j] = 0.f;
+  f32x16 low[T::DUAL ? T::FM : 1][T::DUAL ? T::FN : 1] = {};
   const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem));
   const auto issue = [&](int stage) {
     oa.load(lds + stage * T::STAGE, wave);
@@ -231,10 +233,11 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
 #pragma unroll
       for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-        for (int j = 0; j < T::FN; ++j)
-          acc[i][j] = ROW_LANES
-                          ? __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][q == 1][i], fb[set][q == 0][j], acc[i][j], 0, 0, 0)
-                          : __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[set][q == 0][j], fa[set][q == 1][i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < T::FN; ++j) {
+          f32x16& c = T::DUAL && q < 2 ? low[T::DUAL ? i : 0][T::DUAL ? j : 0] : acc[i][j];
+          c = ROW_LANES ? __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][q == 1][i], fb[set][q == 0][j], c, 0, 0, 0)
+                        : __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[set][q == 0][j], fa[set][q == 1][i], c, 0, 0, 0);
+        }
     // The next slab's reads go out among the first products.
     constexpr int READS = 2 * T::FM + 2 * T::FN * (COLS ? 2 : 1), PRODUCTS = 3 * T::FM * T::FN;
 #pragma unroll
@@ -262,6 +265,12 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
   slab(integral_constant<int, 1>{}, N1{}, false);
   slab(integral_constant<int, 2>{}, N0{}, false);
   slab(integral_constant<int, 3>{}, N0{}, false);
+  if constexpr (T::DUAL) {
+#pragma unroll
+    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < T::FN; ++j) acc[i][j] += low[i][j];
+  }
 }
 
 // Lanes 4 i .. 4 i + 3 hold four values each, a 4 x 4 block by columns; returns
