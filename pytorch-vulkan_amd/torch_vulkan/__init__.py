@@ -287,4 +287,4 @@ def Event(enable_timing: bool = False, blocking: bool = False, interprocess: boo
 
 torch._register_device_module("vulkan", sys.modules[__name__])
 
-from . import optim  # noqa: E402,F401
+from . import nn, optim  # noqa: E402,F401

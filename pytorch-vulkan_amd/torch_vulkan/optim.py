@@ -1,6 +1,10 @@
-"""Opt-in fused AdamW for ``"vulkan"`` parameters.
+"""Opt-in fused AdamW and Muon for ``"vulkan"`` parameters.
 
-Interface of the reference's ``torch_vulkan.optim.AdamW``
+``Muon`` keeps the constructor keywords and the state key (``momentum_buffer``)
+of ``torch.optim.Muon``; every parameter group is one call of
+``torch.ops.torch_vulkan.muon_step_``, in FP32 throughout.
+
+AdamW: interface of the reference's ``torch_vulkan.optim.AdamW``
 (torch_vulkan/optim.py:13-75 there): the constructor keywords ``lr``,
 ``betas``, ``eps``, ``weight_decay``, ``batched`` and ``amsgrad``, and per
 parameter the state keys of ``torch.optim.AdamW`` (``step``, ``exp_avg``,
@@ -152,4 +156,52 @@ class AdamW(torch.optim.Optimizer):
             beta1, beta2 = group["betas"]
             hyper = (group["lr"], beta1, beta2, group["eps"], group["weight_decay"])
             batch.launch(hyper, group.get("batched", True))
+        return loss
+
+
+class Muon(torch.optim.Optimizer):
+    """Orthogonalised momentum for matrices (two-dimensional FP32 parameters):
+    matrices of one shape go through the Newton-Schulz products together."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None):
+        problems = [name for name, ok in (("lr", lr >= 0), ("weight_decay", weight_decay >= 0),
+                                          ("momentum", 0 <= momentum <= 1), ("eps", eps > 0), ("ns_steps", ns_steps >= 0),
+                                          ("ns_coefficients", len(ns_coefficients) == 3),
+                                          ("adjust_lr_fn", adjust_lr_fn in (None, "original", "match_rms_adamw"))) if not ok]
+        if problems:
+            raise ValueError(f"Muon: out-of-range hyperparameter(s) {', '.join(problems)}")
+        super().__init__(params, {"lr": lr, "weight_decay": weight_decay, "momentum": momentum, "nesterov": nesterov,
+                                  "ns_coefficients": tuple(ns_coefficients), "eps": eps, "ns_steps": ns_steps,
+                                  "adjust_lr_fn": adjust_lr_fn})
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError(f"Muon: only matrices are supported, got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params, grads, buffers = [], [], []
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("torch_vulkan Muon: sparse gradients are not supported")
+                if p.device.type != "vulkan":
+                    raise RuntimeError(f"torch_vulkan Muon: parameter on {p.device}, expected a vulkan tensor")
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p.grad, memory_format=torch.contiguous_format)
+                params.append(p)
+                grads.append(p.grad)
+                buffers.append(state["momentum_buffer"])
+            if params:
+                _backend_ops().muon_step_(params, grads, buffers, group["lr"], group["weight_decay"], group["momentum"],
+                                          group["nesterov"], list(group["ns_coefficients"]), group["ns_steps"],
+                                          group["eps"], group["adjust_lr_fn"] or "original")
         return loss
