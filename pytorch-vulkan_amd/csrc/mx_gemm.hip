@@ -46,11 +46,13 @@ struct GemmArgs {
   int act;
   const float* residual;
   float* z;
+  const int* only_if;  // null, or a word that is zero where there is nothing to do
 };
 
 template <class C, Mode MA, Mode MB, bool EPI>
 MX_TILE_KERNEL(C) void gemm_kernel(GemmArgs p) {
   __shared__ __attribute__((aligned(16))) float smem[C::SMEM_FLOATS];
+  if (p.only_if && *p.only_if == 0) return;
   int tm, tn;
   tile_coords(xcd_remap(blockIdx.x, p.tiles_m * p.tiles_n), p.tiles_m, p.tiles_n, tm, tn);
   const int row0 = tm * C::BM, col0 = tn * C::BN;
@@ -488,7 +490,7 @@ int64_t partial_bytes(const GemmArgs& p) { return p.splits > 1 ? int64_t(p.split
 }  // namespace
 
 int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const float* bias, float* c, int64_t partials,
-                hipStream_t s, const GemmEpilogue* epi, void* given) {
+                hipStream_t s, const GemmEpilogue* epi, void* given, const int* only_if) {
   GemmPlan g;
   MX_TRY(plan_gemm(d, a, b, bias, c, std::min(partials, kMaxSplitBytes), &g));
   if (g.empty) return MX_OK;
@@ -496,6 +498,7 @@ int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const flo
   MX_REQUIRE(c, MX_ERR_INVALID, "mx_gemm_f32: null output");
   MX_REQUIRE(d->bias_kind == MX_BIAS_NONE || bias, MX_ERR_INVALID, "mx_gemm_f32: null bias");
   GemmArgs& p = g.p;
+  p.only_if = only_if;
   if (epi) {
     p.act = epi->act;
     p.residual = epi->residual;
@@ -525,6 +528,7 @@ int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const flo
       p.act = was.act;
       p.residual = was.residual;
       p.z = was.z;
+      p.only_if = only_if;
     }
   }
   if (epi) {

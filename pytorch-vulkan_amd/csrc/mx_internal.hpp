@@ -88,9 +88,11 @@ struct GemmEpilogue {
 
 // mx_gemm_f32 with at most `partials` bytes of scratch for a K split (the
 // caller's where `given` is not null), and the kernels and scratch of such a
-// call (mx_gemm.hip).
+// call (mx_gemm.hip).  only_if: a device word; the launches do nothing where it
+// is zero.
 int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const float* bias, float* c, int64_t partials,
-                hipStream_t s, const GemmEpilogue* epi = nullptr, void* given = nullptr);
+                hipStream_t s, const GemmEpilogue* epi = nullptr, void* given = nullptr,
+                const int* only_if = nullptr);
 int gemm_describe(const mx_gemm_desc* d, const float* a, const float* b, int64_t partials, std::string* name,
                   int64_t* bytes);
 

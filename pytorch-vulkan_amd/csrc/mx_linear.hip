@@ -4,16 +4,33 @@
 //   z = x w^T + bias,  y = act(z) + residual
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_m dz
 //
-// The forward is one product (mx_gemm.hip) whose stores apply the rest.  The
-// backward makes dz in one pass that sums its columns on the way (the products
-// would otherwise evaluate the slope once for every tile that reads the
-// element), then takes the two products of it.
+// The forward is one product whose stores apply the rest.  The backward makes
+// dz in one pass that sums its columns on the way (the products would otherwise
+// evaluate the slope once for every tile that reads the element), then takes the
+// two products of it.
+//
+// Two forms of the products.  Large ones run on operands packed as two fp16
+// pieces (mx_pieces.hpp): a pass over each operand finds its largest element,
+// rows and columns on the way, a second one writes the pieces, scaled by a power
+// of two for the whole operand, and the products take half the matrix
+// instructions of three bf16 pieces.  Small ones, for which the two passes cost
+// more than they save, take mx_gemm.hip's products as they are.
+//
+// What one scale holds: an element is off by at most 2^-23 of itself or 2^-39 of
+// the operand's largest.  Rows and columns all within 2^8 of that keep FP32's
+// accuracy, each by itself and also where sizes of rows and columns multiply (an
+// element small for both is 2^-16 of the largest); zero ones count for nothing.
+// The second pass notes an operand with others, or one that is not finite or
+// whose largest is below 2^-100, and its products are then taken by
+// mx_gemm.hip's kernels, which follow on the stream and end at once where
+// nothing was noted.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "mx_activation.hpp"
 #include "mx_internal.hpp"
+#include "mx_pieces.hpp"
 
 namespace mx {
 namespace {
@@ -21,46 +38,272 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// dz = dy * act'(z) (not written where dz is null; z null: the slope is 1), and
-// the column sums of dz over the workgroup's rows to part[blockIdx.y][n] where
-// part is not null.  A thread holds W columns; 64 threads lie along a row and
-// the workgroup's four waves take a row each.  W == 4 for n >= 4: the last
-// thread of a row takes its last four elements (it and its neighbour write the
-// same values).
-template <int W>
-__global__ __launch_bounds__(256) void slope_kernel(const float* dy, const float* z, int act, int64_t m, int n,
-                                                    int64_t rows_per, float* dz, float* part) {
+// One operand's first pass: where `z` is not null src is dy and the values are
+// dz = dy act'(z), written to dz.  Column sums to sums[part][n] where that is
+// not null; with TOPS, largest magnitudes (as bits: NaN counts above infinity) of
+// rows to row_top[column block][m], of columns to col_top[part][n] and of the
+// workgroup's block to top[workgroup].
+struct ScanOp {
+  const float* src;
+  const float* z;
+  float* dz;
+  float* sums;
+  uint32_t *row_top, *col_top, *top;
+  int64_t m;
+  int n;
+  int64_t rows_per;
+  int col_blocks, parts;
+  int first;  // first workgroup
+};
+struct ScanArgs {
+  ScanOp op[3];
+  int count, act;
+  int* bad;  // cleared
+};
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// A thread holds W columns; 64 threads lie along a row and the workgroup's four
+// waves take a row each.  W == 4 for n >= 4: the last thread of a row takes its
+// last four elements (it and its neighbour write the same values).  TOPS: the
+// largest magnitudes are wanted.
+template <int W, bool TOPS>
+__global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
   typedef float vec __attribute__((ext_vector_type(W)));
   typedef float vecu __attribute__((ext_vector_type(W), aligned(4)));
+  typedef uint32_t uvec __attribute__((ext_vector_type(W)));
+  typedef uint32_t uvecu __attribute__((ext_vector_type(W), aligned(4)));
   __shared__ vec sums[256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t col = (int64_t(blockIdx.x) * 64 + lane) * W;
+  __shared__ uvec tops[TOPS ? 256 : 1];
+  if (p.bad && blockIdx.x == 0 && threadIdx.x < 2) p.bad[threadIdx.x] = 0;
+  int k = 0;
+  while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
+  const ScanOp& o = p.op[k];
+  const int id = blockIdx.x - o.first, bx = id % o.col_blocks, by = id / o.col_blocks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = o.n;
+  const int64_t col = (int64_t(bx) * 64 + lane) * W;
   const bool in = col < n;
   const int64_t at = min(col, int64_t(n - W));
-  const int64_t r0 = blockIdx.y * rows_per, r1 = min(m, r0 + rows_per);
+  const int64_t r0 = by * o.rows_per, r1 = min(o.m, r0 + o.rows_per);
+  const float* const src = o.src;
+  const float* const z = o.z;
   vec s = 0.f;
-  if (in) {
-#pragma unroll 4
-    for (int64_t r = r0 + wave; r < r1; r += 4) {
-      vec d = *reinterpret_cast<const vecu*>(dy + r * n + at);
-      if (z) {
-        const vec t = *reinterpret_cast<const vecu*>(z + r * n + at);
+  uvec top = 0u;
+  constexpr int ROWS = 4;  // of a wave, on their way together
+  for (int64_t r = r0 + wave; r < r1; r += 4 * ROWS) {
+    vec d[ROWS], t[ROWS];
 #pragma unroll
-        for (int e = 0; e < W; ++e) d[e] *= activate_slope(act, t[e]);
-        if (dz) *reinterpret_cast<vecu*>(dz + r * n + at) = d;
+    for (int u = 0; u < ROWS; ++u) {
+      const bool ok = in && r + 4 * u < r1;
+      d[u] = t[u] = 0.f;
+      if (ok) d[u] = *reinterpret_cast<const vecu*>(src + (r + 4 * u) * n + at);
+      if (ok && z) t[u] = *reinterpret_cast<const vecu*>(z + (r + 4 * u) * n + at);
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      if (z) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) d[u][e] *= activate_slope(p.act, t[u][e]);
+        if (o.dz && in && r + 4 * u < r1) *reinterpret_cast<vecu*>(o.dz + (r + 4 * u) * n + at) = d[u];
       }
-      s += d;
+      s += d[u];
+      if constexpr (TOPS) {
+        uint32_t row = 0;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const uint32_t v = magnitude(d[u][e]);
+          top[e] = max(top[e], v);
+          row = max(row, v);
+        }
+#pragma unroll
+        for (int q = 1; q < 64; q <<= 1) row = max(row, uint32_t(__shfl_xor(int(row), q, 64)));
+        if (lane == 0 && r + 4 * u < r1) o.row_top[int64_t(bx) * o.m + r + 4 * u] = row;
+      }
     }
   }
-  if (!part) return;
+  if (!o.sums && !TOPS) return;
   sums[threadIdx.x] = s;
+  if constexpr (TOPS) tops[threadIdx.x] = top;
   __syncthreads();
-  if (wave == 0 && in) {
+  if (wave != 0) return;
+  if (o.sums && in) {
     s += sums[64 + lane];
     s += sums[128 + lane];
     s += sums[192 + lane];
-    *reinterpret_cast<vecu*>(part + int64_t(blockIdx.y) * n + at) = s;
+    *reinterpret_cast<vecu*>(o.sums + int64_t(by) * n + at) = s;
   }
+  if constexpr (TOPS) {
+    uint32_t all = 0;
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      top[e] = max(max(top[e], tops[64 + lane][e]), max(tops[128 + lane][e], tops[192 + lane][e]));
+      all = max(all, top[e]);
+    }
+    if (in) *reinterpret_cast<uvecu*>(o.col_top + int64_t(by) * n + at) = top;
+#pragma unroll
+    for (int q = 1; q < 64; q <<= 1) all = max(all, uint32_t(__shfl_xor(int(all), q, 64)));
+    if (lane == 0) o.top[id] = all;
+  }
+}
+
+// Second pass: the pieces of an operand [m][n], padded with zeros to
+// [planes.rows] x 64 columns_of_64, times 2^(14 - e) where 2^e is its largest
+// element's power, e to *exponent.  The words of `bad` whose bits `flags` has are
+// set where some row or column is too far below that, or nothing can be scaled.
+struct PackOp {
+  const float* src;
+  int m, n;
+  pieces::Planes to;
+  const uint32_t *row_top, *col_top, *top;
+  int col_blocks, parts, tops;
+  int flags;
+  int* exponent;
+  int wide;   // workgroups along a row
+  int first;  // first workgroup
+};
+struct PackArgs {
+  PackOp op[3];
+  int count;
+  int* bad;
+};
+
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
+  __shared__ uint32_t tops[4];
+  int k = 0;
+  while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
+  const PackOp& o = p.op[k];
+  const int id = blockIdx.x - o.first, bx = id % o.wide, by = id / o.wide, tid = threadIdx.x;
+  const int row = by * 32 + (tid & 31), col = bx * 64 + (tid >> 5) * 8;
+  // This thread's eight columns of a row, on their way while the largest is found.
+  float v[8] = {};
+  if (row < o.m && col < o.n) {
+    const float* const from = o.src + int64_t(row) * o.n + col;
+    if (col + 8 <= o.n) {
+      const f32x4 a = *reinterpret_cast<const f32x4u*>(from), b = *reinterpret_cast<const f32x4u*>(from + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = col + e < o.n ? from[e] : 0.f;
+    }
+  }
+  uint32_t top = 0;
+  for (int i = tid; i < o.tops; i += 256) top = max(top, o.top[i]);
+#pragma unroll
+  for (int q = 1; q < 64; q <<= 1) top = max(top, uint32_t(__shfl_xor(int(top), q, 64)));
+  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  const float largest = __uint_as_float(top);
+  const bool fits = top == 0 || (top < 0x7F800000u && largest >= 0x1p-100f);
+  const int e = top == 0 || !fits ? 0 : int(top >> 23) - 127;
+  if (id == 0 && tid == 0) {
+    *o.exponent = e;
+  }
+  bool bad = !fits;
+  const auto low = [&](uint32_t t) { return t != 0 && __uint_as_float(t) < largest * 0x1p-8f; };
+  if (bx == 0 && tid < 32 && row < o.m) {
+    uint32_t t = 0;
+    for (int i = 0; i < o.col_blocks; ++i) t = max(t, o.row_top[int64_t(i) * o.m + row]);
+    bad = bad || low(t);
+  }
+  if (by == 0 && tid < 64 && bx * 64 + tid < o.n) {
+    uint32_t t = 0;
+#pragma unroll 8
+    for (int i = 0; i < o.parts; ++i) t = max(t, o.col_top[int64_t(i) * o.n + bx * 64 + tid]);
+    bad = bad || low(t);
+  }
+  if (bad) {
+    if (o.flags & 1) p.bad[0] = 1;
+    if (o.flags & 2) p.bad[1] = 1;
+  }
+  pieces::half8 hi, lo;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float f = ldexpf(v[q], 14 - e);
+    hi[q] = _Float16(f);
+    lo[q] = _Float16(f - float(hi[q]));
+  }
+  _Float16* const to = o.to.at + (int64_t(col >> 3) * o.to.rows + row) * 8;
+  *reinterpret_cast<pieces::half8*>(to) = hi;
+  *reinterpret_cast<pieces::half8*>(to + o.to.plane) = lo;
+}
+
+// A product of packed operands: out[m][n], whole 128-byte lines of a row to a
+// half wave.  EPI: bias, activation and residual, z where it is not null.
+struct PieceArgs {
+  pieces::Planes a, b;
+  int nk, tiles_m, tiles_n;
+  pieces::Shares share;
+  const int *bad, *ea, *eb;
+  int m, n;
+  float* out;
+  const float *bias, *residual;
+  float* z;
+  int act;
+};
+
+template <bool EPI>
+__device__ __forceinline__ void finish_piece(const PieceArgs& p, int m, int n, const pieces::f32x16& acc) {
+  const int lane = threadIdx.x & 63, col = n + (lane & 31), row0 = m + 4 * (lane >> 5), up = *p.ea + *p.eb - 28;
+  const bool in = col < p.n;
+  const int64_t at = int64_t(row0) * p.n + col;
+  float bias = 0.f, res[16];
+  if constexpr (EPI) {
+    if (p.bias && in) bias = p.bias[col];
+    if (p.residual) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i >> 2) + (i & 3);
+        res[i] = in && row0 + r < p.m ? p.residual[at + int64_t(r) * p.n] : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 8 * (i >> 2) + (i & 3);
+    if (!in || row0 + r >= p.m) continue;
+    float v = ldexpf(acc[i], up);
+    if constexpr (EPI) {
+      v += bias;
+      if (p.z) p.z[at + int64_t(r) * p.n] = v;
+      v = activate(p.act, v) + (p.residual ? res[i] : 0.f);
+    }
+    p.out[at + int64_t(r) * p.n] = v;
+  }
+}
+
+template <class T, bool A_COLS, bool B_COLS, bool EPI>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void piece_kernel(PieceArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
+  if (*p.bad) return;
+  const pieces::Unit unit = pieces::unit_of(p.share, blockIdx.x, p.nk);
+  int tm, tn;
+  mfma::tile_coords(unit.tile, p.tiles_m, p.tiles_n, tm, tn);
+  pieces::f32x16 acc[T::FM][T::FN];
+  pieces::product<T, A_COLS, B_COLS, true>(acc, p.a, p.b, tm * T::BM, tn * T::BN, unit.k0, unit.k1 - unit.k0, smem);
+  if (unit.tile >= p.share.whole) {
+    pieces::store_sums<T>(acc, p.share, unit);
+    return;
+  }
+  const int wave = threadIdx.x >> 6;
+  const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
+#pragma unroll
+  for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::FN; ++j) finish_piece<EPI>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+}
+
+template <class T, bool EPI>
+__global__ __launch_bounds__(64) void piece_join_kernel(PieceArgs p) {
+  if (*p.bad) return;
+  int tile, m, n, tm, tn;
+  const pieces::f32x16 v = pieces::join_sums<T>(p.share, tile, m, n);
+  mfma::tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn);
+  finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v);
 }
 
 // out[c] = sum of part[p][c] in the order of p: 32 columns and 32 groups of
@@ -89,14 +332,15 @@ __global__ void zero_kernel(float* out, int64_t n) {
 
 int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
 
-// Row ranges of the elementwise pass: enough workgroups to fill the chip
-// without splitting a range below 16 rows.
-struct SlopePlan {
+// Row ranges of the first pass: enough workgroups to fill the chip without
+// splitting a range below 16 rows.
+struct ScanPlan {
   int64_t rows_per;
   int parts, col_blocks;
+  int blocks() const { return parts * col_blocks; }
 };
-SlopePlan plan_slope(int64_t m, int64_t n) {
-  SlopePlan p{};
+ScanPlan plan_scan(int64_t m, int64_t n) {
+  ScanPlan p{};
   const int w = n >= 4 ? 4 : 1;
   p.col_blocks = int((n + 64 * w - 1) / (64 * w));
   const int64_t want = std::max<int64_t>(1, int64_t(cu_count()) * 8 / p.col_blocks);
@@ -150,22 +394,220 @@ int check(const char* who, int64_t m, int64_t k, int64_t n, int act) {
   return MX_OK;
 }
 
-struct BackwardPlan {
-  int64_t dz, sums, gemm;  // bytes
+// Carves a workspace (or, with a null base, adds up what it takes).
+struct Carve {
+  char* base;
+  int64_t used = 0;
+  explicit Carve(void* p) : base(static_cast<char*>(p)) {}
+  template <class T>
+  T* take(int64_t count) {
+    T* const at = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += up256(count * int64_t(sizeof(T)));
+    return at;
+  }
 };
-int plan_backward(int64_t m, int64_t k, int64_t n, int act, BackwardPlan* p) {
-  *p = BackwardPlan{};
-  if (m == 0 || n == 0) return MX_OK;
-  if (act != MX_ACT_NONE) p->dz = up256(m * n * 4);
-  const SlopePlan sp = plan_slope(m, n);
-  if (sp.parts > 1) p->sums = up256(int64_t(sp.parts) * n * 4);
-  if (k == 0) return MX_OK;
-  int64_t a = 0, b = 0;
-  MX_TRY(partials(dx_desc(m, k, n), &a));
-  MX_TRY(partials(dw_desc(m, k, n), &b));
-  p->gemm = std::max(a, b);
+
+// ------------------------------------------------------------ packed products
+// An operand [m][n] of packed products: what its passes write.
+struct Packed {
+  int64_t m, n;
+  ScanPlan scan;
+  ScanOp first;
+  PackOp second;
+};
+
+Packed packed(int64_t m, int64_t n, int pad, int flags, Carve* c) {
+  Packed o{};
+  o.m = m;
+  o.n = n;
+  o.scan = plan_scan(m, n);
+  const int64_t mp = (m + pad - 1) / pad * pad, np = (n + pad - 1) / pad * pad;
+  o.first.m = m;
+  o.first.n = int(n);
+  o.first.rows_per = o.scan.rows_per;
+  o.first.col_blocks = o.scan.col_blocks;
+  o.first.parts = o.scan.parts;
+  o.first.row_top = c->take<uint32_t>(m * o.scan.col_blocks);
+  o.first.col_top = c->take<uint32_t>(n * o.scan.parts);
+  o.first.top = c->take<uint32_t>(o.scan.blocks());
+  o.second.m = int(m);
+  o.second.n = int(n);
+  o.second.to = {c->take<_Float16>(2 * mp * np), mp * np, int(mp)};
+  o.second.row_top = o.first.row_top;
+  o.second.col_top = o.first.col_top;
+  o.second.top = o.first.top;
+  o.second.col_blocks = o.scan.col_blocks;
+  o.second.parts = o.scan.parts;
+  o.second.tops = o.scan.blocks();
+  o.second.flags = flags;
+  o.second.wide = int(np / 64);
+  return o;
+}
+
+// One product's tile and how its tiles are dealt; sides padded to `pad`.
+struct PieceDeal {
+  int tile;  // index into pieces::kTiles
+  pieces::Deal deal;
+};
+PieceDeal plan_piece(int64_t m, int64_t n, int64_t k, int pad) {
+  PieceDeal best{};
+  const auto pd = [&](int64_t v) { return (v + pad - 1) / pad * pad; };
+  for (int i = 1; i < 3; ++i) {
+    const pieces::TileCost& c = pieces::kTiles[i];
+    if (pad % c.tile) continue;
+    const pieces::Deal d = pieces::deal(c, pd(m) / c.tile * (pd(n) / c.tile), pd(k) / pieces::kBK, cu_count());
+    if (!best.tile || d.time < best.deal.time) best = {i, d};
+  }
+  return best;
+}
+
+// What padding a call's products want: 128 or 256.
+int pick_pad(int64_t m, int64_t k, int64_t n, bool backward) {
+  double time[2];
+  for (int i = 0; i < 2; ++i) {
+    const int pad = 128 << i;
+    time[i] = backward ? plan_piece(m, k, n, pad).deal.time + plan_piece(n, k, m, pad).deal.time
+                       : plan_piece(m, n, k, pad).deal.time;
+  }
+  return time[1] < time[0] ? 256 : 128;
+}
+
+// Largest packed scratch of a call.
+constexpr int64_t kMostPacked = int64_t(4) << 30;
+
+// Whether a call's products run on packed operands: PACKED_RULE
+bool use_packed(int64_t m, int64_t k, int64_t n, bool backward) {
+  if (m < 4 || k < 4 || n < 4) return false;
+  if ((m * k + k * n + (backward ? m * n : 0)) * 5 > kMostPacked) return false;
+  if (const char* e = std::getenv("MXLP")) return e[0] == '1';
+  return 2.0 * double(m) * double(n) * double(k) >= 4e9;
+}
+
+template <class T, bool A_COLS, bool B_COLS, bool EPI>
+int launch_piece(const PieceArgs& p, int tiles, hipStream_t s) {
+  const int rest = tiles - p.share.whole;
+  hipLaunchKernelGGL((piece_kernel<T, A_COLS, B_COLS, EPI>), dim3(unsigned(p.share.whole + rest * p.share.parts)),
+                     dim3(T::THREADS), 0, s, p);
+  MX_HIP(hipGetLastError());
+  if (rest) {
+    hipLaunchKernelGGL((piece_join_kernel<T, EPI>), dim3(unsigned(rest * T::WAVES * T::FM * T::FN)), dim3(64), 0, s, p);
+    MX_HIP(hipGetLastError());
+  }
   return MX_OK;
 }
+
+// out [m][n] over k: operands a (its rows, or A_COLS columns, are m) and b.
+template <bool A_COLS, bool B_COLS, bool EPI>
+int run_piece(PieceArgs p, const PieceDeal& d, const Packed& a, const Packed& b, const int* bad, float* sums, int pad,
+              hipStream_t s) {
+  const int tile = pieces::kTiles[d.tile].tile;
+  const auto pd = [&](int64_t v) { return int((v + pad - 1) / pad * pad); };
+  p.a = a.second.to;
+  p.b = b.second.to;
+  p.ea = a.second.exponent;
+  p.eb = b.second.exponent;
+  p.bad = bad;
+  p.m = int(A_COLS ? a.n : a.m);
+  p.n = int(B_COLS ? b.n : b.m);
+  p.nk = pd(A_COLS ? a.m : a.n) / pieces::kBK;
+  p.tiles_m = pd(p.m) / tile;
+  p.tiles_n = pd(p.n) / tile;
+  p.share = {int(d.deal.whole), d.deal.parts, sums};
+  if (d.tile == 1) return launch_piece<pieces::Tile128, A_COLS, B_COLS, EPI>(p, int(d.deal.tiles), s);
+  return launch_piece<pieces::Tile256, A_COLS, B_COLS, EPI>(p, int(d.deal.tiles), s);
+}
+
+// First and second pass of a call's operands.
+template <bool TOPS>
+int run_scan(ScanArgs* p, hipStream_t s) {
+  int blocks = 0;
+  for (int i = 0; i < p->count; ++i) {
+    p->op[i].first = blocks;
+    blocks += p->op[i].col_blocks * p->op[i].parts;
+  }
+  if (p->op[0].n >= 4)
+    hipLaunchKernelGGL((scan_kernel<4, TOPS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+  else
+    hipLaunchKernelGGL((scan_kernel<1, TOPS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+  MX_HIP(hipGetLastError());
+  return MX_OK;
+}
+int run_pack(PackArgs* p, hipStream_t s) {
+  int blocks = 0;
+  for (int i = 0; i < p->count; ++i) {
+    p->op[i].first = blocks;
+    blocks += p->op[i].wide * (p->op[i].to.rows / 32);
+  }
+  hipLaunchKernelGGL(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+  MX_HIP(hipGetLastError());
+  return MX_OK;
+}
+
+// ----------------------------------------------------------------- the calls
+// Workspace of a forward: the packed operands, or the product's K split.
+struct Forward {
+  bool packed;
+  int pad = 0;
+  Packed x, w;
+  int* head = nullptr;  // two flags, three exponents
+  PieceDeal deal{};
+  float* sums = nullptr;
+  int64_t partial = 0;
+  Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(use_packed(m, k, n, false)) {
+    if (!packed) return;
+    pad = pick_pad(m, k, n, false);
+    head = c->take<int>(8);
+    x = mx::packed(m, k, pad, 1, c);
+    w = mx::packed(n, k, pad, 1, c);
+    deal = plan_piece(m, n, k, pad);
+    sums = c->take<float>(deal.deal.sum_bytes(pieces::kTiles[deal.tile].tile) / 4);
+  }
+};
+
+int forward_bytes(int64_t m, int64_t k, int64_t n, int64_t* bytes) {
+  *bytes = 0;
+  if (m == 0 || n == 0 || k == 0) return MX_OK;
+  Carve c(nullptr);
+  const Forward f(m, k, n, &c);
+  *bytes = c.used;
+  return f.packed ? MX_OK : partials(forward_desc(m, k, n, true), bytes);
+}
+
+// Workspace of a backward.
+struct Backward {
+  bool packed;
+  int pad = 0;
+  ScanPlan scan;  // of dz
+  float *dz = nullptr, *part = nullptr, *sums = nullptr;
+  int* head = nullptr;
+  Packed g, x, w;
+  PieceDeal to_x{}, to_w{};
+  int64_t gemm = 0;
+  void* split = nullptr;
+  int status = MX_OK;
+  Backward(int64_t m, int64_t k, int64_t n, bool slope, bool want_x, bool want_w, bool want_b, bool split_room, Carve* c)
+      : packed((want_x || want_w) && use_packed(m, k, n, true)), scan(plan_scan(m, n)) {
+    if (slope && (want_x || want_w)) dz = c->take<float>(m * n);
+    if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
+    if (packed) {
+      pad = pick_pad(m, k, n, true);
+      head = c->take<int>(8);
+      g = mx::packed(m, n, pad, (want_x ? 1 : 0) | (want_w ? 2 : 0), c);
+      if (want_w) x = mx::packed(m, k, pad, 2, c);
+      if (want_x) w = mx::packed(n, k, pad, 1, c);
+      to_x = plan_piece(m, k, n, pad);
+      to_w = plan_piece(n, k, m, pad);
+      sums = c->take<float>(std::max(want_x ? to_x.deal.sum_bytes(pieces::kTiles[to_x.tile].tile) : 0,
+                                     want_w ? to_w.deal.sum_bytes(pieces::kTiles[to_w.tile].tile) : 0) / 4);
+    } else if (split_room && k > 0) {
+      int64_t a = 0, b = 0;
+      if (want_x) status = partials(dx_desc(m, k, n), &a);
+      if (want_w && status == MX_OK) status = partials(dw_desc(m, k, n), &b);
+      gemm = std::max(a, b);
+      split = c->take<char>(gemm);
+    }
+  }
+};
 
 }  // namespace
 }  // namespace mx
@@ -178,14 +620,11 @@ extern "C" int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activati
   MX_REQUIRE(bytes, MX_ERR_INVALID, "mx_linear_workspace: null result");
   *bytes = 0;
   if (m == 0 || n == 0) return MX_OK;
-  if (backward) {
-    BackwardPlan p;
-    MX_TRY(plan_backward(m, k, n, activation, &p));
-    *bytes = p.dz + p.sums + p.gemm;
-  } else if (k > 0) {
-    MX_TRY(partials(forward_desc(m, k, n, true), bytes));
-  }
-  return MX_OK;
+  if (!backward) return forward_bytes(m, k, n, bytes);
+  Carve c(nullptr);
+  const Backward b(m, k, n, activation != MX_ACT_NONE, k > 0, k > 0, true, true, &c);
+  *bytes = c.used;
+  return b.status;
   MX_ABI_END
 }
 
@@ -193,18 +632,44 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
                                  int64_t k, int64_t n, int activation, float* y, float* z, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  MX_TRY(check("mx_linear_forward", m, k, n, activation));
+  const char* const who = "mx_linear_forward";
+  MX_TRY(check(who, m, k, n, activation));
   if (m == 0 || n == 0) return MX_OK;
-  MX_REQUIRE(y && (k == 0 || (x && w)), MX_ERR_INVALID, "mx_linear_forward: null buffer");
+  MX_REQUIRE(y && (k == 0 || (x && w)), MX_ERR_INVALID, who, ": null buffer");
+  hipStream_t s = resolve_stream(stream);
   const mx_gemm_desc d = forward_desc(m, k, n, bias != nullptr);
-  int64_t need = 0;
-  if (workspace && k > 0) {
-    MX_TRY(partials(d, &need));
-    MX_REQUIRE(workspace_bytes >= need, MX_ERR_WORKSPACE, "mx_linear_forward: workspace of ", workspace_bytes, " bytes, ",
-               need, " needed");
-  }
   const GemmEpilogue epi{activation, residual, z};
-  return gemm_within(&d, x, w, bias, y, kPartials, resolve_stream(stream), &epi, workspace);
+  int64_t need = 0;
+  Workspace ws;
+  if (!use_packed(m, k, n, false)) {
+    // The product's own scratch is optional: without the caller's, it allocates
+    // where it may.
+    if (workspace) {
+      MX_TRY(forward_bytes(m, k, n, &need));
+      MX_TRY(ws.take(who, workspace, workspace_bytes, need, s));
+    }
+    return gemm_within(&d, x, w, bias, y, kPartials, s, &epi, ws.as<void>());
+  }
+  MX_TRY(forward_bytes(m, k, n, &need));
+  MX_TRY(ws.take(who, workspace, workspace_bytes, need, s));
+  Carve c(ws.as<void>());
+  Forward f(m, k, n, &c);
+  f.x.first.src = f.x.second.src = x;
+  f.w.first.src = f.w.second.src = w;
+  f.x.second.exponent = f.head + 2;
+  f.w.second.exponent = f.head + 3;
+  ScanArgs scan{{f.x.first, f.w.first}, 2, activation, f.head};
+  MX_TRY(run_scan<true>(&scan, s));
+  PackArgs pack{{f.x.second, f.w.second}, 2, f.head};
+  MX_TRY(run_pack(&pack, s));
+  PieceArgs p{};
+  p.out = y;
+  p.bias = bias;
+  p.residual = residual;
+  p.z = z;
+  p.act = activation;
+  MX_TRY((run_piece<false, false, true>(p, f.deal, f.x, f.w, f.head, f.sums, f.pad, s)));
+  return gemm_within(&d, x, w, bias, y, 0, s, &epi, nullptr, f.head);
   MX_ABI_END
 }
 
@@ -212,7 +677,8 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
                                   int64_t n, int activation, float* dx, float* dw, float* db, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  MX_TRY(check("mx_linear_backward", m, k, n, activation));
+  const char* const who = "mx_linear_backward";
+  MX_TRY(check(who, m, k, n, activation));
   hipStream_t s = resolve_stream(stream);
   const auto zero = [&](float* p, int64_t count) -> int {
     if (!p || count == 0) return MX_OK;
@@ -226,46 +692,79 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
     return zero(db, n);
   }
   const bool slope = activation != MX_ACT_NONE;
-  MX_REQUIRE(dy && (!slope || z) && (k == 0 || ((!dx || w) && (!dw || x))), MX_ERR_INVALID,
-             "mx_linear_backward: null buffer");
+  MX_REQUIRE(dy && (!slope || z) && (k == 0 || ((!dx || w) && (!dw || x))), MX_ERR_INVALID, who, ": null buffer");
   if (k == 0) dx = dw = nullptr;
   if (!dx && !dw && !db) return MX_OK;
-  BackwardPlan plan;
-  MX_TRY(plan_backward(m, k, n, activation, &plan));
-  const bool products = dx || dw;
-  if (!products) plan.dz = plan.gemm = 0;
-  if (!db) plan.sums = 0;
-  // Captured calls without a workspace take the products in one pass each.
-  const bool caller = workspace != nullptr;
-  if (!caller) plan.gemm = 0;
+  // Without the caller's workspace the K splits of products that are not packed
+  // are left to them (captured calls take one pass each).
+  Carve size(nullptr);
+  const Backward want(m, k, n, slope, dx, dw, db, workspace != nullptr, &size);
+  MX_TRY(want.status);
   Workspace ws;
-  MX_TRY(ws.take("mx_linear_backward", workspace, workspace_bytes, plan.dz + plan.sums + plan.gemm, s));
-  char* const base = ws.as<char>();
-  float* const dz = plan.dz ? reinterpret_cast<float*>(base) : nullptr;
-  const SlopePlan sp = plan_slope(m, n);
-  if (db || dz) {
-    float* const part = !db ? nullptr : sp.parts > 1 ? reinterpret_cast<float*>(base + plan.dz) : db;
-    const dim3 grid{unsigned(sp.col_blocks), unsigned(sp.parts)};
-    const float* const zz = slope ? z : nullptr;
-    if (n >= 4)
-      hipLaunchKernelGGL(slope_kernel<4>, grid, dim3(256), 0, s, dy, zz, activation, m, int(n), sp.rows_per, dz, part);
-    else
-      hipLaunchKernelGGL(slope_kernel<1>, grid, dim3(256), 0, s, dy, zz, activation, m, int(n), sp.rows_per, dz, part);
-    MX_HIP(hipGetLastError());
-    if (db && sp.parts > 1) {
-      hipLaunchKernelGGL(column_sum_kernel, dim3(unsigned((n + 31) / 32)), dim3(1024), 0, s, part, sp.parts, int(n), db);
-      MX_HIP(hipGetLastError());
-    }
+  MX_TRY(ws.take(who, workspace, workspace_bytes, size.used, s));
+  Carve c(ws.as<void>());
+  Backward b(m, k, n, slope, dx, dw, db, workspace != nullptr, &c);
+  const float* const g = b.dz ? b.dz : dy;
+  // First pass: dz, its column sums and, for packed products, everyone's largest.
+  ScanArgs scan{};
+  scan.act = activation;
+  scan.count = 1;
+  ScanOp& first = scan.op[0];
+  if (b.packed) {
+    first = b.g.first;
+  } else {
+    first.m = m;
+    first.n = int(n);
+    first.rows_per = b.scan.rows_per;
+    first.col_blocks = b.scan.col_blocks;
+    first.parts = b.scan.parts;
   }
-  const float* const g = dz ? dz : dy;
-  void* const partial = caller && plan.gemm ? base + plan.dz + plan.sums : nullptr;
+  first.src = dy;
+  first.z = slope ? z : nullptr;
+  first.dz = b.dz;
+  first.sums = !db ? nullptr : b.scan.parts > 1 ? b.part : db;
+  if (b.packed) {
+    scan.bad = b.head;
+    b.g.second.src = g;
+    b.g.second.exponent = b.head + 2;
+    PackArgs pack{};
+    pack.bad = b.head;
+    pack.op[pack.count++] = b.g.second;
+    if (dw) {
+      b.x.first.src = b.x.second.src = x;
+      b.x.second.exponent = b.head + 3;
+      scan.op[scan.count++] = b.x.first;
+      pack.op[pack.count++] = b.x.second;
+    }
+    if (dx) {
+      b.w.first.src = b.w.second.src = w;
+      b.w.second.exponent = b.head + 4;
+      scan.op[scan.count++] = b.w.first;
+      pack.op[pack.count++] = b.w.second;
+    }
+    MX_TRY(run_scan<true>(&scan, s));
+    MX_TRY(run_pack(&pack, s));
+  } else if (db || b.dz) {
+    MX_TRY(run_scan<false>(&scan, s));
+  }
+  if (db && b.scan.parts > 1) {
+    hipLaunchKernelGGL(column_sum_kernel, dim3(unsigned((n + 31) / 32)), dim3(1024), 0, s, b.part, b.scan.parts, int(n), db);
+    MX_HIP(hipGetLastError());
+  }
+  const int64_t room = b.packed ? 0 : kPartials;
   if (dx) {
+    PieceArgs p{};
+    p.out = dx;
+    if (b.packed) MX_TRY((run_piece<false, true, false>(p, b.to_x, b.g, b.w, b.head, b.sums, b.pad, s)));
     const mx_gemm_desc d = dx_desc(m, k, n);
-    MX_TRY(gemm_within(&d, g, w, nullptr, dx, kPartials, s, nullptr, partial));
+    MX_TRY(gemm_within(&d, g, w, nullptr, dx, room, s, nullptr, b.split, b.packed ? b.head : nullptr));
   }
   if (dw) {
+    PieceArgs p{};
+    p.out = dw;
+    if (b.packed) MX_TRY((run_piece<true, true, false>(p, b.to_w, b.g, b.x, b.head + 1, b.sums, b.pad, s)));
     const mx_gemm_desc d = dw_desc(m, k, n);
-    MX_TRY(gemm_within(&d, g, x, nullptr, dw, kPartials, s, nullptr, partial));
+    MX_TRY(gemm_within(&d, g, x, nullptr, dw, room, s, nullptr, b.split, b.packed ? b.head + 1 : nullptr));
   }
   return MX_OK;
   MX_ABI_END

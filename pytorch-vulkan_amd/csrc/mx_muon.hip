@@ -174,10 +174,7 @@ struct StepArgs {
   int a_rows, b_rows, out_rows;
   int nk;                 // slabs
   int tiles_m, tiles_n, batch;
-  // Tiles from `whole` on are taken by `parts` workgroups each, which leave
-  // their sums of a share of the slabs in `sums` for join_kernel.
-  int whole, parts;
-  float* sums;
+  Shares share;
   float alpha;            // product of pieces -> stored value
   float diag, lin, unit;  // kPoly: a (the last iteration's) and b times the stored scale, 1 / G's scale
   float keep;             // kNext: a times the stored scale over X's
@@ -297,35 +294,18 @@ template <class T, int KIND>
 __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void step_kernel(StepArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
   constexpr bool SYM = symmetric(KIND);
-  int id = blockIdx.x, part = 0, k0 = 0, k1 = p.nk;
-  if (id < p.whole) {
-    id = mfma::xcd_remap(id, p.whole);
-  } else {
-    part = (id - p.whole) % p.parts;
-    k0 = part * (p.nk / 4) / p.parts * 4;
-    k1 = (part + 1) * (p.nk / 4) / p.parts * 4;
-    id = p.whole + (id - p.whole) / p.parts;
-  }
+  const Unit unit = unit_of(p.share, blockIdx.x, p.nk);
   int b, tm, tn;
-  tile_of<KIND>(p, id, b, tm, tn);
+  tile_of<KIND>(p, unit.tile, b, tm, tn);
   const Planes pa{const_cast<_Float16*>(p.a) + b * 2 * p.a_plane, p.a_plane, p.a_rows};
   const Planes pb{const_cast<_Float16*>(p.b) + b * 2 * p.b_plane, p.b_plane, p.b_rows};
   f32x16 acc[T::FM][T::FN];
-  product<T, !SYM, KIND == kLastRows>(acc, pa, pb, tm * T::BM, tn * T::BN, k0, k1 - k0, smem);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (id >= p.whole) {
-    f32x4* const to = reinterpret_cast<f32x4*>(p.sums) +
-                      ((int64_t(id - p.whole) * p.parts + part) * T::WAVES + wave) * (T::FM * T::FN * 256) + lane;
-#pragma unroll
-    for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-      for (int j = 0; j < T::FN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          to[((i * T::FN + j) * 4 + q) * 64] =
-              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+  product<T, false, !SYM, KIND == kLastRows>(acc, pa, pb, tm * T::BM, tn * T::BN, unit.k0, unit.k1 - unit.k0, smem);
+  if (unit.tile >= p.share.whole) {
+    store_sums<T>(acc, p.share, unit);
     return;
   }
+  const int wave = threadIdx.x >> 6;
   const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
 #pragma unroll
   for (int i = 0; i < T::FM; ++i)
@@ -333,27 +313,13 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
     for (int j = 0; j < T::FN; ++j) finish<KIND>(p, b, tm != tn, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
 }
 
-// The tiles that were taken in parts: a wave per 32 x 32 fragment sums the
-// parts in their order.
+// The tiles that were taken in parts.
 template <class T, int KIND>
 __global__ __launch_bounds__(64) void join_kernel(StepArgs p) {
-  constexpr int FRAGS = T::FM * T::FN, PER = T::WAVES * FRAGS;
-  const int tile = blockIdx.x / PER, wave = blockIdx.x % PER / FRAGS, f = blockIdx.x % FRAGS;
-  int b, tm, tn;
-  tile_of<KIND>(p, p.whole + tile, b, tm, tn);
-  const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) +
-                      ((int64_t(tile) * p.parts * T::WAVES + wave) * FRAGS + f) * 256 + threadIdx.x;
-  f32x4 s[4] = {};
-#pragma unroll 4
-  for (int q = 0; q < p.parts; ++q) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) s[g] += from[int64_t(q) * PER * 256 + g * 64];
-  }
-  f32x16 v;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) v[e] = s[e >> 2][e & 3];
-  finish<KIND>(p, b, tm != tn, tm * T::BM + wave / T::WN * (T::BM / T::WM) + f / T::FN * 32,
-               tn * T::BN + wave % T::WN * (T::BN / T::WN) + f % T::FN * 32, v);
+  int tile, m, n, b, tm, tn;
+  const f32x16 v = join_sums<T>(p.share, tile, m, n);
+  tile_of<KIND>(p, tile, b, tm, tn);
+  finish<KIND>(p, b, tm != tn, tm * T::BM + m, tn * T::BN + n, v);
 }
 
 // steps == 0: the scaled matrix itself.
@@ -369,14 +335,10 @@ __global__ __launch_bounds__(256) void scaled_kernel(Table tab, Update up, int64
   }
 }
 
-using Tile64 = Tile<64, 64, 2, 2, 4>;     // 4 waves of 32 x 32
-using Tile128 = Tile<128, 128, 2, 2, 2>;  // 4 waves of 64 x 64
-using Tile256 = Tile<256, 256, 2, 4, 2>;  // 8 waves of 128 x 64
-
 template <class T, int KIND>
 int launch(const StepArgs& p, int tiles, hipStream_t s) {
-  const int rest = tiles - p.whole;
-  hipLaunchKernelGGL((step_kernel<T, KIND>), dim3(unsigned(p.whole + rest * p.parts)), dim3(T::THREADS), 0, s, p);
+  const int rest = tiles - p.share.whole;
+  hipLaunchKernelGGL((step_kernel<T, KIND>), dim3(unsigned(p.share.whole + rest * p.share.parts)), dim3(T::THREADS), 0, s, p);
   MX_HIP(hipGetLastError());
   if (rest) {
     hipLaunchKernelGGL((join_kernel<T, KIND>), dim3(unsigned(rest * T::WAVES * T::FM * T::FN)), dim3(64), 0, s, p);
@@ -398,48 +360,11 @@ int launch_kind(int kind, const StepArgs& p, int tiles, hipStream_t s) {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// A CU's time per slab with n workgroups of a tile on it, and how many it
-// holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.  Over
-// 25 sets from one 64 x 100 to 16 x 1024^2 and 4096^2, all nine pairs of tiles
-// with and without parts timed: the choice takes 0.8% more than the best on
-// average, 11% at most.
-struct TileCost {
-  int tile, per_cu;
-  double fixed, each;
-  double slab(double n) const { return fixed + each * n; }
-};
-constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.05, 0.285}, {256, 1, 0.0, 1.15}};
-
-// How a product's tiles are dealt: whole rounds of the chip, then what is left
-// over in parts along K where a join (a launch and a pass over the sums) costs
-// less than the round that it shortens.
-struct Deal {
-  int64_t tiles, whole;
-  int parts;
-  double time;
-};
-Deal deal(const TileCost& c, int64_t tiles, int64_t nk, int64_t cu) {
-  Deal d{tiles, tiles, 1, 3.0};
-  const int64_t slots = cu * c.per_cu, full = tiles / slots, rest = tiles - full * slots;
-  d.time += double(full * nk) * c.slab(c.per_cu);
-  if (!rest) return d;
-  const double plain = double(nk) * c.slab(double((rest + cu - 1) / cu));
-  double least = plain;
-  for (int64_t parts = 2; parts <= 16 && parts * rest <= slots && parts * 8 <= nk; ++parts) {
-    const double share = double((nk / 4 + parts - 1) / parts * 4);
-    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 4.0 +
-                         double(rest * parts) * c.tile * c.tile * 8.0 / 6e6;
-    if (split >= least) continue;
-    least = split;
-    d.whole = full * slots;
-    d.parts = int(parts);
-  }
-  d.time += least;
-  return d;
-}
-
 // Tiles of a set's products (the symmetric ones and the others), what its sides
 // are padded to, and how the tiles are dealt.
+// Over 25 sets from one 64 x 100 to 16 x 1024^2 and 4096^2, all nine pairs of
+// tiles with and without parts timed, the choice takes 0.8% more than the best
+// on average, 11% at most.
 struct Plan {
   Geometry g;
   int sym, next;  // indexes into kTiles
@@ -472,8 +397,7 @@ Plan plan_set(int64_t rows, int64_t cols, int64_t batch) {
       const double time = p.gram.time + p.poly.time + p.update.time;
       if (least >= 0 && time >= least) continue;
       least = time;
-      const auto bytes = [](const Deal& d, int tile) { return (d.tiles - d.whole) * d.parts * tile * tile * 4; };
-      p.sums = std::max({bytes(p.gram, a.tile), bytes(p.poly, a.tile), bytes(p.update, c.tile)});
+      p.sums = std::max({p.gram.sum_bytes(a.tile), p.poly.sum_bytes(a.tile), p.update.sum_bytes(c.tile)});
       best = p;
     }
   return best;
@@ -644,11 +568,11 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
   p.muon = fin.up.muon;
   p.decay = decay;
   p.step = step;
-  p.sums = reinterpret_cast<float*>(poly + batch * 2 * g.g_plane());
+  p.share.sums = reinterpret_cast<float*>(poly + batch * 2 * g.g_plane());
   const auto run = [&](int kind, const Deal& d, int t) -> int {
     const int tile = kTiles[t].tile;
-    p.whole = int(d.whole);
-    p.parts = d.parts;
+    p.share.whole = int(d.whole);
+    p.share.parts = d.parts;
     p.tiles_m = g.sp / tile;
     p.tiles_n = (symmetric(kind) ? g.sp : g.lp) / tile;
     if (t == 0) return launch_kind<Tile64>(kind, p, int(d.tiles), s);

@@ -24,6 +24,8 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "mfma_core.hpp"
+
 namespace mx {
 namespace pieces {
 
@@ -95,6 +97,7 @@ __device__ __forceinline__ const char* uniform(const void* p) {
 // that the transposing reads of 16 lanes meet every bank once.
 template <int T, int LOADS, int WAVES, bool COLS>
 struct Operand {
+  static constexpr int PARTS = COLS ? 2 : 1;  // LDS reads of a fragment
   const char* src[LOADS];  // the wave's part of the next slab
   uint32_t lane_off;
   int64_t step;
@@ -135,7 +138,7 @@ struct Operand {
   }
   // The fragment of plane pl, 32 j rows (columns) on, from the LDS address of
   // this lane's parts; `off` is the slab's.
-  static __device__ __forceinline__ half8 frag(const uint32_t (&at)[COLS ? 2 : 1], int off, int pl, int j) {
+  static __device__ __forceinline__ half8 frag(const uint32_t (&at)[PARTS], int off, int pl, int j) {
     const int to = off + pl * T * kBK * 2 + j * 32 * (COLS ? 32 : 16);
     if constexpr (COLS) {
       s16x4 q[2];
@@ -164,19 +167,19 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// acc[i][j] = rows m0 + 32 i.. of A with rows (COLS: columns) n0 + 32 j.. of B
-// over nk slabs from slab0 (nk a multiple of four, at least four).  The matrix instruction's
+// acc[i][j] = rows (A_COLS: columns) m0 + 32 i.. of A with rows (B_COLS:
+// columns) n0 + 32 j.. of B over nk slabs from slab0 (nk a multiple of four, at least four).  The matrix instruction's
 // row operand is B, so that a lane ends with four consecutive columns n of one
 // row m, 8 bytes of a plane (ROW_LANES: A, and it ends with four rows of one
 // column, neighbours beside it).
 //
 // Slab t's products run from registers while slab t + 1's fragments are read
 // from LDS and slabs t + 2 and t + 3 come from memory, one barrier a slab.
-template <class T, bool COLS, bool ROW_LANES = false>
+template <class T, bool A_COLS, bool B_COLS, bool ROW_LANES = false>
 __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Planes& a, const Planes& b, int m0, int n0,
                                         int slab0, int nk, char* smem) {
-  using OpA = Operand<T::BM, T::LA, T::WAVES, false>;
-  using OpB = Operand<T::BN, T::LB, T::WAVES, COLS>;
+  using OpA = Operand<T::BM, T::LA, T::WAVES, A_COLS>;
+  using OpB = Operand<T::BN, T::LB, T::WAVES, B_COLS>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / T::WN * (T::BM / T::WM), wn = wave % T::WN * (T::BN / T::WN);
   OpA oa;
@@ -197,13 +200,16 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
   // LDS addresses of this lane's parts, for the lower and the upper two slabs
   // (an instruction's own offset reaches 64 KiB).  Opaque to the compiler,
   // which would keep an address register for every read otherwise.
-  uint32_t pa[2][1], pb[2][COLS ? 2 : 1];
+  uint32_t pa[2][OpA::PARTS], pb[2][OpB::PARTS];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    pa[half][0] = lds + half * 2 * T::STAGE + OpA::lane_offset(wm, lane, 0);
-    asm volatile("" : "+v"(pa[half][0]));
 #pragma unroll
-    for (int h = 0; h < (COLS ? 2 : 1); ++h) {
+    for (int h = 0; h < OpA::PARTS; ++h) {
+      pa[half][h] = lds + half * 2 * T::STAGE + OpA::lane_offset(wm, lane, h);
+      asm volatile("" : "+v"(pa[half][h]));
+    }
+#pragma unroll
+    for (int h = 0; h < OpB::PARTS; ++h) {
       pb[half][h] = lds + half * 2 * T::STAGE + T::A_BYTES + OpB::lane_offset(wn, lane, h);
       asm volatile("" : "+v"(pb[half][h]));
     }
@@ -239,7 +245,7 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
                         : __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[set][q == 0][j], fa[set][q == 1][i], c, 0, 0, 0);
         }
     // The next slab's reads go out among the first products.
-    constexpr int READS = 2 * T::FM + 2 * T::FN * (COLS ? 2 : 1), PRODUCTS = 3 * T::FM * T::FN;
+    constexpr int READS = 2 * T::FM * OpA::PARTS + 2 * T::FN * OpB::PARTS, PRODUCTS = 3 * T::FM * T::FN;
 #pragma unroll
     for (int r = 0; r < (READS < PRODUCTS ? READS : PRODUCTS); ++r) {
       __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
@@ -294,6 +300,104 @@ __device__ __forceinline__ half4 transpose4(half4 v) {
 // Element (row, col .. col + 3) of a plane, col % 4 == 0.
 __device__ __forceinline__ int64_t elem(const Planes& p, int row, int col) {
   return (int64_t(col >> 3) * p.rows + row) * 8 + (col & 7);
+}
+
+// ------------------------------------------------------------- tiles to CUs
+// Workgroups take whole tiles, `whole` of them; the tiles after those are taken
+// by `parts` workgroups each, which leave their sums of a share of the slabs in
+// `sums` for a second launch to join.
+struct Shares {
+  int whole, parts;
+  float* sums;
+};
+
+// Tile, part and slabs [k0, k1) of a workgroup.
+struct Unit {
+  int tile, part, k0, k1;
+};
+__device__ __forceinline__ Unit unit_of(const Shares& p, int id, int nk) {
+  if (id < p.whole) return {mfma::xcd_remap(id, p.whole), 0, 0, nk};
+  const int part = (id - p.whole) % p.parts;
+  return {p.whole + (id - p.whole) / p.parts, part, part * (nk / 4) / p.parts * 4, (part + 1) * (nk / 4) / p.parts * 4};
+}
+
+template <class T>
+__device__ __forceinline__ void store_sums(const f32x16 (&acc)[T::FM][T::FN], const Shares& p, const Unit& u) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  f32x4* const to = reinterpret_cast<f32x4*>(p.sums) +
+                    ((int64_t(u.tile - p.whole) * p.parts + u.part) * T::WAVES + wave) * (T::FM * T::FN * 256) + lane;
+#pragma unroll
+  for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < T::FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        to[((i * T::FN + j) * 4 + q) * 64] =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+}
+
+// One 32 x 32 fragment of a joined tile, workgroups of one wave: the parts in
+// their order.  m and n are the fragment's place in the tile.
+template <class T>
+__device__ __forceinline__ f32x16 join_sums(const Shares& p, int& tile, int& m, int& n) {
+  constexpr int FRAGS = T::FM * T::FN, PER = T::WAVES * FRAGS;
+  const int at = blockIdx.x / PER, wave = blockIdx.x % PER / FRAGS, f = blockIdx.x % FRAGS;
+  const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) +
+                      ((int64_t(at) * p.parts * T::WAVES + wave) * FRAGS + f) * 256 + threadIdx.x;
+  f32x4 s[4] = {};
+#pragma unroll 4
+  for (int q = 0; q < p.parts; ++q) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) s[g] += from[int64_t(q) * PER * 256 + g * 64];
+  }
+  f32x16 v;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = s[e >> 2][e & 3];
+  tile = p.whole + at;
+  m = wave / T::WN * (T::BM / T::WM) + f / T::FN * 32;
+  n = wave % T::WN * (T::BN / T::WN) + f % T::FN * 32;
+  return v;
+}
+
+using Tile64 = Tile<64, 64, 2, 2, 4>;     // 4 waves of 32 x 32
+using Tile128 = Tile<128, 128, 2, 2, 2>;  // 4 waves of 64 x 64
+using Tile256 = Tile<256, 256, 2, 4, 2>;  // 8 waves of 128 x 64
+
+// A CU's time per slab with n workgroups of a tile on it, and how many it
+// holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.
+struct TileCost {
+  int tile, per_cu;
+  double fixed, each;
+  double slab(double n) const { return fixed + each * n; }
+};
+constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.05, 0.285}, {256, 1, 0.0, 1.15}};
+
+// How a product's tiles are dealt: whole rounds of the chip, then what is left
+// over in parts along K where a join (a launch and a pass over the sums) costs
+// less than the round that it shortens.
+struct Deal {
+  int64_t tiles, whole;
+  int parts;
+  double time;  // microseconds
+  int64_t sum_bytes(int tile) const { return (tiles - whole) * parts * tile * tile * 4; }
+};
+inline Deal deal(const TileCost& c, int64_t tiles, int64_t nk, int64_t cu) {
+  Deal d{tiles, tiles, 1, 3.0};
+  const int64_t slots = cu * c.per_cu, full = tiles / slots, rest = tiles - full * slots;
+  d.time += double(full * nk) * c.slab(c.per_cu);
+  if (!rest) return d;
+  double least = double(nk) * c.slab(double((rest + cu - 1) / cu));
+  for (int64_t parts = 2; parts <= 16 && parts * rest <= slots && parts * 8 <= nk; ++parts) {
+    const double share = double((nk / 4 + parts - 1) / parts * 4);
+    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 4.0 +
+                         double(rest * parts) * c.tile * c.tile * 8.0 / 6e6;
+    if (split >= least) continue;
+    least = split;
+    d.whole = full * slots;
+    d.parts = int(parts);
+  }
+  d.time += least;
+  return d;
 }
 
 }  // namespace pieces
