@@ -61,6 +61,21 @@ struct ScanArgs {
   int* bad;  // cleared
 };
 
+// Largest over a wave, in lane 63, by moves within the vector unit (a shuffle
+// goes through LDS).
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+  const auto with = [&](auto ctrl) {
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), decltype(ctrl)::value, 0xF, 0xF, false)));
+  };
+  with(std::integral_constant<int, 0x111>{});  // row_shr:1, 2, 4, 8 within 16 lanes
+  with(std::integral_constant<int, 0x112>{});
+  with(std::integral_constant<int, 0x114>{});
+  with(std::integral_constant<int, 0x118>{});
+  with(std::integral_constant<int, 0x142>{});  // row_bcast:15, 31 across them
+  with(std::integral_constant<int, 0x143>{});
+  return v;
+}
+
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // A thread holds W columns; 64 threads lie along a row and the workgroup's four
@@ -115,9 +130,8 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
           top[e] = max(top[e], v);
           row = max(row, v);
         }
-#pragma unroll
-        for (int q = 1; q < 64; q <<= 1) row = max(row, uint32_t(__shfl_xor(int(row), q, 64)));
-        if (lane == 0 && r + 4 * u < r1) o.row_top[int64_t(bx) * o.m + r + 4 * u] = row;
+        row = wave_top(row);
+        if (lane == 63 && r + 4 * u < r1) o.row_top[int64_t(bx) * o.m + r + 4 * u] = row;
       }
     }
   }
@@ -140,9 +154,8 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
       all = max(all, top[e]);
     }
     if (in) *reinterpret_cast<uvecu*>(o.col_top + int64_t(by) * n + at) = top;
-#pragma unroll
-    for (int q = 1; q < 64; q <<= 1) all = max(all, uint32_t(__shfl_xor(int(all), q, 64)));
-    if (lane == 0) o.top[id] = all;
+    all = wave_top(all);
+    if (lane == 63) o.top[id] = all;
   }
 }
 
@@ -168,7 +181,7 @@ struct PackArgs {
 };
 
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
-  __shared__ uint32_t tops[4];
+  __shared__ uint32_t tops[4], col_tops[256];
   int k = 0;
   while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
   const PackOp& o = p.op[k];
@@ -192,9 +205,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   }
   uint32_t top = 0;
   for (int i = tid; i < o.tops; i += 256) top = max(top, o.top[i]);
-#pragma unroll
-  for (int q = 1; q < 64; q <<= 1) top = max(top, uint32_t(__shfl_xor(int(top), q, 64)));
-  if ((tid & 63) == 0) tops[tid >> 6] = top;
+  top = wave_top(top);
+  if ((tid & 63) == 63) tops[tid >> 6] = top;
   __syncthreads();
   top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
   const float largest = __uint_as_float(top);
@@ -210,11 +222,16 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     for (int i = 0; i < o.col_blocks; ++i) t = max(t, o.row_top[int64_t(i) * o.m + row]);
     bad = bad || low(t);
   }
-  if (by == 0 && tid < 64 && bx * 64 + tid < o.n) {
+  if (by == 0) {
+    const int c = bx * 64 + (tid & 63);
     uint32_t t = 0;
-#pragma unroll 8
-    for (int i = 0; i < o.parts; ++i) t = max(t, o.col_top[int64_t(i) * o.n + bx * 64 + tid]);
-    bad = bad || low(t);
+    if (c < o.n) {
+#pragma unroll 16
+      for (int i = tid >> 6; i < o.parts; i += 4) t = max(t, o.col_top[int64_t(i) * o.n + c]);
+    }
+    col_tops[tid] = t;
+    __syncthreads();
+    if (tid < 64) bad = bad || low(max(max(t, col_tops[64 + tid]), max(col_tops[128 + tid], col_tops[192 + tid])));
   }
   if (bad) {
     if (o.flags & 1) p.bad[0] = 1;
@@ -246,34 +263,42 @@ struct PieceArgs {
   int act;
 };
 
-template <bool EPI>
-__device__ __forceinline__ void finish_piece(const PieceArgs& p, int m, int n, const pieces::f32x16& acc) {
-  const int lane = threadIdx.x & 63, col = n + (lane & 31), row0 = m + 4 * (lane >> 5), up = *p.ea + *p.eb - 28;
-  const bool in = col < p.n;
+template <bool EPI, bool WHOLE>
+__device__ __forceinline__ void store_piece(const PieceArgs& p, int m, int n, const pieces::f32x16& acc, int up) {
+  const int lane = threadIdx.x & 63, col = n + (lane & 31), row0 = m + 4 * (lane >> 5);
+  const auto in = [&](int r) { return WHOLE || (col < p.n && row0 + r < p.m); };
   const int64_t at = int64_t(row0) * p.n + col;
   float bias = 0.f, res[16];
   if constexpr (EPI) {
-    if (p.bias && in) bias = p.bias[col];
+    if (p.bias && (WHOLE || col < p.n)) bias = p.bias[col];
     if (p.residual) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = 8 * (i >> 2) + (i & 3);
-        res[i] = in && row0 + r < p.m ? p.residual[at + int64_t(r) * p.n] : 0.f;
+        res[i] = in(r) ? p.residual[at + int64_t(r) * p.n] : 0.f;
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int r = 8 * (i >> 2) + (i & 3);
-    if (!in || row0 + r >= p.m) continue;
     float v = ldexpf(acc[i], up);
     if constexpr (EPI) {
       v += bias;
-      if (p.z) p.z[at + int64_t(r) * p.n] = v;
+      if (p.z && in(r)) p.z[at + int64_t(r) * p.n] = v;
       v = activate(p.act, v) + (p.residual ? res[i] : 0.f);
     }
-    p.out[at + int64_t(r) * p.n] = v;
+    if (in(r)) p.out[at + int64_t(r) * p.n] = v;
   }
+}
+
+// A 32 x 32 fragment at row m, column n.
+template <bool EPI>
+__device__ __forceinline__ void finish_piece(const PieceArgs& p, int m, int n, const pieces::f32x16& acc, int up) {
+  if (m + 32 <= p.m && n + 32 <= p.n)
+    store_piece<EPI, true>(p, m, n, acc, up);
+  else if (m < p.m && n < p.n)
+    store_piece<EPI, false>(p, m, n, acc, up);
 }
 
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
@@ -289,12 +314,12 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
     pieces::store_sums<T>(acc, p.share, unit);
     return;
   }
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), up = *p.ea + *p.eb - 28;
   const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
 #pragma unroll
   for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < T::FN; ++j) finish_piece<EPI>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+    for (int j = 0; j < T::FN; ++j) finish_piece<EPI>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j], up);
 }
 
 template <class T, bool EPI>
@@ -303,7 +328,7 @@ __global__ __launch_bounds__(64) void piece_join_kernel(PieceArgs p) {
   int tile, m, n, tm, tn;
   const pieces::f32x16 v = pieces::join_sums<T>(p.share, tile, m, n);
   mfma::tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn);
-  finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v);
+  finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, *p.ea + *p.eb - 28);
 }
 
 // out[c] = sum of part[p][c] in the order of p: 32 columns and 32 groups of
@@ -408,6 +433,17 @@ struct Carve {
 };
 
 // ------------------------------------------------------------ packed products
+// Products of packed operands run on 128 x 128 tiles, two workgroups to a CU, so
+// that one's stores and activations go on beside the other's products (4096 x
+// 1024 -> 4096 with GELU: 114 us, on 256 x 256 tiles 150; without an epilogue 91
+// and 88).
+using PieceTile = pieces::Tile128;
+constexpr int kPad = PieceTile::BM;
+int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
+pieces::Deal plan_piece(int64_t m, int64_t n, int64_t k) {
+  return pieces::deal(pieces::kTiles[1], padded(m) / kPad * (padded(n) / kPad), padded(k) / pieces::kBK, cu_count());
+}
+
 // An operand [m][n] of packed products: what its passes write.
 struct Packed {
   int64_t m, n;
@@ -416,12 +452,12 @@ struct Packed {
   PackOp second;
 };
 
-Packed packed(int64_t m, int64_t n, int pad, int flags, Carve* c) {
+Packed packed(int64_t m, int64_t n, int flags, Carve* c) {
   Packed o{};
   o.m = m;
   o.n = n;
   o.scan = plan_scan(m, n);
-  const int64_t mp = (m + pad - 1) / pad * pad, np = (n + pad - 1) / pad * pad;
+  const int64_t mp = padded(m), np = padded(n);
   o.first.m = m;
   o.first.n = int(n);
   o.first.rows_per = o.scan.rows_per;
@@ -444,48 +480,48 @@ Packed packed(int64_t m, int64_t n, int pad, int flags, Carve* c) {
   return o;
 }
 
-// One product's tile and how its tiles are dealt; sides padded to `pad`.
-struct PieceDeal {
-  int tile;  // index into pieces::kTiles
-  pieces::Deal deal;
-};
-PieceDeal plan_piece(int64_t m, int64_t n, int64_t k, int pad) {
-  PieceDeal best{};
-  const auto pd = [&](int64_t v) { return (v + pad - 1) / pad * pad; };
-  for (int i = 1; i < 3; ++i) {
-    const pieces::TileCost& c = pieces::kTiles[i];
-    if (pad % c.tile) continue;
-    const pieces::Deal d = pieces::deal(c, pd(m) / c.tile * (pd(n) / c.tile), pd(k) / pieces::kBK, cu_count());
-    if (!best.tile || d.time < best.deal.time) best = {i, d};
-  }
-  return best;
-}
-
-// What padding a call's products want: 128 or 256.
-int pick_pad(int64_t m, int64_t k, int64_t n, bool backward) {
-  double time[2];
-  for (int i = 0; i < 2; ++i) {
-    const int pad = 128 << i;
-    time[i] = backward ? plan_piece(m, k, n, pad).deal.time + plan_piece(n, k, m, pad).deal.time
-                       : plan_piece(m, n, k, pad).deal.time;
-  }
-  return time[1] < time[0] ? 256 : 128;
-}
-
 // Largest packed scratch of a call.
 constexpr int64_t kMostPacked = int64_t(4) << 30;
 
-// Whether a call's products run on packed operands: PACKED_RULE
+// Whether a call's products run on packed operands: where the time that they
+// save passes what the two passes take, both fitted to measurements
+// (microseconds, mx_gemm.hip's products / packed, with GELU):
+//   m x k -> n            forward     backward
+//   4096 x 1024 -> 4096   216 / 137   481 / 279
+//   8192 x 4096 -> 512    199 / 214   396 / 331
+//   2048 x 2048 -> 2048   110 /  86   228 / 139
+//   256 x 4096 -> 4096     60 /  85   121 / 117
+//   2048 x 1024 -> 1024    38 /  41    92 /  71
+//   1024 x 1024 -> 1024    27 /  33    60 /  56
+//   1537 x 765 -> 2050     64 /  49   133 /  84   (rows not 16-byte aligned)
+//   700 x 700 -> 700       16 /  31    41 /  49
 bool use_packed(int64_t m, int64_t k, int64_t n, bool backward) {
   if (m < 4 || k < 4 || n < 4) return false;
-  if ((m * k + k * n + (backward ? m * n : 0)) * 5 > kMostPacked) return false;
-  if (const char* e = std::getenv("MXLP")) return e[0] == '1';
-  return 2.0 * double(m) * double(n) * double(k) >= 4e9;
+  const double mn = double(m) * double(n), sides = double(m) * double(k) + double(n) * double(k);
+  if ((sides + mn) * 5 > double(kMostPacked)) return false;
+  const bool vec = k % 4 == 0 && (!backward || n % 4 == 0);
+  const double saved = mn * double(k) * (backward ? 4e-9 : 2e-9) * (vec ? 3.0 : 10.0);
+  const double passes = backward ? 10.0 + (8.0 * mn + 16.0 * sides) / 7e6 : 12.0 + 20.0 * sides / 7e6;
+  return saved > passes;
 }
 
-template <class T, bool A_COLS, bool B_COLS, bool EPI>
-int launch_piece(const PieceArgs& p, int tiles, hipStream_t s) {
-  const int rest = tiles - p.share.whole;
+// out [m][n] over k: operands a (its rows, or A_COLS columns, are m) and b.
+template <bool A_COLS, bool B_COLS, bool EPI>
+int run_piece(PieceArgs p, const pieces::Deal& d, const Packed& a, const Packed& b, const int* bad, float* sums,
+              hipStream_t s) {
+  using T = PieceTile;
+  p.a = a.second.to;
+  p.b = b.second.to;
+  p.ea = a.second.exponent;
+  p.eb = b.second.exponent;
+  p.bad = bad;
+  p.m = int(A_COLS ? a.n : a.m);
+  p.n = int(B_COLS ? b.n : b.m);
+  p.nk = int(padded(A_COLS ? a.m : a.n) / pieces::kBK);
+  p.tiles_m = int(padded(p.m) / kPad);
+  p.tiles_n = int(padded(p.n) / kPad);
+  p.share = {int(d.whole), d.parts, sums};
+  const int rest = int(d.tiles - d.whole);
   hipLaunchKernelGGL((piece_kernel<T, A_COLS, B_COLS, EPI>), dim3(unsigned(p.share.whole + rest * p.share.parts)),
                      dim3(T::THREADS), 0, s, p);
   MX_HIP(hipGetLastError());
@@ -494,27 +530,6 @@ int launch_piece(const PieceArgs& p, int tiles, hipStream_t s) {
     MX_HIP(hipGetLastError());
   }
   return MX_OK;
-}
-
-// out [m][n] over k: operands a (its rows, or A_COLS columns, are m) and b.
-template <bool A_COLS, bool B_COLS, bool EPI>
-int run_piece(PieceArgs p, const PieceDeal& d, const Packed& a, const Packed& b, const int* bad, float* sums, int pad,
-              hipStream_t s) {
-  const int tile = pieces::kTiles[d.tile].tile;
-  const auto pd = [&](int64_t v) { return int((v + pad - 1) / pad * pad); };
-  p.a = a.second.to;
-  p.b = b.second.to;
-  p.ea = a.second.exponent;
-  p.eb = b.second.exponent;
-  p.bad = bad;
-  p.m = int(A_COLS ? a.n : a.m);
-  p.n = int(B_COLS ? b.n : b.m);
-  p.nk = pd(A_COLS ? a.m : a.n) / pieces::kBK;
-  p.tiles_m = pd(p.m) / tile;
-  p.tiles_n = pd(p.n) / tile;
-  p.share = {int(d.deal.whole), d.deal.parts, sums};
-  if (d.tile == 1) return launch_piece<pieces::Tile128, A_COLS, B_COLS, EPI>(p, int(d.deal.tiles), s);
-  return launch_piece<pieces::Tile256, A_COLS, B_COLS, EPI>(p, int(d.deal.tiles), s);
 }
 
 // First and second pass of a call's operands.
@@ -547,20 +562,18 @@ int run_pack(PackArgs* p, hipStream_t s) {
 // Workspace of a forward: the packed operands, or the product's K split.
 struct Forward {
   bool packed;
-  int pad = 0;
   Packed x, w;
   int* head = nullptr;  // two flags, three exponents
-  PieceDeal deal{};
+  pieces::Deal deal{};
   float* sums = nullptr;
   int64_t partial = 0;
   Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(use_packed(m, k, n, false)) {
     if (!packed) return;
-    pad = pick_pad(m, k, n, false);
     head = c->take<int>(8);
-    x = mx::packed(m, k, pad, 1, c);
-    w = mx::packed(n, k, pad, 1, c);
-    deal = plan_piece(m, n, k, pad);
-    sums = c->take<float>(deal.deal.sum_bytes(pieces::kTiles[deal.tile].tile) / 4);
+    x = mx::packed(m, k, 1, c);
+    w = mx::packed(n, k, 1, c);
+    deal = plan_piece(m, n, k);
+    sums = c->take<float>(deal.sum_bytes(kPad) / 4);
   }
 };
 
@@ -576,12 +589,11 @@ int forward_bytes(int64_t m, int64_t k, int64_t n, int64_t* bytes) {
 // Workspace of a backward.
 struct Backward {
   bool packed;
-  int pad = 0;
   ScanPlan scan;  // of dz
   float *dz = nullptr, *part = nullptr, *sums = nullptr;
   int* head = nullptr;
   Packed g, x, w;
-  PieceDeal to_x{}, to_w{};
+  pieces::Deal to_x{}, to_w{};
   int64_t gemm = 0;
   void* split = nullptr;
   int status = MX_OK;
@@ -590,15 +602,13 @@ struct Backward {
     if (slope && (want_x || want_w)) dz = c->take<float>(m * n);
     if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
     if (packed) {
-      pad = pick_pad(m, k, n, true);
       head = c->take<int>(8);
-      g = mx::packed(m, n, pad, (want_x ? 1 : 0) | (want_w ? 2 : 0), c);
-      if (want_w) x = mx::packed(m, k, pad, 2, c);
-      if (want_x) w = mx::packed(n, k, pad, 1, c);
-      to_x = plan_piece(m, k, n, pad);
-      to_w = plan_piece(n, k, m, pad);
-      sums = c->take<float>(std::max(want_x ? to_x.deal.sum_bytes(pieces::kTiles[to_x.tile].tile) : 0,
-                                     want_w ? to_w.deal.sum_bytes(pieces::kTiles[to_w.tile].tile) : 0) / 4);
+      g = mx::packed(m, n, (want_x ? 1 : 0) | (want_w ? 2 : 0), c);
+      if (want_w) x = mx::packed(m, k, 2, c);
+      if (want_x) w = mx::packed(n, k, 1, c);
+      to_x = plan_piece(m, k, n);
+      to_w = plan_piece(n, k, m);
+      sums = c->take<float>(std::max(want_x ? to_x.sum_bytes(kPad) : 0, want_w ? to_w.sum_bytes(kPad) : 0) / 4);
     } else if (split_room && k > 0) {
       int64_t a = 0, b = 0;
       if (want_x) status = partials(dx_desc(m, k, n), &a);
@@ -668,7 +678,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   p.residual = residual;
   p.z = z;
   p.act = activation;
-  MX_TRY((run_piece<false, false, true>(p, f.deal, f.x, f.w, f.head, f.sums, f.pad, s)));
+  MX_TRY((run_piece<false, false, true>(p, f.deal, f.x, f.w, f.head, f.sums, s)));
   return gemm_within(&d, x, w, bias, y, 0, s, &epi, nullptr, f.head);
   MX_ABI_END
 }
@@ -755,14 +765,14 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   if (dx) {
     PieceArgs p{};
     p.out = dx;
-    if (b.packed) MX_TRY((run_piece<false, true, false>(p, b.to_x, b.g, b.w, b.head, b.sums, b.pad, s)));
+    if (b.packed) MX_TRY((run_piece<false, true, false>(p, b.to_x, b.g, b.w, b.head, b.sums, s)));
     const mx_gemm_desc d = dx_desc(m, k, n);
     MX_TRY(gemm_within(&d, g, w, nullptr, dx, room, s, nullptr, b.split, b.packed ? b.head : nullptr));
   }
   if (dw) {
     PieceArgs p{};
     p.out = dw;
-    if (b.packed) MX_TRY((run_piece<true, true, false>(p, b.to_w, b.g, b.x, b.head + 1, b.sums, b.pad, s)));
+    if (b.packed) MX_TRY((run_piece<true, true, false>(p, b.to_w, b.g, b.x, b.head + 1, b.sums, s)));
     const mx_gemm_desc d = dw_desc(m, k, n);
     MX_TRY(gemm_within(&d, g, x, nullptr, dw, room, s, nullptr, b.split, b.packed ? b.head + 1 : nullptr));
   }

@@ -444,3 +444,164 @@ def test_calls_on_another_stream_and_in_a_graph(mx):
         torch.cuda.synchronize()
         for a, b_ in zip(eager[i], state()):
             assert torch.equal(a, b_), f"replay {i}"
+
+
+# ------------------------------------------- linear layers on packed operands
+# Sizes at which the library packs its operands into two fp16 pieces, forward and
+# backward: whole tiles, ragged ones, rows at no 16-byte boundary.
+PACKED_SHAPES = [(2048, 2048, 2048), (1537, 765, 2050), (3001, 1003, 2999), (1290, 2052, 1924)]
+
+
+def packed_case(m, k, n):
+    g = gen(m + n)
+    return rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, n, scale=0.3), rand(g, m, n), rand(g, m, n, scale=0.1)
+
+
+def run_linear(mx, x, w, b, res, dy, code):
+    m, k, n = *x.shape, w.shape[0]
+    (y, t0), (z, t1), (dx, t2), (dw, t3), (db, t4) = guarded(m, n), guarded(m, n), guarded(m, k), guarded(n, k), guarded(n)
+    mx.linear_forward(x, w, b, y, activation=code, residual=res, z=z, stream=stream())
+    mx.linear_backward(dy, x, w, z, dx, dw, db, activation=code, stream=stream())
+    intact(t0, t1, t2, t3, t4)
+    return y, z, dx, dw, db
+
+
+def check_linear(x, w, b, res, dy, act, out, what):
+    """A packed element is off by 2 u of itself or, as rows and columns lie within
+    2^8 of the largest, of 2^-16 of that at the least; u / 4 of every term is
+    dropped, and a sum of k terms rounds at most 3 k / 16 + 3 times."""
+    y, z, dx, dw, db = out
+    d = lambda t: t.double()
+    k, n, m = x.shape[1], w.shape[0], x.shape[0]
+    zr, yr = linear_ref(d(x), d(w), d(b), d(res), act)
+    mag = d(x).abs() @ d(w).abs().t() + d(b).abs()
+    floor = 2.0 ** -39 * float(x.abs().max()) * d(w).abs().sum(1) + 2.0 ** -39 * float(w.abs().max()) * d(x).abs().sum(1)[:, None]
+    z_err = (3 * k / 16 + 12) * U * mag + floor
+    within(z, zr, z_err, what + " z")
+    within(y, yr, 1.13 * z_err + 16 * U * (zr.abs() + 1) + 4 * U * yr.abs(), what + " y")
+    zl = d(z).cpu().requires_grad_()
+    dz = torch.autograd.grad(ACT64[act](zl), zl, d(dy).cpu())[0].cuda()
+    dz_err = 16 * U * d(dy).abs() * (d(z).abs() + 1)
+    top = 2.0 ** -39 * float(dz.abs().max())
+    f_x = top * d(w).abs().sum(0) + 2.0 ** -39 * float(w.abs().max()) * dz.abs().sum(1)[:, None]
+    f_w = top * d(x).abs().sum(0) + 2.0 ** -39 * float(x.abs().max()) * dz.abs().sum(0)[:, None]
+    within(dx, dz @ d(w), ((3 * n / 16 + 12) * U * dz.abs() + dz_err) @ d(w).abs() + f_x + 1e-30, what + " dx")
+    within(dw, dz.t() @ d(x), ((3 * m / 16 + 12) * U * dz.abs() + dz_err).t() @ d(x).abs() + f_w + 1e-30, what + " dw")
+    within(db, dz.sum(0), ((m / 64 + 64) * U * dz.abs() + dz_err).sum(0) + 1e-30, what + " db")
+
+
+@pytest.mark.parametrize("m,k,n", PACKED_SHAPES)
+@pytest.mark.parametrize("act", ["none", "gelu", "silu"])
+def test_linear_packed(mx, m, k, n, act):
+    print("packed linear", m, k, n, act, flush=True)
+    case = packed_case(m, k, n)
+    code = mx.ACTIVATIONS[act]
+    out = run_linear(mx, *case, code)
+    check_linear(*case, act, out, act)
+    # Accuracy is FP32's: no further from float64 than twice torch's FP32 product.
+    x, w, b = case[:3]
+    want = x.double() @ w.double().t() + b.double()
+    err = lambda t: float((t.double() - want).norm())
+    assert err(out[1]) <= 2 * err(torch.addmm(b, x, w.t()))
+    # Masked tokens: rows of zeros cost nothing and stay zero.
+    x, w, b, res, dy = case
+    dy = dy.clone()
+    dy[::3] = 0
+    out = run_linear(mx, x, w, b, res, dy, code)
+    check_linear(x, w, b, res, dy, act, out, act + " masked")
+    assert float(out[2][::3].abs().max()) == 0
+
+
+def test_linear_packed_scales(mx):
+    """Operands far from 1, each as a whole: one scale holds them."""
+    m, k, n = 2048, 2048, 2048
+    x, w, b, res, dy = packed_case(m, k, n)
+    for sx, sw, sg in ((2.0 ** 40, 2.0 ** -30, 2.0 ** 20), (2.0 ** -60, 2.0 ** 50, 2.0 ** -60)):
+        y = torch.empty(m, n, device="cuda")
+        z = torch.empty_like(y)
+        mx.linear_forward(x * sx, w * sw, None, y, z=z, stream=stream())
+        base = torch.empty_like(y)
+        mx.linear_forward(x, w, None, base, stream=stream())
+        assert torch.equal(y, base * (sx * sw)), "powers of two change nothing but the exponent"
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        dx1, dw1 = torch.empty_like(x), torch.empty_like(w)
+        mx.linear_backward(dy * sg, x * sx, w * sw, None, dx, dw, None, stream=stream())
+        mx.linear_backward(dy, x, w, None, dx1, dw1, None, stream=stream())
+        assert torch.equal(dx, dx1 * (sg * sw)) and torch.equal(dw, dw1 * (sg * sx))
+
+
+def misfits(x, w, dy):
+    """Operands that one scale cannot hold, by name."""
+    m, k, n = *x.shape, w.shape[0]
+    ramp = lambda c, e: torch.exp2(torch.linspace(-e, e, c, device="cuda"))
+    yield "rows of x", x * ramp(m, 30)[:, None], w, dy
+    yield "a dead column of x", torch.cat([x[:, :1] * 1e-6, x[:, 1:]], 1), w, dy
+    yield "channels against each other", x * ramp(k, 20), w * ramp(k, -20), dy
+    yield "columns of dy against rows of w", x, w * ramp(n, -40)[:, None], dy * ramp(n, 30)
+    yield "a huge element", x, w.index_put((torch.tensor([5], device="cuda"), torch.tensor([7], device="cuda")),
+                                           torch.tensor([1e30], device="cuda")), dy
+    yield "tiny", x * 1e-36, w, dy * 1e-36
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_linear_packed_misfits(mx, which):
+    m, k, n = 2048, 2048, 2048
+    x, w, b, res, dy = packed_case(m, k, n)
+    name, x, w, dy = list(misfits(x, w, dy))[which]
+    print("misfit", name, flush=True)
+    y, dx, dw, db = torch.empty(m, n, device="cuda"), torch.empty(m, k, device="cuda"), torch.empty(n, k, device="cuda"), torch.empty(n, device="cuda")
+    mx.linear_forward(x, w, None, y, stream=stream())
+    mx.linear_backward(dy, x, w, None, dx, dw, db, stream=stream())
+    d = lambda t: t.double()
+    within(y, d(x) @ d(w).t(), (k / 8 + 8) * U * (d(x).abs() @ d(w).abs().t()) + 1e-44, name + " y")
+    within(dx, d(dy) @ d(w), (n / 8 + 8) * U * (d(dy).abs() @ d(w).abs()) + 1e-44, name + " dx")
+    within(dw, d(dy).t() @ d(x), (m / 8 + 8) * U * (d(dy).abs().t() @ d(x).abs()) + 1e-44, name + " dw")
+
+
+def test_linear_packed_special_values(mx):
+    m, k, n = 2048, 2048, 2048
+    x, w, b, res, dy = packed_case(m, k, n)
+    x[3, 5], x[7, 9] = float("inf"), float("nan")
+    y = torch.empty(m, n, device="cuda")
+    mx.linear_forward(x, w, b, y, activation=mx.ACT_RELU, stream=stream())
+    ref = F.relu(x.cpu() @ w.cpu().t() + b.cpu())
+    got = y.cpu()
+    assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.isposinf(), ref.isposinf())
+    zero = torch.zeros_like(x)
+    mx.linear_forward(zero, w, b, y, stream=stream())
+    assert torch.equal(y, b.expand(m, n))
+
+
+def test_linear_packed_in_a_graph(mx):
+    m, k, n = 2048, 2048, 2048
+    x, w, b, res, dy = packed_case(m, k, n)
+    y, z = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    ws = torch.empty(max(mx.linear_workspace(m, k, n, mx.ACT_GELU), mx.linear_workspace(m, k, n, mx.ACT_GELU, True)),
+                     dtype=torch.uint8, device="cuda")
+
+    def step():
+        mx.linear_forward(x, w, b, y, activation=mx.ACT_GELU, residual=res, z=z, workspace=ws, stream=stream())
+        mx.linear_backward(dy, x, w, z, dx, dw, db, activation=mx.ACT_GELU, workspace=ws, stream=stream())
+
+    step()
+    want = [t.clone() for t in (y, z, dx, dw, db)]
+    spread = x * torch.exp2(torch.linspace(-30, 30, m, device="cuda"))[:, None]
+    keep = x.clone()
+    x.copy_(spread)
+    step()
+    want_spread = [t.clone() for t in (y, z, dx, dw, db)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for inputs, ref in ((keep, want), (spread, want_spread), (keep, want), (spread, want_spread)):
+        x.copy_(inputs)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b_ in zip((y, z, dx, dw, db), ref):
+            assert torch.equal(a, b_)
+    with pytest.raises(mx.MXError, match="workspace"):
+        side = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(side):
+            mx.linear_forward(x, w, b, y, stream=stream())
