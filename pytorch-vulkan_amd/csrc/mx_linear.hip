@@ -435,13 +435,13 @@ struct Carve {
 // ------------------------------------------------------------ packed products
 // Products of packed operands run on 128 x 128 tiles, two workgroups to a CU, so
 // that one's stores and activations go on beside the other's products (4096 x
-// 1024 -> 4096 with GELU: 114 us, on 256 x 256 tiles 150; without an epilogue 91
-// and 88).
+// 1024 -> 4096 with GELU: 113 us, on 256 x 256 tiles 103 to 116; without an
+// epilogue 90 and 87: not worth kernels of their own).
 using PieceTile = pieces::Tile128;
 constexpr int kPad = PieceTile::BM;
 int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
 pieces::Deal plan_piece(int64_t m, int64_t n, int64_t k) {
-  return pieces::deal(pieces::kTiles[1], padded(m) / kPad * (padded(n) / kPad), padded(k) / pieces::kBK, cu_count());
+  return pieces::deal(pieces::kTiles[pieces::kTile128], padded(m) / kPad * (padded(n) / kPad), padded(k) / pieces::kBK, cu_count());
 }
 
 // An operand [m][n] of packed products: what its passes write.

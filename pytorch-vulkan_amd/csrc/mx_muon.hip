@@ -111,27 +111,16 @@ struct Geometry {
   int s, l;           // shorter and longer side
   int sp, lp;         // padded
   bool turned;        // X = U^T
-  int64_t x_plane() const { return int64_t(sp) * lp; }
-  int64_t g_plane() const { return int64_t(sp) * sp; }
+  __host__ __device__ int64_t x_plane() const { return int64_t(sp) * lp; }
+  __host__ __device__ int64_t g_plane() const { return int64_t(sp) * sp; }
 };
 
-// X's pieces: 32 rows of X and 64 of its columns to a workgroup, eight columns
-// of a row to a thread.
-__global__ __launch_bounds__(256) void pack_kernel(Table tab, Update up, Geometry g, const double* parts, int nparts,
-                                                   double eps, float scale, double growth, _Float16* x,
-                                                   float* lift) {
-  const int b = blockIdx.z;
-  // |X|_F is 1, unless eps is what divides: then X is kept times 2^e, which no
-  // iteration's growth takes past the bounds, so that fp16 holds it.
-  const double n = norm_of(parts + b * kNormParts, nparts), d = n < eps ? eps : n, small = n / d * growth;
-  const int up2 = small > 0 && small < 1 ? int(floor(-log2(small))) : 0;
-  const double inv = ldexp(double(scale), up2) / d;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) lift[b] = float(ldexp(1.0, -up2));
-  const float* const in = tab.in[b];
-  const float* const buf = tab.buf[b];
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), col = blockIdx.x * 64 + (threadIdx.x >> 5) * 8;
-  float u[8] = {}, m[8] = {};
+// U's elements at X's row and eight columns from col, zeros past X's end.
+__device__ __forceinline__ void take_u(const Table& tab, const Update& up, const Geometry& g, int b, int row, int col,
+                                       float (&u)[8]) {
   const auto take = [&](const float* from, float (&to)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to[e] = 0.f;
     if (row >= g.s || col >= g.l) return;
     if (g.turned) {  // neighbours along U's rows in neighbouring lanes
 #pragma unroll
@@ -149,16 +138,44 @@ __global__ __launch_bounds__(256) void pack_kernel(Table tab, Update up, Geometr
       for (int e = 0; e < 8; ++e) to[e] = col + e < g.l ? from[int64_t(row) * g.cols + col + e] : 0.f;
     }
   };
-  take(in, u);
-  if (up.muon) take(buf, m);
+  take(tab.in[b], u);
+  if (!up.muon) return;
+  float m[8];
+  take(tab.buf[b], m);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = up.u(m[e], u[e]);
+}
+
+// What U's elements are multiplied by to become X's stored value.  |X|_F is 1,
+// unless eps is what divides: then X is kept times 2^up2, which no iteration's
+// growth takes past the bounds, so that fp16 holds it.
+__device__ __forceinline__ double scale_of(const double* parts, int nparts, double eps, double growth, float scale,
+                                           int& up2) {
+  const double n = norm_of(parts, nparts), d = n < eps ? eps : n, small = n / d * growth;
+  up2 = small > 0 && small < 1 ? int(floor(-log2(small))) : 0;
+  return ldexp(double(scale), up2) / d;
+}
+
+// X's pieces: 32 rows of X and 64 of its columns to a workgroup, eight columns
+// of a row to a thread.
+__global__ __launch_bounds__(256) void pack_kernel(Table tab, Update up, Geometry g, const double* parts, int nparts,
+                                                   double eps, float scale, double growth, _Float16* x,
+                                                   float* lift) {
+  const int b = blockIdx.z;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), col = blockIdx.x * 64 + (threadIdx.x >> 5) * 8;
+  float u[8];
+  take_u(tab, up, g, b, row, col, u);
+  int up2;
+  const double inv = scale_of(parts + b * kNormParts, nparts, eps, growth, scale, up2);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) lift[b] = float(ldexp(1.0, -up2));
   half8 hi, lo;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float v = float(double(up.muon ? up.u(m[e], u[e]) : u[e]) * inv);
+    const float v = float(double(u[e]) * inv);
     hi[e] = _Float16(v);
     lo[e] = _Float16(v - float(hi[e]));
   }
-  const int64_t plane = int64_t(g.sp) * g.lp;
+  const int64_t plane = g.x_plane();
   _Float16* const to = x + b * 2 * plane + (int64_t(col >> 3) * g.sp + row) * 8;
   *reinterpret_cast<half8*>(to) = hi;
   *reinterpret_cast<half8*>(to + plane) = lo;
@@ -335,6 +352,240 @@ __global__ __launch_bounds__(256) void scaled_kernel(Table tab, Update up, int64
   }
 }
 
+// ------------------------------------------------------- one launch a step
+// Matrices of at most 64 rows: an iteration is one launch.  Each workgroup sums
+// the partial G's that the workgroups of the launch before it left, makes P of it
+// for itself, moves its own columns of X by it, and leaves its part of the next
+// G.  X stays where it is.  The first launch packs X; the last one stores the
+// factor.  Bound by the launches and by the barriers within one (use_small()).
+struct SmallArgs {
+  Table tab;
+  Update up;
+  Geometry g;
+  const double* norms;
+  int nparts;
+  double eps, growth;
+  float scale;            // of X's first pieces
+  float* lift;
+  _Float16* x;
+  const float* from;      // partial G's of the launch before, [matrix][workgroup][fragment][256][4]
+  float* to;
+  float gram;             // pieces of X, product -> G's stored value
+  float alpha, diag, lin, unit;  // P
+  float move, keep;       // X: product -> stored value, X's pieces -> stored value
+  float decay, step;
+};
+enum SmallMode { kSmallFirst, kSmallNext, kSmallLast };
+constexpr int kSmall = 64;       // X's rows, padded
+constexpr int kSmallWide = 16;   // most workgroups of a matrix: each reads every other's part of G
+
+template <int MODE>
+__global__ __launch_bounds__(256) void small_kernel(SmallArgs p) {
+  constexpr int SP = kSmall, F = SP / 32, NF = F * (F + 1) / 2;  // fragments of a side, of the triangle
+  constexpr int ITEMS = SP * 8 / 256;                            // groups of eight columns of a thread
+  __shared__ __attribute__((aligned(16))) char gp[MODE == kSmallFirst ? 16 : 2 * SP * SP * 2];
+  __shared__ __attribute__((aligned(16))) char xs[2 * SP * 64 * 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = blockIdx.x, nw = gridDim.x, b = blockIdx.y;
+  // Three waves hold the triangle's fragments (0, 0), (1, 0), (1, 1).
+  const bool mine = wave < NF;
+  const int fr = wave == 0 ? 0 : 1, fc = wave == 2 ? 1 : 0;
+  // 16 bytes of G's or P's plane pl: eight columns from 8 kg of a row; of X's, rows
+  // of a group rearranged so that transposing reads meet every bank once.
+  const auto g_at = [&](int pl, int kg, int row) { return gp + ((pl * (SP / 8) + kg) * SP + row) * 16; };
+  const auto x_at = [&](int pl, int kg, int row) { return xs + ((pl * 8 + kg) * SP + (row ^ ((kg & 3) << 2))) * 16; };
+  const auto mul = [](f32x16& acc, const half8 (&fb)[2], const half8 (&fa)[2]) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[1], fa[0], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[0], fa[1], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[0], fa[0], acc, 0, 0, 0);
+  };
+  const auto store_g = [&](int m, int n, const float (&o)[16]) {
+    const int r = m + (lane & 31);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = n + 8 * q + 4 * (lane >> 5);
+      const float v[4] = {o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
+      half4 h[2];
+      split4(v, h[0], h[1]);
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) {
+        *reinterpret_cast<half4*>(g_at(pl, c >> 3, r) + (c & 7) * 2) = h[pl];
+        if (m != n) *reinterpret_cast<half4*>(g_at(pl, r >> 3, c + (r & 3)) + (r & 4) * 2) = transpose4(h[pl]);
+      }
+    }
+  };
+  if constexpr (MODE != kSmallFirst) {
+    float p_of[16];
+    const float gram = p.gram * p.lift[b] * p.lift[b];
+    if (mine) {
+      f32x4 s[4] = {};
+      const f32x4* at = reinterpret_cast<const f32x4*>(p.from) + (int64_t(b) * nw * NF + wave) * 256 + lane;
+#pragma unroll 4
+      for (int w = 0; w < nw; ++w) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[q] += at[int64_t(w) * NF * 256 + q * 64];
+      }
+      float o[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[e] = s[e >> 2][e & 3] * gram;
+      store_g(32 * fr, 32 * fc, o);
+    }
+    __syncthreads();
+    if (mine) {
+      f32x16 acc = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < SP / 16; ++ks) {
+        half8 fa[2], fb[2];
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl) {
+          fa[pl] = *reinterpret_cast<const half8*>(g_at(pl, 2 * ks + (lane >> 5), 32 * fr + (lane & 31)));
+          fb[pl] = *reinterpret_cast<const half8*>(g_at(pl, 2 * ks + (lane >> 5), 32 * fc + (lane & 31)));
+        }
+        mul(acc, fb, fa);
+      }
+      const int r = 32 * fr + (lane & 31);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * fc + 8 * q + 4 * (lane >> 5);
+        const half4 h = *reinterpret_cast<const half4*>(g_at(0, c >> 3, r) + (c & 7) * 2);
+        const half4 l = *reinterpret_cast<const half4*>(g_at(1, c >> 3, r) + (c & 7) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          p_of[4 * q + e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(h[e]) + float(l[e])) * p.unit) + p.alpha * acc[4 * q + e];
+      }
+    }
+    __syncthreads();
+    if (mine) store_g(32 * fr, 32 * fc, p_of);
+  }
+  const int64_t plane = p.g.x_plane();
+  _Float16* const x = p.x + b * 2 * plane;
+  const int blocks = p.g.lp / 64, first = j * blocks / nw, end = (j + 1) * blocks / nw;
+  double inv = 0;
+  if constexpr (MODE == kSmallFirst) {
+    int up2;
+    inv = scale_of(p.norms + b * kNormParts, p.nparts, p.eps, p.growth, p.scale, up2);
+    if (j == 0 && tid == 0) p.lift[b] = float(ldexp(1.0, -up2));
+  }
+  f32x16 acc = 0.f;  // this wave's part of the next G
+  half8 held[ITEMS][2];
+  const auto fetch = [&](int cb) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int item = tid + 256 * i, row = item % SP, kg = item / SP;
+      const _Float16* const at = x + (int64_t(cb * 8 + kg) * SP + row) * 8;
+      held[i][0] = *reinterpret_cast<const half8*>(at);
+      held[i][1] = *reinterpret_cast<const half8*>(at + plane);
+    }
+  };
+  if (MODE != kSmallFirst && first < end) fetch(first);
+  for (int cb = first; cb < end; ++cb) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int item = tid + 256 * i, row = item % SP, kg = item / SP;
+      if constexpr (MODE == kSmallFirst) {
+        float v[8];
+        take_u(p.tab, p.up, p.g, b, row, cb * 64 + kg * 8, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float f = float(double(v[e]) * inv);
+          held[i][0][e] = _Float16(f);
+          held[i][1][e] = _Float16(f - float(held[i][0][e]));
+        }
+        _Float16* const at = x + (int64_t(cb * 8 + kg) * SP + row) * 8;
+        *reinterpret_cast<half8*>(at) = held[i][0];
+        *reinterpret_cast<half8*>(at + plane) = held[i][1];
+      }
+#pragma unroll
+      for (int pl = 0; pl < 2; ++pl) *reinterpret_cast<half8*>(x_at(pl, kg, row)) = held[i][pl];
+    }
+    __syncthreads();
+    if constexpr (MODE != kSmallFirst) {
+      if (cb + 1 < end) fetch(cb + 1);
+      half4 moved[4][2];
+      const int m = wave / 2 * 32, n = wave % 2 * 32;
+      {
+        f32x16 v = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < SP / 16; ++ks) {
+          half8 fa[2], fb[2];
+          const int c = lane & 15, kg = n / 8 + ((lane & 16) >> 3) + ((c & 3) >> 1);
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) {
+            fa[pl] = *reinterpret_cast<const half8*>(g_at(pl, 2 * ks + (lane >> 5), m + (lane & 31)));
+            s16x4 q[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              q[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) s16x4*)(x_at(pl, kg, 16 * ks + 8 * (lane >> 5) + (c >> 2) + 4 * h) + 8 * (c & 1)));
+            fb[pl] = __builtin_bit_cast(half8, __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7));
+          }
+          mul(v, fb, fa);
+        }
+        const int r = m + (lane & 31);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = n + 8 * q + 4 * (lane >> 5);
+          if constexpr (MODE == kSmallLast) {
+            const float alpha = p.move * p.lift[b];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = cb * 64 + c + e;
+              if (r >= p.g.s || col >= p.g.l) continue;
+              float* const at = p.tab.out[b] + (p.g.turned ? int64_t(col) * p.g.cols + r : int64_t(r) * p.g.cols + col);
+              const float f = v[4 * q + e] * alpha;
+              *at = p.up.muon ? *at * p.decay - p.step * f : f;
+            }
+          } else {
+            const half4 h = *reinterpret_cast<const half4*>(x_at(0, c >> 3, r) + (c & 7) * 2);
+            const half4 l = *reinterpret_cast<const half4*>(x_at(1, c >> 3, r) + (c & 7) * 2);
+            float o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = p.move * v[4 * q + e] + p.keep * (float(h[e]) + float(l[e]));
+            split4(o, moved[q][0], moved[q][1]);
+          }
+        }
+      }
+      if constexpr (MODE == kSmallNext) {
+        __syncthreads();
+        const int r = m + (lane & 31);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = n + 8 * q + 4 * (lane >> 5);
+          _Float16* const at = x + (int64_t(cb * 8 + (c >> 3)) * SP + r) * 8 + (c & 7);
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) {
+            *reinterpret_cast<half4*>(x_at(pl, c >> 3, r) + (c & 7) * 2) = moved[q][pl];
+            *reinterpret_cast<half4*>(at + pl * plane) = moved[q][pl];
+          }
+        }
+        __syncthreads();
+      }
+    }
+    if constexpr (MODE != kSmallLast) {
+      if (mine) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          half8 fa[2], fb[2];
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) {
+            fa[pl] = *reinterpret_cast<const half8*>(x_at(pl, 2 * ks + (lane >> 5), 32 * fr + (lane & 31)));
+            fb[pl] = *reinterpret_cast<const half8*>(x_at(pl, 2 * ks + (lane >> 5), 32 * fc + (lane & 31)));
+          }
+          mul(acc, fb, fa);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (MODE != kSmallLast) {
+    if (mine) {
+      f32x4* const at = reinterpret_cast<f32x4*>(p.to) + ((int64_t(b) * nw + j) * NF + wave) * 256 + lane;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) at[q * 64] = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    }
+  }
+}
+
 template <class T, int KIND>
 int launch(const StepArgs& p, int tiles, hipStream_t s) {
   const int rest = tiles - p.share.whole;
@@ -370,14 +621,34 @@ struct Plan {
   int sym, next;  // indexes into kTiles
   Deal gram, poly, update;
   int64_t sums;   // bytes of partial sums
+  int wide;       // one launch a step, this many workgroups a matrix; 0: by products
 };
+
+// Sets of one launch a step, microseconds by products / so: one 32 x 32 61 / 35,
+// one 64 x 100 61 / 39, one 64 x 4096 97 / 85, sixteen 64 x 4096 132 / 112, forty
+// 64 x 2048 142 / 156.  (128 rows in one workgroup's LDS the same way: one 100 x
+// 128 68 / 84, one 128 x 4096 103 / 291.)
+bool use_small(int64_t s, int64_t l, int64_t batch) { return s <= kSmall && l * batch <= 65536; }
 
 Plan plan_set(int64_t rows, int64_t cols, int64_t batch) {
   Plan best{};
   double least = -1;
   const int64_t cu = cu_count(), s = std::min(rows, cols), l = std::max(rows, cols);
-  for (int i = 0; i < 3; ++i)
-    for (int j = 0; j < 3; ++j) {
+  if (use_small(s, l, batch)) {
+    Geometry& g = best.g;
+    g.rows = int(rows);
+    g.cols = int(cols);
+    g.turned = rows > cols;
+    g.s = int(s);
+    g.l = int(l);
+    g.sp = kSmall;
+    g.lp = int(up(l, 64));
+    best.wide = std::min(g.lp / 64, kSmallWide);
+    best.sums = 2 * batch * best.wide * 3 * 4096;  // of two launches, three fragments a workgroup
+    return best;
+  }
+  for (int i = 0; i < kTileCount; ++i)
+    for (int j = 0; j < kTileCount; ++j) {
       const TileCost &a = kTiles[i], &c = kTiles[j];
       const int pad = std::max(a.tile, c.tile);
       const int64_t sp = up(s, pad), lp = up(l, pad), n = sp / a.tile;
@@ -407,6 +678,7 @@ Plan plan_set(int64_t rows, int64_t cols, int64_t batch) {
 // partial sums.
 int64_t head_bytes(int64_t batch) { return up(batch * (kNormParts * 8 + 4), 256); }
 int64_t set_bytes(const Plan& p, int64_t batch) {
+  if (p.wide) return batch * p.g.x_plane() * 4 + head_bytes(batch) + p.sums;
   return batch * (2 * p.g.x_plane() * 4 + 2 * p.g.g_plane() * 4) + head_bytes(batch) + p.sums;
 }
 
@@ -557,6 +829,48 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
     MX_HIP(hipGetLastError());
     return MX_OK;
   }
+  if (plan.wide) {
+    SmallArgs a{};
+    a.tab = tab;
+    a.up = fin.up;
+    a.g = g;
+    a.norms = parts;
+    a.nparts = nparts;
+    a.eps = ns.eps;
+    a.growth = sc[0].growth;
+    a.scale = sc[0].x;
+    a.lift = lift;
+    a.x = x;
+    a.decay = decay;
+    a.step = step;
+    a.to = reinterpret_cast<float*>(x + batch * 2 * g.x_plane());
+    a.from = a.to + plan.sums / 8;
+    const auto run = [&](int mode) -> int {
+      const dim3 grid(unsigned(plan.wide), unsigned(batch)), block(256);
+      if (mode == kSmallFirst) hipLaunchKernelGGL(small_kernel<kSmallFirst>, grid, block, 0, s, a);
+      if (mode == kSmallNext) hipLaunchKernelGGL(small_kernel<kSmallNext>, grid, block, 0, s, a);
+      if (mode == kSmallLast) hipLaunchKernelGGL(small_kernel<kSmallLast>, grid, block, 0, s, a);
+      MX_HIP(hipGetLastError());
+      float* const was = a.to;
+      a.to = const_cast<float*>(a.from);
+      a.from = was;
+      return MX_OK;
+    };
+    MX_TRY(run(kSmallFirst));
+    for (int64_t i = 0; i < ns.steps; ++i) {
+      const Scales c = sc[size_t(i)];
+      const bool last = i + 1 == ns.steps;
+      a.gram = c.g / c.x / c.x;
+      a.alpha = float(ns.c) * (c.p / c.g / c.g);
+      a.diag = last ? float(ns.a) * c.p : 0.f;
+      a.lin = float(ns.b) * c.p;
+      a.unit = 1.f / c.g;
+      a.move = (last ? 1.f : sc[size_t(i) + 1].x) / c.p / c.x;
+      a.keep = last ? 0.f : float(ns.a) * (sc[size_t(i) + 1].x / c.x);
+      MX_TRY(run(last ? kSmallLast : kSmallNext));
+    }
+    return MX_OK;
+  }
   hipLaunchKernelGGL(pack_kernel, dim3(unsigned(g.lp / 64), unsigned(g.sp / 32), unsigned(batch)), dim3(256), 0, s, tab,
                      fin.up, g, parts, nparts, ns.eps, sc[0].x, sc[0].growth, x, lift);
   MX_HIP(hipGetLastError());
@@ -575,8 +889,9 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
     p.share.parts = d.parts;
     p.tiles_m = g.sp / tile;
     p.tiles_n = (symmetric(kind) ? g.sp : g.lp) / tile;
-    if (t == 0) return launch_kind<Tile64>(kind, p, int(d.tiles), s);
-    if (t == 1) return launch_kind<Tile128>(kind, p, int(d.tiles), s);
+    if (t == kTile64Deep) return launch_kind<Tile64Deep>(kind, p, int(d.tiles), s);
+    if (t == kTile64) return launch_kind<Tile64>(kind, p, int(d.tiles), s);
+    if (t == kTile128) return launch_kind<Tile128>(kind, p, int(d.tiles), s);
     return launch_kind<Tile256>(kind, p, int(d.tiles), s);
   };
   for (int64_t i = 0; i < ns.steps; ++i) {

@@ -35,8 +35,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBK = 16;     // columns of a slab: one step of the matrix instruction
-constexpr int kStages = 4;  // slabs in LDS
+constexpr int kBK = 16;  // columns of a slab: one step of the matrix instruction
 
 // Planes of a matrix: hi at `at`, lo `plane` elements behind.
 struct Planes {
@@ -53,13 +52,15 @@ __device__ __forceinline__ void split4(const float (&v)[4], half4& hi, half4& lo
   }
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int OCC_>
+// STAGES: slabs in LDS, four or eight.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int OCC_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, OCC = OCC_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, OCC = OCC_;
   static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
   static constexpr int A_BYTES = 2 * BM * kBK * 2, B_BYTES = 2 * BN * kBK * 2, STAGE = A_BYTES + B_BYTES;
-  static constexpr int SMEM = kStages * STAGE;
+  static constexpr int SMEM = STAGES * STAGE;
+  static constexpr int BASES = (SMEM + 65535) / 65536, PER_BASE = STAGES / BASES;  // LDS addresses, slabs that one reaches
   static constexpr int LA = A_BYTES / 1024 / WAVES, LB = B_BYTES / 1024 / WAVES;  // wave-wide loads of a slab
   static constexpr bool DUAL = FM * FN <= 4;  // hi lo and lo hi in accumulators of their own
   static_assert(LA * WAVES * 1024 == A_BYTES && LB * WAVES * 1024 == B_BYTES, "whole loads");
@@ -197,25 +198,25 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
     ob.load(lds + stage * T::STAGE + T::A_BYTES, wave);
   };
   half8 fa[2][2][T::FM], fb[2][2][T::FN];  // [set][plane]
-  // LDS addresses of this lane's parts, for the lower and the upper two slabs
-  // (an instruction's own offset reaches 64 KiB).  Opaque to the compiler,
-  // which would keep an address register for every read otherwise.
-  uint32_t pa[2][OpA::PARTS], pb[2][OpB::PARTS];
+  // LDS addresses of this lane's parts, one for each 64 KiB (what an
+  // instruction's own offset reaches).  Opaque to the compiler, which would keep
+  // an address register for every read otherwise.
+  uint32_t pa[T::BASES][OpA::PARTS], pb[T::BASES][OpB::PARTS];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < T::BASES; ++half) {
 #pragma unroll
     for (int h = 0; h < OpA::PARTS; ++h) {
-      pa[half][h] = lds + half * 2 * T::STAGE + OpA::lane_offset(wm, lane, h);
+      pa[half][h] = lds + half * T::PER_BASE * T::STAGE + OpA::lane_offset(wm, lane, h);
       asm volatile("" : "+v"(pa[half][h]));
     }
 #pragma unroll
     for (int h = 0; h < OpB::PARTS; ++h) {
-      pb[half][h] = lds + half * 2 * T::STAGE + T::A_BYTES + OpB::lane_offset(wn, lane, h);
+      pb[half][h] = lds + half * T::PER_BASE * T::STAGE + T::A_BYTES + OpB::lane_offset(wn, lane, h);
       asm volatile("" : "+v"(pb[half][h]));
     }
   }
   const auto read = [&](int set, int stage) {
-    const int half = stage >> 1, off = (stage & 1) * T::STAGE;
+    const int half = stage / T::PER_BASE, off = stage % T::PER_BASE * T::STAGE;
 #pragma unroll
     for (int pl = 1; pl >= 0; --pl) {
 #pragma unroll
@@ -224,16 +225,14 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
       for (int i = 0; i < T::FM; ++i) fa[set][pl][i] = OpA::frag(pa[half], off, pl, i);
     }
   };
-  constexpr int NL = T::LA + T::LB;
-  // One slab, its number's last two bits u, WAIT of this wave's loads left in
-  // flight: then slab t + 1 has landed for every wave, and every wave has long
-  // left slab t - 1, whose stage takes slab t + 3.
-  const auto slab = [&](auto u_, auto wait_, bool more) {
+  constexpr int S = T::STAGES, NL = T::LA + T::LB;
+  // Slab t of stage u: its products, the next slab's reads among the first of
+  // them, slab t + S - 1 on its way into the stage that slab t - 1 has left.
+  const auto slab = [&](auto u_, bool more) {
     constexpr int u = decltype(u_)::value, set = u & 1;
-    wait_loads<decltype(wait_)::value>();
     barrier();
-    if (more) issue((u + 3) % kStages);
-    read(set ^ 1, (u + 1) % kStages);
+    if (more) issue((u + S - 1) % S);
+    read(set ^ 1, (u + 1) % S);
 #pragma unroll
     for (int q = 0; q < 3; ++q)  // lo hi, hi lo, hi hi
 #pragma unroll
@@ -244,7 +243,6 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
           c = ROW_LANES ? __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[set][q == 1][i], fb[set][q == 0][j], c, 0, 0, 0)
                         : __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[set][q == 0][j], fa[set][q == 1][i], c, 0, 0, 0);
         }
-    // The next slab's reads go out among the first products.
     constexpr int READS = 2 * T::FM * OpA::PARTS + 2 * T::FN * OpB::PARTS, PRODUCTS = 3 * T::FM * T::FN;
 #pragma unroll
     for (int r = 0; r < (READS < PRODUCTS ? READS : PRODUCTS); ++r) {
@@ -253,24 +251,58 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
     }
   };
   using std::integral_constant;
-  using N0 = integral_constant<int, 0>;
-  using N1 = integral_constant<int, NL>;
-  issue(0);
-  issue(1);
-  issue(2);
-  wait_loads<2 * NL>();
+  // Before slab t's barrier a wave waits until its part of slab t + 1 has landed:
+  // after the barrier everyone's has.
+#pragma unroll
+  for (int t = 0; t < S - 1; ++t)
+    if (t < 4 || t < nk) issue(t);
+  if (nk >= S)
+    wait_loads<(S - 2) * NL>();
+  else
+    wait_loads<0>();
   barrier();
   read(0, 0);
-  for (int t = kStages; t < nk; t += kStages) {
-    slab(N0{}, N1{}, true);
-    slab(integral_constant<int, 1>{}, N1{}, true);
-    slab(integral_constant<int, 2>{}, N1{}, true);
-    slab(integral_constant<int, 3>{}, N1{}, true);
+  const auto four = [&](auto u_, int t) {
+    constexpr int u = decltype(u_)::value;
+    const auto one = [&](auto v_) {
+      constexpr int v = decltype(v_)::value;
+      if (t + v + S - 1 < nk) {
+        wait_loads<(S - 3) * NL>();
+        slab(integral_constant<int, u + v>{}, true);
+      } else {
+        wait_loads<0>();
+        slab(integral_constant<int, u + v>{}, false);
+      }
+    };
+    one(integral_constant<int, 0>{});
+    one(integral_constant<int, 1>{});
+    one(integral_constant<int, 2>{});
+    one(integral_constant<int, 3>{});
+  };
+  if constexpr (S == 4) {
+    using N1 = integral_constant<int, 1>;
+    const auto all = [&](auto wait_, auto u_, bool more) {
+      wait_loads<decltype(wait_)::value>();
+      slab(u_, more);
+    };
+    using A = integral_constant<int, NL>;
+    using Z = integral_constant<int, 0>;
+    for (int t = 4; t < nk; t += 4) {
+      all(A{}, Z{}, true);
+      all(A{}, N1{}, true);
+      all(A{}, integral_constant<int, 2>{}, true);
+      all(A{}, integral_constant<int, 3>{}, true);
+    }
+    all(A{}, Z{}, true);
+    all(A{}, N1{}, false);
+    all(Z{}, integral_constant<int, 2>{}, false);
+    all(Z{}, integral_constant<int, 3>{}, false);
+  } else {
+    for (int t = 0; t < nk; t += S) {
+      four(integral_constant<int, 0>{}, t);
+      if (t + 4 < nk) four(integral_constant<int, S - 4>{}, t + 4);
+    }
   }
-  slab(N0{}, N1{}, true);
-  slab(integral_constant<int, 1>{}, N1{}, false);
-  slab(integral_constant<int, 2>{}, N0{}, false);
-  slab(integral_constant<int, 3>{}, N0{}, false);
   if constexpr (T::DUAL) {
 #pragma unroll
     for (int i = 0; i < T::FM; ++i)
@@ -359,9 +391,14 @@ __device__ __forceinline__ f32x16 join_sums(const Shares& p, int& tile, int& m, 
   return v;
 }
 
-using Tile64 = Tile<64, 64, 2, 2, 4>;     // 4 waves of 32 x 32
-using Tile128 = Tile<128, 128, 2, 2, 2>;  // 4 waves of 64 x 64
-using Tile256 = Tile<256, 256, 2, 4, 2>;  // 8 waves of 128 x 64
+// 64 x 64: 4 waves of 32 x 32.  A slab is 96 cycles of a wave's products, a load
+// some 1500: with one workgroup to a CU eight slabs in LDS shorten it (one
+// product of 1024^3 0.18 -> 0.13 us a slab), with four of them four do as well and
+// leave them room.
+using Tile64Deep = Tile<64, 64, 2, 2, 8, 2>;
+using Tile64 = Tile<64, 64, 2, 2, 4, 4>;
+using Tile128 = Tile<128, 128, 2, 2, 4, 2>;  // 4 waves of 64 x 64
+using Tile256 = Tile<256, 256, 2, 4, 4, 2>;  // 8 waves of 128 x 64
 
 // A CU's time per slab with n workgroups of a tile on it, and how many it
 // holds; microseconds, fitted to products of 16 x 1024^3 and of 4096^3.
@@ -370,7 +407,8 @@ struct TileCost {
   double fixed, each;
   double slab(double n) const { return fixed + each * n; }
 };
-constexpr TileCost kTiles[] = {{64, 4, 0.11, 0.077}, {128, 2, 0.05, 0.285}, {256, 1, 0.0, 1.15}};
+enum TileIndex { kTile64Deep, kTile64, kTile128, kTile256, kTileCount };
+constexpr TileCost kTiles[kTileCount] = {{64, 2, -0.062, 0.19}, {64, 4, 0.11, 0.077}, {128, 2, 0.05, 0.285}, {256, 1, 0.0, 1.15}};
 
 // How a product's tiles are dealt: whole rounds of the chip, then what is left
 // over in parts along K where a join (a launch and a pass over the sums) costs
@@ -389,8 +427,8 @@ inline Deal deal(const TileCost& c, int64_t tiles, int64_t nk, int64_t cu) {
   double least = double(nk) * c.slab(double((rest + cu - 1) / cu));
   for (int64_t parts = 2; parts <= 16 && parts * rest <= slots && parts * 8 <= nk; ++parts) {
     const double share = double((nk / 4 + parts - 1) / parts * 4);
-    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 4.0 +
-                         double(rest * parts) * c.tile * c.tile * 8.0 / 6e6;
+    const double split = share * c.slab(double((rest * parts + cu - 1) / cu)) + 6.0 +
+                         double(rest * parts) * c.tile * c.tile * 8.0 / 3e6;
     if (split >= least) continue;
     least = split;
     d.whole = full * slots;
