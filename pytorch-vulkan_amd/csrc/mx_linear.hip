@@ -76,6 +76,20 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
   return v;
 }
 
+// Sum over a wave, in lane 63, the same way.
+__device__ __forceinline__ float wave_sum(float v) {
+  const auto with = [&](auto ctrl) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  with(std::integral_constant<int, 0x111>{});
+  with(std::integral_constant<int, 0x112>{});
+  with(std::integral_constant<int, 0x114>{});
+  with(std::integral_constant<int, 0x118>{});
+  with(std::integral_constant<int, 0x142>{});
+  with(std::integral_constant<int, 0x143>{});
+  return v;
+}
+
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // A thread holds W columns; 64 threads lie along a row and the workgroup's four
@@ -331,6 +345,253 @@ __global__ __launch_bounds__(64) void piece_join_kernel(PieceArgs p) {
   finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, *p.ea + *p.eb - 28);
 }
 
+// A few tokens: y[m][n] for m <= M.  A workgroup takes R rows of w and splits k
+// between its four waves, lane after lane along it; a wave's partial sums meet in
+// LDS.  Every weight is read once, 16 bytes a lane and all rows of a stretch on
+// their way together, which is what bounds it (4 x 1024 -> 4096: 5.0 us, 4096 -> 16384 for one token 44 us, 6.0 TB/s);
+// x comes from L2, M / R times the weights.
+template <int M, int R>
+__global__ __launch_bounds__(256) void few_kernel(const float* x, const float* w, const float* bias, const float* residual,
+                                                  int m, int64_t k, int n, int act, float* y, float* z) {
+  static_assert(M * R <= 128, "an output to a thread at most");
+  __shared__ float sums[4][M * R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = int64_t(blockIdx.x) * R;
+  float acc[M][R] = {};
+  for (int64_t k0 = wave * 256; k0 < k; k0 += 1024) {
+    // The lane that k ends in takes its last four elements and leaves out those
+    // that its neighbour has.
+    const int64_t kk = k0 + lane * 4, at = min(kk, k - 4);
+    const int skip = kk < k ? int(kk - at) : 4;
+    f32x4 wv[R], xv[M];
+#pragma unroll
+    for (int r = 0; r < R; ++r) wv[r] = *reinterpret_cast<const f32x4u*>(w + min(n0 + r, int64_t(n - 1)) * k + at);
+#pragma unroll
+    for (int i = 0; i < M; ++i) xv[i] = *reinterpret_cast<const f32x4u*>(x + int64_t(min(i, m - 1)) * k + at);
+    if (skip) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e >= skip) continue;
+#pragma unroll
+        for (int r = 0; r < R; ++r) wv[r][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < M; ++i) xv[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[i][r] = fmaf(xv[i][e], wv[r][e], acc[i][r]);
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float s = wave_sum(acc[i][r]);
+      if (lane == 63) sums[wave][i * R + r] = s;
+    }
+  __syncthreads();
+  const int t = threadIdx.x;
+  if (t >= M * R) return;
+  const int i = t / R;
+  const int64_t col = n0 + t % R;
+  if (i >= m || col >= n) return;
+  float v = ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])) + (bias ? bias[col] : 0.f);
+  const int64_t to = int64_t(i) * n + col;
+  if (z) z[to] = v;
+  v = activate(act, v);
+  y[to] = v + (residual ? residual[to] : 0.f);
+}
+
+// ------------------------------------------------------------ small products
+// out[M][N] = sum_k a[m][k] b[n][k] for products whose time is latency: 32 x 32
+// outputs to a wave, whose lanes read their eight k of a row straight from memory
+// into registers, four steps of 16 k ahead, and split them there into three bf16
+// pieces (the arithmetic of mx_gemm.hip's tiles).  No LDS and no barrier until the
+// WK waves of a workgroup, which share K where it is long enough, join their sums
+// (WK == 1: a tile to each of its four waves).  Values past tiles' edges are read
+// twice and not stored.
+//
+// A backward's two products go in one launch, and the tiles of dw's first column
+// sum their rows of dz into db.  (With dz evaluated from dy and z as it is read,
+// every tile of a row over again, a step took three times as long.)
+struct DirectProduct {
+  const float *a, *b;
+  float *out, *row_sums;
+  int m, n, k;
+  int64_t a_stride, b_stride;  // of a row where k is contiguous, else of k
+  bool a_along;                // a's k is contiguous (b's too in a forward)
+  int tiles_n, first;          // first tile
+};
+struct DirectArgs {
+  DirectProduct p[2];
+  int count, tiles, act;
+  const float *bias, *residual;
+  float* z;
+};
+
+constexpr int kAhead = 4;
+
+// A lane's row of an operand.  ALONG: k contiguous.
+template <bool ALONG>
+struct DirectRow {
+  const float* p;
+  int64_t stride;
+  int k;
+  __device__ __forceinline__ DirectRow(const float* base, int64_t stride_, int row, int k_)
+      : p(base + (ALONG ? row * stride_ : int64_t(row))), stride(stride_), k(k_) {}
+  // Eight k from k0, zeros past K; whole: none of the wave's 16 is past it.
+  __device__ __forceinline__ void read(float (&v)[8], int k0, bool whole) const {
+    if constexpr (ALONG) {
+      if (whole) {
+        const f32x4 a = *reinterpret_cast<const f32x4u*>(p + k0), b = *reinterpret_cast<const f32x4u*>(p + k0 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = a[e];
+          v[4 + e] = b[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k0 + e < k ? p[k0 + e] : 0.f;
+      }
+    } else {
+      const float* const at = p + int64_t(k0) * stride;
+      if (whole) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = at[e * stride];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k0 + e < k ? at[e * stride] : 0.f;
+      }
+    }
+  }
+};
+
+struct DirectRegs {
+  float a[8], b[8];
+};
+
+// acc (times the returned factor) = steps [s0, s1) of a tile's product; sum: this
+// lane's part of its row of a.
+template <bool A_ALONG, bool B_ALONG>
+__device__ __forceinline__ float direct_product(const DirectProduct& p, int row, int col, int s0, int s1,
+                                                mfma::f32x16& acc, float& sum) {
+  const int lane = threadIdx.x & 63, half = 8 * (lane >> 5);
+  const DirectRow<A_ALONG> ra(p.a, p.a_stride, min(row + (lane & 31), p.m - 1), p.k);
+  const DirectRow<B_ALONG> rb(p.b, p.b_stride, min(col + (lane & 31), p.n - 1), p.k);
+  const auto load = [&](DirectRegs& g, int s) {
+    if (s >= s1) return;
+    const bool whole = 16 * s + 16 <= p.k;
+    ra.read(g.a, 16 * s + half, whole);
+    rb.read(g.b, 16 * s + half, whole);
+  };
+  DirectRegs g[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) load(g[u], s0 + u);
+  acc = 0.f;
+  sum = 0.f;
+  const auto quads = [](const float (&v)[8]) {
+    const float f = mfma::kPieceScale;
+    return mfma::split8(mfma::f32x4{v[0] * f, v[1] * f, v[2] * f, v[3] * f}, mfma::f32x4{v[4] * f, v[5] * f, v[6] * f, v[7] * f});
+  };
+  for (int s = s0; s < s1; s += kAhead) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s + u >= s1) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += g[u].a[e];
+      const mfma::Frag3 a = quads(g[u].a), b = quads(g[u].b);
+      load(g[u], s + u + kAhead);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, acc, 0, 0, 0);
+    }
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(acc[e]) << 1);
+  if (!__any(top >= 0xFF000000u)) return mfma::kProductScale;
+  // Pieces cannot hold an operand or a sum: again on the FP32 instruction.
+  acc = 0.f;
+  for (int s = s0; s < s1; ++s) {
+    load(g[0], s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(g[0].a[e], g[0].b[e], acc, 0, 0, 0);
+  }
+  return 1.f;
+}
+
+template <bool FORWARD, int WK>
+__global__ __launch_bounds__(WK > 1 ? 64 * WK : 256) void direct_kernel(DirectArgs d) {
+  __shared__ float sums[WK > 1 ? WK * 1024 : 1], rows[WK > 1 ? WK * 32 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tile = WK > 1 ? int(blockIdx.x) : int(blockIdx.x) * 4 + wave;
+  if (tile >= d.tiles) return;  // whole workgroups where waves meet at barriers
+  const DirectProduct& p = d.p[!FORWARD && d.count > 1 && tile >= d.p[1].first ? 1 : 0];
+  tile -= p.first;
+  const int row = tile / p.tiles_n * 32, col = tile % p.tiles_n * 32;
+  const int steps = (p.k + 15) / 16, s0 = WK > 1 ? wave * steps / WK : 0, s1 = WK > 1 ? (wave + 1) * steps / WK : steps;
+  mfma::f32x16 acc;
+  float sum, scale;
+  if constexpr (FORWARD)
+    scale = direct_product<true, true>(p, row, col, s0, s1, acc, sum);
+  else if (p.a_along)
+    scale = direct_product<true, false>(p, row, col, s0, s1, acc, sum);
+  else
+    scale = direct_product<false, false>(p, row, col, s0, s1, acc, sum);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] *= scale;
+  // Both halves of a wave hold half of a row's k.
+  const bool want_rows = !FORWARD && p.row_sums && col == 0;
+  if (want_rows) sum += __shfl_xor(sum, 32, 64);
+  constexpr int MINE = WK > 1 ? 16 / WK : 16;  // this wave's registers of the joined tile
+  float v[MINE];
+  const int e0 = WK > 1 ? MINE * wave : 0;
+  if constexpr (WK > 1) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[(wave * 16 + e) * 64 + lane] = acc[e];
+    if (want_rows && lane < 32) rows[wave * 32 + lane] = sum;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+      const float* const at = sums + (e0 + q) * 64 + lane;
+      v[q] = at[0];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) v[q] += at[w * 1024];
+    }
+    if (want_rows && wave == 0 && lane < 32) {
+      sum = rows[lane];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) sum += rows[w * 32 + lane];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = acc[e];
+  }
+  if (want_rows && (WK == 1 || wave == 0) && lane < 32 && row + lane < p.m) p.row_sums[row + lane] = sum;
+  const int c = col + (lane & 31);
+  if (c >= p.n || !p.out) return;
+  const float bias = FORWARD && d.bias ? d.bias[c] : 0.f;
+#pragma unroll
+  for (int q = 0; q < MINE; ++q) {
+    const int e = e0 + q, r = row + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+    if (r >= p.m) continue;
+    const int64_t to = int64_t(r) * p.n + c;
+    float o = v[q];
+    if constexpr (FORWARD) {
+      o += bias;
+      if (d.z) d.z[to] = o;
+      o = activate(d.act, o) + (d.residual ? d.residual[to] : 0.f);
+    }
+    p.out[to] = o;
+  }
+}
+
 // out[c] = sum of part[p][c] in the order of p: 32 columns and 32 groups of
 // partials to a workgroup.
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, int parts, int n, float* out) {
@@ -577,14 +838,97 @@ struct Forward {
   }
 };
 
+// Whether products go as small ones: where their time is below that of
+// mx_gemm.hip's tiles, both as fitted to measurements (microseconds, tiles /
+// small, with GELU):
+//   m x k -> n           forward       backward
+//   17 x 512 -> 512      14.5 /  6.6   24.7 / 11.2
+//   90 x 512 -> 512      15.4 /  7.3   26.7 / 12.2
+//   256 x 256 -> 256     10.5 /  5.3   23.9 / 10.2
+//   512 x 512 -> 512     16.0 /  7.7   36.1 / 16.4
+//   300 x 500 -> 700     16.0 /  7.2   29.8 / 16.9
+//   128 x 1024 -> 1024   12.5 / 11.5   25.8 / 17.5
+//   8192 x 64 -> 64       7.3 /  5.1   27.5 / 70.9
+//   64 x 4096 -> 1024    15.3 / 32.0   31.2 / 29.4
+//   64 x 4096 -> 4096    26.6 / 33.2   57.3 / 78.0
+// A step of 16 k takes four waves 0.45 us, a CU one workgroup's at a time.
+bool use_direct(int64_t m, int64_t k, int64_t n, bool backward) {
+  const auto up = [](int64_t v, int64_t to) { return double((v + to - 1) / to); };
+  const double gflop = 2e-9 * double(m) * double(k) * double(n), cu = cu_count();
+  if (!backward) {
+    const double steps = up(k, 16);
+    return 4.0 + 0.11 * steps * std::max(1.0, up(m, 32) * up(n, 32) / cu) < std::min(5.0 + 0.34 * steps, 12.0) + 6.7 * gflop;
+  }
+  const double work = up(m, 32) * up(k, 32) * up(n, 64) + up(n, 32) * up(k, 32) * up(m, 64);
+  return 8.5 + 0.48 * std::max(up(std::max(m, n), 64), work / cu) < 22.0 + 26.0 * gflop;
+}
+
+// Waves that share a tile's K, each with a step of it: eight for a forward's few
+// tiles; four for a backward (of the layer's longer product, whichever gradients
+// are asked for: their sums do not depend on it), most of whose tiles have short K.
+int direct_waves(int64_t m, int64_t k, int64_t n, bool backward) {
+  const int64_t steps = ((backward ? std::max(m, n) : k) + 15) / 16;
+  return steps >= 8 && !backward ? 8 : steps >= 4 ? 4 : 1;
+}
+
+DirectProduct direct_product_of(const float* a, const float* b, float* out, int64_t m, int64_t n, int64_t k,
+                                int64_t a_stride, int64_t b_stride, bool a_along) {
+  DirectProduct p{};
+  p.a = a;
+  p.b = b;
+  p.out = out;
+  p.m = int(m);
+  p.n = int(n);
+  p.k = int(k);
+  p.a_stride = a_stride;
+  p.b_stride = b_stride;
+  p.a_along = a_along;
+  p.tiles_n = int((n + 31) / 32);
+  return p;
+}
+
+template <bool FORWARD>
+int run_direct(DirectArgs* d, int wk, hipStream_t s) {
+  d->tiles = 0;
+  for (int i = 0; i < d->count; ++i) {
+    d->p[i].first = d->tiles;
+    d->tiles += (d->p[i].m + 31) / 32 * d->p[i].tiles_n;
+  }
+  const dim3 grid(unsigned(wk == 1 ? (d->tiles + 3) / 4 : d->tiles)), block(unsigned(wk == 1 ? 256 : 64 * wk));
+  if (wk == 8)
+    hipLaunchKernelGGL((direct_kernel<FORWARD, 8>), grid, block, 0, s, *d);
+  else if (wk == 4)
+    hipLaunchKernelGGL((direct_kernel<FORWARD, 4>), grid, block, 0, s, *d);
+  else
+    hipLaunchKernelGGL((direct_kernel<FORWARD, 1>), grid, block, 0, s, *d);
+  MX_HIP(hipGetLastError());
+  return MX_OK;
+}
+
+// Tokens that few_kernel takes.
+constexpr int64_t kFew = 16;
+bool use_few(int64_t m, int64_t k) { return m <= kFew && k >= 4; }
+
+template <int M, int R>
+int run_few(const float* x, const float* w, const float* bias, const float* residual, int64_t m, int64_t k, int64_t n, int act,
+            float* y, float* z, hipStream_t s) {
+  hipLaunchKernelGGL((few_kernel<M, R>), dim3(unsigned((n + R - 1) / R)), dim3(256), 0, s, x, w, bias, residual, int(m), k,
+                     int(n), act, y, z);
+  MX_HIP(hipGetLastError());
+  return MX_OK;
+}
+
 int forward_bytes(int64_t m, int64_t k, int64_t n, int64_t* bytes) {
   *bytes = 0;
-  if (m == 0 || n == 0 || k == 0) return MX_OK;
+  if (m == 0 || n == 0 || k == 0 || use_few(m, k) || use_direct(m, k, n, false)) return MX_OK;
   Carve c(nullptr);
   const Forward f(m, k, n, &c);
   *bytes = c.used;
   return f.packed ? MX_OK : partials(forward_desc(m, k, n, true), bytes);
 }
+
+// Workspace of small products' backward.
+float* small_dz(int64_t m, int64_t n, bool slope, Carve* c) { return slope ? c->take<float>(m * n) : nullptr; }
 
 // Workspace of a backward.
 struct Backward {
@@ -632,6 +976,11 @@ extern "C" int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activati
   if (m == 0 || n == 0) return MX_OK;
   if (!backward) return forward_bytes(m, k, n, bytes);
   Carve c(nullptr);
+  if (k > 0 && use_direct(m, k, n, true)) {
+    (void)small_dz(m, n, activation != MX_ACT_NONE, &c);
+    *bytes = c.used;
+    return MX_OK;
+  }
   const Backward b(m, k, n, activation != MX_ACT_NONE, k > 0, k > 0, true, true, &c);
   *bytes = c.used;
   return b.status;
@@ -647,6 +996,27 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   if (m == 0 || n == 0) return MX_OK;
   MX_REQUIRE(y && (k == 0 || (x && w)), MX_ERR_INVALID, who, ": null buffer");
   hipStream_t s = resolve_stream(stream);
+  if (use_few(m, k)) {
+    const auto run = [&](auto mm, auto r) {
+      return run_few<decltype(mm)::value, decltype(r)::value>(x, w, bias, residual, m, k, n, activation, y, z, s);
+    };
+    using std::integral_constant;
+    if (m == 1) return run(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    if (m == 2) return run(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    if (m <= 4) return run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    if (m <= 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    return run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  }
+  if (k > 0 && use_direct(m, k, n, false)) {
+    DirectArgs a{};
+    a.count = 1;
+    a.act = activation;
+    a.bias = bias;
+    a.residual = residual;
+    a.z = z;
+    a.p[0] = direct_product_of(x, w, y, m, n, k, k, k, true);
+    return run_direct<true>(&a, direct_waves(m, k, n, false), s);
+  }
   const mx_gemm_desc d = forward_desc(m, k, n, bias != nullptr);
   const GemmEpilogue epi{activation, residual, z};
   int64_t need = 0;
@@ -705,6 +1075,40 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   MX_REQUIRE(dy && (!slope || z) && (k == 0 || ((!dx || w) && (!dw || x))), MX_ERR_INVALID, who, ": null buffer");
   if (k == 0) dx = dw = nullptr;
   if (!dx && !dw && !db) return MX_OK;
+  if (k > 0 && use_direct(m, k, n, true)) {
+    Carve size(nullptr);
+    (void)small_dz(m, n, slope, &size);
+    Workspace ws;
+    MX_TRY(ws.take(who, workspace, workspace_bytes, size.used, s));
+    Carve c(ws.as<void>());
+    const float* g = dy;
+    if (slope) {
+      float* const dz = small_dz(m, n, slope, &c);
+      const ScanPlan sp = plan_scan(m, n);
+      ScanArgs scan{};
+      scan.act = activation;
+      scan.count = 1;
+      ScanOp& o = scan.op[0];
+      o.src = dy;
+      o.z = z;
+      o.dz = dz;
+      o.m = m;
+      o.n = int(n);
+      o.rows_per = sp.rows_per;
+      o.col_blocks = sp.col_blocks;
+      o.parts = sp.parts;
+      MX_TRY(run_scan<false>(&scan, s));
+      g = dz;
+    }
+    DirectArgs a{};
+    if (dx) a.p[a.count++] = direct_product_of(g, w, dx, m, k, n, n, k, true);
+    if (dw || db) {  // db alone: the first column of dw's tiles, not stored
+      DirectProduct& p = a.p[a.count++];
+      p = direct_product_of(g, dw ? x : g, dw, n, dw ? k : 1, m, n, dw ? k : 0, false);
+      p.row_sums = db;
+    }
+    return run_direct<false>(&a, direct_waves(m, k, n, true), s);
+  }
   // Without the caller's workspace the K splits of products that are not packed
   // are left to them (captured calls take one pass each).
   Carve size(nullptr);
