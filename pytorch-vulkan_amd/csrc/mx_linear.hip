@@ -192,10 +192,32 @@ struct PackArgs {
   PackOp op[3];
   int count;
   int* bad;
+  // Column sums of the first pass, by workgroups from first_sum on: out[c] = sum of
+  // part[p][c] in the order of p, 32 columns and 8 groups of partials to each.
+  const float* part;
+  int parts, n, first_sum;
+  float* out;
 };
 
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   __shared__ uint32_t tops[4], col_tops[256];
+  if (int(blockIdx.x) >= p.first_sum) {
+    __shared__ float sums[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int(blockIdx.x) - p.first_sum) * 32 + tx;
+    float s = 0.f;
+    if (c < p.n) {
+#pragma unroll 16
+      for (int i = ty; i < p.parts; i += 8) s += p.part[int64_t(i) * p.n + c];
+    }
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && c < p.n) {
+#pragma unroll
+      for (int g = 1; g < 8; ++g) s += sums[g][tx];
+      p.out[c] = s;
+    }
+    return;
+  }
   int k = 0;
   while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
   const PackOp& o = p.op[k];
@@ -315,11 +337,17 @@ __device__ __forceinline__ void finish_piece(const PieceArgs& p, int m, int n, c
     store_piece<EPI, false>(p, m, n, acc, up);
 }
 
+// Both products of a backward go in one launch: 256 tiles of each leave room for
+// the other's on every CU.
+struct PieceLaunch {
+  PieceArgs p[2];
+  int second;  // first workgroup of p[1]
+};
+
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
-__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void piece_kernel(PieceArgs p) {
-  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
+__device__ __forceinline__ void piece_tile(const PieceArgs& p, int id, char* smem) {
   if (*p.bad) return;
-  const pieces::Unit unit = pieces::unit_of(p.share, blockIdx.x, p.nk);
+  const pieces::Unit unit = pieces::unit_of(p.share, id, p.nk);
   int tm, tn;
   mfma::tile_coords(unit.tile, p.tiles_m, p.tiles_n, tm, tn);
   pieces::f32x16 acc[T::FM][T::FN];
@@ -336,11 +364,29 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
     for (int j = 0; j < T::FN; ++j) finish_piece<EPI>(p, m0 + 32 * i, n0 + 32 * j, acc[i][j], up);
 }
 
+template <class T>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void piece_forward_kernel(PieceArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
+  piece_tile<T, false, false, true>(p, blockIdx.x, smem);
+}
+
+// p[0]: dx = dz w, p[1]: dw = dz^T x.
+template <class T>
+__global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void piece_backward_kernel(PieceLaunch l) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
+  if (int(blockIdx.x) < l.second)
+    piece_tile<T, false, true, false>(l.p[0], blockIdx.x, smem);
+  else
+    piece_tile<T, true, true, false>(l.p[1], int(blockIdx.x) - l.second, smem);
+}
+
 template <class T, bool EPI>
-__global__ __launch_bounds__(64) void piece_join_kernel(PieceArgs p) {
+__global__ __launch_bounds__(64) void piece_join_kernel(PieceLaunch l) {
+  const bool second = int(blockIdx.x) >= l.second;
+  const PieceArgs& p = l.p[second ? 1 : 0];
   if (*p.bad) return;
   int tile, m, n, tm, tn;
-  const pieces::f32x16 v = pieces::join_sums<T>(p.share, tile, m, n);
+  const pieces::f32x16 v = pieces::join_sums<T>(p.share, int(blockIdx.x) - (second ? l.second : 0), tile, m, n);
   mfma::tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn);
   finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, *p.ea + *p.eb - 28);
 }
@@ -701,8 +747,11 @@ struct Carve {
 using PieceTile = pieces::Tile128;
 constexpr int kPad = PieceTile::BM;
 int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
-pieces::Deal plan_piece(int64_t m, int64_t n, int64_t k) {
-  return pieces::deal(pieces::kTiles[pieces::kTile128], padded(m) / kPad * (padded(n) / kPad), padded(k) / pieces::kBK, cu_count());
+double piece_work(int64_t m, int64_t n, int64_t k) { return double(padded(m) / kPad * (padded(n) / kPad)) * double(padded(k)); }
+// share: the part of the chip that the product has, the rest beside it another's.
+pieces::Deal plan_piece(int64_t m, int64_t n, int64_t k, double share) {
+  return pieces::deal(pieces::kTiles[pieces::kTile128], padded(m) / kPad * (padded(n) / kPad), padded(k) / pieces::kBK,
+                      std::max<int64_t>(1, int64_t(double(cu_count()) * share)));
 }
 
 // An operand [m][n] of packed products: what its passes write.
@@ -766,31 +815,50 @@ bool use_packed(int64_t m, int64_t k, int64_t n, bool backward) {
   return saved > passes;
 }
 
-// out [m][n] over k: operands a (its rows, or A_COLS columns, are m) and b.
-template <bool A_COLS, bool B_COLS, bool EPI>
-int run_piece(PieceArgs p, const pieces::Deal& d, const Packed& a, const Packed& b, const int* bad, float* sums,
-              hipStream_t s) {
+// out [m][n] over k: operands a (its rows, or where a_cols its columns, are m) and
+// b, dealt as d.
+void fill_piece(PieceArgs* p, const pieces::Deal& d, const Packed& a, bool a_cols, const Packed& b, bool b_cols,
+                const int* bad, float* sums) {
+  p->a = a.second.to;
+  p->b = b.second.to;
+  p->ea = a.second.exponent;
+  p->eb = b.second.exponent;
+  p->bad = bad;
+  p->m = int(a_cols ? a.n : a.m);
+  p->n = int(b_cols ? b.n : b.m);
+  p->nk = int(padded(a_cols ? a.m : a.n) / pieces::kBK);
+  p->tiles_m = int(padded(p->m) / kPad);
+  p->tiles_n = int(padded(p->n) / kPad);
+  p->share = {int(d.whole), d.parts, sums};
+}
+int piece_blocks(const PieceArgs& p) {
+  return p.share.whole + (p.tiles_m * p.tiles_n - p.share.whole) * p.share.parts;
+}
+template <bool EPI>
+int run_joins(PieceLaunch l, hipStream_t s) {
   using T = PieceTile;
-  p.a = a.second.to;
-  p.b = b.second.to;
-  p.ea = a.second.exponent;
-  p.eb = b.second.exponent;
-  p.bad = bad;
-  p.m = int(A_COLS ? a.n : a.m);
-  p.n = int(B_COLS ? b.n : b.m);
-  p.nk = int(padded(A_COLS ? a.m : a.n) / pieces::kBK);
-  p.tiles_m = int(padded(p.m) / kPad);
-  p.tiles_n = int(padded(p.n) / kPad);
-  p.share = {int(d.whole), d.parts, sums};
-  const int rest = int(d.tiles - d.whole);
-  hipLaunchKernelGGL((piece_kernel<T, A_COLS, B_COLS, EPI>), dim3(unsigned(p.share.whole + rest * p.share.parts)),
-                     dim3(T::THREADS), 0, s, p);
+  constexpr int PER = T::WAVES * T::FM * T::FN;
+  l.second = (l.p[0].tiles_m * l.p[0].tiles_n - l.p[0].share.whole) * PER;
+  const int blocks = l.second + (l.p[1].tiles_m * l.p[1].tiles_n - l.p[1].share.whole) * PER;
+  if (!blocks) return MX_OK;
+  hipLaunchKernelGGL((piece_join_kernel<T, EPI>), dim3(unsigned(blocks)), dim3(64), 0, s, l);
   MX_HIP(hipGetLastError());
-  if (rest) {
-    hipLaunchKernelGGL((piece_join_kernel<T, EPI>), dim3(unsigned(rest * T::WAVES * T::FM * T::FN)), dim3(64), 0, s, p);
-    MX_HIP(hipGetLastError());
-  }
   return MX_OK;
+}
+int run_forward(const PieceArgs& p, hipStream_t s) {
+  using T = PieceTile;
+  hipLaunchKernelGGL(piece_forward_kernel<T>, dim3(unsigned(piece_blocks(p))), dim3(T::THREADS), 0, s, p);
+  MX_HIP(hipGetLastError());
+  PieceLaunch l{};
+  l.p[0] = p;
+  return run_joins<true>(l, s);
+}
+int run_backward(PieceLaunch l, hipStream_t s) {
+  using T = PieceTile;
+  l.second = piece_blocks(l.p[0]);
+  hipLaunchKernelGGL(piece_backward_kernel<T>, dim3(unsigned(l.second + piece_blocks(l.p[1]))), dim3(T::THREADS), 0, s, l);
+  MX_HIP(hipGetLastError());
+  return run_joins<false>(l, s);
 }
 
 // First and second pass of a call's operands.
@@ -814,6 +882,8 @@ int run_pack(PackArgs* p, hipStream_t s) {
     p->op[i].first = blocks;
     blocks += p->op[i].wide * (p->op[i].to.rows / 32);
   }
+  p->first_sum = blocks;
+  if (p->out) blocks += (p->n + 31) / 32;
   hipLaunchKernelGGL(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, *p);
   MX_HIP(hipGetLastError());
   return MX_OK;
@@ -833,7 +903,7 @@ struct Forward {
     head = c->take<int>(8);
     x = mx::packed(m, k, 1, c);
     w = mx::packed(n, k, 1, c);
-    deal = plan_piece(m, n, k);
+    deal = plan_piece(m, n, k, 1.0);
     sums = c->take<float>(deal.sum_bytes(kPad) / 4);
   }
 };
@@ -934,7 +1004,7 @@ float* small_dz(int64_t m, int64_t n, bool slope, Carve* c) { return slope ? c->
 struct Backward {
   bool packed;
   ScanPlan scan;  // of dz
-  float *dz = nullptr, *part = nullptr, *sums = nullptr;
+  float *dz = nullptr, *part = nullptr, *sums_x = nullptr, *sums_w = nullptr;
   int* head = nullptr;
   Packed g, x, w;
   pieces::Deal to_x{}, to_w{};
@@ -950,9 +1020,12 @@ struct Backward {
       g = mx::packed(m, n, (want_x ? 1 : 0) | (want_w ? 2 : 0), c);
       if (want_w) x = mx::packed(m, k, 2, c);
       if (want_x) w = mx::packed(n, k, 1, c);
-      to_x = plan_piece(m, k, n);
-      to_w = plan_piece(n, k, m);
-      sums = c->take<float>(std::max(want_x ? to_x.sum_bytes(kPad) : 0, want_w ? to_w.sum_bytes(kPad) : 0) / 4);
+      // Dealt as if both were wanted: a gradient's sums do not depend on the other.
+      const double wx = piece_work(m, k, n), ww = piece_work(n, k, m);
+      to_x = plan_piece(m, k, n, wx / (wx + ww));
+      to_w = plan_piece(n, k, m, ww / (wx + ww));
+      sums_x = c->take<float>(want_x ? to_x.sum_bytes(kPad) / 4 : 0);
+      sums_w = c->take<float>(want_w ? to_w.sum_bytes(kPad) / 4 : 0);
     } else if (split_room && k > 0) {
       int64_t a = 0, b = 0;
       if (want_x) status = partials(dx_desc(m, k, n), &a);
@@ -1040,7 +1113,11 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   f.w.second.exponent = f.head + 3;
   ScanArgs scan{{f.x.first, f.w.first}, 2, activation, f.head};
   MX_TRY(run_scan<true>(&scan, s));
-  PackArgs pack{{f.x.second, f.w.second}, 2, f.head};
+  PackArgs pack{};
+  pack.count = 2;
+  pack.bad = f.head;
+  pack.op[0] = f.x.second;
+  pack.op[1] = f.w.second;
   MX_TRY(run_pack(&pack, s));
   PieceArgs p{};
   p.out = y;
@@ -1048,7 +1125,8 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   p.residual = residual;
   p.z = z;
   p.act = activation;
-  MX_TRY((run_piece<false, false, true>(p, f.deal, f.x, f.w, f.head, f.sums, s)));
+  fill_piece(&p, f.deal, f.x, false, f.w, false, f.head, f.sums);
+  MX_TRY(run_forward(p, s));
   return gemm_within(&d, x, w, bias, y, 0, s, &epi, nullptr, f.head);
   MX_ABI_END
 }
@@ -1157,26 +1235,38 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
       pack.op[pack.count++] = b.w.second;
     }
     MX_TRY(run_scan<true>(&scan, s));
+    if (db && b.scan.parts > 1) {
+      pack.part = b.part;
+      pack.parts = b.scan.parts;
+      pack.n = int(n);
+      pack.out = db;
+    }
     MX_TRY(run_pack(&pack, s));
   } else if (db || b.dz) {
     MX_TRY(run_scan<false>(&scan, s));
   }
-  if (db && b.scan.parts > 1) {
+  if (db && b.scan.parts > 1 && !b.packed) {
     hipLaunchKernelGGL(column_sum_kernel, dim3(unsigned((n + 31) / 32)), dim3(1024), 0, s, b.part, b.scan.parts, int(n), db);
     MX_HIP(hipGetLastError());
   }
   const int64_t room = b.packed ? 0 : kPartials;
+  if (b.packed) {
+    PieceLaunch l{};
+    if (dx) {
+      l.p[0].out = dx;
+      fill_piece(&l.p[0], b.to_x, b.g, false, b.w, true, b.head, b.sums_x);
+    }
+    if (dw) {
+      l.p[1].out = dw;
+      fill_piece(&l.p[1], b.to_w, b.g, true, b.x, true, b.head + 1, b.sums_w);
+    }
+    MX_TRY(run_backward(l, s));
+  }
   if (dx) {
-    PieceArgs p{};
-    p.out = dx;
-    if (b.packed) MX_TRY((run_piece<false, true, false>(p, b.to_x, b.g, b.w, b.head, b.sums, s)));
     const mx_gemm_desc d = dx_desc(m, k, n);
     MX_TRY(gemm_within(&d, g, w, nullptr, dx, room, s, nullptr, b.split, b.packed ? b.head : nullptr));
   }
   if (dw) {
-    PieceArgs p{};
-    p.out = dw;
-    if (b.packed) MX_TRY((run_piece<true, true, false>(p, b.to_w, b.g, b.x, b.head + 1, b.sums, s)));
     const mx_gemm_desc d = dw_desc(m, k, n);
     MX_TRY(gemm_within(&d, g, x, nullptr, dw, room, s, nullptr, b.split, b.packed ? b.head + 1 : nullptr));
   }

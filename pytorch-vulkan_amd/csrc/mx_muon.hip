@@ -334,7 +334,7 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
 template <class T, int KIND>
 __global__ __launch_bounds__(64) void join_kernel(StepArgs p) {
   int tile, m, n, b, tm, tn;
-  const f32x16 v = join_sums<T>(p.share, tile, m, n);
+  const f32x16 v = join_sums<T>(p.share, blockIdx.x, tile, m, n);
   tile_of<KIND>(p, tile, b, tm, tn);
   finish<KIND>(p, b, tm != tn, tm * T::BM + m, tn * T::BN + n, v);
 }

@@ -368,12 +368,12 @@ __device__ __forceinline__ void store_sums(const f32x16 (&acc)[T::FM][T::FN], co
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
 }
 
-// One 32 x 32 fragment of a joined tile, workgroups of one wave: the parts in
-// their order.  m and n are the fragment's place in the tile.
+// Fragment `id` of the joined tiles (32 x 32, workgroups of one wave): the parts in
+// their order.  m and n are its place in the tile.
 template <class T>
-__device__ __forceinline__ f32x16 join_sums(const Shares& p, int& tile, int& m, int& n) {
+__device__ __forceinline__ f32x16 join_sums(const Shares& p, int id, int& tile, int& m, int& n) {
   constexpr int FRAGS = T::FM * T::FN, PER = T::WAVES * FRAGS;
-  const int at = blockIdx.x / PER, wave = blockIdx.x % PER / FRAGS, f = blockIdx.x % FRAGS;
+  const int at = id / PER, wave = id % PER / FRAGS, f = id % FRAGS;
   const f32x4* from = reinterpret_cast<const f32x4*>(p.sums) +
                       ((int64_t(at) * p.parts * T::WAVES + wave) * FRAGS + f) * 256 + threadIdx.x;
   f32x4 s[4] = {};
