@@ -192,8 +192,8 @@ struct PackArgs {
   PackOp op[3];
   int count;
   int* bad;
-  // Column sums of the first pass, by workgroups from first_sum on: out[c] = sum of
-  // part[p][c] in the order of p, 32 columns and 8 groups of partials to each.
+  // Column sums of the first pass, by workgroups from first_sum on: 32 columns to
+  // each, in column_sum_kernel's order, so that they are the same bits asked alone.
   const float* part;
   int parts, n, first_sum;
   float* out;
@@ -202,19 +202,23 @@ struct PackArgs {
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   __shared__ uint32_t tops[4], col_tops[256];
   if (int(blockIdx.x) >= p.first_sum) {
-    __shared__ float sums[8][33];
+    __shared__ float sums[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int(blockIdx.x) - p.first_sum) * 32 + tx;
-    float s = 0.f;
+    float s[4] = {};
     if (c < p.n) {
-#pragma unroll 16
-      for (int i = ty; i < p.parts; i += 8) s += p.part[int64_t(i) * p.n + c];
+#pragma unroll 4
+      for (int i = ty; i < p.parts; i += 32)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (i + 8 * g < p.parts) s[g] += p.part[int64_t(i + 8 * g) * p.n + c];
     }
-    sums[ty][tx] = s;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) sums[ty + 8 * g][tx] = s[g];
     __syncthreads();
     if (ty == 0 && c < p.n) {
 #pragma unroll
-      for (int g = 1; g < 8; ++g) s += sums[g][tx];
-      p.out[c] = s;
+      for (int g = 1; g < 32; ++g) s[0] += sums[g][tx];
+      p.out[c] = s[0];
     }
     return;
   }
@@ -638,8 +642,8 @@ __global__ __launch_bounds__(WK > 1 ? 64 * WK : 256) void direct_kernel(DirectAr
   }
 }
 
-// out[c] = sum of part[p][c] in the order of p: 32 columns and 32 groups of
-// partials to a workgroup.
+// out[c] = sum of part[p][c]: 32 columns to a workgroup, and 32 groups of partials
+// (every 32nd p), each summed in the order of p and then group after group.
 __global__ __launch_bounds__(1024) void column_sum_kernel(const float* part, int parts, int n, float* out) {
   __shared__ float sum[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;

@@ -234,6 +234,19 @@ def test_linear(mx, m, k, n, act):
         assert torch.equal(one[name], want), name
 
 
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 70), (300, 64, 64), (515, 765, 1026), (2048, 1024, 2048), (3001, 1500, 1501), (20000, 16, 20)])
+def test_linear_bias_gradient_alone(mx, m, k, n, act):
+    print("linear db alone", m, k, n, act, flush=True)
+    g = gen(m + n)
+    x, w, z, dy = rand(g, m, k), rand(g, n, k), rand(g, m, n), rand(g, m, n)
+    z = None if act == "none" else z
+    dx, dw, db, alone = torch.empty_like(x), torch.empty_like(w), torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    mx.linear_backward(dy, x, w, z, dx, dw, db, activation=mx.ACTIVATIONS[act], stream=stream())
+    mx.linear_backward(dy, x, w, z, None, None, alone, activation=mx.ACTIVATIONS[act], stream=stream())
+    assert torch.equal(db, alone)
+
+
 def test_linear_rows_of_any_magnitude(mx):
     """Rows, columns and channels far apart in size keep FP32's accuracy each."""
     g = gen(8)
