@@ -342,10 +342,14 @@ __device__ __forceinline__ void finish_piece(const PieceArgs& p, int m, int n, c
 }
 
 // Both products of a backward go in one launch: 256 tiles of each leave room for
-// the other's on every CU.
+// the other's on every CU.  The one with the longer K goes first, so that the
+// launch does not end on a few long workgroups (a backward of 8192 x 4096 ->
+// 512, whose dw has 128 tiles with K 8192: 375 us, in the other order 413, in two
+// launches 418; of 4096 x 1024 -> 4096, both K 4096: 257, in two launches 266).
 struct PieceLaunch {
   PieceArgs p[2];
-  int second;  // first workgroup of p[1]
+  int second;    // first workgroup of the product that goes second
+  bool swapped;  // p[1] goes first
 };
 
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
@@ -378,10 +382,12 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
 template <class T>
 __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::OCC, T::OCC))) void piece_backward_kernel(PieceLaunch l) {
   __shared__ __attribute__((aligned(1024))) char smem[T::SMEM];
-  if (int(blockIdx.x) < l.second)
-    piece_tile<T, false, true, false>(l.p[0], blockIdx.x, smem);
+  const bool second = int(blockIdx.x) >= l.second;
+  const int id = int(blockIdx.x) - (second ? l.second : 0);
+  if (second == l.swapped)
+    piece_tile<T, false, true, false>(l.p[0], id, smem);
   else
-    piece_tile<T, true, true, false>(l.p[1], int(blockIdx.x) - l.second, smem);
+    piece_tile<T, true, true, false>(l.p[1], id, smem);
 }
 
 template <class T, bool EPI>
@@ -859,8 +865,10 @@ int run_forward(const PieceArgs& p, hipStream_t s) {
 }
 int run_backward(PieceLaunch l, hipStream_t s) {
   using T = PieceTile;
-  l.second = piece_blocks(l.p[0]);
-  hipLaunchKernelGGL(piece_backward_kernel<T>, dim3(unsigned(l.second + piece_blocks(l.p[1]))), dim3(T::THREADS), 0, s, l);
+  const int blocks[2] = {piece_blocks(l.p[0]), piece_blocks(l.p[1])};
+  l.swapped = l.p[1].nk > l.p[0].nk;
+  l.second = blocks[l.swapped];
+  hipLaunchKernelGGL(piece_backward_kernel<T>, dim3(unsigned(blocks[0] + blocks[1])), dim3(T::THREADS), 0, s, l);
   MX_HIP(hipGetLastError());
   return run_joins<false>(l, s);
 }
