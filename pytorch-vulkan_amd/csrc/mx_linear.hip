@@ -803,26 +803,48 @@ Packed packed(int64_t m, int64_t n, int flags, Carve* c) {
 // Largest packed scratch of a call.
 constexpr int64_t kMostPacked = int64_t(4) << 30;
 
-// Whether a call's products run on packed operands: where the time that they
-// save passes what the two passes take, both fitted to measurements
-// (microseconds, mx_gemm.hip's products / packed, with GELU):
-//   m x k -> n            forward     backward
-//   4096 x 1024 -> 4096   216 / 137   481 / 279
-//   8192 x 4096 -> 512    199 / 214   396 / 331
-//   2048 x 2048 -> 2048   110 /  86   228 / 139
-//   256 x 4096 -> 4096     60 /  85   121 / 117
-//   2048 x 1024 -> 1024    38 /  41    92 /  71
-//   1024 x 1024 -> 1024    27 /  33    60 /  56
-//   1537 x 765 -> 2050     64 /  49   133 /  84   (rows not 16-byte aligned)
-//   700 x 700 -> 700       16 /  31    41 /  49
-bool use_packed(int64_t m, int64_t k, int64_t n, bool backward) {
-  if (m < 4 || k < 4 || n < 4) return false;
-  const double mn = double(m) * double(n), sides = double(m) * double(k) + double(n) * double(k);
-  if ((sides + mn) * 5 > double(kMostPacked)) return false;
-  const bool vec = k % 4 == 0 && (!backward || n % 4 == 0);
-  const double saved = mn * double(k) * (backward ? 4e-9 : 2e-9) * (vec ? 3.0 : 10.0);
-  const double passes = backward ? 10.0 + (8.0 * mn + 16.0 * sides) / 7e6 : 12.0 + 20.0 * sides / 7e6;
-  return saved > passes;
+// How a call's products run: as mx_gemm.hip's tiles, as small ones without
+// staging, or on packed operands.
+enum class Form { kTiles, kSmall, kPacked };
+
+// The form whose time is least, each as fitted to measurements of 113 shapes from
+// 17 to 8192 rows and 48 to 4096 columns (which take 1.6 % longer so than with the
+// best form of each).  Microseconds, tiles / small / packed, with GELU:
+//   m x k -> n            forward              backward
+//   17 x 512 -> 512       15 /   7 /  -         25 /  11 /  -
+//   512 x 512 -> 512      16 /   8 /  -         36 /  16 /  -
+//   700 x 700 -> 700      17 /  15 /  31        42 /  32 /  35
+//   64 x 4096 -> 4096     27 /  33 /  81        59 /  79 /  93
+//   8192 x 256 -> 1024    41 /  94 /  48       102 / 135 /  79
+//   1024 x 1024 -> 1024   27 /  35 /  43        61 /  59 /  39
+//   601 x 803 -> 1205     29 /  23 /  43        60 /  46 /  39   (rows not 16-byte aligned)
+//   1000 x 701 -> 1999    41 /  62 /  47        99 /  88 /  51   (the same)
+//   256 x 4096 -> 4096    61 / 118 /  99       121 / 201 / 119
+//   2048 x 2048 -> 2048  113 / 229 /  85       224 / 370 / 128
+//   8192 x 4096 -> 512   205 / 455 / 206       383 / 752 / 375
+//   4096 x 1024 -> 4096  216 /   - / 137       481 /   - / 257
+// Tiles and small products pay for odd rows, small ones by a CU's share of
+// workgroups (a step of 16 k takes four waves 0.45 us), packed ones for two
+// passes over each operand.
+Form form_of(int64_t m, int64_t k, int64_t n, bool backward) {
+  const auto up = [](int64_t v, int64_t to) { return double((v + to - 1) / to); };
+  const double out = 1e-6 * double(m) * double(n), sides = 1e-6 * double(k) * double(m + n), cu = cu_count();
+  const double gflop = (backward ? 4e-3 : 2e-3) * out * double(k);
+  const bool odd = k % 4 || (backward && n % 4);
+  double tiles, small, packed;
+  if (backward) {
+    const double workgroups = up(m, 32) * up(k, 32) * up(n, 64) + up(n, 32) * up(k, 32) * up(m, 64);
+    tiles = std::min(19.0 + 0.45 * up(std::min(m, n), 16), 32.0) + (odd ? 10.0 : 5.0) * gflop + 3.5 * out + 1.4 * sides;
+    small = 9.5 + (odd ? 0.44 : 0.34) * std::max(up(std::max(m, n), 64), workgroups / cu) + 6.5 * out + 2.4 * sides;
+    packed = 26.0 + 1.9 * gflop + 3.4 * sides + 5.0 * out;
+  } else {
+    tiles = std::min(6.0 + 0.23 * up(k, 16), 11.0) + (odd ? 10.8 : 5.7) * gflop + out + 0.7 * sides;
+    small = 3.8 + (odd ? 0.165 : 0.11) * up(k, 16) * std::max(1.0, up(m, 32) * up(n, 32) / cu) + 3.4 * out;
+    packed = 26.5 + 2.0 * gflop + 2.7 * sides + 1.6 * out;
+  }
+  const bool can = std::min({m, k, n}) >= 4 && (out + sides) * 5e6 <= double(kMostPacked);
+  if (can && packed < std::min(tiles, small)) return Form::kPacked;
+  return small < tiles ? Form::kSmall : Form::kTiles;
 }
 
 // out [m][n] over k: operands a (its rows, or where a_cols its columns, are m) and
@@ -910,7 +932,7 @@ struct Forward {
   pieces::Deal deal{};
   float* sums = nullptr;
   int64_t partial = 0;
-  Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(use_packed(m, k, n, false)) {
+  Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(form_of(m, k, n, false) == Form::kPacked) {
     if (!packed) return;
     head = c->take<int>(8);
     x = mx::packed(m, k, 1, c);
@@ -919,31 +941,6 @@ struct Forward {
     sums = c->take<float>(deal.sum_bytes(kPad) / 4);
   }
 };
-
-// Whether products go as small ones: where their time is below that of
-// mx_gemm.hip's tiles, both as fitted to measurements (microseconds, tiles /
-// small, with GELU):
-//   m x k -> n           forward       backward
-//   17 x 512 -> 512      14.5 /  6.6   24.7 / 11.2
-//   90 x 512 -> 512      15.4 /  7.3   26.7 / 12.2
-//   256 x 256 -> 256     10.5 /  5.3   23.9 / 10.2
-//   512 x 512 -> 512     16.0 /  7.7   36.1 / 16.4
-//   300 x 500 -> 700     16.0 /  7.2   29.8 / 16.9
-//   128 x 1024 -> 1024   12.5 / 11.5   25.8 / 17.5
-//   8192 x 64 -> 64       7.3 /  5.1   27.5 / 70.9
-//   64 x 4096 -> 1024    15.3 / 32.0   31.2 / 29.4
-//   64 x 4096 -> 4096    26.6 / 33.2   57.3 / 78.0
-// A step of 16 k takes four waves 0.45 us, a CU one workgroup's at a time.
-bool use_direct(int64_t m, int64_t k, int64_t n, bool backward) {
-  const auto up = [](int64_t v, int64_t to) { return double((v + to - 1) / to); };
-  const double gflop = 2e-9 * double(m) * double(k) * double(n), cu = cu_count();
-  if (!backward) {
-    const double steps = up(k, 16);
-    return 4.0 + 0.11 * steps * std::max(1.0, up(m, 32) * up(n, 32) / cu) < std::min(5.0 + 0.34 * steps, 12.0) + 6.7 * gflop;
-  }
-  const double work = up(m, 32) * up(k, 32) * up(n, 64) + up(n, 32) * up(k, 32) * up(m, 64);
-  return 8.5 + 0.48 * std::max(up(std::max(m, n), 64), work / cu) < 22.0 + 26.0 * gflop;
-}
 
 // Waves that share a tile's K, each with a step of it: eight for a forward's few
 // tiles; four for a backward (of the layer's longer product, whichever gradients
@@ -1002,7 +999,7 @@ int run_few(const float* x, const float* w, const float* bias, const float* resi
 
 int forward_bytes(int64_t m, int64_t k, int64_t n, int64_t* bytes) {
   *bytes = 0;
-  if (m == 0 || n == 0 || k == 0 || use_few(m, k) || use_direct(m, k, n, false)) return MX_OK;
+  if (m == 0 || n == 0 || k == 0 || use_few(m, k) || form_of(m, k, n, false) == Form::kSmall) return MX_OK;
   Carve c(nullptr);
   const Forward f(m, k, n, &c);
   *bytes = c.used;
@@ -1024,7 +1021,7 @@ struct Backward {
   void* split = nullptr;
   int status = MX_OK;
   Backward(int64_t m, int64_t k, int64_t n, bool slope, bool want_x, bool want_w, bool want_b, bool split_room, Carve* c)
-      : packed((want_x || want_w) && use_packed(m, k, n, true)), scan(plan_scan(m, n)) {
+      : packed((want_x || want_w) && form_of(m, k, n, true) == Form::kPacked), scan(plan_scan(m, n)) {
     if (slope && (want_x || want_w)) dz = c->take<float>(m * n);
     if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
     if (packed) {
@@ -1061,7 +1058,7 @@ extern "C" int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activati
   if (m == 0 || n == 0) return MX_OK;
   if (!backward) return forward_bytes(m, k, n, bytes);
   Carve c(nullptr);
-  if (k > 0 && use_direct(m, k, n, true)) {
+  if (k > 0 && form_of(m, k, n, true) == Form::kSmall) {
     (void)small_dz(m, n, activation != MX_ACT_NONE, &c);
     *bytes = c.used;
     return MX_OK;
@@ -1092,7 +1089,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
     if (m <= 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{});
     return run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
   }
-  if (k > 0 && use_direct(m, k, n, false)) {
+  if (k > 0 && form_of(m, k, n, false) == Form::kSmall) {
     DirectArgs a{};
     a.count = 1;
     a.act = activation;
@@ -1106,7 +1103,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   const GemmEpilogue epi{activation, residual, z};
   int64_t need = 0;
   Workspace ws;
-  if (!use_packed(m, k, n, false)) {
+  if (form_of(m, k, n, false) != Form::kPacked) {
     // The product's own scratch is optional: without the caller's, it allocates
     // where it may.
     if (workspace) {
@@ -1165,7 +1162,7 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   MX_REQUIRE(dy && (!slope || z) && (k == 0 || ((!dx || w) && (!dw || x))), MX_ERR_INVALID, who, ": null buffer");
   if (k == 0) dx = dw = nullptr;
   if (!dx && !dw && !db) return MX_OK;
-  if (k > 0 && use_direct(m, k, n, true)) {
+  if (k > 0 && form_of(m, k, n, true) == Form::kSmall) {
     Carve size(nullptr);
     (void)small_dz(m, n, slope, &size);
     Workspace ws;
