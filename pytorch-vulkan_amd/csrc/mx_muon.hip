@@ -237,30 +237,60 @@ __device__ __forceinline__ void tile_of(const StepArgs& p, int id, int& b, int& 
     mfma::tile_coords(id - b * per, p.tiles_m, p.tiles_n, tm, tn);
 }
 
+// What a fragment adds to its product: pieces (kPoly: of G, kNext: of X) or, for
+// the last product of a Muon step, the parameter.
+template <int KIND>
+struct Before {
+  half4 hi[4], lo[4];
+};
+template <>
+struct Before<kGram> {};
+struct Parameter {
+  float was[16];
+};
+template <>
+struct Before<kLast> : Parameter {};
+template <>
+struct Before<kLastRows> : Parameter {};
+
+// Reads that for the 32 x 32 fragment at row m, column n.
+template <int KIND>
+__device__ __forceinline__ void read_before(const StepArgs& p, int b, int m, int n, Before<KIND>& o) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (KIND == kLast || KIND == kLastRows) {
+    if (!p.muon) return;
+    const int col = min((KIND == kLast ? m : n) + (lane & 31), p.g.cols - 1), row0 = (KIND == kLast ? n : m) + 4 * (lane >> 5);
+    const float* const at = p.tab.out[b] + col;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o.was[i] = at[int64_t(min(row0 + 8 * (i >> 2) + (i & 3), p.g.rows - 1)) * p.g.cols];
+  } else if constexpr (KIND != kGram) {
+    const int r = m + (lane & 31), c0 = n + 4 * (lane >> 5);
+    const int64_t plane = KIND == kPoly ? p.a_plane : p.b_plane;
+    const Planes po{p.out, p.out_plane, p.out_rows};
+    const _Float16* const was = (KIND == kPoly ? p.a : p.b) + b * 2 * plane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      o.hi[q] = *reinterpret_cast<const half4*>(was + elem(po, r, c0 + 8 * q));
+      o.lo[q] = *reinterpret_cast<const half4*>(was + plane + elem(po, r, c0 + 8 * q));
+    }
+  }
+}
+
 // Stores a 32 x 32 fragment of a product at row m, column n (of X for the last
 // product).  mirror: its transpose too.
 template <int KIND>
-__device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, int m, int n, const f32x16& v) {
+__device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, int m, int n, const f32x16& v, const Before<KIND>& was) {
   const int lane = threadIdx.x & 63;
   if constexpr (KIND == kLast || KIND == kLastRows) {
     // A wave writes whole 128-byte lines of U's rows either way round.
     const float alpha = p.alpha * p.lift[b];
     const int col = (KIND == kLast ? m : n) + (lane & 31), row0 = (KIND == kLast ? n : m) + 4 * (lane >> 5);
     float* const to = p.tab.out[b] + int64_t(row0) * p.g.cols + col;
-    const bool in = col < p.g.cols;
-    float was[16];
-    if (p.muon) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = 8 * (i >> 2) + (i & 3);
-        was[i] = in && row0 + r < p.g.rows ? to[int64_t(r) * p.g.cols] * p.decay : 0.f;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int r = 8 * (i >> 2) + (i & 3);
       const float x = v[i] * alpha;
-      if (in && row0 + r < p.g.rows) to[int64_t(r) * p.g.cols] = p.muon ? was[i] - p.step * x : x;
+      if (col < p.g.cols && row0 + r < p.g.rows) to[int64_t(r) * p.g.cols] = p.muon ? was.was[i] * p.decay - p.step * x : x;
     }
   } else {
     // G's pieces hold G itself: where X is tiny, all of it that b G and c G^2
@@ -268,16 +298,6 @@ __device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, in
     const float alpha = KIND == kGram ? p.alpha * p.lift[b] * p.lift[b] : p.alpha;
     const Planes po{p.out + b * 2 * p.out_plane, p.out_plane, p.out_rows};
     const int r = m + (lane & 31), c0 = n + 4 * (lane >> 5);
-    half4 wh[4], wl[4];  // G's or X's pieces here
-    if constexpr (KIND != kGram) {
-      const int64_t plane = KIND == kPoly ? p.a_plane : p.b_plane;
-      const _Float16* const was = (KIND == kPoly ? p.a : p.b) + b * 2 * plane;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        wh[q] = *reinterpret_cast<const half4*>(was + elem(po, r, c0 + 8 * q));
-        wl[q] = *reinterpret_cast<const half4*>(was + plane + elem(po, r, c0 + 8 * q));
-      }
-    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int c = c0 + 8 * q;
@@ -287,8 +307,8 @@ __device__ __forceinline__ void finish(const StepArgs& p, int b, bool mirror, in
       for (int e = 0; e < 4; ++e) {
         o[e] = alpha * v[4 * q + e];
         if constexpr (KIND == kPoly)
-          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(wh[q][e]) + float(wl[q][e])) * p.unit) + o[e];
-        if constexpr (KIND == kNext) o[e] += p.keep * (float(wh[q][e]) + float(wl[q][e]));
+          o[e] = (r == c + e ? p.diag : 0.f) + p.lin * ((float(was.hi[q][e]) + float(was.lo[q][e])) * p.unit) + o[e];
+        if constexpr (KIND == kNext) o[e] += p.keep * (float(was.hi[q][e]) + float(was.lo[q][e]));
       }
       half4 hi, lo;
       split4(o, hi, lo);
@@ -324,10 +344,21 @@ __global__ __launch_bounds__(T::THREADS) __attribute__((amdgpu_waves_per_eu(T::O
   }
   const int wave = threadIdx.x >> 6;
   const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
+  // What fragments add is read that far ahead: behind the stores of the one
+  // before, which might be to the same place, each would wait for memory anew (the
+  // last product of a step over 16 x 1024^2 took 160 us so and takes 114, over 6 x 1000
+  // x 513 32 and 20; the pieces that the others read are still in the caches).
+  constexpr int F = T::FM * T::FN, AHEAD = F > 4 ? 2 : F;
+  Before<KIND> was[AHEAD];
+  const auto read = [&](int f) { read_before<KIND>(p, b, m0 + f / T::FN * 32, n0 + f % T::FN * 32, was[f % AHEAD]); };
 #pragma unroll
-  for (int i = 0; i < T::FM; ++i)
+  for (int f = 0; f < AHEAD; ++f) read(f);
 #pragma unroll
-    for (int j = 0; j < T::FN; ++j) finish<KIND>(p, b, tm != tn, m0 + 32 * i, n0 + 32 * j, acc[i][j]);
+  for (int f = 0; f < F; ++f) {
+    const Before<KIND> mine = was[f % AHEAD];
+    if (f + AHEAD < F) read(f + AHEAD);
+    finish<KIND>(p, b, tm != tn, m0 + f / T::FN * 32, n0 + f % T::FN * 32, acc[f / T::FN][f % T::FN], mine);
+  }
 }
 
 // The tiles that were taken in parts.
@@ -336,7 +367,11 @@ __global__ __launch_bounds__(64) void join_kernel(StepArgs p) {
   int tile, m, n, b, tm, tn;
   const f32x16 v = join_sums<T>(p.share, blockIdx.x, tile, m, n);
   tile_of<KIND>(p, tile, b, tm, tn);
-  finish<KIND>(p, b, tm != tn, tm * T::BM + m, tn * T::BN + n, v);
+  m += tm * T::BM;
+  n += tn * T::BN;
+  Before<KIND> was;
+  read_before<KIND>(p, b, m, n, was);
+  finish<KIND>(p, b, tm != tn, m, n, v, was);
 }
 
 // steps == 0: the scaled matrix itself.
