@@ -752,8 +752,8 @@ struct Carve {
 // ------------------------------------------------------------ packed products
 // Products of packed operands run on 128 x 128 tiles, two workgroups to a CU, so
 // that one's stores and activations go on beside the other's products (4096 x
-// 1024 -> 4096 with GELU: 113 us, on 256 x 256 tiles 103 to 116; without an
-// epilogue 90 and 87: not worth kernels of their own).
+// 1024 -> 4096 with GELU: 113 us, on 256 x 256 tiles 103 to 116; a lone
+// product without an epilogue 90 and 87: not worth kernels of their own).
 using PieceTile = pieces::Tile128;
 constexpr int kPad = PieceTile::BM;
 int64_t padded(int64_t v) { return (v + kPad - 1) / kPad * kPad; }
