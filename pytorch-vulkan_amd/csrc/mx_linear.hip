@@ -17,13 +17,15 @@
 // more than they save, take mx_gemm.hip's products as they are.
 //
 // What one scale holds: an element is off by at most 2^-23 of itself or 2^-39 of
-// the operand's largest.  Rows and columns all within 2^8 of that keep FP32's
-// accuracy, each by itself and also where sizes of rows and columns multiply (an
-// element small for both is 2^-16 of the largest); zero ones count for nothing.
-// The second pass notes an operand with others, or one that is not finite or
-// whose largest is below 2^-100, and its products are then taken by
-// mx_gemm.hip's kernels, which follow on the stream and end at once where
-// nothing was noted.
+// the operand's largest.  A row's or a column's depth is the power of two by which
+// its largest element lies below that; zero ones count for nothing.  The second
+// pass notes the deepest of each.  While the two add up to 16 at most, an element
+// of its row's and its column's size is held to 2^-23, whatever the other operand
+// is (the same for both, 8, sent tokens of unlike sizes the long way: a backward
+// of 4096 x 1024 -> 4096 whose rows go down to 2^-12 595 us, so 273).  The
+// products leave an operand beyond that, or one that is not finite or whose
+// largest is below 2^-100, to mx_gemm.hip's kernels, which follow on the stream
+// and end at once otherwise.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -43,6 +45,24 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 // not null; with TOPS, largest magnitudes (as bits: NaN counts above infinity) of
 // rows to row_top[column block][m], of columns to col_top[part][n] and of the
 // workgroup's block to top[workgroup].
+// What the second pass tells of an operand: its scale's power and the depths of
+// its deepest row and column.
+struct About {
+  int exponent, rows, columns;
+};
+constexpr int kMisfit = 1 << 20, kDepth = 16;
+// Depths up to this count as this, so that operands of even sizes write nothing
+// (with a note from every workgroup a backward of 1024 x 1024 -> 1024 takes 41.6
+// us, so 39.3).
+constexpr int kFlat = 3;
+// A call's operands, and for each product whether it is left to mx_gemm.hip's
+// kernels.
+struct Head {
+  About a, b, c;
+  int left[2];
+};
+constexpr int kHeadWords = sizeof(Head) / 4;
+
 struct ScanOp {
   const float* src;
   const float* z;
@@ -58,7 +78,7 @@ struct ScanOp {
 struct ScanArgs {
   ScanOp op[3];
   int count, act;
-  int* bad;  // cleared
+  int* head;  // kHeadWords, cleared
 };
 
 // Largest over a wave, in lane 63, by moves within the vector unit (a shuffle
@@ -104,7 +124,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
   typedef uint32_t uvecu __attribute__((ext_vector_type(W), aligned(4)));
   __shared__ vec sums[256];
   __shared__ uvec tops[TOPS ? 256 : 1];
-  if (p.bad && blockIdx.x == 0 && threadIdx.x < 2) p.bad[threadIdx.x] = 0;
+  if (p.head && blockIdx.x == 0 && threadIdx.x < kHeadWords) p.head[threadIdx.x] = 0;
   int k = 0;
   while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
   const ScanOp& o = p.op[k];
@@ -175,23 +195,20 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
 
 // Second pass: the pieces of an operand [m][n], padded with zeros to
 // [planes.rows] x 64 columns_of_64, times 2^(14 - e) where 2^e is its largest
-// element's power, e to *exponent.  The words of `bad` whose bits `flags` has are
-// set where some row or column is too far below that, or nothing can be scaled.
+// element's power.  What the products need to know of it goes to *about.
 struct PackOp {
   const float* src;
   int m, n;
   pieces::Planes to;
   const uint32_t *row_top, *col_top, *top;
   int col_blocks, parts, tops;
-  int flags;
-  int* exponent;
+  About* about;
   int wide;   // workgroups along a row
   int first;  // first workgroup
 };
 struct PackArgs {
   PackOp op[3];
   int count;
-  int* bad;
   // Column sums of the first pass, by workgroups from first_sum on: 32 columns to
   // each, in column_sum_kernel's order, so that they are the same bits asked alone.
   const float* part;
@@ -253,14 +270,20 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   const bool fits = top == 0 || (top < 0x7F800000u && largest >= 0x1p-100f);
   const int e = top == 0 || !fits ? 0 : int(top >> 23) - 127;
   if (id == 0 && tid == 0) {
-    *o.exponent = e;
+    o.about->exponent = e;
+    if (!fits) atomicMax(&o.about->rows, kMisfit);
   }
-  bool bad = !fits;
-  const auto low = [&](uint32_t t) { return t != 0 && __uint_as_float(t) < largest * 0x1p-8f; };
-  if (bx == 0 && tid < 32 && row < o.m) {
+  const auto depth = [&](uint32_t t) { return t == 0 ? 0u : uint32_t(max(e + 127 - int(t >> 23), 0)); };
+  // By the first wave, its deepest in lane 63.
+  const auto note = [&](uint32_t t, int* word) {
+    const int d = int(wave_top(depth(t)));
+    if (tid == 63 && d > kFlat) atomicMax(word, d);
+  };
+  if (bx == 0 && tid < 64) {
     uint32_t t = 0;
-    for (int i = 0; i < o.col_blocks; ++i) t = max(t, o.row_top[int64_t(i) * o.m + row]);
-    bad = bad || low(t);
+    if (tid < 32 && row < o.m)
+      for (int i = 0; i < o.col_blocks; ++i) t = max(t, o.row_top[int64_t(i) * o.m + row]);
+    note(t, &o.about->rows);
   }
   if (by == 0) {
     const int c = bx * 64 + (tid & 63);
@@ -271,11 +294,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     }
     col_tops[tid] = t;
     __syncthreads();
-    if (tid < 64) bad = bad || low(max(max(t, col_tops[64 + tid]), max(col_tops[128 + tid], col_tops[192 + tid])));
-  }
-  if (bad) {
-    if (o.flags & 1) p.bad[0] = 1;
-    if (o.flags & 2) p.bad[1] = 1;
+    if (tid < 64) note(max(max(t, col_tops[64 + tid]), max(col_tops[128 + tid], col_tops[192 + tid])), &o.about->columns);
   }
   pieces::half8 hi, lo;
 #pragma unroll
@@ -295,7 +314,8 @@ struct PieceArgs {
   pieces::Planes a, b;
   int nk, tiles_m, tiles_n;
   pieces::Shares share;
-  const int *bad, *ea, *eb;
+  const About *ea, *eb;
+  int* left;
   int m, n;
   float* out;
   const float *bias, *residual;
@@ -354,7 +374,11 @@ struct PieceLaunch {
 
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
 __device__ __forceinline__ void piece_tile(const PieceArgs& p, int id, char* smem) {
-  if (*p.bad) return;
+  const About ea = *p.ea, eb = *p.eb;
+  const auto depth = [](const About& e) { return max(e.rows, kFlat) + max(e.columns, kFlat); };
+  const bool left = max(depth(ea), depth(eb)) > kDepth;
+  if (id == 0 && threadIdx.x == 0) *p.left = left;
+  if (left) return;
   const pieces::Unit unit = pieces::unit_of(p.share, id, p.nk);
   int tm, tn;
   mfma::tile_coords(unit.tile, p.tiles_m, p.tiles_n, tm, tn);
@@ -364,7 +388,7 @@ __device__ __forceinline__ void piece_tile(const PieceArgs& p, int id, char* sme
     pieces::store_sums<T>(acc, p.share, unit);
     return;
   }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), up = *p.ea + *p.eb - 28;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), up = ea.exponent + eb.exponent - 28;
   const int m0 = tm * T::BM + wave / T::WN * (T::BM / T::WM), n0 = tn * T::BN + wave % T::WN * (T::BN / T::WN);
 #pragma unroll
   for (int i = 0; i < T::FM; ++i)
@@ -394,11 +418,11 @@ template <class T, bool EPI>
 __global__ __launch_bounds__(64) void piece_join_kernel(PieceLaunch l) {
   const bool second = int(blockIdx.x) >= l.second;
   const PieceArgs& p = l.p[second ? 1 : 0];
-  if (*p.bad) return;
+  if (*p.left) return;
   int tile, m, n, tm, tn;
   const pieces::f32x16 v = pieces::join_sums<T>(p.share, int(blockIdx.x) - (second ? l.second : 0), tile, m, n);
   mfma::tile_coords(tile, p.tiles_m, p.tiles_n, tm, tn);
-  finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, *p.ea + *p.eb - 28);
+  finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, p.ea->exponent + p.eb->exponent - 28);
 }
 
 // A few tokens: y[m][n] for m <= M.  A workgroup takes R rows of w and splits k
@@ -772,7 +796,7 @@ struct Packed {
   PackOp second;
 };
 
-Packed packed(int64_t m, int64_t n, int flags, Carve* c) {
+Packed packed(int64_t m, int64_t n, Carve* c) {
   Packed o{};
   o.m = m;
   o.n = n;
@@ -795,7 +819,6 @@ Packed packed(int64_t m, int64_t n, int flags, Carve* c) {
   o.second.col_blocks = o.scan.col_blocks;
   o.second.parts = o.scan.parts;
   o.second.tops = o.scan.blocks();
-  o.second.flags = flags;
   o.second.wide = int(np / 64);
   return o;
 }
@@ -850,12 +873,12 @@ Form form_of(int64_t m, int64_t k, int64_t n, bool backward) {
 // out [m][n] over k: operands a (its rows, or where a_cols its columns, are m) and
 // b, dealt as d.
 void fill_piece(PieceArgs* p, const pieces::Deal& d, const Packed& a, bool a_cols, const Packed& b, bool b_cols,
-                const int* bad, float* sums) {
+                int* left, float* sums) {
   p->a = a.second.to;
   p->b = b.second.to;
-  p->ea = a.second.exponent;
-  p->eb = b.second.exponent;
-  p->bad = bad;
+  p->ea = a.second.about;
+  p->eb = b.second.about;
+  p->left = left;
   p->m = int(a_cols ? a.n : a.m);
   p->n = int(b_cols ? b.n : b.m);
   p->nk = int(padded(a_cols ? a.m : a.n) / pieces::kBK);
@@ -928,15 +951,15 @@ int run_pack(PackArgs* p, hipStream_t s) {
 struct Forward {
   bool packed;
   Packed x, w;
-  int* head = nullptr;  // two flags, three exponents
+  Head* head = nullptr;
   pieces::Deal deal{};
   float* sums = nullptr;
   int64_t partial = 0;
   Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(form_of(m, k, n, false) == Form::kPacked) {
     if (!packed) return;
-    head = c->take<int>(8);
-    x = mx::packed(m, k, 1, c);
-    w = mx::packed(n, k, 1, c);
+    head = c->take<Head>(1);
+    x = mx::packed(m, k, c);
+    w = mx::packed(n, k, c);
     deal = plan_piece(m, n, k, 1.0);
     sums = c->take<float>(deal.sum_bytes(kPad) / 4);
   }
@@ -1014,7 +1037,7 @@ struct Backward {
   bool packed;
   ScanPlan scan;  // of dz
   float *dz = nullptr, *part = nullptr, *sums_x = nullptr, *sums_w = nullptr;
-  int* head = nullptr;
+  Head* head = nullptr;
   Packed g, x, w;
   pieces::Deal to_x{}, to_w{};
   int64_t gemm = 0;
@@ -1025,10 +1048,10 @@ struct Backward {
     if (slope && (want_x || want_w)) dz = c->take<float>(m * n);
     if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
     if (packed) {
-      head = c->take<int>(8);
-      g = mx::packed(m, n, (want_x ? 1 : 0) | (want_w ? 2 : 0), c);
-      if (want_w) x = mx::packed(m, k, 2, c);
-      if (want_x) w = mx::packed(n, k, 1, c);
+      head = c->take<Head>(1);
+      g = mx::packed(m, n, c);
+      if (want_w) x = mx::packed(m, k, c);
+      if (want_x) w = mx::packed(n, k, c);
       // Dealt as if both were wanted: a gradient's sums do not depend on the other.
       const double wx = piece_work(m, k, n), ww = piece_work(n, k, m);
       to_x = plan_piece(m, k, n, wx / (wx + ww));
@@ -1118,13 +1141,12 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   Forward f(m, k, n, &c);
   f.x.first.src = f.x.second.src = x;
   f.w.first.src = f.w.second.src = w;
-  f.x.second.exponent = f.head + 2;
-  f.w.second.exponent = f.head + 3;
-  ScanArgs scan{{f.x.first, f.w.first}, 2, activation, f.head};
+  f.x.second.about = &f.head->a;
+  f.w.second.about = &f.head->b;
+  ScanArgs scan{{f.x.first, f.w.first}, 2, activation, reinterpret_cast<int*>(f.head)};
   MX_TRY(run_scan<true>(&scan, s));
   PackArgs pack{};
   pack.count = 2;
-  pack.bad = f.head;
   pack.op[0] = f.x.second;
   pack.op[1] = f.w.second;
   MX_TRY(run_pack(&pack, s));
@@ -1134,9 +1156,9 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   p.residual = residual;
   p.z = z;
   p.act = activation;
-  fill_piece(&p, f.deal, f.x, false, f.w, false, f.head, f.sums);
+  fill_piece(&p, f.deal, f.x, false, f.w, false, f.head->left, f.sums);
   MX_TRY(run_forward(p, s));
-  return gemm_within(&d, x, w, bias, y, 0, s, &epi, nullptr, f.head);
+  return gemm_within(&d, x, w, bias, y, 0, s, &epi, nullptr, f.head->left);
   MX_ABI_END
 }
 
@@ -1225,21 +1247,20 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   first.dz = b.dz;
   first.sums = !db ? nullptr : b.scan.parts > 1 ? b.part : db;
   if (b.packed) {
-    scan.bad = b.head;
+    scan.head = reinterpret_cast<int*>(b.head);
     b.g.second.src = g;
-    b.g.second.exponent = b.head + 2;
+    b.g.second.about = &b.head->a;
     PackArgs pack{};
-    pack.bad = b.head;
     pack.op[pack.count++] = b.g.second;
     if (dw) {
       b.x.first.src = b.x.second.src = x;
-      b.x.second.exponent = b.head + 3;
+      b.x.second.about = &b.head->b;
       scan.op[scan.count++] = b.x.first;
       pack.op[pack.count++] = b.x.second;
     }
     if (dx) {
       b.w.first.src = b.w.second.src = w;
-      b.w.second.exponent = b.head + 4;
+      b.w.second.about = &b.head->c;
       scan.op[scan.count++] = b.w.first;
       pack.op[pack.count++] = b.w.second;
     }
@@ -1263,21 +1284,21 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
     PieceLaunch l{};
     if (dx) {
       l.p[0].out = dx;
-      fill_piece(&l.p[0], b.to_x, b.g, false, b.w, true, b.head, b.sums_x);
+      fill_piece(&l.p[0], b.to_x, b.g, false, b.w, true, b.head->left, b.sums_x);
     }
     if (dw) {
       l.p[1].out = dw;
-      fill_piece(&l.p[1], b.to_w, b.g, true, b.x, true, b.head + 1, b.sums_w);
+      fill_piece(&l.p[1], b.to_w, b.g, true, b.x, true, b.head->left + 1, b.sums_w);
     }
     MX_TRY(run_backward(l, s));
   }
   if (dx) {
     const mx_gemm_desc d = dx_desc(m, k, n);
-    MX_TRY(gemm_within(&d, g, w, nullptr, dx, room, s, nullptr, b.split, b.packed ? b.head : nullptr));
+    MX_TRY(gemm_within(&d, g, w, nullptr, dx, room, s, nullptr, b.split, b.packed ? b.head->left : nullptr));
   }
   if (dw) {
     const mx_gemm_desc d = dw_desc(m, k, n);
-    MX_TRY(gemm_within(&d, g, x, nullptr, dw, room, s, nullptr, b.split, b.packed ? b.head + 1 : nullptr));
+    MX_TRY(gemm_within(&d, g, x, nullptr, dw, room, s, nullptr, b.split, b.packed ? b.head->left + 1 : nullptr));
   }
   return MX_OK;
   MX_ABI_END

@@ -571,6 +571,28 @@ def test_linear_packed_misfits(mx, which):
     within(dw, d(dy).t() @ d(x), (m / 8 + 8) * U * (d(dy).abs().t() @ d(x).abs()) + 1e-44, name + " dw")
 
 
+@pytest.mark.parametrize("rows,columns", [(0, 14), (14, 0), (7, 7), (10, 4), (9, 9), (2, 20), (20, 2)])
+def test_linear_packed_depths(mx, rows, columns):
+    """Half the rows of both operands and half their shared columns far below the
+    others: outlier channels and quiet tokens, on both sides of what one scale holds."""
+    print("depths", rows, columns, flush=True)
+    m, k, n = 2048, 1024, 2048
+    x, w, b, res, dy = packed_case(m, k, n)
+    step = lambda c, e: torch.where(torch.arange(c, device="cuda") % 2 == 0, 1.0, 2.0 ** -e)
+    d = lambda t: t.double()
+    # The columns' steps of both operands the same way round, and against each other.
+    for turn in (0, 1):
+        x1 = x * step(m, rows)[:, None] * step(k, columns)
+        w1 = w * step(n, rows)[:, None] * step(k, columns).roll(turn)
+        dy1 = dy * step(m, columns)[:, None].roll(turn, 0) * step(n, rows)
+        y, dx, dw = torch.empty(m, n, device="cuda"), torch.empty(m, k, device="cuda"), torch.empty(n, k, device="cuda")
+        mx.linear_forward(x1, w1, None, y, stream=stream())
+        mx.linear_backward(dy1, x1, w1, None, dx, dw, None, stream=stream())
+        within(y, d(x1) @ d(w1).t(), (k / 8 + 8) * U * (d(x1).abs() @ d(w1).abs().t()), f"y {turn}")
+        within(dx, d(dy1) @ d(w1), (n / 8 + 8) * U * (d(dy1).abs() @ d(w1).abs()), f"dx {turn}")
+        within(dw, d(dy1).t() @ d(x1), (m / 8 + 8) * U * (d(dy1).abs().t() @ d(x1).abs()), f"dw {turn}")
+
+
 def test_linear_packed_special_values(mx):
     m, k, n = 2048, 2048, 2048
     x, w, b, res, dy = packed_case(m, k, n)
