@@ -29,6 +29,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "mx_activation.hpp"
 #include "mx_internal.hpp"
@@ -425,18 +426,26 @@ __global__ __launch_bounds__(64) void piece_join_kernel(PieceLaunch l) {
   finish_piece<EPI>(p, tm * T::BM + m, tn * T::BN + n, v, p.ea->exponent + p.eb->exponent - 28);
 }
 
-// A few tokens: y[m][n] for m <= M.  A workgroup takes R rows of w and splits k
-// between its four waves, lane after lane along it; a wave's partial sums meet in
-// LDS.  Every weight is read once, 16 bytes a lane and all rows of a stretch on
-// their way together, which is what bounds it (4 x 1024 -> 4096: 5.0 us, 4096 -> 16384 for one token 44 us, 6.0 TB/s);
-// x comes from L2, M / R times the weights.
-template <int M, int R>
+constexpr int kFewRows = 4, kFewTokens = 4;  // of w to a workgroup, of x at most
+
+// A few tokens, `groups` of M.  A workgroup takes a group and R rows of w and splits
+// k between its four waves, lane after lane along it; a wave's partial sums meet in
+// LDS.  A weight is 16 bytes to a lane, all rows of a stretch on their way together.
+// One group is bound by reading the weights (4 x 1024 -> 4096: 4.2 us, 4096 -> 16384
+// for one token 44 us, 6.0 TB/s).  More groups take the same rows on the same XCD
+// one after another, so that all but the first find them in its L2: 16 x 4096 ->
+// 1024 8.3 us, where all tokens to a workgroup took 14.1 (M = 8: 7.6, but 5.9
+// against 5.8 for 8 x 1024 -> 4096 and 9.0 against 7.5 for 12).
+template <int M>
 __global__ __launch_bounds__(256) void few_kernel(const float* x, const float* w, const float* bias, const float* residual,
-                                                  int m, int64_t k, int n, int act, float* y, float* z) {
-  static_assert(M * R <= 128, "an output to a thread at most");
+                                                  int tokens, int groups, int64_t k, int n, int act, float* y, float* z) {
+  constexpr int R = kFewRows;
   __shared__ float sums[4][M * R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n0 = int64_t(blockIdx.x) * R;
+  const int turn = int(blockIdx.x) / 8, group = turn % groups, first = group * M, m = min(M, tokens - first);
+  const int64_t n0 = (int64_t(turn / groups) * 8 + int(blockIdx.x) % 8) * R;
+  if (n0 >= n) return;
+  x += int64_t(first) * k;
   float acc[M][R] = {};
   for (int64_t k0 = wave * 256; k0 < k; k0 += 1024) {
     // The lane that k ends in takes its last four elements and leaves out those
@@ -479,7 +488,7 @@ __global__ __launch_bounds__(256) void few_kernel(const float* x, const float* w
   const int64_t col = n0 + t % R;
   if (i >= m || col >= n) return;
   float v = ((sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t])) + (bias ? bias[col] : 0.f);
-  const int64_t to = int64_t(i) * n + col;
+  const int64_t to = int64_t(first + i) * n + col;
   if (z) z[to] = v;
   v = activate(act, v);
   y[to] = v + (residual ? residual[to] : 0.f);
@@ -827,8 +836,8 @@ Packed packed(int64_t m, int64_t n, Carve* c) {
 constexpr int64_t kMostPacked = int64_t(4) << 30;
 
 // How a call's products run: as mx_gemm.hip's tiles, as small ones without
-// staging, or on packed operands.
-enum class Form { kTiles, kSmall, kPacked };
+// staging, on packed operands, or (a forward) as a few tokens.
+enum class Form { kTiles, kSmall, kPacked, kFew };
 
 // The form whose time is least, each as fitted to measurements of 113 shapes from
 // 17 to 8192 rows and 48 to 4096 columns (which take 1.6 % longer so than with the
@@ -846,9 +855,16 @@ enum class Form { kTiles, kSmall, kPacked };
 //   2048 x 2048 -> 2048  113 / 229 /  85       224 / 370 / 128
 //   8192 x 4096 -> 512   205 / 455 / 206       383 / 752 / 375
 //   4096 x 1024 -> 4096  216 /   - / 137       481 /   - / 257
+// and a forward of few tokens, best of the others / few:
+//   m                     4           8           16          32          48
+//   64 -> 2000            3.7 / 3.5   3.9 / 3.6   4.0 / 4.7   4.2 / 7.2   4.2 / 9.6
+//   3000 -> 300           11 / 4.1    11 / 4.2    11 / 4.6    12 / 5.6    12 / 6.7
+//   1024 -> 4096          9.7 / 4.2   10 / 5.8    11 / 9.1    12 / 15     12 / 22
+//   4096 -> 1024          13 / 5.2    14 / 5.5    14 / 8.3    15 / 12     15 / 17
+//   4096 -> 4096          23 / 12     24 / 14     24 / 21     25 / 38     26 / 58
 // Tiles and small products pay for odd rows, small ones by a CU's share of
 // workgroups (a step of 16 k takes four waves 0.45 us), packed ones for two
-// passes over each operand.
+// passes over each operand, few tokens for every group's pass over the weights.
 Form form_of(int64_t m, int64_t k, int64_t n, bool backward) {
   const auto up = [](int64_t v, int64_t to) { return double((v + to - 1) / to); };
   const double out = 1e-6 * double(m) * double(n), sides = 1e-6 * double(k) * double(m + n), cu = cu_count();
@@ -865,9 +881,13 @@ Form form_of(int64_t m, int64_t k, int64_t n, bool backward) {
     small = 3.8 + (odd ? 0.165 : 0.11) * up(k, 16) * std::max(1.0, up(m, 32) * up(n, 32) / cu) + 3.4 * out;
     packed = 26.5 + 2.0 * gflop + 2.7 * sides + 1.6 * out;
   }
-  const bool can = std::min({m, k, n}) >= 4 && (out + sides) * 5e6 <= double(kMostPacked);
-  if (can && packed < std::min(tiles, small)) return Form::kPacked;
-  return small < tiles ? Form::kSmall : Form::kTiles;
+  if (std::min({m, k, n}) < 4 || (out + sides) * 5e6 > double(kMostPacked)) packed = INFINITY;
+  double few = INFINITY;
+  const double groups = up(m, kFewTokens), turns = groups * up(n, kFewRows);
+  if (!backward && m <= 64 && k >= 4 && turns <= 1 << 20)  // as measured, and what a grid holds
+    few = 2.7 + 3e-4 * double(k) + 0.05 * sides + 1e-3 * turns * (0.83 + 7.5e-4 * double(k));
+  const double least = std::min({tiles, small, packed, few});
+  return least == few ? Form::kFew : least == packed ? Form::kPacked : least == small ? Form::kSmall : Form::kTiles;
 }
 
 // out [m][n] over k: operands a (its rows, or where a_cols its columns, are m) and
@@ -1007,22 +1027,21 @@ int run_direct(DirectArgs* d, int wk, hipStream_t s) {
   return MX_OK;
 }
 
-// Tokens that few_kernel takes.
-constexpr int64_t kFew = 16;
-bool use_few(int64_t m, int64_t k) { return m <= kFew && k >= 4; }
-
-template <int M, int R>
+template <int M>
 int run_few(const float* x, const float* w, const float* bias, const float* residual, int64_t m, int64_t k, int64_t n, int act,
             float* y, float* z, hipStream_t s) {
-  hipLaunchKernelGGL((few_kernel<M, R>), dim3(unsigned((n + R - 1) / R)), dim3(256), 0, s, x, w, bias, residual, int(m), k,
-                     int(n), act, y, z);
+  const int64_t groups = (m + M - 1) / M, blocks = (n + kFewRows - 1) / kFewRows;
+  hipLaunchKernelGGL(few_kernel<M>, dim3(unsigned((blocks + 7) / 8 * 8 * groups)), dim3(256), 0, s, x, w, bias, residual,
+                     int(m), int(groups), k, int(n), act, y, z);
   MX_HIP(hipGetLastError());
   return MX_OK;
 }
 
 int forward_bytes(int64_t m, int64_t k, int64_t n, int64_t* bytes) {
   *bytes = 0;
-  if (m == 0 || n == 0 || k == 0 || use_few(m, k) || form_of(m, k, n, false) == Form::kSmall) return MX_OK;
+  if (m == 0 || n == 0 || k == 0) return MX_OK;
+  const Form form = form_of(m, k, n, false);
+  if (form == Form::kFew || form == Form::kSmall) return MX_OK;
   Carve c(nullptr);
   const Forward f(m, k, n, &c);
   *bytes = c.used;
@@ -1101,16 +1120,11 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   if (m == 0 || n == 0) return MX_OK;
   MX_REQUIRE(y && (k == 0 || (x && w)), MX_ERR_INVALID, who, ": null buffer");
   hipStream_t s = resolve_stream(stream);
-  if (use_few(m, k)) {
-    const auto run = [&](auto mm, auto r) {
-      return run_few<decltype(mm)::value, decltype(r)::value>(x, w, bias, residual, m, k, n, activation, y, z, s);
-    };
-    using std::integral_constant;
-    if (m == 1) return run(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    if (m == 2) return run(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    if (m <= 4) return run(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    if (m <= 8) return run(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    return run(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  if (k > 0 && form_of(m, k, n, false) == Form::kFew) {
+    static_assert(kFewTokens == 4);
+    if (m == 1) return run_few<1>(x, w, bias, residual, m, k, n, activation, y, z, s);
+    if (m == 2) return run_few<2>(x, w, bias, residual, m, k, n, activation, y, z, s);
+    return run_few<kFewTokens>(x, w, bias, residual, m, k, n, activation, y, z, s);
   }
   if (k > 0 && form_of(m, k, n, false) == Form::kSmall) {
     DirectArgs a{};

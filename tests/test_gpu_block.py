@@ -247,6 +247,22 @@ def test_linear_bias_gradient_alone(mx, m, k, n, act):
     assert torch.equal(db, alone)
 
 
+@pytest.mark.parametrize("k,n", [(4, 1), (5, 3), (64, 200), (255, 129), (1023, 61), (1100, 1003), (4096, 40)])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 7, 8, 9, 13, 16, 17, 31, 33, 64])
+def test_linear_few_tokens(mx, m, k, n):
+    print("few tokens", m, k, n, flush=True)
+    g = gen(m * 7 + k + n)
+    x, w, b, res = rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, n, scale=0.3), rand(g, m, n)
+    (y, t0), (z, t1) = guarded(m, n), guarded(m, n)
+    mx.linear_forward(x, w, b, y, activation=mx.ACT_GELU, residual=res, z=z, stream=stream())
+    d = lambda t: t.double()
+    zr, yr = linear_ref(d(x), d(w), d(b), d(res), "gelu")
+    z_err = (k / 8 + 8) * U * (d(x).abs() @ d(w).abs().t() + d(b).abs())
+    within(z, zr, z_err, "z")
+    within(y, yr, 1.13 * z_err + 16 * U * (zr.abs() + 1) + 4 * U * yr.abs(), "y")
+    intact(t0, t1)
+
+
 def test_linear_rows_of_any_magnitude(mx):
     """Rows, columns and channels far apart in size keep FP32's accuracy each."""
     g = gen(8)
