@@ -772,35 +772,37 @@ float scale_for(double bound) {
   return float(std::exp2(std::floor(std::log2(60000.0 / (1.05 * std::max(bound, 0x1p-40))))));
 }
 
-// Bounds of X, G and P before and through each iteration: the largest of
-// |sigma (a + b sigma^2 + c sigma^4)| on [0, B] is at an end or where the
-// derivative vanishes.
+// Bounds of X, G and P before and through each iteration, for singular values in
+// [0, B]: X's is B, G's B^2.  P holds b t + c t^2 (t = sigma^2), and a besides in
+// the last iteration; the next B is the largest of |sigma (a + b t + c t^2)|.
+// Each is reached at an end or where the derivative vanishes.  What P holds without
+// a can be the larger: of a = 1, b = -2 it is 2 where a + b t stays within 1.
 int scales_of(const char* who, const mx_newton_schulz& ns, std::vector<Scales>* out) {
   const auto poly = [&](double t) { return ns.a + t * (ns.b + t * ns.c); };
   double b = 1.0;
   for (int64_t i = 0; i < ns.steps; ++i) {
-    const double t1 = b * b;
+    const double t1 = b * b, held = i + 1 < ns.steps ? ns.a : 0.0;  // what P leaves to the update
     double q = std::max(std::fabs(poly(0)), std::fabs(poly(t1))), n = b * std::fabs(poly(t1));
-    const auto at = [&](double t, bool deriv) {
-      if (!(t > 0 && t < t1)) return;
-      if (deriv)
-        n = std::max(n, std::sqrt(t) * std::fabs(poly(t)));
-      else
-        q = std::max(q, std::fabs(poly(t)));
-    };
+    double stored = std::max(std::fabs(poly(0) - held), std::fabs(poly(t1) - held));
+    const auto inside = [&](double t) { return t > 0 && t < t1; };
     if (ns.c != 0) {
-      at(-ns.b / (2 * ns.c), false);
+      const double turn = -ns.b / (2 * ns.c);
+      if (inside(turn)) {
+        q = std::max(q, std::fabs(poly(turn)));
+        stored = std::max(stored, std::fabs(poly(turn) - held));
+      }
       const double disc = 9 * ns.b * ns.b - 20 * ns.a * ns.c;  // a + 3 b t + 5 c t^2 = 0
-      if (disc >= 0) {
-        at((-3 * ns.b + std::sqrt(disc)) / (10 * ns.c), true);
-        at((-3 * ns.b - std::sqrt(disc)) / (10 * ns.c), true);
+      for (const double sign : {1.0, -1.0}) {
+        const double t = disc >= 0 ? (-3 * ns.b + sign * std::sqrt(disc)) / (10 * ns.c) : -1.0;
+        if (inside(t)) n = std::max(n, std::sqrt(t) * std::fabs(poly(t)));
       }
     } else if (ns.b != 0) {
-      at(-ns.a / (3 * ns.b), true);
+      const double t = -ns.a / (3 * ns.b);
+      if (inside(t)) n = std::max(n, std::sqrt(t) * std::fabs(poly(t)));
     }
-    MX_REQUIRE(std::isfinite(q) && std::isfinite(n) && q < kMostBound && n < kMostBound, MX_ERR_INVALID, who,
-               ": the iterations diverge (step ", i, ")");
-    out->push_back({scale_for(b), scale_for(t1), scale_for(q), std::max(1.0, q)});
+    MX_REQUIRE(std::isfinite(q) && std::isfinite(n) && std::isfinite(stored) && q < kMostBound && n < kMostBound, MX_ERR_INVALID,
+               who, ": the iterations diverge (step ", i, ")");
+    out->push_back({scale_for(b), scale_for(t1), scale_for(stored), std::max(1.0, q)});
     b = n;
   }
   for (size_t i = out->size(); i-- > 1;) (*out)[i - 1].growth *= (*out)[i].growth;

@@ -1,0 +1,103 @@
+"""GPU parity of the feed-forward block's operators (C ABI on torch's GPU
+tensors) where their number formats, forms and buffers meet their limits:
+polynomials that turn negative, operands whose elements lie far apart, outputs
+over inputs, sizes that take each form.
+
+Bounds come from the operations' roundings, u = 2^-24 (half a step of FP32
+relative to a value)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def mx():
+    from torch_vulkan import mx as m
+    m.lib()
+    return m
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rand(g, *shape, scale=1.0, mean=0.0):
+    return torch.randn(*shape, device="cuda", generator=g) * scale + mean
+
+
+def within(got, ref, bound, what):
+    err = (got.double() - ref).abs()
+    bad = ~(err <= bound)
+    assert not bool(bad.any()), (
+        f"{what}: {int(bad.sum())}/{bad.numel()} outside; worst err/bound {float((err / bound).nan_to_num(1e30).max()):.3g}")
+
+
+# ---------------------------------------------------- orthogonalised momentum
+def orth(u, steps, coef, eps=1e-7):
+    a, b, c = coef
+    x = u / u.norm().clamp_min(eps)
+    x = x.t() if u.shape[0] > u.shape[1] else x
+    for _ in range(steps):
+        s = x @ x.t()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.t() if u.shape[0] > u.shape[1] else x
+
+
+def few_singular_values(shape, sigma):
+    """Rows and columns far apart, one element each: singular values sigma."""
+    u = torch.zeros(*shape, device="cuda")
+    for i, s in enumerate(sigma):
+        u[i * (shape[0] - 1) // max(1, len(sigma) - 1), i * (shape[1] - 1) // max(1, len(sigma) - 1)] = s
+    return u
+
+
+# (coefficients, singular values whose squares add up to 1).  The second pair of
+# the last polynomial is where it reaches its largest value, 1.165, at which the
+# next iteration's b t + c t^2 is largest.
+TURNING = [((3.0, -5.0, 1.0), (1.0,)), ((1.0, -2.0, 0.0), (1.0,)), ((-1.0, 2.0, 0.0), (1.0,)),
+           ((3.4445, -4.775, 1.2), (0.5208, 0.85368)), ((3.0, -5.0, 1.0), (0.6, 0.8))]
+
+
+@pytest.mark.parametrize("shape", [(2, 9), (9, 2), (40, 70), (70, 40), (130, 257), (300, 200)])
+@pytest.mark.parametrize("coef,sigma", TURNING)
+def test_orthogonalize_polynomials_that_turn_negative(mx, shape, coef, sigma):
+    """b t + c t^2 without a reaches further than a + b t + c t^2 does."""
+    print("turning", shape, coef, sigma, flush=True)
+    a, b, c = coef
+    for steps in (1, 2, 3):
+        for scale in (1.0, 1e-12):  # below eps the matrix is divided by eps
+            u = few_singular_values(shape, sigma) * scale
+            o = torch.full_like(u, 7.0)
+            mx.orthogonalize([u], [o], steps=steps, coefficients=coef, stream=stream())
+            want = orth(u.double(), steps, coef)
+            # An iteration is off by 2^-21 of its terms' magnitudes (operands of 23
+            # bits, 2^-22 of dropped pieces, FP32 sums) and multiplies an error by
+            # the polynomial's slope, 7 at most for these on [0, 1.17].
+            terms = abs(a) + 1.4 * abs(b) + 1.9 * abs(c)
+            tol = 2.0 ** -21 * terms * sum(7.0 ** i for i in range(steps)) * (1.2 if scale == 1.0 else float(want.norm()))
+            assert float((o.double() - want).norm()) <= tol + 1e-30, (steps, scale, float((o.double() - want).norm()), tol)
+
+
+@pytest.mark.parametrize("count", [1, 3])
+def test_muon_polynomial_that_turns_negative(mx, count):
+    g = gen(count)
+    p, m = rand(g, count, 40, 70, scale=1e-2), torch.zeros(count, 40, 70, device="cuda")
+    gr = torch.zeros_like(m)
+    gr[:, 17] = rand(g, count, 70)  # one nonzero row
+    p0, coef = p.clone(), (3.0, -5.0, 1.0)
+    mx.muon_step(p.unbind(0), gr.unbind(0), m.unbind(0), lr=0.5, weight_decay=0.0, momentum=0.5, steps=3, coefficients=coef,
+                 stream=stream())
+    for i in range(count):
+        want = orth(gr[i].double(), 3, coef)  # momentum and Nesterov scale it, the norm divides that out
+        moved = (p0[i].double() - p[i].double()) / 0.5
+        tol = 2.0 ** -21 * (3 + 7 + 1.9) * 57 * 1.2 + 4 * U * float(p0[i].double().norm()) / 0.5
+        assert float((moved - want).norm()) <= tol
