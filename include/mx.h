@@ -512,12 +512,13 @@ int mx_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t src_pitc
 /* Layer norm over the last axis of x [rows, cols]:
  *   y = (x - mean) * rstd * gamma + beta,  rstd = 1/sqrt(var + eps), biased variance.
  * gamma and beta may be NULL (1 and 0); mean and rstd [rows] may be NULL (not
- * kept).  rows == 0 is a no-op, cols == 0 with rows is invalid. */
+ * kept).  y may be x; no other operands may overlap an output.  rows == 0 is a
+ * no-op, cols == 0 with rows is invalid. */
 int mx_layer_norm_forward(const float* x, const float* gamma, const float* beta, int64_t rows, int64_t cols,
                           float eps, float* y, float* mean, float* rstd, void* stream);
 /* Gradients from the saved mean / rstd.  Any of dx, dgamma, dbeta may be NULL
- * (not computed); rows == 0 writes zero dgamma / dbeta.  Column sums are taken
- * in a fixed order. */
+ * (not computed); dx may be dy or x, no other operands may overlap an output.
+ * rows == 0 writes zero dgamma / dbeta.  Column sums are taken in a fixed order. */
 int mx_layer_norm_backward(const float* dy, const float* x, const float* mean, const float* rstd, const float* gamma,
                            int64_t rows, int64_t cols, float* dx, float* dgamma, float* dbeta, void* workspace,
                            int64_t workspace_bytes, void* stream);

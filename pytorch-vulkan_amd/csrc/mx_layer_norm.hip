@@ -82,8 +82,9 @@ __global__ __launch_bounds__(block_of(L)) void ln_fwd_kernel(const float* x, con
   int flip = 0;
   const int64_t step = int64_t(gridDim.x) * RPB;
   for (int64_t row0 = int64_t(blockIdx.x) * RPB; row0 < rows; row0 += step) {
-    // Groups past the last row repeat it (the same values go to the same place).
-    const int64_t row = min(row0 + int(threadIdx.x) / L, rows - 1);
+    // Groups past the last row read it again and store nothing: where y is x, the
+    // row's own group may have stored it before they read.
+    const int64_t mine = row0 + int(threadIdx.x) / L, row = min(mine, rows - 1);
     const float* xr = x + row * cols;
     f32x4 v[V];
 #pragma unroll
@@ -127,6 +128,7 @@ __global__ __launch_bounds__(block_of(L)) void ln_fwd_kernel(const float* x, con
         m2 += p[W + w] + float(n) * d * d;
       }
     }
+    if (mine >= rows) continue;  // at W > 1 a workgroup has one row, so none is here
     const float rs = 1.f / sqrtf(m2 / float(cols) + eps);
     float* yr = y + row * cols;
 #pragma unroll
@@ -211,6 +213,7 @@ __global__ __launch_bounds__(block_of(L)) void ln_bwd_kernel(const float* dy, co
         s2 += p[W + w];
       }
     }
+    if (mine >= rows) continue;  // as in the forward, where dx is dy or x
     s1 *= inv_n;
     s2 *= inv_n;
     float* o = dx + row * cols;

@@ -101,3 +101,41 @@ def test_muon_polynomial_that_turns_negative(mx, count):
         moved = (p0[i].double() - p[i].double()) / 0.5
         tol = 2.0 ** -21 * (3 + 7 + 1.9) * 57 * 1.2 + 4 * U * float(p0[i].double().norm()) / 0.5
         assert float((moved - want).norm()) <= tol
+
+
+# ---------------------------------------------------------------- layer norm
+def ln_case(rows, cols):
+    g = gen(rows + cols)
+    return rand(g, rows, cols) * 3 + 1, rand(g, cols, mean=2.0), rand(g, cols, mean=-1.0), rand(g, rows, cols)
+
+
+# Every width class, and last rows that leave groups of lanes without one.
+IN_PLACE = [(1, 40), (15, 61), (37, 130), (11, 131), (9, 256), (3, 400), (6, 511), (5, 1000), (700, 1023), (3, 2048), (2, 5000), (2, 16001)]
+
+
+@pytest.mark.parametrize("rows,cols", IN_PLACE)
+def test_layer_norm_forward_over_its_input(mx, rows, cols):
+    print("layer norm in place", rows, cols, flush=True)
+    x, gamma, beta, _ = ln_case(rows, cols)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    mx.layer_norm_forward(x, gamma, beta, 1e-5, y, mean, rstd, stream=stream())
+    for _ in range(5):
+        over, m, r = x.clone(), torch.empty_like(mean), torch.empty_like(rstd)
+        mx.layer_norm_forward(over, gamma, beta, 1e-5, over, m, r, stream=stream())
+        assert torch.equal(over, y) and torch.equal(m, mean) and torch.equal(r, rstd)
+
+
+@pytest.mark.parametrize("rows,cols", IN_PLACE)
+@pytest.mark.parametrize("which", ["dy", "x"])
+def test_layer_norm_backward_over_an_input(mx, rows, cols, which):
+    print("layer norm backward in place", rows, cols, which, flush=True)
+    x, gamma, beta, dy = ln_case(rows, cols)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    mx.layer_norm_forward(x, gamma, beta, 1e-5, y, mean, rstd, stream=stream())
+    dx, dg, db = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(gamma)
+    mx.layer_norm_backward(dy, x, mean, rstd, gamma, dx, dg, db, stream=stream())
+    for _ in range(5):
+        t = {"dy": dy.clone(), "x": x.clone()}
+        g, b = torch.empty_like(dg), torch.empty_like(db)
+        mx.layer_norm_backward(t["dy"], t["x"], mean, rstd, gamma, t[which], g, b, stream=stream())
+        assert torch.equal(t[which], dx) and torch.equal(g, dg) and torch.equal(b, db)
