@@ -478,6 +478,12 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
   float* const part = ws.as<float>();
   int parts = 1;
   if (shape == kWalk) {
+    if (affine) {  // before dx, which may be stored over dy or x
+      parts = walk_parts(rows);
+      hipLaunchKernelGGL(ln_cols_walk_kernel, dim3(unsigned((cols + 255) / 256), unsigned(parts)), dim3(256), 0, s, dy, x,
+                         mean, rstd, rows, cols, part);
+      MX_HIP(hipGetLastError());
+    }
     if (dx) {
       const int threads = cols < 1024 ? 64 : 1024;
       hipLaunchKernelGGL(ln_bwd_walk_kernel, dim3(unsigned(std::min<int64_t>(rows, 65535))), dim3(threads), 0, s, dy, x,
@@ -485,10 +491,6 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
       MX_HIP(hipGetLastError());
     }
     if (!affine) return MX_OK;
-    parts = walk_parts(rows);
-    hipLaunchKernelGGL(ln_cols_walk_kernel, dim3(unsigned((cols + 255) / 256), unsigned(parts)), dim3(256), 0, s, dy, x,
-                       mean, rstd, rows, cols, part);
-    MX_HIP(hipGetLastError());
   } else {
     parts = bwd_blocks(shape, rows);
     with_shape(shape, [&](auto l, auto v) {

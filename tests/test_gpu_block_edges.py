@@ -113,7 +113,11 @@ def ln_case(rows, cols):
 IN_PLACE = [(1, 40), (15, 61), (37, 130), (11, 131), (9, 256), (3, 400), (6, 511), (5, 1000), (700, 1023), (3, 2048), (2, 5000), (2, 16001)]
 
 
-@pytest.mark.parametrize("rows,cols", IN_PLACE)
+# Widths that are walked from memory.
+WALKED = [(5, 1), (70, 3), (3, 16389), (130, 20000)]
+
+
+@pytest.mark.parametrize("rows,cols", IN_PLACE + WALKED)
 def test_layer_norm_forward_over_its_input(mx, rows, cols):
     print("layer norm in place", rows, cols, flush=True)
     x, gamma, beta, _ = ln_case(rows, cols)
@@ -125,7 +129,7 @@ def test_layer_norm_forward_over_its_input(mx, rows, cols):
         assert torch.equal(over, y) and torch.equal(m, mean) and torch.equal(r, rstd)
 
 
-@pytest.mark.parametrize("rows,cols", IN_PLACE)
+@pytest.mark.parametrize("rows,cols", IN_PLACE + WALKED)
 @pytest.mark.parametrize("which", ["dy", "x"])
 def test_layer_norm_backward_over_an_input(mx, rows, cols, which):
     print("layer norm backward in place", rows, cols, which, flush=True)
