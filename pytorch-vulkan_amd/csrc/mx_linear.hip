@@ -9,23 +9,32 @@
 // evaluate the slope once for every tile that reads the element), then takes the
 // two products of it.
 //
-// Two forms of the products.  Large ones run on operands packed as two fp16
-// pieces (mx_pieces.hpp): a pass over each operand finds its largest element,
-// rows and columns on the way, a second one writes the pieces, scaled by a power
-// of two for the whole operand, and the products take half the matrix
-// instructions of three bf16 pieces.  Small ones, for which the two passes cost
-// more than they save, take mx_gemm.hip's products as they are.
+// Four forms of the products (form_of).  Large ones run on operands packed as two
+// fp16 pieces (mx_pieces.hpp): a pass over each operand finds its largest and its
+// least element on the way, a second one writes the pieces, scaled by a power of two
+// for the whole operand, and the products take half the matrix instructions of
+// three bf16 pieces.  Where the two passes cost more than they save, the products
+// are mx_gemm.hip's, or small ones without staging, or for a few tokens sums of
+// vector instructions.
 //
-// What one scale holds: an element is off by at most 2^-23 of itself or 2^-39 of
-// the operand's largest.  A row's or a column's depth is the power of two by which
-// its largest element lies below that; zero ones count for nothing.  The second
-// pass notes the deepest of each.  While the two add up to 16 at most, an element
-// of its row's and its column's size is held to 2^-23, whatever the other operand
-// is (the same for both, 8, sent tokens of unlike sizes the long way: a backward
-// of 4096 x 1024 -> 4096 whose rows go down to 2^-12 595 us, so 273).  The
-// products leave an operand beyond that, or one that is not finite or whose
-// largest is below 2^-100, to mx_gemm.hip's kernels, which follow on the stream
-// and end at once otherwise.
+// What one scale holds: an element is off by at most 2^-23 of itself or, with raised
+// lo pieces, 2^-51 of the operand's largest (both as powers of two).  An element d
+// powers below that largest is therefore off by 2^(d - 51) of itself, and while no
+// nonzero one of either operand is deeper than 23 + log2 k, a sum over k is off by at
+// most (k / 8) 2^-24 of its terms' magnitudes by that, whatever the operands are.
+// Of normal random operands with 2^24 elements and k = 1024 one in 200 has a deeper
+// one.
+//
+// Deeper ones (the tails of GELU and SiLU have them) are lost only in sums without
+// larger terms, so the second pass counts, for every row and column that a product
+// takes, the elements that are within 2^-14 of the largest.  Where any two rows
+// of the operands have k + 64 of them together, 64 terms at least have both, which
+// is 64 2^-28 of the largest product, against at most 4 k 2^-51 that the deep
+// elements are off by: (k / 8) 2^-24 of the terms again.  Rows of zeros need none.
+//
+// The products leave operands that neither holds for, that are not finite or whose
+// largest is below 2^-100, to mx_gemm.hip's kernels, which follow on the stream and
+// end at once otherwise.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -41,35 +50,36 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// One operand's first pass: where `z` is not null src is dy and the values are
-// dz = dy act'(z), written to dz.  Column sums to sums[part][n] where that is
-// not null; with TOPS, largest magnitudes (as bits: NaN counts above infinity) of
-// rows to row_top[column block][m], of columns to col_top[part][n] and of the
-// workgroup's block to top[workgroup].
-// What the second pass tells of an operand: its scale's power and the depths of
-// its deepest row and column.
+// What the second pass tells of an operand: its largest element's power, and by
+// how many powers its least nonzero one lies below that.
 struct About {
-  int exponent, rows, columns;
+  int exponent, depth;
 };
-constexpr int kMisfit = 1 << 20, kDepth = 16;
-// Depths up to this count as this, so that operands of even sizes write nothing
-// (with a note from every workgroup a backward of 1024 x 1024 -> 1024 takes 41.6
-// us, so 39.3).
-constexpr int kFlat = 3;
+constexpr int kMisfit = 1 << 20;          // depth of an operand that no scale holds
+constexpr int kLargeDepth = 14, kShared = 64;  // of the counted elements, and how many any two rows share
 // A call's operands, and for each product whether it is left to mx_gemm.hip's
 // kernels.
 struct Head {
   About a, b, c;
   int left[2];
 };
-constexpr int kHeadWords = sizeof(Head) / 4;
 
+// Large elements of a row or a column in the low word; the high one is zero for a row
+// of zeros.
+typedef unsigned long long Large;
+
+// One operand's first pass: where `z` is not null src is dy and the values are
+// dz = dy act'(z), written to dz.  Column sums to sums[part][n] where that is
+// not null; with ENDS the largest magnitude (as bits: NaN counts above infinity)
+// and the least one's negative (0: all are zero) of the workgroup's block to
+// ends[workgroup], and the counts cleared for the second pass.
 struct ScanOp {
   const float* src;
   const float* z;
   float* dz;
   float* sums;
-  uint32_t *row_top, *col_top, *top;
+  uint2* ends;
+  Large *row_large, *col_large;  // null where no product asks
   int64_t m;
   int n;
   int64_t rows_per;
@@ -79,7 +89,6 @@ struct ScanOp {
 struct ScanArgs {
   ScanOp op[3];
   int count, act;
-  int* head;  // kHeadWords, cleared
 };
 
 // Largest over a wave, in lane 63, by moves within the vector unit (a shuffle
@@ -115,17 +124,14 @@ __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(
 
 // A thread holds W columns; 64 threads lie along a row and the workgroup's four
 // waves take a row each.  W == 4 for n >= 4: the last thread of a row takes its
-// last four elements (it and its neighbour write the same values).  TOPS: the
-// largest magnitudes are wanted.
-template <int W, bool TOPS>
+// last four elements (it and its neighbour write the same values).  ENDS: the
+// second pass follows.
+template <int W, bool ENDS>
 __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
   typedef float vec __attribute__((ext_vector_type(W)));
   typedef float vecu __attribute__((ext_vector_type(W), aligned(4)));
-  typedef uint32_t uvec __attribute__((ext_vector_type(W)));
-  typedef uint32_t uvecu __attribute__((ext_vector_type(W), aligned(4)));
   __shared__ vec sums[256];
-  __shared__ uvec tops[TOPS ? 256 : 1];
-  if (p.head && blockIdx.x == 0 && threadIdx.x < kHeadWords) p.head[threadIdx.x] = 0;
+  __shared__ uint2 ends[4];
   int k = 0;
   while (k + 1 < p.count && int(blockIdx.x) >= p.op[k + 1].first) ++k;
   const ScanOp& o = p.op[k];
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
   const float* const src = o.src;
   const float* const z = o.z;
   vec s = 0.f;
-  uvec top = 0u;
+  uint32_t top = 0, low = 0;
   constexpr int ROWS = 4;  // of a wave, on their way together
   for (int64_t r = r0 + wave; r < r1; r += 4 * ROWS) {
     vec d[ROWS], t[ROWS];
@@ -157,22 +163,29 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
         if (o.dz && in && r + 4 * u < r1) *reinterpret_cast<vecu*>(o.dz + (r + 4 * u) * n + at) = d[u];
       }
       s += d[u];
-      if constexpr (TOPS) {
-        uint32_t row = 0;
+      if constexpr (ENDS) {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           const uint32_t v = magnitude(d[u][e]);
-          top[e] = max(top[e], v);
-          row = max(row, v);
+          top = max(top, v);
+          low = max(low, 0u - v);
         }
-        row = wave_top(row);
-        if (lane == 63 && r + 4 * u < r1) o.row_top[int64_t(bx) * o.m + r + 4 * u] = row;
       }
     }
   }
-  if (!o.sums && !TOPS) return;
+  if constexpr (ENDS) {
+    if (o.row_large && bx == 0)
+      for (int64_t r = r0 + threadIdx.x; r < r1; r += 256) o.row_large[r] = 0;
+    if (o.col_large && by == 0 && threadIdx.x < 64 * W && int64_t(bx) * 64 * W + threadIdx.x < n)
+      o.col_large[int64_t(bx) * 64 * W + threadIdx.x] = 0;
+  }
+  if (!o.sums && !ENDS) return;
   sums[threadIdx.x] = s;
-  if constexpr (TOPS) tops[threadIdx.x] = top;
+  if constexpr (ENDS) {
+    top = wave_top(top);
+    low = wave_top(low);
+    if (lane == 63) ends[wave] = {top, low};
+  }
   __syncthreads();
   if (wave != 0) return;
   if (o.sums && in) {
@@ -181,28 +194,24 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
     s += sums[192 + lane];
     *reinterpret_cast<vecu*>(o.sums + int64_t(by) * n + at) = s;
   }
-  if constexpr (TOPS) {
-    uint32_t all = 0;
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      top[e] = max(max(top[e], tops[64 + lane][e]), max(tops[128 + lane][e], tops[192 + lane][e]));
-      all = max(all, top[e]);
-    }
-    if (in) *reinterpret_cast<uvecu*>(o.col_top + int64_t(by) * n + at) = top;
-    all = wave_top(all);
-    if (lane == 63) o.top[id] = all;
+  if constexpr (ENDS) {
+    if (lane == 0)
+      o.ends[id] = {max(max(ends[0].x, ends[1].x), max(ends[2].x, ends[3].x)),
+                    max(max(ends[0].y, ends[1].y), max(ends[2].y, ends[3].y))};
   }
 }
 
 // Second pass: the pieces of an operand [m][n], padded with zeros to
 // [planes.rows] x 64 columns_of_64, times 2^(14 - e) where 2^e is its largest
-// element's power.  What the products need to know of it goes to *about.
+// element's power.  What the products need to know of it goes to *about, and its
+// large elements (of at least 1 then) are counted.
 struct PackOp {
   const float* src;
   int m, n;
   pieces::Planes to;
-  const uint32_t *row_top, *col_top, *top;
-  int col_blocks, parts, tops;
+  const uint2* ends;
+  int blocks;  // of the first pass
+  Large *row_large, *col_large;
   About* about;
   int wide;   // workgroups along a row
   int first;  // first workgroup
@@ -218,7 +227,8 @@ struct PackArgs {
 };
 
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
-  __shared__ uint32_t tops[4], col_tops[256];
+  __shared__ uint2 ends[4];
+  __shared__ int found[4][32];
   if (int(blockIdx.x) >= p.first_sum) {
     __shared__ float sums[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = (int(blockIdx.x) - p.first_sum) * 32 + tx;
@@ -261,48 +271,56 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
       for (int e = 0; e < 8; ++e) v[e] = col + e < o.n ? from[e] : 0.f;
     }
   }
-  uint32_t top = 0;
-  for (int i = tid; i < o.tops; i += 256) top = max(top, o.top[i]);
+  uint32_t top = 0, low = 0;
+  for (int i = tid; i < o.blocks; i += 256) {
+    const uint2 e = o.ends[i];
+    top = max(top, e.x);
+    low = max(low, e.y);
+  }
   top = wave_top(top);
-  if ((tid & 63) == 63) tops[tid >> 6] = top;
+  low = wave_top(low);
+  if ((tid & 63) == 63) ends[tid >> 6] = {top, low};
   __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-  const float largest = __uint_as_float(top);
-  const bool fits = top == 0 || (top < 0x7F800000u && largest >= 0x1p-100f);
+  top = max(max(ends[0].x, ends[1].x), max(ends[2].x, ends[3].x));
+  const bool fits = top == 0 || (top < 0x7F800000u && __uint_as_float(top) >= 0x1p-100f);
   const int e = top == 0 || !fits ? 0 : int(top >> 23) - 127;
   if (id == 0 && tid == 0) {
-    o.about->exponent = e;
-    if (!fits) atomicMax(&o.about->rows, kMisfit);
-  }
-  const auto depth = [&](uint32_t t) { return t == 0 ? 0u : uint32_t(max(e + 127 - int(t >> 23), 0)); };
-  // By the first wave, its deepest in lane 63.
-  const auto note = [&](uint32_t t, int* word) {
-    const int d = int(wave_top(depth(t)));
-    if (tid == 63 && d > kFlat) atomicMax(word, d);
-  };
-  if (bx == 0 && tid < 64) {
-    uint32_t t = 0;
-    if (tid < 32 && row < o.m)
-      for (int i = 0; i < o.col_blocks; ++i) t = max(t, o.row_top[int64_t(i) * o.m + row]);
-    note(t, &o.about->rows);
-  }
-  if (by == 0) {
-    const int c = bx * 64 + (tid & 63);
-    uint32_t t = 0;
-    if (c < o.n) {
-#pragma unroll 16
-      for (int i = tid >> 6; i < o.parts; i += 4) t = max(t, o.col_top[int64_t(i) * o.n + c]);
-    }
-    col_tops[tid] = t;
-    __syncthreads();
-    if (tid < 64) note(max(max(t, col_tops[64 + tid]), max(col_tops[128 + tid], col_tops[192 + tid])), &o.about->columns);
+    const uint32_t least = 0u - max(max(ends[0].y, ends[1].y), max(ends[2].y, ends[3].y));
+    // A subnormal's own power is not in its bits: as the least there is.
+    const int power = least < 0x00800000u ? -149 : int(least >> 23) - 127;
+    *o.about = {e, top == 0 ? 0 : fits ? e - power : kMisfit};
   }
   pieces::half8 hi, lo;
+  int large = 0, column = 0;
+  bool some = false;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const float f = ldexpf(v[q], 14 - e);
     hi[q] = _Float16(f);
-    lo[q] = _Float16(f - float(hi[q]));
+    lo[q] = _Float16((f - float(hi[q])) * float(1 << pieces::kRaised));
+    static_assert(kLargeDepth == 14);
+    const bool is = fabsf(f) >= 1.f;
+    large += is;
+    some |= v[q] != 0.f;
+    if (o.col_large) {
+      // Half a wave holds 32 rows of a column: their count to the half's lane q.
+      const uint64_t which = __ballot(is);
+      asm("v_writelane_b32 %0, %1, %2" : "+v"(column) : "s"(__popc(uint32_t(which))), "i"(q));
+      asm("v_writelane_b32 %0, %1, %2" : "+v"(column) : "s"(__popc(uint32_t(which >> 32))), "i"(32 + q));
+    }
+  }
+  const int at = col + (tid & 31);
+  if (o.col_large && (tid & 31) < 8 && at < o.n) atomicAdd(o.col_large + at, Large(1) << 32 | uint32_t(column));
+  if (o.row_large) {
+    // The row's eight groups of eight: two to a wave.
+    large |= int(some) << 16;
+    large += __shfl_xor(large, 32, 64);
+    if ((tid & 63) < 32) found[tid >> 6][tid & 31] = large;
+    __syncthreads();
+    if (tid < 32 && row < o.m) {
+      large = (found[0][tid] + found[1][tid]) + (found[2][tid] + found[3][tid]);
+      if (large) atomicAdd(o.row_large + row, Large(large >> 16) << 32 | (large & 0xFFFF));
+    }
   }
   _Float16* const to = o.to.at + (int64_t(col >> 3) * o.to.rows + row) * 8;
   *reinterpret_cast<pieces::half8*>(to) = hi;
@@ -316,8 +334,9 @@ struct PieceArgs {
   int nk, tiles_m, tiles_n;
   pieces::Shares share;
   const About *ea, *eb;
+  const Large *large_a, *large_b;  // of a's rows m and b's rows n (columns where the product runs along them)
   int* left;
-  int m, n;
+  int m, n, k;
   float* out;
   const float *bias, *residual;
   float* z;
@@ -373,18 +392,48 @@ struct PieceLaunch {
   bool swapped;  // p[1] goes first
 };
 
+// A thread's least count of `count` rows that are not zero, eight loads on their way
+// together; negative, as in the first pass, of one more (0: there is none).
+__device__ __forceinline__ uint32_t least_large(const Large* of, int count) {
+  uint32_t low = 0;
+  for (int i = threadIdx.x; i < count; i += 8 * blockDim.x) {
+    Large c[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) c[u] = of[min(i + u * int(blockDim.x), count - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) low = max(low, c[u] ? 0u - (uint32_t(c[u]) + 1) : 0u);
+  }
+  return low;
+}
+
+// Whether the product is left to mx_gemm.hip's kernels.
+__device__ __forceinline__ bool left_out(const PieceArgs& p, const About& ea, const About& eb, char* smem) {
+  const int deepest = max(ea.depth, eb.depth);
+  if (deepest >= kMisfit) return true;
+  if (deepest <= max(28, 23 + 31 - __clz(p.k))) return false;
+  uint2* const lds = reinterpret_cast<uint2*>(smem);
+  uint2 low = {least_large(p.large_a, p.m), least_large(p.large_b, p.n)};
+  low = {wave_top(low.x), wave_top(low.y)};
+  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = low;
+  __syncthreads();
+  low = lds[0];
+  for (int w = 1; w < int(blockDim.x >> 6); ++w) low = {max(low.x, lds[w].x), max(low.y, lds[w].y)};
+  __syncthreads();
+  const auto count = [](uint32_t v) { return v ? uint64_t(0u - v) - 1 : uint64_t(1) << 32; };
+  return count(low.x) + count(low.y) < uint64_t(p.k) + kShared;
+}
+
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
 __device__ __forceinline__ void piece_tile(const PieceArgs& p, int id, char* smem) {
   const About ea = *p.ea, eb = *p.eb;
-  const auto depth = [](const About& e) { return max(e.rows, kFlat) + max(e.columns, kFlat); };
-  const bool left = max(depth(ea), depth(eb)) > kDepth;
+  const bool left = left_out(p, ea, eb, smem);
   if (id == 0 && threadIdx.x == 0) *p.left = left;
   if (left) return;
   const pieces::Unit unit = pieces::unit_of(p.share, id, p.nk);
   int tm, tn;
   mfma::tile_coords(unit.tile, p.tiles_m, p.tiles_n, tm, tn);
   pieces::f32x16 acc[T::FM][T::FN];
-  pieces::product<T, A_COLS, B_COLS, true>(acc, p.a, p.b, tm * T::BM, tn * T::BN, unit.k0, unit.k1 - unit.k0, smem);
+  pieces::product<T, A_COLS, B_COLS, true, pieces::kRaised>(acc, p.a, p.b, tm * T::BM, tn * T::BN, unit.k0, unit.k1 - unit.k0, smem);
   if (unit.tile >= p.share.whole) {
     pieces::store_sums<T>(acc, p.share, unit);
     return;
@@ -805,7 +854,8 @@ struct Packed {
   PackOp second;
 };
 
-Packed packed(int64_t m, int64_t n, Carve* c) {
+// by_rows, by_cols: products run along its rows, its columns.
+Packed packed(int64_t m, int64_t n, bool by_rows, bool by_cols, Carve* c) {
   Packed o{};
   o.m = m;
   o.n = n;
@@ -816,18 +866,16 @@ Packed packed(int64_t m, int64_t n, Carve* c) {
   o.first.rows_per = o.scan.rows_per;
   o.first.col_blocks = o.scan.col_blocks;
   o.first.parts = o.scan.parts;
-  o.first.row_top = c->take<uint32_t>(m * o.scan.col_blocks);
-  o.first.col_top = c->take<uint32_t>(n * o.scan.parts);
-  o.first.top = c->take<uint32_t>(o.scan.blocks());
+  o.first.ends = c->take<uint2>(o.scan.blocks());
+  o.first.row_large = by_rows ? c->take<Large>(m) : nullptr;
+  o.first.col_large = by_cols ? c->take<Large>(n) : nullptr;
   o.second.m = int(m);
   o.second.n = int(n);
   o.second.to = {c->take<_Float16>(2 * mp * np), mp * np, int(mp)};
-  o.second.row_top = o.first.row_top;
-  o.second.col_top = o.first.col_top;
-  o.second.top = o.first.top;
-  o.second.col_blocks = o.scan.col_blocks;
-  o.second.parts = o.scan.parts;
-  o.second.tops = o.scan.blocks();
+  o.second.ends = o.first.ends;
+  o.second.blocks = o.scan.blocks();
+  o.second.row_large = o.first.row_large;
+  o.second.col_large = o.first.col_large;
   o.second.wide = int(np / 64);
   return o;
 }
@@ -898,10 +946,13 @@ void fill_piece(PieceArgs* p, const pieces::Deal& d, const Packed& a, bool a_col
   p->b = b.second.to;
   p->ea = a.second.about;
   p->eb = b.second.about;
+  p->large_a = a_cols ? a.second.col_large : a.second.row_large;
+  p->large_b = b_cols ? b.second.col_large : b.second.row_large;
   p->left = left;
   p->m = int(a_cols ? a.n : a.m);
   p->n = int(b_cols ? b.n : b.m);
-  p->nk = int(padded(a_cols ? a.m : a.n) / pieces::kBK);
+  p->k = int(a_cols ? a.m : a.n);
+  p->nk = int(padded(p->k) / pieces::kBK);
   p->tiles_m = int(padded(p->m) / kPad);
   p->tiles_n = int(padded(p->n) / kPad);
   p->share = {int(d.whole), d.parts, sums};
@@ -939,7 +990,7 @@ int run_backward(PieceLaunch l, hipStream_t s) {
 }
 
 // First and second pass of a call's operands.
-template <bool TOPS>
+template <bool ENDS>
 int run_scan(ScanArgs* p, hipStream_t s) {
   int blocks = 0;
   for (int i = 0; i < p->count; ++i) {
@@ -947,9 +998,9 @@ int run_scan(ScanArgs* p, hipStream_t s) {
     blocks += p->op[i].col_blocks * p->op[i].parts;
   }
   if (p->op[0].n >= 4)
-    hipLaunchKernelGGL((scan_kernel<4, TOPS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+    hipLaunchKernelGGL((scan_kernel<4, ENDS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
   else
-    hipLaunchKernelGGL((scan_kernel<1, TOPS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+    hipLaunchKernelGGL((scan_kernel<1, ENDS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
   MX_HIP(hipGetLastError());
   return MX_OK;
 }
@@ -978,8 +1029,8 @@ struct Forward {
   Forward(int64_t m, int64_t k, int64_t n, Carve* c) : packed(form_of(m, k, n, false) == Form::kPacked) {
     if (!packed) return;
     head = c->take<Head>(1);
-    x = mx::packed(m, k, c);
-    w = mx::packed(n, k, c);
+    x = mx::packed(m, k, true, false, c);
+    w = mx::packed(n, k, true, false, c);
     deal = plan_piece(m, n, k, 1.0);
     sums = c->take<float>(deal.sum_bytes(kPad) / 4);
   }
@@ -1068,9 +1119,9 @@ struct Backward {
     if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
     if (packed) {
       head = c->take<Head>(1);
-      g = mx::packed(m, n, c);
-      if (want_w) x = mx::packed(m, k, c);
-      if (want_x) w = mx::packed(n, k, c);
+      g = mx::packed(m, n, want_x, want_w, c);
+      if (want_w) x = mx::packed(m, k, false, true, c);
+      if (want_x) w = mx::packed(n, k, false, true, c);
       // Dealt as if both were wanted: a gradient's sums do not depend on the other.
       const double wx = piece_work(m, k, n), ww = piece_work(n, k, m);
       to_x = plan_piece(m, k, n, wx / (wx + ww));
@@ -1157,7 +1208,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
   f.w.first.src = f.w.second.src = w;
   f.x.second.about = &f.head->a;
   f.w.second.about = &f.head->b;
-  ScanArgs scan{{f.x.first, f.w.first}, 2, activation, reinterpret_cast<int*>(f.head)};
+  ScanArgs scan{{f.x.first, f.w.first}, 2, activation};
   MX_TRY(run_scan<true>(&scan, s));
   PackArgs pack{};
   pack.count = 2;
@@ -1261,7 +1312,6 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   first.dz = b.dz;
   first.sums = !db ? nullptr : b.scan.parts > 1 ? b.part : db;
   if (b.packed) {
-    scan.head = reinterpret_cast<int*>(b.head);
     b.g.second.src = g;
     b.g.second.about = &b.head->a;
     PackArgs pack{};

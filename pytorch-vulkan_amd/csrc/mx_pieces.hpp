@@ -1,12 +1,14 @@
 // Products of FP32 matrices held as two fp16 pieces, on gfx950 matrix
 // instructions.
 //
-// A value x is kept as s x = hi + lo, hi the nearest fp16 of s x, lo the
-// nearest fp16 of what hi leaves, s a power of two chosen by the caller so that
-// no entry of the matrix passes fp16's largest.  hi + lo is off by at most
+// A value x is kept as s x = hi + 2^-r lo, hi the nearest fp16 of s x, lo the
+// nearest fp16 of 2^r times what hi leaves, s a power of two chosen by the caller
+// so that no entry of the matrix passes fp16's largest.  hi + lo is off by at most
 // 2^-23 of x (one FP32 place) while x is within 2^-17 of the largest entry that
-// s allows for, and by at most 2^-40 of that entry below it.  A product is
-// hi hi + hi lo + lo hi in FP32 accumulators; lo lo is below 2^-22 of a term.
+// s allows for, and by at most 2^-40 of that entry below it; with r = 12
+// (kRaised), which keeps lo from fp16's subnormals for as long as hi, within 2^-28
+// and by 2^-51.  A product is hi hi + hi lo + lo hi in FP32 accumulators, the last
+// two in one of their own where lo is raised; lo lo is below 2^-22 of a term.
 // Against six products of three bf16 pieces this halves the matrix
 // instructions and two thirds of the operands' bytes, and it needs what those
 // do not: a bound on the entries.
@@ -36,6 +38,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBK = 16;  // columns of a slab: one step of the matrix instruction
+// r of raised lo pieces: what hi leaves of entries below 2^15 is at most 2^3.
+constexpr int kRaised = 12;
 
 // Planes of a matrix: hi at `at`, lo `plane` elements behind.
 struct Planes {
@@ -172,13 +176,14 @@ __device__ __forceinline__ void barrier() {
 // columns) n0 + 32 j.. of B over nk slabs from slab0 (nk a multiple of four, at least four).  The matrix instruction's
 // row operand is B, so that a lane ends with four consecutive columns n of one
 // row m, 8 bytes of a plane (ROW_LANES: A, and it ends with four rows of one
-// column, neighbours beside it).
+// column, neighbours beside it).  RAISE: r of both operands' lo.
 //
 // Slab t's products run from registers while slab t + 1's fragments are read
 // from LDS and slabs t + 2 and t + 3 come from memory, one barrier a slab.
-template <class T, bool A_COLS, bool B_COLS, bool ROW_LANES = false>
+template <class T, bool A_COLS, bool B_COLS, bool ROW_LANES = false, int RAISE = 0>
 __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Planes& a, const Planes& b, int m0, int n0,
                                         int slab0, int nk, char* smem) {
+  static_assert(RAISE == 0 || T::DUAL, "raised products need accumulators of their own");
   using OpA = Operand<T::BM, T::LA, T::WAVES, A_COLS>;
   using OpB = Operand<T::BN, T::LB, T::WAVES, B_COLS>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -307,7 +312,7 @@ __device__ __forceinline__ void product(f32x16 (&acc)[T::FM][T::FN], const Plane
 #pragma unroll
     for (int i = 0; i < T::FM; ++i)
 #pragma unroll
-      for (int j = 0; j < T::FN; ++j) acc[i][j] += low[i][j];
+      for (int j = 0; j < T::FN; ++j) acc[i][j] += RAISE ? low[i][j] * (1.f / float(1 << RAISE)) : low[i][j];
   }
 }
 

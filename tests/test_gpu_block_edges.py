@@ -143,3 +143,66 @@ def test_layer_norm_backward_over_an_input(mx, rows, cols, which):
         g, b = torch.empty_like(dg), torch.empty_like(db)
         mx.layer_norm_backward(t["dy"], t["x"], mean, rstd, gamma, t[which], g, b, stream=stream())
         assert torch.equal(t[which], dx) and torch.equal(g, dg) and torch.equal(b, db)
+
+
+# -------------------------------------------------------------------- linear
+F = torch.nn.functional
+
+
+def check_products(mx, x, w, dy, what):
+    """Every product within what FP32 products of whole operands are off by: 8 u of
+    a term's roundings and dropped pieces, u of the sum every 8 terms."""
+    m, k, n = *x.shape, w.shape[0]
+    y, dx, dw = torch.empty(m, n, device="cuda"), torch.empty(m, k, device="cuda"), torch.empty(n, k, device="cuda")
+    mx.linear_forward(x, w, None, y, stream=stream())
+    mx.linear_backward(dy, x, w, None, dx, dw, None, stream=stream())
+    d = lambda t: t.double()
+    within(y, d(x) @ d(w).t(), (k / 8 + 8) * U * (d(x).abs() @ d(w).abs().t()) + 1e-44, what + " y")
+    within(dx, d(dy) @ d(w), (n / 8 + 8) * U * (d(dy).abs() @ d(w).abs()) + 1e-44, what + " dx")
+    within(dw, d(dy).t() @ d(x), (m / 8 + 8) * U * (d(dy).abs().t() @ d(x).abs()) + 1e-44, what + " dw")
+
+
+def activations(g, kind, *shape):
+    return {"silu": lambda: F.silu(rand(g, *shape, scale=6.0)), "gelu": lambda: F.gelu(rand(g, *shape, scale=2.0)),
+            "squared relu": lambda: F.relu(rand(g, *shape)) ** 2, "cubes": lambda: rand(g, *shape) ** 9,
+            "subnormal": lambda: rand(g, *shape).index_put_((torch.tensor([3], device="cuda"),), torch.tensor(1e-41, device="cuda"))}[kind]()
+
+
+def weights(g, kind, n, k):
+    if kind == "identity":
+        return torch.eye(n, k, device="cuda")
+    if kind == "dense":
+        return rand(g, n, k, scale=k ** -0.5)
+    w = torch.zeros(n, k, device="cuda")  # one or four nonzero elements a row
+    for _ in range(1 if kind == "one a row" else 4):
+        w[torch.arange(n, device="cuda"), torch.randint(k, (n,), device="cuda", generator=g)] = rand(g, n)
+    return w
+
+
+@pytest.mark.parametrize("m,k,n", [(2048, 2048, 2048), (1537, 1025, 2050)])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "squared relu", "cubes", "subnormal"])
+@pytest.mark.parametrize("weight", ["identity", "one a row", "four a row", "dense"])
+def test_linear_elements_far_below_the_largest(mx, m, k, n, kind, weight):
+    """Elements far below their operand's largest, alone or nearly alone in a sum."""
+    print("far below", m, k, n, kind, weight, flush=True)
+    g = gen(m + len(kind))
+    x, w = activations(g, kind, m, k), weights(g, weight, n, k)
+    check_products(mx, x, w, activations(g, kind, m, n), f"{kind} {weight}")
+    # Either operand's, and those of a sparse gradient.
+    check_products(mx, rand(g, m, k), activations(g, kind, n, k), weights(g, weight, m, n), f"{kind} {weight} turned")
+
+
+@pytest.mark.parametrize("depth", [20, 24, 28, 30, 34, 40, 60])
+def test_linear_sums_of_small_elements_alone(mx, depth):
+    """Quarters of x far below the others, met by those columns of w that are not zero."""
+    print("checkerboard", depth, flush=True)
+    m, k, n = 2048, 1024, 2048
+    g = gen(depth)
+    upper = lambda c: torch.arange(c, device="cuda") < c // 2
+    even = lambda c: torch.arange(c, device="cuda") % 2 == 0
+    board = lambda r, c, low: torch.where(even(r)[:, None] == upper(c)[None], 1.0, low)
+    x = rand(g, m, k) * board(m, k, 2.0 ** -depth)
+    w = rand(g, n, k) * board(n, k, 0.0)
+    dy = rand(g, m, n) * board(m, n, 2.0 ** -depth)
+    check_products(mx, x, w, dy, f"checkerboard {depth}")
+    check_products(mx, x * 2.0 ** 40, w, dy * board(m, n, 0.0), f"checkerboard {depth}, half of dy")
