@@ -13,11 +13,17 @@
 namespace mx {
 
 constexpr float kInvSqrt2Pi = 0.39894228040143268f, kLog2E = 1.44269504088896341f;
+constexpr float kLog2ELow = 1.92596299e-8f, kLn2 = 0.69314718055994531f;  // kLog2E + kLog2ELow = log2(e) to 48 bits
 constexpr float kSqrt2OverPi = 0.79788456080286536f, kTanhCubic = 0.044715f;
 
-// 1 / (1 + e^-v): 0 and 1 at the infinities.
+// 1 / (1 + e^-v): 0 and 1 at the infinities.  The rounding of log2(e) v and log2(e)'s
+// own are up to 2^-24 of it each, so that e^-v alone would be off by 31 u of itself
+// at v = -40 (u = 2^-24): what they leave out, r, comes back as the factor 1 + r ln 2.
+// Where log2(e) v is infinite so is r, or NaN, and the plain exp2 is the result.
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2E * v));
+  const float t = -kLog2E * v, r = fmaf(-kLog2ELow, v, fmaf(-kLog2E, v, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return __builtin_amdgcn_rcpf(1.f + (fabsf(t) < 128.f ? fmaf(e, r * kLn2, e) : e));
 }
 
 // Normal distribution's integral from -inf to z; density gets e^(-z^2 / 2).

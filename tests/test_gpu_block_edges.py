@@ -206,3 +206,25 @@ def test_linear_sums_of_small_elements_alone(mx, depth):
     dy = rand(g, m, n) * board(m, n, 2.0 ** -depth)
     check_products(mx, x, w, dy, f"checkerboard {depth}")
     check_products(mx, x * 2.0 ** 40, w, dy * board(m, n, 0.0), f"checkerboard {depth}, half of dy")
+
+
+def test_linear_silu_tails(mx):
+    """Relative to the value itself: exp2 and the reciprocal are good to 2 u each,
+    and four roundings make it 8 u; results of less than 2^-126 may go to zero.  An
+    identity weight, so that z is the input's own value."""
+    z = torch.cat([-torch.linspace(2.0 ** -10, 100, 6000, device="cuda"), torch.linspace(0, 100, 2000, device="cuda"),
+                   torch.tensor([-1e4, -3e38, 3e38, 200.0], device="cuda")]).view(-1, 4)
+    eye, y, kept = torch.eye(4, device="cuda"), torch.empty_like(z), torch.empty_like(z)
+    mx.linear_forward(z, eye, None, y, activation=mx.ACT_SILU, z=kept, stream=stream())
+    assert torch.equal(kept, z)
+    v = z.double()
+    s = torch.sigmoid(v)
+    small = 2.0 ** -126 * (v.abs() + 1)
+    within(y, v * s, 8 * U * (v * s).abs() + small, "y")
+    # s (1 + z (1 - s)): s to 7 u, 1 - s to u + 7 u s, the product and the sum to u each.
+    dx = torch.empty_like(z)
+    mx.linear_backward(torch.ones_like(z), z, eye, z, dx, None, None, activation=mx.ACT_SILU, stream=stream())
+    inner = v * (1 - s)
+    want = s * (1 + inner)
+    bound = U * s * (9 * (1 + inner).abs() + v.abs() * (1 + 7 * s) + inner.abs() + 1) + 2.0 ** -126 * (v.abs() + 1) ** 2
+    within(dx, want, bound, "slope")
