@@ -27,10 +27,11 @@ __device__ __forceinline__ float sigmoid(float v) {
 }
 
 // Normal distribution's integral from -inf to z; density gets e^(-z^2 / 2).
-// The tail beyond |z| is density t P(t) / 2 with t = 1 / (1 + 0.3 |z| / sqrt 2)
-// and P the degree 8 polynomial nearest to erfcx / t in relative error on
-// |z| < 20 (least squares reweighted towards the largest error: 3.9e-8); in
-// FP32 the whole is within 2.2e-7, and a lower tail keeps its own accuracy.
+// The tail beyond |z| is density t P(t) with t = 1 / (1 + 0.3 |z| / sqrt 2) and P
+// the degree 8 polynomial nearest to erfcx / (2 t) in relative error on |z| < 20
+// (least squares reweighted towards the largest error, which is 6.0e-8, at 0); in
+// FP32 the whole is within 2.4e-7, and a lower tail within 11 u of itself down to
+// z = -3, from where the rounding of z^2 grows on it (32 u at -6; u = 2^-24).
 __device__ __forceinline__ float normal_cdf(float z, float& density) {
   density = __builtin_amdgcn_exp2f(-0.5f * kLog2E * z * z);
   const float t = __builtin_amdgcn_rcpf(fmaf(0.21213203435596426f, fabsf(z), 1.f));
