@@ -18,9 +18,7 @@ ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        # The activation's input is kept only where a gradient will ask for it.
-        keep = activation != "none" and any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, bias, residual, activation, keep):
         y, z = torch.ops.torch_vulkan.linear_act(x, weight, bias, residual, activation, keep)
         ctx.activation = activation
         ctx.save_for_backward(x, weight, z if keep else None)
@@ -35,7 +33,7 @@ class _Linear(torch.autograd.Function):
         if any(want[:3]):
             got = torch.ops.torch_vulkan.linear_act_backward(dy, x, weight, z, ctx.activation, list(want[:3]))
             dx, dw, db = (g if w else None for g, w in zip(got, want))
-        return dx, dw, db, dy if want[3] else None, None
+        return dx, dw, db, dy if want[3] else None, None, None
 
 
 def linear(x, weight, bias=None, activation="none", residual=None):
@@ -49,7 +47,12 @@ def linear(x, weight, bias=None, activation="none", residual=None):
     flat = x.reshape(math.prod(shape[:-1]), x.shape[-1])
     if residual is not None:
         residual = residual.expand(shape).reshape(flat.shape[0], shape[-1])
-    return _Linear.apply(flat, weight, bias, residual, activation).view(shape)
+    # The activation's input is kept only where a gradient will ask for it.  Within
+    # the function a parameter needs its gradient under no_grad too, and the mode is
+    # off whatever the caller's.
+    keep = activation != "none" and torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (flat, weight, bias))
+    return _Linear.apply(flat, weight, bias, residual, activation, keep).view(shape)
 
 
 class Linear(torch.nn.Linear):
