@@ -68,6 +68,19 @@ struct Head {
 // of zeros.
 typedef unsigned long long Large;
 
+// Those of an operand's rows, or columns.  Each is the sum of `reps` words `len`
+// apart, to which the workgroups along it add in turn, up to 64 of them to a word (a
+// packed backward of 200000 x 129 -> 129, deep operands: 750 us, all to one 851).
+// A list of more than kListed words is gone over by a launch of its own, which leaves
+// the products kListEnds of them (by every workgroup of the products: 893 us there; for
+// 65536 rows of 512 500 either way, for 16384 of 1030 168 with it and 164 without).
+struct Counts {
+  Large* at;  // null where no product asks
+  int len, reps;
+  Large* ends;  // of a long list
+};
+constexpr int kListed = 65536, kListEnds = 64;
+
 // One operand's first pass: where `z` is not null src is dy and the values are
 // dz = dy act'(z), written to dz.  Column sums to sums[part][n] where that is
 // not null; with ENDS the largest magnitude (as bits: NaN counts above infinity)
@@ -79,7 +92,7 @@ struct ScanOp {
   float* dz;
   float* sums;
   uint2* ends;
-  Large *row_large, *col_large;  // null where no product asks
+  Counts rows, columns;
   int64_t m;
   int n;
   int64_t rows_per;
@@ -174,10 +187,13 @@ __global__ __launch_bounds__(256) void scan_kernel(ScanArgs p) {
     }
   }
   if constexpr (ENDS) {
-    if (o.row_large && bx == 0)
-      for (int64_t r = r0 + threadIdx.x; r < r1; r += 256) o.row_large[r] = 0;
-    if (o.col_large && by == 0 && threadIdx.x < 64 * W && int64_t(bx) * 64 * W + threadIdx.x < n)
-      o.col_large[int64_t(bx) * 64 * W + threadIdx.x] = 0;
+    const auto clear = [](const Counts& c, int64_t i) {
+      for (int rep = 0; rep < c.reps; ++rep) c.at[int64_t(rep) * c.len + i] = 0;
+    };
+    if (o.rows.at && bx == 0)
+      for (int64_t r = r0 + threadIdx.x; r < r1; r += 256) clear(o.rows, r);
+    if (o.columns.at && by == 0 && threadIdx.x < 64 * W && int64_t(bx) * 64 * W + threadIdx.x < n)
+      clear(o.columns, int64_t(bx) * 64 * W + threadIdx.x);
   }
   if (!o.sums && !ENDS) return;
   sums[threadIdx.x] = s;
@@ -211,7 +227,7 @@ struct PackOp {
   pieces::Planes to;
   const uint2* ends;
   int blocks;  // of the first pass
-  Large *row_large, *col_large;
+  Counts rows, columns;
   About* about;
   int wide;   // workgroups along a row
   int first;  // first workgroup
@@ -302,7 +318,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     const bool is = fabsf(f) >= 1.f;
     large += is;
     some |= v[q] != 0.f;
-    if (o.col_large) {
+    if (o.columns.at) {
       // Half a wave holds 32 rows of a column: their count to the half's lane q.
       const uint64_t which = __ballot(is);
       asm("v_writelane_b32 %0, %1, %2" : "+v"(column) : "s"(__popc(uint32_t(which))), "i"(q));
@@ -310,8 +326,9 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     }
   }
   const int at = col + (tid & 31);
-  if (o.col_large && (tid & 31) < 8 && at < o.n) atomicAdd(o.col_large + at, Large(1) << 32 | uint32_t(column));
-  if (o.row_large) {
+  if (o.columns.at && (tid & 31) < 8 && at < o.n)
+    atomicAdd(o.columns.at + int64_t(by % o.columns.reps) * o.n + at, Large(1) << 32 | uint32_t(column));
+  if (o.rows.at) {
     // The row's eight groups of eight: two to a wave.
     large |= int(some) << 16;
     large += __shfl_xor(large, 32, 64);
@@ -319,7 +336,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     __syncthreads();
     if (tid < 32 && row < o.m) {
       large = (found[0][tid] + found[1][tid]) + (found[2][tid] + found[3][tid]);
-      if (large) atomicAdd(o.row_large + row, Large(large >> 16) << 32 | (large & 0xFFFF));
+      if (large)
+        atomicAdd(o.rows.at + int64_t(bx % o.rows.reps) * o.m + row, Large(large >> 16) << 32 | (large & 0xFFFF));
     }
   }
   _Float16* const to = o.to.at + (int64_t(col >> 3) * o.to.rows + row) * 8;
@@ -334,7 +352,7 @@ struct PieceArgs {
   int nk, tiles_m, tiles_n;
   pieces::Shares share;
   const About *ea, *eb;
-  const Large *large_a, *large_b;  // of a's rows m and b's rows n (columns where the product runs along them)
+  Counts large_a, large_b;  // of a's and b's rows (columns where the product runs along them)
   int* left;
   int m, n, k;
   float* out;
@@ -392,18 +410,34 @@ struct PieceLaunch {
   bool swapped;  // p[1] goes first
 };
 
-// A thread's least count of `count` rows that are not zero, eight loads on their way
-// together; negative, as in the first pass, of one more (0: there is none).
-__device__ __forceinline__ uint32_t least_large(const Large* of, int count) {
+// The least of counts [first, first + step, ...) of rows that are not zero, eight on
+// their way together; negative, as in the first pass, of one more (0: there is none).
+__device__ __forceinline__ uint32_t least_large(const Counts& of, int first, int step) {
   uint32_t low = 0;
-  for (int i = threadIdx.x; i < count; i += 8 * blockDim.x) {
-    Large c[8];
+  for (int i = first; i < of.len; i += 8 * step) {
+    Large c[8] = {};
+    for (int rep = 0; rep < of.reps; ++rep)
 #pragma unroll
-    for (int u = 0; u < 8; ++u) c[u] = of[min(i + u * int(blockDim.x), count - 1)];
+      for (int u = 0; u < 8; ++u) c[u] += of.at[int64_t(rep) * of.len + min(int64_t(i) + u * int64_t(step), int64_t(of.len - 1))];
 #pragma unroll
     for (int u = 0; u < 8; ++u) low = max(low, c[u] ? 0u - (uint32_t(c[u]) + 1) : 0u);
   }
   return low;
+}
+
+// Long lists' least counts, kListEnds workgroups to each.
+struct ListArgs {
+  Counts of[4];
+};
+__global__ __launch_bounds__(256) void list_kernel(ListArgs p) {
+  __shared__ uint32_t low[4];
+  const Counts& c = p.of[blockIdx.y];
+  const uint32_t l = wave_top(least_large(c, blockIdx.x * 256 + threadIdx.x, kListEnds * 256));
+  if ((threadIdx.x & 63) == 63) low[threadIdx.x >> 6] = l;
+  __syncthreads();
+  if (threadIdx.x) return;
+  const uint32_t all = max(max(low[0], low[1]), max(low[2], low[3]));
+  c.ends[blockIdx.x] = all ? Large(1) << 32 | (0u - all - 1) : 0;
 }
 
 // Whether the product is left to mx_gemm.hip's kernels.
@@ -412,7 +446,7 @@ __device__ __forceinline__ bool left_out(const PieceArgs& p, const About& ea, co
   if (deepest >= kMisfit) return true;
   if (deepest <= max(28, 23 + 31 - __clz(p.k))) return false;
   uint2* const lds = reinterpret_cast<uint2*>(smem);
-  uint2 low = {least_large(p.large_a, p.m), least_large(p.large_b, p.n)};
+  uint2 low = {least_large(p.large_a, threadIdx.x, blockDim.x), least_large(p.large_b, threadIdx.x, blockDim.x)};
   low = {wave_top(low.x), wave_top(low.y)};
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = low;
   __syncthreads();
@@ -854,6 +888,16 @@ struct Packed {
   PackOp second;
 };
 
+// groups: of a row's elements, as many workgroups of the second pass.
+Counts counts_of(int64_t len, int64_t groups, Carve* c) {
+  Counts o{};
+  o.len = int(len);
+  o.reps = int(std::clamp<int64_t>(len > kListed ? 16 : kListed / len, 1, (groups + 63) / 64));
+  o.at = c->take<Large>(len * o.reps);
+  if (len > kListed) o.ends = c->take<Large>(kListEnds);
+  return o;
+}
+
 // by_rows, by_cols: products run along its rows, its columns.
 Packed packed(int64_t m, int64_t n, bool by_rows, bool by_cols, Carve* c) {
   Packed o{};
@@ -867,15 +911,15 @@ Packed packed(int64_t m, int64_t n, bool by_rows, bool by_cols, Carve* c) {
   o.first.col_blocks = o.scan.col_blocks;
   o.first.parts = o.scan.parts;
   o.first.ends = c->take<uint2>(o.scan.blocks());
-  o.first.row_large = by_rows ? c->take<Large>(m) : nullptr;
-  o.first.col_large = by_cols ? c->take<Large>(n) : nullptr;
+  if (by_rows) o.first.rows = counts_of(m, np / 64, c);
+  if (by_cols) o.first.columns = counts_of(n, mp / 32, c);
   o.second.m = int(m);
   o.second.n = int(n);
   o.second.to = {c->take<_Float16>(2 * mp * np), mp * np, int(mp)};
   o.second.ends = o.first.ends;
   o.second.blocks = o.scan.blocks();
-  o.second.row_large = o.first.row_large;
-  o.second.col_large = o.first.col_large;
+  o.second.rows = o.first.rows;
+  o.second.columns = o.first.columns;
   o.second.wide = int(np / 64);
   return o;
 }
@@ -946,8 +990,9 @@ void fill_piece(PieceArgs* p, const pieces::Deal& d, const Packed& a, bool a_col
   p->b = b.second.to;
   p->ea = a.second.about;
   p->eb = b.second.about;
-  p->large_a = a_cols ? a.second.col_large : a.second.row_large;
-  p->large_b = b_cols ? b.second.col_large : b.second.row_large;
+  const auto listed = [](const Counts& c) { return c.ends ? Counts{c.ends, kListEnds, 1, nullptr} : c; };
+  p->large_a = listed(a_cols ? a.second.columns : a.second.rows);
+  p->large_b = listed(b_cols ? b.second.columns : b.second.rows);
   p->left = left;
   p->m = int(a_cols ? a.n : a.m);
   p->n = int(b_cols ? b.n : b.m);
@@ -1013,6 +1058,14 @@ int run_pack(PackArgs* p, hipStream_t s) {
   p->first_sum = blocks;
   if (p->out) blocks += (p->n + 31) / 32;
   hipLaunchKernelGGL(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, *p);
+  MX_HIP(hipGetLastError());
+  ListArgs lists{};
+  int count = 0;
+  for (int i = 0; i < p->count; ++i)
+    for (const Counts* c : {&p->op[i].rows, &p->op[i].columns})
+      if (c->ends) lists.of[count++] = *c;
+  if (!count) return MX_OK;
+  hipLaunchKernelGGL(list_kernel, dim3(kListEnds, unsigned(count)), dim3(256), 0, s, lists);
   MX_HIP(hipGetLastError());
   return MX_OK;
 }

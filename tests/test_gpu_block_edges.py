@@ -228,3 +228,17 @@ def test_linear_silu_tails(mx):
     want = s * (1 + inner)
     bound = U * s * (9 * (1 + inner).abs() + v.abs() * (1 + 7 * s) + inner.abs() + 1) + 2.0 ** -126 * (v.abs() + 1) ** 2
     within(dx, want, bound, "slope")
+
+
+@pytest.mark.parametrize("m,k,n", [(9000, 300, 1030), (70000, 514, 520), (200, 4096, 70000)])
+def test_linear_far_below_in_long_lists(mx, m, k, n):
+    """Rows and columns whose counts are in several words, and in lists of more than
+    65536; weights that cover the small elements, and weights that do not."""
+    print("long lists", m, k, n, flush=True)
+    g = gen(m)
+    x, dy = F.gelu(rand(g, m, k, scale=2.0)), F.gelu(rand(g, m, n, scale=2.0))
+    check_products(mx, x, rand(g, n, k, scale=k ** -0.5), dy, "dense")
+    # One column of w alone meets x's, one row of it dy's.
+    w = torch.zeros(n, k, device="cuda")
+    w[:, 7], w[11] = rand(g, n), rand(g, k)
+    check_products(mx, x, w, dy, "one column and row")
