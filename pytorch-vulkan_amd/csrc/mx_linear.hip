@@ -64,22 +64,23 @@ struct Head {
   int left[2];
 };
 
-// Large elements of a row or a column in the low word; the high one is zero for a row
-// of zeros.
-typedef unsigned long long Large;
+// Large elements of a row or a column: for each group of its elements (as many as a
+// workgroup of the second pass holds) theirs and 1.  A row's groups of zeros add
+// nothing, which tells rows of zeros (masked tokens) from others.
+typedef uint32_t Large;
 
 // Those of an operand's rows, or columns.  Each is the sum of `reps` words `len`
-// apart, to which the workgroups along it add in turn, up to 64 of them to a word (a
-// packed backward of 200000 x 129 -> 129, deep operands: 750 us, all to one 851).
-// A list of more than kListed words is gone over by a launch of its own, which leaves
-// the products kListEnds of them (by every workgroup of the products: 893 us there; for
-// 65536 rows of 512 500 either way, for 16384 of 1030 168 with it and 164 without).
+// apart, to which its groups add in turn, up to kAdds of them to a word (a packed
+// backward of 200000 x 129 -> 129, deep operands: 747 us, all to one 817; 100000 x 256
+// -> 512 561 and 592; 64 or 256 to a word the same as 128).  A list of more than kListed
+// words is gone over by a launch of its own, which leaves the products kListEnds of
+// them (by every workgroup of the products: 844 and 600 us).
 struct Counts {
   Large* at;  // null where no product asks
-  int len, reps;
+  int len, reps, groups;
   Large* ends;  // of a long list
 };
-constexpr int kListed = 65536, kListEnds = 64;
+constexpr int kAdds = 128, kListed = 65536, kListEnds = 64;
 
 // One operand's first pass: where `z` is not null src is dy and the values are
 // dz = dy act'(z), written to dz.  Column sums to sums[part][n] where that is
@@ -327,7 +328,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
   }
   const int at = col + (tid & 31);
   if (o.columns.at && (tid & 31) < 8 && at < o.n)
-    atomicAdd(o.columns.at + int64_t(by % o.columns.reps) * o.n + at, Large(1) << 32 | uint32_t(column));
+    atomicAdd(o.columns.at + int64_t(by % o.columns.reps) * o.n + at, Large(column) + 1);
   if (o.rows.at) {
     // The row's eight groups of eight: two to a wave.
     large |= int(some) << 16;
@@ -336,8 +337,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs p) {
     __syncthreads();
     if (tid < 32 && row < o.m) {
       large = (found[0][tid] + found[1][tid]) + (found[2][tid] + found[3][tid]);
-      if (large)
-        atomicAdd(o.rows.at + int64_t(bx % o.rows.reps) * o.m + row, Large(large >> 16) << 32 | (large & 0xFFFF));
+      if (large) atomicAdd(o.rows.at + int64_t(bx % o.rows.reps) * o.m + row, Large(large & 0xFFFF) + 1);
     }
   }
   _Float16* const to = o.to.at + (int64_t(col >> 3) * o.to.rows + row) * 8;
@@ -410,8 +410,8 @@ struct PieceLaunch {
   bool swapped;  // p[1] goes first
 };
 
-// The least of counts [first, first + step, ...) of rows that are not zero, eight on
-// their way together; negative, as in the first pass, of one more (0: there is none).
+// The least of words [first, first + step, ...) that are not zero, eight on their way
+// together; negative, as in the first pass (0: there is none).
 __device__ __forceinline__ uint32_t least_large(const Counts& of, int first, int step) {
   uint32_t low = 0;
   for (int i = first; i < of.len; i += 8 * step) {
@@ -420,12 +420,12 @@ __device__ __forceinline__ uint32_t least_large(const Counts& of, int first, int
 #pragma unroll
       for (int u = 0; u < 8; ++u) c[u] += of.at[int64_t(rep) * of.len + min(int64_t(i) + u * int64_t(step), int64_t(of.len - 1))];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) low = max(low, c[u] ? 0u - (uint32_t(c[u]) + 1) : 0u);
+    for (int u = 0; u < 8; ++u) low = max(low, 0u - c[u]);
   }
   return low;
 }
 
-// Long lists' least counts, kListEnds workgroups to each.
+// Long lists' least words, kListEnds workgroups to each.
 struct ListArgs {
   Counts of[4];
 };
@@ -435,9 +435,7 @@ __global__ __launch_bounds__(256) void list_kernel(ListArgs p) {
   const uint32_t l = wave_top(least_large(c, blockIdx.x * 256 + threadIdx.x, kListEnds * 256));
   if ((threadIdx.x & 63) == 63) low[threadIdx.x >> 6] = l;
   __syncthreads();
-  if (threadIdx.x) return;
-  const uint32_t all = max(max(low[0], low[1]), max(low[2], low[3]));
-  c.ends[blockIdx.x] = all ? Large(1) << 32 | (0u - all - 1) : 0;
+  if (threadIdx.x == 0) c.ends[blockIdx.x] = 0u - max(max(low[0], low[1]), max(low[2], low[3]));
 }
 
 // Whether the product is left to mx_gemm.hip's kernels.
@@ -453,8 +451,9 @@ __device__ __forceinline__ bool left_out(const PieceArgs& p, const About& ea, co
   low = lds[0];
   for (int w = 1; w < int(blockDim.x >> 6); ++w) low = {max(low.x, lds[w].x), max(low.y, lds[w].y)};
   __syncthreads();
-  const auto count = [](uint32_t v) { return v ? uint64_t(0u - v) - 1 : uint64_t(1) << 32; };
-  return count(low.x) + count(low.y) < uint64_t(p.k) + kShared;
+  // Without the groups' own; rows of zeros have nothing to cover.
+  const auto count = [](uint32_t v, int groups) { return v ? max(int64_t(0u - v) - groups, int64_t(0)) : int64_t(1) << 32; };
+  return count(low.x, p.large_a.groups) + count(low.y, p.large_b.groups) < int64_t(p.k) + kShared;
 }
 
 template <class T, bool A_COLS, bool B_COLS, bool EPI>
@@ -888,11 +887,11 @@ struct Packed {
   PackOp second;
 };
 
-// groups: of a row's elements, as many workgroups of the second pass.
 Counts counts_of(int64_t len, int64_t groups, Carve* c) {
   Counts o{};
   o.len = int(len);
-  o.reps = int(std::clamp<int64_t>(len > kListed ? 16 : kListed / len, 1, (groups + 63) / 64));
+  o.groups = int(groups);
+  o.reps = int(std::clamp<int64_t>(len > kListed ? 16 : kListed / len, 1, (groups + kAdds - 1) / kAdds));
   o.at = c->take<Large>(len * o.reps);
   if (len > kListed) o.ends = c->take<Large>(kListEnds);
   return o;
@@ -990,7 +989,7 @@ void fill_piece(PieceArgs* p, const pieces::Deal& d, const Packed& a, bool a_col
   p->b = b.second.to;
   p->ea = a.second.about;
   p->eb = b.second.about;
-  const auto listed = [](const Counts& c) { return c.ends ? Counts{c.ends, kListEnds, 1, nullptr} : c; };
+  const auto listed = [](const Counts& c) { return c.ends ? Counts{c.ends, kListEnds, 1, c.groups, nullptr} : c; };
   p->large_a = listed(a_cols ? a.second.columns : a.second.rows);
   p->large_b = listed(b_cols ? b.second.columns : b.second.rows);
   p->left = left;
