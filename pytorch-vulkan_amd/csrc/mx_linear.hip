@@ -923,8 +923,9 @@ Packed packed(int64_t m, int64_t n, bool by_rows, bool by_cols, Carve* c) {
   return o;
 }
 
-// Largest packed scratch of a call.
-constexpr int64_t kMostPacked = int64_t(4) << 30;
+// Most that a call's packed operands (and dz with them) may take: 3 % of the card's
+// memory.
+constexpr double kMostPacked = 8.0 * (int64_t(1) << 30);
 
 // How a call's products run: as mx_gemm.hip's tiles, as small ones without
 // staging, on packed operands, or (a forward) as a few tokens.
@@ -932,20 +933,24 @@ enum class Form { kTiles, kSmall, kPacked, kFew };
 
 // The form whose time is least, each as fitted to measurements of 113 shapes from
 // 17 to 8192 rows and 48 to 4096 columns (which take 1.6 % longer so than with the
-// best form of each).  Microseconds, tiles / small / packed, with GELU:
+// best form of each), packed ones on the sizes that they are padded to: of 37 backward
+// shapes, tall and narrow ones among them, the choice takes 1.3 % longer than the
+// best, 23 % at most (30000 x 384 -> 384 200 us packed, 162 in tiles); on their own
+// sizes 6.8 %, and 200000 x 129 -> 129, padded to 256, ran for 747 us, in tiles for 405.
+// Microseconds, tiles / small / packed, with GELU:
 //   m x k -> n            forward              backward
 //   17 x 512 -> 512       15 /   7 /  -         25 /  11 /  -
 //   512 x 512 -> 512      16 /   8 /  -         36 /  16 /  -
-//   700 x 700 -> 700      17 /  15 /  31        42 /  32 /  35
-//   64 x 4096 -> 4096     27 /  33 /  81        59 /  79 /  93
-//   8192 x 256 -> 1024    41 /  94 /  48       102 / 135 /  79
-//   1024 x 1024 -> 1024   27 /  35 /  43        61 /  59 /  39
-//   601 x 803 -> 1205     29 /  23 /  43        60 /  46 /  39   (rows not 16-byte aligned)
-//   1000 x 701 -> 1999    41 /  62 /  47        99 /  88 /  51   (the same)
-//   256 x 4096 -> 4096    61 / 118 /  99       121 / 201 / 119
-//   2048 x 2048 -> 2048  113 / 229 /  85       224 / 370 / 128
-//   8192 x 4096 -> 512   205 / 455 / 206       383 / 752 / 375
-//   4096 x 1024 -> 4096  216 /   - / 137       481 /   - / 257
+//   700 x 700 -> 700      17 /  15 /  29        42 /  32 /  34
+//   64 x 4096 -> 4096     27 /  38 /  80        60 /  79 /  88
+//   8192 x 256 -> 1024    42 /  94 /  46       103 / 135 /  96
+//   1024 x 1024 -> 1024   30 /  35 /  42        65 /  59 /  40
+//   601 x 803 -> 1205     30 /  23 /  42        60 /  46 /  39   (rows not 16-byte aligned)
+//   1000 x 701 -> 1999    39 /  62 /  46        96 /  88 /  52   (the same)
+//   256 x 4096 -> 4096    62 / 118 /  97       123 / 201 / 117
+//   2048 x 2048 -> 2048  114 / 229 /  82       228 / 370 / 133
+//   8192 x 4096 -> 512   203 / 455 / 204       395 / 752 / 395
+//   4096 x 1024 -> 4096  203 /   - / 128       438 /   - / 268
 // and a forward of few tokens, best of the others / few:
 //   m                     4           8           16          32          48
 //   64 -> 2000            3.7 / 3.5   3.9 / 3.6   4.0 / 4.7   4.2 / 7.2   4.2 / 9.6
@@ -961,18 +966,22 @@ Form form_of(int64_t m, int64_t k, int64_t n, bool backward) {
   const double out = 1e-6 * double(m) * double(n), sides = 1e-6 * double(k) * double(m + n), cu = cu_count();
   const double gflop = (backward ? 4e-3 : 2e-3) * out * double(k);
   const bool odd = k % 4 || (backward && n % 4);
+  // Packed operands are padded: 129 columns take 256.
+  const double mp = double(padded(m)), kp = double(padded(k)), np = double(padded(n));
+  const double out_p = 1e-6 * mp * np, sides_p = 1e-6 * kp * (mp + np), gflop_p = (backward ? 4e-3 : 2e-3) * out_p * kp;
   double tiles, small, packed;
   if (backward) {
     const double workgroups = up(m, 32) * up(k, 32) * up(n, 64) + up(n, 32) * up(k, 32) * up(m, 64);
     tiles = std::min(19.0 + 0.45 * up(std::min(m, n), 16), 32.0) + (odd ? 10.0 : 5.0) * gflop + 3.5 * out + 1.4 * sides;
     small = 9.5 + (odd ? 0.44 : 0.34) * std::max(up(std::max(m, n), 64), workgroups / cu) + 6.5 * out + 2.4 * sides;
-    packed = 26.0 + 1.9 * gflop + 3.4 * sides + 5.0 * out;
+    packed = 25.0 + 1.8 * gflop_p + 3.4 * sides_p + 5.0 * out_p;
   } else {
     tiles = std::min(6.0 + 0.23 * up(k, 16), 11.0) + (odd ? 10.8 : 5.7) * gflop + out + 0.7 * sides;
     small = 3.8 + (odd ? 0.165 : 0.11) * up(k, 16) * std::max(1.0, up(m, 32) * up(n, 32) / cu) + 3.4 * out;
-    packed = 26.5 + 2.0 * gflop + 2.7 * sides + 1.6 * out;
+    packed = 26.5 + 2.0 * gflop_p + 2.7 * sides_p + 1.6 * out_p;
   }
-  if (std::min({m, k, n}) < 4 || (out + sides) * 5e6 > double(kMostPacked)) packed = INFINITY;
+  const double scratch = 4e6 * (sides_p + (backward ? out_p + out : 0.0));
+  if (std::min({m, k, n}) < 4 || scratch > kMostPacked) packed = INFINITY;
   double few = INFINITY;
   const double groups = up(m, kFewTokens), turns = groups * up(n, kFewRows);
   if (!backward && m <= 64 && k >= 4 && turns <= 1 << 20)  // as measured, and what a grid holds
