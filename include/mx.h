@@ -533,7 +533,8 @@ enum mx_activation { MX_ACT_NONE = 0, MX_ACT_RELU = 1, MX_ACT_SILU = 2, MX_ACT_G
  * products hold an element of x, w and dz to 2^-23 of itself or 2^-51 of the
  * operand's largest; where a sum could show the latter (elements far below the
  * largest, without enough larger ones around them in both operands) they take
- * slower products that hold every element. */
+ * slower products that hold every element, and where the allocator has no room
+ * for their scratch, products that need none (the backward's: dz alone). */
 int mx_linear_forward(const float* x, const float* w, const float* bias, const float* residual, int64_t m, int64_t k,
                       int64_t n, int activation, float* y, float* z, void* workspace, int64_t workspace_bytes,
                       void* stream);

@@ -1174,8 +1174,9 @@ struct Backward {
   int64_t gemm = 0;
   void* split = nullptr;
   int status = MX_OK;
-  Backward(int64_t m, int64_t k, int64_t n, bool slope, bool want_x, bool want_w, bool want_b, bool split_room, Carve* c)
-      : packed((want_x || want_w) && form_of(m, k, n, true) == Form::kPacked), scan(plan_scan(m, n)) {
+  Backward(int64_t m, int64_t k, int64_t n, bool slope, bool want_x, bool want_w, bool want_b, bool split_room,
+           bool piece_room, Carve* c)
+      : packed(piece_room && (want_x || want_w) && form_of(m, k, n, true) == Form::kPacked), scan(plan_scan(m, n)) {
     if (slope && (want_x || want_w)) dz = c->take<float>(m * n);
     if (want_b && scan.parts > 1) part = c->take<float>(int64_t(scan.parts) * n);
     if (packed) {
@@ -1217,7 +1218,7 @@ extern "C" int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activati
     *bytes = c.used;
     return MX_OK;
   }
-  const Backward b(m, k, n, activation != MX_ACT_NONE, k > 0, k > 0, true, true, &c);
+  const Backward b(m, k, n, activation != MX_ACT_NONE, k > 0, k > 0, true, true, true, &c);
   *bytes = c.used;
   return b.status;
   MX_ABI_END
@@ -1262,7 +1263,12 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
     return gemm_within(&d, x, w, bias, y, kPartials, s, &epi, ws.as<void>());
   }
   MX_TRY(forward_bytes(m, k, n, &need));
-  MX_TRY(ws.take(who, workspace, workspace_bytes, need, s));
+  const int room = ws.take(who, workspace, workspace_bytes, need, s);
+  if (room == MX_ERR_OOM) {  // no room for pieces: tiles need none
+    clear_error();
+    return gemm_within(&d, x, w, bias, y, kPartials, s, &epi);
+  }
+  MX_TRY(room);
   Carve c(ws.as<void>());
   Forward f(m, k, n, &c);
   f.x.first.src = f.x.second.src = x;
@@ -1346,13 +1352,22 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   }
   // Without the caller's workspace the K splits of products that are not packed
   // are left to them (captured calls take one pass each).
-  Carve size(nullptr);
-  const Backward want(m, k, n, slope, dx, dw, db, workspace != nullptr, &size);
-  MX_TRY(want.status);
   Workspace ws;
-  MX_TRY(ws.take(who, workspace, workspace_bytes, size.used, s));
+  const auto take = [&](bool piece_room) -> int {
+    Carve size(nullptr);
+    const Backward want(m, k, n, slope, dx, dw, db, workspace != nullptr, piece_room, &size);
+    MX_TRY(want.status);
+    return ws.take(who, workspace, workspace_bytes, size.used, s);
+  };
+  int room_for = take(true);
+  const bool piece_room = room_for != MX_ERR_OOM;
+  if (!piece_room) {  // none for pieces: tiles need dz and its column sums alone
+    clear_error();
+    room_for = take(false);
+  }
+  MX_TRY(room_for);
   Carve c(ws.as<void>());
-  Backward b(m, k, n, slope, dx, dw, db, workspace != nullptr, &c);
+  Backward b(m, k, n, slope, dx, dw, db, workspace != nullptr, piece_room, &c);
   const float* const g = b.dz ? b.dz : dy;
   // First pass: dz, its column sums and, for packed products, everyone's largest.
   ScanArgs scan{};

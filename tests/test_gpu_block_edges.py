@@ -242,3 +242,61 @@ def test_linear_far_below_in_long_lists(mx, m, k, n):
     w = torch.zeros(n, k, device="cuda")
     w[:, 7], w[11] = rand(g, n), rand(g, k)
     check_products(mx, x, w, dy, "one column and row")
+
+
+def test_linear_without_room_for_pieces(mx):
+    """A card so full that packed operands (0.56 GiB for the backward, 0.06 forward) find
+    no room, while dz (0.25 GiB) does: the products without scratch take the call."""
+    m, k, n = 8192, 1024, 8192
+    g = gen(2)
+    x, w, dy, b = rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, m, n), rand(g, n)
+    y, z, dx, dw, db = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda"), torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+
+    def forward():
+        mx.linear_forward(x, w, b, y, activation=mx.ACT_GELU, residual=dy, z=z, stream=stream())
+
+    def backward():
+        mx.linear_backward(dy, x, w, z, dx, dw, db, activation=mx.ACT_GELU, stream=stream())
+
+    def release():
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        mx.check(mx.lib().mx_empty_cache())
+
+    assert mx.linear_workspace(m, k, n, mx.ACT_GELU) > 64 << 20 and mx.linear_workspace(m, k, n, mx.ACT_GELU, True) > 560 << 20
+    forward()
+    backward()
+    want = [t.clone() for t in (y, z, dx, dw, db)]
+    for t in (y, dx, dw, db):  # z is an argument of the backward, which runs first
+        t.fill_(float("nan"))
+    fillers = []
+
+    def fill(left):  # the driver finds a little more once most is taken
+        release()
+        for _ in range(8):
+            over = torch.cuda.mem_get_info()[0] - left
+            if over < 4 << 20:
+                break
+            fillers.append(torch.empty(over, dtype=torch.uint8, device="cuda"))
+        assert torch.cuda.mem_get_info()[0] <= left + (8 << 20)
+
+    try:
+        fill(400 << 20)
+        backward()
+        torch.cuda.synchronize()
+        fill(40 << 20)
+        forward()
+        torch.cuda.synchronize()
+    finally:
+        fillers.clear()
+        release()
+    # Both are within FP32's bound of the terms, so of each other within twice that.
+    mag = x.abs() @ w.abs().t() + b.abs()
+    z_err = 2 * (k / 8 + 8) * U * mag.double()
+    within(z, want[1].double(), z_err, "z")
+    within(y, want[0].double(), 1.13 * z_err + 32 * U * (want[1].double().abs() + 1) + 8 * U * want[0].double().abs(), "y")
+    dz_err = 32 * U * dy.double().abs() * (want[1].double().abs() + 1)
+    dz = (dy * 1.13).abs().double()
+    within(dx, want[2].double(), (2 * (n / 8 + 8) * U * dz + dz_err) @ w.double().abs(), "dx")
+    within(dw, want[3].double(), (2 * (m / 8 + 8) * U * dz + dz_err).t() @ x.double().abs(), "dw")
+    within(db, want[4].double(), (2 * (m / 64 + 64) * U * dz + dz_err).sum(0), "db")
