@@ -559,7 +559,8 @@ typedef struct mx_matrix_pair {
   float* out; /* may be `in` */
   int64_t rows, cols;
 } mx_matrix_pair;
-/* out[i] = that factor of in[i], matrices of one shape side by side. */
+/* out[i] = that factor of in[i], matrices of one shape side by side.  No out may
+ * overlap another matrix of the call but its own `in`, whole (MX_ERR_INVALID). */
 int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
                      int64_t workspace_bytes, void* stream);
 int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_t count, int64_t* bytes);
@@ -568,7 +569,8 @@ int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_t count, in
  *   buf += (1 - momentum) (grad - buf);  u = nesterov ? grad + momentum (buf - grad) : buf
  *   param = param (1 - lr weight_decay) - lr r orth(u),
  * r = sqrt(max(1, rows / cols)) (MX_MUON_ORIGINAL) or 0.2 sqrt(max(rows, cols))
- * (MX_MUON_MATCH_RMS_ADAMW).  Tensors are [rows, cols], no two of which may overlap. */
+ * (MX_MUON_MATCH_RMS_ADAMW).  Tensors are [rows, cols]; no param or momentum_buffer
+ * may overlap another tensor of the call (MX_ERR_INVALID). */
 enum mx_muon_adjust { MX_MUON_ORIGINAL = 0, MX_MUON_MATCH_RMS_ADAMW = 1 };
 typedef struct mx_muon_tensor {
   float* param;

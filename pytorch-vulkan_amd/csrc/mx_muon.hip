@@ -963,13 +963,39 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
   return MX_OK;
 }
 
+// Buffers of a call, which runs its matrices side by side and a set after the other:
+// what it writes may not overlap anything else of it.
+struct Buffer {
+  uintptr_t at, end;
+  int64_t matrix;
+  bool written;
+};
+void add(std::vector<Buffer>* list, const float* p, int64_t rows, int64_t cols, int64_t matrix, bool written) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  if (rows > 0 && cols > 0) list->push_back({at, at + uintptr_t(rows) * uintptr_t(cols) * sizeof(float), matrix, written});
+}
+int check_apart(const char* who, std::vector<Buffer>* list) {
+  std::sort(list->begin(), list->end(), [](const Buffer& a, const Buffer& b) { return a.at < b.at; });
+  // The one that reaches furthest of those before, of all and of the written ones.
+  const Buffer *any = nullptr, *out = nullptr;
+  for (const Buffer& b : *list) {
+    const Buffer* const over = b.written ? any : out;
+    MX_REQUIRE(!over || over->end <= b.at, MX_ERR_INVALID, who, ": a written tensor appears twice or overlaps another (matrices ",
+               over->matrix, " and ", b.matrix, ")");
+    if (!any || b.end > any->end) any = &b;
+    if (b.written && (!out || b.end > out->end)) out = &b;
+  }
+  return MX_OK;
+}
+
 template <class Fill>
-int run_all(const char* who, const std::vector<Set>& sets, const mx_newton_schulz& ns, const Finish& fin, void* workspace,
-            int64_t workspace_bytes, hipStream_t s, Fill&& fill) {
+int run_all(const char* who, const std::vector<Set>& sets, const mx_newton_schulz& ns, const Finish& fin, std::vector<Buffer>* buffers,
+            void* workspace, int64_t workspace_bytes, hipStream_t s, Fill&& fill) {
   std::vector<Scales> sc;
   MX_TRY(scales_of(who, ns, &sc));
   Workspace ws;
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_of(sets), s));
+  MX_TRY(check_apart(who, buffers));
   for (const Set& f : sets) {
     const int64_t batch = int64_t(f.at.size());
     Table tab{};
@@ -1018,7 +1044,13 @@ extern "C" int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, c
   for (int64_t i = 0; i < count; ++i)
     MX_REQUIRE(matrices[i].rows == 0 || matrices[i].cols == 0 || (matrices[i].in && matrices[i].out), MX_ERR_INVALID, who,
                ": null buffer at ", i);
-  return run_all(who, sets_of(matrices, count), *ns, Finish{}, workspace, workspace_bytes, resolve_stream(stream),
+  std::vector<Buffer> buffers;
+  for (int64_t i = 0; i < count; ++i) {
+    const mx_matrix_pair& t = matrices[i];
+    add(&buffers, t.out, t.rows, t.cols, i, true);
+    if (t.in != t.out) add(&buffers, t.in, t.rows, t.cols, i, false);
+  }
+  return run_all(who, sets_of(matrices, count), *ns, Finish{}, &buffers, workspace, workspace_bytes, resolve_stream(stream),
                  [&](int64_t i, Table* tab, int64_t at) {
                    tab->in[at] = matrices[i].in;
                    tab->out[at] = matrices[i].out;
@@ -1051,12 +1083,19 @@ extern "C" int mx_muon_step(const mx_muon_tensor* tensors, int64_t count, const 
     MX_REQUIRE(tensors[i].rows == 0 || tensors[i].cols == 0 ||
                    (tensors[i].param && tensors[i].grad && tensors[i].momentum_buffer),
                MX_ERR_INVALID, who, ": null buffer at ", i);
+  std::vector<Buffer> buffers;
+  for (int64_t i = 0; i < count; ++i) {
+    const mx_muon_tensor& t = tensors[i];
+    add(&buffers, t.param, t.rows, t.cols, i, true);
+    add(&buffers, t.momentum_buffer, t.rows, t.cols, i, true);
+    add(&buffers, t.grad, t.rows, t.cols, i, false);
+  }
   Finish fin{};
   fin.up = {1, hp->nesterov != 0, float(hp->momentum), float(1.0 - hp->momentum)};
   fin.lr = hp->lr;
   fin.decay = hp->weight_decay;
   fin.adjust = hp->adjust_lr;
-  return run_all(who, sets_of(tensors, count), hp->ns, fin, workspace, workspace_bytes, resolve_stream(stream),
+  return run_all(who, sets_of(tensors, count), hp->ns, fin, &buffers, workspace, workspace_bytes, resolve_stream(stream),
                  [&](int64_t i, Table* tab, int64_t at) {
                    tab->in[at] = tensors[i].grad;
                    tab->buf[at] = tensors[i].momentum_buffer;

@@ -10,7 +10,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
 
-#include <algorithm>
 #include <array>
 #include <optional>
 #include <tuple>
@@ -219,8 +218,6 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   c10::DeviceGuard guard(params[0].device());
   std::vector<at::Tensor> held;
   std::vector<mx_muon_tensor> tab;
-  // One table entry per written tensor: the library runs a list side by side.
-  std::vector<const void*> written;
   for (size_t i = 0; i < count; ++i) {
     const at::Tensor &p = params[i], &m = momentum_buffers[i];
     check_matrix(who, "param", i, p, p);
@@ -230,13 +227,8 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
     TORCH_CHECK(p.is_contiguous() && m.is_contiguous(), who, ": parameters and momentum buffers must be contiguous (", i, ")");
     held.push_back(packed(grads[i]));
     if (p.numel() == 0) continue;
-    written.push_back(p.data_ptr());
-    written.push_back(m.data_ptr());
     tab.push_back({ptr(p), cptr(held.back()), ptr(m), p.size(0), p.size(1)});
   }
-  std::sort(written.begin(), written.end());
-  TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(),
-              "muon_step_: a parameter or momentum buffer appears twice");
   GpuTimer timer(gpu_timing_enabled() ? "muon_step" : "");
   TVK_MX(mx_muon_step(tab.data(), int64_t(tab.size()), &hp, nullptr, 0, current_stream()));
   launched(2 + 3 * int(steps));

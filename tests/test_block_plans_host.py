@@ -50,3 +50,50 @@ def test_no_call_takes_more_than_the_bound(mx, m, k, n, backward):
     assert got <= max(8 * GIB, 4 * m * n * backward) + 17 * 4 * (m + n + k) + (256 << 20)
     if planes(m, k, n, backward) + 4 * m * n * backward > 8 * GIB:
         assert got <= 4 * m * n * backward + (160 << 20), "in tiles"
+
+
+# ------------------------------------------------ overlapping buffers of one call
+def refused(mx, call, *args):
+    with pytest.raises(mx.MXError) as e:
+        mx.check(getattr(mx.lib(), call)(*args))
+    return e.value
+
+
+AT = 1 << 20   # addresses that no refused call reads
+SIZE = 8 * 9 * 4
+
+
+def matrices(mx, *rows):
+    return (mx.MatrixPair * len(rows))(*[mx.MatrixPair(i, o, 8, 9) for i, o in rows]), len(rows)
+
+
+@pytest.mark.parametrize("rows", [
+    [(AT, 2 * AT), (3 * AT, 2 * AT)],                    # one output twice
+    [(AT, 2 * AT), (3 * AT, 2 * AT + SIZE - 4)],         # the last element of one
+    [(AT, 2 * AT), (2 * AT + 4, 3 * AT)],                # an output under another's input
+    [(AT, AT + 4)],                                      # its own input, not whole
+    [(AT, 2 * AT), (2 * AT - 4, 2 * AT - 4)],
+    [(2 * AT, 2 * AT), (2 * AT, 4 * AT)],                # in place, and another's input
+])
+def test_orthogonalize_refuses_overlaps(mx, rows):
+    import ctypes as C
+    arr, count = matrices(mx, *rows)
+    ns = mx.NewtonSchulz(5, 3.4445, -4.775, 2.0315, 1e-7)
+    e = refused(mx, "mx_orthogonalize", arr, count, C.byref(ns), AT // 2, 1 << 30, None)
+    assert e.status == mx.MX_ERR_INVALID and "overlaps" in str(e)
+
+
+@pytest.mark.parametrize("rows", [
+    [(AT, 2 * AT, 3 * AT), (AT, 4 * AT, 5 * AT)],             # a parameter twice
+    [(AT, 2 * AT, 3 * AT), (4 * AT, 5 * AT, 3 * AT)],         # a momentum buffer twice
+    [(AT, 2 * AT, AT)],                                       # its own parameter as its momentum
+    [(AT, AT, 3 * AT)],                                       # as its gradient
+    [(AT, 2 * AT, 3 * AT), (AT + SIZE - 4, 4 * AT, 5 * AT)],  # views of one storage
+    [(AT, 2 * AT, 3 * AT), (4 * AT, 3 * AT + 40, 5 * AT)],    # a gradient over another's momentum
+])
+def test_muon_refuses_overlaps(mx, rows):
+    import ctypes as C
+    arr = (mx.MuonTensor * len(rows))(*[mx.MuonTensor(p, g, m, 8, 9) for p, g, m in rows])
+    hp = mx.MuonHParams(0.02, 0.1, 0.95, 1, 0, mx.NewtonSchulz(5, 3.4445, -4.775, 2.0315, 1e-7))
+    e = refused(mx, "mx_muon_step", arr, len(rows), C.byref(hp), AT // 2, 1 << 30, None)
+    assert e.status == mx.MX_ERR_INVALID and "overlaps" in str(e)
