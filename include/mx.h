@@ -509,6 +509,10 @@ int mx_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t src_pitc
 /* must not do (MX_ERR_WORKSPACE).                                            */
 /* ------------------------------------------------------------------------ */
 
+/* Kernels that this thread's last mx_layer_norm_*, mx_linear_*, mx_orthogonalize
+ * or mx_muon_step has launched (its workspace queries launch none and count none). */
+int64_t mx_last_launches(void);
+
 /* Layer norm over the last axis of x [rows, cols]:
  *   y = (x - mean) * rstd * gamma + beta,  rstd = 1/sqrt(var + eps), biased variance.
  * gamma and beta may be NULL (1 and 0); mean and rstd [rows] may be NULL (not

@@ -252,7 +252,7 @@ int launch3(GemmArgs p, hipStream_t s) {
     p.batch0 = b0;
     const dim3 grid(ntiles, p.splits, std::min(p.batch - b0, 65535));
     hipLaunchKernelGGL((gemm_kernel<D, MA, MB, EPI>), grid, dim3(kThreads), 0, s, p);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
   }
   return MX_OK;
 }
@@ -479,7 +479,7 @@ int launch_sum(const GemmArgs& p, hipStream_t s) {
     hipLaunchKernelGGL((gemm_sum_kernel<true, EPI>), dim3(blocks), dim3(256), 0, s, p);
   else
     hipLaunchKernelGGL((gemm_sum_kernel<false, EPI>), dim3(blocks), dim3(256), 0, s, p);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 
@@ -511,7 +511,7 @@ int gemm_within(const mx_gemm_desc* d, const float* a, const float* b, const flo
       hipLaunchKernelGGL(gemm_k0_kernel<true>, dim3(blocks), dim3(256), 0, s, p);
     else
       hipLaunchKernelGGL(gemm_k0_kernel<false>, dim3(blocks), dim3(256), 0, s, p);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
     return MX_OK;
   }
   MX_REQUIRE(a && b, MX_ERR_INVALID, "mx_gemm_f32: null operand");

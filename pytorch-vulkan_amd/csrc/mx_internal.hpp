@@ -27,6 +27,9 @@ std::string cat(const Args&... args) {
 hipStream_t resolve_stream(void* s);
 int current_device();
 
+// Kernels that this thread's current call has launched (MX_LAUNCHED behind each).
+extern thread_local int64_t launches_of_call;
+
 // Stream-ordered scratch: freed (returned to the cache) when it goes out of
 // scope; later work on the same stream is ordered after the kernels that use it.
 struct Scratch {
@@ -103,6 +106,12 @@ int gemm_describe(const mx_gemm_desc* d, const float* a, const float* b, int64_t
     hipError_t mx_e_ = (expr);                                                        \
     if (mx_e_ != hipSuccess)                                                          \
       return ::mx::set_error(MX_ERR_HIP, ::mx::cat(#expr, ": ", hipGetErrorString(mx_e_))); \
+  } while (0)
+
+#define MX_LAUNCHED()            \
+  do {                           \
+    MX_HIP(hipGetLastError());   \
+    ++::mx::launches_of_call;    \
   } while (0)
 
 #define MX_REQUIRE(cond, code, ...) \

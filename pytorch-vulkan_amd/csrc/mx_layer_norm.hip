@@ -424,6 +424,7 @@ using namespace mx;
 extern "C" int mx_layer_norm_forward(const float* x, const float* gamma, const float* beta, int64_t rows, int64_t cols,
                                      float eps, float* y, float* mean, float* rstd, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   MX_TRY(check("mx_layer_norm_forward", rows, cols));
   if (rows == 0) return MX_OK;
   MX_REQUIRE(x && y, MX_ERR_INVALID, "mx_layer_norm_forward: null buffer");
@@ -441,7 +442,7 @@ extern "C" int mx_layer_norm_forward(const float* x, const float* gamma, const f
                          eps, y, mean, rstd);
     });
   }
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
   MX_ABI_END
 }
@@ -459,6 +460,7 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
                                       const float* gamma, int64_t rows, int64_t cols, float* dx, float* dgamma,
                                       float* dbeta, void* workspace, int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   MX_TRY(check("mx_layer_norm_backward", rows, cols));
   const bool affine = dgamma || dbeta;
   if (!dx && !affine) return MX_OK;
@@ -467,7 +469,7 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
     if (!affine || cols == 0) return MX_OK;
     hipLaunchKernelGGL(ln_zero_kernel, dim3(unsigned(std::min<int64_t>((cols + 255) / 256, 1024))), dim3(256), 0, s,
                        dgamma, dbeta, cols);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
     return MX_OK;
   }
   MX_REQUIRE(dy && x && mean && rstd, MX_ERR_INVALID, "mx_layer_norm_backward: null buffer");
@@ -482,13 +484,13 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
       parts = walk_parts(rows);
       hipLaunchKernelGGL(ln_cols_walk_kernel, dim3(unsigned((cols + 255) / 256), unsigned(parts)), dim3(256), 0, s, dy, x,
                          mean, rstd, rows, cols, part);
-      MX_HIP(hipGetLastError());
+      MX_LAUNCHED();
     }
     if (dx) {
       const int threads = cols < 1024 ? 64 : 1024;
       hipLaunchKernelGGL(ln_bwd_walk_kernel, dim3(unsigned(std::min<int64_t>(rows, 65535))), dim3(threads), 0, s, dy, x,
                          mean, rstd, gamma, rows, cols, dx);
-      MX_HIP(hipGetLastError());
+      MX_LAUNCHED();
     }
     if (!affine) return MX_OK;
   } else {
@@ -504,12 +506,12 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
                            gamma, rows, int(cols), dx, part, dgamma, dbeta);
       }
     });
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
     if (!affine || parts == 1) return MX_OK;
   }
   hipLaunchKernelGGL(ln_cols_kernel, dim3(unsigned((2 * cols + 31) / 32)), dim3(1024), 0, s, part, parts, cols, dgamma,
                      dbeta);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
   MX_ABI_END
 }

@@ -1021,13 +1021,13 @@ int run_joins(PieceLaunch l, hipStream_t s) {
   const int blocks = l.second + (l.p[1].tiles_m * l.p[1].tiles_n - l.p[1].share.whole) * PER;
   if (!blocks) return MX_OK;
   hipLaunchKernelGGL((piece_join_kernel<T, EPI>), dim3(unsigned(blocks)), dim3(64), 0, s, l);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 int run_forward(const PieceArgs& p, hipStream_t s) {
   using T = PieceTile;
   hipLaunchKernelGGL(piece_forward_kernel<T>, dim3(unsigned(piece_blocks(p))), dim3(T::THREADS), 0, s, p);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   PieceLaunch l{};
   l.p[0] = p;
   return run_joins<true>(l, s);
@@ -1038,7 +1038,7 @@ int run_backward(PieceLaunch l, hipStream_t s) {
   l.swapped = l.p[1].nk > l.p[0].nk;
   l.second = blocks[l.swapped];
   hipLaunchKernelGGL(piece_backward_kernel<T>, dim3(unsigned(blocks[0] + blocks[1])), dim3(T::THREADS), 0, s, l);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return run_joins<false>(l, s);
 }
 
@@ -1054,7 +1054,7 @@ int run_scan(ScanArgs* p, hipStream_t s) {
     hipLaunchKernelGGL((scan_kernel<4, ENDS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
   else
     hipLaunchKernelGGL((scan_kernel<1, ENDS>), dim3(unsigned(blocks)), dim3(256), 0, s, *p);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 int run_pack(PackArgs* p, hipStream_t s) {
@@ -1066,7 +1066,7 @@ int run_pack(PackArgs* p, hipStream_t s) {
   p->first_sum = blocks;
   if (p->out) blocks += (p->n + 31) / 32;
   hipLaunchKernelGGL(pack_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, *p);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   ListArgs lists{};
   int count = 0;
   for (int i = 0; i < p->count; ++i)
@@ -1074,7 +1074,7 @@ int run_pack(PackArgs* p, hipStream_t s) {
       if (c->ends) lists.of[count++] = *c;
   if (!count) return MX_OK;
   hipLaunchKernelGGL(list_kernel, dim3(kListEnds, unsigned(count)), dim3(256), 0, s, lists);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 
@@ -1135,7 +1135,7 @@ int run_direct(DirectArgs* d, int wk, hipStream_t s) {
     hipLaunchKernelGGL((direct_kernel<FORWARD, 4>), grid, block, 0, s, *d);
   else
     hipLaunchKernelGGL((direct_kernel<FORWARD, 1>), grid, block, 0, s, *d);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 
@@ -1145,7 +1145,7 @@ int run_few(const float* x, const float* w, const float* bias, const float* resi
   const int64_t groups = (m + M - 1) / M, blocks = (n + kFewRows - 1) / kFewRows;
   hipLaunchKernelGGL(few_kernel<M>, dim3(unsigned((blocks + 7) / 8 * 8 * groups)), dim3(256), 0, s, x, w, bias, residual,
                      int(m), int(groups), k, int(n), act, y, z);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   return MX_OK;
 }
 
@@ -1228,6 +1228,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
                                  int64_t k, int64_t n, int activation, float* y, float* z, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   const char* const who = "mx_linear_forward";
   MX_TRY(check(who, m, k, n, activation));
   if (m == 0 || n == 0) return MX_OK;
@@ -1298,13 +1299,14 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
                                   int64_t n, int activation, float* dx, float* dw, float* db, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   const char* const who = "mx_linear_backward";
   MX_TRY(check(who, m, k, n, activation));
   hipStream_t s = resolve_stream(stream);
   const auto zero = [&](float* p, int64_t count) -> int {
     if (!p || count == 0) return MX_OK;
     hipLaunchKernelGGL(zero_kernel, dim3(unsigned(std::min<int64_t>((count + 255) / 256, 65535))), dim3(256), 0, s, p, count);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
     return MX_OK;
   };
   if (m == 0 || n == 0) {  // empty sums
@@ -1417,7 +1419,7 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
   }
   if (db && b.scan.parts > 1 && !b.packed) {
     hipLaunchKernelGGL(column_sum_kernel, dim3(unsigned((n + 31) / 32)), dim3(1024), 0, s, b.part, b.scan.parts, int(n), db);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
   }
   const int64_t room = b.packed ? 0 : kPartials;
   if (b.packed) {

@@ -625,10 +625,10 @@ template <class T, int KIND>
 int launch(const StepArgs& p, int tiles, hipStream_t s) {
   const int rest = tiles - p.share.whole;
   hipLaunchKernelGGL((step_kernel<T, KIND>), dim3(unsigned(p.share.whole + rest * p.share.parts)), dim3(T::THREADS), 0, s, p);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   if (rest) {
     hipLaunchKernelGGL((join_kernel<T, KIND>), dim3(unsigned(rest * T::WAVES * T::FM * T::FN)), dim3(64), 0, s, p);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
   }
   return MX_OK;
 }
@@ -859,11 +859,11 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
     hipLaunchKernelGGL(norm_kernel<true>, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts);
   else
     hipLaunchKernelGGL(norm_kernel<false>, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   if (ns.steps == 0) {
     hipLaunchKernelGGL(scaled_kernel, dim3(unsigned(nparts), unsigned(batch)), dim3(256), 0, s, tab, fin.up, numel, parts,
                        nparts, ns.eps, decay, step);
-    MX_HIP(hipGetLastError());
+    MX_LAUNCHED();
     return MX_OK;
   }
   if (plan.wide) {
@@ -887,7 +887,7 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
       if (mode == kSmallFirst) hipLaunchKernelGGL(small_kernel<kSmallFirst>, grid, block, 0, s, a);
       if (mode == kSmallNext) hipLaunchKernelGGL(small_kernel<kSmallNext>, grid, block, 0, s, a);
       if (mode == kSmallLast) hipLaunchKernelGGL(small_kernel<kSmallLast>, grid, block, 0, s, a);
-      MX_HIP(hipGetLastError());
+      MX_LAUNCHED();
       float* const was = a.to;
       a.to = const_cast<float*>(a.from);
       a.from = was;
@@ -910,7 +910,7 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
   }
   hipLaunchKernelGGL(pack_kernel, dim3(unsigned(g.lp / 64), unsigned(g.sp / 32), unsigned(batch)), dim3(256), 0, s, tab,
                      fin.up, g, parts, nparts, ns.eps, sc[0].x, sc[0].growth, x, lift);
-  MX_HIP(hipGetLastError());
+  MX_LAUNCHED();
   StepArgs p{};
   p.batch = int(batch);
   p.g = g;
@@ -1037,6 +1037,7 @@ extern "C" int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_
 extern "C" int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   const char* const who = "mx_orthogonalize";
   MX_REQUIRE(ns, MX_ERR_INVALID, who, ": null parameters");
   MX_TRY(check_ns(who, *ns));
@@ -1070,6 +1071,7 @@ extern "C" int mx_muon_workspace(const mx_muon_tensor* tensors, int64_t count, i
 extern "C" int mx_muon_step(const mx_muon_tensor* tensors, int64_t count, const mx_muon_hparams* hp, void* workspace,
                             int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
+  launches_of_call = 0;
   const char* const who = "mx_muon_step";
   MX_REQUIRE(hp, MX_ERR_INVALID, who, ": null hyperparameters");
   MX_REQUIRE(hp->lr >= 0 && hp->weight_decay >= 0 && hp->momentum >= 0 && hp->momentum <= 1 && std::isfinite(hp->lr) &&

@@ -167,6 +167,7 @@ extern "C" {
 
 const char* mx_last_error(void) { return g_last_error; }
 int mx_abi_version(void) { return 3; }
+int64_t mx_last_launches(void) { return launches_of_call; }
 
 int mx_init(int ordinal) {
   MX_ABI_BEGIN
@@ -636,6 +637,8 @@ int upload(const void* host, size_t bytes, hipStream_t s, Scratch& holder) {
   g_ring_head = off + sz;
   return MX_OK;
 }
+
+thread_local int64_t launches_of_call = 0;
 
 // ---------------------------------------------------------------- workspaces
 bool may_allocate(hipStream_t s) {

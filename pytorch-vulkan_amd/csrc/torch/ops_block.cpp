@@ -30,7 +30,7 @@ const float* cptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>(
 float* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 OptT to_cpu(const OptT& t) { return present(t) ? OptT(t->cpu()) : OptT(); }
 at::Tensor to_dev(const at::Tensor& t, const at::Device& d) { return t.defined() ? t.to(d) : t; }
-void launched(int n = 1) { counters().kernel_launches += uint64_t(n); }
+void launched() { counters().kernel_launches += uint64_t(mx_last_launches()); }  // by the call before
 
 // ---------------------------------------------------------------- LayerNorm
 struct Rows {
@@ -101,7 +101,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> native_layer_norm_backward_vk(
   GpuTimer timer(gpu_timing_enabled() ? "layer_norm_backward" : "");
   TVK_MX(mx_layer_norm_backward(cptr(dyc), cptr(xc), cptr(mc), cptr(rc), cptr(wc), r.rows, r.cols, ptr(dx), ptr(dw),
                                 ptr(db), nullptr, 0, current_stream()));
-  launched(2);
+  launched();
   return {dx, dw, db};
 }
 
@@ -162,7 +162,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_act_backward(const at::Ten
                  2.0 * double(m) * double(n) * double(k) * (int(mask[0]) + int(mask[1])));
   TVK_MX(mx_linear_backward(cptr(dyc), cptr(xc), cptr(wc), cptr(zc), m, k, n, act, ptr(dx), ptr(dw), ptr(db), nullptr, 0,
                             current_stream()));
-  launched(2);
+  launched();
   return {dx, dw, db};
 }
 
@@ -194,7 +194,7 @@ std::vector<at::Tensor> orthogonalize(at::TensorList inputs, at::ArrayRef<double
   }
   GpuTimer timer(gpu_timing_enabled() ? "orthogonalize" : "");
   TVK_MX(mx_orthogonalize(tab.data(), int64_t(tab.size()), &ns, nullptr, 0, current_stream()));
-  launched(2 + 3 * int(steps));
+  launched();
   return out;
 }
 
@@ -231,7 +231,7 @@ void muon_step_(at::TensorList params, at::TensorList grads, at::TensorList mome
   }
   GpuTimer timer(gpu_timing_enabled() ? "muon_step" : "");
   TVK_MX(mx_muon_step(tab.data(), int64_t(tab.size()), &hp, nullptr, 0, current_stream()));
-  launched(2 + 3 * int(steps));
+  launched();
 }
 
 }  // namespace

@@ -45,7 +45,7 @@ EXPORTS = [
     "mx_foreach_f32", "mx_conv2d_plan", "mx_gemm_variant", "mx_conv2d_backward_weight_noalloc",
     "mx_conv2d_backward_one_launch", "mx_layer_norm_forward", "mx_layer_norm_backward",
     "mx_layer_norm_backward_workspace", "mx_linear_forward", "mx_linear_backward", "mx_linear_workspace",
-    "mx_orthogonalize", "mx_orthogonalize_workspace", "mx_muon_step", "mx_muon_workspace",
+    "mx_orthogonalize", "mx_orthogonalize_workspace", "mx_muon_step", "mx_muon_workspace", "mx_last_launches",
 ]
 
 
@@ -202,6 +202,7 @@ def lib() -> C.CDLL:
             "mx_orthogonalize_workspace": ([C.POINTER(MatrixPair), i64, C.POINTER(i64)], i32),
             "mx_muon_step": ([C.POINTER(MuonTensor), i64, C.POINTER(MuonHParams), vp, i64, vp], i32),
             "mx_muon_workspace": ([C.POINTER(MuonTensor), i64, C.POINTER(i64)], i32),
+            "mx_last_launches": ([], i64),
             "mx_foreach_f32": ([i32, C.POINTER(ForeachTensor), i64, C.POINTER(i64), vp], i32),
         }
         for name, (args, res) in sig.items():
@@ -463,6 +464,11 @@ def _workspace_query(fn, *args) -> int:
     out = C.c_int64(0)
     check(fn(*args, C.byref(out)))
     return out.value
+
+
+def last_launches() -> int:
+    """Kernels launched by this thread's last layer norm, linear, orthogonalize or Muon call."""
+    return lib().mx_last_launches()
 
 
 def layer_norm_forward(x, gamma, beta, eps, y, mean, rstd, stream=None) -> None:

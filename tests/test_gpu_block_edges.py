@@ -300,3 +300,42 @@ def test_linear_without_room_for_pieces(mx):
     within(dx, want[2].double(), (2 * (n / 8 + 8) * U * dz + dz_err) @ w.double().abs(), "dx")
     within(dw, want[3].double(), (2 * (m / 8 + 8) * U * dz + dz_err).t() @ x.double().abs(), "dw")
     within(db, want[4].double(), (2 * (m / 64 + 64) * U * dz + dz_err).sum(0), "db")
+
+
+# ------------------------------------------------------------ launches counted
+def test_launches_are_counted(mx):
+    """Of calls whose launches are known from their sizes, and on the device surface."""
+    g = gen(1)
+    e = lambda *s: torch.empty(*s, device="cuda")
+    x, w, b = rand(g, 9, 64), rand(g, 32, 64), rand(g, 32)
+    mean, rstd = e(9), e(9)
+    mx.layer_norm_forward(x, None, None, 1e-5, e(9, 64), mean, rstd, stream=stream())
+    assert mx.last_launches() == 1
+    mx.layer_norm_backward(x, x, mean, rstd, None, e(9, 64), None, None, stream=stream())
+    assert mx.last_launches() == 1
+    big = rand(g, 5000, 64)
+    mean, rstd = e(5000), e(5000)
+    mx.layer_norm_forward(big, None, None, 1e-5, e(5000, 64), mean, rstd, stream=stream())
+    mx.layer_norm_backward(big, big, mean, rstd, None, e(5000, 64), e(64), e(64), stream=stream())
+    assert mx.last_launches() == 2, "the rows, and the column sums' second part"
+    mx.linear_forward(x, w, b, e(9, 32), stream=stream())
+    assert mx.last_launches() == 1
+    m = rand(g, 30, 50)
+    for steps in (0, 1, 5):
+        mx.orthogonalize([m], [torch.empty_like(m)], steps=steps, stream=stream())
+        assert mx.last_launches() == (2 + steps), "norm, first, one a step; or norm and scaling"
+    x, w = rand(g, 2048, 2048), rand(g, 2048, 2048)
+    mx.linear_forward(x, w, None, e(2048, 2048), stream=stream())
+    assert mx.last_launches() in (4, 5), "two passes, product, (join,) the products behind"
+    mx.linear_backward(x, x, w, None, e(2048, 2048), e(2048, 2048), None, stream=stream())
+    assert mx.last_launches() in (5, 6)
+    mx.linear_backward(x[:0], x[:0], w, None, None, None, None, stream=stream())
+    assert mx.last_launches() == 0
+
+    import torch_vulkan as vk
+    from torch_vulkan.nn import linear
+    xv, wv = x.cpu().to("vulkan"), w.cpu().to("vulkan")
+    before = vk.execution_stats()["kernel_launches"]
+    with torch.no_grad():
+        linear(xv, wv)
+    assert vk.execution_stats()["kernel_launches"] - before in (4, 5)
