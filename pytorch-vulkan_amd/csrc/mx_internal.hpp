@@ -30,6 +30,9 @@ int current_device();
 // Kernels that this thread's current call has launched (MX_LAUNCHED behind each).
 extern thread_local int64_t launches_of_call;
 
+// Returns a block to its pool; the call's error message, if it is failing, stays.
+void release_scratch(void* ptr);
+
 // Stream-ordered scratch: freed (returned to the cache) when it goes out of
 // scope; later work on the same stream is ordered after the kernels that use it.
 struct Scratch {
@@ -38,11 +41,11 @@ struct Scratch {
   Scratch(const Scratch&) = delete;
   Scratch& operator=(const Scratch&) = delete;
   ~Scratch() {
-    if (ptr) mx_free(ptr);
+    if (ptr) release_scratch(ptr);
   }
   int alloc(size_t bytes, hipStream_t s) {
     if (ptr) {
-      mx_free(ptr);
+      release_scratch(ptr);
       ptr = nullptr;
     }
     return mx_malloc(&ptr, bytes, s);

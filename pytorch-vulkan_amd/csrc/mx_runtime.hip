@@ -155,7 +155,40 @@ void release_cached(int dev) {
   pool.free_blocks.clear();
 }
 
+// Returns a block to its pool.
+int free_block(void* ptr) {
+  if (!ptr) return MX_OK;
+  std::lock_guard<std::mutex> lock(g_alloc_mu);
+  auto it = g_live.find(ptr);
+  MX_REQUIRE(it != g_live.end(), MX_ERR_INVALID, "mx_free: pointer not owned by the allocator");
+  Block* b = it->second;
+  g_live.erase(it);
+  g_stats.allocated_bytes -= b->size;
+  auto& pool = g_pools[b->device];
+  if (b->uses.empty()) {
+    pool.free_blocks.insert(b);
+  } else {
+    Pending p{b, {}};
+    for (hipStream_t s : b->uses) {
+      hipEvent_t ev;
+      if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) continue;
+      (void)hipEventRecord(ev, s);
+      p.events.push_back(ev);
+    }
+    pool.pending.push_back(std::move(p));
+  }
+  g_stats.cached_blocks = pool.free_blocks.size();
+  return MX_OK;
+}
+
 }  // namespace
+
+void release_scratch(void* ptr) {
+  try {
+    (void)free_block(ptr);
+  } catch (...) {  // the block stays out of its pool
+  }
+}
 
 void release_host_cache();  // the page-locked host block cache, below
 
@@ -381,28 +414,7 @@ int mx_malloc(void** ptr, size_t bytes, void* stream) {
 
 int mx_free(void* ptr) {
   MX_ABI_BEGIN
-  if (!ptr) return MX_OK;
-  std::lock_guard<std::mutex> lock(g_alloc_mu);
-  auto it = g_live.find(ptr);
-  MX_REQUIRE(it != g_live.end(), MX_ERR_INVALID, "mx_free: pointer not owned by the allocator");
-  Block* b = it->second;
-  g_live.erase(it);
-  g_stats.allocated_bytes -= b->size;
-  auto& pool = g_pools[b->device];
-  if (b->uses.empty()) {
-    pool.free_blocks.insert(b);
-  } else {
-    Pending p{b, {}};
-    for (hipStream_t s : b->uses) {
-      hipEvent_t ev;
-      if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) continue;
-      (void)hipEventRecord(ev, s);
-      p.events.push_back(ev);
-    }
-    pool.pending.push_back(std::move(p));
-  }
-  g_stats.cached_blocks = pool.free_blocks.size();
-  return MX_OK;
+  return mx::free_block(ptr);
   MX_ABI_END
 }
 

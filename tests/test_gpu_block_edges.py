@@ -339,3 +339,16 @@ def test_launches_are_counted(mx):
     with torch.no_grad():
         linear(xv, wv)
     assert vk.execution_stats()["kernel_launches"] - before in (4, 5)
+
+
+def test_refusal_behind_an_allocation_keeps_its_message():
+    """Overlapping views, found once the call has taken its scratch from the allocator."""
+    import torch_vulkan  # noqa: F401  (the device's operators)
+    ops = torch.ops.torch_vulkan
+    flat = torch.ones(100).to("vulkan")
+    a, b = flat[:60].view(6, 10), flat[50:].view(5, 10)
+    z = lambda t: torch.zeros(t.shape).to("vulkan")
+    with pytest.raises(RuntimeError, match="overlaps another"):
+        ops.muon_step_([a, b], [z(a), z(b)], [z(a), z(b)], 0.1, 0.0, 0.9, True, [1.0, 0.0, 0.0], 1, 1e-7, "original")
+    ops.muon_step_([a], [z(a)], [z(a)], 0.1, 0.5, 0.9, True, [1.0, 0.0, 0.0], 1, 1e-7, "original")
+    assert torch.equal(flat.cpu(), torch.cat([torch.full((60,), 1 - 0.1 * 0.5), torch.ones(40)]))
