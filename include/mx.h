@@ -550,6 +550,9 @@ int mx_linear_backward(const float* dy, const float* x, const float* w, const fl
                        int64_t workspace_bytes, void* stream);
 /* Bytes that a forward (`backward` == 0) or a backward of these sizes takes. */
 int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activation, int backward, int64_t* bytes);
+/* How such a call's products run on 256-byte aligned operands: "few", "small<waves>",
+ * "packed", or the names that mx_gemm_variant gives them (a backward's dx, then dw). */
+int mx_linear_variant(int64_t m, int64_t k, int64_t n, int backward, char* buf, size_t len);
 
 /* The polar factor's approximation by `steps` Newton-Schulz iterations
  * X <- a X + (b G + c G^2) X, G = X X^T (on the shorter side), of
@@ -568,6 +571,10 @@ typedef struct mx_matrix_pair {
 int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
                      int64_t workspace_bytes, void* stream);
 int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_t count, int64_t* bytes);
+/* How `count` matrices of one shape (at most 48, what goes side by side) run:
+ * "one_launch<workgroups a matrix>", or each product's tile, its whole tiles and those
+ * that several workgroups share, as in "gram<128>512+16x11 poly<128>... update<256>...". */
+int mx_orthogonalize_variant(int64_t rows, int64_t cols, int64_t count, char* buf, size_t len);
 
 /* Orthogonalised momentum step (torch.optim.Muon's update):
  *   buf += (1 - momentum) (grad - buf);  u = nesterov ? grad + momentum (buf - grad) : buf

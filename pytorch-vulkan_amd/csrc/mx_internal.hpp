@@ -23,6 +23,11 @@ std::string cat(const Args&... args) {
   return os.str();
 }
 
+// A name to a caller's buffer of len bytes, cut to fit.
+inline void copy_name(const std::string& name, char* buf, size_t len) {
+  if (len) buf[name.copy(buf, len - 1)] = 0;
+}
+
 // `stream` argument -> hipStream_t (NULL stays HIP's null stream).
 hipStream_t resolve_stream(void* s);
 int current_device();

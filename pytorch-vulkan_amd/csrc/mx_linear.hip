@@ -1224,6 +1224,35 @@ extern "C" int mx_linear_workspace(int64_t m, int64_t k, int64_t n, int activati
   MX_ABI_END
 }
 
+extern "C" int mx_linear_variant(int64_t m, int64_t k, int64_t n, int backward, char* buf, size_t len) {
+  MX_ABI_BEGIN
+  MX_TRY(check("mx_linear_variant", m, k, n, MX_ACT_NONE));
+  MX_REQUIRE(buf || !len, MX_ERR_INVALID, "mx_linear_variant: null buffer");
+  std::string name = "none";
+  if (m > 0 && n > 0 && k > 0) {
+    switch (form_of(m, k, n, backward != 0)) {
+      case Form::kFew: name = "few"; break;
+      case Form::kSmall: name = cat("small<", direct_waves(m, k, n, backward != 0), ">"); break;
+      case Form::kPacked: name = "packed"; break;
+      default: {
+        const float* const at = reinterpret_cast<const float*>(256);
+        int64_t bytes;
+        const mx_gemm_desc d = backward ? dx_desc(m, k, n) : forward_desc(m, k, n, true);
+        MX_TRY(gemm_describe(&d, at, at, kPartials, &name, &bytes));
+        if (backward) {
+          std::string other;
+          const mx_gemm_desc dw = dw_desc(m, k, n);
+          MX_TRY(gemm_describe(&dw, at, at, kPartials, &other, &bytes));
+          name += " " + other;
+        }
+      }
+    }
+  }
+  copy_name(name, buf, len);
+  return MX_OK;
+  MX_ABI_END
+}
+
 extern "C" int mx_linear_forward(const float* x, const float* w, const float* bias, const float* residual, int64_t m,
                                  int64_t k, int64_t n, int activation, float* y, float* z, void* workspace,
                                  int64_t workspace_bytes, void* stream) {

@@ -1034,6 +1034,25 @@ extern "C" int mx_orthogonalize_workspace(const mx_matrix_pair* matrices, int64_
   MX_ABI_END
 }
 
+extern "C" int mx_orthogonalize_variant(int64_t rows, int64_t cols, int64_t count, char* buf, size_t len) {
+  MX_ABI_BEGIN
+  const char* const who = "mx_orthogonalize_variant";
+  MX_TRY(check_shape(who, 0, rows, cols));
+  MX_REQUIRE(count >= 0 && count <= kBatch && (buf || !len), MX_ERR_INVALID, who, ": count must lie in [0, ", kBatch, "]");
+  std::string name = "none";
+  if (rows > 0 && cols > 0 && count > 0) {
+    const Plan p = plan_set(rows, cols, count);
+    const auto product = [](const char* what, const Deal& d, int t) {
+      return cat(what, "<", kTiles[t].tile, t == kTile64Deep ? ",deep>" : ">", d.whole, d.tiles > d.whole ? cat("+", d.tiles - d.whole, "x", d.parts) : "");
+    };
+    name = p.wide ? cat("one_launch<", p.wide, ">")
+                  : product("gram", p.gram, p.sym) + product(" poly", p.poly, p.sym) + product(" update", p.update, p.next);
+  }
+  copy_name(name, buf, len);
+  return MX_OK;
+  MX_ABI_END
+}
+
 extern "C" int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN

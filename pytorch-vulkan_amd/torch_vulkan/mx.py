@@ -46,6 +46,7 @@ EXPORTS = [
     "mx_conv2d_backward_one_launch", "mx_layer_norm_forward", "mx_layer_norm_backward",
     "mx_layer_norm_backward_workspace", "mx_linear_forward", "mx_linear_backward", "mx_linear_workspace",
     "mx_orthogonalize", "mx_orthogonalize_workspace", "mx_muon_step", "mx_muon_workspace", "mx_last_launches",
+    "mx_linear_variant", "mx_orthogonalize_variant",
 ]
 
 
@@ -203,6 +204,8 @@ def lib() -> C.CDLL:
             "mx_muon_step": ([C.POINTER(MuonTensor), i64, C.POINTER(MuonHParams), vp, i64, vp], i32),
             "mx_muon_workspace": ([C.POINTER(MuonTensor), i64, C.POINTER(i64)], i32),
             "mx_last_launches": ([], i64),
+            "mx_linear_variant": ([i64, i64, i64, i32, C.c_char_p, C.c_size_t], i32),
+            "mx_orthogonalize_variant": ([i64, i64, i64, C.c_char_p, C.c_size_t], i32),
             "mx_foreach_f32": ([i32, C.POINTER(ForeachTensor), i64, C.POINTER(i64), vp], i32),
         }
         for name, (args, res) in sig.items():
@@ -510,6 +513,22 @@ def linear_backward(dy, x, w, z, dx, dw, db, activation=ACT_NONE, workspace=None
 
 def linear_workspace(m: int, k: int, n: int, activation=ACT_NONE, backward=False) -> int:
     return _workspace_query(lib().mx_linear_workspace, m, k, n, activation, 1 if backward else 0)
+
+
+def _name(fn, *args) -> str:
+    buf = C.create_string_buffer(256)
+    check(fn(*args, buf, 256))
+    return buf.value.decode()
+
+
+def linear_variant(m: int, k: int, n: int, backward=False) -> str:
+    """How the products of a linear layer's call run (aligned operands)."""
+    return _name(lib().mx_linear_variant, m, k, n, 1 if backward else 0)
+
+
+def orthogonalize_variant(rows: int, cols: int, count: int = 1) -> str:
+    """How ``count`` matrices of one shape are orthogonalised."""
+    return _name(lib().mx_orthogonalize_variant, rows, cols, count)
 
 
 def _newton_schulz(steps, coefficients, eps) -> NewtonSchulz:

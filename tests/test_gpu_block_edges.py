@@ -6,6 +6,7 @@ over inputs, sizes that take each form.
 Bounds come from the operations' roundings, u = 2^-24 (half a step of FP32
 relative to a value)."""
 import math
+import re
 
 import pytest
 import torch
@@ -352,3 +353,182 @@ def test_refusal_behind_an_allocation_keeps_its_message():
         ops.muon_step_([a, b], [z(a), z(b)], [z(a), z(b)], 0.1, 0.0, 0.9, True, [1.0, 0.0, 0.0], 1, 1e-7, "original")
     ops.muon_step_([a], [z(a)], [z(a)], 0.1, 0.5, 0.9, True, [1.0, 0.0, 0.0], 1, 1e-7, "original")
     assert torch.equal(flat.cpu(), torch.cat([torch.full((60,), 1 - 0.1 * 0.5), torch.ones(40)]))
+
+
+# ---------------------------------------- every tile, split and direction of a product
+# Sizes whose plan takes them, and what the plan has to name so that a changed choice
+# of tiles does not empty the list: whole tiles, tiles shared by several workgroups
+# (0+n x parts), or both.
+ORTH_PLANS = [
+    ((4096, 4096, 1), r"gram<128>512\+\d+x\d+ poly<128>512\+\d+x\d+ update<256>\d+$"),
+    ((1024, 1024, 16), r"gram<128>\d+ poly<128>\d+ update<256>\d+$"),
+    ((2300, 700, 8), r"gram<128>\d+ poly<128>\d+ update<256>\d+$"),
+    ((1500, 2048, 1), r"gram<128>0\+\d+x\d+ poly<128>0\+\d+x\d+ update<128>\d+$"),
+    ((2048, 1536, 1), r"gram<128>0\+\d+x\d+ poly<128>0\+\d+x\d+ update<128>\d+$"),
+    ((1280, 1600, 4), r"gram<128>\d+ poly<128>\d+ update<128>\d+\+\d+x\d+"),
+    ((1600, 1280, 4), r"gram<128>\d+ poly<128>\d+ update<128>\d+\+\d+x\d+"),
+    ((1500, 1536, 2), r"update<64>\d+\+\d+x\d+"),
+    ((2300, 2048, 1), r"update<64>\d+\+\d+x\d+"),
+    ((2048, 2300, 2), r"gram<64>\d+\+\d+x\d+ poly<64>\d+\+\d+x\d+ update<128>\d+\+\d+x\d+"),
+    ((1600, 1000, 8), r"gram<64>\d+\+\d+x\d+ poly<64>\d+\+\d+x\d+ update<256>\d+$"),
+    ((1000, 513, 6), r"gram<64>\d+ poly<64>\d+ update<128>\d+$"),
+    ((200, 4100, 2), r"gram<64,deep>0\+\d+x\d+ poly<64,deep>\d+ update<128>\d+$"),
+    ((915, 915, 22), r"gram<256>\d+ poly<256>\d+"),
+    ((3011, 8394, 1), r"gram<256>0\+\d+x\d+ poly<256>0\+\d+x\d+"),
+    ((4257, 4257, 1), r"update<256>\d+\+\d+x\d+"),
+    ((7525, 2707, 1), r"update<256>\d+\+\d+x\d+"),
+]
+# Of |X| after five iterations: 2^-21 in each, multiplied by 3.9 at most in every later one.
+ORTH_TOL = 310 * 2.0 ** -21
+NS = (3.4445, -4.7750, 2.0315)
+
+
+@pytest.mark.parametrize("shape,plan", ORTH_PLANS)
+def test_orthogonalize_on_every_tile(mx, shape, plan):
+    rows, cols, count = shape
+    name = mx.orthogonalize_variant(rows, cols, count)
+    print("orthogonalize", shape, name, flush=True)
+    assert re.search(plan, name), name
+    g = gen(rows + cols)
+    ins = rand(g, count, rows, cols) + 3 * rand(g, count, rows, 4) @ rand(g, count, 4, cols)
+    flat = torch.full((count * rows * cols + 64,), 12345.0, device="cuda")
+    outs = flat[:-64].view(count, rows, cols)
+    mx.orthogonalize(ins.unbind(0), outs.unbind(0), stream=stream())
+    assert bool((flat[-64:] == 12345.0).all()), "wrote past the end"
+    for i in {0, count // 2, count - 1}:
+        want = orth(ins[i].double(), 5, NS)
+        rel = float((outs[i].double() - want).norm() / want.norm())
+        assert rel <= ORTH_TOL, (i, rel)
+        # The same bound holds of the error's largest singular value, of 1.2 at most: of every row.
+        worst = float((outs[i].double() - want).norm(dim=1).max())
+        assert worst <= 1.2 * ORTH_TOL, (i, worst)
+
+
+@pytest.mark.parametrize("shape,plan", [p for p in ORTH_PLANS if p[0] in (
+    (1280, 1600, 4), (1600, 1280, 4), (1024, 1024, 16), (2300, 700, 8), (1500, 1536, 2), (2300, 2048, 1), (7525, 2707, 1))])
+def test_muon_on_every_tile(mx, shape, plan):
+    """The last product's stores, and the joins of its shared tiles, on a parameter."""
+    rows, cols, count = shape
+    assert re.search(plan, mx.orthogonalize_variant(rows, cols, count))
+    print("muon", shape, flush=True)
+    g = gen(rows)
+    p, gr, m = (rand(g, count, rows, cols, scale=s) for s in (1e-2, 1e-3, 1e-3))
+    p0, m0 = p.clone(), m.clone()
+    lr, wd, mu = 0.5, 0.1, 0.95
+    mx.muon_step(p.unbind(0), gr.unbind(0), m.unbind(0), lr=lr, weight_decay=wd, momentum=mu, stream=stream())
+    for i in {0, count - 1}:
+        mr = m0[i].double() + (1 - mu) * (gr[i].double() - m0[i].double())
+        within(m[i], mr, 4 * U * (mr.abs() + gr[i].double().abs() + m0[i].double().abs()), "momentum")
+        o = orth(gr[i].double() + mu * (mr - gr[i].double()), 5, NS)
+        r = math.sqrt(max(1, rows / cols))
+        moved = (p0[i].double() * (1 - lr * wd) - p[i].double()) / (lr * r)
+        tol = ORTH_TOL * float(o.norm()) + 4 * U * float(p0[i].double().norm()) / (lr * r) + 310 * 4 * U * float(o.norm())
+        assert float((moved - o).norm()) <= tol
+
+
+# --------------------------------------- linear forwards and gradients on every form
+# (m, k, n), the start of the products' names, forward or backward.
+LINEAR_PLANS = [
+    ((256, 4096, 4096), r"gemm_kernel<128x128x16,KVEC,KVEC>\+split"),
+    ((128, 4096, 4094), r"gemm_kernel<64x64x16,KVEC,KVEC>\+split"),
+    ((100, 2048, 1000), r"gemm_kernel<64x64x16,KVEC,KVEC>\+split"),
+    ((100, 6001, 1000), r"gemm_kernel<64x64x16,KSCALAR,KSCALAR>\+split"),
+    ((8192, 256, 1024), r"gemm_kernel<128x128x16,KVEC,KVEC>\+bias"),
+    ((600, 300, 5000), r"gemm_kernel<64x64x16,KVEC,KVEC>\+bias"),
+    ((20001, 65, 300), r"gemm_kernel<128x128x16,KSCALAR,KSCALAR>\+bias"),
+    ((700, 700, 700), r"small<8>"),
+    ((700, 40, 700), r"small<1>"),
+    ((300, 100, 700), r"small<4>"),
+    ((33, 4096, 64), r"few"),
+    ((2048, 2048, 2048), r"packed"),
+]
+
+
+def slope(act, z):
+    """The activations' derivatives, in the type of z."""
+    if act == "relu":
+        return (z > 0).to(z.dtype)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if act == "gelu":
+        return 0.5 * torch.special.erfc(-z / math.sqrt(2)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    c = math.sqrt(2 / math.pi)
+    s = torch.sigmoid(2 * c * (z + 0.044715 * z ** 3))
+    return s + 2 * c * z * s * (1 - s) * (1 + 3 * 0.044715 * z * z)
+
+
+def check_layer(mx, x, w, b, res, dy, act, workspace=False, what=""):
+    """One layer, forward with everything in its epilogue and backward, against 64 bits."""
+    m, k, n = *x.shape, w.shape[0]
+    code = mx.ACTIVATIONS[act]
+    fn = dict(relu=F.relu, silu=F.silu, gelu=F.gelu, gelu_tanh=lambda v: F.gelu(v, approximate="tanh"))[act]
+    room = lambda back: torch.empty(max(16, mx.linear_workspace(m, k, n, code, back)), dtype=torch.uint8, device="cuda") if workspace else None
+    nan = lambda *s: torch.full(s, float("nan"), device="cuda")
+    y, z, dx, dw, db = nan(m, n), nan(m, n), nan(m, k), nan(n, k), nan(n)
+    mx.linear_forward(x, w, b, y, activation=code, residual=res, z=z, workspace=room(False), stream=stream())
+    into = res.clone()
+    mx.linear_forward(x, w, b, into, activation=code, residual=into, workspace=room(False), stream=stream())
+    assert torch.equal(into, y), what + ": into the residual's buffer"
+    mx.linear_backward(dy, x, w, z, dx, dw, db, activation=code, workspace=room(True), stream=stream())
+    d = lambda t: t.double()
+    zr = d(x) @ d(w).t() + d(b)
+    z_err = (k / 8 + 8) * U * (d(x).abs() @ d(w).abs().t() + d(b).abs())
+    yr = fn(zr) + d(res)
+    within(z, zr, z_err, what + " z")
+    within(y, yr, 1.13 * z_err + 16 * U * (zr.abs() + 1) + 4 * U * yr.abs(), what + " y")
+    dz = d(dy) * slope(act, d(z))
+    dz_err = 16 * U * d(dy).abs() * (d(z).abs() + 1)
+    within(dx, dz @ d(w), ((n / 8 + 8) * U * dz.abs() + dz_err) @ d(w).abs() + 1e-30, what + " dx")
+    within(dw, dz.t() @ d(x), ((m / 8 + 8) * U * dz.abs() + dz_err).t() @ d(x).abs() + 1e-30, what + " dw")
+    within(db, dz.sum(0), ((m / 64 + 64) * U * dz.abs() + dz_err).sum(0) + 1e-30, what + " db")
+
+
+@pytest.mark.parametrize("shape,plan", LINEAR_PLANS)
+@pytest.mark.parametrize("workspace", [False, True])
+def test_linear_on_every_form(mx, shape, plan, workspace):
+    m, k, n = shape
+    print("linear form", shape, mx.linear_variant(*shape), "|", mx.linear_variant(*shape, True), flush=True)
+    assert re.match(plan, mx.linear_variant(*shape)), mx.linear_variant(*shape)
+    g = gen(m + k)
+    act = ["gelu", "silu", "gelu_tanh", "relu"][(m + k + n) % 4]
+    check_layer(mx, rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, n, scale=0.3), rand(g, m, n), rand(g, m, n), act,
+                workspace, str(shape))
+
+
+LINEAR_BACKWARD_PLANS = [
+    ((128, 4096, 4096), r"gemm_kernel<64x64x16,KVEC,RVEC>\+split gemm_kernel<256x128x16,RVEC,RVEC>"),
+    ((20000, 64, 300), r"gemm_kernel<64x64x16,KVEC,RVEC> gemm_kernel<64x64x16,RVEC,RVEC>\+split"),
+    ((200000, 129, 129), r"gemm_kernel<\w+,KSCALAR,RSCALAR> gemm_kernel<64x64x16,RSCALAR,RSCALAR>\+split"),
+    ((8192, 256, 1024), r"packed"),
+    ((100, 2048, 1000), r"small<4>"),
+    ((8, 40, 30), r"small<1>"),
+]
+
+
+@pytest.mark.parametrize("shape,plan", LINEAR_BACKWARD_PLANS)
+@pytest.mark.parametrize("workspace", [False, True])
+def test_linear_backward_on_every_form(mx, shape, plan, workspace):
+    m, k, n = shape
+    print("linear backward form", shape, mx.linear_variant(*shape, True), flush=True)
+    assert re.match(plan, mx.linear_variant(*shape, True)), mx.linear_variant(*shape, True)
+    g = gen(m + n)
+    check_layer(mx, rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, n, scale=0.3), rand(g, m, n), rand(g, m, n), "gelu",
+                workspace, str(shape))
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2", "3"])
+@pytest.mark.parametrize("shape", [(2048, 2048, 2048), (2049, 2052, 2060), (2050, 1025, 2047)])
+def test_linear_left_to_the_other_products(mx, monkeypatch, tile, shape):
+    """Operands that packed products leave, with everything in the epilogue of the
+    kernels that take them, on each of their tiles (256-wide ones where k % 4 == 0)."""
+    m, k, n = shape
+    assert mx.linear_variant(m, k, n) == "packed" and mx.linear_variant(m, k, n, True) == "packed"
+    monkeypatch.setenv("MX_GEMM_TILE", tile)
+    print("left out", shape, tile, flush=True)
+    g = gen(k)
+    spread = torch.exp2(torch.linspace(-30, 10, m, device="cuda"))[:, None]
+    sparse = torch.zeros(n, k, device="cuda")
+    sparse[torch.arange(n, device="cuda"), torch.randint(k, (n,), device="cuda", generator=g)] = rand(g, n)
+    check_layer(mx, rand(g, m, k) * spread, sparse, rand(g, n, scale=0.3), rand(g, m, n), rand(g, m, n) * spread, "gelu", False,
+                f"{shape} tile {tile}")
