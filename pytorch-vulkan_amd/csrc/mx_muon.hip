@@ -190,7 +190,7 @@ struct StepArgs {
   int64_t a_plane, b_plane, out_plane;
   int a_rows, b_rows, out_rows;
   int nk;                 // slabs
-  int tiles_m, tiles_n, batch;
+  int tiles_m, tiles_n;
   Shares share;
   float alpha;            // product of pieces -> stored value
   float diag, lin, unit;  // kPoly: a (the last iteration's) and b times the stored scale, 1 / G's scale
@@ -912,7 +912,6 @@ int run_set(const Table& tab, int64_t batch, const Plan& plan, const mx_newton_s
                      fin.up, g, parts, nparts, ns.eps, sc[0].x, sc[0].growth, x, lift);
   MX_LAUNCHED();
   StepArgs p{};
-  p.batch = int(batch);
   p.g = g;
   p.tab = tab;
   p.lift = lift;
