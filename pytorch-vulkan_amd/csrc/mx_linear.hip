@@ -22,7 +22,7 @@
 // powers below that largest is therefore off by 2^(d - 51) of itself, and while no
 // nonzero one of either operand is deeper than 23 + log2 k, a sum over k is off by at
 // most (k / 8) 2^-24 of its terms' magnitudes by that, whatever the operands are.
-// Of normal random operands with 2^24 elements and k = 1024 one in 200 has a deeper
+// Of normal random operands with 2^24 elements and k = 1024 one in 160 has a deeper
 // one.
 //
 // Deeper ones (the tails of GELU and SiLU have them) are lost only in sums without

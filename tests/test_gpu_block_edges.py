@@ -6,6 +6,7 @@ over inputs, sizes that take each form.
 Bounds come from the operations' roundings, u = 2^-24 (half a step of FP32
 relative to a value)."""
 import math
+import random
 import re
 
 import pytest
@@ -532,3 +533,66 @@ def test_linear_left_to_the_other_products(mx, monkeypatch, tile, shape):
     sparse[torch.arange(n, device="cuda"), torch.randint(k, (n,), device="cuda", generator=g)] = rand(g, n)
     check_layer(mx, rand(g, m, k) * spread, sparse, rand(g, n, scale=0.3), rand(g, m, n), rand(g, m, n) * spread, "gelu", False,
                 f"{shape} tile {tile}")
+
+
+@pytest.mark.parametrize("at", [0, 31, 32, 777, 2047, 2048])
+@pytest.mark.parametrize("low", [2.0 ** -45, 0.0])
+def test_linear_one_row_or_column_far_below(mx, at, low):
+    """One row or column of an operand alone is small (or zero: masked), everything else
+    dense with a few deep elements, so that the counts decide."""
+    print("one row", at, low, flush=True)
+    m = k = n = 2049
+    assert mx.linear_variant(m, k, n) == "packed" and mx.linear_variant(m, k, n, True) == "packed"
+    g = gen(at)
+
+    def operand():
+        t = rand(g, m, k)
+        t.view(-1)[torch.randint(m * k, (5,), device="cuda", generator=g)] = 2.0 ** -48
+        return t
+
+    for which in range(6):
+        x, w, dy = operand(), operand(), operand()
+        t = (x, w, dy)[which % 3]
+        if which < 3:
+            t[at] *= low
+        else:
+            t[:, at] *= low
+        check_products(mx, x, w, dy, f"{'x w dy'.split()[which % 3]} {'row' if which < 3 else 'column'} {at} {low}")
+
+
+def test_calls_stay_within_their_workspaces(mx):
+    """Guards behind the bytes that the queries name, over random sizes and addresses."""
+    rng = random.Random(5)
+    g = gen(5)
+
+    def room(need):
+        t = torch.full((max(need, 16) + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+        return t[:max(need, 16)], t[max(need, 16):]
+
+    def unaligned(*s):
+        return rand(g, math.prod(s) + 1)[1:].view(*s) if rng.random() < 0.3 else rand(g, *s)
+
+    log = lambda hi: max(1, round(math.exp(rng.uniform(0, math.log(hi)))))
+    for i in range(60):
+        m, k, n = log(5000), log(3000), log(3000)
+        act = rng.randrange(5)
+        print("workspace", i, m, k, n, act, mx.linear_variant(m, k, n), "|", mx.linear_variant(m, k, n, True), flush=True)
+        x, w, dy, z = unaligned(m, k), unaligned(n, k), unaligned(m, n), unaligned(m, n)
+        y, dx, dw, db = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(w), torch.empty(n, device="cuda")
+        ws, guard = room(mx.linear_workspace(m, k, n, act))
+        mx.linear_forward(x, w, db, y, activation=act, workspace=ws, stream=stream())
+        ws, guard2 = room(mx.linear_workspace(m, k, n, act, True))
+        mx.linear_backward(dy, x, w, z, dx, dw, db, activation=act, workspace=ws, stream=stream())
+        rows, cols = log(3000), log(20000)
+        x, y = unaligned(rows, cols), torch.empty(rows, cols, device="cuda")
+        mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+        ws, guard3 = room(mx.layer_norm_backward_workspace(rows, cols))
+        mx.layer_norm_backward(x, x, mean, rstd, None, y, torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda"),
+                               workspace=ws, stream=stream())
+        mats = [unaligned(r, c) for r, c in [(log(1500), log(1500))] * rng.randint(1, 5) + [(log(200), log(3000))]]
+        ws, guard4 = room(mx.orthogonalize_workspace(mats))
+        mx.orthogonalize(mats, [torch.empty_like(t) for t in mats], workspace=ws, stream=stream())
+        ws, guard5 = room(mx.muon_workspace(mats))
+        mx.muon_step([t.clone() for t in mats], mats, [torch.zeros_like(t) for t in mats], workspace=ws, stream=stream())
+        for at, t in enumerate((guard, guard2, guard3, guard4, guard5)):
+            assert bool((t == 0x5A).all()), (i, at)
