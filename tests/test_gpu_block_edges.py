@@ -596,3 +596,93 @@ def test_calls_stay_within_their_workspaces(mx):
         mx.muon_step([t.clone() for t in mats], mats, [torch.zeros_like(t) for t in mats], workspace=ws, stream=stream())
         for at, t in enumerate((guard, guard2, guard3, guard4, guard5)):
             assert bool((t == 0x5A).all()), (i, at)
+
+
+# ------------------------------------------------- more than 2^31 elements to a tensor
+def sampled(count):
+    """The first and last rows, and some between."""
+    return torch.cat([torch.arange(16), torch.arange(count // 2, count // 2 + 16), torch.arange(count - 32, count)]).to("cuda")
+
+
+@pytest.mark.parametrize("k,plan", [(64, "gemm_kernel"), (512, "packed")])
+def test_linear_outputs_past_32_bit_offsets(mx, k, plan):
+    m, n = 66001, 33001  # 2.18e9 elements
+    assert mx.linear_variant(m, k, n).startswith(plan)
+    print("large linear", m, k, n, mx.linear_variant(m, k, n), "|", mx.linear_variant(m, k, n, True), flush=True)
+    g = gen(k)
+    x, w, b, dy = rand(g, m, k), rand(g, n, k, scale=k ** -0.5), rand(g, n), rand(g, m, n)
+    y, z = torch.empty(m, n, device="cuda"), torch.empty(m, n, device="cuda")
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    mx.linear_forward(x, w, b, y, activation=mx.ACT_SILU, residual=dy, z=z, stream=stream())
+    mx.linear_backward(dy, x, w, z, dx, dw, db, activation=mx.ACT_SILU, stream=stream())
+    d = lambda t: t.double()
+    r = sampled(m)
+    zr = d(x[r]) @ d(w).t() + d(b)
+    z_err = (k / 8 + 8) * U * (d(x[r]).abs() @ d(w).abs().t() + d(b).abs())
+    yr = F.silu(zr) + d(dy[r])
+    within(z[r], zr, z_err, "z")
+    within(y[r], yr, 1.13 * z_err + 16 * U * (zr.abs() + 1) + 4 * U * yr.abs(), "y")
+    dz, err = d(dy[r]) * slope("silu", d(z[r])), 16 * U * d(dy[r]).abs() * (d(z[r]).abs() + 1)
+    within(dx[r], dz @ d(w), ((n / 8 + 8) * U * dz.abs() + err) @ d(w).abs(), "dx")
+    c = sampled(n)
+    dz, err = d(dy[:, c]) * slope("silu", d(z[:, c])), 16 * U * d(dy[:, c]).abs() * (d(z[:, c]).abs() + 1)
+    within(dw[c], dz.t() @ d(x), ((m / 8 + 8) * U * dz.abs() + err).t() @ d(x).abs(), "dw")
+    within(db[c], dz.sum(0), ((m / 64 + 64) * U * dz.abs() + err).sum(0), "db")
+
+
+@pytest.mark.parametrize("rows,cols", [(140001, 16001), (70001, 32001)])
+def test_layer_norm_past_32_bit_offsets(mx, rows, cols):
+    print("large layer norm", rows, cols, flush=True)
+    g = gen(rows)
+    x, gamma, beta, dy = rand(g, rows, cols), rand(g, cols, mean=1.0), rand(g, cols), rand(g, rows, cols)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    mx.layer_norm_forward(x, gamma, beta, 1e-5, y, mean, rstd, stream=stream())
+    r = sampled(rows)
+    dg, db = torch.empty_like(gamma), torch.empty_like(beta)
+    xd, dyd, gd = x[r].double(), dy[r].double(), gamma.double()
+    rr = 1 / torch.sqrt(xd.var(1, correction=0, keepdim=True) + 1e-5)
+    xh = (xd - xd.mean(1, keepdim=True)) * rr
+    # unit rows: the statistics are off by 40 u, and everything behind them by a few u more
+    within(y[r], xh * gd + beta.double(), 60 * U * ((xh.abs() + 1) * gd.abs() + beta.double().abs()), "y")
+    c = sampled(cols)
+    xc = (x[:, c].double() - mean.double()[:, None]) * rstd.double()[:, None]
+    dyc = dy[:, c].double()
+    mx.layer_norm_backward(dy, x, mean, rstd, gamma, y, dg, db, stream=stream())
+    gr = dyd * gd
+    want = rr * (gr - gr.mean(1, keepdim=True) - xh * (gr * xh).mean(1, keepdim=True))
+    within(y[r], want, 100 * U * (gr.abs() + gr.abs().mean(1, keepdim=True) + xh.abs()) * rr, "dx")
+    deep = 64 + rows / 64
+    within(dg[c], (dyc * xc).sum(0), (deep * U * (dyc * xc).abs()).sum(0), "dgamma")
+    within(db[c], dyc.sum(0), (deep * U * dyc.abs()).sum(0), "dbeta")
+
+
+@pytest.mark.parametrize("rows,cols", [(900, 2400001), (2400001, 900), (130, 16777216)])
+def test_orthogonalize_past_32_bit_offsets(mx, rows, cols):
+    print("large orthogonalize", rows, cols, mx.orthogonalize_variant(rows, cols), flush=True)
+    g = gen(rows)
+    u = rand(g, rows, cols)
+    o = torch.empty_like(u)
+    mx.orthogonalize([u], [o], stream=stream())
+    mx.check(mx.lib().mx_empty_cache())
+    turned = rows > cols
+    x = u.t() if turned else u
+    s = min(rows, cols)
+    gram = torch.zeros(s, s, dtype=torch.double, device="cuda")
+    for part in x.split(1 << 18, dim=1):
+        p = part.double()
+        gram += p @ p.t()
+    norm2 = gram.diagonal().sum()
+    a, b, c = NS
+    eye = torch.eye(s, dtype=torch.double, device="cuda")
+    total, gram = eye / norm2.sqrt(), gram / norm2
+    for _ in range(5):  # X stays a polynomial of its first Gram matrix times itself
+        q = a * eye + b * gram + c * gram @ gram
+        total, gram = q @ total, q @ gram @ q
+    at = sampled(max(rows, cols))
+    want = total @ x[:, at].double()
+    got = (o[at].t() if turned else o[:, at]).double()
+    # FP32 sums of l terms, 16 to a rounding, are off by a walk of l / 16 of them in each
+    # iteration, which the later ones multiply as they do the pieces' errors.
+    worst = float(((got - want).norm(dim=0) / want.norm(dim=0)).max())
+    assert worst <= ORTH_TOL + 310 * U * math.sqrt(max(rows, cols) / 16), worst
+    print("worst column", worst)
