@@ -32,8 +32,13 @@ inline void copy_name(const std::string& name, char* buf, size_t len) {
 hipStream_t resolve_stream(void* s);
 int current_device();
 
-// Kernels that this thread's current call has launched (MX_LAUNCHED behind each).
-extern thread_local int64_t launches_of_call;
+// Kernels that this thread has launched (MX_LAUNCHED behind each), and how many of
+// them its last counted call did.
+extern thread_local int64_t launches, launches_of_call;
+struct CountedCall {
+  const int64_t from = launches;
+  ~CountedCall() { launches_of_call = launches - from; }
+};
 
 // Returns a block to its pool; the call's error message, if it is failing, stays.
 void release_scratch(void* ptr);
@@ -119,7 +124,7 @@ int gemm_describe(const mx_gemm_desc* d, const float* a, const float* b, int64_t
 #define MX_LAUNCHED()            \
   do {                           \
     MX_HIP(hipGetLastError());   \
-    ++::mx::launches_of_call;    \
+    ++::mx::launches;            \
   } while (0)
 
 #define MX_REQUIRE(cond, code, ...) \

@@ -432,7 +432,7 @@ using namespace mx;
 extern "C" int mx_layer_norm_forward(const float* x, const float* gamma, const float* beta, int64_t rows, int64_t cols,
                                      float eps, float* y, float* mean, float* rstd, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   MX_TRY(check("mx_layer_norm_forward", rows, cols));
   if (rows == 0) return MX_OK;
   MX_REQUIRE(x && y, MX_ERR_INVALID, "mx_layer_norm_forward: null buffer");
@@ -468,7 +468,7 @@ extern "C" int mx_layer_norm_backward(const float* dy, const float* x, const flo
                                       const float* gamma, int64_t rows, int64_t cols, float* dx, float* dgamma,
                                       float* dbeta, void* workspace, int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   MX_TRY(check("mx_layer_norm_backward", rows, cols));
   const bool affine = dgamma || dbeta;
   if (!dx && !affine) return MX_OK;

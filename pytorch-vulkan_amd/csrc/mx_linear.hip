@@ -1257,7 +1257,7 @@ extern "C" int mx_linear_forward(const float* x, const float* w, const float* bi
                                  int64_t k, int64_t n, int activation, float* y, float* z, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   const char* const who = "mx_linear_forward";
   MX_TRY(check(who, m, k, n, activation));
   if (m == 0 || n == 0) return MX_OK;
@@ -1328,7 +1328,7 @@ extern "C" int mx_linear_backward(const float* dy, const float* x, const float* 
                                   int64_t n, int activation, float* dx, float* dw, float* db, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   const char* const who = "mx_linear_backward";
   MX_TRY(check(who, m, k, n, activation));
   hipStream_t s = resolve_stream(stream);

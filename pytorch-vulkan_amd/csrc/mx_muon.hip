@@ -1055,7 +1055,7 @@ extern "C" int mx_orthogonalize_variant(int64_t rows, int64_t cols, int64_t coun
 extern "C" int mx_orthogonalize(const mx_matrix_pair* matrices, int64_t count, const mx_newton_schulz* ns, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   const char* const who = "mx_orthogonalize";
   MX_REQUIRE(ns, MX_ERR_INVALID, who, ": null parameters");
   MX_TRY(check_ns(who, *ns));
@@ -1089,7 +1089,7 @@ extern "C" int mx_muon_workspace(const mx_muon_tensor* tensors, int64_t count, i
 extern "C" int mx_muon_step(const mx_muon_tensor* tensors, int64_t count, const mx_muon_hparams* hp, void* workspace,
                             int64_t workspace_bytes, void* stream) {
   MX_ABI_BEGIN
-  launches_of_call = 0;
+  const CountedCall counted;
   const char* const who = "mx_muon_step";
   MX_REQUIRE(hp, MX_ERR_INVALID, who, ": null hyperparameters");
   MX_REQUIRE(hp->lr >= 0 && hp->weight_decay >= 0 && hp->momentum >= 0 && hp->momentum <= 1 && std::isfinite(hp->lr) &&

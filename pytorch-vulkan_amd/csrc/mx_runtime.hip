@@ -650,7 +650,7 @@ int upload(const void* host, size_t bytes, hipStream_t s, Scratch& holder) {
   return MX_OK;
 }
 
-thread_local int64_t launches_of_call = 0;
+thread_local int64_t launches = 0, launches_of_call = 0;
 
 // ---------------------------------------------------------------- workspaces
 bool may_allocate(hipStream_t s) {

@@ -331,6 +331,10 @@ def test_launches_are_counted(mx):
     assert mx.last_launches() in (4, 5), "two passes, product, (join,) the products behind"
     mx.linear_backward(x, x, w, None, e(2048, 2048), e(2048, 2048), None, stream=stream())
     assert mx.last_launches() in (5, 6)
+    before = mx.last_launches()
+    mx.gemm(w, w, e(2048, 2048), stream=stream())
+    mx.linear_workspace(64, 64, 64)
+    assert mx.last_launches() == before, "other calls do not count"
     mx.linear_backward(x[:0], x[:0], w, None, None, None, None, stream=stream())
     assert mx.last_launches() == 0
 
