@@ -208,17 +208,7 @@ def _inputs(case, seed):
 
 
 def prepare(case, seed):
-    state = dict(_inputs(case, seed), case=case)
-    if own:
-        # What a program keeps from call to call beside its tensors: the
-        # rotation's table, the cache and the batch's shape.
-        mx = _mx()
-        if case["kind"] == "rotary":
-            state["plan"] = mx.Rotary(_frequencies(case), interleaved=case["interleaved"])
-        elif case["kind"] != "attention":
-            state["cache"] = mx.KVCache(state["kc"], state["vc"], state.get("ks"), state.get("vs"))
-            state["batch"] = mx.KVBatch(state["table"], state["lengths"], case["sequences"] * case["new"])
-    return state
+    return dict(_inputs(case, seed), case=case)
 
 
 # --------------------------------------------------------------- operators
@@ -366,19 +356,33 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def _kept(t, name, make):
+    """What a program keeps from call to call beside its tensors: made on a state's first pass."""
+    if name not in t:
+        t[name] = make()
+    return t[name]
+
+
+def _cache(t, c):
+    mx = _mx()
+    return (_kept(t, "cache", lambda: mx.KVCache(t["kc"], t["vc"], t.get("ks"), t.get("vs"))),
+            _kept(t, "batch", lambda: mx.KVBatch(t["table"], t["lengths"], c["sequences"] * c["new"])))
+
+
 def _own_rotary(t, c):
     mx, q, k = _mx(), t["q"], t["k"]
+    plan = _kept(t, "plan", lambda: mx.Rotary(_frequencies(c), interleaved=c["interleaved"]))
     norm = dict(q_weight=t["qw"], k_weight=t["kw"], eps=EPS) if c["norm"] else {}
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-    mx.qk_norm_rotary_forward(q, k, t["positions"], t["plan"], q_out, k_out, stream=_stream(), **norm)
+    mx.qk_norm_rotary_forward(q, k, t["positions"], plan, q_out, k_out, stream=_stream(), **norm)
     if not c["train"]:
         return [q_out, k_out]
     dq, dk = torch.empty_like(q), torch.empty_like(k)
     if not c["norm"]:
-        mx.qk_norm_rotary_backward(t["dq"], t["dk"], None, None, t["positions"], t["plan"], dq, dk, stream=_stream())
+        mx.qk_norm_rotary_backward(t["dq"], t["dk"], None, None, t["positions"], plan, dq, dk, stream=_stream())
         return [q_out, k_out, dq, dk]
     dqw, dkw = torch.empty_like(t["qw"]), torch.empty_like(t["kw"])
-    mx.qk_norm_rotary_backward(t["dq"], t["dk"], q, k, t["positions"], t["plan"], dq, dk, dqw, dkw, stream=_stream(), **norm)
+    mx.qk_norm_rotary_backward(t["dq"], t["dk"], q, k, t["positions"], plan, dq, dk, dqw, dkw, stream=_stream(), **norm)
     return [q_out, k_out, dq, dqw, dk, dkw]
 
 
@@ -399,14 +403,16 @@ def _own_attention(t, c):
 def _own_cache(t, c):
     mx, s = _mx(), _stream()
     k, v = torch.empty_like(t["k"]), torch.empty_like(t["v"])
-    mx.kv_cache_write(t["cache"], t["batch"], t["k"], t["v"], stream=s)
-    mx.kv_cache_read(t["cache"], t["batch"], k, v, stream=s)
+    cache, batch = _cache(t, c)
+    mx.kv_cache_write(cache, batch, t["k"], t["v"], stream=s)
+    mx.kv_cache_read(cache, batch, k, v, stream=s)
     return [k, v]
 
 
 def _own_paged(t, c):
     out = torch.empty_like(t["q"])
-    _mx().attention_paged(t["cache"], t["batch"], t["q"], out, window=c["window"], sinks=c["sinks"], stream=_stream())
+    cache, batch = _cache(t, c)
+    _mx().attention_paged(cache, batch, t["q"], out, window=c["window"], sinks=c["sinks"], stream=_stream())
     return [out]
 
 
