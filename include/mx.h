@@ -509,8 +509,8 @@ int mx_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t src_pitc
 /* must not do (MX_ERR_WORKSPACE).                                            */
 /* ------------------------------------------------------------------------ */
 
-/* Kernels that this thread's last mx_layer_norm_*, mx_linear_*, mx_orthogonalize
- * or mx_muon_step has launched (its workspace queries launch none and count none). */
+/* Kernels that this thread's last mx_layer_norm_*, mx_linear_*, mx_orthogonalize,
+ * mx_muon_step, mx_qk_norm_rotary_*, mx_attention_* or mx_kv_cache_* has launched (its workspace queries launch none and count none). */
 int64_t mx_last_launches(void);
 
 /* Layer norm over the last axis of x [rows, cols]:
@@ -598,6 +598,116 @@ typedef struct mx_muon_hparams {
 int mx_muon_step(const mx_muon_tensor* tensors, int64_t count, const mx_muon_hparams* hp, void* workspace,
                  int64_t workspace_bytes, void* stream);
 int mx_muon_workspace(const mx_muon_tensor* tensors, int64_t count, int64_t* bytes);
+
+/* ------------------------------------------------------------------------ */
+/* The attention layer of a language model (FP32).  No counterparts in the    */
+/* reference.  Scratch as for the block above; mx_last_launches counts these   */
+/* calls too.  Tokens of several sequences lie behind each other ("packed"),   */
+/* [tokens, heads, head_dim] with the last axis contiguous and the strides of  */
+/* the others, in elements, in the descriptor.                                */
+/* ------------------------------------------------------------------------ */
+
+/* Norm of queries and keys for each head, and rotary positions, in one pass:
+ *   xh = x / sqrt(mean(x^2) + eps) * weight   (norm != 0; weight NULL: 1)   or   xh = x,
+ *   (a, b) -> magnitude (a cos t - b sin t, b cos t + a sin t),  t = positions[token] frequencies[i],
+ * on pairs i < rotary_dim / 2 of the head's first rotary_dim elements: (2 i, 2 i + 1)
+ * where interleaved, else (i, i + rotary_dim / 2); the others stay xh.  frequencies is
+ * host memory, read during the call: any scaling for long contexts is in it and in
+ * magnitude.  Angles are reduced in 64 bits. */
+typedef struct mx_rotary_desc {
+  int64_t tokens, q_heads, k_heads; /* either number of heads may be 0 */
+  int64_t head_dim;                 /* 1 to 256 */
+  int64_t rotary_dim;               /* even, 0 to head_dim */
+  int64_t q_token, q_head, k_token, k_head; /* strides of q and k */
+  const int64_t* positions;         /* device, [tokens]; may be NULL where rotary_dim is 0 */
+  const double* frequencies;        /* host, [rotary_dim / 2] */
+  double magnitude;
+  double eps;
+  int interleaved, norm;
+} mx_rotary_desc;
+/* q_out and k_out are contiguous; each may be its own input where that is
+ * contiguous, no other operands may overlap an output. */
+int mx_qk_norm_rotary_forward(const mx_rotary_desc* d, const float* q, const float* k, const float* q_weight,
+                              const float* k_weight, float* q_out, float* k_out, void* stream);
+/* Gradients with respect to q, k and the weights, from those of the outputs
+ * (contiguous, as are dq and dk).  Any of dq, dk, dq_weight, dk_weight may be NULL
+ * (not computed); q and k are read with a norm only.  dq may be dq_out and dk
+ * dk_out.  The weights' sums are taken in a fixed order. */
+int mx_qk_norm_rotary_backward(const mx_rotary_desc* d, const float* dq_out, const float* dk_out, const float* q,
+                               const float* k, const float* q_weight, const float* k_weight, float* dq, float* dk,
+                               float* dq_weight, float* dk_weight, void* workspace, int64_t workspace_bytes, void* stream);
+int mx_qk_norm_rotary_workspace(const mx_rotary_desc* d, int64_t* bytes);
+
+/* Causal attention of packed sequences: row i of a sequence sees its keys j <= i
+ * with i - j < window or j < sinks (window == 0: all of them),
+ *   out_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i),
+ * heads / kv_heads query heads to a key head.  Rows that belong to no sequence are left
+ * as they are, in every output.  A row that sees a NaN or an infinity is NaN, and so are
+ * the gradients that it reaches; those of keys and queries that a row does not see
+ * have no effect on it. */
+typedef struct mx_attention_desc {
+  int64_t tokens, sequences;
+  const int32_t* starts; /* device, [sequences + 1], ascending: sequence b is rows starts[b] .. starts[b + 1] - 1;
+                          * NULL: tokens / sequences each.  Entries outside 0 .. tokens count as the nearer end. */
+  int64_t heads, kv_heads;
+  int64_t head_dim;      /* 1 to 128 */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides of q, k and v */
+  int64_t window, sinks;
+  double scale;
+} mx_attention_desc;
+/* out [tokens, heads, head_dim] and lse [heads, tokens] (may be NULL) are contiguous.
+ * FP32 products throughout: an element is held to 24 bits down to 2^-110, below to 2^-134. */
+int mx_attention_forward(const mx_attention_desc* d, const float* q, const float* k, const float* v, float* out,
+                         float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+/* From the forward's out and lse; dout and the gradients are contiguous, dq with dk
+ * and dv or either side alone (NULL: not computed).  Sums are taken in a fixed order. */
+int mx_attention_backward(const mx_attention_desc* d, const float* dout, const float* q, const float* k, const float* v,
+                          const float* out, const float* lse, float* dq, float* dk, float* dv, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int mx_attention_workspace(const mx_attention_desc* d, int backward, int64_t* bytes);
+
+/* A paged cache of keys and values: k [pages, heads, page_size, head_dim] and
+ * v [pages, heads, head_dim, page_size], contiguous, 16-byte aligned, page_size and head_dim multiples of
+ * 16, head_dim at most 128.  MX_KV_I8 keeps x as a signed byte n and a scale of its token and head
+ * ([pages, heads, page_size] for k and for v): scale = max|x| / 127, n = x / scale rounded half to even
+ * (0 where the scale is 0), x = n scale; a row with NaN or an infinity has a NaN scale. */
+enum mx_kv_type { MX_KV_F32 = 0, MX_KV_I8 = 1 };
+typedef struct mx_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale; /* NULL for MX_KV_F32 */
+  int64_t pages, heads, page_size, head_dim;
+  int type;
+} mx_kv_cache;
+/* New tokens of several sequences, packed, and where their sequences lie in a cache:
+ * position p of sequence b is place p % page_size of page table[b][p / page_size].  lengths[b]
+ * counts the sequence's tokens with its new ones, which are its last.  A position that is negative, past
+ * the table, or whose page is not one of the cache's is absent: not written, read as zero,
+ * seen by no row (a window's released pages may stay in the table as -1). */
+typedef struct mx_kv_batch {
+  int64_t tokens, sequences, table_width;
+  const int32_t* starts;  /* device, as in mx_attention_desc */
+  const int32_t* lengths; /* device, [sequences] */
+  const int32_t* table;   /* device, [sequences, table_width] */
+} mx_kv_batch;
+/* Writes k and v [tokens, cache->heads, head_dim] (strides of the token and the head) to
+ * the cache.  Two new tokens that share a place leave either one's row or a mixture. */
+int mx_kv_cache_write(const mx_kv_cache* c, const mx_kv_batch* b, const float* k, int64_t k_token, int64_t k_head,
+                      const float* v, int64_t v_token, int64_t v_head, void* stream);
+/* Reads them back into contiguous k and v (lengths' last tokens; all of a sequence where
+ * it has as many rows as lengths says).  Rows that belong to no sequence are left as they are. */
+int mx_kv_cache_read(const mx_kv_cache* c, const mx_kv_batch* b, float* k, float* v, void* stream);
+/* Attention of the new tokens over the cache, which holds them already: a row at
+ * position i sees positions j as in mx_attention_desc.  q has the given strides, out
+ * [tokens, heads, head_dim] is contiguous; a row that sees nothing is 0. */
+typedef struct mx_paged_desc {
+  int64_t heads;
+  int64_t q_token, q_head;
+  int64_t window, sinks;
+  double scale;
+} mx_paged_desc;
+int mx_attention_paged(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b, const float* q, float* out,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int mx_attention_paged_workspace(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b, int64_t* bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,371 @@
+// Norm of queries and keys for each head and rotary positions, in one pass (FP32).
+//
+//   forward   r = (mean x^2 + eps)^-1/2,  xh = x r w   (without a norm xh = x)
+//             y_a = xh_a c - xh_b s,  y_b = xh_b c + xh_a s   on the pairs (a, b) of the
+//             head's first rotary_dim elements, c and s = magnitude (cos, sin)(position f_i)
+//   backward  g = the same rotation by the opposite angle of dy,  gw = g w,
+//             dx = r (gw - x r mean(gw x r)),  dw = sum over tokens and heads g x r
+//
+// Bound by memory: 8 bytes an element forward, 12 backward with a norm.  A row (one
+// head of one token) stays in the registers of a group of 8 to 64 lanes, four
+// elements each; what an element is paired with is read again from the row, which the
+// first-level cache holds.  A workgroup takes all heads of its tokens, so an angle is
+// evaluated once a token: in 64 bits down to a fraction of a turn (a position of 10^6
+// at frequency 1 has 20 bits before the point, and FP32 would leave 4 behind), then
+// sine and cosine of that fraction in FP32.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "mx_internal.hpp"
+
+namespace mx {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kMaxDim = 256, kThreads = 256, kAngles = 2048;  // kAngles: pairs of a workgroup's tokens in LDS
+
+struct Rotary {
+  int tokens, q_heads, k_heads, dim, rot;
+  int64_t q_token, q_head, k_token, k_head;
+  const int64_t* positions;
+  float magnitude, eps;
+  int interleaved, norm, group;  // group: tokens that a workgroup turns together
+  double turns[kMaxDim / 2];     // frequencies / 2 pi
+};
+
+struct Operands {  // q's and k's
+  const float *x[2], *dy[2], *w[2];
+  float *out[2], *part;
+  bool wanted[2];  // a side that nothing is asked of is not read
+};
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < L; m <<= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// Elements e .. e + 3 of a row of n, zero past its end.
+__device__ __forceinline__ f32x4 load4(const float* row, int e, int n) {
+  if (e + 4 <= n) return *reinterpret_cast<const f32x4u*>(row + e);
+  f32x4 v{};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (e + i < n) v[i] = row[e + i];
+  return v;
+}
+__device__ __forceinline__ void store4(float* row, int e, int n, f32x4 v) {
+  if (e + 4 <= n) {
+    *reinterpret_cast<f32x4u*>(row + e) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (e + i < n) row[e + i] = v[i];
+}
+
+// Which element e is paired with, and whether it is a pair's first.
+__device__ __forceinline__ int partner(const Rotary& p, int e, bool& first) {
+  if (e >= p.rot) return first = true, e;
+  const int half = p.rot >> 1;
+  first = p.interleaved ? !(e & 1) : e < half;
+  return p.interleaved ? e ^ 1 : first ? e + half : e - half;
+}
+
+// cos and sin (times the magnitude) of a workgroup's tokens, [token][pair].
+__device__ __forceinline__ void angles(const Rotary& p, int first, int count, float* cs, float* sn) {
+  const int half = p.rot >> 1;
+  for (int i = threadIdx.x; i < count * half; i += kThreads) {
+    const int t = i / half, pair = i - t * half;
+    const double turn = double(p.positions[first + t]) * p.turns[pair];
+    const float frac = float(turn - rint(turn));
+    float s, c;
+    sincospif(2.f * frac, &s, &c);
+    cs[i] = c * p.magnitude;
+    sn[i] = s * p.magnitude;
+  }
+  __syncthreads();
+}
+
+// The rows of tokens first .. first + count - 1: q's heads of each, then k's.  A group of L
+// lanes takes every kThreads / L-th, whichever side is wanted, so that the weights' sums
+// keep their order; f(which of q and k, token, its place, head).
+template <int L, class F>
+__device__ __forceinline__ void rows(const Rotary& p, const bool (&wanted)[2], int first, int count, F&& f) {
+  const int heads = p.q_heads + p.k_heads;
+  for (int r = threadIdx.x / L; r < count * heads; r += kThreads / L) {
+    const int t = r / heads, h = r - t * heads, k = h >= p.q_heads;
+    if (k ? wanted[1] : wanted[0]) f(k, first + t, t, k ? h - p.q_heads : h);
+  }
+}
+
+template <int L, bool BACK>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const Operands o) {
+  __shared__ float cs[kAngles], sn[kAngles], sums[BACK ? 2 * kMaxDim : 1];
+  const int lane = threadIdx.x % L, e = lane * 4, half = p.rot >> 1;
+  f32x4 w[2] = {f32x4{1, 1, 1, 1}, f32x4{1, 1, 1, 1}};
+  int with[4], pair[4];  // each element's partner and pair
+  bool head[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    with[i] = min(partner(p, e + i, head[i]), p.dim - 1);
+    pair[i] = e + i >= p.rot ? -1 : p.interleaved ? (e + i) >> 1 : (e + i) % half;
+  }
+  // A lane's four partners lie together, the same four for neighbouring pairs.
+  const bool own = p.interleaved || p.rot == 0, run = !own && half % 4 == 0 && e < p.rot;
+  float wp[2][4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (p.norm && o.w[k]) w[k] = load4(o.w[k], e, p.dim);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wp[k][i] = p.norm && o.w[k] ? o.w[k][with[i]] : 1.f;
+  }
+  f32x4 dw[2] = {};
+  for (int first = blockIdx.x * p.group; first < p.tokens; first += gridDim.x * p.group) {
+    const int count = min(p.group, p.tokens - first);
+    if (half) angles(p, first, count, cs, sn);
+    rows<L>(p, o.wanted, first, count, [&](int k, int token, int place, int h) {
+      const int heads = k ? p.k_heads : p.q_heads;
+      const int64_t flat = (int64_t(token) * heads + h) * p.dim;
+      const int64_t at = token * (k ? p.k_token : p.q_token) + h * (k ? p.k_head : p.q_head);
+      const float* const turned = BACK ? o.dy[k] + flat : o.x[k] + at;  // the row that the rotation is applied to
+      const f32x4 v = load4(turned, e, p.dim);
+      f32x4 u = v;  // its partners
+      if (!own) {
+        if (run) {
+          u = *reinterpret_cast<const f32x4u*>(turned + with[0]);
+        } else if (e < p.rot) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[i] = turned[with[i]];
+        }
+      } else if (p.rot) {
+        u = f32x4{v[1], v[0], v[3], v[2]};
+      }
+      f32x4 c, s;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = pair[i] < 0 ? 1.f : cs[place * half + pair[i]];
+        s[i] = pair[i] < 0 ? 0.f : sn[place * half + pair[i]];
+        if (head[i] != BACK) s[i] = -s[i];
+      }
+      f32x4 y;
+      if constexpr (!BACK) {
+        float r = 1;
+        if (p.norm) {
+          r = 1.f / sqrtf(lanes_sum<L>(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]) / p.dim + p.eps);
+          const f32x4 wk = k ? w[1] : w[0];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float xh = v[i] * r * wk[i], xp = u[i] * r * (k ? wp[1][i] : wp[0][i]);
+            y[i] = pair[i] < 0 ? xh : fmaf(xp, s[i], xh * c[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = pair[i] < 0 ? v[i] : fmaf(u[i], s[i], v[i] * c[i]);
+        }
+      } else {
+        f32x4 g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = pair[i] < 0 ? v[i] : fmaf(u[i], s[i], v[i] * c[i]);
+        y = g;
+        if (p.norm) {
+          const f32x4 x = load4(o.x[k] + at, e, p.dim), wk = k ? w[1] : w[0];
+          const float r = 1.f / sqrtf(lanes_sum<L>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) / p.dim + p.eps);
+          const f32x4 xr = x * r, gw = g * wk;
+          const float m = lanes_sum<L>(gw[0] * xr[0] + gw[1] * xr[1] + gw[2] * xr[2] + gw[3] * xr[3]) / p.dim;
+          y = (gw - xr * m) * r;
+          if (k) dw[1] += g * xr;
+          else dw[0] += g * xr;
+        }
+      }
+      if (float* const out = o.out[k]) store4(out + flat, e, p.dim, y);
+    });
+    if (half) __syncthreads();
+  }
+  if constexpr (BACK) {
+    if (!o.part) return;
+    // Column sums of the workgroup, its lane groups one after the other.
+    for (int g = 0; g < kThreads / L; ++g) {
+      if (int(threadIdx.x) / L == g) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float* const at = sums + k * kMaxDim + e + i;
+            *at = g ? *at + dw[k][i] : dw[k][i];
+          }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 2 * p.dim; i += kThreads)
+      o.part[int64_t(blockIdx.x) * 2 * p.dim + i] = sums[i / p.dim * kMaxDim + i % p.dim];
+  }
+}
+
+// dw[i] = the sum of the workgroups' parts: 32 columns to a workgroup, 32 rows of threads.
+__global__ __launch_bounds__(1024) void rotary_weights_kernel(const float* part, int parts, int dim, float* dqw, float* dkw) {
+  __shared__ float sums[32][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  float s = 0;
+  if (col < 2 * dim)
+    for (int i = row; i < parts; i += 32) s += part[int64_t(i) * 2 * dim + col];
+  sums[row][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (row || col >= 2 * dim) return;
+  s = 0;
+  for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
+  float* const out = col < dim ? dqw : dkw;
+  if (out) out[col % dim] = s;
+}
+
+__global__ void rotary_zero_kernel(float* a, float* b, int dim) {
+  const int i = threadIdx.x;
+  if (i < dim && a) a[i] = 0;
+  if (i < dim && b) b[i] = 0;
+}
+
+int check(const char* who, const mx_rotary_desc* d) {
+  MX_REQUIRE(d, MX_ERR_INVALID, who, ": null descriptor");
+  MX_REQUIRE(d->tokens >= 0 && d->q_heads >= 0 && d->k_heads >= 0, MX_ERR_INVALID, who, ": negative size");
+  MX_REQUIRE(d->head_dim >= 1 && d->head_dim <= kMaxDim, MX_ERR_INVALID, who, ": head_dim must be 1 to ", kMaxDim, ", got ",
+             d->head_dim);
+  MX_REQUIRE(d->rotary_dim >= 0 && d->rotary_dim <= d->head_dim && d->rotary_dim % 2 == 0, MX_ERR_INVALID, who,
+             ": rotary_dim must be even and at most head_dim, got ", d->rotary_dim);
+  MX_REQUIRE(d->tokens <= (1 << 30) && d->q_heads <= (1 << 20) && d->k_heads <= (1 << 20), MX_ERR_INVALID, who,
+             ": size out of range");
+  MX_REQUIRE(d->rotary_dim == 0 || d->frequencies, MX_ERR_INVALID, who, ": null frequencies");
+  for (int64_t i = 0; i < d->rotary_dim / 2; ++i)
+    MX_REQUIRE(std::isfinite(d->frequencies[i]), MX_ERR_INVALID, who, ": frequencies must be finite");
+  MX_REQUIRE(std::isfinite(d->magnitude), MX_ERR_INVALID, who, ": the magnitude must be finite");
+  MX_REQUIRE(!d->norm || (std::isfinite(d->eps) && d->eps >= 0), MX_ERR_INVALID, who, ": eps must not be negative");
+  return MX_OK;
+}
+
+Rotary params(const mx_rotary_desc* d) {
+  Rotary p{};
+  p.tokens = int(d->tokens), p.q_heads = int(d->q_heads), p.k_heads = int(d->k_heads);
+  p.dim = int(d->head_dim), p.rot = int(d->rotary_dim);
+  p.q_token = d->q_token, p.q_head = d->q_head, p.k_token = d->k_token, p.k_head = d->k_head;
+  p.positions = d->positions;
+  p.magnitude = float(d->magnitude), p.eps = float(d->eps);
+  p.interleaved = d->interleaved, p.norm = d->norm;
+  for (int i = 0; i < p.rot / 2; ++i) p.turns[i] = d->frequencies[i] / 6.283185307179586476925286766559;
+  return p;
+}
+
+int lanes_of(int dim) {
+  for (int l = 8; l < 64; l *= 2)
+    if (dim <= 4 * l) return l;
+  return 64;
+}
+
+// Tokens that a workgroup turns together: two rows for each of its lane groups, as far as
+// their angles fit LDS.
+int group_of(int dim, int rot, int64_t heads) {
+  const int64_t slots = kThreads / lanes_of(dim);
+  int64_t g = std::max<int64_t>(1, 2 * slots / heads);
+  if (rot) g = std::min<int64_t>(g, kAngles / (rot / 2));
+  return int(g);
+}
+
+int blocks_of(const Rotary& p, bool parts) {
+  const int64_t all = (p.tokens + p.group - 1) / p.group;
+  return int(std::min<int64_t>(all, int64_t(cu_count()) * (parts ? 8 : 64)));
+}
+
+template <bool BACK>
+void launch(const Rotary& p, const Operands& o, int blocks, hipStream_t s) {
+  switch (lanes_of(p.dim)) {
+    case 8: hipLaunchKernelGGL((rotary_kernel<8, BACK>), dim3(blocks), dim3(kThreads), 0, s, p, o); break;
+    case 16: hipLaunchKernelGGL((rotary_kernel<16, BACK>), dim3(blocks), dim3(kThreads), 0, s, p, o); break;
+    case 32: hipLaunchKernelGGL((rotary_kernel<32, BACK>), dim3(blocks), dim3(kThreads), 0, s, p, o); break;
+    default: hipLaunchKernelGGL((rotary_kernel<64, BACK>), dim3(blocks), dim3(kThreads), 0, s, p, o); break;
+  }
+}
+
+}  // namespace
+}  // namespace mx
+
+using namespace mx;
+
+extern "C" int mx_qk_norm_rotary_forward(const mx_rotary_desc* d, const float* q, const float* k, const float* q_weight,
+                                         const float* k_weight, float* q_out, float* k_out, void* stream) {
+  MX_ABI_BEGIN
+  const CountedCall counted;
+  const char* const who = "mx_qk_norm_rotary_forward";
+  MX_TRY(check(who, d));
+  const int64_t heads = d->q_heads + d->k_heads;
+  if (d->tokens == 0 || heads == 0) return MX_OK;
+  MX_REQUIRE((d->q_heads == 0 || (q && q_out)) && (d->k_heads == 0 || (k && k_out)) && (d->rotary_dim == 0 || d->positions),
+             MX_ERR_INVALID, who, ": null buffer");
+  Rotary p = params(d);
+  p.group = group_of(p.dim, p.rot, heads);
+  const Operands o{{q, k}, {nullptr, nullptr}, {q_weight, k_weight}, {q_out, k_out}, nullptr, {true, true}};
+  launch<false>(p, o, blocks_of(p, false), resolve_stream(stream));
+  MX_LAUNCHED();
+  return MX_OK;
+  MX_ABI_END
+}
+
+namespace {
+// Bytes of the workgroups' parts of the weights' gradients.
+int64_t rotary_workspace(const mx_rotary_desc* d) {
+  const int64_t heads = d->q_heads + d->k_heads;
+  if (!d->norm || d->tokens == 0 || heads == 0) return 0;
+  const int64_t group = group_of(int(d->head_dim), int(d->rotary_dim), heads);
+  return std::min<int64_t>((d->tokens + group - 1) / group, int64_t(cu_count()) * 8) * 2 * d->head_dim * 4;
+}
+}  // namespace
+
+extern "C" int mx_qk_norm_rotary_workspace(const mx_rotary_desc* d, int64_t* bytes) {
+  MX_ABI_BEGIN
+  MX_TRY(check("mx_qk_norm_rotary_workspace", d));
+  MX_REQUIRE(bytes, MX_ERR_INVALID, "mx_qk_norm_rotary_workspace: null result");
+  *bytes = rotary_workspace(d);
+  return MX_OK;
+  MX_ABI_END
+}
+
+extern "C" int mx_qk_norm_rotary_backward(const mx_rotary_desc* d, const float* dq_out, const float* dk_out, const float* q,
+                                          const float* k, const float* q_weight, const float* k_weight, float* dq,
+                                          float* dk, float* dq_weight, float* dk_weight, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
+  MX_ABI_BEGIN
+  const CountedCall counted;
+  const char* const who = "mx_qk_norm_rotary_backward";
+  MX_TRY(check(who, d));
+  MX_REQUIRE(d->norm || (!dq_weight && !dk_weight), MX_ERR_INVALID, who, ": gradients of weights without a norm");
+  const int64_t heads = d->q_heads + d->k_heads;
+  hipStream_t s = resolve_stream(stream);
+  const bool weights = dq_weight || dk_weight;
+  if (d->tokens == 0 || heads == 0) {
+    if (!weights) return MX_OK;
+    hipLaunchKernelGGL(rotary_zero_kernel, dim3(1), dim3(kMaxDim), 0, s, dq_weight, dk_weight, int(d->head_dim));
+    MX_LAUNCHED();
+    return MX_OK;
+  }
+  if (!dq && !dk && !weights) return MX_OK;
+  const bool qs = dq || dq_weight, ks = dk || dk_weight;
+  MX_REQUIRE((!qs || d->q_heads == 0 || (dq_out && (!d->norm || q))) && (!ks || d->k_heads == 0 || (dk_out && (!d->norm || k))) &&
+                 (d->rotary_dim == 0 || d->positions),
+             MX_ERR_INVALID, who, ": null buffer");
+  Workspace ws;
+  if (weights) MX_TRY(ws.take(who, workspace, workspace_bytes, rotary_workspace(d), s));
+  Rotary p = params(d);
+  p.group = group_of(p.dim, p.rot, heads);
+  const Operands o{{q, k}, {dq_out, dk_out}, {q_weight, k_weight}, {dq, dk}, ws.as<float>(), {qs, ks}};
+  const int blocks = blocks_of(p, weights);
+  launch<true>(p, o, blocks, s);
+  MX_LAUNCHED();
+  if (!weights) return MX_OK;
+  hipLaunchKernelGGL(rotary_weights_kernel, dim3((2 * p.dim + 31) / 32), dim3(1024), 0, s, ws.as<float>(), blocks, p.dim,
+                     dq_weight, dk_weight);
+  MX_LAUNCHED();
+  return MX_OK;
+  MX_ABI_END
+}

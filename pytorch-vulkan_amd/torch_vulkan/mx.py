@@ -47,6 +47,9 @@ EXPORTS = [
     "mx_layer_norm_backward_workspace", "mx_linear_forward", "mx_linear_backward", "mx_linear_workspace",
     "mx_orthogonalize", "mx_orthogonalize_workspace", "mx_muon_step", "mx_muon_workspace", "mx_last_launches",
     "mx_linear_variant", "mx_orthogonalize_variant",
+    "mx_qk_norm_rotary_forward", "mx_qk_norm_rotary_backward", "mx_qk_norm_rotary_workspace", "mx_attention_forward",
+    "mx_attention_backward", "mx_attention_workspace", "mx_kv_cache_write", "mx_kv_cache_read", "mx_attention_paged",
+    "mx_attention_paged_workspace",
 ]
 
 
@@ -108,6 +111,34 @@ class MuonTensor(C.Structure):
 class MuonHParams(C.Structure):
     _fields_ = [("lr", C.c_double), ("weight_decay", C.c_double), ("momentum", C.c_double), ("nesterov", C.c_int),
                 ("adjust_lr", C.c_int), ("ns", NewtonSchulz)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [*((n, C.c_int64) for n in ("tokens", "q_heads", "k_heads", "head_dim", "rotary_dim", "q_token", "q_head",
+                                           "k_token", "k_head")),
+                ("positions", C.c_void_p), ("frequencies", C.c_void_p), ("magnitude", C.c_double), ("eps", C.c_double),
+                ("interleaved", C.c_int), ("norm", C.c_int)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("sequences", C.c_int64), ("starts", C.c_void_p),
+                *((n, C.c_int64) for n in ("heads", "kv_heads", "head_dim", "q_token", "q_head", "k_token", "k_head",
+                                           "v_token", "v_head", "window", "sinks")),
+                ("scale", C.c_double)]
+
+
+class KVCacheDesc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                *((n, C.c_int64) for n in ("pages", "heads", "page_size", "head_dim")), ("type", C.c_int)]
+
+
+class KVBatchDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("sequences", C.c_int64), ("table_width", C.c_int64), ("starts", C.c_void_p),
+                ("lengths", C.c_void_p), ("table", C.c_void_p)]
+
+
+class PagedDesc(C.Structure):
+    _fields_ = [*((n, C.c_int64) for n in ("heads", "q_token", "q_head", "window", "sinks")), ("scale", C.c_double)]
 
 
 class MemoryStats(C.Structure):
@@ -193,6 +224,18 @@ def lib() -> C.CDLL:
             "mx_mse_loss_f32": ([vp, vp, i64, i32, vp, vp], i32),
             "mx_mse_loss_backward_f32": ([vp, vp, vp, i64, i32, vp, vp], i32),
             "mx_copy_rows": ([vp, i64, vp, i64, i64, i64, vp], i32),
+            "mx_qk_norm_rotary_forward": ([C.POINTER(RotaryDesc)] + [vp] * 7, i32),
+            "mx_qk_norm_rotary_backward": ([C.POINTER(RotaryDesc)] + [vp] * 11 + [i64, vp], i32),
+            "mx_qk_norm_rotary_workspace": ([C.POINTER(RotaryDesc), C.POINTER(i64)], i32),
+            "mx_attention_forward": ([C.POINTER(AttentionDesc)] + [vp] * 6 + [i64, vp], i32),
+            "mx_attention_backward": ([C.POINTER(AttentionDesc)] + [vp] * 10 + [i64, vp], i32),
+            "mx_attention_workspace": ([C.POINTER(AttentionDesc), i32, C.POINTER(i64)], i32),
+            "mx_kv_cache_write": ([C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, i64, i64, vp, i64, i64, vp], i32),
+            "mx_kv_cache_read": ([C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, vp, vp], i32),
+            "mx_attention_paged": ([C.POINTER(PagedDesc), C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, vp, vp, i64, vp],
+                                   i32),
+            "mx_attention_paged_workspace": ([C.POINTER(PagedDesc), C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc),
+                                              C.POINTER(i64)], i32),
             "mx_layer_norm_forward": ([vp, vp, vp, i64, i64, C.c_float, vp, vp, vp, vp], i32),
             "mx_layer_norm_backward": ([vp, vp, vp, vp, vp, i64, i64, vp, vp, vp, vp, i64, vp], i32),
             "mx_layer_norm_backward_workspace": ([i64, i64, C.POINTER(i64)], i32),
@@ -587,6 +630,220 @@ def muon_step(params, grads, momentum_buffers, *, lr=1e-3, weight_decay=0.1, mom
 
 def muon_workspace(params) -> int:
     return _workspace_query(lib().mx_muon_workspace, _muon_table(params, params, params), len(params))
+
+
+class Rotary:
+    """What a rotation of queries and keys keeps from call to call: the angle a
+    position of each pair, the pairs' layout, and the factor on cos and sin."""
+
+    def __init__(self, frequencies, interleaved=False, magnitude=1.0):
+        self.rotary_dim = 2 * len(frequencies)
+        self.frequencies = (C.c_double * max(1, len(frequencies)))(*frequencies)
+        self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
+
+
+def _packed(name, t, dim=None):
+    """Strides of a packed tensor [tokens, heads, head_dim] whose last axis is contiguous."""
+    if t.dim() != 3 or t.dtype != torch.float32 or (t.stride(2) != 1 and t.shape[2] > 1 and t.numel()):
+        raise ValueError(f"{name}: expected float32 [tokens, heads, head_dim] with a contiguous last axis, got "
+                         f"{t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+    return t.stride(0), t.stride(1)
+
+
+def _flat(name, t, shape, dtype=None):
+    if t is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.dtype != (dtype or torch.float32)):
+        raise ValueError(f"{name}: expected a contiguous {dtype or torch.float32} tensor {tuple(shape)}, got {t.dtype} "
+                         f"{tuple(t.shape)} of strides {t.stride()}")
+
+
+def _rotary_desc(q, k, positions, rotary, eps, like):
+    """like: (tokens, q heads, k heads, head_dim)."""
+    tokens, hq, hk, dim = like
+    if positions is None and rotary.rotary_dim:
+        raise ValueError("qk_norm_rotary: no positions")
+    _flat("positions", positions, (tokens,), torch.int64)
+    qs = _packed("q", q) if q is not None else (0, 0)
+    ks = _packed("k", k) if k is not None else (0, 0)
+    return RotaryDesc(tokens, hq, hk, dim, rotary.rotary_dim, *qs, *ks, ptr(positions),
+                      C.cast(rotary.frequencies, C.c_void_p), rotary.magnitude, 0.0 if eps is None else eps,
+                      int(rotary.interleaved), 0 if eps is None else 1)
+
+
+def _sides(q, k):
+    """(tokens, q heads, k heads, head_dim) of two packed tensors, either of which may be None."""
+    a = q if q is not None else k
+    if a is None:
+        raise ValueError("qk_norm_rotary: neither queries nor keys")
+    if k is not None and (k.shape[0] != a.shape[0] or k.shape[2] != a.shape[2]):
+        raise ValueError(f"qk_norm_rotary: queries {tuple(a.shape)} and keys {tuple(k.shape)} do not fit")
+    return a.shape[0], 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], a.shape[2]
+
+
+def qk_norm_rotary_forward(q, k, positions, rotary, q_out, k_out, q_weight=None, k_weight=None, eps=None,
+                           stream=None) -> None:
+    """Norm of each head (eps None: none) and rotation of packed queries and keys
+    [tokens, heads, head_dim]; q or k (with its output) may be None."""
+    like = _sides(q, k)
+    d = _rotary_desc(q, k, positions, rotary, eps, like)
+    for n, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if x is not None:
+            _flat(n, t, x.shape)
+    for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _flat(n, w, (like[3],))
+    check(lib().mx_qk_norm_rotary_forward(C.byref(d), ptr(q), ptr(k), ptr(q_weight), ptr(k_weight), ptr(q_out), ptr(k_out),
+                                          stream))
+
+
+def qk_norm_rotary_backward(dq_out, dk_out, q, k, positions, rotary, dq, dk, dq_weight=None, dk_weight=None, q_weight=None,
+                            k_weight=None, eps=None, workspace=None, stream=None) -> None:
+    """Gradients of qk_norm_rotary_forward; any of dq, dk, dq_weight, dk_weight
+    may be None, q and k too without a norm."""
+    like = _sides(dq_out, dk_out)
+    for n, t, x in (("q", q, dq_out), ("k", k, dk_out)):
+        if t is not None and (x is None or t.shape != x.shape):
+            raise ValueError(f"qk_norm_rotary_backward: {n} does not have the shape of its output's gradient")
+    for n, t, x in (("dq_out", dq_out, dq_out), ("dk_out", dk_out, dk_out), ("dq", dq, dq_out), ("dk", dk, dk_out)):
+        if t is not None:
+            if x is None:
+                raise ValueError(f"qk_norm_rotary_backward: {n} without its output's gradient")
+            _flat(n, t, x.shape)
+    for n, w in (("q_weight", q_weight), ("k_weight", k_weight), ("dq_weight", dq_weight), ("dk_weight", dk_weight)):
+        _flat(n, w, (like[3],))
+    d = _rotary_desc(q, k, positions, rotary, eps, like)
+    check(lib().mx_qk_norm_rotary_backward(C.byref(d), ptr(dq_out), ptr(dk_out), ptr(q), ptr(k), ptr(q_weight),
+                                           ptr(k_weight), ptr(dq), ptr(dk), ptr(dq_weight), ptr(dk_weight), ptr(workspace),
+                                           _bytes(workspace), stream))
+
+
+def qk_norm_rotary_workspace(tokens, q_heads, k_heads, head_dim, rotary, eps) -> int:
+    """Bytes that the backward's gradients of the weights take."""
+    d = RotaryDesc(tokens, q_heads, k_heads, head_dim, rotary.rotary_dim, 0, 0, 0, 0, None,
+                   C.cast(rotary.frequencies, C.c_void_p), rotary.magnitude, 0.0 if eps is None else eps,
+                   int(rotary.interleaved), 0 if eps is None else 1)
+    return _workspace_query(lib().mx_qk_norm_rotary_workspace, C.byref(d))
+
+
+def _attention_desc(q, k, v, starts, sequences, window, sinks, scale):
+    qs, ks, vs = _packed("q", q), _packed("k", k), _packed("v", v)
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    if starts is not None:
+        if starts.dim() != 1 or starts.numel() < 1:
+            raise ValueError("attention: starts must name every sequence's first row and the end of the last")
+        _flat("starts", starts, starts.shape, torch.int32)
+        sequences = starts.numel() - 1
+    return AttentionDesc(q.shape[0], sequences, ptr(starts), q.shape[1], k.shape[1], q.shape[2], *qs, *ks, *vs, window, sinks,
+                         q.shape[2] ** -0.5 if scale is None else scale)
+
+
+def attention_forward(q, k, v, out, starts=None, sequences=1, window=0, sinks=0, scale=None, lse=None, workspace=None,
+                      stream=None) -> None:
+    """Causal attention of packed sequences [tokens, heads, head_dim]; k and v may
+    have fewer heads.  starts: int32 [sequences + 1] on the device, or None for
+    ``sequences`` of equal length; window 0: every earlier token; sinks: first
+    tokens that stay visible; scale None: head_dim ** -0.5.  lse, if given
+    ([heads, tokens]), is what the backward needs."""
+    d = _attention_desc(q, k, v, starts, sequences, window, sinks, scale)
+    _flat("out", out, q.shape)
+    _flat("lse", lse, (q.shape[1], q.shape[0]))
+    check(lib().mx_attention_forward(C.byref(d), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(workspace),
+                                     _bytes(workspace), stream))
+
+
+def attention_backward(dout, q, k, v, out, lse, dq, dk, dv, starts=None, sequences=1, window=0, sinks=0, scale=None,
+                       workspace=None, stream=None) -> None:
+    """Gradients of attention_forward; any of dq, dk, dv may be None."""
+    d = _attention_desc(q, k, v, starts, sequences, window, sinks, scale)
+    for n, t, x in (("dout", dout, q), ("out", out, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        _flat(n, t, x.shape)
+    _flat("lse", lse, (q.shape[1], q.shape[0]))
+    check(lib().mx_attention_backward(C.byref(d), ptr(dout), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(dq), ptr(dk),
+                                      ptr(dv), ptr(workspace), _bytes(workspace), stream))
+
+
+def attention_workspace(tokens, sequences, heads, kv_heads, head_dim, backward=False) -> int:
+    d = AttentionDesc(tokens, sequences, _ANY_ADDRESS, heads, kv_heads, head_dim, 0, 0, 0, 0, 0, 0, 0, 0, 1.0)
+    return _workspace_query(lib().mx_attention_workspace, C.byref(d), 1 if backward else 0)
+
+
+# Any address: workspace queries do not read the sequences' starts.
+_ANY_ADDRESS = 16
+
+KV_F32, KV_I8 = 0, 1
+
+
+class KVCache:
+    """A paged cache: k [pages, heads, page_size, head_dim] and v [pages, heads,
+    head_dim, page_size], float32, or int8 with k_scale and v_scale
+    [pages, heads, page_size]."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        if k.dim() != 4 or k.dtype not in (torch.float32, torch.int8):
+            raise ValueError(f"KVCache: expected float32 or int8 [pages, heads, page_size, head_dim], got {k.dtype} "
+                             f"{tuple(k.shape)}")
+        pages, heads, page, dim = k.shape
+        _flat("KVCache: k", k, k.shape, k.dtype)
+        _flat("KVCache: v", v, (pages, heads, dim, page), k.dtype)
+        i8 = k.dtype == torch.int8
+        if i8 != (k_scale is not None) or i8 != (v_scale is not None):
+            raise ValueError("KVCache: scales go with an int8 cache, and with no other")
+        _flat("KVCache: k_scale", k_scale, (pages, heads, page))
+        _flat("KVCache: v_scale", v_scale, (pages, heads, page))
+        self.tensors = (k, v, k_scale, v_scale)
+        self.heads, self.head_dim = heads, dim
+        self.desc = KVCacheDesc(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page, dim, KV_I8 if i8 else KV_F32)
+
+
+class KVBatch:
+    """Where the new tokens of several sequences lie in a cache: table [sequences,
+    pages of the longest] and lengths [sequences] (new tokens included), int32 on
+    the device; starts as in attention_forward, None for tokens / sequences each."""
+
+    def __init__(self, table, lengths, tokens, starts=None):
+        if table.dim() != 2:
+            raise ValueError(f"KVBatch: expected a table [sequences, pages], got {tuple(table.shape)}")
+        _flat("KVBatch: table", table, table.shape, torch.int32)
+        _flat("KVBatch: lengths", lengths, (table.shape[0],), torch.int32)
+        _flat("KVBatch: starts", starts, (table.shape[0] + 1,), torch.int32)
+        self.tensors, self.tokens = (table, lengths, starts), tokens
+        self.desc = KVBatchDesc(tokens, table.shape[0], table.shape[1], ptr(starts), ptr(lengths), ptr(table))
+
+
+def kv_cache_write(cache, batch, k, v, stream=None) -> None:
+    """Writes the batch's new tokens [tokens, heads, head_dim] to the cache."""
+    ks, vs = _packed("k", k), _packed("v", v)
+    for n, t in (("k", k), ("v", v)):
+        if tuple(t.shape) != (batch.tokens, cache.heads, cache.head_dim):
+            raise ValueError(f"kv_cache_write: {n} {tuple(t.shape)} does not fit the batch and the cache")
+    check(lib().mx_kv_cache_write(C.byref(cache.desc), C.byref(batch.desc), ptr(k), *ks, ptr(v), *vs, stream))
+
+
+def kv_cache_read(cache, batch, k, v, stream=None) -> None:
+    """Reads them back into contiguous k and v."""
+    for n, t in (("k", k), ("v", v)):
+        _flat(n, t, (batch.tokens, cache.heads, cache.head_dim))
+    check(lib().mx_kv_cache_read(C.byref(cache.desc), C.byref(batch.desc), ptr(k), ptr(v), stream))
+
+
+def _paged_desc(cache, batch, heads, strides, window, sinks, scale):
+    return PagedDesc(heads, *strides, window, sinks, cache.head_dim ** -0.5 if scale is None else scale)
+
+
+def attention_paged(cache, batch, q, out, window=0, sinks=0, scale=None, workspace=None, stream=None) -> None:
+    """Attention of the batch's new tokens [tokens, heads, head_dim], which the
+    cache holds already, over the cache."""
+    strides = _packed("q", q)
+    if q.shape[0] != batch.tokens or q.shape[2] != cache.head_dim:
+        raise ValueError(f"attention_paged: q {tuple(q.shape)} does not fit the batch and the cache")
+    _flat("out", out, q.shape)
+    d = _paged_desc(cache, batch, q.shape[1], strides, window, sinks, scale)
+    check(lib().mx_attention_paged(C.byref(d), C.byref(cache.desc), C.byref(batch.desc), ptr(q), ptr(out), ptr(workspace),
+                                   _bytes(workspace), stream))
+
+
+def attention_paged_workspace(cache, batch, heads, window=0, sinks=0) -> int:
+    d = _paged_desc(cache, batch, heads, (0, 0), window, sinks, 1.0)
+    return _workspace_query(lib().mx_attention_paged_workspace, C.byref(d), C.byref(cache.desc), C.byref(batch.desc))
 
 
 def conv2d_kernel_name(d: ConvDesc, phase: int, algo: int = ALGO_AUTO) -> str:
