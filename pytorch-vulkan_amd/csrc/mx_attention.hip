@@ -7,25 +7,26 @@
 // Bound by the matrix instructions: 4 head_dim operations a visible pair forward and 14
 // backward, each FP32 product six bf16 products of pieces.
 //
-// Every call first packs its operands (pack_kernel): a tile of 32 rows of one head is
-// split into pieces once and stored in the order in which a wave's lanes feed the
-// matrix instruction, 1 KiB a fragment and piece, so that the products read whole
-// fragments from consecutive addresses whatever the strides, the head's size (padded
-// with zeros to 32, 64, 96 or 128) or a sequence's first row.  Two orders are needed:
-//   R  what runs along the head's elements (q k, dout v): lane l holds row
-//      tile_row(l % 32), elements 16 s + 8 (l / 32) + 0 .. 7 of step s
-//   T  what runs along the tile's rows (p v, ds k, p dout, ds q): lane l holds element
-//      32 b + tile_row(l % 32) of block b, rows 16 (l / 32) + 8 t + 0 .. 7 of step t
-// Forward: each wave has 32 queries and walks over the keys that any of them sees with a
-// running maximum and sum.  Backward: one kernel in that form for dq, and one in which
-// each wave has 32 keys and walks over the queries (of all heads that share the key
-// head) for dk and dv, so nothing is added up in an order that changes.
+// Every call first packs what is read many times (pack_kernel): a tile of 32 rows of one
+// head is split into pieces once and stored in the order in which a wave's lanes feed the
+// matrix instruction, 1 KiB a fragment and piece, whatever the strides, the head's size
+// (padded with zeros to 32, 64, 96 or 128) or a sequence's first row: lane l holds row
+// tile_row(l % 32), elements 16 s + 8 (l / 32) + 0 .. 7 of step s.  So tiles go from memory
+// to LDS in whole lines without passing through registers, for all four waves of a
+// workgroup, one tile ahead of the products; what runs along the head's elements (q k,
+// dout v) takes fragments as they lie, and what runs along the tile's rows (p v, ds k, p
+// dout, ds q) through transposing reads.
+// Forward: each wave has 32 queries and walks over the keys that any of its workgroup's
+// sees, with a running maximum and sum.  Backward: one kernel in that form for dq, and
+// one in which each wave has 32 keys and walks over the queries (of all heads that share
+// the key head) for dk and dv, so nothing is added up in an order that changes.
 //
 // A NaN or an infinity among a tile's rows would reach every row of a product along
-// those rows, times a probability of 0.  T fragments hold zeros in their place, and the
-// row's scores are NaN instead (R fragments, or lse in the backward), which the mask
-// keeps from rows that do not see it.
+// those rows, times a probability of 0.  Such rows are packed as zeros, and what sees
+// them is made NaN through the scores, which the mask keeps apart: by a NaN in the key's
+// other operand in the forward, by lse (the forward's, or its own) in the backward.
 #include "mx_attention.hpp"
+#include "mx_pieces.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -35,6 +36,8 @@ namespace mx {
 namespace {
 
 using namespace attn;
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256, kMaxDim = 128;
 
@@ -50,17 +53,31 @@ struct Strided {
   int64_t token, head;
 };
 
-// Fragments of a tensor: [head][tile][step or block][piece][lane], DP / 16 steps a tile;
-// lanes' parts of a tile, and where a head's tile starts.
+// A packed tensor: [head][tile][step][piece][lane], DP / 16 steps; bytes of a tile, and where a
+// head's tile starts.
 template <int DP>
-constexpr int kTileParts = DP / 16 * 3 * 64;
+constexpr int kTileBytes = DP / 16 * 3 * 1024;
 template <int DP>
 __device__ __forceinline__ int64_t tile_at(const Shape& s, int head, int tile) {
-  return (int64_t(head) * s.tiles + tile) * kTileParts<DP>;
+  return (int64_t(head) * s.tiles + tile) * kTileBytes<DP>;
 }
-__device__ __forceinline__ Frag3 frag(const bf16x8* tile, int step, int lane) {
-  const bf16x8* const f = tile + step * 3 * 64 + lane;
-  return {f[0], f[64], f[128]};
+// Lane l's place in a fragment: the halves' lines are exchanged in fours, so that a
+// transposing read's 16 lanes, 8 bytes of four rows from both halves, meet every bank once.
+__device__ __forceinline__ int slot(int lane) { return lane ^ (lane >> 5 << 2); }
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Elements e .. e + 7 of a row, zero from `dim` on.
+__device__ __forceinline__ void load8(const float* row, int e, int dim, f32x4 (&v)[2]) {
+  v[0] = v[1] = f32x4{};
+  if (e + 8 <= dim) {
+    v[0] = *reinterpret_cast<const f32x4u*>(row + e);
+    v[1] = *reinterpret_cast<const f32x4u*>(row + e + 4);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e + i < dim) v[i >> 2][i & 3] = row[e + i];
+  }
 }
 
 // ------------------------------------------------------------------ packing
@@ -68,137 +85,160 @@ struct PackArgs {
   Shape s;
   Strided q, k, v, dout, out;
   const float* lse;
-  bf16x8 *qr, *qt, *kr, *kt, *vr, *vt, *dr, *dt;  // null: not needed
-  float *stats;                                     // [head][tile][2][32]: lse log2(e), delta
+  char *qp, *kp, *vp, *dp;  // kp, vp: by key head; qp, dp: by head, null in the forward
+  float* stats;             // [head][tile][2][32]: lse log2(e), delta
 };
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
-
-// A tile's rows into LDS (zeros past the sequence's end and the head's), and per row whether
-// all of it is finite.
-template <int DP>
-struct Stage {
-  static constexpr int kPitch = DP + 4;
-  float x[kTile][kPitch];
-  __device__ __forceinline__ bool load(const Strided& t, int head, int row0, int rows, int dim) {
-    constexpr int C = DP / 8;  // a row's elements of each of the 8 threads that share it
-    const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
-    const float* const src = t.at + (int64_t(row0) + r) * t.token + head * t.head;
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < C; i += 4) {
-      const int e = i * 8 + c * 4;
-      f32x4 v{};
-      if (r < rows) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (e + j < dim) v[j] = src[e + j];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ok = ok && finite(v[j]);
-      *reinterpret_cast<f32x4*>(&x[r][e]) = v;
-    }
-    return ok;
-  }
-  // Fragments of the staged tile; rows whose bit is set in `bad` are NaN in R and 0 in T.
-  __device__ __forceinline__ void rows_out(bf16x8* to, uint32_t bad) const {
-    const int lane = threadIdx.x & 63, row = tile_row(lane & 31), h = lane >> 5;
-    for (int s = threadIdx.x >> 6; s < DP / 16; s += 4) {
-      const float* const at = &x[row][s * 16 + h * 8];
-      f32x4 a = *reinterpret_cast<const f32x4*>(at), b = *reinterpret_cast<const f32x4*>(at + 4);
-      if (bad >> row & 1) a = f32x4{1, 1, 1, 1} * __builtin_nanf(""), b = a;
-      put(to, s, lane, split8(a, b));
-    }
-  }
-  __device__ __forceinline__ void cols_out(bf16x8* to, uint32_t bad) const {
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    for (int s = threadIdx.x >> 6; s < DP / 16; s += 4) {
-      const int e = (s >> 1) * 32 + tile_row(lane & 31), r0 = h * 16 + (s & 1) * 8;
-      f32x4 v[2];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j >> 2][j & 3] = bad >> (r0 + j) & 1 ? 0.f : x[r0 + j][e];
-      put(to, s, lane, split8(v[0], v[1]));
-    }
-  }
-  static __device__ __forceinline__ void put(bf16x8* to, int s, int lane, const Frag3& f) {
-    bf16x8* const at = to + s * 3 * 64 + lane;
-    at[0] = f.hi, at[64] = f.mid, at[128] = f.lo;
-  }
-};
-
-// One bit a row: whether any of the row's 8 threads has `flag`.
-__device__ __forceinline__ uint32_t row_bits(bool flag, uint32_t* lds) {
+// One bit a row, from its two lanes (l and l + 32) in a wave that has all rows.
+__device__ __forceinline__ uint32_t row_bits(bool flag) {
   const uint64_t b = __ballot(flag);
-  uint32_t bits = 0;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) bits |= uint32_t((b >> (8 * r) & 0xFF) != 0) << r;
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = bits;
-  __syncthreads();
-  const uint32_t all = lds[0] | lds[1] << 8 | lds[2] << 16 | lds[3] << 24;
-  return all;
+  return uint32_t(b) | uint32_t(b >> 32);
 }
 
-// grid (tiles, heads + kv_heads): a query head's q (and dout, delta, lse), or a key head's k and v.
+// A tile of one head, straight from memory to fragments: a wave takes every fourth step, so
+// the rows that are not finite are known to the workgroup before anything is stored.
+template <int DP>
+struct Pack {
+  static constexpr int N = (DP / 16 + 3) / 4;
+  f32x4 x[N][2];
+  bool bad = false;
+  // rows: of the tile; r and h: the lane's row and half
+  __device__ __forceinline__ void load(const Strided& t, int head, int row0, int rows, int dim, int wave, int r, int h) {
+    const float* const row = t.at + (int64_t(row0) + r) * t.token + head * t.head;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int s = wave + 4 * i;
+      x[i][0] = x[i][1] = f32x4{};
+      if (s < DP / 16 && r < rows) load8(row, s * 16 + h * 8, dim, x[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bad = bad || !finite(x[i][j >> 2][j & 3]);
+    }
+  }
+  __device__ __forceinline__ void store(char* to, int wave, int lane, bool replace, float with, float scale) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int s = wave + 4 * i;
+      if (s >= DP / 16) break;
+      f32x4 v[2] = {x[i][0] * scale, x[i][1] * scale};
+      if (replace) v[0] = v[1] = f32x4{with, with, with, with};
+      const Frag3 f = split8(v[0], v[1]);
+      bf16x8* const at = reinterpret_cast<bf16x8*>(to) + s * 3 * 64 + slot(lane);
+      at[0] = f.hi, at[64] = f.mid, at[128] = f.lo;
+    }
+  }
+};
+
+// grid (tiles, heads + kv_heads, or kv_heads alone): a key head's k and v, or a query head's q, dout,
+// lse and delta.
 template <int DP>
 __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
-  __shared__ Stage<DP> st[2];
   __shared__ uint32_t bits[2][4];
+  __shared__ float sums[4][kTile];
   const Shape& s = a.s;
   SequenceTile t;
   if (!locate<kTile>(s.seqs, blockIdx.x, t) || t.index * kTile >= t.len) return;
   const int row0 = t.start + t.index * kTile, rows = min(kTile, t.len - t.index * kTile);
-  const bool key = int(blockIdx.y) >= s.heads;
-  const int head = key ? blockIdx.y - s.heads : blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+  const int r = tile_row(lane & 31);
+  const bool key = int(blockIdx.y) < s.kv_heads;
+  const int head = key ? blockIdx.y : blockIdx.y - s.kv_heads;
   const int64_t o = tile_at<DP>(s, head, blockIdx.x);
+  Pack<DP> x, y;
+  x.load(key ? a.k : a.q, head, row0, rows, s.dim, wave, r, h);
+  y.load(key ? a.v : a.dout, head, row0, rows, s.dim, wave, r, h);
+  const uint32_t bx = row_bits(x.bad), by = row_bits(y.bad);
+  if (lane == 0) bits[0][wave] = bx, bits[1][wave] = by;
+  if (!key) {
+    // A row's part of delta in this wave's steps.
+    float delta = 0;
+    const float* const out = a.out.at + (int64_t(row0) + r) * a.out.token + head * a.out.head;
+#pragma unroll
+    for (int i = 0; i < Pack<DP>::N; ++i) {
+      f32x4 v[2] = {};
+      if (wave + 4 * i < DP / 16 && r < rows) load8(out, (wave + 4 * i) * 16 + h * 8, s.dim, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(y.x[i][j >> 2][j & 3], v[j >> 2][j & 3], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (h == 0) sums[wave][r] = delta;
+  }
+  __syncthreads();
+  const uint32_t bad_x = bits[0][0] | bits[0][1] | bits[0][2] | bits[0][3];
+  const uint32_t bad_y = bits[1][0] | bits[1][1] | bits[1][2] | bits[1][3];
+  const bool bad = (bad_x | bad_y) >> (lane & 31) & 1;
   if (key) {
-    const bool k_ok = st[0].load(a.k, head, row0, rows, s.dim), v_ok = st[1].load(a.v, head, row0, rows, s.dim);
-    const uint32_t bad = row_bits(!(k_ok && v_ok), bits[0]);
-    if (a.kr) st[0].rows_out(a.kr + o, bad);
-    if (a.vr) st[1].rows_out(a.vr + o, bad);
-    if (a.kt) st[0].cols_out(a.kt + o, bad);
-    if (a.vt) st[1].cols_out(a.vt + o, bad);
+    x.store(a.kp + o, wave, lane, bad, a.stats ? 0.f : __builtin_nanf(""), 1.f);
+    y.store(a.vp + o, wave, lane, bad, 0.f, 1.f);
     return;
   }
-  const uint32_t bad_q = row_bits(!st[0].load(a.q, head, row0, rows, s.dim), bits[0]);
-  if (a.qr) st[0].rows_out(a.qr + o, bad_q);
-  if (a.qt) st[0].cols_out(a.qt + o, bad_q);
-  if (!a.stats) return;
-  const uint32_t bad_o = row_bits(!st[1].load(a.dout, head, row0, rows, s.dim), bits[1]);
-  if (a.dr) st[1].rows_out(a.dr + o, bad_o);
-  if (a.dt) st[1].cols_out(a.dt + o, bad_o);
-  // delta, and lse in the exponent's base.  Past the end lse is infinite: no probability.
-  const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
-  float delta = 0;
-  if (r < rows) {
-    const float* const out = a.out.at + (int64_t(row0) + r) * a.out.token + head * a.out.head;
-    for (int e = c; e < s.dim; e += 8) delta = fmaf(st[1].x[r][e], out[e], delta);
-  }
-#pragma unroll
-  for (int m = 1; m < 8; m <<= 1) delta += __shfl_xor(delta, m, 64);
-  if (c == 0) {
+  x.store(a.qp + o, wave, lane, bad, 0.f, s.scale * kLog2E);
+  y.store(a.dp + o, wave, lane, bad, 0.f, 1.f);
+  // Past the sequence's end lse is infinite: no probability.
+  if (wave == 0 && h == 0) {
     float* const to = a.stats + (int64_t(head) * s.tiles + blockIdx.x) * 64 + r;
     float l = __builtin_inff();
-    if (r < rows) l = (bad_q | bad_o) >> r & 1 ? __builtin_nanf("") : a.lse[int64_t(head) * s.seqs.tokens + row0 + r] * kLog2E;
-    to[0] = l, to[32] = delta;
+    if (r < rows) l = bad ? __builtin_nanf("") : a.lse[int64_t(head) * s.seqs.tokens + row0 + r] * kLog2E;
+    to[0] = l, to[32] = r < rows ? sums[0][r] + sums[1][r] + sums[2][r] + sums[3][r] : 0.f;
   }
 }
 
-// ------------------------------------------------------------------ forward
-struct FwdArgs {
-  Shape s;
-  const bf16x8 *qr, *kr, *vt;
-  float *out, *lse;
-};
-
-template <int DP>
-__device__ __forceinline__ void load_frags(Frag3 (&f)[DP / 16], const bf16x8* tile, int lane) {
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) f[s] = frag(tile, s, lane);
+// ------------------------------------------------- tiles in LDS, and products
+__device__ __forceinline__ uint32_t lds_address(char* p) {
+  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)p));
 }
 
-// a b along the head's elements: a's fragments from memory, b's in registers.
+// Two tensors' tiles (and 256 bytes of statistics) in LDS, two stages.
+template <int DP, bool STATS = false>
+struct Stages {
+  static constexpr int kBytes = 2 * kTileBytes<DP> + (STATS ? 1024 : 0);
+  static constexpr int kSecond = kTileBytes<DP>, kStats = 2 * kTileBytes<DP>;
+  uint32_t lds;
+  __device__ __forceinline__ void load(int stage, const char* a, const char* b, const char* stats, int wave, int lane) const {
+    const uint32_t to = lds + stage * kBytes;
+    const char *const pa = pieces::uniform(a), *const pb = pieces::uniform(b);
+    constexpr int F = DP / 16 * 3;
+#pragma unroll
+    for (int i = 0; i < F / 2; ++i) {
+      const int f = wave + 4 * i;  // a's fragments, then b's
+      pieces::load_lds16(f < F ? pa + f * 1024 : pb + (f - F) * 1024, lane * 16, to + f * 1024);
+    }
+    if constexpr (STATS)
+      if (wave == 0) load_lds4(pieces::uniform(stats), lane * 4, to + kStats);
+  }
+  // 4 bytes a lane from memory to LDS (as pieces::load_lds16).
+  static __device__ __forceinline__ void load_lds4(const char* base, uint32_t lane_off, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(at), "v"(lane_off), "s"(base) : "memory");
+  }
+};
+
+__device__ __forceinline__ Frag3 frag(uint32_t tile, int step, int lane) {
+  const uint32_t at = tile + step * 3072 + slot(lane) * 16;
+  return {*pieces::lds_at<const bf16x8>(at), *pieces::lds_at<const bf16x8>(at + 1024), *pieces::lds_at<const bf16x8>(at + 2048)};
+}
+
+// Rows 16 h + 8 t + 0 .. 7 (h: the lane's half) of element 32 b + l % 32, by transposing reads: 16
+// lanes name 4 elements of one of 4 rows each, and get 4 rows of one element.
+__device__ __forceinline__ uint32_t column_base(int lane) {
+  const int c = lane & 15, g = lane >> 4 & 1, h = lane >> 5, other = c >> 1 & 1;
+  return uint32_t(g * 3072 + other * 512 + (((h ^ other) << 2) + (c >> 2)) * 16 + (c & 1) * 8);
+}
+__device__ __forceinline__ Frag3 frag_columns(uint32_t tile_and_base, int b, int t) {
+  bf16x8 f[3];
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    mfma::s16x4 q[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      q[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          pieces::lds_at<mfma::s16x4>(tile_and_base + b * 6144 + p * 1024 + (2 * t + i) * 128));
+    f[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  return {f[0], f[1], f[2]};
+}
+
+// a b along the head's elements: a's tile in LDS, b's fragments in registers.
 template <int DP>
-__device__ __forceinline__ f32x16 product(const bf16x8* a, const Frag3 (&b)[DP / 16], int lane) {
+__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane) {
   f32x16 small{}, large{};
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
@@ -209,45 +249,93 @@ __device__ __forceinline__ f32x16 product(const bf16x8* a, const Frag3 (&b)[DP /
   return large + small;
 }
 
-// Block b of a p along the tile's rows: a's T fragments, p's pieces.
-__device__ __forceinline__ f32x16 product_rows(const bf16x8* a, int b, const Frag3 (&p)[2], int lane) {
+// Block b of a p along the tile's rows: a's tile in LDS (and the lane's column_base), p's pieces.
+__device__ __forceinline__ f32x16 product_rows(uint32_t a, int b, const Frag3 (&p)[2]) {
   f32x16 acc{};
-  const Frag3 f0 = frag(a, 2 * b, lane), f1 = frag(a, 2 * b + 1, lane);
+  const Frag3 f0 = frag_columns(a, b, 0), f1 = frag_columns(a, b, 1);
   acc = mma_small(f0, p[0], acc);
   acc = mma_small(f1, p[1], acc);
   acc = mma_large(f0, p[0], acc);
   return mma_large(f1, p[1], acc);
 }
 
-// Stores a lane's 16 elements of block b of one row.
-__device__ __forceinline__ void store_block(float* row, const f32x16& v, int b, int h, int dim) {
-  const int e0 = b * 32 + h * 16;
+// Own rows as fragments in registers, straight from memory.
+template <int DP>
+__device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const Strided& t, int head, int64_t row, bool live, int dim, int h,
+                                         float scale) {
+  const float* const at = t.at + row * t.token + head * t.head;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (e0 + i < dim) row[e0 + i] = v[i];
+  for (int s = 0; s < DP / 16; ++s) {
+    f32x4 v[2] = {};
+    if (live) load8(at, s * 16 + h * 8, dim, v);
+    f[s] = split8(v[0] * scale, v[1] * scale);
+  }
 }
+// The same from a packed tile.
+template <int DP>
+__device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const char* tile, int lane) {
+  const bf16x8* const at = reinterpret_cast<const bf16x8*>(tile) + slot(lane);
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) f[s] = {at[s * 192], at[s * 192 + 64], at[s * 192 + 128]};
+}
+
+// Stores a lane's 16 elements of block b of one row: 8 k + 4 h + 0 .. 3.
+__device__ __forceinline__ void store_block(float* row, const f32x16& v, int b, int h, int dim) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int e = b * 32 + 8 * k + 4 * h;
+    const f32x4 four{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+    if (e + 4 <= dim) *reinterpret_cast<f32x4u*>(row + e) = four;
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (e + i < dim) row[e + i] = four[i];
+  }
+}
+
+// Blocks of 128 rows, four tiles of one sequence; the workgroups' order puts what has the most
+// to do first and keeps a head's on as few XCDs as there are heads for.
+constexpr int kBlock = 4 * kTile;
+
+// ------------------------------------------------------------------ forward
+struct FwdArgs {
+  Shape s;
+  Strided q;
+  const char *kp, *vp;
+  float *out, *lse;
+};
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
+  using St = Stages<DP>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int tile = blockIdx.x * 4 + wave, head = blockIdx.y;
+  const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
   SequenceTile t;
-  if (!locate<kTile>(s.seqs, tile, t) || t.index * kTile >= t.len) return;
-  const int64_t keys0 = tile_at<DP>(s, head / s.group, t.base);
+  if (!locate<kBlock>(s.seqs, block, t) || t.index * kBlock >= t.len) return;
+  const int64_t keys0 = tile_at<DP>(s, head / s.group, t.start / kTile + t.seq);
+  const int b0 = t.index * kBlock, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
+  const St st{lds_address(smem)};
+  const KeyTiles keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
+  const auto fetch = [&](int n) {
+    const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
+    st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
+  };
+  fetch(0);
   Frag3 q[DP / 16];
-  load_frags<DP>(q, a.qr + tile_at<DP>(s, head, tile), lane);
-  const int i0 = t.index * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
-  const float c = s.scale * kLog2E;
+  own_rows<DP>(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
   f32x16 o[DP / 32] = {};
   float m = -__builtin_inff(), l = 0;  // of the exponents
-  const KeyTiles keys(s.mask, i0, i1);
+  const uint32_t columns = column_base(lane);
   for (int n = 0; n < keys.count; ++n) {
-    const int j = keys.tile(n), j0 = j * kTile;
-    const int64_t at = keys0 + int64_t(j) * kTileParts<DP>;
-    f32x16 x = product<DP>(a.kr + at, q, lane);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] *= c;
+    pieces::wait_loads<0>();
+    pieces::barrier();
+    if (n + 1 < keys.count) fetch(n + 1);
+    const int j0 = keys.tile(n) * kTile;
+    if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
+    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    f32x16 x = product<DP>(tile, q, lane);
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -269,12 +357,12 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
     m = next;
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) o[b] = o[b] * keep + product_rows(a.vt + at, b, p, lane);
+    for (int b = 0; b < DP / 32; ++b) o[b] = o[b] * keep + product_rows(tile + St::kSecond + columns, b, p);
   }
   l += __shfl_xor(l, 32, 64);
   if (qi >= t.len) return;
   const float r = 1.f / l;
-  const int64_t row = t.start + qi;
+  const int64_t row = int64_t(t.start) + qi;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) store_block(a.out + (row * s.heads + head) * s.dim, o[b] * r, b, h, s.dim);
   if (a.lse && h == 0) a.lse[int64_t(head) * s.seqs.tokens + row] = (m + log2f(l)) * kLn2;
@@ -283,35 +371,52 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
 // ----------------------------------------------------------------- backward
 struct BwdArgs {
   Shape s;
-  const bf16x8 *qr, *qt, *kr, *kt, *vr, *dr, *dt;
+  const char *qp, *kp, *vp, *dp;
   const float* stats;
   float *dq, *dk, *dv;
+  int parts;            // of a key head's query heads
+  float *dk_p, *dv_p;  // [part][token][key head][dim] where there are several
 };
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
+  using St = Stages<DP>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int tile = blockIdx.x * 4 + wave, head = blockIdx.y;
+  const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
   SequenceTile t;
-  if (!locate<kTile>(s.seqs, tile, t) || t.index * kTile >= t.len) return;
-  const int64_t mine = tile_at<DP>(s, head, tile), keys0 = tile_at<DP>(s, head / s.group, t.base);
+  if (!locate<kBlock>(s.seqs, block, t) || t.index * kBlock >= t.len) return;
+  const int base32 = t.start / kTile + t.seq;
+  const int64_t keys0 = tile_at<DP>(s, head / s.group, base32);
+  const int b0 = t.index * kBlock, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
+  const St st{lds_address(smem)};
+  const KeyTiles keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
+  const auto fetch = [&](int n) {
+    const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
+    st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
+  };
+  fetch(0);
+  // A wave past the sequence's end repeats its last tile, and stores nothing.
+  const int mine = base32 + min(i0, t.len - 1) / kTile;
   Frag3 q[DP / 16], g[DP / 16];
-  load_frags<DP>(q, a.qr + mine, lane);
-  load_frags<DP>(g, a.dr + mine, lane);
-  const int row = tile_row(lane & 31);
-  const float* const st = a.stats + (int64_t(head) * s.tiles + tile) * 64 + row;
-  const float lse = st[0], delta = st[32], c = s.scale * kLog2E;
-  const int i0 = t.index * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + row;
+  own_rows<DP>(q, a.qp + tile_at<DP>(s, head, mine), lane);
+  own_rows<DP>(g, a.dp + tile_at<DP>(s, head, mine), lane);
+  const float* const stat = a.stats + (int64_t(head) * s.tiles + mine) * 64 + row;
+  const float lse = stat[0], delta = stat[32];
   f32x16 dq[DP / 32] = {};
-  const KeyTiles keys(s.mask, i0, i1);
+  const uint32_t columns = column_base(lane);
   for (int n = 0; n < keys.count; ++n) {
-    const int j = keys.tile(n), j0 = j * kTile;
-    const int64_t o = keys0 + int64_t(j) * kTileParts<DP>;
-    f32x16 x = product<DP>(a.kr + o, q, lane);
-    const f32x16 dp = product<DP>(a.vr + o, g, lane);
+    pieces::wait_loads<0>();
+    pieces::barrier();
+    if (n + 1 < keys.count) fetch(n + 1);
+    const int j0 = keys.tile(n) * kTile;
+    if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
+    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    f32x16 x = product<DP>(tile, q, lane);
+    const f32x16 dp = product<DP>(tile + St::kSecond, g, lane);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = exp2_(fmaf(x[r], c, -lse)) * (dp[r] - delta);
+    for (int r = 0; r < 16; ++r) x[r] = exp2_(x[r] - lse) * (dp[r] - delta);
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
@@ -319,61 +424,104 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     }
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dq[b] += product_rows(a.kt + o, b, p, lane);
+    for (int b = 0; b < DP / 32; ++b) dq[b] += product_rows(tile + columns, b, p);
   }
   if (qi >= t.len) return;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
-    store_block(a.dq + ((t.start + qi) * int64_t(s.heads) + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
+    store_block(a.dq + ((int64_t(t.start) + qi) * s.heads + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
 }
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
+  using St = Stages<DP, true>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int tile = blockIdx.x * 4 + wave, kv_head = blockIdx.y;
+  const int across = s.kv_heads * a.parts, kv_head = blockIdx.x % across / a.parts, part = blockIdx.x % across % a.parts;
   SequenceTile t;
-  if (!locate<kTile>(s.seqs, tile, t) || t.index * kTile >= t.len) return;
-  const int64_t mine = tile_at<DP>(s, kv_head, tile);
+  if (!locate<kBlock>(s.seqs, blockIdx.x / across, t) || t.index * kBlock >= t.len) return;
+  const int base32 = t.start / kTile + t.seq;
+  const int b0 = t.index * kBlock, j0 = b0 + wave * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
+  const St st{lds_address(smem)};
+  // The tiles of queries that see any of the workgroup's keys, of each head in turn.
+  const int last = s.mask.window && b0 >= s.mask.sinks ? min(t.len - 1, b0 + kBlock - 1 + min(s.mask.window, t.len) - 1) : t.len - 1;
+  const int from = b0 / kTile, tiles = last / kTile + 1 - from;
+  const int heads = s.group / a.parts, head0 = kv_head * s.group + part * heads, count = heads * tiles;
+  const auto fetch = [&](int n) {
+    const int head = head0 + n / tiles, tile = base32 + from + n % tiles;
+    const int64_t at = tile_at<DP>(s, head, tile);
+    st.load(n & 1, a.qp + at, a.dp + at, reinterpret_cast<const char*>(a.stats + (int64_t(head) * s.tiles + tile) * 64), wave, lane);
+  };
+  fetch(0);
+  const int64_t mine = tile_at<DP>(s, kv_head, base32 + min(j0, t.len - 1) / kTile);
   Frag3 k[DP / 16], v[DP / 16];
-  load_frags<DP>(k, a.kr + mine, lane);
-  load_frags<DP>(v, a.vr + mine, lane);
-  const int j0 = t.index * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
-  const float c = s.scale * kLog2E;
-  // The last query that sees any of these keys.
-  const int last = s.mask.window && j0 >= s.mask.sinks ? min(t.len - 1, j1 + min(s.mask.window, t.len) - 1) : t.len - 1;
+  own_rows<DP>(k, a.kp + mine, lane);
+  own_rows<DP>(v, a.vp + mine, lane);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  for (int head = kv_head * s.group; head < (kv_head + 1) * s.group; ++head) {
-    for (int i = t.index; i <= last / kTile; ++i) {
-      const int64_t o = tile_at<DP>(s, head, t.base + i);
-      const float* const st = a.stats + (int64_t(head) * s.tiles + t.base + i) * 64 + 16 * h;
-      f32x16 x = product<DP>(a.qr + o, k, lane);
-      f32x16 dp = product<DP>(a.dr + o, v, lane);
+  const uint32_t columns = column_base(lane);
+  for (int n = 0; n < count; ++n) {
+    pieces::wait_loads<0>();
+    pieces::barrier();
+    if (n + 1 < count) fetch(n + 1);
+    const int i0 = (from + n % tiles) * kTile;
+    if (s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
+    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    f32x16 x = product<DP>(tile, k, lane);
+    f32x16 dp = product<DP>(tile + St::kSecond, v, lane);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        x[r] = exp2_(fmaf(x[r], c, -st[r]));
-        dp[r] = x[r] * (dp[r] - st[32 + r]);
-      }
-      const int i0 = i * kTile;
-      if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) {
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = tile + St::kStats + (16 * h + 4 * i) * 4;
+      const f32x4 lse = *pieces::lds_at<const f32x4>(at), delta = *pieces::lds_at<const f32x4>(at + 128);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!s.mask.sees(i0 + 16 * h + r, kj)) x[r] = 0, dp[r] = 0;
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * i + e;
+        x[r] = exp2_(x[r] - lse[e]);
+        dp[r] = x[r] * (dp[r] - delta[e]);
       }
-      const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)}, ds[2] = {split_half(dp, 0), split_half(dp, 1)};
+    }
+    if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) {
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) {
-        dv[b] += product_rows(a.dt + o, b, p, lane);
-        dk[b] += product_rows(a.qt + o, b, ds, lane);
-      }
+      for (int r = 0; r < 16; ++r)
+        if (!s.mask.sees(i0 + 16 * h + r, kj)) x[r] = 0, dp[r] = 0;
+    }
+    const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)}, ds[2] = {split_half(dp, 0), split_half(dp, 1)};
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+      dv[b] += product_rows(tile + St::kSecond + columns, b, p);
+      dk[b] += product_rows(tile + columns, b, ds);
     }
   }
   if (kj >= t.len) return;
-  const int64_t row = ((t.start + kj) * int64_t(s.kv_heads) + kv_head) * s.dim;
+  const int64_t at = ((int64_t(t.start) + kj) * s.kv_heads + kv_head) * s.dim;
+  const int64_t whole = a.parts > 1 ? int64_t(part) * s.seqs.tokens * s.kv_heads * s.dim : 0;
+  float* const to_k = a.parts > 1 ? a.dk_p : a.dk;
+  float* const to_v = a.parts > 1 ? a.dv_p : a.dv;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) {
-    if (a.dk) store_block(a.dk + row, dk[b] * s.scale, b, h, s.dim);
-    if (a.dv) store_block(a.dv + row, dv[b], b, h, s.dim);
+    // q was packed times scale log2(e)
+    if (a.dk) store_block(to_k + whole + at, dk[b] * kLn2, b, h, s.dim);
+    if (a.dv) store_block(to_v + whole + at, dv[b], b, h, s.dim);
+  }
+}
+
+// dk and dv: the parts' sums, in order; a workgroup takes a tile of rows of one key head.
+__global__ __launch_bounds__(kThreads) void join_kernel(const BwdArgs a) {
+  const Shape& s = a.s;
+  SequenceTile t;
+  if (!locate<kTile>(s.seqs, blockIdx.x, t) || t.index * kTile >= t.len) return;
+  const int rows = min(kTile, t.len - t.index * kTile);
+  const int64_t step = int64_t(s.seqs.tokens) * s.kv_heads * s.dim;
+  for (int i = threadIdx.x; i < rows * s.dim; i += kThreads) {
+    const int r = i / s.dim;
+    const int64_t at = ((int64_t(t.start) + t.index * kTile + r) * s.kv_heads + blockIdx.y) * s.dim + i - r * s.dim;
+    float k = 0, v = 0;
+    for (int p = 0; p < a.parts; ++p) {
+      if (a.dk) k += a.dk_p[p * step + at];
+      if (a.dv) v += a.dv_p[p * step + at];
+    }
+    if (a.dk) a.dk[at] = k;
+    if (a.dv) a.dv[at] = v;
   }
 }
 
@@ -388,6 +536,7 @@ int check(const char* who, const mx_attention_desc* d) {
              " heads do not share ", d->kv_heads, " key heads evenly");
   MX_REQUIRE(d->tokens <= (1 << 30) && d->sequences <= (1 << 24) && d->heads + d->kv_heads <= 65535, MX_ERR_INVALID, who,
              ": size out of range");
+  MX_REQUIRE((d->tokens / kBlock + d->sequences) * d->heads < (int64_t(1) << 31), MX_ERR_INVALID, who, ": size out of range");
   MX_REQUIRE(d->tokens == 0 || d->sequences > 0, MX_ERR_INVALID, who, ": tokens of no sequence");
   MX_REQUIRE(d->starts || d->sequences == 0 || d->tokens % d->sequences == 0, MX_ERR_INVALID, who, ": ", d->tokens,
              " tokens do not divide into ", d->sequences, " sequences");
@@ -421,31 +570,41 @@ struct Carve {
 };
 
 struct Buffers {
-  bf16x8 *qr, *qt, *kr, *kt, *vr, *vt, *dr, *dt;
-  float* stats;
+  char *qp, *kp, *vp, *dp;
+  float *stats, *dk_p, *dv_p;
 };
-Buffers carve(const Shape& s, bool backward, Carve& c) {
+Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
   const int64_t tile = padded(s.dim) / 16 * 3 * 1024, q = tile * s.tiles * s.heads, k = tile * s.tiles * s.kv_heads;
   Buffers b{};
-  b.qr = c.take<bf16x8>(q);
-  b.kr = c.take<bf16x8>(k);
-  if (!backward) {
-    b.vt = c.take<bf16x8>(k);
-    return b;
-  }
-  b.qt = c.take<bf16x8>(q);
-  b.dr = c.take<bf16x8>(q);
-  b.dt = c.take<bf16x8>(q);
-  b.kt = c.take<bf16x8>(k);
-  b.vr = c.take<bf16x8>(k);
+  b.kp = c.take<char>(k);
+  b.vp = c.take<char>(k);
+  if (!backward) return b;
+  b.qp = c.take<char>(q);
+  b.dp = c.take<char>(q);
   b.stats = c.take<float>(int64_t(s.heads) * s.tiles * 256);
+  if (parts > 1) {
+    const int64_t part = (int64_t(parts) * s.seqs.tokens * s.kv_heads * s.dim * 4 + 255) / 256 * 256;
+    b.dk_p = c.take<float>(part);
+    b.dv_p = c.take<float>(part);
+  }
   return b;
+}
+
+int64_t blocks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kBlock); }
+
+// Parts that a key head's query heads are dealt into: as few as give every CU four
+// workgroups of 128 keys (the first keys of a sequence have the most to do).
+int parts_of(const Shape& s) {
+  for (int p = 1; p <= s.group; ++p)
+    if (s.group % p == 0 && blocks_of(s) * s.kv_heads * p >= int64_t(cu_count()) * 4) return p;
+  return s.group;
 }
 
 int64_t workspace_bytes_of(const mx_attention_desc* d, bool backward) {
   if (d->tokens == 0 || d->heads == 0) return 0;
   Carve c{nullptr};
-  carve(shape_of(d), backward, c);
+  const Shape s = shape_of(d);
+  carve(s, backward, backward ? parts_of(s) : 1, c);
   return c.used;
 }
 
@@ -486,18 +645,18 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   Workspace ws;
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_bytes_of(d, false), st));
   Carve c{ws.as<char>()};
-  const Buffers b = carve(s, false, c);
+  const Buffers b = carve(s, false, 1, c);
   PackArgs p{};
   p.s = s;
-  p.q = {q, d->q_token, d->q_head}, p.k = {k, d->k_token, d->k_head}, p.v = {v, d->v_token, d->v_head};
-  p.qr = b.qr, p.kr = b.kr, p.vt = b.vt;
-  const FwdArgs f{s, b.qr, b.kr, b.vt, out, lse};
+  p.k = {k, d->k_token, d->k_head}, p.v = {v, d->v_token, d->v_head};
+  p.kp = b.kp, p.vp = b.vp;
+  const FwdArgs f{s, {q, d->q_token, d->q_head}, b.kp, b.vp, out, lse};
   with_dim(s.dim, [&](auto dp) {
-    hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
   with_dim(s.dim, [&](auto dp) {
-    hipLaunchKernelGGL((fwd_kernel<decltype(dp)::value>), dim3((s.tiles + 3) / 4, s.heads), dim3(kThreads), 0, st, f);
+    hipLaunchKernelGGL((fwd_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, f);
   });
   MX_LAUNCHED();
   return MX_OK;
@@ -518,32 +677,35 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   Workspace ws;
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_bytes_of(d, true), st));
   Carve c{ws.as<char>()};
-  const Buffers b = carve(s, true, c);
+  const int parts = parts_of(s);
+  const Buffers b = carve(s, true, parts, c);
   PackArgs p{};
   p.s = s;
   p.q = {q, d->q_token, d->q_head}, p.k = {k, d->k_token, d->k_head}, p.v = {v, d->v_token, d->v_head};
   p.dout = {dout, d->heads * d->head_dim, d->head_dim}, p.out = {out, d->heads * d->head_dim, d->head_dim};
   p.lse = lse;
-  p.qr = b.qr, p.kr = b.kr, p.vr = b.vr, p.dr = b.dr;
-  if (dk || dv) p.qt = b.qt, p.dt = b.dt;
-  if (dq) p.kt = b.kt;
-  p.stats = b.stats;
-  const BwdArgs g{s, b.qr, b.qt, b.kr, b.kt, b.vr, b.dr, b.dt, b.stats, dq, dk, dv};
+  p.qp = b.qp, p.kp = b.kp, p.vp = b.vp, p.dp = b.dp, p.stats = b.stats;
+  const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p};
   with_dim(s.dim, [&](auto dp) {
     hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
   if (dq) {
     with_dim(s.dim, [&](auto dp) {
-      hipLaunchKernelGGL((dq_kernel<decltype(dp)::value>), dim3((s.tiles + 3) / 4, s.heads), dim3(kThreads), 0, st, g);
+      hipLaunchKernelGGL((dq_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
   }
   if (dk || dv) {
     with_dim(s.dim, [&](auto dp) {
-      hipLaunchKernelGGL((dkv_kernel<decltype(dp)::value>), dim3((s.tiles + 3) / 4, s.kv_heads), dim3(kThreads), 0, st, g);
+      hipLaunchKernelGGL((dkv_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.kv_heads * parts)), dim3(kThreads),
+                         0, st, g);
     });
     MX_LAUNCHED();
+    if (parts > 1) {
+      hipLaunchKernelGGL(join_kernel, dim3(s.tiles, s.kv_heads), dim3(kThreads), 0, st, g);
+      MX_LAUNCHED();
+    }
   }
   return MX_OK;
   MX_ABI_END

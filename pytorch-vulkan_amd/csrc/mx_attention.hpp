@@ -60,9 +60,12 @@ struct Mask {
   __device__ __forceinline__ bool sees(int i, int j) const {
     return j <= i && (window == 0 || i - j < window || j < sinks);
   }
-  // Every one of queries i0 .. i1 sees every one of keys j0 .. j1.
+  // Every one of queries i0 .. i1 sees every one of keys j0 .. j1; none sees any of them.
   __device__ __forceinline__ bool all(int i0, int i1, int j0, int j1) const {
     return j1 <= i0 && (window == 0 || i1 - j0 < window || j1 < sinks);
+  }
+  __device__ __forceinline__ bool none(int i0, int i1, int j0, int j1) const {
+    return j0 > i1 || (window != 0 && i0 - j1 >= window && j0 >= sinks);
   }
 };
 
