@@ -188,7 +188,7 @@ __device__ __forceinline__ uint32_t lds_address(char* p) {
 }
 
 // Two tensors' tiles (and 256 bytes of statistics) in LDS, two stages.
-template <int DP, bool STATS = false>
+template <int DP, int WAVES, bool STATS = false>
 struct Stages {
   static constexpr int kBytes = 2 * kTileBytes<DP> + (STATS ? 1024 : 0);
   static constexpr int kSecond = kTileBytes<DP>, kStats = 2 * kTileBytes<DP>;
@@ -198,9 +198,9 @@ struct Stages {
     const char *const pa = pieces::uniform(a), *const pb = pieces::uniform(b);
     constexpr int F = DP / 16 * 3;
 #pragma unroll
-    for (int i = 0; i < F / 2; ++i) {
-      const int f = wave + 4 * i;  // a's fragments, then b's
-      pieces::load_lds16(f < F ? pa + f * 1024 : pb + (f - F) * 1024, lane * 16, to + f * 1024);
+    for (int i = 0; i < (2 * F + WAVES - 1) / WAVES; ++i) {
+      const int f = wave + WAVES * i;  // a's fragments, then b's
+      if (2 * F % WAVES == 0 || f < 2 * F) pieces::load_lds16(f < F ? pa + f * 1024 : pb + (f - F) * 1024, lane * 16, to + f * 1024);
     }
     if constexpr (STATS)
       if (wave == 0) load_lds4(pieces::uniform(stats), lane * 4, to + kStats);
@@ -236,17 +236,29 @@ __device__ __forceinline__ Frag3 frag_columns(uint32_t tile_and_base, int b, int
   return {f[0], f[1], f[2]};
 }
 
+// Exponents of scores that are not seen (a NaN among them) have no probability.  The branch is the same for a wave; the
+// barrier keeps the compiler from comparing in every tile, seen as a whole or not.
+template <class F>
+__device__ __forceinline__ void hide(f32x16& x, F&& sees) {
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (!sees(r)) x[r] = -__builtin_inff();
+}
+// a b, 0 where either is 0: what a probability of 0 meets may be anything.
+extern "C" __device__ float mx_mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float times(float a, float b) { return mx_mul_legacy(a, b); }
+
 // a b along the head's elements: a's tile in LDS, b's fragments in registers.
 template <int DP>
 __device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane) {
-  f32x16 small{}, large{};
+  f32x16 acc{};
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     const Frag3 f = frag(a, s, lane);
-    small = mma_small(f, b[s], small);
-    large = mma_large(f, b[s], large);
+    acc = mma_large(f, b[s], mma_small(f, b[s], acc));
   }
-  return large + small;
+  return acc;
 }
 
 // Block b of a p along the tile's rows: a's tile in LDS (and the lane's column_base), p's pieces.
@@ -305,19 +317,20 @@ struct FwdArgs {
   float *out, *lse;
 };
 
-template <int DP>
-__global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
-  using St = Stages<DP>;
+template <int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP > 96 ? 1 : 2))) void fwd_kernel(const FwdArgs a) {
+  using St = Stages<DP, WAVES>;
+  constexpr int kRows = WAVES * kTile;
   __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
   SequenceTile t;
-  if (!locate<kBlock>(s.seqs, block, t) || t.index * kBlock >= t.len) return;
+  if (!locate<kRows>(s.seqs, block, t) || t.index * kRows >= t.len) return;
   const int64_t keys0 = tile_at<DP>(s, head / s.group, t.start / kTile + t.seq);
-  const int b0 = t.index * kBlock, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
+  const int b0 = t.index * kRows, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
   const St st{lds_address(smem)};
-  const KeyTiles keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
+  const KeyTiles keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
   const auto fetch = [&](int n) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
     st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
@@ -336,11 +349,7 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
     if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
     f32x16 x = product<DP>(tile, q, lane);
-    if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!s.mask.sees(qi, j0 + 16 * h + r)) x[r] = -__builtin_inff();
-    }
+    if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
     float top = x[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
@@ -357,7 +366,10 @@ __global__ __launch_bounds__(kThreads) void fwd_kernel(const FwdArgs a) {
     m = next;
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) o[b] = o[b] * keep + product_rows(tile + St::kSecond + columns, b, p);
+    for (int b = 0; b < DP / 32; ++b) {
+      if (DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
+      o[b] = o[b] * keep + product_rows(tile + St::kSecond + columns, b, p);
+    }
   }
   l += __shfl_xor(l, 32, 64);
   if (qi >= t.len) return;
@@ -380,7 +392,7 @@ struct BwdArgs {
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
-  using St = Stages<DP>;
+  using St = Stages<DP, 4>;
   __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -413,15 +425,11 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     const int j0 = keys.tile(n) * kTile;
     if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
-    f32x16 x = product<DP>(tile, q, lane);
+    f32x16 x = product<DP>(tile, q, lane) - lse;
+    if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
     const f32x16 dp = product<DP>(tile + St::kSecond, g, lane);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = exp2_(x[r] - lse) * (dp[r] - delta);
-    if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!s.mask.sees(qi, j0 + 16 * h + r)) x[r] = 0;
-    }
+    for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dq[b] += product_rows(tile + columns, b, p);
@@ -434,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
-  using St = Stages<DP, true>;
+  using St = Stages<DP, 4, true>;
   __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -467,23 +475,20 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
     const int i0 = (from + n % tiles) * kTile;
     if (s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
-    f32x16 x = product<DP>(tile, k, lane);
-    f32x16 dp = product<DP>(tile + St::kSecond, v, lane);
+    f32x16 x = product<DP>(tile, k, lane), delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t at = tile + St::kStats + (16 * h + 4 * i) * 4;
-      const f32x4 lse = *pieces::lds_at<const f32x4>(at), delta = *pieces::lds_at<const f32x4>(at + 128);
+      const f32x4 lse = *pieces::lds_at<const f32x4>(at), d = *pieces::lds_at<const f32x4>(at + 128);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * i + e;
-        x[r] = exp2_(x[r] - lse[e]);
-        dp[r] = x[r] * (dp[r] - delta[e]);
-      }
+      for (int e = 0; e < 4; ++e) x[4 * i + e] -= lse[e], delta[4 * i + e] = d[e];
     }
-    if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) {
+    if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) hide(x, [&](int r) { return s.mask.sees(i0 + 16 * h + r, kj); });
+    f32x16 dp = product<DP>(tile + St::kSecond, v, lane);
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!s.mask.sees(i0 + 16 * h + r, kj)) x[r] = 0, dp[r] = 0;
+    for (int r = 0; r < 16; ++r) {
+      x[r] = exp2_(x[r]);
+      dp[r] = times(x[r], dp[r] - delta[r]);
     }
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)}, ds[2] = {split_half(dp, 0), split_half(dp, 1)};
 #pragma unroll
@@ -590,6 +595,8 @@ Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
   return b;
 }
 
+constexpr int fwd_waves(int dp) { return dp > 96 ? 4 : 8; }
+
 int64_t blocks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kBlock); }
 
 // Parts that a key head's query heads are dealt into: as few as give every CU four
@@ -656,7 +663,9 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   });
   MX_LAUNCHED();
   with_dim(s.dim, [&](auto dp) {
-    hipLaunchKernelGGL((fwd_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, f);
+    constexpr int W = fwd_waves(decltype(dp)::value);
+    const int64_t blocks = sequence_tiles(s.seqs.tokens, s.seqs.count, W * kTile);
+    hipLaunchKernelGGL((fwd_kernel<decltype(dp)::value, W>), dim3(unsigned(blocks * s.heads)), dim3(64 * W), 0, st, f);
   });
   MX_LAUNCHED();
   return MX_OK;
