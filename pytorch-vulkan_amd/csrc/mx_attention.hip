@@ -245,10 +245,6 @@ __device__ __forceinline__ void hide(f32x16& x, F&& sees) {
   for (int r = 0; r < 16; ++r)
     if (!sees(r)) x[r] = -__builtin_inff();
 }
-// a b, 0 where either is 0: what a probability of 0 meets may be anything.
-extern "C" __device__ float mx_mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
-__device__ __forceinline__ float times(float a, float b) { return mx_mul_legacy(a, b); }
-
 // a b along the head's elements: a's tile in LDS, b's fragments in registers.
 template <int DP>
 __device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane) {
@@ -330,7 +326,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP >
   const int64_t keys0 = tile_at<DP>(s, head / s.group, t.start / kTile + t.seq);
   const int b0 = t.index * kRows, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
   const St st{lds_address(smem)};
-  const KeyTiles keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
+  const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
   const auto fetch = [&](int n) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
     st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
@@ -403,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   const int64_t keys0 = tile_at<DP>(s, head / s.group, base32);
   const int b0 = t.index * kBlock, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
   const St st{lds_address(smem)};
-  const KeyTiles keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
+  const KeyTiles<> keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
   const auto fetch = [&](int n) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
     st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);

@@ -54,6 +54,10 @@ __device__ __forceinline__ Frag3 split_half(const f32x16& v, int t) {
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// a b, 0 where either is 0: what a probability of 0 meets may be anything.
+extern "C" __device__ float mx_mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float times(float a, float b) { return mx_mul_legacy(a, b); }
+
 // Whether the query at position i sees the key at position j.
 struct Mask {
   int window, sinks;  // window 0: every earlier key
@@ -69,13 +73,14 @@ struct Mask {
   }
 };
 
-// The tiles of keys that queries i0 .. i1 see, first those of the first tokens.
+// The tiles of U keys that queries i0 .. i1 see, first those of the first tokens.
+template <int U = kTile>
 struct KeyTiles {
   int sinks, from, count;  // tiles 0 .. sinks - 1, then from ..; `count` in all
   __device__ __forceinline__ KeyTiles(const Mask& m, int i0, int i1) {
-    from = m.window ? max(0, i0 - m.window + 1) / kTile : 0;
-    const int end = i1 < 0 ? 0 : i1 / kTile + 1;
-    sinks = m.window ? min((m.sinks + kTile - 1) / kTile, min(from, end)) : 0;
+    from = m.window ? max(0, i0 - m.window + 1) / U : 0;
+    const int end = i1 < 0 ? 0 : i1 / U + 1;
+    sinks = m.window ? min((m.sinks + U - 1) / U, min(from, end)) : 0;
     count = sinks + max(0, end - from);
   }
   __device__ __forceinline__ int tile(int n) const { return n < sinks ? n : from + n - sinks; }

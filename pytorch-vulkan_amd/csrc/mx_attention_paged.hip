@@ -9,9 +9,12 @@
 // byte is a bf16 number: products with it take three matrix instructions (the row's
 // three pieces) in place of six, and the scales go to the scores and the probabilities.
 //
-// A wave takes tiles of 32 keys straight from the cache into operand fragments: lane l
-// reads 16 elements of key tile_row(l % 32) and 16 keys of element tile_row(l % 32), each
-// from consecutive places, in half l / 32 of the tile (which may lie in another page).
+// A wave takes tiles of 64 keys straight from the cache into operand fragments of
+// v_mfma_f32_16x16x32_bf16 (16 rows: a token's query heads seldom are more, and both its
+// registers and its matrix instructions are half of the 32 x 32 form's).  Quarter g of the
+// wave holds keys 16 g .. 16 g + 15 of a tile: the scores that it ends with, and the
+// values that it reads, 16 consecutive places of one element; a key's elements are read 16
+// at a time too.  Keys are read a tile ahead of their products, their pages two.
 // The keys of a row tile are dealt to the workgroup's waves, and to several workgroups
 // where there are few rows; waves join through LDS, workgroups through the workspace and a
 // second launch, both in a fixed order.
@@ -32,23 +35,38 @@ using mfma::f32x2;
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256, kWaves = 4, kRows = 16, kKeys = 64;
 
 struct PagedArgs {
   Cache c;
   Batch b;
   const float* q;
   int64_t q_token, q_head;
-  int heads, group, tiles, splits;
+  int heads, group, tiles, splits, span;  // span: tiles of keys to a workgroup
   Mask mask;
   float scale;
   float *out, *part;
 };
 
-// The workgroups' parts: [tile][kv head][split] of 32 maxima, 32 sums and 32 rows of dim.
+// The workgroups' parts: [row tile][kv head][split] of 16 maxima, 16 sums and 16 rows of dim.
 __device__ __forceinline__ int64_t part_at(const PagedArgs& a, int tile, int head, int split) {
-  return ((int64_t(tile) * a.c.heads + head) * a.splits + split) * (kTile * (2 + a.c.dim));
+  return ((int64_t(tile) * a.c.heads + head) * a.splits + split) * (kRows * (2 + a.c.dim));
 }
+
+// What a row tile sees: its sequence's tokens, positions and tiles of keys.
+struct RowTile {
+  SequenceTile t;
+  int length, first, i0, i1;  // tokens of the sequence, its first new one, the tile's positions
+  __device__ __forceinline__ bool find(const PagedArgs& a, int tile) {
+    if (!locate<kRows>(a.b.seqs, tile, t) || t.index * kRows >= t.len) return false;
+    const int last = a.b.lengths[t.seq];
+    length = int(min(int64_t(max(last, 0)), int64_t(a.b.width) * a.c.page_size));
+    first = last - t.len / a.group;
+    i0 = first + t.index * kRows / a.group;
+    i1 = min(first + (min(t.len, (t.index + 1) * kRows) - 1) / a.group, length - 1);
+    return true;
+  }
+};
 
 // 16 elements as operand pieces: one where they are bytes, three where they are FP32.
 template <bool I8>
@@ -80,122 +98,150 @@ struct Sixteen<false> {
   __device__ __forceinline__ Frag3 half(int t) const { return split8(raw[2 * t], raw[2 * t + 1]); }
 };
 
-__device__ __forceinline__ void mma_all(const bf16x8& a, const Frag3& b, f32x16& small, f32x16& large) {
-  small = mma(a, b.lo, small);
-  small = mma(a, b.mid, small);
-  large = mma(a, b.hi, large);
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ void mma_all(const Frag3& a, const Frag3& b, f32x16& small, f32x16& large) {
-  small = mma_small(a, b, small);
-  large = mma_large(a, b, large);
+__device__ __forceinline__ f32x4 mma_all(const bf16x8& a, const Frag3& b, f32x4 c) {
+  return mma16(a, b.hi, mma16(a, b.mid, mma16(a, b.lo, c)));
+}
+__device__ __forceinline__ f32x4 mma_all(const Frag3& a, const Frag3& b, f32x4 c) {
+  c = mma16(a.lo, b.hi, c);
+  c = mma16(a.hi, b.lo, c);
+  c = mma16(a.mid, b.mid, c);
+  c = mma16(a.mid, b.hi, c);
+  return mma16(a.hi, b.hi, mma16(a.hi, b.mid, c));
 }
 
+// Over the wave's quarters, which hold the same 16 rows.
+__device__ __forceinline__ float quarters_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// The page of a lane's group of 16 keys, and the group's first place in it.
+struct Place {
+  int page, place;
+  __device__ __forceinline__ void find(const Cache& c, const Batch& b, int seq, int tile, int group) {
+    page = kv::page_of(c, b, seq, tile * (kKeys / 16) + group, place);
+  }
+};
+
 template <int DP, bool I8>
-__global__ __launch_bounds__(kThreads) void paged_kernel(const PagedArgs a) {
-  constexpr int kUnits = DP / 32, kPitch = DP + 4;
-  __shared__ float stat[2][kWaves][kTile], sum[kTile][kPitch];
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2 : 1))) void paged_kernel(const PagedArgs a) {
+  constexpr int kUnits = DP / 64, kBlocks = DP / 16, kPitch = DP + 4;
+  __shared__ float stat[2][kWaves][kRows], sum[kRows][kPitch];
   using E = std::conditional_t<I8, int8_t, float>;
   const Cache& c = a.c;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int kv_head = blockIdx.y;
-  SequenceTile t;
-  if (!locate<kTile>(a.b.seqs, blockIdx.x, t) || t.index * kTile >= t.len) return;
-  const int length = int(min(int64_t(max(a.b.lengths[t.seq], 0)), int64_t(a.b.width) * c.page_size));
-  const int first = a.b.lengths[t.seq] - t.len / a.group;  // position of the sequence's first new token
+  RowTile rt;
+  if (!rt.find(a, blockIdx.x)) return;
+  const SequenceTile& t = rt.t;
+  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.i1);
+  // This workgroup's tiles of keys, dealt to its waves.
+  const int begin = blockIdx.z * a.span, end = c.pages ? min(keys.count, begin + a.span) : 0;
+  if (blockIdx.z && begin >= end) return;
   // The lane's row: a token and a query head.
-  const int row = t.index * kTile + (lane & 31), last_row = min(t.len, (t.index + 1) * kTile) - 1;
-  const int token = min(row, t.len - 1) / a.group, pos = first + token;
-  const int head = kv_head * a.group + min(row, t.len - 1) - token * a.group;
-  const int64_t flat = t.start / a.group + token;
+  const int row = min(t.index * kRows + col, t.len - 1), token = row / a.group, pos = rt.first + token;
+  const int head = kv_head * a.group + row - token * a.group;
+  const int kg = col >> 2;  // the group of the keys whose elements this lane reads
+  Place kp, vp;             // of this tile's keys and values
+  const auto find = [&](int n, Place& k, Place& v) {
+    const int tile = keys.tile(min(n, end - 1));
+    k.find(c, a.b, t.seq, tile, kg);
+    v.find(c, a.b, t.seq, tile, g);
+  };
+  // Key 16 kg + 4 i + col % 4 is row col of the tile's i-th block of 16.
+  Sixteen<I8> k[4][kUnits];
+  const auto fetch = [&](const Place& at) {
+    const E* const from = static_cast<const E*>(c.k) +
+                          ((int64_t(max(at.page, 0)) * c.heads + kv_head) * c.page_size + at.place + (col & 3)) * c.dim + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        k[i][u] = {};
+        if (64 * u + 16 * g < c.dim) k[i][u].load(from + 4 * i * c.dim + 64 * u);
+      }
+  };
+  const int from = begin + wave;
   Frag3 q[2 * kUnits];
-  {
-    const float* const src = a.q + flat * a.q_token + head * a.q_head + 16 * h;
+  if (from < end) {
+    find(from, kp, vp);
+    const float* const src = a.q + (t.start / a.group + token) * a.q_token + head * a.q_head + 16 * g;
+    const float scale = a.scale * kLog2E;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       f32x4 v[4] = {};
-      if (32 * u + 16 * h < c.dim) {
+      if (64 * u + 16 * g < c.dim) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4u*>(src + 32 * u + 4 * i);
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const f32x4u*>(src + 64 * u + 4 * i) * scale;
       }
       q[2 * u] = split8(v[0], v[1]);
       q[2 * u + 1] = split8(v[2], v[3]);
     }
+    fetch(kp);
   }
-  const int i0 = first + t.index * kTile / a.group, i1 = min(first + last_row / a.group, length - 1);
-  const float scale = a.scale * kLog2E;
-  f32x16 o[kUnits] = {};
-  float m = -__builtin_inff(), l = 0;
-  const KeyTiles keys(a.mask, max(i0, 0), i1);
-  const int64_t token_bytes = c.dim * int64_t(sizeof(E));
-  const int count = c.pages ? keys.count : 0;
-  for (int n = blockIdx.z * kWaves + wave; n < count; n += kWaves * a.splits) {
-    const int j0 = keys.tile(n) * kTile;
-    int place[2], page[2];
-#pragma unroll
-    for (int g = 0; g < 2; ++g) page[g] = kv::page_of(c, a.b, t.seq, (j0 >> 4) + g, place[g]);
-    const bool whole = page[0] >= 0 && page[1] >= 0 && j0 + kTile <= length;
-    int64_t at[2];  // places' rows in the cache; those of absent pages are page 0's, and seen by no row
-#pragma unroll
-    for (int g = 0; g < 2; ++g) at[g] = (int64_t(max(page[g], 0)) * c.heads + kv_head) * c.page_size;
-    const int kg = lane >> 2 & 1, kr = (lane & 31) >> 3 << 2 | (lane & 3);  // tile_row's half and rest
-    const char* const krow = static_cast<const char*>(c.k) + ((kg ? at[1] + place[1] : at[0] + place[0]) + kr) * token_bytes;
-    const int64_t mine = h ? at[1] : at[0];
-    const int in_page = h ? place[1] : place[0];
-    // ---- scores
-    f32x16 x{}, small{};
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      Sixteen<I8> k{};
-      if (32 * u + 16 * h < c.dim) k.load(krow + (32 * u + 16 * h) * sizeof(E));
-      mma_all(k.half(0), q[2 * u], small, x);
-      mma_all(k.half(1), q[2 * u + 1], small, x);
-    }
-    x += small;
-    f32x16 vscale;
+  f32x4 o[kBlocks] = {};
+  float m = -__builtin_inff(), l = 0;  // of the exponents
+  for (int n = from; n < end; n += kWaves) {
+    const int j0 = keys.tile(n) * kKeys, j = j0 + 16 * g;  // the lane's 16 keys: j ..
+    const bool here = vp.page >= 0;
+    const int64_t places = (int64_t(max(vp.page, 0)) * c.heads + kv_head) * c.page_size;
+    Place kn, vn;
+    find(n + kWaves, kn, vn);
+    // ---- scales and values, while the scores are computed
+    f32x4 ks[4], vs[4];
     if constexpr (I8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 ks = *reinterpret_cast<const f32x4*>(c.ks + mine + in_page + 4 * i);
-        const f32x4 vs = *reinterpret_cast<const f32x4*>(c.vs + mine + in_page + 4 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * i + e] *= ks[e], vscale[4 * i + e] = vs[e];
+        ks[i] = *reinterpret_cast<const f32x4*>(c.ks + places + vp.place + 4 * i);
+        vs[i] = *reinterpret_cast<const f32x4*>(c.vs + places + vp.place + 4 * i);
       }
     }
-    const bool part = !whole || !a.mask.all(i0, i1, j0, j0 + kTile - 1);
-    const bool here = (h ? page[1] : page[0]) >= 0;
+    Sixteen<I8> v[kBlocks];
+    const E* const vfrom = static_cast<const E*>(c.v) + places * c.dim + int64_t(col) * c.page_size + vp.place;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] *= scale;
+    for (int b = 0; b < kBlocks; ++b) {
+      v[b] = {};
+      if (16 * b < c.dim) v[b].load(vfrom + int64_t(16 * b) * c.page_size);
+    }
+    // ---- scores: block i gives the lane keys j + 4 i .. + 3
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc{};
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (64 * u >= c.dim) continue;
+        acc = mma_all(k[i][u].half(0), q[2 * u], acc);
+        acc = mma_all(k[i][u].half(1), q[2 * u + 1], acc);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = I8 ? acc[e] * ks[i][e] : acc[e];
+    }
+    if (n + kWaves < end) fetch(kn);
+    const bool part = __any(!here || j + 16 > rt.length) || !a.mask.all(rt.i0, rt.i1, j0, j0 + kKeys - 1);
     if (part) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = j0 + 16 * h + r;
-        if (!here || j >= length || !a.mask.sees(pos, j)) x[r] = -__builtin_inff();
-      }
-    }
-    // ---- values
-    Sixteen<I8> v[kUnits];
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const int d = 32 * u + tile_row(lane & 31);
-      v[u] = {};
-      if (d < c.dim) v[u].load(static_cast<const E*>(c.v) + mine * c.dim + int64_t(d) * c.page_size + in_page);
-    }
-    if constexpr (!I8) {
-      // What no row sees counts as zero, and a value that is not finite as a NaN score of its key.
-      if (part) {
+      for (int r = 0; r < 16; ++r)
+        if (!here || j + r >= rt.length || !a.mask.sees(pos, j + r)) x[r] = -__builtin_inff();
+      if constexpr (!I8) {
+        // What no row sees counts as zero, and a value that is not finite as a NaN score of its key.
         uint32_t bad = 0;
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u)
+        for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float e = v[u].raw[r >> 2][r & 3];
-            const bool no = !here || j0 + 16 * h + r >= length, odd = !(fabsf(e) <= 3.402823466e38f);
+            const float e = v[b].raw[r >> 2][r & 3];
+            const bool no = !here || j + r >= rt.length, odd = !(fabsf(e) <= 3.402823466e38f);
             if (odd && !no) bad |= 1u << r;
-            if (no || odd) v[u].raw[r >> 2][r & 3] = 0;
+            if (no || odd) v[b].raw[r >> 2][r & 3] = 0;
           }
         if (__any(bad != 0)) {
 #pragma unroll
-          for (int s = 1; s < 32; s <<= 1) bad |= __shfl_xor(int(bad), s, 64);
+          for (int s = 1; s < 16; s <<= 1) bad |= __shfl_xor(int(bad), s, 64);
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (bad >> r & 1 && x[r] != -__builtin_inff()) x[r] = __builtin_nanf("");
@@ -206,8 +252,7 @@ __global__ __launch_bounds__(kThreads) void paged_kernel(const PagedArgs a) {
     float top = x[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float next = fmaxf(m, top), base = next == -__builtin_inff() ? 0.f : next;
+    const float next = fmaxf(m, quarters_max(top)), base = next == -__builtin_inff() ? 0.f : next;
     const float keep = exp2_(m - base);
     float add = 0;
 #pragma unroll
@@ -219,80 +264,98 @@ __global__ __launch_bounds__(kThreads) void paged_kernel(const PagedArgs a) {
     m = next;
     if constexpr (I8) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = x[r] == 0 ? 0.f : x[r] * vscale[r];  // an unseen scale may be anything
+      for (int r = 0; r < 16; ++r) x[r] = times(x[r], vs[r >> 2][r & 3]);  // an unseen scale may be anything
     }
-    const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
+    const Frag3 p[2] = {split8(f32x4{x[0], x[1], x[2], x[3]}, f32x4{x[4], x[5], x[6], x[7]}),
+                        split8(f32x4{x[8], x[9], x[10], x[11]}, f32x4{x[12], x[13], x[14], x[15]})};
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      f32x16 acc{}, lower{};
-      mma_all(v[u].half(0), p[0], lower, acc);
-      mma_all(v[u].half(1), p[1], lower, acc);
-      o[u] = o[u] * keep + (acc + lower);
-    }
+    for (int b = 0; b < kBlocks; ++b)
+      if (16 * b < c.dim) o[b] = o[b] * keep + mma_all(v[b].half(1), p[1], mma_all(v[b].half(0), p[0], f32x4{}));
+    kp = kn, vp = vn;
   }
+  l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   // ---- the workgroup's waves, in order
-  if (h == 0) stat[0][wave][lane] = m, stat[1][wave][lane] = l;
+  if (g == 0) stat[0][wave][col] = m, stat[1][wave][col] = l;
   __syncthreads();
   float all = -__builtin_inff(), total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, stat[0][w][lane & 31]);
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, stat[0][w][col]);
   const float base = all == -__builtin_inff() ? 0.f : all;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) total = fmaf(stat[1][w][lane & 31], exp2_(stat[0][w][lane & 31] - base), total);
+  for (int w = 0; w < kWaves; ++w) total = fmaf(stat[1][w][col], exp2_(stat[0][w][col] - base), total);
   const float mul = exp2_(m - base);
   for (int w = 0; w < kWaves; ++w) {
     if (w == wave) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4* const to = reinterpret_cast<f32x4*>(&sum[lane & 31][32 * u + 16 * h + 4 * i]);
-          f32x4 add;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) add[e] = o[u][4 * i + e] * mul;
-          *to = w ? *to + add : add;
-        }
+      for (int b = 0; b < kBlocks; ++b) {
+        f32x4* const to = reinterpret_cast<f32x4*>(&sum[col][16 * b + 4 * g]);
+        *to = w ? *to + o[b] * mul : o[b] * mul;
+      }
     }
     __syncthreads();
   }
-  // ---- out: 8 threads a row
-  const int r = threadIdx.x >> 3, cc = threadIdx.x & 7, orow = t.index * kTile + r;
-  if (wave == 0 && h == 0) stat[0][0][lane] = all, stat[1][0][lane] = total;
+  // ---- out: 16 threads a row
+  if (wave == 0 && g == 0) stat[0][0][lane] = all, stat[1][0][lane] = total;
   __syncthreads();
+  const int r = threadIdx.x >> 4, cc = threadIdx.x & 15, orow = t.index * kRows + r;
   if (orow >= t.len) return;
   if (a.splits > 1) {
     float* const to = a.part + part_at(a, blockIdx.x, kv_head, blockIdx.z);
-    if (cc == 0) to[r] = stat[0][0][r], to[kTile + r] = stat[1][0][r];
-    for (int e = cc * 4; e < c.dim; e += 32)
-      *reinterpret_cast<f32x4*>(to + 2 * kTile + r * c.dim + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]);
+    if (cc == 0) to[r] = stat[0][0][r], to[kRows + r] = stat[1][0][r];
+    for (int e = cc * 4; e < c.dim; e += 64)
+      *reinterpret_cast<f32x4*>(to + 2 * kRows + r * c.dim + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]);
     return;
   }
   const float den = stat[1][0][r], inv = den == 0 ? 0.f : 1.f / den;
   const int otoken = orow / a.group;
   float* const to = a.out + ((t.start / a.group + otoken) * int64_t(a.heads) + kv_head * a.group + orow - otoken * a.group) * c.dim;
-  for (int e = cc * 4; e < c.dim; e += 32) *reinterpret_cast<f32x4u*>(to + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]) * inv;
+  for (int e = cc * 4; e < c.dim; e += 64) *reinterpret_cast<f32x4u*>(to + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]) * inv;
 }
 
-// The workgroups that shared a row tile's keys, in order: 8 threads a row.
+// The workgroups that shared a row tile's keys, in order: 16 threads a row, which first share
+// out the workgroups' weights.
+constexpr int kMaxSplits = 64;
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedArgs a) {
-  SequenceTile t;
-  if (!locate<kTile>(a.b.seqs, blockIdx.x, t) || t.index * kTile >= t.len) return;
-  const int r = threadIdx.x >> 3, cc = threadIdx.x & 7, row = t.index * kTile + r, kv_head = blockIdx.y;
-  if (row >= t.len) return;
+  __shared__ float weight[kRows][kMaxSplits];
+  RowTile rt;
+  if (!rt.find(a, blockIdx.x)) return;
+  const SequenceTile& t = rt.t;
+  const int r = threadIdx.x >> 4, cc = threadIdx.x & 15, row = t.index * kRows + r, kv_head = blockIdx.y;
+  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.i1);
+  const int splits = a.c.pages ? max(1, (keys.count + a.span - 1) / a.span) : 1;  // those that have left a part
   const float* const part = a.part + part_at(a, blockIdx.x, kv_head, 0);
-  const int64_t step = kTile * (2 + a.c.dim);
-  float all = -__builtin_inff(), total = 0;
-  for (int i = 0; i < a.splits; ++i) all = fmaxf(all, part[i * step + r]);
+  const int64_t step = kRows * (2 + a.c.dim);
+  float m[kMaxSplits / 16], l[kMaxSplits / 16], all = -__builtin_inff(), total = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 16; ++i) {
+    const int at = cc + 16 * i;
+    const bool has = at < splits && row < t.len;
+    m[i] = has ? part[at * step + r] : -__builtin_inff();
+    l[i] = has ? part[at * step + kRows + r] : 0.f;
+    all = fmaxf(all, m[i]);
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) all = fmaxf(all, __shfl_xor(all, s, 64));
   const float base = all == -__builtin_inff() ? 0.f : all;
-  for (int i = 0; i < a.splits; ++i) total = fmaf(part[i * step + kTile + r], exp2_(part[i * step + r] - base), total);
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 16; ++i) {
+    const float w = exp2_(m[i] - base);
+    weight[r][cc + 16 * i] = w;
+    total = fmaf(l[i], w, total);
+  }
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1) total += __shfl_xor(total, s, 64);
+  __syncthreads();
+  if (row >= t.len) return;
   const float inv = total == 0 ? 0.f : 1.f / total;
   const int token = row / a.group;
   float* const to = a.out + ((t.start / a.group + token) * int64_t(a.heads) + kv_head * a.group + row - token * a.group) * a.c.dim;
-  for (int e = cc * 4; e < a.c.dim; e += 32) {
+  for (int e = cc * 4; e < a.c.dim; e += 64) {
+    const float* const from = part + 2 * kRows + r * a.c.dim + e;
     f32x4 v{};
-    for (int i = 0; i < a.splits; ++i)
-      v += *reinterpret_cast<const f32x4*>(part + i * step + 2 * kTile + r * a.c.dim + e) * exp2_(part[i * step + r] - base);
+#pragma unroll 8
+    for (int i = 0; i < splits; ++i) v += *reinterpret_cast<const f32x4*>(from + i * step) * weight[r][i];
     *reinterpret_cast<f32x4u*>(to + e) = v * inv;
   }
 }
@@ -310,23 +373,31 @@ int check(const char* who, const mx_paged_desc* d, const mx_kv_cache* c, const m
   return MX_OK;
 }
 
-// How many workgroups share a row tile's keys: as many as fill the chip twice, each wave
-// with two tiles of keys at least.
-int splits_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b, int64_t tiles) {
-  int64_t keys = b->table_width * c->page_size;
-  if (d->window) keys = std::min(keys, d->window + d->sinks + b->tokens);
-  const int64_t most = std::max<int64_t>(1, keys / (kTile * kWaves * 2));
-  return int(std::max<int64_t>(1, std::min<int64_t>({most, int64_t(cu_count()) * 2 / std::max<int64_t>(1, tiles * c->heads), 64})));
+int64_t row_tiles(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
+  return sequence_tiles(b->tokens * (d->heads / c->heads), b->sequences, kRows);
 }
 
-int64_t row_tiles(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
-  return sequence_tiles(b->tokens * (d->heads / c->heads), b->sequences, kTile);
+// How a row tile's keys are dealt: `span` tiles of 64 to a workgroup.  As many workgroups as
+// fill the chip twice and even out lengths that the host does not know, each wave with
+// two tiles at least.
+struct Split {
+  int splits, span;
+};
+Split split_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
+  int64_t keys = b->table_width * c->page_size;
+  if (d->window) keys = std::min(keys, d->window + std::min(d->sinks, keys) + b->tokens + 2 * kKeys);
+  const int64_t most = std::max<int64_t>(1, (keys + kKeys - 1) / kKeys), rows = std::max<int64_t>(1, row_tiles(d, c, b) * c->heads);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(int64_t(cu_count()) * 8 / rows, kMaxSplits));
+  // a tile of keys to a wave where even that leaves CUs idle, else four
+  const int64_t least = rows * ((most + kWaves - 1) / kWaves) <= cu_count() * 2 ? kWaves : kWaves * 4;
+  const int64_t span = std::max<int64_t>(((most + want - 1) / want + kWaves - 1) / kWaves * kWaves, least);
+  return {int((most + span - 1) / span), int(span)};
 }
 
 int64_t paged_workspace(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
   if (b->tokens == 0 || d->heads == 0) return 0;
-  const int64_t tiles = row_tiles(d, c, b), splits = splits_of(d, c, b, tiles);
-  return splits == 1 ? 0 : tiles * c->heads * splits * kTile * (2 + c->head_dim) * 4;
+  const int64_t splits = split_of(d, c, b).splits;
+  return splits == 1 ? 0 : row_tiles(d, c, b) * c->heads * splits * kRows * (2 + c->head_dim) * 4;
 }
 
 template <int DP>
@@ -368,17 +439,14 @@ extern "C" int mx_attention_paged(const mx_paged_desc* d, const mx_kv_cache* c, 
   a.b.seqs.per = a.group;
   a.q = q, a.q_token = d->q_token, a.q_head = d->q_head;
   a.tiles = int(row_tiles(d, c, b));
-  a.splits = splits_of(d, c, b, a.tiles);
+  const Split split = split_of(d, c, b);
+  a.splits = split.splits, a.span = split.span;
   a.mask = {int(std::min<int64_t>(d->window, 1 << 30)), int(std::min<int64_t>(d->sinks, 1 << 30))};
   a.scale = float(d->scale);
   a.out = out, a.part = ws.as<float>();
   const dim3 grid(unsigned(a.tiles), unsigned(a.c.heads), unsigned(a.splits));
-  switch ((a.c.dim + 31) / 32) {
-    case 1: launch<32>(a, c->type, grid, s); break;
-    case 2: launch<64>(a, c->type, grid, s); break;
-    case 3: launch<96>(a, c->type, grid, s); break;
-    default: launch<128>(a, c->type, grid, s); break;
-  }
+  if (a.c.dim <= 64) launch<64>(a, c->type, grid, s);
+  else launch<128>(a, c->type, grid, s);
   MX_LAUNCHED();
   if (a.splits > 1) {
     hipLaunchKernelGGL(paged_join_kernel, dim3(grid.x, grid.y), dim3(kThreads), 0, s, a);
