@@ -506,23 +506,29 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
   }
 }
 
-// dk and dv: the parts' sums, in order; a workgroup takes a tile of rows of one key head.
+// dk and dv: the parts' sums, in order, over the rows from the first sequence's start to the
+// last one's end.
 __global__ __launch_bounds__(kThreads) void join_kernel(const BwdArgs a) {
   const Shape& s = a.s;
-  SequenceTile t;
-  if (!locate<kTile>(s.seqs, blockIdx.x, t) || t.index * kTile >= t.len) return;
-  const int rows = min(kTile, t.len - t.index * kTile);
-  const int64_t step = int64_t(s.seqs.tokens) * s.kv_heads * s.dim;
-  for (int i = threadIdx.x; i < rows * s.dim; i += kThreads) {
-    const int r = i / s.dim;
-    const int64_t at = ((int64_t(t.start) + t.index * kTile + r) * s.kv_heads + blockIdx.y) * s.dim + i - r * s.dim;
-    float k = 0, v = 0;
-    for (int p = 0; p < a.parts; ++p) {
-      if (a.dk) k += a.dk_p[p * step + at];
-      if (a.dv) v += a.dv_p[p * step + at];
+  const int64_t row = int64_t(s.kv_heads) * s.dim, step = s.seqs.tokens * row;
+  const int64_t end = s.seqs.start(s.seqs.count) * row;
+  const float* const from = blockIdx.y ? a.dv_p : a.dk_p;
+  float* const to = blockIdx.y ? a.dv : a.dk;
+  if (!to) return;
+  for (int64_t i = s.seqs.start(0) * row + (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4; i < end;
+       i += int64_t(gridDim.x) * kThreads * 4) {
+    if (i + 4 <= end) {
+      f32x4 v{};
+#pragma unroll 4
+      for (int p = 0; p < a.parts; ++p) v += *reinterpret_cast<const f32x4u*>(from + p * step + i);
+      *reinterpret_cast<f32x4u*>(to + i) = v;
+    } else {
+      for (int64_t e = i; e < end; ++e) {
+        float v = 0;
+        for (int p = 0; p < a.parts; ++p) v += from[p * step + e];
+        to[e] = v;
+      }
     }
-    if (a.dk) a.dk[at] = k;
-    if (a.dv) a.dv[at] = v;
   }
 }
 
@@ -708,7 +714,9 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
     });
     MX_LAUNCHED();
     if (parts > 1) {
-      hipLaunchKernelGGL(join_kernel, dim3(s.tiles, s.kv_heads), dim3(kThreads), 0, st, g);
+      const int64_t fours = (d->tokens * d->kv_heads * d->head_dim + 3) / 4;
+      const unsigned blocks = unsigned(std::min<int64_t>((fours + kThreads - 1) / kThreads, int64_t(cu_count()) * 8));
+      hipLaunchKernelGGL(join_kernel, dim3(blocks, 2), dim3(kThreads), 0, st, g);
       MX_LAUNCHED();
     }
   }
