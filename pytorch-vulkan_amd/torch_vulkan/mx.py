@@ -640,43 +640,45 @@ class Rotary:
         self.rotary_dim = 2 * len(frequencies)
         self.frequencies = (C.c_double * max(1, len(frequencies)))(*frequencies)
         self.interleaved, self.magnitude = bool(interleaved), float(magnitude)
+        self.address = C.addressof(self.frequencies)
 
 
-def _packed(name, t, dim=None):
+def _packed(name, t):
     """Strides of a packed tensor [tokens, heads, head_dim] whose last axis is contiguous."""
-    if t.dim() != 3 or t.dtype != torch.float32 or (t.stride(2) != 1 and t.shape[2] > 1 and t.numel()):
-        raise ValueError(f"{name}: expected float32 [tokens, heads, head_dim] with a contiguous last axis, got "
-                         f"{t.dtype} {tuple(t.shape)} of strides {t.stride()}")
-    return t.stride(0), t.stride(1)
+    if t.dtype is torch.float32 and t.dim() == 3:
+        token, head, last = t.stride()
+        if last == 1 or t.shape[2] <= 1 or not t.numel():
+            return token, head
+    raise ValueError(f"{name}: expected float32 [tokens, heads, head_dim] with a contiguous last axis, got "
+                     f"{t.dtype} {tuple(t.shape)} of strides {t.stride()}")
 
 
-def _flat(name, t, shape, dtype=None):
-    if t is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.dtype != (dtype or torch.float32)):
-        raise ValueError(f"{name}: expected a contiguous {dtype or torch.float32} tensor {tuple(shape)}, got {t.dtype} "
+def _flat(name, t, shape, dtype=torch.float32):
+    if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor {tuple(shape)}, got {t.dtype} "
                          f"{tuple(t.shape)} of strides {t.stride()}")
 
 
 def _rotary_desc(q, k, positions, rotary, eps, like):
     """like: (tokens, q heads, k heads, head_dim)."""
-    tokens, hq, hk, dim = like
     if positions is None and rotary.rotary_dim:
         raise ValueError("qk_norm_rotary: no positions")
-    _flat("positions", positions, (tokens,), torch.int64)
+    _flat("positions", positions, like[:1], torch.int64)
     qs = _packed("q", q) if q is not None else (0, 0)
     ks = _packed("k", k) if k is not None else (0, 0)
-    return RotaryDesc(tokens, hq, hk, dim, rotary.rotary_dim, *qs, *ks, ptr(positions),
-                      C.cast(rotary.frequencies, C.c_void_p), rotary.magnitude, 0.0 if eps is None else eps,
-                      int(rotary.interleaved), 0 if eps is None else 1)
+    return RotaryDesc(*like, rotary.rotary_dim, *qs, *ks, ptr(positions), rotary.address, rotary.magnitude,
+                      0.0 if eps is None else eps, rotary.interleaved, eps is not None)
 
 
 def _sides(q, k):
     """(tokens, q heads, k heads, head_dim) of two packed tensors, either of which may be None."""
-    a = q if q is not None else k
-    if a is None:
+    if q is None and k is None:
         raise ValueError("qk_norm_rotary: neither queries nor keys")
-    if k is not None and (k.shape[0] != a.shape[0] or k.shape[2] != a.shape[2]):
-        raise ValueError(f"qk_norm_rotary: queries {tuple(a.shape)} and keys {tuple(k.shape)} do not fit")
-    return a.shape[0], 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], a.shape[2]
+    tokens, hq, dim = q.shape if q is not None else (k.shape[0], 0, k.shape[2])
+    other, hk, dim_k = k.shape if k is not None else (tokens, 0, dim)
+    if other != tokens or dim_k != dim:
+        raise ValueError(f"qk_norm_rotary: queries {tuple(q.shape)} and keys {tuple(k.shape)} do not fit")
+    return tokens, hq, hk, dim
 
 
 def qk_norm_rotary_forward(q, k, positions, rotary, q_out, k_out, q_weight=None, k_weight=None, eps=None,
@@ -685,11 +687,12 @@ def qk_norm_rotary_forward(q, k, positions, rotary, q_out, k_out, q_weight=None,
     [tokens, heads, head_dim]; q or k (with its output) may be None."""
     like = _sides(q, k)
     d = _rotary_desc(q, k, positions, rotary, eps, like)
-    for n, t, x in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if x is not None:
-            _flat(n, t, x.shape)
-    for n, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        _flat(n, w, (like[3],))
+    if q is not None:
+        _flat("q_out", q_out, q.shape)
+    if k is not None:
+        _flat("k_out", k_out, k.shape)
+    _flat("q_weight", q_weight, like[3:])
+    _flat("k_weight", k_weight, like[3:])
     check(lib().mx_qk_norm_rotary_forward(C.byref(d), ptr(q), ptr(k), ptr(q_weight), ptr(k_weight), ptr(q_out), ptr(k_out),
                                           stream))
 
@@ -718,7 +721,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, positions, rotary, dq, dk, dq_
 def qk_norm_rotary_workspace(tokens, q_heads, k_heads, head_dim, rotary, eps) -> int:
     """Bytes that the backward's gradients of the weights take."""
     d = RotaryDesc(tokens, q_heads, k_heads, head_dim, rotary.rotary_dim, 0, 0, 0, 0, None,
-                   C.cast(rotary.frequencies, C.c_void_p), rotary.magnitude, 0.0 if eps is None else eps,
+                   rotary.address, rotary.magnitude, 0.0 if eps is None else eps,
                    int(rotary.interleaved), 0 if eps is None else 1)
     return _workspace_query(lib().mx_qk_norm_rotary_workspace, C.byref(d))
 
@@ -732,8 +735,9 @@ def _attention_desc(q, k, v, starts, sequences, window, sinks, scale):
             raise ValueError("attention: starts must name every sequence's first row and the end of the last")
         _flat("starts", starts, starts.shape, torch.int32)
         sequences = starts.numel() - 1
-    return AttentionDesc(q.shape[0], sequences, ptr(starts), q.shape[1], k.shape[1], q.shape[2], *qs, *ks, *vs, window, sinks,
-                         q.shape[2] ** -0.5 if scale is None else scale)
+    tokens, heads, dim = q.shape
+    return AttentionDesc(tokens, sequences, ptr(starts), heads, k.shape[1], dim, *qs, *ks, *vs, window, sinks,
+                         dim ** -0.5 if scale is None else scale)
 
 
 def attention_forward(q, k, v, out, starts=None, sequences=1, window=0, sinks=0, scale=None, lse=None, workspace=None,
@@ -790,7 +794,7 @@ class KVCache:
         _flat("KVCache: k_scale", k_scale, (pages, heads, page))
         _flat("KVCache: v_scale", v_scale, (pages, heads, page))
         self.tensors = (k, v, k_scale, v_scale)
-        self.heads, self.head_dim = heads, dim
+        self.row, self.head_dim = (heads, dim), dim
         self.desc = KVCacheDesc(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page, dim, KV_I8 if i8 else KV_F32)
 
 
@@ -812,16 +816,17 @@ class KVBatch:
 def kv_cache_write(cache, batch, k, v, stream=None) -> None:
     """Writes the batch's new tokens [tokens, heads, head_dim] to the cache."""
     ks, vs = _packed("k", k), _packed("v", v)
-    for n, t in (("k", k), ("v", v)):
-        if tuple(t.shape) != (batch.tokens, cache.heads, cache.head_dim):
-            raise ValueError(f"kv_cache_write: {n} {tuple(t.shape)} does not fit the batch and the cache")
+    if not k.shape == v.shape == (batch.tokens, *cache.row):
+        raise ValueError(f"kv_cache_write: k {tuple(k.shape)} and v {tuple(v.shape)} do not fit the batch and the cache: "
+                         f"{(batch.tokens, *cache.row)}")
     check(lib().mx_kv_cache_write(C.byref(cache.desc), C.byref(batch.desc), ptr(k), *ks, ptr(v), *vs, stream))
 
 
 def kv_cache_read(cache, batch, k, v, stream=None) -> None:
     """Reads them back into contiguous k and v."""
-    for n, t in (("k", k), ("v", v)):
-        _flat(n, t, (batch.tokens, cache.heads, cache.head_dim))
+    shape = (batch.tokens, *cache.row)
+    _flat("k", k, shape)
+    _flat("v", v, shape)
     check(lib().mx_kv_cache_read(C.byref(cache.desc), C.byref(batch.desc), ptr(k), ptr(v), stream))
 
 

@@ -219,7 +219,7 @@ def test_python_binding_checks_shapes(mx):
     with pytest.raises(ValueError, match="lengths"):
         mx.KVBatch(t(3, 2, dtype=torch.int32), t(2, dtype=torch.int32), 3)
     b = mx.KVBatch(t(3, 2, dtype=torch.int32), t(3, dtype=torch.int32), 3)
-    with pytest.raises(ValueError, match="does not fit"):
+    with pytest.raises(ValueError, match="do not fit"):
         mx.kv_cache_write(c, b, t(3, 1, 32), t(3, 2, 32))
     with pytest.raises(ValueError, match="does not fit"):
         mx.attention_paged(c, b, t(4, 2, 32), t(4, 2, 32))
