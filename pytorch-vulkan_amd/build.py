@@ -44,7 +44,7 @@ HIP_FLAGS = [
 MX_SOURCES = ["mx_runtime.hip", "mx_gemm.hip", "mx_conv.hip", "mx_conv_fwd.hip", "mx_conv_dx.hip", "mx_conv_dw.hip",
               "mx_winograd.hip", "mx_adamw.hip", "mx_util.hip", "mx_nn.hip", "mx_foreach.hip",
               "mx_layer_norm.hip", "mx_linear.hip", "mx_muon.hip", "mx_rotary.hip", "mx_attention.hip",
-              "mx_kv_cache.hip", "mx_attention_paged.hip"]
+              "mx_kv_cache.hip", "mx_attention_paged.hip", "mx_attention_chunk.hip"]
 EXT_SOURCES = ["backend.cpp", "ops_conv.cpp", "ops_gemm.cpp", "ops_adamw.cpp", "ops_plumbing.cpp", "ops_nn.cpp", "ops_foreach.cpp",
                "ops_block.cpp", "ops_attention.cpp"]
 

@@ -26,7 +26,6 @@
 // them is made NaN through the scores, which the mask keeps apart: by a NaN in the key's
 // other operand in the forward, by lse (the forward's, or its own) in the backward.
 #include "mx_attention.hpp"
-#include "mx_pieces.hpp"
 
 #include <algorithm>
 #include <cmath>
@@ -37,8 +36,6 @@ namespace {
 
 using namespace attn;
 
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-
 constexpr int kThreads = 256, kMaxDim = 128;
 
 struct Shape {
@@ -48,38 +45,11 @@ struct Shape {
   float scale;
 };
 
-struct Strided {
-  const float* at;
-  int64_t token, head;
-};
-
-// A packed tensor: [head][tile][step][piece][lane], DP / 16 steps; bytes of a tile, and where a
-// head's tile starts.
-template <int DP>
-constexpr int kTileBytes = DP / 16 * 3 * 1024;
+// Where a head's tile of a packed tensor [head][tile] starts.
 template <int DP>
 __device__ __forceinline__ int64_t tile_at(const Shape& s, int head, int tile) {
   return (int64_t(head) * s.tiles + tile) * kTileBytes<DP>;
 }
-// Lane l's place in a fragment: the halves' lines are exchanged in fours, so that a
-// transposing read's 16 lanes, 8 bytes of four rows from both halves, meet every bank once.
-__device__ __forceinline__ int slot(int lane) { return lane ^ (lane >> 5 << 2); }
-
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
-
-// Elements e .. e + 7 of a row, zero from `dim` on.
-__device__ __forceinline__ void load8(const float* row, int e, int dim, f32x4 (&v)[2]) {
-  v[0] = v[1] = f32x4{};
-  if (e + 8 <= dim) {
-    v[0] = *reinterpret_cast<const f32x4u*>(row + e);
-    v[1] = *reinterpret_cast<const f32x4u*>(row + e + 4);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (e + i < dim) v[i >> 2][i & 3] = row[e + i];
-  }
-}
-
 // ------------------------------------------------------------------ packing
 struct PackArgs {
   Shape s;
@@ -182,123 +152,12 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
   }
 }
 
-// ------------------------------------------------- tiles in LDS, and products
-__device__ __forceinline__ uint32_t lds_address(char* p) {
-  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)p));
-}
-
-// Two tensors' tiles (and 256 bytes of statistics) in LDS, two stages.
-template <int DP, int WAVES, bool STATS = false>
-struct Stages {
-  static constexpr int kBytes = 2 * kTileBytes<DP> + (STATS ? 1024 : 0);
-  static constexpr int kSecond = kTileBytes<DP>, kStats = 2 * kTileBytes<DP>;
-  uint32_t lds;
-  __device__ __forceinline__ void load(int stage, const char* a, const char* b, const char* stats, int wave, int lane) const {
-    const uint32_t to = lds + stage * kBytes;
-    const char *const pa = pieces::uniform(a), *const pb = pieces::uniform(b);
-    constexpr int F = DP / 16 * 3;
-#pragma unroll
-    for (int i = 0; i < (2 * F + WAVES - 1) / WAVES; ++i) {
-      const int f = wave + WAVES * i;  // a's fragments, then b's
-      if (2 * F % WAVES == 0 || f < 2 * F) pieces::load_lds16(f < F ? pa + f * 1024 : pb + (f - F) * 1024, lane * 16, to + f * 1024);
-    }
-    if constexpr (STATS)
-      if (wave == 0) load_lds4(pieces::uniform(stats), lane * 4, to + kStats);
-  }
-  // 4 bytes a lane from memory to LDS (as pieces::load_lds16).
-  static __device__ __forceinline__ void load_lds4(const char* base, uint32_t lane_off, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(at), "v"(lane_off), "s"(base) : "memory");
-  }
-};
-
-__device__ __forceinline__ Frag3 frag(uint32_t tile, int step, int lane) {
-  const uint32_t at = tile + step * 3072 + slot(lane) * 16;
-  return {*pieces::lds_at<const bf16x8>(at), *pieces::lds_at<const bf16x8>(at + 1024), *pieces::lds_at<const bf16x8>(at + 2048)};
-}
-
-// Rows 16 h + 8 t + 0 .. 7 (h: the lane's half) of element 32 b + l % 32, by transposing reads: 16
-// lanes name 4 elements of one of 4 rows each, and get 4 rows of one element.
-__device__ __forceinline__ uint32_t column_base(int lane) {
-  const int c = lane & 15, g = lane >> 4 & 1, h = lane >> 5, other = c >> 1 & 1;
-  return uint32_t(g * 3072 + other * 512 + (((h ^ other) << 2) + (c >> 2)) * 16 + (c & 1) * 8);
-}
-__device__ __forceinline__ Frag3 frag_columns(uint32_t tile_and_base, int b, int t) {
-  bf16x8 f[3];
-#pragma unroll
-  for (int p = 0; p < 3; ++p) {
-    mfma::s16x4 q[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      q[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          pieces::lds_at<mfma::s16x4>(tile_and_base + b * 6144 + p * 1024 + (2 * t + i) * 128));
-    f[p] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7));
-  }
-  return {f[0], f[1], f[2]};
-}
-
-// Exponents of scores that are not seen (a NaN among them) have no probability.  The branch is the same for a wave; the
-// barrier keeps the compiler from comparing in every tile, seen as a whole or not.
-template <class F>
-__device__ __forceinline__ void hide(f32x16& x, F&& sees) {
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int r = 0; r < 16; ++r)
-    if (!sees(r)) x[r] = -__builtin_inff();
-}
-// a b along the head's elements: a's tile in LDS, b's fragments in registers.
-template <int DP>
-__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane) {
-  f32x16 acc{};
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const Frag3 f = frag(a, s, lane);
-    acc = mma_large(f, b[s], mma_small(f, b[s], acc));
-  }
-  return acc;
-}
-
-// Block b of a p along the tile's rows: a's tile in LDS (and the lane's column_base), p's pieces.
-__device__ __forceinline__ f32x16 product_rows(uint32_t a, int b, const Frag3 (&p)[2]) {
-  f32x16 acc{};
-  const Frag3 f0 = frag_columns(a, b, 0), f1 = frag_columns(a, b, 1);
-  acc = mma_small(f0, p[0], acc);
-  acc = mma_small(f1, p[1], acc);
-  acc = mma_large(f0, p[0], acc);
-  return mma_large(f1, p[1], acc);
-}
-
-// Own rows as fragments in registers, straight from memory.
-template <int DP>
-__device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const Strided& t, int head, int64_t row, bool live, int dim, int h,
-                                         float scale) {
-  const float* const at = t.at + row * t.token + head * t.head;
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    f32x4 v[2] = {};
-    if (live) load8(at, s * 16 + h * 8, dim, v);
-    f[s] = split8(v[0] * scale, v[1] * scale);
-  }
-}
-// The same from a packed tile.
+// Own rows from a packed tile.
 template <int DP>
 __device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const char* tile, int lane) {
   const bf16x8* const at = reinterpret_cast<const bf16x8*>(tile) + slot(lane);
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) f[s] = {at[s * 192], at[s * 192 + 64], at[s * 192 + 128]};
-}
-
-// Stores a lane's 16 elements of block b of one row: 8 k + 4 h + 0 .. 3.
-__device__ __forceinline__ void store_block(float* row, const f32x16& v, int b, int h, int dim) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int e = b * 32 + 8 * k + 4 * h;
-    const f32x4 four{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
-    if (e + 4 <= dim) *reinterpret_cast<f32x4u*>(row + e) = four;
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (e + i < dim) row[e + i] = four[i];
-  }
 }
 
 // Blocks of 128 rows, four tiles of one sequence; the workgroups' order puts what has the most
@@ -313,11 +172,15 @@ struct FwdArgs {
   float *out, *lse;
 };
 
+// Steps whose queries' smallest piece waits in LDS, where two waves a SIMD have no registers for it.
+constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0; }
+
 template <int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP > 96 ? 1 : 2))) void fwd_kernel(const FwdArgs a) {
-  using St = Stages<DP, WAVES>;
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 8 || DP <= 96 ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
+  using St = Stages<DP, 3, WAVES, 0>;
   constexpr int kRows = WAVES * kTile;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
+  constexpr int kAside = aside(DP, WAVES);
+  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes + kAside * WAVES * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
@@ -334,6 +197,10 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP >
   fetch(0);
   Frag3 q[DP / 16];
   own_rows<DP>(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
+  bf16x8* const mine = reinterpret_cast<bf16x8*>(smem + 2 * St::kBytes) + wave * kAside * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < kAside; ++i) mine[i * 64] = q[i].lo;
+  const auto low = [&](int i) { return i < kAside ? mine[i * 64] : q[i].lo; };
   f32x16 o[DP / 32] = {};
   float m = -__builtin_inff(), l = 0;  // of the exponents
   const uint32_t columns = column_base(lane);
@@ -344,7 +211,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP >
     const int j0 = keys.tile(n) * kTile;
     if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
-    f32x16 x = product<DP>(tile, q, lane);
+    f32x16 x = product<DP, 3>(tile, q, lane, low);
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
     float top = x[0];
 #pragma unroll
@@ -364,7 +231,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(DP >
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
       if (DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
-      o[b] = o[b] * keep + product_rows(tile + St::kSecond + columns, b, p);
+      o[b] = o[b] * keep + product_columns(tile + St::kSecond + columns, b, p);
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -388,7 +255,7 @@ struct BwdArgs {
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
-  using St = Stages<DP, 4>;
+  using St = Stages<DP, 3, 4, 0>;
   __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -421,14 +288,14 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     const int j0 = keys.tile(n) * kTile;
     if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
-    f32x16 x = product<DP>(tile, q, lane) - lse;
+    f32x16 x = product<DP, 3>(tile, q, lane) - lse;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
-    const f32x16 dp = product<DP>(tile + St::kSecond, g, lane);
+    const f32x16 dp = product<DP, 3>(tile + St::kSecond, g, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dq[b] += product_rows(tile + columns, b, p);
+    for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(tile + columns, b, p);
   }
   if (qi >= t.len) return;
 #pragma unroll
@@ -438,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
-  using St = Stages<DP, 4, true>;
+  using St = Stages<DP, 3, 4, 1>;
   __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -471,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
     const int i0 = (from + n % tiles) * kTile;
     if (s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
-    f32x16 x = product<DP>(tile, k, lane), delta;
+    f32x16 x = product<DP, 3>(tile, k, lane), delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t at = tile + St::kStats + (16 * h + 4 * i) * 4;
@@ -480,7 +347,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
       for (int e = 0; e < 4; ++e) x[4 * i + e] -= lse[e], delta[4 * i + e] = d[e];
     }
     if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) hide(x, [&](int r) { return s.mask.sees(i0 + 16 * h + r, kj); });
-    f32x16 dp = product<DP>(tile + St::kSecond, v, lane);
+    f32x16 dp = product<DP, 3>(tile + St::kSecond, v, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = exp2_(x[r]);
@@ -489,8 +356,8 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)}, ds[2] = {split_half(dp, 0), split_half(dp, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
-      dv[b] += product_rows(tile + St::kSecond + columns, b, p);
-      dk[b] += product_rows(tile + columns, b, ds);
+      dv[b] += product_columns(tile + St::kSecond + columns, b, p);
+      dk[b] += product_columns(tile + columns, b, ds);
     }
   }
   if (kj >= t.len) return;
@@ -597,8 +464,6 @@ Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
   return b;
 }
 
-constexpr int fwd_waves(int dp) { return dp > 96 ? 4 : 8; }
-
 int64_t blocks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kBlock); }
 
 // Parts that a key head's query heads are dealt into: as few as give every CU four
@@ -665,9 +530,13 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   });
   MX_LAUNCHED();
   with_dim(s.dim, [&](auto dp) {
-    constexpr int W = fwd_waves(decltype(dp)::value);
-    const int64_t blocks = sequence_tiles(s.seqs.tokens, s.seqs.count, W * kTile);
-    hipLaunchKernelGGL((fwd_kernel<decltype(dp)::value, W>), dim3(unsigned(blocks * s.heads)), dim3(64 * W), 0, st, f);
+    constexpr int DP = decltype(dp)::value;
+    const int64_t wide = sequence_tiles(s.seqs.tokens, s.seqs.count, 8 * kTile) * s.heads;
+      if (wide_blocks(wide)) {
+        hipLaunchKernelGGL((fwd_kernel<DP, 8>), dim3(unsigned(wide)), dim3(512), 0, st, f);
+        return;
+      }
+    hipLaunchKernelGGL((fwd_kernel<DP, 4>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
   });
   MX_LAUNCHED();
   return MX_OK;

@@ -21,8 +21,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "mx_attention.hpp"
-#include "mx_kv_cache.hpp"
+#include "mx_attention_paged.hpp"
 
 namespace mx {
 namespace {
@@ -30,73 +29,18 @@ namespace {
 using namespace attn;
 using kv::Batch;
 using kv::Cache;
-using mfma::bf16x2;
-using mfma::f32x2;
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = 4, kRows = 16, kKeys = 64;
 
-struct PagedArgs {
-  Cache c;
-  Batch b;
-  const float* q;
-  int64_t q_token, q_head;
-  int heads, group, tiles, splits, span;  // span: tiles of keys to a workgroup
-  Mask mask;
-  float scale;
-  float *out, *part;
+struct PagedArgs : Paged {
+  int tiles, splits, span;  // span: tiles of keys to a workgroup
+  float* part;
 };
 
 // The workgroups' parts: [row tile][kv head][split] of 16 maxima, 16 sums and 16 rows of dim.
 __device__ __forceinline__ int64_t part_at(const PagedArgs& a, int tile, int head, int split) {
   return ((int64_t(tile) * a.c.heads + head) * a.splits + split) * (kRows * (2 + a.c.dim));
 }
-
-// What a row tile sees: its sequence's tokens, positions and tiles of keys.
-struct RowTile {
-  SequenceTile t;
-  int length, first, i0, i1;  // tokens of the sequence, its first new one, the tile's positions
-  __device__ __forceinline__ bool find(const PagedArgs& a, int tile) {
-    if (!locate<kRows>(a.b.seqs, tile, t) || t.index * kRows >= t.len) return false;
-    const int last = a.b.lengths[t.seq];
-    length = int(min(int64_t(max(last, 0)), int64_t(a.b.width) * a.c.page_size));
-    first = last - t.len / a.group;
-    i0 = first + t.index * kRows / a.group;
-    i1 = min(first + (min(t.len, (t.index + 1) * kRows) - 1) / a.group, length - 1);
-    return true;
-  }
-};
-
-// 16 elements as operand pieces: one where they are bytes, three where they are FP32.
-template <bool I8>
-struct Sixteen;
-template <>
-struct Sixteen<true> {
-  i32x4 raw;
-  __device__ __forceinline__ void load(const void* p) { raw = *static_cast<const i32x4*>(p); }
-  // Elements 8 t .. 8 t + 7.
-  __device__ __forceinline__ bf16x8 half(int t) const {
-    mfma::u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int x = raw[2 * t + i];
-      w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{float(int8_t(x)), float(int8_t(x >> 8))}), bf16x2));
-      w[2 * i + 1] =
-          __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{float(int8_t(x >> 16)), float(x >> 24)}), bf16x2));
-    }
-    return __builtin_bit_cast(bf16x8, w);
-  }
-};
-template <>
-struct Sixteen<false> {
-  f32x4 raw[4];
-  __device__ __forceinline__ void load(const void* p) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = static_cast<const f32x4*>(p)[i];
-  }
-  __device__ __forceinline__ Frag3 half(int t) const { return split8(raw[2 * t], raw[2 * t + 1]); }
-};
 
 __device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -134,7 +78,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
   const Cache& c = a.c;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
   const int kv_head = blockIdx.y;
-  RowTile rt;
+  RowTile<kRows> rt;
   if (!rt.find(a, blockIdx.x)) return;
   const SequenceTile& t = rt.t;
   const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.i1);
@@ -318,7 +262,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
 constexpr int kMaxSplits = 64;
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedArgs a) {
   __shared__ float weight[kRows][kMaxSplits];
-  RowTile rt;
+  RowTile<kRows> rt;
   if (!rt.find(a, blockIdx.x)) return;
   const SequenceTile& t = rt.t;
   const int r = threadIdx.x >> 4, cc = threadIdx.x & 15, row = t.index * kRows + r, kv_head = blockIdx.y;
@@ -396,6 +340,7 @@ Split split_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* 
 
 int64_t paged_workspace(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
   if (b->tokens == 0 || d->heads == 0) return 0;
+  if (const int64_t chunk = chunk_workspace(d, c, b)) return chunk;
   const int64_t splits = split_of(d, c, b).splits;
   return splits == 1 ? 0 : row_tiles(d, c, b) * c->heads * splits * kRows * (2 + c->head_dim) * 4;
 }
@@ -437,13 +382,14 @@ extern "C" int mx_attention_paged(const mx_paged_desc* d, const mx_kv_cache* c, 
   a.b = kv::batch_of(b);
   a.heads = int(d->heads), a.group = int(d->heads / c->heads);
   a.b.seqs.per = a.group;
-  a.q = q, a.q_token = d->q_token, a.q_head = d->q_head;
+  a.out = out, a.q = q, a.q_token = d->q_token, a.q_head = d->q_head;
+  a.mask = {int(std::min<int64_t>(d->window, 1 << 30)), int(std::min<int64_t>(d->sinks, 1 << 30))};
+  a.scale = float(d->scale);
+  if (chunk_workspace(d, c, b)) return chunk_attention(a, d, c, b, ws.as<char>(), s);
   a.tiles = int(row_tiles(d, c, b));
   const Split split = split_of(d, c, b);
   a.splits = split.splits, a.span = split.span;
-  a.mask = {int(std::min<int64_t>(d->window, 1 << 30)), int(std::min<int64_t>(d->sinks, 1 << 30))};
-  a.scale = float(d->scale);
-  a.out = out, a.part = ws.as<float>();
+  a.part = ws.as<float>();
   const dim3 grid(unsigned(a.tiles), unsigned(a.c.heads), unsigned(a.splits));
   if (a.c.dim <= 64) launch<64>(a, c->type, grid, s);
   else launch<128>(a, c->type, grid, s);
