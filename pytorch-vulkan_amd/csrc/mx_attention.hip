@@ -251,7 +251,23 @@ struct BwdArgs {
   float *dq, *dk, *dv;
   int parts;            // of a key head's query heads
   float *dk_p, *dv_p;  // [part][token][key head][dim] where there are several
+  int near, far_blocks;  // workgroups' blocks of keys, and of those that are seen past the window
+  float* far;            // [chunk][block][key head][part][dk, dv][128][dim]
 };
+
+// First tokens that stay visible are seen by every later query, other keys by a window's.
+// So that their workgroup is not the last by far, the queries past the window of its block are
+// dealt to workgroups of their own, chunks of 1024 rows of a sequence, whose sums far_kernel
+// adds in order (8 sequences of up to 2048, window 512, 4 first tokens, 12 heads of 80: dk and dv
+// TODO us).
+constexpr int kChunk = 1024;
+__device__ __forceinline__ float* far_at(const BwdArgs& a, int chunk, int block, int kv_head, int part) {
+  return a.far + (((int64_t(chunk) * a.far_blocks + block) * a.s.kv_heads + kv_head) * a.parts + part) * (2 * kBlock * a.s.dim);
+}
+// The last row whose window reaches a key of the block at b0.
+__device__ __forceinline__ int near_last(const Mask& m, int b0, int len) {
+  return m.window ? min(len - 1, b0 + kBlock - 1 + min(m.window, len) - 1) : len - 1;
+}
 
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
@@ -304,20 +320,31 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
 }
 
 template <int DP>
-__global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
   using St = Stages<DP, 3, 4, 1>;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
+  constexpr int kAside = DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
+  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes + kAside * 4 * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int across = s.kv_heads * a.parts, kv_head = blockIdx.x % across / a.parts, part = blockIdx.x % across % a.parts;
+  const int block = blockIdx.x / across;
+  const bool far = block >= a.near;
+  const int chunk = far ? (block - a.near) / a.far_blocks : 0, far_block = far ? (block - a.near) % a.far_blocks : 0;
   SequenceTile t;
-  if (!locate<kBlock>(s.seqs, blockIdx.x / across, t) || t.index * kBlock >= t.len) return;
+  if (far ? !locate<kChunk>(s.seqs, chunk, t) : !locate<kBlock>(s.seqs, block, t)) return;
+  const int b0 = far ? far_block * kBlock : t.index * kBlock;
+  if (b0 >= t.len) return;
   const int base32 = t.start / kTile + t.seq;
-  const int b0 = t.index * kBlock, j0 = b0 + wave * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
+  const int j0 = b0 + wave * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
   const St st{lds_address(smem)};
   // The tiles of queries that see any of the workgroup's keys, of each head in turn.
-  const int last = s.mask.window && b0 >= s.mask.sinks ? min(t.len - 1, b0 + kBlock - 1 + min(s.mask.window, t.len) - 1) : t.len - 1;
-  const int from = b0 / kTile, tiles = last / kTile + 1 - from;
+  int from = b0 / kTile, to = near_last(s.mask, b0, t.len) / kTile;
+  if (far) {
+    from = max(to + 1, t.index * (kChunk / kTile));
+    to = min(t.len - 1, (t.index + 1) * kChunk - 1) / kTile;
+  }
+  const int tiles = to + 1 - from;
+  if (tiles <= 0) return;
   const int heads = s.group / a.parts, head0 = kv_head * s.group + part * heads, count = heads * tiles;
   const auto fetch = [&](int n) {
     const int head = head0 + n / tiles, tile = base32 + from + n % tiles;
@@ -329,6 +356,10 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
   Frag3 k[DP / 16], v[DP / 16];
   own_rows<DP>(k, a.kp + mine, lane);
   own_rows<DP>(v, a.vp + mine, lane);
+  bf16x8* const aside_at = reinterpret_cast<bf16x8*>(smem + 2 * St::kBytes) + wave * kAside * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < kAside; ++i) aside_at[i * 64] = v[i].lo;
+  const auto low = [&](int i) { return i < kAside ? aside_at[i * 64] : v[i].lo; };
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const uint32_t columns = column_base(lane);
   for (int n = 0; n < count; ++n) {
@@ -347,30 +378,62 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const BwdArgs a) {
       for (int e = 0; e < 4; ++e) x[4 * i + e] -= lse[e], delta[4 * i + e] = d[e];
     }
     if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) hide(x, [&](int r) { return s.mask.sees(i0 + 16 * h + r, kj); });
-    f32x16 dp = product<DP, 3>(tile + St::kSecond, v, lane);
+    f32x16 dp = product<DP, 3>(tile + St::kSecond, v, lane, low);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = exp2_(x[r]);
       dp[r] = times(x[r], dp[r] - delta[r]);
     }
-    const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)}, ds[2] = {split_half(dp, 0), split_half(dp, 1)};
+    {
+      const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) {
-      dv[b] += product_columns(tile + St::kSecond + columns, b, p);
-      dk[b] += product_columns(tile + columns, b, ds);
+      for (int b = 0; b < DP / 32; ++b) dv[b] += product_columns(tile + St::kSecond + columns, b, p);
     }
+    const Frag3 ds[2] = {split_half(dp, 0), split_half(dp, 1)};
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(tile + columns, b, ds);
   }
-  if (kj >= t.len) return;
-  const int64_t at = ((int64_t(t.start) + kj) * s.kv_heads + kv_head) * s.dim;
-  const int64_t whole = a.parts > 1 ? int64_t(part) * s.seqs.tokens * s.kv_heads * s.dim : 0;
-  float* const to_k = a.parts > 1 ? a.dk_p : a.dk;
-  float* const to_v = a.parts > 1 ? a.dv_p : a.dv;
+  if (kj >= t.len || (far && j0 >= s.mask.sinks)) return;
+  float *to_k = a.dk, *to_v = a.dv;
+  int64_t at = ((int64_t(t.start) + kj) * s.kv_heads + kv_head) * s.dim;
+  if (far) {
+    to_k = far_at(a, chunk, far_block, kv_head, part), to_v = to_k + kBlock * s.dim;
+    at = int64_t(kj - b0) * s.dim;
+  } else if (a.parts > 1) {
+    to_k = a.dk_p, to_v = a.dv_p;
+    at += int64_t(part) * s.seqs.tokens * s.kv_heads * s.dim;
+  }
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) {
     // q was packed times scale log2(e)
-    if (a.dk) store_block(to_k + whole + at, dk[b] * kLn2, b, h, s.dim);
-    if (a.dv) store_block(to_v + whole + at, dv[b], b, h, s.dim);
+    if (a.dk) store_block(to_k + at, dk[b] * kLn2, b, h, s.dim);
+    if (a.dv) store_block(to_v + at, dv[b], b, h, s.dim);
   }
+}
+
+// What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of 128
+// keys times workgroups of a block, key heads, sequences).
+__global__ __launch_bounds__(kThreads) void far_kernel(const BwdArgs a) {
+  const Shape& s = a.s;
+  const int per = gridDim.x / a.far_blocks, block = blockIdx.x / per, b0 = block * kBlock;
+  const int start = s.seqs.start(blockIdx.z), len = max(0, s.seqs.start(blockIdx.z + 1) - start);
+  if (b0 >= len) return;
+  const int from = (near_last(s.mask, b0, len) / kTile + 1) * kTile / kChunk, to = (len - 1) / kChunk;
+  if (near_last(s.mask, b0, len) / kTile == (len - 1) / kTile) return;  // no queries past the window
+  const int rows = min(min(kBlock, len - b0), (s.mask.sinks - b0 + kTile - 1) / kTile * kTile), base = start / kChunk + blockIdx.z;
+  const int i = (blockIdx.x - block * per) * kThreads + threadIdx.x;
+  if (i >= rows * s.dim) return;
+  const int64_t at = ((int64_t(start) + b0 + i / s.dim) * s.kv_heads + blockIdx.y) * s.dim + i % s.dim;
+  float k = a.dk ? a.dk[at] : 0.f, v = a.dv ? a.dv[at] : 0.f;
+  for (int c = from; c <= to; ++c)
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) {
+      const float* const sum = far_at(a, base + c, block, blockIdx.y, p) + i;
+      if (a.dk) k += sum[0];
+      if (a.dv) v += sum[kBlock * s.dim];
+    }
+  if (a.dk) a.dk[at] = k;
+  if (a.dv) a.dv[at] = v;
 }
 
 // dk and dv: the parts' sums, in order, over the rows from the first sequence's start to the
@@ -445,8 +508,15 @@ struct Carve {
 
 struct Buffers {
   char *qp, *kp, *vp, *dp;
-  float *stats, *dk_p, *dv_p;
+  float *stats, *dk_p, *dv_p, *far;
 };
+
+// Blocks of keys that are seen past the window, and chunks of queries.
+int64_t far_blocks_of(const Shape& s) {
+  return s.mask.window && s.mask.window < s.seqs.tokens ? (std::min(s.mask.sinks, s.seqs.tokens) + int64_t(kBlock) - 1) / kBlock : 0;
+}
+int64_t chunks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kChunk); }
+
 Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
   const int64_t tile = padded(s.dim) / 16 * 3 * 1024, q = tile * s.tiles * s.heads, k = tile * s.tiles * s.kv_heads;
   Buffers b{};
@@ -461,6 +531,7 @@ Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
     b.dk_p = c.take<float>(part);
     b.dv_p = c.take<float>(part);
   }
+  b.far = c.take<float>(chunks_of(s) * far_blocks_of(s) * s.kv_heads * parts * (2 * kBlock * int64_t(s.dim) * 4));
   return b;
 }
 
@@ -565,7 +636,7 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   p.dout = {dout, d->heads * d->head_dim, d->head_dim}, p.out = {out, d->heads * d->head_dim, d->head_dim};
   p.lse = lse;
   p.qp = b.qp, p.kp = b.kp, p.vp = b.vp, p.dp = b.dp, p.stats = b.stats;
-  const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p};
+  const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p, int(blocks_of(s)), int(far_blocks_of(s)), b.far};
   with_dim(s.dim, [&](auto dp) {
     hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
   });
@@ -578,14 +649,21 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   }
   if (dk || dv) {
     with_dim(s.dim, [&](auto dp) {
-      hipLaunchKernelGGL((dkv_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.kv_heads * parts)), dim3(kThreads),
-                         0, st, g);
+      const int64_t blocks = blocks_of(s) + chunks_of(s) * far_blocks_of(s);
+      hipLaunchKernelGGL((dkv_kernel<decltype(dp)::value>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
     if (parts > 1) {
       const int64_t fours = (d->tokens * d->kv_heads * d->head_dim + 3) / 4;
       const unsigned blocks = unsigned(std::min<int64_t>((fours + kThreads - 1) / kThreads, int64_t(cu_count()) * 8));
       hipLaunchKernelGGL(join_kernel, dim3(blocks, 2), dim3(kThreads), 0, st, g);
+      MX_LAUNCHED();
+    }
+    if (g.far_blocks) {
+      const int rows = std::min(kBlock, (std::min(s.mask.sinks, kBlock) + kTile - 1) / kTile * kTile);
+      const unsigned per = unsigned((rows * s.dim + kThreads - 1) / kThreads);
+      hipLaunchKernelGGL(far_kernel, dim3(unsigned(g.far_blocks) * per, unsigned(s.kv_heads), unsigned(s.seqs.count)),
+                         dim3(kThreads), 0, st, g);
       MX_LAUNCHED();
     }
   }

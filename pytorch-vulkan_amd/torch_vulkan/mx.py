@@ -765,8 +765,8 @@ def attention_backward(dout, q, k, v, out, lse, dq, dk, dv, starts=None, sequenc
                                       ptr(dv), ptr(workspace), _bytes(workspace), stream))
 
 
-def attention_workspace(tokens, sequences, heads, kv_heads, head_dim, backward=False) -> int:
-    d = AttentionDesc(tokens, sequences, _ANY_ADDRESS, heads, kv_heads, head_dim, 0, 0, 0, 0, 0, 0, 0, 0, 1.0)
+def attention_workspace(tokens, sequences, heads, kv_heads, head_dim, backward=False, window=0, sinks=0) -> int:
+    d = AttentionDesc(tokens, sequences, _ANY_ADDRESS, heads, kv_heads, head_dim, 0, 0, 0, 0, 0, 0, window, sinks, 1.0)
     return _workspace_query(lib().mx_attention_workspace, C.byref(d), 1 if backward else 0)
 
 

@@ -244,7 +244,11 @@ ATTENTION = [
     ([63, 0, 65], 2, 1, 20, 0, 0), ([64], 4, 2, 64, 7, 0), ([127], 2, 1, 80, 1, 0), ([128], 2, 2, 96, 32, 3),
     ([129, 1, 1, 200], 6, 2, 128, 64, 1), ([300], 3, 1, 65, 33, 40), ([257], 8, 1, 64, 100, 4), ([5, 700], 2, 2, 128, 0, 0),
     ([513], 4, 4, 48, 512, 600), ([0, 0, 40, 0], 2, 1, 128, 16, 2), ([1000], 2, 1, 128, 130, 70),
-    ([1] * 70, 1, 1, 8, 0, 0), ([3, 30, 300] * 30, 2, 1, 32, 20, 5), ([2049], 1, 1, 64, 0, 0), ([640], 12, 3, 80, 128, 4)]
+    ([1] * 70, 1, 1, 8, 0, 0), ([3, 30, 300] * 30, 2, 1, 32, 20, 5), ([2049], 1, 1, 64, 0, 0), ([640], 12, 3, 80, 128, 4),
+    # first tokens seen from past the window: several chunks of queries, several blocks of keys
+    ([2500, 31, 1100], 4, 2, 64, 40, 4), ([3100], 2, 1, 96, 200, 150), ([70, 1025, 400], 6, 2, 128, 1, 33), ([900, 900], 8, 1, 40, 600, 129),
+    # enough rows for workgroups of eight waves
+    ([2600, 1500], 64, 32, 32, 0, 0), ([4200], 64, 2, 128, 300, 2)]
 
 
 @pytest.mark.parametrize("lengths,h,kv,d,window,sinks", ATTENTION)
@@ -414,7 +418,7 @@ def test_attention_captured(mx):
     t = sum(n)
     q, k, v, do = rand(g, t, h, d), rand(g, t, kv, d), rand(g, t, kv, d), rand(g, t, h, d)
     out, lse, dq, dk, dv = torch.empty_like(q), q.new_empty(h, t), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    ws = torch.empty(max(mx.attention_workspace(t, 2, h, kv, d), mx.attention_workspace(t, 2, h, kv, d, True)),
+    ws = torch.empty(max(mx.attention_workspace(t, 2, h, kv, d), mx.attention_workspace(t, 2, h, kv, d, True, window=30, sinks=2)),
                      dtype=torch.uint8, device="cuda")
     starts = starts_of(n)
 
@@ -607,7 +611,11 @@ def paged_ref(q, k, v, pos, seen, scale):
 PAGED = [([1], [1], 16, 1, 1, 16, 0, 0), ([1], [33], 16, 4, 1, 32, 0, 0), ([1, 1], [500, 7], 64, 8, 2, 128, 0, 0),
          ([5], [5], 16, 2, 2, 80, 0, 0), ([40, 3], [100, 3], 32, 6, 2, 64, 0, 0), ([1] * 9, [60 * i + 1 for i in range(9)], 48, 3, 3, 96, 0, 0),
          ([1], [3000], 64, 16, 1, 128, 0, 0), ([2, 0, 1], [900, 4, 333], 16, 12, 4, 48, 100, 5), ([130], [700], 64, 4, 2, 112, 64, 40),
-         ([70], [70], 16, 33, 1, 16, 1, 0), ([1, 30], [5000, 4000], 128, 2, 1, 64, 1000, 16), ([257], [2000], 32, 5, 5, 32, 0, 0)]
+         ([70], [70], 16, 33, 1, 16, 1, 0), ([1, 30], [5000, 4000], 128, 2, 1, 64, 1000, 16), ([257], [2000], 32, 5, 5, 32, 0, 0),
+         # chunks of many rows: packed tiles, keys of a row shared by workgroups, eight waves where there are rows enough
+         ([400], [1100], 64, 8, 2, 128, 0, 0), ([330, 0, 350], [400, 90, 350], 16, 6, 2, 96, 100, 5), ([200, 210], [900, 210], 32, 16, 2, 48, 64, 40),
+         ([900], [950], 128, 4, 4, 32, 0, 0), ([900] * 5, [901 + 13 * i for i in range(5)], 48, 60, 10, 64, 70, 2),
+         ([1] * 3 + [2500], [5, 600, 1, 2600], 16, 3, 1, 80, 33, 1)]
 
 
 def fill(mx, g, cache, table, lengths, page, kv, d, kind):
