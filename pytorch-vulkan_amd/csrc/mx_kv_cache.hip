@@ -21,27 +21,39 @@ using kv::Cache;
 
 constexpr int kThreads = 256, kGroup = 16, kMaxDim = 128;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <class E>
+struct alignas(4 * sizeof(E)) Four {
+  E e[4];
+};
+
 struct Rows {  // one of k and v, outside the cache
   float* at;
   int64_t token, head;
 };
 
-// x / scale rounded half to even: of the exact quotient, whose FP32 rounding could
-// land on a half step.  n + 1/2 times the scale has at most 32 bits, so the fused
-// multiply-add has the sign of x's distance from it (which FP32's least numbers would
-// round away: small rows are lifted first).
-__device__ __forceinline__ int steps(float x, float scale) {
-  if (!(scale > 0)) return 0;
-  if (scale < 0x1p-60f) x *= 0x1p90f, scale *= 0x1p90f;
-  float n = rintf(x / scale);
-  if (fabsf(n) <= 127.f) {
-    const float up = fmaf(-(n + 0.5f), scale, x), down = fmaf(-(n - 0.5f), scale, x);
-    const bool odd = int(n) & 1;
-    if (up > 0 || (up == 0 && odd)) n += 1;
-    else if (down < 0 || (down == 0 && odd)) n -= 1;
+// x / scale rounded half to even, of the exact quotient: a product with the reciprocal is off
+// by a step at most, and what it leaves of x is exact (a fused multiply-add; FP32's least numbers
+// would round it away: small rows are lifted first).
+struct Steps {
+  float lift, scale, half, inv;
+  __device__ __forceinline__ explicit Steps(float s) {
+    lift = s < 0x1p-60f ? 0x1p90f : 1.f;
+    scale = s * lift;
+    half = s > 0 ? 0.5f * scale : __builtin_inff();
+    inv = s > 0 ? 1.f / scale : 0.f;  // (rows of a scale of 0 or NaN: no steps)
   }
-  return int(fminf(fmaxf(n, -127.f), 127.f));
-}
+  __device__ __forceinline__ int operator()(float x) const {
+    x *= lift;
+    float n = rintf(x * inv);
+    const float rest = fmaf(-n, scale, x);
+    const bool odd = int(n) & 1;
+    if (rest > half || (rest == half && odd)) n += 1;
+    if (rest < -half || (rest == -half && odd)) n -= 1;
+    return int(fminf(fmaxf(n, -127.f), 127.f));
+  }
+};
 
 template <int L>
 __device__ __forceinline__ float lanes_max(float v) {
@@ -73,39 +85,53 @@ __device__ __forceinline__ bool places(const Cache& c, const Batch& b, int tile,
 template <bool I8>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const Cache c, const Batch b, const Rows k, const Rows v) {
   using E = std::conditional_t<I8, int8_t, float>;
-  __shared__ E cols[kMaxDim][kGroup + (I8 ? 0 : 1)];
+  __shared__ __attribute__((aligned(16))) E held[kGroup][kMaxDim + 4];  // values by row (the pitch keeps banks apart)
   Places g;
   if (!places(c, b, blockIdx.x, g) || g.page < 0) return;
   const int head = blockIdx.y, row = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const bool mine = row >= g.lo && row < g.hi;
   const int64_t at = (int64_t(g.page) * c.heads + head) * c.page_size + g.place;  // place 0's row in the cache
+  // A row's 16 lanes have every sixteenth four of its elements.
+  constexpr int N = kMaxDim / 64;
+  f32x4 val[2][N];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const Rows& src = which ? v : k;
     const float* const x = src.at + (g.row + row) * src.token + head * src.head;
-    float val[kMaxDim / 16];
-    float most = 0, bad = 0;
 #pragma unroll
-    for (int i = 0; i < kMaxDim / 16; ++i) {
-      val[i] = mine && i * 16 < c.dim ? x[i * 16 + lane] : 0.f;
-      most = fmaxf(most, fabsf(val[i]));
-      bad = fmaxf(bad, fabsf(val[i]) <= 3.402823466e38f ? 0.f : 1.f);
+    for (int i = 0; i < N; ++i) {
+      const int d = (i * 16 + lane) * 4;
+      val[which][i] = mine && d < c.dim ? *reinterpret_cast<const f32x4u*>(x + d) : f32x4{};
     }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
     float scale = 0;
     if constexpr (I8) {
+      float most = 0, bad = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          most = fmaxf(most, fabsf(val[which][i][j]));
+          bad = fmaxf(bad, fabsf(val[which][i][j]) <= 3.402823466e38f ? 0.f : 1.f);
+        }
       scale = lanes_max<16>(most) / 127.f;
       if (lanes_max<16>(bad) > 0) scale = __builtin_nanf("");
       if (mine && lane == 0) (which ? c.vs : c.ks)[at + row] = scale;
     }
+    const Steps steps(scale);
 #pragma unroll
-    for (int i = 0; i < kMaxDim / 16; ++i) {
-      if (i * 16 >= c.dim || !mine) continue;
-      const int d = i * 16 + lane;
-      E e;
-      if constexpr (I8) e = E(steps(val[i], scale));
-      else e = val[i];
-      if (which) cols[d][row] = e;
-      else static_cast<E*>(c.k)[(at + row) * c.dim + d] = e;
+    for (int i = 0; i < N; ++i) {
+      const int d = (i * 16 + lane) * 4;
+      if (d >= c.dim || !mine) continue;
+      Four<E> e;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (I8) e.e[j] = E(steps(val[which][i][j]));
+        else e.e[j] = val[which][i][j];
+      }
+      *reinterpret_cast<Four<E>*>(which ? &held[row][d] : static_cast<E*>(c.k) + (at + row) * c.dim + d) = e;
     }
   }
   __syncthreads();
@@ -114,14 +140,11 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const Cache c, const
     const int d = i >> 2, p = (i & 3) * 4;
     E* const to = out + int64_t(d) * c.page_size + p;
     if (p >= g.lo && p + 4 <= g.hi) {
-      struct alignas(4 * sizeof(E)) Four {
-        E e[4];
-      };
-      *reinterpret_cast<Four*>(to) = Four{cols[d][p], cols[d][p + 1], cols[d][p + 2], cols[d][p + 3]};
+      *reinterpret_cast<Four<E>*>(to) = Four<E>{held[p][d], held[p + 1][d], held[p + 2][d], held[p + 3][d]};
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (p + j >= g.lo && p + j < g.hi) to[j] = cols[d][p + j];
+        if (p + j >= g.lo && p + j < g.hi) to[j] = held[p + j][d];
     }
   }
 }
@@ -129,7 +152,7 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const Cache c, const
 template <bool I8>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Cache c, const Batch b, const Rows k, const Rows v) {
   using E = std::conditional_t<I8, int8_t, float>;
-  __shared__ E cols[kMaxDim][kGroup + (I8 ? 0 : 1)];
+  __shared__ __attribute__((aligned(16))) E held[kGroup][kMaxDim + 4];  // values by row (the pitch keeps banks apart)
   Places g;
   if (!places(c, b, blockIdx.x, g)) return;
   const bool here = g.page >= 0;
@@ -138,13 +161,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Cache c, const 
   if (here) {
     const E* const in = static_cast<const E*>(c.v) + (at - g.place) * c.dim + g.place;
     for (int i = threadIdx.x; i < c.dim * 4; i += kThreads) {
-      struct alignas(4 * sizeof(E)) Four {
-        E e[4];
-      };
       const int d = i >> 2, p = (i & 3) * 4;
-      const Four f = *reinterpret_cast<const Four*>(in + int64_t(d) * c.page_size + p);
+      const Four<E> f = *reinterpret_cast<const Four<E>*>(in + int64_t(d) * c.page_size + p);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) cols[d][p + j] = f.e[j];
+      for (int j = 0; j < 4; ++j) held[p + j][d] = f.e[j];
     }
   }
   __syncthreads();
@@ -153,9 +173,16 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Cache c, const 
   if (I8 && here) ks = c.ks[at + row], vs = c.vs[at + row];
   float* const ko = k.at + (g.row + row) * k.token + head * k.head;
   float* const vo = v.at + (g.row + row) * v.token + head * v.head;
-  for (int d = lane; d < c.dim; d += 16) {
-    ko[d] = here ? float(static_cast<const E*>(c.k)[(at + row) * c.dim + d]) * ks : 0.f;
-    vo[d] = here ? float(cols[d][row]) * vs : 0.f;
+  for (int d = lane * 4; d < c.dim; d += 64) {
+    f32x4 a{}, b{};
+    if (here) {
+      const Four<E> e = *reinterpret_cast<const Four<E>*>(static_cast<const E*>(c.k) + (at + row) * c.dim + d);
+      const Four<E> f = *reinterpret_cast<const Four<E>*>(&held[row][d]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = float(e.e[j]) * ks, b[j] = float(f.e[j]) * vs;
+    }
+    *reinterpret_cast<f32x4u*>(ko + d) = a;
+    *reinterpret_cast<f32x4u*>(vo + d) = b;
   }
 }
 

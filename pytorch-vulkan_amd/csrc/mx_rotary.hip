@@ -27,15 +27,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kMaxDim = 256, kThreads = 256, kAngles = 2048;  // kAngles: pairs of a workgroup's tokens in LDS
-// Rows of a lane group at a time.  The backward has three loads to a row, and with four rows
-// at a time (registers of three waves a SIMD) took 99 us in place of 74 for 8192 x 20 x 128.
+// Rows of a lane group at a time.  (The backward has three loads to a row: two rows and four measure
+// the same, 95 us for both directions of 8192 tokens x 20 heads x 128, three 101.)
 constexpr int unroll(bool back) { return back ? 2 : 4; }
 
 struct Rotary {
   int tokens, q_heads, k_heads, dim, rot;
   int64_t q_token, q_head, k_token, k_head;
   const int64_t* positions;
-  float magnitude, eps;
+  float magnitude, eps, per;  // per: 1 / dim
   int interleaved, norm, group;  // group: tokens that a workgroup turns together
   double turns[kMaxDim / 2];     // frequencies / 2 pi
 };
@@ -116,7 +116,7 @@ __device__ __forceinline__ int64_t flat(const Rotary& p, const RowAt& r) {
 }
 template <int L>
 __device__ __forceinline__ float rstd(const Rotary& p, f32x4 x) {
-  return 1.f / sqrtf(lanes_sum<L>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) / p.dim + p.eps);
+  return rsqrtf(lanes_sum<L>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) * p.per + p.eps);
 }
 
 template <int L, bool BACK>
@@ -148,24 +148,24 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
     if (half) angles(p, first, count, cs, sn);
     // A group of L lanes takes every kThreads / L-th row, U at a time (their loads are in
     // flight together), whichever side is wanted: the weights' sums keep their order.
-    const int heads = p.q_heads + p.k_heads, all = count * heads;
-    for (int r0 = threadIdx.x / L; r0 < all; r0 += U * (kThreads / L)) {
+    const int heads = p.q_heads + p.k_heads;
+    int place = threadIdx.x / L / heads, h = threadIdx.x / L - place * heads;  // of the next row
+    while (place < count) {
       RowAt at[U];
       f32x4 v[U], u[U], x[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int r = r0 + j * (kThreads / L);
-        at[j].place = min(r, all - 1) / heads;
-        at[j].head = min(r, all - 1) - at[j].place * heads;
-        at[j].token = first + at[j].place;
-        at[j].k = at[j].head >= p.q_heads;
-        if (at[j].k) at[j].head -= p.q_heads;
-        at[j].live = r < all && (at[j].k ? o.wanted[1] : o.wanted[0]);
+        at[j].k = h >= p.q_heads;
+        at[j].place = place;
+        at[j].head = at[j].k ? h - p.q_heads : h;
+        at[j].token = first + place;
+        at[j].live = place < count && (at[j].k ? o.wanted[1] : o.wanted[0]);
+        for (h += kThreads / L; h >= heads; h -= heads) ++place;
         v[j] = u[j] = x[j] = f32x4{};
         if (!at[j].live) continue;
-        const float* const in = o.x[at[j].k] + at[j].token * (at[j].k ? p.k_token : p.q_token) + at[j].head * (at[j].k ? p.k_head : p.q_head);
+        const float* const in = (at[j].k ? o.x[1] : o.x[0]) + at[j].token * (at[j].k ? p.k_token : p.q_token) + at[j].head * (at[j].k ? p.k_head : p.q_head);
         // the row that the rotation is applied to, its elements' partners, and the norm's input
-        const float* const turned = BACK ? o.dy[at[j].k] + flat(p, at[j]) : in;
+        const float* const turned = BACK ? (at[j].k ? o.dy[1] : o.dy[0]) + flat(p, at[j]) : in;
         v[j] = load4(turned, e, p.dim);
         if (run) {
           u[j] = *reinterpret_cast<const f32x4u*>(turned + with[0]);
@@ -200,21 +200,21 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
           for (int i = 0; i < 4; ++i) {
             const float xh = p.norm ? v[j][i] * r * (k ? w[1][i] : w[0][i]) : v[j][i];
             const float xp = p.norm ? u[j][i] * r * (k ? wp[1][i] : wp[0][i]) : u[j][i];
-            y[i] = pair[i] < 0 ? xh : fmaf(xp, s[i], xh * c[i]);
+            y[i] = fmaf(xp, s[i], xh * c[i]);  // (unturned: cosine 1, sine 0)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = pair[i] < 0 ? v[j][i] : fmaf(u[j][i], s[i], v[j][i] * c[i]);
+          for (int i = 0; i < 4; ++i) y[i] = fmaf(u[j][i], s[i], v[j][i] * c[i]);
           if (p.norm) {
             const float r = rstd<L>(p, x[j]);
             const f32x4 g = y, xr = x[j] * r, gw = g * (k ? w[1] : w[0]);
-            const float m = lanes_sum<L>(gw[0] * xr[0] + gw[1] * xr[1] + gw[2] * xr[2] + gw[3] * xr[3]) / p.dim;
+            const float m = lanes_sum<L>(gw[0] * xr[0] + gw[1] * xr[1] + gw[2] * xr[2] + gw[3] * xr[3]) * p.per;
             y = (gw - xr * m) * r;
             if (k) dw[1] += g * xr;
             else dw[0] += g * xr;
           }
         }
-        if (float* const out = o.out[k]) store4(out + flat(p, at[j]), e, p.dim, y);
+        if (float* const out = k ? o.out[1] : o.out[0]) store4(out + flat(p, at[j]), e, p.dim, y);
       }
     }
     if (half) __syncthreads();
@@ -286,7 +286,7 @@ Rotary params(const mx_rotary_desc* d) {
   p.dim = int(d->head_dim), p.rot = int(d->rotary_dim);
   p.q_token = d->q_token, p.q_head = d->q_head, p.k_token = d->k_token, p.k_head = d->k_head;
   p.positions = d->positions;
-  p.magnitude = float(d->magnitude), p.eps = float(d->eps);
+  p.magnitude = float(d->magnitude), p.eps = float(d->eps), p.per = 1.f / float(d->head_dim);
   p.interleaved = d->interleaved, p.norm = d->norm;
   for (int i = 0; i < p.rot / 2; ++i) p.turns[i] = d->frequencies[i] / 6.283185307179586476925286766559;
   return p;

@@ -548,7 +548,7 @@ def test_cache_ties_and_special_rows(mx):
     assert k[1, 0, :4].tolist() == [127.0, 0.0, 2.0, -2.0]
     assert bool(k[4:7].isnan().all()), "NaN and infinities"
     steps = cache.tensors[0][2, 0, 3:12].double()
-    assert bool((steps.abs() <= 127).all())
+    assert bool((steps.abs() <= 127).all()) and bool((cache.tensors[0][2, 0, 10] == 0).all()), "no steps of a scale of 0"
     # random rows and scales: every step is the rounding of the exact quotient
     g = gen(12)
     x = rand(g, 4000, 1, 128) * torch.exp2(torch.randint(-60, 60, (4000, 1, 1), device="cuda", generator=g).float())
