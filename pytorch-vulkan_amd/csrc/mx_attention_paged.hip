@@ -71,7 +71,7 @@ struct Place {
 };
 
 template <int DP, bool I8>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2 : 1))) void paged_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void paged_kernel(const PagedArgs a) {
   constexpr int kUnits = DP / 64, kBlocks = DP / 16, kPitch = DP + 4;
   __shared__ float stat[2][kWaves][kRows], sum[kRows][kPitch];
   using E = std::conditional_t<I8, int8_t, float>;
@@ -95,17 +95,20 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
     k.find(c, a.b, t.seq, tile, kg);
     v.find(c, a.b, t.seq, tile, g);
   };
-  // Key 16 kg + 4 i + col % 4 is row col of the tile's i-th block of 16.
-  Sixteen<I8> k[4][kUnits];
-  const auto fetch = [&](const Place& at) {
+  // Key 16 kg + 4 i + col % 4 is row col of the tile's i-th block of 16.  (FP32 keys have no registers
+  // to wait in with two waves a SIMD, which gains more than reading ahead does.)
+  constexpr bool kAhead = I8;
+  Sixteen<I8> k[kAhead ? 4 : 1][kUnits];
+  const auto fetch = [&](const Place& at, int i0, int i1) {
     const E* const from = static_cast<const E*>(c.k) +
                           ((int64_t(max(at.page, 0)) * c.heads + kv_head) * c.page_size + at.place + (col & 3)) * c.dim + 16 * g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = i0; i < i1; ++i)
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
-        k[i][u] = {};
-        if (64 * u + 16 * g < c.dim) k[i][u].load(from + 4 * i * c.dim + 64 * u);
+        Sixteen<I8>& to = k[kAhead ? i : 0][u];
+        to = {};
+        if (64 * u + 16 * g < c.dim) to.load(from + 4 * i * c.dim + 64 * u);
       }
   };
   const int from = begin + wave;
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
       q[2 * u] = split8(v[0], v[1]);
       q[2 * u + 1] = split8(v[2], v[3]);
     }
-    fetch(kp);
+    if (kAhead) fetch(kp, 0, 4);
   }
   f32x4 o[kBlocks] = {};
   float m = -__builtin_inff(), l = 0;  // of the exponents
@@ -143,28 +146,33 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
         vs[i] = *reinterpret_cast<const f32x4*>(c.vs + places + vp.place + 4 * i);
       }
     }
-    Sixteen<I8> v[kBlocks];
     const E* const vfrom = static_cast<const E*>(c.v) + places * c.dim + int64_t(col) * c.page_size + vp.place;
+    const auto values = [&](int b) {
+      Sixteen<I8> v{};
+      if (16 * b < c.dim) v.load(vfrom + int64_t(16 * b) * c.page_size);
+      return v;
+    };
+    Sixteen<I8> v[kAhead ? kBlocks : 1];
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      v[b] = {};
-      if (16 * b < c.dim) v[b].load(vfrom + int64_t(16 * b) * c.page_size);
+      for (int b = 0; b < kBlocks; ++b) v[b] = values(b);
     }
     // ---- scores: block i gives the lane keys j + 4 i .. + 3
     float x[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x4 acc{};
+      if (!kAhead) fetch(kp, i, i + 1);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         if (64 * u >= c.dim) continue;
-        acc = mma_all(k[i][u].half(0), q[2 * u], acc);
-        acc = mma_all(k[i][u].half(1), q[2 * u + 1], acc);
+        acc = mma_all(k[kAhead ? i : 0][u].half(0), q[2 * u], acc);
+        acc = mma_all(k[kAhead ? i : 0][u].half(1), q[2 * u + 1], acc);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * i + e] = I8 ? acc[e] * ks[i][e] : acc[e];
     }
-    if (n + kWaves < end) fetch(kn);
+    if (kAhead && n + kWaves < end) fetch(kn, 0, 4);
     const bool part = __any(!here || j + 16 > rt.length) || !a.mask.all(rt.i0, rt.i1, j0, j0 + kKeys - 1);
     if (part) {
       __builtin_amdgcn_sched_barrier(0);
@@ -172,17 +180,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
       for (int r = 0; r < 16; ++r)
         if (!here || j + r >= rt.length || !a.mask.sees(pos, j + r)) x[r] = -__builtin_inff();
       if constexpr (!I8) {
-        // What no row sees counts as zero, and a value that is not finite as a NaN score of its key.
+        // A value that is not finite is a NaN score of its key, and zero (below).
         uint32_t bad = 0;
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
+        for (int b = 0; b < kBlocks; ++b) {
+          if (16 * b >= c.dim) continue;
+          const Sixteen<I8> e = values(b);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float e = v[b].raw[r >> 2][r & 3];
-            const bool no = !here || j + r >= rt.length, odd = !(fabsf(e) <= 3.402823466e38f);
-            if (odd && !no) bad |= 1u << r;
-            if (no || odd) v[b].raw[r >> 2][r & 3] = 0;
-          }
+          for (int r = 0; r < 16; ++r)
+            if (!finite(e.raw[r >> 2][r & 3]) && here && j + r < rt.length) bad |= 1u << r;
+        }
         if (__any(bad != 0)) {
 #pragma unroll
           for (int s = 1; s < 16; s <<= 1) bad |= __shfl_xor(int(bad), s, 64);
@@ -213,8 +220,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(I8 ? 2
     const Frag3 p[2] = {split8(f32x4{x[0], x[1], x[2], x[3]}, f32x4{x[4], x[5], x[6], x[7]}),
                         split8(f32x4{x[8], x[9], x[10], x[11]}, f32x4{x[12], x[13], x[14], x[15]})};
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-      if (16 * b < c.dim) o[b] = o[b] * keep + mma_all(v[b].half(1), p[1], mma_all(v[b].half(0), p[0], f32x4{}));
+    for (int b = 0; b < kBlocks; ++b) {
+      if (16 * b >= c.dim) continue;
+      if constexpr (!kAhead) {
+        v[0] = values(b);
+        if (part) {  // what no row sees, or no finite number, counts as zero
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!here || j + r >= rt.length || !finite(v[0].raw[r >> 2][r & 3])) v[0].raw[r >> 2][r & 3] = 0;
+        }
+      }
+      const Sixteen<I8>& e = v[kAhead ? b : 0];
+      o[b] = o[b] * keep + mma_all(e.half(1), p[1], mma_all(e.half(0), p[0], f32x4{}));
+    }
     kp = kn, vp = vn;
   }
   l += __shfl_xor(l, 16, 64);
