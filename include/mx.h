@@ -644,7 +644,7 @@ int mx_qk_norm_rotary_workspace(const mx_rotary_desc* d, int64_t* bytes);
  * heads / kv_heads query heads to a key head.  Rows that belong to no sequence are left
  * as they are, in every output.  A row that sees a NaN or an infinity is NaN, and so are
  * the gradients that it reaches; those of keys and queries that a row does not see
- * have no effect on it. */
+ * have no effect on it.  No operand may overlap an output. */
 typedef struct mx_attention_desc {
   int64_t tokens, sequences;
   const int32_t* starts; /* device, [sequences + 1], ascending: sequence b is rows starts[b] .. starts[b + 1] - 1;
@@ -664,6 +664,8 @@ int mx_attention_forward(const mx_attention_desc* d, const float* q, const float
 int mx_attention_backward(const mx_attention_desc* d, const float* dout, const float* q, const float* k, const float* v,
                           const float* out, const float* lse, float* dq, float* dk, float* dv, void* workspace,
                           int64_t workspace_bytes, void* stream);
+/* Bytes that a forward (`backward` == 0) or a backward of such a descriptor takes (its window and
+ * sinks count; starts is not read). */
 int mx_attention_workspace(const mx_attention_desc* d, int backward, int64_t* bytes);
 
 /* A paged cache of keys and values: k [pages, heads, page_size, head_dim] and
@@ -690,7 +692,8 @@ typedef struct mx_kv_batch {
   const int32_t* table;   /* device, [sequences, table_width] */
 } mx_kv_batch;
 /* Writes k and v [tokens, cache->heads, head_dim] (strides of the token and the head) to
- * the cache.  Two new tokens that share a place leave either one's row or a mixture. */
+ * the cache.  Two new tokens that share a place leave either one's row or a mixture; a page that a
+ * call writes may be read by no call that can run at the same time. */
 int mx_kv_cache_write(const mx_kv_cache* c, const mx_kv_batch* b, const float* k, int64_t k_token, int64_t k_head,
                       const float* v, int64_t v_token, int64_t v_head, void* stream);
 /* Reads them back into contiguous k and v (lengths' last tokens; all of a sequence where

@@ -100,6 +100,8 @@ struct Pack {
 
 // grid (tiles, heads + kv_heads, or kv_heads alone): a key head's k and v, or a query head's q, dout,
 // lse and delta.
+// Bound by memory: 4 bytes read and 6 written an element (45 us for q, dout, out, k and v of 2 x 2048
+// tokens, 16 and 4 heads of 128: 4.9 TB/s).
 template <int DP>
 __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
   __shared__ uint32_t bits[2][4];
@@ -175,6 +177,12 @@ struct FwdArgs {
 // Steps whose queries' smallest piece waits in LDS, where two waves a SIMD have no registers for it.
 constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0; }
 
+// A wave's 32 queries stay in registers as pieces, with their sums.  Bound by the matrix
+// instructions: 16384 tokens, 16 heads of 64, window 4096 1340 us, 180 TFLOP/s, six piece products of which
+// are 1.08 PFLOP/s (a library's bf16 product of 8192^3 1.25 on this card); 2 x 2048, 16 heads of 128 250 us,
+// 137 TFLOP/s, where one wave a SIMD hides neither LDS's latency nor the softmax behind
+// products, and workgroups of eight waves, which do (4.5 us a tile of 256 rows for 3.7 of 128), have too
+// uneven work (289 us).
 template <int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 8 || DP <= 96 ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
   using St = Stages<DP, 3, WAVES, 0>;
@@ -209,7 +217,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     pieces::barrier();
     if (n + 1 < keys.count) fetch(n + 1);
     const int j0 = keys.tile(n) * kTile;
-    if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
+    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
     f32x16 x = product<DP, 3>(tile, q, lane, low);
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
@@ -259,16 +267,21 @@ struct BwdArgs {
 // So that their workgroup is not the last by far, the queries past the window of its block are
 // dealt to workgroups of their own, chunks of 1024 rows of a sequence, whose sums far_kernel
 // adds in order (8 sequences of up to 2048, window 512, 4 first tokens, 12 heads of 80: dk and dv
-// TODO us).
-constexpr int kChunk = 1024;
+// 270 us with them in the block's own workgroup, 243 + 7 so).
+constexpr int kChunk = 1024, kFarBlocks = 4;
 __device__ __forceinline__ float* far_at(const BwdArgs& a, int chunk, int block, int kv_head, int part) {
   return a.far + (((int64_t(chunk) * a.far_blocks + block) * a.s.kv_heads + kv_head) * a.parts + part) * (2 * kBlock * a.s.dim);
 }
-// The last row whose window reaches a key of the block at b0.
-__device__ __forceinline__ int near_last(const Mask& m, int b0, int len) {
-  return m.window ? min(len - 1, b0 + kBlock - 1 + min(m.window, len) - 1) : len - 1;
+// The last row that the workgroup of the block at b0 takes: of its keys' window, or of the sequence
+// where no other workgroup has what lies past it.
+__device__ __forceinline__ int near_last(const BwdArgs& a, int b0, int len) {
+  const Mask& m = a.s.mask;
+  const bool all = m.window == 0 || (b0 < m.sinks && b0 >= a.far_blocks * kBlock);
+  return all ? len - 1 : min(len - 1, b0 + kBlock - 1 + min(m.window, len) - 1);
 }
 
+// Three products of a tile, two of them computed again by dkv_kernel: the scores' gradients would be
+// 6 bytes a pair in memory.  318 us for 2 x 2048, 16 heads of 128: 162 TFLOP/s, 0.97 PFLOP/s of pieces.
 template <int DP>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   using St = Stages<DP, 3, 4, 0>;
@@ -302,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     pieces::barrier();
     if (n + 1 < keys.count) fetch(n + 1);
     const int j0 = keys.tile(n) * kTile;
-    if (s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
+    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
     f32x16 x = product<DP, 3>(tile, q, lane) - lse;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
@@ -319,6 +332,8 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     store_block(a.dq + ((int64_t(t.start) + qi) * s.heads + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
 }
 
+// Four products of a tile, the scores straight (a lane has 16 queries of a key), so that both sums run
+// along what a lane holds.  416 us for 2 x 2048, 16 heads of 128: 165 TFLOP/s, 0.99 PFLOP/s of pieces.
 template <int DP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
   using St = Stages<DP, 3, 4, 1>;
@@ -338,7 +353,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
   const int j0 = b0 + wave * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
   const St st{lds_address(smem)};
   // The tiles of queries that see any of the workgroup's keys, of each head in turn.
-  int from = b0 / kTile, to = near_last(s.mask, b0, t.len) / kTile;
+  int from = b0 / kTile, to = near_last(a, b0, t.len) / kTile;
   if (far) {
     from = max(to + 1, t.index * (kChunk / kTile));
     to = min(t.len - 1, (t.index + 1) * kChunk - 1) / kTile;
@@ -367,7 +382,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     pieces::barrier();
     if (n + 1 < count) fetch(n + 1);
     const int i0 = (from + n % tiles) * kTile;
-    if (s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
+    if (j0 >= t.len || s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes;
     f32x16 x = product<DP, 3>(tile, k, lane), delta;
 #pragma unroll
@@ -412,32 +427,33 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
 }
 
 // What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of 128
-// keys times workgroups of a block, key heads, sequences).
+// keys times workgroups of a block, key heads, sequences or fewer).
 __global__ __launch_bounds__(kThreads) void far_kernel(const BwdArgs a) {
   const Shape& s = a.s;
   const int per = gridDim.x / a.far_blocks, block = blockIdx.x / per, b0 = block * kBlock;
-  const int start = s.seqs.start(blockIdx.z), len = max(0, s.seqs.start(blockIdx.z + 1) - start);
-  if (b0 >= len) return;
-  const int from = (near_last(s.mask, b0, len) / kTile + 1) * kTile / kChunk, to = (len - 1) / kChunk;
-  if (near_last(s.mask, b0, len) / kTile == (len - 1) / kTile) return;  // no queries past the window
-  const int rows = min(min(kBlock, len - b0), (s.mask.sinks - b0 + kTile - 1) / kTile * kTile), base = start / kChunk + blockIdx.z;
   const int i = (blockIdx.x - block * per) * kThreads + threadIdx.x;
-  if (i >= rows * s.dim) return;
-  const int64_t at = ((int64_t(start) + b0 + i / s.dim) * s.kv_heads + blockIdx.y) * s.dim + i % s.dim;
-  float k = a.dk ? a.dk[at] : 0.f, v = a.dv ? a.dv[at] : 0.f;
-  for (int c = from; c <= to; ++c)
+  for (int seq = blockIdx.z; seq < s.seqs.count; seq += gridDim.z) {
+    const int start = s.seqs.start(seq), len = max(0, s.seqs.start(seq + 1) - start);
+    if (b0 >= len || near_last(a, b0, len) / kTile == (len - 1) / kTile) continue;  // no queries past the window
+    const int from = (near_last(a, b0, len) / kTile + 1) * kTile / kChunk, to = (len - 1) / kChunk, base = start / kChunk + seq;
+    const int rows = min(min(kBlock, len - b0), (s.mask.sinks - b0 + kTile - 1) / kTile * kTile);
+    if (i >= rows * s.dim) continue;
+    const int64_t at = ((int64_t(start) + b0 + i / s.dim) * s.kv_heads + blockIdx.y) * s.dim + i % s.dim;
+    float k = a.dk ? a.dk[at] : 0.f, v = a.dv ? a.dv[at] : 0.f;
+    for (int c = from; c <= to; ++c)
 #pragma unroll 4
-    for (int p = 0; p < a.parts; ++p) {
-      const float* const sum = far_at(a, base + c, block, blockIdx.y, p) + i;
-      if (a.dk) k += sum[0];
-      if (a.dv) v += sum[kBlock * s.dim];
-    }
-  if (a.dk) a.dk[at] = k;
-  if (a.dv) a.dv[at] = v;
+      for (int p = 0; p < a.parts; ++p) {
+        const float* const sum = far_at(a, base + c, block, blockIdx.y, p) + i;
+        if (a.dk) k += sum[0];
+        if (a.dv) v += sum[kBlock * s.dim];
+      }
+    if (a.dk) a.dk[at] = k;
+    if (a.dv) a.dv[at] = v;
+  }
 }
 
 // dk and dv: the parts' sums, in order, over the rows from the first sequence's start to the
-// last one's end.
+// last one's end (14 us for four parts of 4096 x 4 x 128: 6 TB/s, in part from the cache).
 __global__ __launch_bounds__(kThreads) void join_kernel(const BwdArgs a) {
   const Shape& s = a.s;
   const int64_t row = int64_t(s.kv_heads) * s.dim, step = s.seqs.tokens * row;
@@ -471,9 +487,10 @@ int check(const char* who, const mx_attention_desc* d) {
              d->head_dim);
   MX_REQUIRE(d->heads == 0 || (d->kv_heads > 0 && d->heads % d->kv_heads == 0), MX_ERR_INVALID, who, ": ", d->heads,
              " heads do not share ", d->kv_heads, " key heads evenly");
-  MX_REQUIRE(d->tokens <= (1 << 30) && d->sequences <= (1 << 24) && d->heads + d->kv_heads <= 65535, MX_ERR_INVALID, who,
-             ": size out of range");
-  MX_REQUIRE((d->tokens / kBlock + d->sequences) * d->heads < (int64_t(1) << 31), MX_ERR_INVALID, who, ": size out of range");
+  // (a grid's work-items are counted in 32 bits; the largest has far blocks' chunks among its blocks)
+  MX_REQUIRE(d->tokens <= (1 << 28) && d->sequences <= (1 << 21) && d->heads + d->kv_heads <= 65535 &&
+                 (d->tokens / kBlock + d->sequences + kFarBlocks * (d->tokens / kChunk + d->sequences)) * d->heads < (1 << 24),
+             MX_ERR_INVALID, who, ": size out of range");
   MX_REQUIRE(d->tokens == 0 || d->sequences > 0, MX_ERR_INVALID, who, ": tokens of no sequence");
   MX_REQUIRE(d->starts || d->sequences == 0 || d->tokens % d->sequences == 0, MX_ERR_INVALID, who, ": ", d->tokens,
              " tokens do not divide into ", d->sequences, " sequences");
@@ -511,9 +528,11 @@ struct Buffers {
   float *stats, *dk_p, *dv_p, *far;
 };
 
-// Blocks of keys that are seen past the window, and chunks of queries.
+// Blocks of keys that are seen past the window by workgroups of their own (of more first tokens
+// the blocks behind have as much to do as each other), and chunks of queries.
 int64_t far_blocks_of(const Shape& s) {
-  return s.mask.window && s.mask.window < s.seqs.tokens ? (std::min(s.mask.sinks, s.seqs.tokens) + int64_t(kBlock) - 1) / kBlock : 0;
+  if (!s.mask.window || s.mask.window >= s.seqs.tokens) return 0;
+  return std::min<int64_t>((std::min(s.mask.sinks, s.seqs.tokens) + kBlock - 1) / kBlock, kFarBlocks);
 }
 int64_t chunks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kChunk); }
 
@@ -662,7 +681,7 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
     if (g.far_blocks) {
       const int rows = std::min(kBlock, (std::min(s.mask.sinks, kBlock) + kTile - 1) / kTile * kTile);
       const unsigned per = unsigned((rows * s.dim + kThreads - 1) / kThreads);
-      hipLaunchKernelGGL(far_kernel, dim3(unsigned(g.far_blocks) * per, unsigned(s.kv_heads), unsigned(s.seqs.count)),
+      hipLaunchKernelGGL(far_kernel, dim3(unsigned(g.far_blocks) * per, unsigned(s.kv_heads), unsigned(std::min(s.seqs.count, 4096))),
                          dim3(kThreads), 0, st, g);
       MX_LAUNCHED();
     }

@@ -37,7 +37,8 @@ __device__ __forceinline__ KeyTiles<> seen_by_all(const ChunkArgs& a, const RowT
   return KeyTiles<>(a.mask, max(rt.first, 0), min(rt.first + rt.t.len / a.group - 1, rt.length - 1));
 }
 
-// grid (tiles, kv heads, sequences): 32 keys of one head and sequence.
+// grid (tiles, kv heads, sequences): 32 keys of one head and sequence.  (22 us for 4 sequences' 4608 keys of 4
+// heads of 128, 57 MB: many short workgroups, each waiting for lengths, table and cache in turn.)
 template <int DP, bool I8>
 __global__ __launch_bounds__(256) void gather_kernel(const ChunkArgs a) {
   constexpr int P = I8 ? 1 : 3;
@@ -135,6 +136,7 @@ __global__ __launch_bounds__(256) void gather_kernel(const ChunkArgs a) {
   }
 }
 
+// 4 x 512 tokens, 16 heads of 128, 8-bit keys, window 4096: 199 us, 346 TFLOP/s, 1.04 PFLOP/s of pieces.
 template <int DP, bool I8, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(I8 || DP <= 96 ? 2 : 1))) void chunk_kernel(
     const ChunkArgs a) {

@@ -36,7 +36,7 @@ struct RowTile {
     return true;
   }
   __device__ __forceinline__ void whole(const Paged& a) {
-    const int last = a.b.lengths[t.seq];
+    const int last = max(a.b.lengths[t.seq], -(1 << 30));
     length = int(min(int64_t(max(last, 0)), int64_t(a.b.width) * a.c.page_size));
     first = last - t.len / a.group;
   }

