@@ -166,6 +166,69 @@ __device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const char* tile, 
 // to do first and keeps a head's on as few XCDs as there are heads for.
 constexpr int kBlock = 4 * kTile;
 
+// A block of a wave's sums in LDS.
+__device__ __forceinline__ void put_block(uint32_t at, int b, const f32x16& v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *pieces::lds_at<f32x4>(at + b * 4096 + i * 1024) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+__device__ __forceinline__ f32x16 get_block(uint32_t at, int b) {
+  f32x16 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 x = *pieces::lds_at<const f32x4>(at + b * 4096 + i * 1024);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * i + e] = x[e];
+  }
+  return v;
+}
+
+// A workgroup's walk over tiles, SPLIT of them at a time: of its four (or more) waves each SPLIT share
+// their rows, and take every SPLIT-th tile.
+template <int DP, int WAVES, int SPLIT, int STATS>
+struct Walk {
+  using St = Stages<DP, 3, WAVES, STATS>;
+  static constexpr int kGroups = WAVES / SPLIT, kRows = kGroups * kTile, kBytes = 2 * SPLIT * St::kBytes;
+  St st;
+  int wave, lane, count;
+  __device__ __forceinline__ int rows() const { return wave % kGroups * kTile; }
+  __device__ __forceinline__ int turn() const { return wave / kGroups; }
+  // load(tile, stage) for each of step n's
+  template <class F>
+  __device__ __forceinline__ void fetch(int n, F&& load) const {
+#pragma unroll
+    for (int u = 0; u < SPLIT; ++u)
+      if (n * SPLIT + u < count) load(n * SPLIT + u, (n & 1) * SPLIT + u);
+  }
+  // take(tile, its address in LDS) for each of the wave's, the next ones on their way
+  template <class F, class G>
+  __device__ __forceinline__ void run(F&& load, G&& take) const {
+    for (int n = 0; n * SPLIT < count; ++n) {
+      pieces::wait_loads<0>();
+      pieces::barrier();
+      fetch(n + 1, load);
+      const int mine = n * SPLIT + turn();
+      if (SPLIT == 1 || mine < count) take(mine, st.lds + ((n & 1) * SPLIT + turn()) * St::kBytes);
+    }
+  }
+  // Behind the walk: adds what the waves that share rows have (BLOCKS blocks) to the first one's,
+  // through LDS.  False in the others.
+  template <int BLOCKS, class F>
+  __device__ __forceinline__ bool join(F&& block) const {
+    if constexpr (SPLIT > 1) {
+      static_assert(SPLIT <= 2 && BLOCKS * 4096 * kGroups <= kBytes);
+      const uint32_t at = st.lds + wave % kGroups * (BLOCKS * 4096) + lane * 16;
+      __syncthreads();
+      if (turn())
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) put_block(at, b, block(b));
+      __syncthreads();
+      if (turn()) return false;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) block(b) += get_block(at, b);
+    }
+    return true;
+  }
+};
 // ------------------------------------------------------------------ forward
 struct FwdArgs {
   Shape s;
@@ -183,42 +246,39 @@ constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0;
 // 137 TFLOP/s, where one wave a SIMD hides neither LDS's latency nor the softmax behind
 // products, and workgroups of eight waves, which do (4.5 us a tile of 256 rows for 3.7 of 128), have too
 // uneven work (289 us).
-template <int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES == 8 || DP <= 96 ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
-  using St = Stages<DP, 3, WAVES, 0>;
-  constexpr int kRows = WAVES * kTile;
+template <int DP, int WAVES, int SPLIT>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && (WAVES == 8 || DP <= 96) ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
+  using W = Walk<DP, WAVES, SPLIT, 0>;
+  constexpr int kRows = W::kRows;
   constexpr int kAside = aside(DP, WAVES);
-  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes + kAside * WAVES * 1024];
+  __shared__ __attribute__((aligned(1024))) char smem[W::kBytes + kAside * WAVES * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
   SequenceTile t;
   if (!locate<kRows>(s.seqs, block, t) || t.index * kRows >= t.len) return;
   const int64_t keys0 = tile_at<DP>(s, head / s.group, t.start / kTile + t.seq);
-  const int b0 = t.index * kRows, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
-  const St st{lds_address(smem)};
+  const int b0 = t.index * kRows;
   const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
-  const auto fetch = [&](int n) {
+  const W walk{{lds_address(smem)}, wave, lane, keys.count};
+  const auto load = [&](int n, int stage) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
-    st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
+    walk.st.load(stage, a.kp + at, a.vp + at, nullptr, wave, lane);
   };
-  fetch(0);
+  walk.fetch(0, load);
+  const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
   Frag3 q[DP / 16];
   own_rows<DP>(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
-  bf16x8* const mine = reinterpret_cast<bf16x8*>(smem + 2 * St::kBytes) + wave * kAside * 64 + lane;
+  bf16x8* const mine = reinterpret_cast<bf16x8*>(smem + W::kBytes) + wave * kAside * 64 + lane;
 #pragma unroll
   for (int i = 0; i < kAside; ++i) mine[i * 64] = q[i].lo;
   const auto low = [&](int i) { return i < kAside ? mine[i * 64] : q[i].lo; };
   f32x16 o[DP / 32] = {};
   float m = -__builtin_inff(), l = 0;  // of the exponents
   const uint32_t columns = column_base(lane);
-  for (int n = 0; n < keys.count; ++n) {
-    pieces::wait_loads<0>();
-    pieces::barrier();
-    if (n + 1 < keys.count) fetch(n + 1);
+  walk.run(load, [&](int n, uint32_t tile) {
     const int j0 = keys.tile(n) * kTile;
-    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
-    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) return;
     f32x16 x = product<DP, 3>(tile, q, lane, low);
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
     float top = x[0];
@@ -239,8 +299,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
       if (DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
-      o[b] = o[b] * keep + product_columns(tile + St::kSecond + columns, b, p);
+      o[b] = o[b] * keep + product_columns(tile + W::St::kSecond + columns, b, p);
     }
+  });
+  if constexpr (SPLIT > 1) {
+    // To the larger of both maxima, then the sums (l among them).
+    float* const top = reinterpret_cast<float*>(smem) + wave * 64 + lane;
+    __syncthreads();
+    *top = m;
+    __syncthreads();
+    const float next = fmaxf(m, top[(walk.turn() ? -1 : 1) * W::kGroups * 64]), keep = exp2_(m - (next == -__builtin_inff() ? 0.f : next));
+    f32x16 sum{};
+    sum[0] = l * keep, m = next;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) o[b] *= keep;
+    if (!walk.template join<DP / 32 + 1>([&](int b) -> f32x16& { return b == DP / 32 ? sum : o[b]; })) return;
+    l = sum[0];
   }
   l += __shfl_xor(l, 32, 64);
   if (qi >= t.len) return;
@@ -259,48 +333,51 @@ struct BwdArgs {
   float *dq, *dk, *dv;
   int parts;            // of a key head's query heads
   float *dk_p, *dv_p;  // [part][token][key head][dim] where there are several
+  int block;             // of keys, 128 or 64
   int near, far_blocks;  // workgroups' blocks of keys, and of those that are seen past the window
-  float* far;            // [chunk][block][key head][part][dk, dv][128][dim]
+  float* far;            // [chunk][block][key head][part][dk, dv][key of the block][dim]
 };
 
 // First tokens that stay visible are seen by every later query, other keys by a window's.
 // So that their workgroup is not the last by far, the queries past the window of its block are
-// dealt to workgroups of their own, chunks of 1024 rows of a sequence, whose sums far_kernel
+// dealt to workgroups of their own, chunks of 512 rows of a sequence, whose sums far_kernel
 // adds in order (8 sequences of up to 2048, window 512, 4 first tokens, 12 heads of 80: dk and dv
 // 270 us with them in the block's own workgroup, 243 + 7 so).
-constexpr int kChunk = 1024, kFarBlocks = 4;
+constexpr int kChunk = 512, kFarBlocks = 4;
 __device__ __forceinline__ float* far_at(const BwdArgs& a, int chunk, int block, int kv_head, int part) {
-  return a.far + (((int64_t(chunk) * a.far_blocks + block) * a.s.kv_heads + kv_head) * a.parts + part) * (2 * kBlock * a.s.dim);
+  return a.far + (((int64_t(chunk) * a.far_blocks + block) * a.s.kv_heads + kv_head) * a.parts + part) * (2 * a.block * a.s.dim);
 }
 // The last row that the workgroup of the block at b0 takes: of its keys' window, or of the sequence
 // where no other workgroup has what lies past it.
 __device__ __forceinline__ int near_last(const BwdArgs& a, int b0, int len) {
   const Mask& m = a.s.mask;
-  const bool all = m.window == 0 || (b0 < m.sinks && b0 >= a.far_blocks * kBlock);
-  return all ? len - 1 : min(len - 1, b0 + kBlock - 1 + min(m.window, len) - 1);
+  const bool all = m.window == 0 || (b0 < m.sinks && b0 >= a.far_blocks * a.block);
+  return all ? len - 1 : min(len - 1, b0 + a.block - 1 + min(m.window, len) - 1);
 }
 
 // Three products of a tile, two of them computed again by dkv_kernel: the scores' gradients would be
 // 6 bytes a pair in memory.  318 us for 2 x 2048, 16 heads of 128: 162 TFLOP/s, 0.97 PFLOP/s of pieces.
-template <int DP>
+template <int DP, int SPLIT>
 __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
-  using St = Stages<DP, 3, 4, 0>;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes];
+  using W = Walk<DP, 4, SPLIT, 0>;
+  constexpr int kRows = W::kRows;
+  __shared__ __attribute__((aligned(1024))) char smem[W::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
   SequenceTile t;
-  if (!locate<kBlock>(s.seqs, block, t) || t.index * kBlock >= t.len) return;
+  if (!locate<kRows>(s.seqs, block, t) || t.index * kRows >= t.len) return;
   const int base32 = t.start / kTile + t.seq;
   const int64_t keys0 = tile_at<DP>(s, head / s.group, base32);
-  const int b0 = t.index * kBlock, i0 = b0 + wave * kTile, i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
-  const St st{lds_address(smem)};
-  const KeyTiles<> keys(s.mask, b0, min(b0 + kBlock, t.len) - 1);
-  const auto fetch = [&](int n) {
+  const int b0 = t.index * kRows;
+  const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
+  const W walk{{lds_address(smem)}, wave, lane, keys.count};
+  const auto load = [&](int n, int stage) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
-    st.load(n & 1, a.kp + at, a.vp + at, nullptr, wave, lane);
+    walk.st.load(stage, a.kp + at, a.vp + at, nullptr, wave, lane);
   };
-  fetch(0);
+  walk.fetch(0, load);
+  const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
   // A wave past the sequence's end repeats its last tile, and stores nothing.
   const int mine = base32 + min(i0, t.len - 1) / kTile;
   Frag3 q[DP / 16], g[DP / 16];
@@ -310,23 +387,19 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   const float lse = stat[0], delta = stat[32];
   f32x16 dq[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  for (int n = 0; n < keys.count; ++n) {
-    pieces::wait_loads<0>();
-    pieces::barrier();
-    if (n + 1 < keys.count) fetch(n + 1);
+  walk.run(load, [&](int n, uint32_t tile) {
     const int j0 = keys.tile(n) * kTile;
-    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
-    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) return;
     f32x16 x = product<DP, 3>(tile, q, lane) - lse;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
-    const f32x16 dp = product<DP, 3>(tile + St::kSecond, g, lane);
+    const f32x16 dp = product<DP, 3>(tile + W::St::kSecond, g, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(tile + columns, b, p);
-  }
-  if (qi >= t.len) return;
+  });
+  if (!walk.template join<DP / 32>([&](int b) -> f32x16& { return dq[b]; }) || qi >= t.len) return;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
     store_block(a.dq + ((int64_t(t.start) + qi) * s.heads + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
@@ -334,24 +407,25 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
 
 // Four products of a tile, the scores straight (a lane has 16 queries of a key), so that both sums run
 // along what a lane holds.  416 us for 2 x 2048, 16 heads of 128: 165 TFLOP/s, 0.99 PFLOP/s of pieces.
-template <int DP>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
-  using St = Stages<DP, 3, 4, 1>;
-  constexpr int kAside = DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
-  __shared__ __attribute__((aligned(1024))) char smem[2 * St::kBytes + kAside * 4 * 1024];
+template <int DP, int SPLIT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
+  using W = Walk<DP, 4, SPLIT, 1>;
+  using St = typename W::St;
+  constexpr int kRows = W::kRows;
+  constexpr int kAside = SPLIT == 1 && DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
+  __shared__ __attribute__((aligned(1024))) char smem[W::kBytes + kAside * 4 * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int across = s.kv_heads * a.parts, kv_head = blockIdx.x % across / a.parts, part = blockIdx.x % across % a.parts;
-  const int block = blockIdx.x / across;
-  const bool far = block >= a.near;
-  const int chunk = far ? (block - a.near) / a.far_blocks : 0, far_block = far ? (block - a.near) % a.far_blocks : 0;
+  // (those first, which have the most to do)
+  const int index = blockIdx.x / across, block = index - (gridDim.x / across - a.near);
+  const bool far = block < 0;
+  const int chunk = far ? index / a.far_blocks : 0, far_block = far ? index % a.far_blocks : 0;
   SequenceTile t;
-  if (far ? !locate<kChunk>(s.seqs, chunk, t) : !locate<kBlock>(s.seqs, block, t)) return;
-  const int b0 = far ? far_block * kBlock : t.index * kBlock;
+  if (far ? !locate<kChunk>(s.seqs, chunk, t) : !locate<kRows>(s.seqs, block, t)) return;
+  const int b0 = (far ? far_block : t.index) * kRows;
   if (b0 >= t.len) return;
   const int base32 = t.start / kTile + t.seq;
-  const int j0 = b0 + wave * kTile, j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
-  const St st{lds_address(smem)};
   // The tiles of queries that see any of the workgroup's keys, of each head in turn.
   int from = b0 / kTile, to = near_last(a, b0, t.len) / kTile;
   if (far) {
@@ -361,29 +435,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
   const int tiles = to + 1 - from;
   if (tiles <= 0) return;
   const int heads = s.group / a.parts, head0 = kv_head * s.group + part * heads, count = heads * tiles;
-  const auto fetch = [&](int n) {
+  const W walk{{lds_address(smem)}, wave, lane, count};
+  const auto load = [&](int n, int stage) {
     const int head = head0 + n / tiles, tile = base32 + from + n % tiles;
     const int64_t at = tile_at<DP>(s, head, tile);
-    st.load(n & 1, a.qp + at, a.dp + at, reinterpret_cast<const char*>(a.stats + (int64_t(head) * s.tiles + tile) * 64), wave, lane);
+    walk.st.load(stage, a.qp + at, a.dp + at, reinterpret_cast<const char*>(a.stats + (int64_t(head) * s.tiles + tile) * 64), wave, lane);
   };
-  fetch(0);
+  walk.fetch(0, load);
+  const int j0 = b0 + walk.rows(), j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
   const int64_t mine = tile_at<DP>(s, kv_head, base32 + min(j0, t.len - 1) / kTile);
   Frag3 k[DP / 16], v[DP / 16];
   own_rows<DP>(k, a.kp + mine, lane);
   own_rows<DP>(v, a.vp + mine, lane);
-  bf16x8* const aside_at = reinterpret_cast<bf16x8*>(smem + 2 * St::kBytes) + wave * kAside * 64 + lane;
+  bf16x8* const aside_at = reinterpret_cast<bf16x8*>(smem + W::kBytes) + wave * kAside * 64 + lane;
 #pragma unroll
   for (int i = 0; i < kAside; ++i) aside_at[i * 64] = v[i].lo;
   const auto low = [&](int i) { return i < kAside ? aside_at[i * 64] : v[i].lo; };
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  for (int n = 0; n < count; ++n) {
-    pieces::wait_loads<0>();
-    pieces::barrier();
-    if (n + 1 < count) fetch(n + 1);
+  walk.run(load, [&](int n, uint32_t tile) {
     const int i0 = (from + n % tiles) * kTile;
-    if (j0 >= t.len || s.mask.none(i0, i0 + kTile - 1, j0, j1)) continue;
-    const uint32_t tile = st.lds + (n & 1) * St::kBytes;
+    if (j0 >= t.len || s.mask.none(i0, i0 + kTile - 1, j0, j1)) return;
     f32x16 x = product<DP, 3>(tile, k, lane), delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -407,12 +479,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
     const Frag3 ds[2] = {split_half(dp, 0), split_half(dp, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(tile + columns, b, ds);
-  }
+  });
+  if (!walk.template join<DP / 16>([&](int b) -> f32x16& { return b < DP / 32 ? dk[b] : dv[b - DP / 32]; })) return;
   if (kj >= t.len || (far && j0 >= s.mask.sinks)) return;
   float *to_k = a.dk, *to_v = a.dv;
   int64_t at = ((int64_t(t.start) + kj) * s.kv_heads + kv_head) * s.dim;
   if (far) {
-    to_k = far_at(a, chunk, far_block, kv_head, part), to_v = to_k + kBlock * s.dim;
+    to_k = far_at(a, chunk, far_block, kv_head, part), to_v = to_k + kRows * s.dim;
     at = int64_t(kj - b0) * s.dim;
   } else if (a.parts > 1) {
     to_k = a.dk_p, to_v = a.dv_p;
@@ -426,17 +499,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(DP <= 
   }
 }
 
-// What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of 128
+// What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of
 // keys times workgroups of a block, key heads, sequences or fewer).
 __global__ __launch_bounds__(kThreads) void far_kernel(const BwdArgs a) {
   const Shape& s = a.s;
-  const int per = gridDim.x / a.far_blocks, block = blockIdx.x / per, b0 = block * kBlock;
+  const int per = gridDim.x / a.far_blocks, block = blockIdx.x / per, b0 = block * a.block;
   const int i = (blockIdx.x - block * per) * kThreads + threadIdx.x;
   for (int seq = blockIdx.z; seq < s.seqs.count; seq += gridDim.z) {
     const int start = s.seqs.start(seq), len = max(0, s.seqs.start(seq + 1) - start);
     if (b0 >= len || near_last(a, b0, len) / kTile == (len - 1) / kTile) continue;  // no queries past the window
     const int from = (near_last(a, b0, len) / kTile + 1) * kTile / kChunk, to = (len - 1) / kChunk, base = start / kChunk + seq;
-    const int rows = min(min(kBlock, len - b0), (s.mask.sinks - b0 + kTile - 1) / kTile * kTile);
+    const int rows = min(min(a.block, len - b0), (s.mask.sinks - b0 + kTile - 1) / kTile * kTile);
     if (i >= rows * s.dim) continue;
     const int64_t at = ((int64_t(start) + b0 + i / s.dim) * s.kv_heads + blockIdx.y) * s.dim + i % s.dim;
     float k = a.dk ? a.dk[at] : 0.f, v = a.dv ? a.dv[at] : 0.f;
@@ -445,7 +518,7 @@ __global__ __launch_bounds__(kThreads) void far_kernel(const BwdArgs a) {
       for (int p = 0; p < a.parts; ++p) {
         const float* const sum = far_at(a, base + c, block, blockIdx.y, p) + i;
         if (a.dk) k += sum[0];
-        if (a.dv) v += sum[kBlock * s.dim];
+        if (a.dv) v += sum[a.block * s.dim];
       }
     if (a.dk) a.dk[at] = k;
     if (a.dv) a.dv[at] = v;
@@ -530,31 +603,13 @@ struct Buffers {
 
 // Blocks of keys that are seen past the window by workgroups of their own (of more first tokens
 // the blocks behind have as much to do as each other), and chunks of queries.
-int64_t far_blocks_of(const Shape& s) {
+int64_t far_blocks_of(const Shape& s, int block) {
   if (!s.mask.window || s.mask.window >= s.seqs.tokens) return 0;
-  return std::min<int64_t>((std::min(s.mask.sinks, s.seqs.tokens) + kBlock - 1) / kBlock, kFarBlocks);
+  return std::min<int64_t>((std::min(s.mask.sinks, s.seqs.tokens) + block - 1) / block, kFarBlocks);
 }
 int64_t chunks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kChunk); }
 
-Buffers carve(const Shape& s, bool backward, int parts, Carve& c) {
-  const int64_t tile = padded(s.dim) / 16 * 3 * 1024, q = tile * s.tiles * s.heads, k = tile * s.tiles * s.kv_heads;
-  Buffers b{};
-  b.kp = c.take<char>(k);
-  b.vp = c.take<char>(k);
-  if (!backward) return b;
-  b.qp = c.take<char>(q);
-  b.dp = c.take<char>(q);
-  b.stats = c.take<float>(int64_t(s.heads) * s.tiles * 256);
-  if (parts > 1) {
-    const int64_t part = (int64_t(parts) * s.seqs.tokens * s.kv_heads * s.dim * 4 + 255) / 256 * 256;
-    b.dk_p = c.take<float>(part);
-    b.dv_p = c.take<float>(part);
-  }
-  b.far = c.take<float>(chunks_of(s) * far_blocks_of(s) * s.kv_heads * parts * (2 * kBlock * int64_t(s.dim) * 4));
-  return b;
-}
-
-int64_t blocks_of(const Shape& s) { return sequence_tiles(s.seqs.tokens, s.seqs.count, kBlock); }
+int64_t blocks_of(const Shape& s, int rows = kBlock) { return sequence_tiles(s.seqs.tokens, s.seqs.count, rows); }
 
 // Parts that a key head's query heads are dealt into: as few as give every CU four
 // workgroups of 128 keys (the first keys of a sequence have the most to do).
@@ -564,11 +619,43 @@ int parts_of(const Shape& s) {
   return s.group;
 }
 
+// Whether workgroups of 128 rows, `blocks` in all, are so few that ones of 64 rows, which take two
+// tiles at a time (one workgroup a CU for LDS), end sooner.  Four sequences of 256, 12 heads of 64: 28, 34 and 39 us
+// for out, dq, and dk and dv with their packing, halved 23, 26 and 30; one of 8192, 4 heads of 64
+// 382, 495 and 647, halved 239, 290 and 384.  From about three workgroups a CU on dq, dk and dv take
+// as long either way (2 x 2048, 20 heads of 64: 222 and 299 us, halved 222 and 287; 4 x 2048, 14 of
+// 96: 481 and 615, halved 512 and 643).  Forward walks need two waves a SIMD sooner: 544 workgroups 154 us,
+// halved 144, 680 159 and 175; with a window, whose walks are alike, 272 36 and 40.
+bool halved(const Shape& s, int64_t blocks, bool forward) {
+  const bool alike = forward && s.mask.window && s.mask.window < s.seqs.tokens;
+  return s.dim <= 96 && blocks < int64_t(cu_count()) * (alike ? 1 : forward ? 2 : 3);
+}
+int key_block_of(const Shape& s) { return halved(s, blocks_of(s) * s.kv_heads * parts_of(s), false) ? kBlock / 2 : kBlock; }
+
+Buffers carve(const Shape& s, bool backward, Carve& c) {
+  const int64_t tile = padded(s.dim) / 16 * 3 * 1024, q = tile * s.tiles * s.heads, k = tile * s.tiles * s.kv_heads;
+  Buffers b{};
+  b.kp = c.take<char>(k);
+  b.vp = c.take<char>(k);
+  if (!backward) return b;
+  const int parts = parts_of(s), block = key_block_of(s);
+  b.qp = c.take<char>(q);
+  b.dp = c.take<char>(q);
+  b.stats = c.take<float>(int64_t(s.heads) * s.tiles * 256);
+  if (parts > 1) {
+    const int64_t part = (int64_t(parts) * s.seqs.tokens * s.kv_heads * s.dim * 4 + 255) / 256 * 256;
+    b.dk_p = c.take<float>(part);
+    b.dv_p = c.take<float>(part);
+  }
+  b.far = c.take<float>(chunks_of(s) * far_blocks_of(s, block) * s.kv_heads * parts * (2 * block * int64_t(s.dim) * 4));
+  return b;
+}
+
 int64_t workspace_bytes_of(const mx_attention_desc* d, bool backward) {
   if (d->tokens == 0 || d->heads == 0) return 0;
   Carve c{nullptr};
   const Shape s = shape_of(d);
-  carve(s, backward, backward ? parts_of(s) : 1, c);
+  carve(s, backward, c);
   return c.used;
 }
 
@@ -609,7 +696,7 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   Workspace ws;
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_bytes_of(d, false), st));
   Carve c{ws.as<char>()};
-  const Buffers b = carve(s, false, 1, c);
+  const Buffers b = carve(s, false, c);
   PackArgs p{};
   p.s = s;
   p.k = {k, d->k_token, d->k_head}, p.v = {v, d->v_token, d->v_head};
@@ -622,11 +709,16 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   with_dim(s.dim, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     const int64_t wide = sequence_tiles(s.seqs.tokens, s.seqs.count, 8 * kTile) * s.heads;
-      if (wide_blocks(wide)) {
-        hipLaunchKernelGGL((fwd_kernel<DP, 8>), dim3(unsigned(wide)), dim3(512), 0, st, f);
+    if (wide_blocks(wide)) {
+      hipLaunchKernelGGL((fwd_kernel<DP, 8, 1>), dim3(unsigned(wide)), dim3(512), 0, st, f);
+      return;
+    }
+    if constexpr (DP <= 96)
+      if (halved(s, blocks_of(s) * s.heads, true)) {
+        hipLaunchKernelGGL((fwd_kernel<DP, 4, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(256), 0, st, f);
         return;
       }
-    hipLaunchKernelGGL((fwd_kernel<DP, 4>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
+    hipLaunchKernelGGL((fwd_kernel<DP, 4, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
   });
   MX_LAUNCHED();
   return MX_OK;
@@ -647,29 +739,41 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   Workspace ws;
   MX_TRY(ws.take(who, workspace, workspace_bytes, workspace_bytes_of(d, true), st));
   Carve c{ws.as<char>()};
-  const int parts = parts_of(s);
-  const Buffers b = carve(s, true, parts, c);
+  const int parts = parts_of(s), block = key_block_of(s);
+  const Buffers b = carve(s, true, c);
   PackArgs p{};
   p.s = s;
   p.q = {q, d->q_token, d->q_head}, p.k = {k, d->k_token, d->k_head}, p.v = {v, d->v_token, d->v_head};
   p.dout = {dout, d->heads * d->head_dim, d->head_dim}, p.out = {out, d->heads * d->head_dim, d->head_dim};
   p.lse = lse;
   p.qp = b.qp, p.kp = b.kp, p.vp = b.vp, p.dp = b.dp, p.stats = b.stats;
-  const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p, int(blocks_of(s)), int(far_blocks_of(s)), b.far};
+  const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p, block, int(blocks_of(s, block)), int(far_blocks_of(s, block)), b.far};
   with_dim(s.dim, [&](auto dp) {
     hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
   if (dq) {
     with_dim(s.dim, [&](auto dp) {
-      hipLaunchKernelGGL((dq_kernel<decltype(dp)::value>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, g);
+      constexpr int DP = decltype(dp)::value;
+      if constexpr (DP <= 96)
+        if (halved(s, blocks_of(s) * s.heads, false)) {
+          hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(kThreads), 0, st, g);
+          return;
+        }
+      hipLaunchKernelGGL((dq_kernel<DP, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
   }
   if (dk || dv) {
     with_dim(s.dim, [&](auto dp) {
-      const int64_t blocks = blocks_of(s) + chunks_of(s) * far_blocks_of(s);
-      hipLaunchKernelGGL((dkv_kernel<decltype(dp)::value>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
+      constexpr int DP = decltype(dp)::value;
+      const int64_t blocks = g.near + chunks_of(s) * g.far_blocks;
+      if constexpr (DP <= 96)
+        if (block < kBlock) {
+          hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
+          return;
+        }
+      hipLaunchKernelGGL((dkv_kernel<DP, 1>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
     if (parts > 1) {
@@ -679,7 +783,7 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
       MX_LAUNCHED();
     }
     if (g.far_blocks) {
-      const int rows = std::min(kBlock, (std::min(s.mask.sinks, kBlock) + kTile - 1) / kTile * kTile);
+      const int rows = std::min(block, (std::min(s.mask.sinks, block) + kTile - 1) / kTile * kTile);
       const unsigned per = unsigned((rows * s.dim + kThreads - 1) / kThreads);
       hipLaunchKernelGGL(far_kernel, dim3(unsigned(g.far_blocks) * per, unsigned(s.kv_heads), unsigned(std::min(s.seqs.count, 4096))),
                          dim3(kThreads), 0, st, g);

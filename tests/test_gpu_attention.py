@@ -248,6 +248,8 @@ ATTENTION = [
     # first tokens seen from past the window: several chunks of queries, several blocks of keys
     ([2500, 31, 1100], 4, 2, 64, 40, 4), ([3100], 2, 1, 96, 200, 150), ([70, 1025, 400], 6, 2, 128, 1, 33), ([900, 900], 8, 1, 40, 600, 129),
     ([2300, 700], 2, 1, 32, 50, 700),  # more first tokens than are dealt out
+    # enough workgroups of 128 rows not to be halved
+    ([200, 33] * 250, 1, 1, 20, 40, 3), ([200, 33] * 250, 1, 1, 64, 0, 0), ([33, 200] * 250, 1, 1, 80, 100, 70),
    
     # enough rows for workgroups of eight waves
     ([2600, 1500], 64, 32, 32, 0, 0), ([4200], 64, 2, 128, 300, 2)]
