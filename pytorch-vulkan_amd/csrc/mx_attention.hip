@@ -241,10 +241,11 @@ struct FwdArgs {
 constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0; }
 
 // A wave's 32 queries stay in registers as pieces, with their sums.  Bound by the matrix
-// instructions: 16384 tokens, 16 heads of 64, window 4096 1340 us, 180 TFLOP/s, six piece products of which
-// are 1.08 PFLOP/s (a library's bf16 product of 8192^3 1.25 on this card); 2 x 2048, 16 heads of 128 250 us,
-// 137 TFLOP/s, where one wave a SIMD hides neither LDS's latency nor the softmax behind
-// products, and workgroups of eight waves, which do (4.5 us a tile of 256 rows for 3.7 of 128), have too
+// instructions: 16384 tokens, 16 heads of 64, window 4096 1290 us, 187 TFLOP/s, six piece products of which
+// are 1.12 PFLOP/s (a library's bf16 product of 8192^3 1.25 on this card); 2 x 2048, 16 heads of 128 207 us,
+// 166 TFLOP/s.  There a wave is alone on its SIMD, which hides neither LDS's latency nor the softmax
+// behind products unless those are another tile's: 250 us with a tile's scores and exponents in turn.
+// Workgroups of eight waves, two a SIMD (4.5 us a tile of 256 rows for 3.7 of 128 then), have too
 // uneven work (289 us).
 template <int DP, int WAVES, int SPLIT>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && (WAVES == 8 || DP <= 96) ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
@@ -261,10 +262,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
   const int b0 = t.index * kRows;
   const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
   const W walk{{lds_address(smem)}, wave, lane, keys.count};
-  const auto load = [&](int n, int stage) {
-    const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
-    walk.st.load(stage, a.kp + at, a.vp + at, nullptr, wave, lane);
-  };
+  // Waves alone on their SIMD take the next tile's scores between this one's exponents: keys are a step
+  // ahead of values.
+  constexpr bool kAhead = SPLIT > 1 || (DP == 128 && WAVES == 4);
+  const auto tile_of = [&](int n) { return keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>; };
+  const auto load = [&](int n, int stage) { walk.st.load(stage, a.kp + tile_of(n), a.vp + tile_of(n), nullptr, wave, lane); };
+  const auto load_keys = [&](int n, int stage) { walk.st.load_one(stage, false, a.kp + tile_of(n), wave, lane); };
+  const auto load_values = [&](int n, int stage) { walk.st.load_one(stage, true, a.vp + tile_of(n), wave, lane); };
   walk.fetch(0, load);
   const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
   Frag3 q[DP / 16];
@@ -276,11 +280,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
   f32x16 o[DP / 32] = {};
   float m = -__builtin_inff(), l = 0;  // of the exponents
   const uint32_t columns = column_base(lane);
-  walk.run(load, [&](int n, uint32_t tile) {
+  const auto seen = [&](int n) {
     const int j0 = keys.tile(n) * kTile;
-    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) return;
-    f32x16 x = product<DP, 3>(tile, q, lane, low);
+    return i0 < t.len && !s.mask.none(i0, i1, j0, j0 + kTile - 1);
+  };
+  const auto scores = [&](uint32_t tile) { return product<DP, 3>(tile, q, lane, low); };
+  const auto masked = [&](int n, f32x16& x) {
+    const int j0 = keys.tile(n) * kTile;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
+  };
+  const auto add = [&](f32x16& x, uint32_t tile) {
     float top = x[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
@@ -298,10 +307,45 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
-      if (DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
+      if (WAVES == 8 && DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
       o[b] = o[b] * keep + product_columns(tile + W::St::kSecond + columns, b, p);
     }
-  });
+  };
+  if constexpr (kAhead) {
+    pieces::wait_loads<0>();
+    pieces::barrier();
+    walk.fetch(1, load_keys);
+    f32x16 x{};
+    const auto at = [&](int n) { return walk.st.lds + ((n & 1) * SPLIT + walk.turn()) * W::St::kBytes; };
+    bool live = walk.turn() < keys.count && seen(walk.turn());
+    if (live) x = scores(at(0)), masked(walk.turn(), x);
+    for (int n = 0; n * SPLIT < keys.count; ++n) {
+      pieces::wait_loads<0>();
+      pieces::barrier();
+      walk.fetch(n + 2, load_keys);
+      walk.fetch(n + 1, load_values);
+      const int ahead = (n + 1) * SPLIT + walk.turn();
+      const bool next = ahead < keys.count && seen(ahead);
+      f32x16 y;
+      if (live) {
+        // (what lies there where no tile is left is not looked at)
+        y = scores(at(n + 1));
+        add(x, at(n));
+      } else {
+        asm volatile("");
+        y = scores(at(n + 1));
+      }
+      if (next) masked(ahead, y);
+      x = y, live = next;
+    }
+  } else {
+    walk.run(load, [&](int n, uint32_t tile) {
+      if (!seen(n)) return;
+      f32x16 x = scores(tile);
+      masked(n, x);
+      add(x, tile);
+    });
+  }
   if constexpr (SPLIT > 1) {
     // To the larger of both maxima, then the sums (l among them).
     float* const top = reinterpret_cast<float*>(smem) + wave * 64 + lane;

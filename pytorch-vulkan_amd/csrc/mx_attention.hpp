@@ -145,6 +145,17 @@ struct Stages {
     }
     if (wave < STATS) load_lds4(pieces::uniform(stats) + wave * 256, lane * 4, to + kStats + wave * 256);
   }
+  // One tensor's tile alone: the first, or the second.
+  __device__ __forceinline__ void load_one(int stage, bool second, const char* from, int wave, int lane) const {
+    const uint32_t to = lds + stage * kBytes + (second ? kSecond : 0);
+    const char* const p = pieces::uniform(from);
+    constexpr int F = DP / 16 * P;
+#pragma unroll
+    for (int i = 0; i < (F + WAVES - 1) / WAVES; ++i) {
+      const int f = wave + WAVES * i;
+      if (F % WAVES == 0 || f < F) pieces::load_lds16(p + f * 1024, lane * 16, to + f * 1024);
+    }
+  }
   // 4 bytes a lane from memory to LDS (as pieces::load_lds16).
   static __device__ __forceinline__ void load_lds4(const char* base, uint32_t lane_off, uint32_t at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(at), "v"(lane_off), "s"(base) : "memory");
