@@ -384,9 +384,10 @@ struct BwdArgs {
 
 // First tokens that stay visible are seen by every later query, other keys by a window's.
 // So that their workgroup is not the last by far, the queries past the window of its block are
-// dealt to workgroups of their own, chunks of 512 rows of a sequence, whose sums far_kernel
-// adds in order (8 sequences of up to 2048, window 512, 4 first tokens, 12 heads of 80: dk and dv
-// 270 us with them in the block's own workgroup, 243 + 7 so).
+// dealt to workgroups of their own, chunks of 512 rows of a sequence, which start first and whose sums
+// far_kernel adds in order (8 sequences of up to 2048, window 512, 4 first tokens, 12 heads of 80: a call
+// for dk and dv 217 us, 286 with chunks of 1024 rows that start last; the kernel alone took 270 with those
+// queries in the block's own workgroup, 243 with such chunks).
 constexpr int kChunk = 512, kFarBlocks = 4;
 __device__ __forceinline__ float* far_at(const BwdArgs& a, int chunk, int block, int kv_head, int part) {
   return a.far + (((int64_t(chunk) * a.far_blocks + block) * a.s.kv_heads + kv_head) * a.parts + part) * (2 * a.block * a.s.dim);
