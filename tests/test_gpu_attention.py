@@ -816,7 +816,16 @@ def test_calls_on_two_streams(mx):
             assert all(torch.equal(got[x], want[x]) for x in want)
 
 
-def test_attention_and_rotation_past_2_to_31_elements(mx):
+@pytest.fixture
+def returned(mx):
+    """What a large test took goes back to the card."""
+    yield
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    mx.check(mx.lib().mx_empty_cache())
+
+
+def test_attention_and_rotation_past_2_to_31_elements(mx, returned):
     """The last sequence of a batch of more than 2^31 elements has the bits that it has alone."""
     g, h, d, n = gen(16), 130, 128, 300
     t = (1 << 31) // (h * d) + 2 * n
@@ -842,7 +851,7 @@ def test_attention_and_rotation_past_2_to_31_elements(mx):
 
 
 @pytest.mark.parametrize("kind", ["i8", "f32"])
-def test_cache_past_2_to_31_elements(mx, kind):
+def test_cache_past_2_to_31_elements(mx, returned, kind):
     g, page, h, kv, d = gen(17), 64, 8, 4, 128
     pages = (1 << 31) // (page * kv * d) + 40
     make = lambda *s, dtype: torch.empty(*s, dtype=dtype, device="cuda")
