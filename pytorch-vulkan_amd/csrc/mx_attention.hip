@@ -182,32 +182,83 @@ __device__ __forceinline__ f32x16 get_block(uint32_t at, int b) {
   return v;
 }
 
-// A workgroup's walk over tiles, SPLIT of them at a time: of its four (or more) waves each SPLIT share
-// their rows, and take every SPLIT-th tile.
+// A workgroup's walk over tiles of two tensors, SPLIT of them at a time: of its four (or more) waves each
+// SPLIT share their rows, and take every SPLIT-th tile.  Both tensors' next tiles are loaded while these are
+// in use; where two stages of both do not fit LDS (kSingle), the second's are in one, and loaded
+// between its last use and the next step's first.
+struct Source {
+  const char *first, *second, *stats;
+};
+struct Staged {
+  uint32_t first, second, stats;
+};
 template <int DP, int WAVES, int SPLIT, int STATS>
 struct Walk {
   using St = Stages<DP, 3, WAVES, STATS>;
-  static constexpr int kGroups = WAVES / SPLIT, kRows = kGroups * kTile, kBytes = 2 * SPLIT * St::kBytes;
+  static constexpr bool kSingle = SPLIT > 1 && DP == 128;
+  static constexpr int kTensor = kTileBytes<DP>, kSlot = kSingle ? St::kBytes - kTensor : St::kBytes;
+  static constexpr int kGroups = WAVES / SPLIT, kRows = kGroups * kTile, kBytes = SPLIT * (2 * kSlot + (kSingle ? kTensor : 0));
   St st;
   int wave, lane, count;
   __device__ __forceinline__ int rows() const { return wave % kGroups * kTile; }
   __device__ __forceinline__ int turn() const { return wave / kGroups; }
-  // load(tile, stage) for each of step n's
+  // Where step n's tile of that turn lies.
+  __device__ __forceinline__ Staged at(int n, int turn) const {
+    const uint32_t first = st.lds + ((n & 1) * SPLIT + turn) * kSlot;
+    if (kSingle) return {first, st.lds + 2 * SPLIT * kSlot + turn * kTensor, first + kTensor};
+    return {first, first + kTensor, first + 2 * kTensor};
+  }
+  // load(tile, its place) for each of step n's
   template <class F>
   __device__ __forceinline__ void fetch(int n, F&& load) const {
 #pragma unroll
     for (int u = 0; u < SPLIT; ++u)
-      if (n * SPLIT + u < count) load(n * SPLIT + u, (n & 1) * SPLIT + u);
+      if (n * SPLIT + u < count) load(n * SPLIT + u, at(n, u));
   }
-  // take(tile, its address in LDS) for each of the wave's, the next ones on their way
-  template <class F, class G>
-  __device__ __forceinline__ void run(F&& load, G&& take) const {
+  // Both tensors' of step n from source(tile), the second's later where it is staged once.
+  template <class F>
+  __device__ __forceinline__ void fetch_both(int n, F&& source) const {
+    fetch(n, [&](int tile, const Staged& to) {
+      const Source s = source(tile);
+      if constexpr (kSingle) {
+        St::load_one(to.first, s.first, wave, lane);
+        St::load_stats(to.stats, s.stats, wave, lane);
+      } else {
+        const St slot{to.first};
+        slot.load(0, s.first, s.second, s.stats, wave, lane);
+      }
+    });
+  }
+  template <class F>
+  __device__ __forceinline__ void fetch_second(int n, F&& source) const {
+    fetch(n, [&](int tile, const Staged& to) { St::load_one(to.second, source(tile).second, wave, lane); });
+  }
+  template <class F>
+  __device__ __forceinline__ void start(F&& source) const {
+    fetch_both(0, source);
+    if constexpr (kSingle) fetch_second(0, source);
+  }
+  // use(tile, at), then finish(tile, at), which does not read the second tensor, for each of the wave's
+  // tiles that it sees.
+  template <class F, class S, class U, class V>
+  __device__ __forceinline__ void run(F&& source, S&& seen, U&& use, V&& finish) const {
     for (int n = 0; n * SPLIT < count; ++n) {
       pieces::wait_loads<0>();
       pieces::barrier();
-      fetch(n + 1, load);
+      fetch_both(n + 1, source);
       const int mine = n * SPLIT + turn();
-      if (SPLIT == 1 || mine < count) take(mine, st.lds + ((n & 1) * SPLIT + turn()) * St::kBytes);
+      const Staged here = at(n, turn());
+      if constexpr (kSingle) {
+        const bool on = mine < count && seen(mine);
+        if (on) use(mine, here);
+        pieces::barrier();
+        fetch_second(n + 1, source);
+        if (on) finish(mine, here);
+      } else {
+        if ((SPLIT > 1 && mine >= count) || !seen(mine)) continue;
+        use(mine, here);
+        finish(mine, here);
+      }
     }
   }
   // Behind the walk: adds what the waves that share rows have (BLOCKS blocks) to the first one's,
@@ -262,14 +313,14 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
   const int b0 = t.index * kRows;
   const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
   const W walk{{lds_address(smem)}, wave, lane, keys.count};
-  // Waves alone on their SIMD take the next tile's scores between this one's exponents: keys are a step
-  // ahead of values.
-  constexpr bool kAhead = SPLIT > 1 || (DP == 128 && WAVES == 4);
-  const auto tile_of = [&](int n) { return keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>; };
-  const auto load = [&](int n, int stage) { walk.st.load(stage, a.kp + tile_of(n), a.vp + tile_of(n), nullptr, wave, lane); };
-  const auto load_keys = [&](int n, int stage) { walk.st.load_one(stage, false, a.kp + tile_of(n), wave, lane); };
-  const auto load_values = [&](int n, int stage) { walk.st.load_one(stage, true, a.vp + tile_of(n), wave, lane); };
-  walk.fetch(0, load);
+  // Waves alone on their SIMD take the next tile's scores between this one's exponents, keys a step
+  // ahead of values, unless one of them is staged once (the keys, which are done with first).
+  constexpr bool kAhead = !W::kSingle && (SPLIT > 1 || (DP == 128 && WAVES == 4));
+  const auto source = [&](int n) {
+    const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
+    return W::kSingle ? Source{a.vp + at, a.kp + at} : Source{a.kp + at, a.vp + at};
+  };
+  walk.start(source);
   const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
   Frag3 q[DP / 16];
   own_rows<DP>(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
@@ -289,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
     const int j0 = keys.tile(n) * kTile;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
   };
-  const auto add = [&](f32x16& x, uint32_t tile) {
+  const auto add = [&](f32x16& x, uint32_t values) {
     float top = x[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
@@ -308,43 +359,42 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) {
       if (WAVES == 8 && DP > 96) __builtin_amdgcn_sched_barrier(0);  // one block's fragments at a time
-      o[b] = o[b] * keep + product_columns(tile + W::St::kSecond + columns, b, p);
+      o[b] = o[b] * keep + product_columns(values + columns, b, p);
     }
   };
   if constexpr (kAhead) {
     pieces::wait_loads<0>();
     pieces::barrier();
+    const auto load_keys = [&](int n, const Staged& to) { W::St::load_one(to.first, source(n).first, wave, lane); };
     walk.fetch(1, load_keys);
     f32x16 x{};
-    const auto at = [&](int n) { return walk.st.lds + ((n & 1) * SPLIT + walk.turn()) * W::St::kBytes; };
+    const auto at = [&](int n) { return walk.at(n, walk.turn()); };
     bool live = walk.turn() < keys.count && seen(walk.turn());
-    if (live) x = scores(at(0)), masked(walk.turn(), x);
+    if (live) x = scores(at(0).first), masked(walk.turn(), x);
     for (int n = 0; n * SPLIT < keys.count; ++n) {
       pieces::wait_loads<0>();
       pieces::barrier();
       walk.fetch(n + 2, load_keys);
-      walk.fetch(n + 1, load_values);
+      walk.fetch_second(n + 1, source);
       const int ahead = (n + 1) * SPLIT + walk.turn();
       const bool next = ahead < keys.count && seen(ahead);
       f32x16 y;
       if (live) {
         // (what lies there where no tile is left is not looked at)
-        y = scores(at(n + 1));
-        add(x, at(n));
+        y = scores(at(n + 1).first);
+        add(x, at(n).second);
       } else {
         asm volatile("");
-        y = scores(at(n + 1));
+        y = scores(at(n + 1).first);
       }
       if (next) masked(ahead, y);
       x = y, live = next;
     }
   } else {
-    walk.run(load, [&](int n, uint32_t tile) {
-      if (!seen(n)) return;
-      f32x16 x = scores(tile);
-      masked(n, x);
-      add(x, tile);
-    });
+    f32x16 x;
+    walk.run(
+        source, seen, [&](int n, const Staged& at) { x = scores(W::kSingle ? at.second : at.first), masked(n, x); },
+        [&](int, const Staged& at) { add(x, W::kSingle ? at.first : at.second); });
   }
   if constexpr (SPLIT > 1) {
     // To the larger of both maxima, then the sums (l among them).
@@ -417,11 +467,11 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   const int b0 = t.index * kRows;
   const KeyTiles<> keys(s.mask, b0, min(b0 + kRows, t.len) - 1);
   const W walk{{lds_address(smem)}, wave, lane, keys.count};
-  const auto load = [&](int n, int stage) {
+  const auto source = [&](int n) {
     const int64_t at = keys0 + int64_t(keys.tile(n)) * kTileBytes<DP>;
-    walk.st.load(stage, a.kp + at, a.vp + at, nullptr, wave, lane);
+    return Source{a.kp + at, a.vp + at};
   };
-  walk.fetch(0, load);
+  walk.start(source);
   const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
   // A wave past the sequence's end repeats its last tile, and stores nothing.
   const int mine = base32 + min(i0, t.len - 1) / kTile;
@@ -432,17 +482,23 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   const float lse = stat[0], delta = stat[32];
   f32x16 dq[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  walk.run(load, [&](int n, uint32_t tile) {
+  Frag3 ds[2];
+  const auto seen = [&](int n) {
     const int j0 = keys.tile(n) * kTile;
-    if (i0 >= t.len || s.mask.none(i0, i1, j0, j0 + kTile - 1)) return;
-    f32x16 x = product<DP, 3>(tile, q, lane) - lse;
+    return i0 < t.len && !s.mask.none(i0, i1, j0, j0 + kTile - 1);
+  };
+  const auto use = [&](int n, const Staged& at) {
+    const int j0 = keys.tile(n) * kTile;
+    f32x16 x = product<DP, 3>(at.first, q, lane) - lse;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
-    const f32x16 dp = product<DP, 3>(tile + W::St::kSecond, g, lane);
+    const f32x16 dp = product<DP, 3>(at.second, g, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
-    const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
+    ds[0] = split_half(x, 0), ds[1] = split_half(x, 1);
+  };
+  walk.run(source, seen, use, [&](int, const Staged& at) {
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(tile + columns, b, p);
+    for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(at.first + columns, b, ds);
   });
   if (!walk.template join<DP / 32>([&](int b) -> f32x16& { return dq[b]; }) || qi >= t.len) return;
 #pragma unroll
@@ -455,7 +511,6 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
 template <int DP, int SPLIT>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
   using W = Walk<DP, 4, SPLIT, 1>;
-  using St = typename W::St;
   constexpr int kRows = W::kRows;
   constexpr int kAside = SPLIT == 1 && DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
   __shared__ __attribute__((aligned(1024))) char smem[W::kBytes + kAside * 4 * 1024];
@@ -481,12 +536,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT 
   if (tiles <= 0) return;
   const int heads = s.group / a.parts, head0 = kv_head * s.group + part * heads, count = heads * tiles;
   const W walk{{lds_address(smem)}, wave, lane, count};
-  const auto load = [&](int n, int stage) {
+  const auto source = [&](int n) {
     const int head = head0 + n / tiles, tile = base32 + from + n % tiles;
     const int64_t at = tile_at<DP>(s, head, tile);
-    walk.st.load(stage, a.qp + at, a.dp + at, reinterpret_cast<const char*>(a.stats + (int64_t(head) * s.tiles + tile) * 64), wave, lane);
+    return Source{a.qp + at, a.dp + at, reinterpret_cast<const char*>(a.stats + (int64_t(head) * s.tiles + tile) * 64)};
   };
-  walk.fetch(0, load);
+  walk.start(source);
   const int j0 = b0 + walk.rows(), j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
   const int64_t mine = tile_at<DP>(s, kv_head, base32 + min(j0, t.len - 1) / kTile);
   Frag3 k[DP / 16], v[DP / 16];
@@ -498,32 +553,36 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT 
   const auto low = [&](int i) { return i < kAside ? aside_at[i * 64] : v[i].lo; };
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  walk.run(load, [&](int n, uint32_t tile) {
+  Frag3 ds[2];
+  const auto seen = [&](int n) {
     const int i0 = (from + n % tiles) * kTile;
-    if (j0 >= t.len || s.mask.none(i0, i0 + kTile - 1, j0, j1)) return;
-    f32x16 x = product<DP, 3>(tile, k, lane), delta;
+    return j0 < t.len && !s.mask.none(i0, i0 + kTile - 1, j0, j1);
+  };
+  const auto use = [&](int n, const Staged& at) {
+    const int i0 = (from + n % tiles) * kTile;
+    f32x16 x = product<DP, 3>(at.first, k, lane), delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t at = tile + St::kStats + (16 * h + 4 * i) * 4;
-      const f32x4 lse = *pieces::lds_at<const f32x4>(at), d = *pieces::lds_at<const f32x4>(at + 128);
+      const uint32_t stats = at.stats + (16 * h + 4 * i) * 4;
+      const f32x4 lse = *pieces::lds_at<const f32x4>(stats), d = *pieces::lds_at<const f32x4>(stats + 128);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[4 * i + e] -= lse[e], delta[4 * i + e] = d[e];
     }
     if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) hide(x, [&](int r) { return s.mask.sees(i0 + 16 * h + r, kj); });
-    f32x16 dp = product<DP, 3>(tile + St::kSecond, v, lane, low);
+    f32x16 dp = product<DP, 3>(at.second, v, lane, low);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = exp2_(x[r]);
       dp[r] = times(x[r], dp[r] - delta[r]);
     }
-    {
-      const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
+    const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) dv[b] += product_columns(tile + St::kSecond + columns, b, p);
-    }
-    const Frag3 ds[2] = {split_half(dp, 0), split_half(dp, 1)};
+    for (int b = 0; b < DP / 32; ++b) dv[b] += product_columns(at.second + columns, b, p);
+    ds[0] = split_half(dp, 0), ds[1] = split_half(dp, 1);
+  };
+  walk.run(source, seen, use, [&](int, const Staged& at) {
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(tile + columns, b, ds);
+    for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(at.first + columns, b, ds);
   });
   if (!walk.template join<DP / 16>([&](int b) -> f32x16& { return b < DP / 32 ? dk[b] : dv[b - DP / 32]; })) return;
   if (kj >= t.len || (far && j0 >= s.mask.sinks)) return;
@@ -666,14 +725,15 @@ int parts_of(const Shape& s) {
 
 // Whether workgroups of 128 rows, `blocks` in all, are so few that ones of 64 rows, which take two
 // tiles at a time (one workgroup a CU for LDS), end sooner.  Four sequences of 256, 12 heads of 64: 28, 34 and 39 us
-// for out, dq, and dk and dv with their packing, halved 23, 26 and 30; one of 8192, 4 heads of 64
-// 382, 495 and 647, halved 239, 290 and 384.  From about three workgroups a CU on dq, dk and dv take
+// for out, dq, and dk and dv with their packing, halved 23, 26 and 30; one of 2048, 8 heads of 128
+// 160, 245 and 329, halved 108, 134 and 187.  From about three workgroups a CU on dq, dk and dv take
 // as long either way (2 x 2048, 20 heads of 64: 222 and 299 us, halved 222 and 287; 4 x 2048, 14 of
-// 96: 481 and 615, halved 512 and 643).  Forward walks need two waves a SIMD sooner: 544 workgroups 154 us,
-// halved 144, 680 159 and 175; with a window, whose walks are alike, 272 36 and 40.
+// 96: 481 and 615, halved 512 and 643).  Forward walks gain less: two waves a SIMD, or for heads of 128
+// scores ahead, go without (544 workgroups of 64 154 us, halved 144, 680 159 and 175; of 128, 320 68 and
+// 68, 544 209 and 237); with a window, whose walks are alike, 272 of 64 36 and 40.
 bool halved(const Shape& s, int64_t blocks, bool forward) {
-  const bool alike = forward && s.mask.window && s.mask.window < s.seqs.tokens;
-  return s.dim <= 96 && blocks < int64_t(cu_count()) * (alike ? 1 : forward ? 2 : 3);
+  const bool alike = s.mask.window && s.mask.window < s.seqs.tokens;
+  return blocks < int64_t(cu_count()) * (!forward ? 3 : alike || s.dim > 96 ? 1 : 2);
 }
 int key_block_of(const Shape& s) { return halved(s, blocks_of(s) * s.kv_heads * parts_of(s), false) ? kBlock / 2 : kBlock; }
 
@@ -758,11 +818,10 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
       hipLaunchKernelGGL((fwd_kernel<DP, 8, 1>), dim3(unsigned(wide)), dim3(512), 0, st, f);
       return;
     }
-    if constexpr (DP <= 96)
-      if (halved(s, blocks_of(s) * s.heads, true)) {
-        hipLaunchKernelGGL((fwd_kernel<DP, 4, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(256), 0, st, f);
-        return;
-      }
+    if (halved(s, blocks_of(s) * s.heads, true)) {
+      hipLaunchKernelGGL((fwd_kernel<DP, 4, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(256), 0, st, f);
+      return;
+    }
     hipLaunchKernelGGL((fwd_kernel<DP, 4, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
   });
   MX_LAUNCHED();
@@ -800,11 +859,10 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   if (dq) {
     with_dim(s.dim, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      if constexpr (DP <= 96)
-        if (halved(s, blocks_of(s) * s.heads, false)) {
-          hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(kThreads), 0, st, g);
-          return;
-        }
+      if (halved(s, blocks_of(s) * s.heads, false)) {
+        hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(kThreads), 0, st, g);
+        return;
+      }
       hipLaunchKernelGGL((dq_kernel<DP, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
@@ -813,11 +871,10 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
     with_dim(s.dim, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
       const int64_t blocks = g.near + chunks_of(s) * g.far_blocks;
-      if constexpr (DP <= 96)
-        if (block < kBlock) {
-          hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
-          return;
-        }
+      if (block < kBlock) {
+        hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
+        return;
+      }
       hipLaunchKernelGGL((dkv_kernel<DP, 1>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();

@@ -143,11 +143,10 @@ struct Stages {
       const int f = wave + WAVES * i;  // a's fragments, then b's
       if (2 * F % WAVES == 0 || f < 2 * F) pieces::load_lds16(f < F ? pa + f * 1024 : pb + (f - F) * 1024, lane * 16, to + f * 1024);
     }
-    if (wave < STATS) load_lds4(pieces::uniform(stats) + wave * 256, lane * 4, to + kStats + wave * 256);
+    load_stats(to + kStats, stats, wave, lane);
   }
-  // One tensor's tile alone: the first, or the second.
-  __device__ __forceinline__ void load_one(int stage, bool second, const char* from, int wave, int lane) const {
-    const uint32_t to = lds + stage * kBytes + (second ? kSecond : 0);
+  // One tensor's tile alone.
+  static __device__ __forceinline__ void load_one(uint32_t to, const char* from, int wave, int lane) {
     const char* const p = pieces::uniform(from);
     constexpr int F = DP / 16 * P;
 #pragma unroll
@@ -155,6 +154,9 @@ struct Stages {
       const int f = wave + WAVES * i;
       if (F % WAVES == 0 || f < F) pieces::load_lds16(p + f * 1024, lane * 16, to + f * 1024);
     }
+  }
+  static __device__ __forceinline__ void load_stats(uint32_t to, const char* stats, int wave, int lane) {
+    if (wave < STATS) load_lds4(pieces::uniform(stats) + wave * 256, lane * 4, to + wave * 256);
   }
   // 4 bytes a lane from memory to LDS (as pieces::load_lds16).
   static __device__ __forceinline__ void load_lds4(const char* base, uint32_t lane_off, uint32_t at) {

@@ -250,6 +250,7 @@ ATTENTION = [
     ([2300, 700], 2, 1, 32, 50, 700),  # more first tokens than are dealt out
     # enough workgroups of 128 rows not to be halved
     ([200, 33] * 250, 1, 1, 20, 40, 3), ([200, 33] * 250, 1, 1, 64, 0, 0), ([33, 200] * 250, 1, 1, 80, 100, 70),
+    ([200, 33] * 250, 1, 1, 128, 0, 0), ([33, 200] * 250, 1, 1, 100, 50, 4), ([900, 40, 311], 6, 2, 112, 0, 0), ([777, 64], 2, 1, 128, 300, 5),
    
     # enough rows for workgroups of eight waves
     ([2600, 1500], 64, 32, 32, 0, 0), ([4200], 64, 2, 128, 300, 2)]
@@ -826,7 +827,7 @@ def returned(mx):
 
 
 def test_attention_and_rotation_past_2_to_31_elements(mx, returned):
-    """The last sequence of a batch of more than 2^31 elements has the bits that it has alone."""
+    """The last sequence of a batch of more than 2^31 elements."""
     g, h, d, n = gen(16), 130, 128, 300
     t = (1 << 31) // (h * d) + 2 * n
     tail = [rand(g, n, h, d) for _ in range(4)]
@@ -844,10 +845,9 @@ def test_attention_and_rotation_past_2_to_31_elements(mx, returned):
     mx.attention_forward(q, k, v, out, starts=starts, lse=lse, workspace=scratch, stream=stream(), **form)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
     mx.attention_backward(do, q, k, v, out, lse, dq, dk, dv, starts=starts, workspace=scratch, stream=stream(), **form)
-    alone = run_attention(mx, *tail, None, **form)
-    for name, x in dict(out=out, dq=dq, dk=dk, dv=dv).items():
-        assert torch.equal(x[-n:], alone[name]), name
-    assert torch.equal(lse[:, -n:], alone["lse"])
+    got = dict(out=out[-n:], lse=lse[:, -n:], dq=dq[-n:], dk=dk[-n:], dv=dv[-n:])
+    for name, (ref, bound) in attention_ref(*tail, 33, 2, d ** -0.5).items():
+        within(got[name], ref, bound + 1e-30, name)
 
 
 @pytest.mark.parametrize("kind", ["i8", "f32"])
