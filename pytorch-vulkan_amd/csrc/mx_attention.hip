@@ -192,6 +192,9 @@ struct Source {
 struct Staged {
   uint32_t first, second, stats;
 };
+struct Halves {
+  Frag3 of[2];
+};
 template <int DP, int WAVES, int SPLIT, int STATS>
 struct Walk {
   using St = Stages<DP, 3, WAVES, STATS>;
@@ -238,8 +241,8 @@ struct Walk {
     fetch_both(0, source);
     if constexpr (kSingle) fetch_second(0, source);
   }
-  // use(tile, at), then finish(tile, at), which does not read the second tensor, for each of the wave's
-  // tiles that it sees.
+  // use(tile, at), then finish(at, what that gave), which does not read the second tensor, for each of the
+  // wave's tiles that it sees.
   template <class F, class S, class U, class V>
   __device__ __forceinline__ void run(F&& source, S&& seen, U&& use, V&& finish) const {
     for (int n = 0; n * SPLIT < count; ++n) {
@@ -250,14 +253,15 @@ struct Walk {
       const Staged here = at(n, turn());
       if constexpr (kSingle) {
         const bool on = mine < count && seen(mine);
-        if (on) use(mine, here);
+        std::remove_const_t<decltype(use(mine, here))> x;
+        if (on) x = use(mine, here);
         pieces::barrier();
         fetch_second(n + 1, source);
-        if (on) finish(mine, here);
+        if (on) finish(here, x);
       } else {
         if ((SPLIT > 1 && mine >= count) || !seen(mine)) continue;
-        use(mine, here);
-        finish(mine, here);
+        auto x = use(mine, here);
+        finish(here, x);
       }
     }
   }
@@ -391,10 +395,12 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
       x = y, live = next;
     }
   } else {
-    f32x16 x;
-    walk.run(
-        source, seen, [&](int n, const Staged& at) { x = scores(W::kSingle ? at.second : at.first), masked(n, x); },
-        [&](int, const Staged& at) { add(x, W::kSingle ? at.first : at.second); });
+    const auto use = [&](int n, const Staged& at) {
+      f32x16 x = scores(W::kSingle ? at.second : at.first);
+      masked(n, x);
+      return x;
+    };
+    walk.run(source, seen, use, [&](const Staged& at, f32x16& x) { add(x, W::kSingle ? at.first : at.second); });
   }
   if constexpr (SPLIT > 1) {
     // To the larger of both maxima, then the sums (l among them).
@@ -450,16 +456,21 @@ __device__ __forceinline__ int near_last(const BwdArgs& a, int b0, int len) {
   return all ? len - 1 : min(len - 1, b0 + a.block - 1 + min(m.window, len) - 1);
 }
 
-// Three products of a tile, two of them computed again by dkv_kernel: the scores' gradients would be
-// 6 bytes a pair in memory.  318 us for 2 x 2048, 16 heads of 128: 162 TFLOP/s, 0.97 PFLOP/s of pieces.
+// Three products of a tile, two of them computed again for dk and dv: the scores' gradients would be
+// 6 bytes a pair in memory.  2 x 2048, 16 heads of 128: 280 us alone, 168 TFLOP/s, 1.0 PFLOP/s of pieces.
+// (workgroup `index` of `count`)
 template <int DP, int SPLIT>
-__global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
+struct Dq {
   using W = Walk<DP, 4, SPLIT, 0>;
+  static constexpr int kBytes = W::kBytes;
+  static __device__ void run(const BwdArgs a, char* smem, int index, int count);
+};
+template <int DP, int SPLIT>
+__device__ __forceinline__ void Dq<DP, SPLIT>::run(const BwdArgs a, char* smem, int index, int count) {
   constexpr int kRows = W::kRows;
-  __shared__ __attribute__((aligned(1024))) char smem[W::kBytes];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int head = blockIdx.x % s.heads, block = gridDim.x / s.heads - 1 - blockIdx.x / s.heads;
+  const int head = index % s.heads, block = count / s.heads - 1 - index / s.heads;
   SequenceTile t;
   if (!locate<kRows>(s.seqs, block, t) || t.index * kRows >= t.len) return;
   const int base32 = t.start / kTile + t.seq;
@@ -482,7 +493,6 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
   const float lse = stat[0], delta = stat[32];
   f32x16 dq[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  Frag3 ds[2];
   const auto seen = [&](int n) {
     const int j0 = keys.tile(n) * kTile;
     return i0 < t.len && !s.mask.none(i0, i1, j0, j0 + kTile - 1);
@@ -494,11 +504,11 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     const f32x16 dp = product<DP, 3>(at.second, g, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
-    ds[0] = split_half(x, 0), ds[1] = split_half(x, 1);
+    return Halves{{split_half(x, 0), split_half(x, 1)}};
   };
-  walk.run(source, seen, use, [&](int, const Staged& at) {
+  walk.run(source, seen, use, [&](const Staged& at, const Halves& ds) {
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(at.first + columns, b, ds);
+    for (int b = 0; b < DP / 32; ++b) dq[b] += product_columns(at.first + columns, b, ds.of);
   });
   if (!walk.template join<DP / 32>([&](int b) -> f32x16& { return dq[b]; }) || qi >= t.len) return;
 #pragma unroll
@@ -506,19 +516,29 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const BwdArgs a) {
     store_block(a.dq + ((int64_t(t.start) + qi) * s.heads + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
 }
 
-// Four products of a tile, the scores straight (a lane has 16 queries of a key), so that both sums run
-// along what a lane holds.  416 us for 2 x 2048, 16 heads of 128: 165 TFLOP/s, 0.99 PFLOP/s of pieces.
 template <int DP, int SPLIT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dq_kernel(const BwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[Dq<DP, SPLIT>::kBytes];
+  Dq<DP, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
+}
+
+// Four products of a tile, the scores straight (a lane has 16 queries of a key), so that both sums run
+// along what a lane holds.  380 us alone for 2 x 2048, 16 heads of 128: 165 TFLOP/s.
+template <int DP, int SPLIT>
+struct Dkv {
   using W = Walk<DP, 4, SPLIT, 1>;
+  static constexpr int kAside = SPLIT == 1 && DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
+  static constexpr int kBytes = W::kBytes + kAside * 4 * 1024;
+  static __device__ void run(const BwdArgs a, char* smem, int number, int workgroups);
+};
+template <int DP, int SPLIT>
+__device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem, int number, int workgroups) {
   constexpr int kRows = W::kRows;
-  constexpr int kAside = SPLIT == 1 && DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
-  __shared__ __attribute__((aligned(1024))) char smem[W::kBytes + kAside * 4 * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  const int across = s.kv_heads * a.parts, kv_head = blockIdx.x % across / a.parts, part = blockIdx.x % across % a.parts;
+  const int across = s.kv_heads * a.parts, kv_head = number % across / a.parts, part = number % across % a.parts;
   // (those first, which have the most to do)
-  const int index = blockIdx.x / across, block = index - (gridDim.x / across - a.near);
+  const int index = number / across, block = index - (workgroups / across - a.near);
   const bool far = block < 0;
   const int chunk = far ? index / a.far_blocks : 0, far_block = far ? index % a.far_blocks : 0;
   SequenceTile t;
@@ -553,7 +573,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT 
   const auto low = [&](int i) { return i < kAside ? aside_at[i * 64] : v[i].lo; };
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   const uint32_t columns = column_base(lane);
-  Frag3 ds[2];
   const auto seen = [&](int n) {
     const int i0 = (from + n % tiles) * kTile;
     return j0 < t.len && !s.mask.none(i0, i0 + kTile - 1, j0, j1);
@@ -578,11 +597,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT 
     const Frag3 p[2] = {split_half(x, 0), split_half(x, 1)};
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b) dv[b] += product_columns(at.second + columns, b, p);
-    ds[0] = split_half(dp, 0), ds[1] = split_half(dp, 1);
+    return Halves{{split_half(dp, 0), split_half(dp, 1)}};
   };
-  walk.run(source, seen, use, [&](int, const Staged& at) {
+  walk.run(source, seen, use, [&](const Staged& at, const Halves& ds) {
 #pragma unroll
-    for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(at.first + columns, b, ds);
+    for (int b = 0; b < DP / 32; ++b) dk[b] += product_columns(at.first + columns, b, ds.of);
   });
   if (!walk.template join<DP / 16>([&](int b) -> f32x16& { return b < DP / 32 ? dk[b] : dv[b - DP / 32]; })) return;
   if (kj >= t.len || (far && j0 >= s.mask.sinks)) return;
@@ -601,6 +620,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT 
     if (a.dk) store_block(to_k + at, dk[b] * kLn2, b, h, s.dim);
     if (a.dv) store_block(to_v + at, dv[b], b, h, s.dim);
   }
+}
+template <int DP, int SPLIT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[Dkv<DP, SPLIT>::kBytes];
+  Dkv<DP, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
+}
+// Both, where workgroups are few: `first` of dk and dv, then those of dq, which fill the CUs that the others
+// leave.  Calls with packing, in two launches and in one: 4 x 256, 12 heads of 64 46 and 38 us, 2048, 8 heads
+// of 128 301 and 192, 2 x 2048, 16 heads of 128 716 and 711 (184 TFLOP/s without packing and the join, 1.1
+// PFLOP/s of pieces).
+template <int DP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void both_kernel(const BwdArgs a, int first) {
+  __shared__ __attribute__((aligned(1024))) char smem[std::max(Dkv<DP, 2>::kBytes, Dq<DP, 2>::kBytes)];
+  if (int(blockIdx.x) < first) Dkv<DP, 2>::run(a, smem, blockIdx.x, first);
+  else Dq<DP, 2>::run(a, smem, blockIdx.x - first, gridDim.x - first);
 }
 
 // What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of
@@ -856,28 +890,32 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
     hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
-  if (dq) {
+  const bool keys = dk || dv, key_halves = block < kBlock, query_halves = halved(s, blocks_of(s) * s.heads, false);
+  const unsigned of_keys = unsigned((g.near + chunks_of(s) * g.far_blocks) * s.kv_heads * parts);
+  const unsigned of_queries = unsigned(blocks_of(s, query_halves ? kBlock / 2 : kBlock) * s.heads);
+  const bool both = dq && keys && key_halves && query_halves;
+  if (both) {
+    with_dim(s.dim, [&](auto dp) {
+      hipLaunchKernelGGL((both_kernel<decltype(dp)::value>), dim3(of_keys + of_queries), dim3(kThreads), 0, st, g, int(of_keys));
+    });
+    MX_LAUNCHED();
+  } else if (dq) {
     with_dim(s.dim, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      if (halved(s, blocks_of(s) * s.heads, false)) {
-        hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(kThreads), 0, st, g);
-        return;
-      }
-      hipLaunchKernelGGL((dq_kernel<DP, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(kThreads), 0, st, g);
+      if (query_halves) hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(of_queries), dim3(kThreads), 0, st, g);
+      else hipLaunchKernelGGL((dq_kernel<DP, 1>), dim3(of_queries), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
   }
-  if (dk || dv) {
-    with_dim(s.dim, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value;
-      const int64_t blocks = g.near + chunks_of(s) * g.far_blocks;
-      if (block < kBlock) {
-        hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
-        return;
-      }
-      hipLaunchKernelGGL((dkv_kernel<DP, 1>), dim3(unsigned(blocks * s.kv_heads * parts)), dim3(kThreads), 0, st, g);
-    });
-    MX_LAUNCHED();
+  if (keys) {
+    if (!both) {
+      with_dim(s.dim, [&](auto dp) {
+        constexpr int DP = decltype(dp)::value;
+        if (key_halves) hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(of_keys), dim3(kThreads), 0, st, g);
+        else hipLaunchKernelGGL((dkv_kernel<DP, 1>), dim3(of_keys), dim3(kThreads), 0, st, g);
+      });
+      MX_LAUNCHED();
+    }
     if (parts > 1) {
       const int64_t fours = (d->tokens * d->kv_heads * d->head_dim + 3) / 4;
       const unsigned blocks = unsigned(std::min<int64_t>((fours + kThreads - 1) / kThreads, int64_t(cu_count()) * 8));
