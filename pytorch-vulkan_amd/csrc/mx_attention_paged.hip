@@ -77,7 +77,7 @@ struct Place {
 template <int DP, bool I8>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void paged_kernel(const PagedArgs a) {
   constexpr int kUnits = DP / 64, kBlocks = DP / 16, kPitch = DP + 4;
-  __shared__ float stat[2][kWaves][kRows], sum[kRows][kPitch];
+  __shared__ __attribute__((aligned(16))) float stat[2][kWaves][kRows], sum[kWaves][kRows][kPitch];
   using E = std::conditional_t<I8, int8_t, float>;
   const Cache& c = a.c;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
@@ -241,42 +241,38 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  // ---- the workgroup's waves, in order
+  // ---- the workgroup's waves, in order: 16 threads a row
   if (g == 0) stat[0][wave][col] = m, stat[1][wave][col] = l;
-  __syncthreads();
-  float all = -__builtin_inff(), total = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, stat[0][w][col]);
-  const float base = all == -__builtin_inff() ? 0.f : all;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) total = fmaf(stat[1][w][col], exp2_(stat[0][w][col] - base), total);
-  const float mul = exp2_(m - base);
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        f32x4* const to = reinterpret_cast<f32x4*>(&sum[col][16 * b + 4 * g]);
-        *to = w ? *to + o[b] * mul : o[b] * mul;
-      }
-    }
-    __syncthreads();
-  }
-  // ---- out: 16 threads a row
-  if (wave == 0 && g == 0) stat[0][0][lane] = all, stat[1][0][lane] = total;
+  for (int b = 0; b < kBlocks; ++b) *reinterpret_cast<f32x4*>(&sum[wave][col][16 * b + 4 * g]) = o[b];
   __syncthreads();
   const int r = threadIdx.x >> 4, cc = threadIdx.x & 15, orow = t.index * kRows + r;
   if (orow >= t.len) return;
+  float all = -__builtin_inff(), total = 0, weight[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all = fmaxf(all, stat[0][w][r]);
+  const float base = all == -__builtin_inff() ? 0.f : all;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    weight[w] = exp2_(stat[0][w][r] - base);
+    total = fmaf(stat[1][w][r], weight[w], total);
+  }
+  const auto joined = [&](int e) {
+    f32x4 v{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += *reinterpret_cast<const f32x4*>(&sum[w][r][e]) * weight[w];
+    return v;
+  };
   if (a.splits > 1) {
     float* const to = a.part + part_at(a, blockIdx.x, kv_head, blockIdx.z);
-    if (cc == 0) to[r] = stat[0][0][r], to[kRows + r] = stat[1][0][r];
-    for (int e = cc * 4; e < c.dim; e += 64)
-      *reinterpret_cast<f32x4*>(to + 2 * kRows + r * c.dim + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]);
+    if (cc == 0) to[r] = all, to[kRows + r] = total;
+    for (int e = cc * 4; e < c.dim; e += 64) *reinterpret_cast<f32x4*>(to + 2 * kRows + r * c.dim + e) = joined(e);
     return;
   }
-  const float den = stat[1][0][r], inv = den == 0 ? 0.f : 1.f / den;
+  const float inv = total == 0 ? 0.f : 1.f / total;
   const int otoken = orow / a.group;
   float* const to = a.out + ((t.start / a.group + otoken) * int64_t(a.heads) + kv_head * a.group + orow - otoken * a.group) * c.dim;
-  for (int e = cc * 4; e < c.dim; e += 64) *reinterpret_cast<f32x4u*>(to + e) = *reinterpret_cast<const f32x4*>(&sum[r][e]) * inv;
+  for (int e = cc * 4; e < c.dim; e += 64) *reinterpret_cast<f32x4u*>(to + e) = joined(e) * inv;
 }
 
 // The workgroups that shared a row tile's keys, in order: 16 threads a row, which first share
