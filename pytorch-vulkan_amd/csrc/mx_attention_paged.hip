@@ -70,10 +70,10 @@ struct Place {
   }
 };
 
-// 64 tokens, 32 heads over 8 key heads of 128, 8-bit contexts of 819 to 8192: 190 to 198 us, 3.4 to 3.5 TB/s (equal contexts
+// 64 tokens, 32 heads over 8 key heads of 128, 8-bit contexts of 819 to 8192: 189 to 197 us, 3.4 to 3.5 TB/s (equal contexts
 // of 8192 4.2 TB/s with the join; a read of as many bytes 4.0, a copy 5.0): uneven lengths leave the chip half full
 // at the end.  Without reading keys ahead 335 us.  17 x 2 tokens, FP32, contexts up to 3001, 9 heads of 80:
-// 51 us, 4.1 TB/s; keys read ahead, at one wave a SIMD, 74.
+// 50 us, 4.2 TB/s; keys read ahead, at one wave a SIMD, 74.
 template <int DP, bool I8>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void paged_kernel(const PagedArgs a) {
   constexpr int kUnits = DP / 64, kBlocks = DP / 16, kPitch = DP + 4;
@@ -341,7 +341,8 @@ int64_t row_tiles(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batc
 
 // How a row tile's keys are dealt: `span` tiles of 64 to a workgroup, as many workgroups as even out
 // lengths that the host does not know: eight a CU if all were of the table's length (the batch
-// above: 273 us with up to four, 212 with eight, 222 with 16, 248 with 32).
+// above: 220 us with up to four, 189 with eight, 188 with 16, 199 with 32; 16 contexts of up to 16384
+// 121, 105, 109 and 109).
 struct Split {
   int splits, span;
 };
@@ -350,7 +351,7 @@ Split split_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* 
   if (d->window) keys = std::min(keys, d->window + std::min(d->sinks, keys) + b->tokens + 2 * kKeys);
   const int64_t most = std::max<int64_t>(1, (keys + kKeys - 1) / kKeys), rows = std::max<int64_t>(1, row_tiles(d, c, b) * c->heads);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(int64_t(cu_count()) * 8 / rows, kMaxSplits));
-  // a tile of keys to a wave where even that leaves CUs idle (one token over 4096 keys: 13.9 us, two tiles 16.0),
+  // a tile of keys to a wave where even that leaves CUs idle (one token over 4096 keys: 13.9 us, two tiles 16.0, before waves joined behind one barrier; 12.7 now),
   // else four
   const int64_t least = rows * ((most + kWaves - 1) / kWaves) <= cu_count() * 2 ? kWaves : kWaves * 4;
   const int64_t span = std::max<int64_t>(((most + want - 1) / want + kWaves - 1) / kWaves * kWaves, least);
