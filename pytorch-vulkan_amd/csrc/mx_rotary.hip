@@ -146,12 +146,11 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
   f32x4 dw[2] = {};
   for (int first = blockIdx.x * p.group; first < p.tokens; first += gridDim.x * p.group) {
     const int count = min(p.group, p.tokens - first);
-    if (half) angles(p, first, count, cs, sn);
     // A group of L lanes takes every kThreads / L-th row, U at a time (their loads are in
     // flight together), whichever side is wanted: the weights' sums keep their order.
     const int heads = p.q_heads + p.k_heads;
     int place = threadIdx.x / L / heads, h = threadIdx.x / L - place * heads;  // of the next row
-    while (place < count) {
+    for (int turn = 0; turn < count * heads; turn += U * (kThreads / L)) {
       RowAt at[U];
       f32x4 v[U], u[U], x[U];
 #pragma unroll
@@ -176,6 +175,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
         }
         if (BACK && p.norm) x[j] = load4(in, e, p.dim);
       }
+      if (half && turn == 0) angles(p, first, count, cs, sn);  // while the first rows are on their way
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         if (!at[j].live) continue;
