@@ -38,6 +38,11 @@ using namespace attn;
 
 constexpr int kThreads = 256, kMaxDim = 128;
 
+// Kernels take a head's elements in steps of 16 (E) where products run along them, and in blocks of 32 where
+// they are the products' columns, as tiles hold them (12 heads of 80 in steps of 96: gradients of 5006 tokens 311 us,
+// of 80 292).
+constexpr int blocked(int e) { return (e + 31) / 32 * 32; }
+
 struct Shape {
   Sequences seqs;
   int heads, kv_heads, group, dim, tiles;  // tiles: of 32 rows, of all sequences
@@ -155,11 +160,11 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
 }
 
 // Own rows from a packed tile.
-template <int DP>
-__device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const char* tile, int lane) {
+template <int N>
+__device__ __forceinline__ void own_rows(Frag3 (&f)[N], const char* tile, int lane) {
   const bf16x8* const at = reinterpret_cast<const bf16x8*>(tile) + slot(lane);
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) f[s] = {at[s * 192], at[s * 192 + 64], at[s * 192 + 128]};
+  for (int s = 0; s < N; ++s) f[s] = {at[s * 192], at[s * 192 + 64], at[s * 192 + 128]};
 }
 
 // Blocks of 128 rows, four tiles of one sequence; the workgroups' order puts what has the most
@@ -293,7 +298,7 @@ struct FwdArgs {
 };
 
 // Steps whose queries' smallest piece waits in LDS, where two waves a SIMD have no registers for it.
-constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0; }
+constexpr int aside(int steps, int waves) { return steps > 6 && waves == 8 ? 7 : 0; }
 
 // A wave's 32 queries stay in registers as pieces, with their sums.  Bound by the matrix
 // instructions: 16384 tokens, 16 heads of 64, window 4096 1290 us, 187 TFLOP/s, six piece products of which
@@ -302,11 +307,12 @@ constexpr int aside(int dp, int waves) { return dp == 128 && waves == 8 ? 7 : 0;
 // behind products unless those are another tile's: 250 us with a tile's scores and exponents in turn.
 // Workgroups of eight waves, two a SIMD (4.5 us a tile of 256 rows for 3.7 of 128 then), have too
 // uneven work (289 us).
-template <int DP, int WAVES, int SPLIT>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && (WAVES == 8 || DP <= 96) ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
+template <int E, int WAVES, int SPLIT>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && (WAVES == 8 || E <= 96) ? 2 : 1))) void fwd_kernel(const FwdArgs a) {
+  constexpr int DP = blocked(E);
   using W = Walk<DP, WAVES, SPLIT, 0>;
   constexpr int kRows = W::kRows;
-  constexpr int kAside = aside(DP, WAVES);
+  constexpr int kAside = aside(E / 16, WAVES);
   __shared__ __attribute__((aligned(1024))) char smem[W::kBytes + kAside * WAVES * 1024];
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -326,8 +332,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
   };
   walk.start(source);
   const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, qi = i0 + tile_row(lane & 31);
-  Frag3 q[DP / 16];
-  own_rows<DP>(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
+  Frag3 q[E / 16];
+  own_rows(q, a.q, head, int64_t(t.start) + qi, qi < t.len, s.dim, h, s.scale * kLog2E);
   bf16x8* const mine = reinterpret_cast<bf16x8*>(smem + W::kBytes) + wave * kAside * 64 + lane;
 #pragma unroll
   for (int i = 0; i < kAside; ++i) mine[i * 64] = q[i].lo;
@@ -339,7 +345,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SPLI
     const int j0 = keys.tile(n) * kTile;
     return i0 < t.len && !s.mask.none(i0, i1, j0, j0 + kTile - 1);
   };
-  const auto scores = [&](uint32_t tile) { return product<DP, 3>(tile, q, lane, low); };
+  const auto scores = [&](uint32_t tile) { return product<3>(tile, q, lane, low); };
   const auto masked = [&](int n, f32x16& x) {
     const int j0 = keys.tile(n) * kTile;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
@@ -459,14 +465,15 @@ __device__ __forceinline__ int near_last(const BwdArgs& a, int b0, int len) {
 // Three products of a tile, two of them computed again for dk and dv: the scores' gradients would be
 // 6 bytes a pair in memory.  2 x 2048, 16 heads of 128: 280 us alone, 168 TFLOP/s, 1.0 PFLOP/s of pieces.
 // (workgroup `index` of `count`)
-template <int DP, int SPLIT>
+template <int E, int SPLIT>
 struct Dq {
+  static constexpr int DP = blocked(E);
   using W = Walk<DP, 4, SPLIT, 0>;
   static constexpr int kBytes = W::kBytes;
   static __device__ void run(const BwdArgs a, char* smem, int index, int count);
 };
-template <int DP, int SPLIT>
-__device__ __forceinline__ void Dq<DP, SPLIT>::run(const BwdArgs a, char* smem, int index, int count) {
+template <int E, int SPLIT>
+__device__ __forceinline__ void Dq<E, SPLIT>::run(const BwdArgs a, char* smem, int index, int count) {
   constexpr int kRows = W::kRows;
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -486,9 +493,9 @@ __device__ __forceinline__ void Dq<DP, SPLIT>::run(const BwdArgs a, char* smem, 
   const int i0 = b0 + walk.rows(), i1 = min(i0 + kTile, t.len) - 1, row = tile_row(lane & 31), qi = i0 + row;
   // A wave past the sequence's end repeats its last tile, and stores nothing.
   const int mine = base32 + min(i0, t.len - 1) / kTile;
-  Frag3 q[DP / 16], g[DP / 16];
-  own_rows<DP>(q, a.qp + tile_at<DP>(s, head, mine), lane);
-  own_rows<DP>(g, a.dp + tile_at<DP>(s, head, mine), lane);
+  Frag3 q[E / 16], g[E / 16];
+  own_rows(q, a.qp + tile_at<DP>(s, head, mine), lane);
+  own_rows(g, a.dp + tile_at<DP>(s, head, mine), lane);
   const float* const stat = a.stats + (int64_t(head) * s.tiles + mine) * 64 + row;
   const float lse = stat[0], delta = stat[32];
   f32x16 dq[DP / 32] = {};
@@ -499,9 +506,9 @@ __device__ __forceinline__ void Dq<DP, SPLIT>::run(const BwdArgs a, char* smem, 
   };
   const auto use = [&](int n, const Staged& at) {
     const int j0 = keys.tile(n) * kTile;
-    f32x16 x = product<DP, 3>(at.first, q, lane) - lse;
+    f32x16 x = product<3>(at.first, q, lane) - lse;
     if (!s.mask.all(i0, i1, j0, j0 + kTile - 1)) hide(x, [&](int r) { return s.mask.sees(qi, j0 + 16 * h + r); });
-    const f32x16 dp = product<DP, 3>(at.second, g, lane);
+    const f32x16 dp = product<3>(at.second, g, lane);
 #pragma unroll
     for (int r = 0; r < 16; ++r) x[r] = times(exp2_(x[r]), dp[r] - delta);
     return Halves{{split_half(x, 0), split_half(x, 1)}};
@@ -516,23 +523,24 @@ __device__ __forceinline__ void Dq<DP, SPLIT>::run(const BwdArgs a, char* smem, 
     store_block(a.dq + ((int64_t(t.start) + qi) * s.heads + head) * s.dim, dq[b] * s.scale, b, h, s.dim);
 }
 
-template <int DP, int SPLIT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dq_kernel(const BwdArgs a) {
-  __shared__ __attribute__((aligned(1024))) char smem[Dq<DP, SPLIT>::kBytes];
-  Dq<DP, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
+template <int E, int SPLIT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && E <= 64 ? 2 : 1))) void dq_kernel(const BwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[Dq<E, SPLIT>::kBytes];
+  Dq<E, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
 }
 
 // Four products of a tile, the scores straight (a lane has 16 queries of a key), so that both sums run
 // along what a lane holds.  380 us alone for 2 x 2048, 16 heads of 128: 165 TFLOP/s.
-template <int DP, int SPLIT>
+template <int E, int SPLIT>
 struct Dkv {
+  static constexpr int DP = blocked(E);
   using W = Walk<DP, 4, SPLIT, 1>;
-  static constexpr int kAside = SPLIT == 1 && DP == 64 ? DP / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
+  static constexpr int kAside = SPLIT == 1 && DP == 64 ? E / 16 : 0;  // steps whose values' smallest piece waits in LDS (two waves a SIMD)
   static constexpr int kBytes = W::kBytes + kAside * 4 * 1024;
   static __device__ void run(const BwdArgs a, char* smem, int number, int workgroups);
 };
-template <int DP, int SPLIT>
-__device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem, int number, int workgroups) {
+template <int E, int SPLIT>
+__device__ __forceinline__ void Dkv<E, SPLIT>::run(const BwdArgs a, char* smem, int number, int workgroups) {
   constexpr int kRows = W::kRows;
   const Shape& s = a.s;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -564,9 +572,9 @@ __device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem,
   walk.start(source);
   const int j0 = b0 + walk.rows(), j1 = j0 + kTile - 1, kj = j0 + tile_row(lane & 31);
   const int64_t mine = tile_at<DP>(s, kv_head, base32 + min(j0, t.len - 1) / kTile);
-  Frag3 k[DP / 16], v[DP / 16];
-  own_rows<DP>(k, a.kp + mine, lane);
-  own_rows<DP>(v, a.vp + mine, lane);
+  Frag3 k[E / 16], v[E / 16];
+  own_rows(k, a.kp + mine, lane);
+  own_rows(v, a.vp + mine, lane);
   bf16x8* const aside_at = reinterpret_cast<bf16x8*>(smem + W::kBytes) + wave * kAside * 64 + lane;
 #pragma unroll
   for (int i = 0; i < kAside; ++i) aside_at[i * 64] = v[i].lo;
@@ -579,7 +587,7 @@ __device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem,
   };
   const auto use = [&](int n, const Staged& at) {
     const int i0 = (from + n % tiles) * kTile;
-    f32x16 x = product<DP, 3>(at.first, k, lane), delta;
+    f32x16 x = product<3>(at.first, k, lane), delta;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t stats = at.stats + (16 * h + 4 * i) * 4;
@@ -588,7 +596,7 @@ __device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem,
       for (int e = 0; e < 4; ++e) x[4 * i + e] -= lse[e], delta[4 * i + e] = d[e];
     }
     if (!s.mask.all(i0, i0 + kTile - 1, j0, j1)) hide(x, [&](int r) { return s.mask.sees(i0 + 16 * h + r, kj); });
-    f32x16 dp = product<DP, 3>(at.second, v, lane, low);
+    f32x16 dp = product<3>(at.second, v, lane, low);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       x[r] = exp2_(x[r]);
@@ -621,20 +629,20 @@ __device__ __forceinline__ void Dkv<DP, SPLIT>::run(const BwdArgs a, char* smem,
     if (a.dv) store_block(to_v + at, dv[b], b, h, s.dim);
   }
 }
-template <int DP, int SPLIT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && DP <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
-  __shared__ __attribute__((aligned(1024))) char smem[Dkv<DP, SPLIT>::kBytes];
-  Dkv<DP, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
+template <int E, int SPLIT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(SPLIT == 1 && E <= 64 ? 2 : 1))) void dkv_kernel(const BwdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[Dkv<E, SPLIT>::kBytes];
+  Dkv<E, SPLIT>::run(a, smem, blockIdx.x, gridDim.x);
 }
 // Both, where workgroups are few: `first` of dk and dv, then those of dq, which fill the CUs that the others
 // leave.  Calls with packing, in two launches and in one: 4 x 256, 12 heads of 64 46 and 38 us, 2048, 8 heads
 // of 128 301 and 192, 2 x 2048, 16 heads of 128 716 and 711 (184 TFLOP/s without packing and the join, 1.1
 // PFLOP/s of pieces).
-template <int DP>
+template <int E>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1))) void both_kernel(const BwdArgs a, int first) {
-  __shared__ __attribute__((aligned(1024))) char smem[std::max(Dkv<DP, 2>::kBytes, Dq<DP, 2>::kBytes)];
-  if (int(blockIdx.x) < first) Dkv<DP, 2>::run(a, smem, blockIdx.x, first);
-  else Dq<DP, 2>::run(a, smem, blockIdx.x - first, gridDim.x - first);
+  __shared__ __attribute__((aligned(1024))) char smem[std::max(Dkv<E, 2>::kBytes, Dq<E, 2>::kBytes)];
+  if (int(blockIdx.x) < first) Dkv<E, 2>::run(a, smem, blockIdx.x, first);
+  else Dq<E, 2>::run(a, smem, blockIdx.x - first, gridDim.x - first);
 }
 
 // What queries past the window give first tokens' dk and dv, added to the rest: grid (blocks of
@@ -720,7 +728,7 @@ Shape shape_of(const mx_attention_desc* d) {
   return s;
 }
 
-int padded(int64_t dim) { return int((dim + 31) / 32 * 32); }
+int padded(int64_t dim) { return blocked(int(dim)); }
 
 // Scratch: the packed tensors in the order in which take() hands them out.
 struct Carve {
@@ -798,14 +806,11 @@ int64_t workspace_bytes_of(const mx_attention_desc* d, bool backward) {
   return c.used;
 }
 
-template <class F>
+// f with the head's elements padded to 16.
+template <int E = 16, class F>
 void with_dim(int dim, F&& f) {
-  switch (padded(dim)) {
-    case 32: return f(std::integral_constant<int, 32>{});
-    case 64: return f(std::integral_constant<int, 64>{});
-    case 96: return f(std::integral_constant<int, 96>{});
-    default: return f(std::integral_constant<int, 128>{});
-  }
+  if (dim <= E) return f(std::integral_constant<int, E>{});
+  if constexpr (E < kMaxDim) with_dim<E + 16>(dim, f);
 }
 
 }  // namespace
@@ -842,21 +847,21 @@ extern "C" int mx_attention_forward(const mx_attention_desc* d, const float* q, 
   p.kp = b.kp, p.vp = b.vp;
   const FwdArgs f{s, {q, d->q_token, d->q_head}, b.kp, b.vp, out, lse};
   with_dim(s.dim, [&](auto dp) {
-    hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.kv_heads), dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((pack_kernel<blocked(decltype(dp)::value)>), dim3(s.tiles, s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
   with_dim(s.dim, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
+    constexpr int E = decltype(dp)::value;
     const int64_t wide = sequence_tiles(s.seqs.tokens, s.seqs.count, 8 * kTile) * s.heads;
     if (wide_blocks(wide)) {
-      hipLaunchKernelGGL((fwd_kernel<DP, 8, 1>), dim3(unsigned(wide)), dim3(512), 0, st, f);
+      hipLaunchKernelGGL((fwd_kernel<E, 8, 1>), dim3(unsigned(wide)), dim3(512), 0, st, f);
       return;
     }
     if (halved(s, blocks_of(s) * s.heads, true)) {
-      hipLaunchKernelGGL((fwd_kernel<DP, 4, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(256), 0, st, f);
+      hipLaunchKernelGGL((fwd_kernel<E, 4, 2>), dim3(unsigned(blocks_of(s, kBlock / 2) * s.heads)), dim3(256), 0, st, f);
       return;
     }
-    hipLaunchKernelGGL((fwd_kernel<DP, 4, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
+    hipLaunchKernelGGL((fwd_kernel<E, 4, 1>), dim3(unsigned(blocks_of(s) * s.heads)), dim3(256), 0, st, f);
   });
   MX_LAUNCHED();
   return MX_OK;
@@ -887,7 +892,7 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   p.qp = b.qp, p.kp = b.kp, p.vp = b.vp, p.dp = b.dp, p.stats = b.stats;
   const BwdArgs g{s, b.qp, b.kp, b.vp, b.dp, b.stats, dq, dk, dv, parts, b.dk_p, b.dv_p, block, int(blocks_of(s, block)), int(far_blocks_of(s, block)), b.far};
   with_dim(s.dim, [&](auto dp) {
-    hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
+    hipLaunchKernelGGL((pack_kernel<blocked(decltype(dp)::value)>), dim3(s.tiles, s.heads + s.kv_heads), dim3(kThreads), 0, st, p);
   });
   MX_LAUNCHED();
   const bool keys = dk || dv, key_halves = block < kBlock, query_halves = halved(s, blocks_of(s) * s.heads, false);
@@ -901,18 +906,18 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
     MX_LAUNCHED();
   } else if (dq) {
     with_dim(s.dim, [&](auto dp) {
-      constexpr int DP = decltype(dp)::value;
-      if (query_halves) hipLaunchKernelGGL((dq_kernel<DP, 2>), dim3(of_queries), dim3(kThreads), 0, st, g);
-      else hipLaunchKernelGGL((dq_kernel<DP, 1>), dim3(of_queries), dim3(kThreads), 0, st, g);
+      constexpr int E = decltype(dp)::value;
+      if (query_halves) hipLaunchKernelGGL((dq_kernel<E, 2>), dim3(of_queries), dim3(kThreads), 0, st, g);
+      else hipLaunchKernelGGL((dq_kernel<E, 1>), dim3(of_queries), dim3(kThreads), 0, st, g);
     });
     MX_LAUNCHED();
   }
   if (keys) {
     if (!both) {
       with_dim(s.dim, [&](auto dp) {
-        constexpr int DP = decltype(dp)::value;
-        if (key_halves) hipLaunchKernelGGL((dkv_kernel<DP, 2>), dim3(of_keys), dim3(kThreads), 0, st, g);
-        else hipLaunchKernelGGL((dkv_kernel<DP, 1>), dim3(of_keys), dim3(kThreads), 0, st, g);
+        constexpr int E = decltype(dp)::value;
+        if (key_halves) hipLaunchKernelGGL((dkv_kernel<E, 2>), dim3(of_keys), dim3(kThreads), 0, st, g);
+        else hipLaunchKernelGGL((dkv_kernel<E, 1>), dim3(of_keys), dim3(kThreads), 0, st, g);
       });
       MX_LAUNCHED();
     }

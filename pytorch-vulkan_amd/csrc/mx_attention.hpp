@@ -207,20 +207,20 @@ __device__ __forceinline__ void hide(f32x16& x, F&& sees) {
 // a b along the head's elements: a's tile in LDS, b's fragments in registers.  (One accumulator:
 // over so few terms the matrix instruction's rounding towards minus infinity does not add up.)
 // low(s): the smallest pieces of b's step s.
-template <int DP, int P, class L>
-__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane, L&& low) {
+template <int P, int N, class L>
+__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[N], int lane, L&& low) {
   f32x16 acc{};
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
+  for (int s = 0; s < N; ++s) {
     const Frag<P> f = frag<P>(a, s, lane);
     const Frag3 o{b[s].hi, b[s].mid, low(s)};
     acc = mma_large(f, o, mma_small(f, o, acc));
   }
   return acc;
 }
-template <int DP, int P>
-__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[DP / 16], int lane) {
-  return product<DP, P>(a, b, lane, [&](int s) { return b[s].lo; });
+template <int P, int N>
+__device__ __forceinline__ f32x16 product(uint32_t a, const Frag3 (&b)[N], int lane) {
+  return product<P>(a, b, lane, [&](int s) { return b[s].lo; });
 }
 
 // f0 and f1's products with a tile's probabilities (or their like), added up among themselves: the
@@ -239,12 +239,12 @@ __device__ __forceinline__ f32x16 product_columns(uint32_t a, int b, const Frag3
 }
 
 // Own rows as fragments in registers, straight from memory.
-template <int DP>
-__device__ __forceinline__ void own_rows(Frag3 (&f)[DP / 16], const Strided& t, int head, int64_t row, bool live, int dim, int h,
+template <int N>
+__device__ __forceinline__ void own_rows(Frag3 (&f)[N], const Strided& t, int head, int64_t row, bool live, int dim, int h,
                                          float scale) {
   const float* const at = t.at + row * t.token + head * t.head;
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
+  for (int s = 0; s < N; ++s) {
     f32x4 v[2] = {};
     if (live) load8(at, s * 16 + h * 8, dim, v);
     f[s] = split8(v[0] * scale, v[1] * scale);

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(I8 |
     const int j0 = keys.tile(n) * kTile;
     if (r0 >= t.len || a.mask.none(i0, i1, j0, j0 + kTile - 1)) continue;
     const uint32_t tile = st.lds + (n & 1) * St::kBytes, stats = tile + St::kStats + 64 * h;
-    f32x16 x = product<DP, P>(tile, q, lane, low);
+    f32x16 x = product<P>(tile, q, lane, low);
     const auto scaled = [&](int which, int i) { return *pieces::lds_at<const f32x4>(stats + 128 * which + 16 * i); };
     if constexpr (I8) {
 #pragma unroll
