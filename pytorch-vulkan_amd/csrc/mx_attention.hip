@@ -659,13 +659,14 @@ __global__ __launch_bounds__(kThreads) void far_kernel(const BwdArgs a) {
     if (i >= rows * s.dim) continue;
     const int64_t at = ((int64_t(start) + b0 + i / s.dim) * s.kv_heads + blockIdx.y) * s.dim + i % s.dim;
     float k = a.dk ? a.dk[at] : 0.f, v = a.dv ? a.dv[at] : 0.f;
-    for (int c = from; c <= to; ++c)
-#pragma unroll 4
-      for (int p = 0; p < a.parts; ++p) {
-        const float* const sum = far_at(a, base + c, block, blockIdx.y, p) + i;
-        if (a.dk) k += sum[0];
-        if (a.dv) v += sum[a.block * s.dim];
-      }
+    // (eight sums on their way at a time; those of a gradient that is not wanted are not looked at)
+    const int sums = (to - from + 1) * a.parts;
+#pragma unroll 8
+    for (int n = 0; n < sums; ++n) {
+      const float* const sum = far_at(a, base + from + n / a.parts, block, blockIdx.y, n % a.parts) + i;
+      k += sum[0];
+      v += sum[a.block * s.dim];
+    }
     if (a.dk) a.dk[at] = k;
     if (a.dv) a.dv[at] = v;
   }
