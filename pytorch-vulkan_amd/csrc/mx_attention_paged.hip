@@ -351,8 +351,8 @@ Split split_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* 
   if (d->window) keys = std::min(keys, d->window + std::min(d->sinks, keys) + b->tokens + 2 * kKeys);
   const int64_t most = std::max<int64_t>(1, (keys + kKeys - 1) / kKeys), rows = std::max<int64_t>(1, row_tiles(d, c, b) * c->heads);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(int64_t(cu_count()) * 8 / rows, kMaxSplits));
-  // a tile of keys to a wave where even that leaves CUs idle (one token over 4096 keys: 13.9 us, two tiles 16.0, before waves joined behind one barrier; 12.7 now),
-  // else four
+  // a tile of keys to a wave where even that leaves CUs idle (one token over 4096 keys 13.9 us, with two
+  // tiles 16.0, before waves joined behind one barrier: 12.7 now), else four
   const int64_t least = rows * ((most + kWaves - 1) / kWaves) <= cu_count() * 2 ? kWaves : kWaves * 4;
   const int64_t span = std::max<int64_t>(((most + want - 1) / want + kWaves - 1) / kWaves * kWaves, least);
   return {int((most + span - 1) / span), int(span)};
