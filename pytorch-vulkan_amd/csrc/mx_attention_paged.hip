@@ -348,7 +348,8 @@ struct Split {
 };
 Split split_of(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batch* b) {
   int64_t keys = b->table_width * c->page_size;
-  if (d->window) keys = std::min(keys, d->window + std::min(d->sinks, keys) + b->tokens + 2 * kKeys);
+  // (never less than a row tile's keys: its window may begin and end inside a tile of 64; a window may be any number)
+  if (d->window) keys = std::min(keys, std::min(d->window, keys) + std::min(d->sinks, keys) + b->tokens + 2 * kKeys);
   const int64_t most = std::max<int64_t>(1, (keys + kKeys - 1) / kKeys), rows = std::max<int64_t>(1, row_tiles(d, c, b) * c->heads);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(int64_t(cu_count()) * 8 / rows, kMaxSplits));
   // a tile of keys to a wave where even that leaves CUs idle (one token over 4096 keys 13.9 us, with two

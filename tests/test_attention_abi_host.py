@@ -223,3 +223,18 @@ def test_python_binding_checks_shapes(mx):
         mx.kv_cache_write(c, b, t(3, 1, 32), t(3, 2, 32))
     with pytest.raises(ValueError, match="does not fit"):
         mx.attention_paged(c, b, t(4, 2, 32), t(4, 2, 32))
+
+
+@pytest.mark.parametrize("kind", ["KV_F32", "KV_I8"])
+@pytest.mark.parametrize("tokens", [1, 3, 700])
+def test_paged_plans_of_the_largest_windows(mx, kind, tokens):
+    """A window that reaches past the table is planned as none."""
+    c, need = cache(mx, type=getattr(mx, kind)), C.c_int64()
+    b = batch(mx, tokens=tokens, sequences=1, table_width=1 << 7)
+    sizes = []
+    for window in (0, 1 << 12, 1 << 40, 2 ** 63 - 200, 2 ** 63 - 1):
+        for sinks in (0, 2 ** 63 - 1):
+            d = mx.PagedDesc(4, 64, 16, window, sinks, 0.25)
+            mx.check(mx.lib().mx_attention_paged_workspace(C.byref(d), C.byref(c), C.byref(b), C.byref(need)))
+            sizes.append(need.value)
+    assert sizes[0] > 0 and sizes == sizes[:1] * len(sizes)

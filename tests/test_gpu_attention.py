@@ -875,3 +875,29 @@ def test_cache_past_2_to_31_elements(mx, returned, kind):
         pos, at = torch.arange(640 - n, 640, device="cuda"), torch.arange(640, device="cuda")
         ref, bound = paged_ref(q, kr, vr, pos, pos[:, None] >= at[None, :], d ** -0.5)
         within(out, ref, bound + 1e-30, f"{n} rows")
+
+
+# ------------------------------------------------------- sizes and values at the borders
+@pytest.mark.parametrize("kind", ["i8", "f32"])
+@pytest.mark.parametrize("new,length", [(1, 1500), (3, 3000), (500, 1500)])
+def test_paged_largest_windows_see_everything(mx, new, length, kind):
+    """A window that no sequence fills is none at all, however large the number."""
+    g, page, h, kv, d = gen(length + new), 64, 8, 2, 64
+    table, pages = tables(g, [length], page)
+    cache = new_cache(mx, g, pages, kv, page, d, kind)
+    fill(mx, g, cache, table, [length], page, kv, d, kind)
+    q, batch = rand(g, new, h, d), mx.KVBatch(table, i32([length]), new)
+    run = lambda window: (out := torch.full_like(q, TAIL), mx.attention_paged(
+        cache, batch, q, out, window=window, stream=stream()))[0]
+    whole = run(0)
+    for window in (2 ** 31, 2 ** 40, 2 ** 63 - 200, 2 ** 63 - 1):
+        assert torch.equal(run(window), whole), window
+
+
+def test_attention_largest_windows_see_everything(mx):
+    g, n = gen(31), 700
+    x = [rand(g, n, h, 64) for h in (4, 2, 2, 4)]
+    whole = run_attention(mx, *x, None)
+    for window in (2 ** 31, 2 ** 63 - 1):
+        got = run_attention(mx, *x, None, window=window, sinks=2 ** 63 - 1)
+        assert all(torch.equal(got[name], whole[name]) for name in whole), window
