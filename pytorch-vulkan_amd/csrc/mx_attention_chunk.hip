@@ -152,7 +152,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(I8 |
   RowTile<1> all;
   all.t = t;
   all.whole(a);
-  const KeyTiles<> packed = seen_by_all(a, all), keys(a.mask, max(rt.i0, 0), rt.i1);
+  const KeyTiles<> packed = seen_by_all(a, all), keys(a.mask, max(rt.i0, 0), rt.end);
   const int span = a.c.pages ? (keys.count + a.splits - 1) / a.splits : 0;
   const int begin = blockIdx.y * span, end = min(keys.count, begin + span);
   // The wave's rows, and the lane's.

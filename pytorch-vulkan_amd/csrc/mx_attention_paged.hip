@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
   RowTile<kRows> rt;
   if (!rt.find(a, blockIdx.x)) return;
   const SequenceTile& t = rt.t;
-  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.i1);
+  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.end);
   // This workgroup's tiles of keys, dealt to its waves.
   const int begin = blockIdx.z * a.span, end = c.pages ? min(keys.count, begin + a.span) : 0;
   if (blockIdx.z && begin >= end) return;
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(const PagedArgs a)
   if (!rt.find(a, blockIdx.x)) return;
   const SequenceTile& t = rt.t;
   const int r = threadIdx.x >> 4, cc = threadIdx.x & 15, row = t.index * kRows + r, kv_head = blockIdx.y;
-  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.i1);
+  const KeyTiles<kKeys> keys(a.mask, max(rt.i0, 0), rt.end);
   const int splits = a.c.pages ? max(1, (keys.count + a.span - 1) / a.span) : 1;  // those that have left a part
   const float* const part = a.part + part_at(a, blockIdx.x, kv_head, 0);
   const int64_t step = kRows * (2 + a.c.dim);

@@ -27,12 +27,14 @@ struct Paged {
 template <int R>
 struct RowTile {
   SequenceTile t;
-  int length, first, i0, i1;  // tokens of the sequence, its first new one, the tile's positions
+  int length, first;  // tokens of the sequence that its table has room for, its first new one's position
+  int i0, i1, end;    // the tile's positions, and the last of them within `length`
   __device__ __forceinline__ bool find(const Paged& a, int tile) {
     if (!locate<R>(a.b.seqs, tile, t) || t.index * R >= t.len) return false;
     whole(a);
     i0 = first + t.index * R / a.group;
-    i1 = min(first + (min(t.len, (t.index + 1) * R) - 1) / a.group, length - 1);
+    i1 = first + (min(t.len, (t.index + 1) * R) - 1) / a.group;
+    end = min(i1, length - 1);
     return true;
   }
   __device__ __forceinline__ void whole(const Paged& a) {

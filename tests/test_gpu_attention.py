@@ -901,3 +901,27 @@ def test_attention_largest_windows_see_everything(mx):
     for window in (2 ** 31, 2 ** 63 - 1):
         got = run_attention(mx, *x, None, window=window, sinks=2 ** 63 - 1)
         assert all(torch.equal(got[name], whole[name]) for name in whole), window
+
+
+@pytest.mark.parametrize("kind", ["i8", "f32"])
+@pytest.mark.parametrize("new,length,window", [(1, 130, 70), (5, 140, 70), (7, 200, 100), (100, 229, 150), (100, 300, 190)])
+def test_paged_positions_past_the_table(mx, new, length, window, kind):
+    """New tokens behind the table's 128 places, with a window that ends inside it: each sees its own window's keys."""
+    g, page, h, kv, d, places = gen(length + new), 64, 16, 2, 64, 128
+    table, pages = tables(g, [places], page)
+    cache = new_cache(mx, g, pages, kv, page, d, kind)
+    k, v = fill(mx, g, cache, table, [places], page, kv, d, kind)
+    q, out = rand(g, new, h, d), torch.empty(new, h, d, device="cuda")
+    mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, out, window=window, stream=stream())
+    pos, keys = torch.arange(length - new, length, device="cuda"), torch.arange(places, device="cuda")
+    back = pos[:, None] - keys[None, :]
+    ref, bound = paged_ref(q, k, v, pos, (back >= 0) & (back < window), d ** -0.5)
+    within(out, ref, bound + 1e-30, "rows past the table")
+    if kind == "f32":
+        # The keys before the last row's window hold anything.
+        first = int(pos[-1]) - window + 1
+        page_of, slot = int(table[0, (first - 1) // page]), (first - 1) % page
+        cache.tensors[0][page_of, 0, slot] = math.nan
+        again = torch.empty_like(out)
+        mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, again, window=window, stream=stream())
+        assert torch.equal(again[-1], out[-1])
