@@ -404,7 +404,8 @@ extern "C" int mx_attention_paged(const mx_paged_desc* d, const mx_kv_cache* c, 
   a.heads = int(d->heads), a.group = int(d->heads / c->heads);
   a.b.seqs.per = a.group;
   a.out = out, a.q = q, a.q_token = d->q_token, a.q_head = d->q_head;
-  a.mask = {int(std::min<int64_t>(d->window, 1 << 30)), int(std::min<int64_t>(d->sinks, 1 << 30))};
+  // (positions go up to 2^31 - 2, keys to 2^30 - 1: these limits hide nothing)
+  a.mask = {int(std::min<int64_t>(d->window, INT32_MAX)), int(std::min<int64_t>(d->sinks, 1 << 30))};
   a.scale = float(d->scale);
   if (chunk_workspace(d, c, b)) return chunk_attention(a, d, c, b, ws.as<char>(), s);
   a.tiles = int(row_tiles(d, c, b));

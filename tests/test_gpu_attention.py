@@ -925,3 +925,23 @@ def test_paged_positions_past_the_table(mx, new, length, window, kind):
         again = torch.empty_like(out)
         mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, again, window=window, stream=stream())
         assert torch.equal(again[-1], out[-1])
+
+
+@pytest.mark.parametrize("kind", ["i8", "f32"])
+@pytest.mark.parametrize("new", [1, 100])
+def test_paged_far_positions_and_large_windows(mx, new, kind):
+    """Positions past 2^30, whose window of 2^30 or more reaches a short table's keys: in part or whole."""
+    g, page, h, kv, d, places = gen(new), 32, 16, 2, 64, 64
+    table, pages = tables(g, [places], page)
+    cache = new_cache(mx, g, pages, kv, page, d, kind)
+    k, v = fill(mx, g, cache, table, [places], page, kv, d, kind)
+    q = rand(g, new, h, d)
+    keys = torch.arange(places, device="cuda")
+    for length in (2 ** 30 + 40, 2 ** 31 - 1):
+        pos = torch.arange(length - new, length, device="cuda")
+        back = pos[:, None] - keys[None, :]
+        for window in (2 ** 30, 2 ** 30 + 77, 2 ** 31 - 30, 2 ** 31 - 1, 2 ** 40, 2 ** 63 - 1):
+            out = torch.empty_like(q)
+            mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, out, window=window, stream=stream())
+            ref, bound = paged_ref(q, k, v, pos, back < window, d ** -0.5)
+            within(out, ref, bound + 1e-30, f"length {length}, window {window}")
