@@ -129,6 +129,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
   f32x4 w[2] = {f32x4{1, 1, 1, 1}, f32x4{1, 1, 1, 1}};
   int with[4], pair[4];  // each element's partner and pair
   bool head[4];
+  // (an element that is not turned has 0 for a partner, in its row and its weight: what lies beside it may be anything)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     with[i] = min(partner(p, e + i, head[i]), p.dim - 1);
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
   for (int k = 0; k < 2; ++k) {
     if (p.norm && o.w[k]) w[k] = load4(o.w[k], e, p.dim);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wp[k][i] = p.norm && o.w[k] ? o.w[k][with[i]] : 1.f;
+    for (int i = 0; i < 4; ++i) wp[k][i] = pair[i] < 0 ? 0.f : p.norm && o.w[k] ? o.w[k][with[i]] : 1.f;
   }
   f32x4 dw[2] = {};
   for (int first = blockIdx.x * p.group; first < p.tokens; first += gridDim.x * p.group) {
@@ -171,7 +172,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
           u[j] = *reinterpret_cast<const f32x4u*>(turned + with[0]);
         } else if (!own && e < p.rot) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[j][i] = turned[with[i]];
+          for (int i = 0; i < 4; ++i) {
+            const float other = turned[with[i]];
+            u[j][i] = pair[i] < 0 ? 0.f : other;
+          }
         }
         if (BACK && p.norm) x[j] = load4(in, e, p.dim);
       }
@@ -180,7 +184,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary p, const 
       for (int j = 0; j < U; ++j) {
         if (!at[j].live) continue;
         const int k = at[j].k;
-        if (own && p.rot) u[j] = f32x4{v[j][1], v[j][0], v[j][3], v[j][2]};
+        if (own && p.rot) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[j][i] = pair[i] < 0 ? 0.f : v[j][i ^ 1];
+        }
         f32x4 c{1, 1, 1, 1}, s{};
         if (run) {  // four neighbouring pairs
           c = *reinterpret_cast<const f32x4*>(&cs[at[j].place * half + pair[0]]);

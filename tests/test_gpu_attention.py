@@ -945,3 +945,37 @@ def test_paged_far_positions_and_large_windows(mx, new, kind):
             mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, out, window=window, stream=stream())
             ref, bound = paged_ref(q, k, v, pos, back < window, d ** -0.5)
             within(out, ref, bound + 1e-30, f"length {length}, window {window}")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(128, 64), (20, 12), (22, 10), (65, 34), (255, 198), (7, 2)])
+def test_rotary_elements_behind_the_turned_part_stay_alone(mx, dim, rot, interleaved):
+    """Elements past rotary_dim pass through, whatever they and their neighbours hold."""
+    g, tokens, h = gen(dim), 9, 3
+    plan, pos = mx.Rotary(frequencies(rot), interleaved=interleaved, magnitude=1.25), torch.arange(tokens, device="cuda")
+    x = rand(g, tokens, h, dim)
+    forward = lambda t, **kw: (out := torch.empty_like(t), mx.qk_norm_rotary_forward(
+        t, None, pos, plan, out, None, stream=stream(), **kw))[0]
+    backward = lambda t, **kw: (out := torch.empty_like(t), mx.qk_norm_rotary_backward(
+        t, None, None, None, pos, plan, out, None, stream=stream(), **kw))[0]
+    for turn in (forward, backward):
+        clean = turn(x)
+        assert torch.equal(clean[..., rot:], x[..., rot:])
+        for value in (math.inf, -math.inf, math.nan, 3.4e38):
+            for e in {rot, rot + (dim - rot) // 2, dim - 1}:
+                y = x.clone()
+                y[4, 1, e] = value
+                got = turn(y)
+                assert torch.equal(got[4, 1, e].nan_to_num(7.0, 8.0, 9.0), y[4, 1, e].nan_to_num(7.0, 8.0, 9.0)), (e, value)
+                got[4, 1, e] = x[4, 1, e]
+                assert torch.equal(got, clean), (e, value)
+    # An infinite weight of one such element, under a norm.
+    w = rand(g, dim, mean=1.0, scale=0.1)
+    clean = forward(x, q_weight=w, eps=1e-6)
+    for e in {rot, dim - 1}:
+        v = w.clone()
+        v[e] = math.inf
+        got = forward(x, q_weight=v, eps=1e-6)
+        assert torch.equal(got[..., e], x[..., e].sign() * math.inf), e
+        got[..., e] = clean[..., e]
+        assert torch.equal(got, clean), e
