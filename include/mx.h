@@ -644,7 +644,8 @@ int mx_qk_norm_rotary_workspace(const mx_rotary_desc* d, int64_t* bytes);
  * heads / kv_heads query heads to a key head.  Rows that belong to no sequence are left
  * as they are, in every output.  A row that sees a NaN or an infinity is NaN, and so are
  * the gradients that it reaches; those of keys and queries that a row does not see
- * have no effect on it.  No operand may overlap an output. */
+ * have no effect on it.  An element from 2^128 (1 - 2^-9) on (of a query: times scale log2(e)) counts as infinite.
+ * No operand may overlap an output. */
 typedef struct mx_attention_desc {
   int64_t tokens, sequences;
   const int32_t* starts; /* device, [sequences + 1], ascending: sequence b is rows starts[b] .. starts[b + 1] - 1;

@@ -77,24 +77,25 @@ struct Pack {
   static constexpr int N = (DP / 16 + 3) / 4;
   f32x4 x[N][2];
   bool bad = false;
-  // rows: of the tile; r and h: the lane's row and half
-  __device__ __forceinline__ void load(const Strided& t, int head, int row0, int rows, int dim, int wave, int r, int h) {
+  // rows: of the tile; r and h: the lane's row and half.  (What is packed is looked at, so scaled.)
+  __device__ __forceinline__ void load(const Strided& t, int head, int row0, int rows, int dim, int wave, int r, int h, float scale) {
     const float* const row = t.at + (int64_t(row0) + r) * t.token + head * t.head;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int s = wave + 4 * i;
       x[i][0] = x[i][1] = f32x4{};
       if (s < DP / 16 && r < rows) load8(row, s * 16 + h * 8, dim, x[i]);
+      x[i][0] *= scale, x[i][1] *= scale;
 #pragma unroll
       for (int j = 0; j < 8; ++j) bad = bad || !finite(x[i][j >> 2][j & 3]);
     }
   }
-  __device__ __forceinline__ void store(char* to, int wave, int lane, bool replace, float with, float scale) const {
+  __device__ __forceinline__ void store(char* to, int wave, int lane, bool replace, float with) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int s = wave + 4 * i;
       if (s >= DP / 16) break;
-      f32x4 v[2] = {x[i][0] * scale, x[i][1] * scale};
+      f32x4 v[2] = {x[i][0], x[i][1]};
       if (replace) v[0] = v[1] = f32x4{with, with, with, with};
       const Frag3 f = split8(v[0], v[1]);
       bf16x8* const at = reinterpret_cast<bf16x8*>(to) + s * 3 * 64 + slot(lane);
@@ -121,8 +122,8 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
   const int head = key ? blockIdx.y : blockIdx.y - s.kv_heads;
   const int64_t o = tile_at<DP>(s, head, blockIdx.x);
   Pack<DP> x, y;
-  x.load(key ? a.k : a.q, head, row0, rows, s.dim, wave, r, h);
-  y.load(key ? a.v : a.dout, head, row0, rows, s.dim, wave, r, h);
+  x.load(key ? a.k : a.q, head, row0, rows, s.dim, wave, r, h, key ? 1.f : s.scale * kLog2E);
+  y.load(key ? a.v : a.dout, head, row0, rows, s.dim, wave, r, h, 1.f);
   const uint32_t bx = row_bits(x.bad), by = row_bits(y.bad);
   if (lane == 0) bits[0][wave] = bx, bits[1][wave] = by;
   if (!key) {
@@ -144,12 +145,12 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const PackArgs a) {
   const uint32_t bad_y = bits[1][0] | bits[1][1] | bits[1][2] | bits[1][3];
   const bool bad = (bad_x | bad_y) >> (lane & 31) & 1;
   if (key) {
-    x.store(a.kp + o, wave, lane, bad, a.stats ? 0.f : __builtin_nanf(""), 1.f);
-    y.store(a.vp + o, wave, lane, bad, 0.f, 1.f);
+    x.store(a.kp + o, wave, lane, bad, a.stats ? 0.f : __builtin_nanf(""));
+    y.store(a.vp + o, wave, lane, bad, 0.f);
     return;
   }
-  x.store(a.qp + o, wave, lane, bad, 0.f, s.scale * kLog2E);
-  y.store(a.dp + o, wave, lane, bad, 0.f, 1.f);
+  x.store(a.qp + o, wave, lane, bad, 0.f);
+  y.store(a.dp + o, wave, lane, bad, 0.f);
   // Past the sequence's end lse is infinite: no probability.
   if (wave == 0 && h == 0) {
     float* const to = a.stats + (int64_t(head) * s.tiles + blockIdx.x) * 64 + r;

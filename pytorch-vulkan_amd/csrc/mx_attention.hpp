@@ -2,7 +2,8 @@
 // (packed sequences) and mx_attention_paged.hip (a cache).
 //
 // FP32 operands are taken as three bf16 pieces and multiplied as six piece products
-// (mfma_core.hpp's split), so the whole range of FP32 is there without a scale.  What is
+// (mfma_core.hpp's split), so FP32's range is there without a scale, but for the numbers from
+// 2^128 (1 - 2^-9) on: their first piece would be infinite, and they count as infinite.  What is
 // multiplied are tiles of 32 rows (queries or keys).  v_mfma_f32_32x32x16_bf16 leaves
 // lane half h of the wave with rows 8 b + 4 h + 0 .. 3 of a 32 x 32 result; row r of an
 // operand therefore stands for tile_row(r), so that a lane ends with the 16 consecutive
@@ -108,7 +109,8 @@ constexpr int kTileBytes = DP / 16 * P * 1024;
 // transposing read's 16 lanes, 8 bytes of four rows from both halves, meet every bank once.
 __device__ __forceinline__ int slot(int lane) { return lane ^ (lane >> 5 << 2); }
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+// Whether all pieces of x are finite: bf16's largest number and half a step rounds up.
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < 0x1.FFp127f; }
 
 // Elements e .. e + 7 of a row, zero from `dim` on.
 __device__ __forceinline__ void load8(const float* row, int e, int dim, f32x4 (&v)[2]) {

@@ -979,3 +979,63 @@ def test_rotary_elements_behind_the_turned_part_stay_alone(mx, dim, rot, interle
         assert torch.equal(got[..., e], x[..., e].sign() * math.inf), e
         got[..., e] = clean[..., e]
         assert torch.equal(got, clean), e
+
+
+def test_attention_keeps_huge_values_that_are_not_seen_apart(mx):
+    """The largest finite numbers, and queries that the scale takes past them, change no bit of rows that do not see them."""
+    g = gen(6)
+    lengths, h, kv, d, window, sinks = [90, 100, 75], 4, 2, 64, 20, 2
+    t = sum(lengths)
+    q, k, v, do = rand(g, t, h, d), rand(g, t, kv, d), rand(g, t, kv, d), rand(g, t, h, d)
+    bad = 90 + 47
+    rows = torch.arange(t, device="cuda")
+    reached = (rows >= bad) & (rows < bad + window)
+    touched = ((rows > bad - window) & (rows < bad + window)) | ((rows >= 90) & (rows < 90 + sinks))
+    keys = ((rows > bad - window) & (rows <= bad)) | ((rows >= 90) & (rows < 90 + sinks))
+    most = torch.finfo(torch.float32).max
+    for scale in (0.125, 4.0):
+        form = dict(window=window, sinks=sinks, scale=scale)
+        clean = run_attention(mx, q, k, v, do, starts_of(lengths), **form)
+        for value in (most, -most, 0.9975 * most, 1e38):
+            for where in ("k", "v"):
+                x = dict(k=k.clone(), v=v.clone())
+                x[where][bad, 1, 3] = value
+                got = run_attention(mx, q, x["k"], x["v"], do, starts_of(lengths), **form)
+                for name in ("out", "dq"):
+                    assert torch.equal(got[name][~reached], clean[name][~reached]), (name, where, value)
+                    assert torch.equal(got[name][:, :2], clean[name][:, :2]), "the other key head's rows"
+                for name in ("dk", "dv"):
+                    assert torch.equal(got[name][~touched], clean[name][~touched]), (name, where, value)
+                    assert torch.equal(got[name][:, 0], clean[name][:, 0])
+            for where in ("q", "do"):
+                x = dict(q=q.clone(), do=do.clone())
+                x[where][bad, 3, 0] = value
+                got = run_attention(mx, x["q"], k, v, x["do"], starts_of(lengths), **form)
+                for name in ("out", "dq"):
+                    assert torch.equal(got[name][rows != bad], clean[name][rows != bad]), (name, where, value)
+                for name in ("dk", "dv"):
+                    assert torch.equal(got[name][~keys], clean[name][~keys]), (name, where, value)
+
+
+@pytest.mark.parametrize("new", [4, 140])
+def test_paged_keeps_huge_values_that_are_not_seen_apart(mx, new):
+    g, page, h, kv, d, length, window = gen(11), 16, 4, 2, 64, 300, 150
+    table, pages = tables(g, [length], page)
+    cache = new_cache(mx, g, pages, kv, page, d, "f32")
+    fill(mx, g, cache, table, [length], page, kv, d, "f32")
+    q = rand(g, new, h, d)
+    run = lambda: (out := torch.empty_like(q), mx.attention_paged(
+        cache, mx.KVBatch(table, i32([length]), new), q, out, window=window, stream=stream()))[0]
+    clean = run()
+    j = length - new - window + 2  # seen by the first two rows or so, and by no later one
+    reached = torch.arange(length - new, length, device="cuda") - j < window
+    at, slot = int(table[0, j // page]), j % page
+    most = torch.finfo(torch.float32).max
+    for which in (0, 1):
+        x = cache.tensors[which][at, 1, slot] if which == 0 else cache.tensors[which][at, 1, :, slot]
+        kept = x.clone()
+        for value in (most, -most, math.inf):
+            x[9] = value
+            got = run()
+            assert torch.equal(got[~reached], clean[~reached]) and torch.equal(got[:, :2], clean[:, :2]), (which, value)
+        x.copy_(kept)
