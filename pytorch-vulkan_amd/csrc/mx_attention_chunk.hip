@@ -127,8 +127,9 @@ __global__ __launch_bounds__(256) void gather_kernel(const ChunkArgs a) {
     const bool ok = there(n);
     if constexpr (I8) {
       const int64_t row = (n >> 4 ? at[1] : at[0]) + (n & 15);
-      to[n] = ok ? c.ks[row] : 0.f;
-      to[32 + n] = ok ? c.vs[row] : 0.f;
+      const float ks = ok ? c.ks[row] : 0.f, vs = ok ? c.vs[row] : 0.f;
+      to[n] = fmaf(vs, 0.f, ks);  // a NaN value: NaN scores, whatever their probability
+      to[32 + n] = vs;
     }
     to[64 + n] = ok ? 0.f : 1.f;
     const bool any = __ballot(!ok) & 0xFFFFFFFFu;

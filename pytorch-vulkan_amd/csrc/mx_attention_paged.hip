@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) v
         acc = mma_all(k[kAhead ? i : 0][u].half(1), q[2 * u + 1], acc);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = I8 ? acc[e] * ks[i][e] : acc[e];
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = I8 ? fmaf(vs[i][e], 0.f, acc[e] * ks[i][e]) : acc[e];  // (a NaN value: a NaN score)
     }
     if (kAhead && n + kWaves < end) fetch(kn, 0, 4);
     const bool part = __any(!here || j + 16 > rt.length) || !a.mask.all(rt.i0, rt.i1, j0, j0 + kKeys - 1);

@@ -1039,3 +1039,21 @@ def test_paged_keeps_huge_values_that_are_not_seen_apart(mx, new):
             got = run()
             assert torch.equal(got[~reached], clean[~reached]) and torch.equal(got[:, :2], clean[:, :2]), (which, value)
         x.copy_(kept)
+
+
+@pytest.mark.parametrize("kind", ["i8", "f32"])
+@pytest.mark.parametrize("new", [1, 110])
+def test_paged_rows_that_see_a_bad_value_with_no_probability(mx, new, kind):
+    """A value that is not finite makes the rows that see it NaN also where its probability is 0."""
+    g, page, h, kv, d, length = gen(12), 16, 16, 2, 64, 250
+    table, pages = tables(g, [length], page)
+    cache = new_cache(mx, g, pages, kv, page, d, kind)
+    k = torch.full((length, kv, d), -8.0, device="cuda")
+    k[10] = 8.0
+    v = rand(g, length, kv, d)
+    v[20, 1, 5] = math.nan
+    mx.kv_cache_write(cache, mx.KVBatch(table, i32([length]), length), k, v, stream=stream())
+    q, out = torch.full((new, h, d), 8.0, device="cuda"), torch.empty(new, h, d, device="cuda")
+    mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, out, stream=stream())
+    within(out[:, :8], v[10, 0].double() if kind == "f32" else quantised(v[10])[0], 64 * U * v[10, 0].double().abs(), "the other key head")
+    assert bool(out[:, 8:, 5].isnan().all()), kind
