@@ -661,7 +661,8 @@ typedef struct mx_attention_desc {
 int mx_attention_forward(const mx_attention_desc* d, const float* q, const float* k, const float* v, float* out,
                          float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 /* From the forward's out and lse; dout and the gradients are contiguous, dq with dk
- * and dv or either side alone (NULL: not computed).  Sums are taken in a fixed order. */
+ * and dv or either side alone (NULL: not computed); without query heads dk and dv are 0 in
+ * the sequences' rows.  Sums are taken in a fixed order. */
 int mx_attention_backward(const mx_attention_desc* d, const float* dout, const float* q, const float* k, const float* v,
                           const float* out, const float* lse, float* dq, float* dk, float* dv, void* workspace,
                           int64_t workspace_bytes, void* stream);

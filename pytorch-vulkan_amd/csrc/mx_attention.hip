@@ -699,6 +699,15 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const BwdArgs a) {
   }
 }
 
+// dk (y 0) and dv (y 1) of key heads without query heads: 0 in the sequences' rows, of `row` elements.
+__global__ __launch_bounds__(kThreads) void no_heads_kernel(const Sequences seqs, int64_t row, float* dk, float* dv) {
+  float* const to = blockIdx.y ? dv : dk;
+  if (!to) return;
+  const int64_t end = seqs.start(seqs.count) * row;
+  for (int64_t i = seqs.start(0) * row + int64_t(blockIdx.x) * kThreads + threadIdx.x; i < end; i += int64_t(gridDim.x) * kThreads)
+    to[i] = 0;
+}
+
 // --------------------------------------------------------------------- host
 int check(const char* who, const mx_attention_desc* d) {
   MX_REQUIRE(d, MX_ERR_INVALID, who, ": null descriptor");
@@ -877,7 +886,16 @@ extern "C" int mx_attention_backward(const mx_attention_desc* d, const float* do
   const CountedCall counted;
   const char* const who = "mx_attention_backward";
   MX_TRY(check(who, d));
-  if (d->tokens == 0 || d->heads == 0 || (!dq && !dk && !dv)) return MX_OK;
+  if (d->tokens == 0 || (!dq && !dk && !dv)) return MX_OK;
+  if (d->heads == 0) {
+    const int64_t row = d->kv_heads * d->head_dim;
+    if (row == 0 || (!dk && !dv)) return MX_OK;
+    const unsigned blocks = unsigned(std::min<int64_t>((d->tokens * row + kThreads - 1) / kThreads, int64_t(cu_count()) * 8));
+    hipLaunchKernelGGL(no_heads_kernel, dim3(blocks, 2), dim3(kThreads), 0, resolve_stream(stream),
+                       Sequences{d->starts, int(d->tokens), int(d->sequences)}, row, dk, dv);
+    MX_LAUNCHED();
+    return MX_OK;
+  }
   MX_REQUIRE(dout && q && k && v && out && lse, MX_ERR_INVALID, who, ": null buffer");
   const Shape s = shape_of(d);
   hipStream_t st = resolve_stream(stream);

@@ -1057,3 +1057,22 @@ def test_paged_rows_that_see_a_bad_value_with_no_probability(mx, new, kind):
     mx.attention_paged(cache, mx.KVBatch(table, i32([length]), new), q, out, stream=stream())
     within(out[:, :8], v[10, 0].double() if kind == "f32" else quantised(v[10])[0], 64 * U * v[10, 0].double().abs(), "the other key head")
     assert bool(out[:, 8:, 5].isnan().all()), kind
+
+
+def test_attention_backward_without_query_heads(mx):
+    """Key heads that no query head shares have gradients of 0, in the sequences' rows alone."""
+    g = gen(13)
+    k = rand(g, 50, 2, 40)
+    none = torch.empty(50, 0, 40, device="cuda")
+    starts = starts_of([20, 0, 23], 3)
+    for want in ((True, True), (True, False), (False, True)):
+        outs = [guarded(50, 2, 40) if w else (None, None) for w in want]
+        mx.attention_backward(none, none, k, k, none, torch.empty(0, 50, device="cuda"), torch.empty_like(none), outs[0][0],
+                              outs[1][0], starts=starts, stream=stream())
+        for x, tail in outs:
+            if x is not None:
+                intact(tail)
+                assert bool((x[3:46] == 0).all())
+    x = torch.full((50, 2, 40), TAIL, device="cuda")
+    mx.attention_backward(none, none, k, k, none, torch.empty(0, 50, device="cuda"), None, x, None, starts=starts, stream=stream())
+    assert bool((x[:3] == TAIL).all()) and bool((x[46:] == TAIL).all()), "rows of no sequence"
