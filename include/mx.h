@@ -703,7 +703,8 @@ int mx_kv_cache_write(const mx_kv_cache* c, const mx_kv_batch* b, const float* k
 int mx_kv_cache_read(const mx_kv_cache* c, const mx_kv_batch* b, float* k, float* v, void* stream);
 /* Attention of the new tokens over the cache, which holds them already: a row at
  * position i sees positions j as in mx_attention_desc.  q has the given strides, out
- * [tokens, heads, head_dim] is contiguous; a row that sees nothing is 0. */
+ * [tokens, heads, head_dim] is contiguous; a row that sees nothing, or nothing but scores that overflow
+ * to minus infinity, is 0. */
 typedef struct mx_paged_desc {
   int64_t heads;
   int64_t q_token, q_head;

@@ -303,7 +303,7 @@ constexpr int aside(int steps, int waves) { return steps > 6 && waves == 8 ? 7 :
 
 // A wave's 32 queries stay in registers as pieces, with their sums.  Bound by the matrix
 // instructions: 16384 tokens, 16 heads of 64, window 4096 1290 us, 187 TFLOP/s, six piece products of which
-// are 1.12 PFLOP/s (a library's bf16 product of 8192^3 1.25 on this card); 2 x 2048, 16 heads of 128 207 us,
+// are 1.12 PFLOP/s (a library's bf16 product of 8192^3 1.25 to 1.33); 2 x 2048, 16 heads of 128 207 us,
 // 166 TFLOP/s.  There a wave is alone on its SIMD, which hides neither LDS's latency nor the softmax
 // behind products unless those are another tile's: 250 us with a tile's scores and exponents in turn.
 // Workgroups of eight waves, two a SIMD (4.5 us a tile of 256 rows for 3.7 of 128 then), have too
@@ -464,7 +464,7 @@ __device__ __forceinline__ int near_last(const BwdArgs& a, int b0, int len) {
 }
 
 // Three products of a tile, two of them computed again for dk and dv: the scores' gradients would be
-// 6 bytes a pair in memory.  2 x 2048, 16 heads of 128: 280 us alone, 168 TFLOP/s, 1.0 PFLOP/s of pieces.
+// 4 bytes a pair in memory, written and read.  2 x 2048, 16 heads of 128: 280 us alone, 168 TFLOP/s, 1.0 PFLOP/s of pieces.
 // (workgroup `index` of `count`)
 template <int E, int SPLIT>
 struct Dq {

@@ -70,9 +70,9 @@ struct Place {
   }
 };
 
-// 64 tokens, 32 heads over 8 key heads of 128, 8-bit contexts of 819 to 8192: 189 to 197 us, 3.4 to 3.5 TB/s (equal contexts
-// of 8192 4.2 TB/s with the join; a read of as many bytes 4.0, a copy 5.0): uneven lengths leave the chip half full
-// at the end.  Without reading keys ahead 335 us.  17 x 2 tokens, FP32, contexts up to 3001, 9 heads of 80:
+// 64 tokens, 32 heads over 8 key heads of 128, 8-bit contexts of 819 to 8192: 186 to 197 us, 3.4 to 3.6 TB/s (equal contexts
+// of 8192 4.2 TB/s with the join; reads alone reach 7.0): waves wait 53 % of their cycles, and uneven lengths leave the chip
+// half full at the end.  Without reading keys ahead 335 us.  17 x 2 tokens, FP32, contexts up to 3001, 9 heads of 80:
 // 50 us, 4.2 TB/s; keys read ahead, at one wave a SIMD, 74.
 template <int DP, bool I8>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2))) void paged_kernel(const PagedArgs a) {
@@ -342,7 +342,8 @@ int64_t row_tiles(const mx_paged_desc* d, const mx_kv_cache* c, const mx_kv_batc
 // How a row tile's keys are dealt: `span` tiles of 64 to a workgroup, as many workgroups as even out
 // lengths that the host does not know: eight a CU if all were of the table's length (the batch
 // above: 220 us with up to four, 189 with eight, 188 with 16, 199 with 32; 16 contexts of up to 16384
-// 121, 105, 109 and 109).
+// 121, 105, 109 and 109).  The table's width stands for the lengths, so a wide table leaves short contexts to few workgroups
+// (one token over 4096, 4 key heads of 128: 12.8 us with a table of 4096 positions, 33.6 of 131072).
 struct Split {
   int splits, span;
 };
