@@ -279,3 +279,34 @@ def test_decoder_trains_on_a_stream(vk):
         losses = m.train(model, *batch, 3)
     vk.current_stream().wait_stream(s)
     assert all(math.isfinite(x) for x in losses)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int8])
+def test_layer_with_the_largest_window(dtype):
+    """window=2 ** 63 - 1 is no window, in training and in serving: a prompt and a token over more keys than a workgroup takes."""
+    from torch_vulkan.nn import Attention, KVCache
+    torch.manual_seed(9)
+    n, page = 1300, 64
+    layers = [Attention(64, 4, 2, window=w) for w in (0, 2 ** 63 - 1)]
+    layers[1].load_state_dict(layers[0].state_dict())
+    x, positions = torch.randn(n, 64).to("vulkan"), torch.arange(n).to("vulkan")
+    table, count = torch.arange(22, dtype=torch.int32)[None].to("vulkan"), lambda v: torch.tensor([v], dtype=torch.int32).to("vulkan")
+    outs = []
+    for layer in layers:
+        layer.to("vulkan")
+        cache = KVCache(22, 2, page, 16, dtype)
+        with torch.no_grad():
+            outs.append([layer(x, positions).cpu(),
+                         layer(x[:-1], positions[:-1], cache=cache, table=table, lengths=count(n - 1)).cpu(),
+                         layer(x[-1:], positions[-1:], cache=cache, table=table, lengths=count(n)).cpu()])
+    for none, largest in zip(*outs):
+        assert torch.equal(none, largest)
+
+
+def test_key_heads_without_query_heads():
+    """Their gradients are zeros, not memory as it was."""
+    from torch_vulkan.nn import attention
+    k, v = (torch.randn(40, 2, 32).to("vulkan").requires_grad_() for _ in range(2))
+    attention(torch.empty(40, 0, 32).to("vulkan"), k, v, scale=1.0).sum().backward()
+    for x in (k, v):
+        assert bool((x.grad.cpu() == 0).all())
